@@ -516,6 +516,197 @@ int pkv_linear_forward(const pkv_linear* args, int device, void* stream);
 int pkv_greedy_tokens(int32_t* token_ids, const float* logits, int64_t row_stride,
                       int64_t num_rows, int64_t vocab_size, int device, void* stream);
 
+/*
+ * Rotary embedding with one to four position axes (for example time, height and width), fused with
+ * the slot-mapped append, for grouped heads: num_heads query heads, num_kv_heads key and value heads.
+ *     q' = rope(q) ; key_pool[slots] = rope(k) ; value_pool[slots] = v
+ * rope turns the first rotary_dim dimensions of a head and copies the rest. With half = rotary_dim /
+ * 2 and frequency i < half of axis a(i): rope(x)[i] = x[i]*cos - x[i+half]*sin, rope(x)[i+half] =
+ * x[i+half]*cos + x[i]*sin, cos/sin = table[positions[a(i)][token]][i]; in float32, each product and
+ * sum rounded separately, then rounded once to the output's type.
+ *
+ * No counterpart in the reference, whose positions have one axis and whose keys as many heads as its
+ * queries (src/paged_kv_serving/engine/model.py:70-81); with one axis, equal head counts and float32
+ * it computes what pkv_rope_append does, bit for bit.
+ *
+ *   rotated_queries      : io_dtype [num_tokens, num_heads, head_dim] at rotated_token_stride. May be
+ *                          `queries` itself (same stride); must not otherwise overlap an input.
+ *   queries, keys, values: io_dtype rows [num_heads | num_kv_heads, head_dim] with token strides.
+ *   positions            : int64, axis a of token t at a * position_axis_stride + t.
+ *   sections             : frequencies of each axis, together rotary_dim / 2. Axis 0's frequencies
+ *                          come first, then axis 1's, and so on; with `interleaved` frequency i
+ *                          belongs to axis i % num_axes while i < num_axes * sections[that axis], and
+ *                          to axis 0 otherwise.
+ *   cos_table, sin_table : float32 [table_rows, rotary_dim / 2].
+ *   key_pool, value_pool : the layer's pools, [num_slots, num_kv_heads, head_dim] of pool_dtype.
+ *   slot_mapping         : int64 [num_tokens].
+ * A token with a position outside [0, table_rows) is skipped entirely (its rotated query is not
+ * written); a slot outside [0, num_slots) skips only that token's pool writes (a padded batch names
+ * slot -1). Duplicate slots in one call leave an unspecified one of the duplicate rows.
+ */
+#define PKV_MAX_ROPE_AXES 4
+
+typedef struct pkv_rope_axes {
+  void* rotated_queries;
+  const void* queries;
+  const void* keys;
+  const void* values;
+  int64_t rotated_token_stride;
+  int64_t query_token_stride;
+  int64_t key_token_stride;
+  int64_t value_token_stride;
+  const int64_t* positions;
+  int64_t position_axis_stride;
+  const float* cos_table;
+  const float* sin_table;
+  int64_t table_rows;
+  void* key_pool;
+  void* value_pool;
+  int64_t num_slots;
+  const int64_t* slot_mapping;
+  int64_t num_tokens;
+  int32_t io_dtype;
+  int32_t pool_dtype;
+  int32_t num_heads;
+  int32_t num_kv_heads;
+  int32_t head_dim;
+  int32_t rotary_dim;
+  int32_t num_axes;
+  int32_t interleaved;
+  int32_t sections[PKV_MAX_ROPE_AXES];
+} pkv_rope_axes;
+
+int pkv_rope_append_axes(const pkv_rope_axes* args, int device, void* stream);
+
+/*
+ * Paged causal attention with a sliding window and sinks, for grouped heads (query head h reads key
+ * head h / (num_heads / num_kv_heads)): a query row at position p of a sequence with context length
+ * c attends to the keys j < min(c, p + 1) with j > p - window or j < sinks. A window of at least the
+ * context is plain causal attention.
+ *
+ * No counterpart in the reference, whose attention sees the whole context
+ * (src/paged_kv_serving/engine/attention.py:42-121); tables, contexts and masking are as there.
+ *
+ *   out, queries    : q_dtype [num_queries, num_heads, head_dim]; out contiguous, queries with a
+ *                     token stride; both 16-byte aligned rows.
+ *   query_positions : int32 [num_queries].
+ *   query_seq       : int32 [num_queries], the sequence each row belongs to. A row outside [0,
+ *                     num_seqs) is padding: its output row is left as it was.
+ *   key_cache,
+ *   value_cache     : the layer's pools, [num_blocks, block_size, num_kv_heads, head_dim], kv_dtype,
+ *                     16-byte aligned.
+ *   block_tables    : int32 [num_seqs, block_table_stride]; block_table_stride * block_size >=
+ *                     max_context_len (checked).
+ *   context_lens    : int32 [num_seqs]; visible lengths are clamped to max_context_len.
+ *   max_query_len   : an upper bound of the rows that one sequence has next to each other. It chooses
+ *                     how the call runs, never its result; rows of one sequence lying next to each
+ *                     other are computed together from PKV_WINDOW_MIN_RUN on.
+ *   num_splits      : workgroups that share a row's keys, 1 to PKV_WINDOW_MAX_SPLITS, or 0 for the
+ *                     library's choice (pkv_window_splits).
+ *   workspace       : float32 scratch of pkv_window_workspace_bytes(...) bytes, 16-byte aligned (may be
+ *                     NULL when that is 0). Nothing in it needs to start at zero.
+ * Rows of one sequence need not lie next to each other, nor in order. A row that sees no key gets
+ * zeros. Block ids outside [0, num_blocks) at a visible position are skipped, as in
+ * pkv_paged_attention. Supported: head_dim 32, 64, 128, 256; float32 queries over float32 or bfloat16
+ * pools, bfloat16 queries over bfloat16 pools; up to PKV_WINDOW_MAX_GROUP query heads per key head.
+ * Scores, softmax and sums are float32; a bfloat16 output is rounded once.
+ */
+#define PKV_WINDOW_MAX_GROUP 64
+#define PKV_WINDOW_MAX_SPLITS 64
+#define PKV_WINDOW_MIN_RUN 4
+
+typedef struct pkv_window {
+  void* out;
+  const void* queries;
+  int64_t query_token_stride;
+  const int32_t* query_positions;
+  const int32_t* query_seq;
+  int64_t num_queries;
+  const void* key_cache;
+  const void* value_cache;
+  int64_t num_blocks;
+  const int32_t* block_tables;
+  const int32_t* context_lens;
+  float* workspace;
+  int64_t workspace_bytes;
+  int32_t q_dtype;
+  int32_t kv_dtype;
+  int32_t block_size;
+  int32_t block_table_stride;
+  int32_t num_seqs;
+  int32_t num_heads;
+  int32_t num_kv_heads;
+  int32_t head_dim;
+  int32_t window;
+  int32_t sinks;
+  int32_t max_context_len;
+  int32_t max_query_len;
+  int32_t num_splits;
+  float scale;
+} pkv_window;
+
+/* Splits the library chooses for a call with num_splits 0 (1 where nothing is split). Host-only. */
+int32_t pkv_window_splits(int64_t num_queries, int32_t num_heads, int32_t num_kv_heads, int32_t window,
+                          int32_t sinks, int32_t max_context_len, int32_t max_query_len);
+
+/* Bytes of workspace for `num_splits` splits (0 for one). Host-only. */
+int64_t pkv_window_workspace_bytes(int64_t num_queries, int32_t num_heads, int32_t head_dim, int32_t num_splits);
+
+int pkv_window_attention(const pkv_window* args, int device, void* stream);
+
+/*
+ * Sampling from logits rows with temperature, top-k, min-p and top-p, with given uniform numbers.
+ *
+ * Extends src/paged_kv_serving/engine/sampling.py:56-74 (one uniform draw per token) to whole batches
+ * on the device; where a row is not drawn (temperature 0) it is pkv_greedy_tokens's token.
+ *
+ * Per row, with T = temperature and w[i] = exp((logit[i] - max) / T): the tokens in order of falling
+ * logits, equal ones in order of their ids; of that order
+ *     the first top_k tokens (all with top_k <= 0), of those the tokens with w >= min_p,
+ *     of those the shortest beginning with a mass of at least top_p of theirs (all with top_p >= 1),
+ *     and the first token whose cumulative mass exceeds uniform * the mass of what is kept.
+ * Weights are 64-bit fixed-point numbers of PKV_SAMPLE_BITS fractional bits (fewer from 2^18
+ * tokens on, so that no sum overflows), rounded from double precision, and their sums are exact: a
+ * result does not depend on how a row is spread over the GPU.
+ *
+ *   token_ids   : int32 [num_rows], output.
+ *   logits      : rows of vocab_size values of `dtype`, row r at element r * row_stride.
+ *   uniforms    : float32 [num_rows], in [0, 1); below (or NaN) counts as 0, above as the last token.
+ *   temperature, top_k, top_p, min_p : one value for every row, or, where the pointer of the same
+ *                 name is given, one for each row (float32, top_k int32). A temperature of 0 or below
+ *                 (or NaN) takes the greedy token. A top_p of 0 or below (or NaN) keeps the first
+ *                 token; a min_p above 1 does too, one of 0 or below (or NaN) keeps all.
+ * A token of -inf is never drawn; tokens of +inf share the whole mass. A row with a NaN, or with
+ * nothing above -inf, yields its greedy token.
+ *   workspace   : scratch of pkv_sample_workspace_bytes(...) bytes, 16-byte aligned (NULL when 0).
+ */
+#define PKV_SAMPLE_BITS 46
+
+typedef struct pkv_sample {
+  int32_t* token_ids;
+  const void* logits;
+  int64_t row_stride;
+  int64_t num_rows;
+  int64_t vocab_size;
+  const float* uniforms;
+  const float* temperatures;
+  const int32_t* top_ks;
+  const float* top_ps;
+  const float* min_ps;
+  void* workspace;
+  int64_t workspace_bytes;
+  int32_t dtype;
+  float temperature;
+  int32_t top_k;
+  float top_p;
+  float min_p;
+} pkv_sample;
+
+/* Bytes of workspace pkv_sample_tokens needs. Host-only. */
+int64_t pkv_sample_workspace_bytes(int64_t num_rows, int64_t vocab_size);
+
+int pkv_sample_tokens(const pkv_sample* args, int device, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

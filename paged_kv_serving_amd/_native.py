@@ -38,7 +38,8 @@ INCLUDE = REPO_ROOT / "include"
 LIB_PATH = PACKAGE_DIR / "libpkv.so"
 SOURCES = (
     CSRC / "pkv_copy.hip", CSRC / "pkv_rope.hip", CSRC / "pkv_attention.hip", CSRC / "pkv_sample.hip",
-    CSRC / "pkv_plan.hip", CSRC / "pkv_model.hip", CSRC / "pkv_linear.hip",
+    CSRC / "pkv_plan.hip", CSRC / "pkv_model.hip", CSRC / "pkv_linear.hip", CSRC / "pkv_rope_axes.hip",
+    CSRC / "pkv_window.hip", CSRC / "pkv_sampling.hip",
 )
 
 # gfx950 only. Packed-FP32 VALU instructions are disabled: the code relies on scalar fp32 FMA.
@@ -94,6 +95,12 @@ EXPORTED_SYMBOLS = (
     "pkv_gather_rows",
     "pkv_sequence_metadata",
     "pkv_linear_forward",
+    "pkv_rope_append_axes",
+    "pkv_window_splits",
+    "pkv_window_workspace_bytes",
+    "pkv_window_attention",
+    "pkv_sample_workspace_bytes",
+    "pkv_sample_tokens",
 )
 
 
@@ -219,6 +226,46 @@ _i64 = ctypes.c_int64
 _ptr = ctypes.c_void_p
 
 
+class RopeAxesArgs(ctypes.Structure):
+    """``pkv_rope_axes`` (include/pkv.h)."""
+
+    _fields_ = [
+        ("rotated_queries", _ptr), ("queries", _ptr), ("keys", _ptr), ("values", _ptr),
+        ("rotated_token_stride", _i64), ("query_token_stride", _i64), ("key_token_stride", _i64),
+        ("value_token_stride", _i64), ("positions", _ptr), ("position_axis_stride", _i64),
+        ("cos_table", _ptr), ("sin_table", _ptr), ("table_rows", _i64), ("key_pool", _ptr),
+        ("value_pool", _ptr), ("num_slots", _i64), ("slot_mapping", _ptr), ("num_tokens", _i64),
+        ("io_dtype", _i32), ("pool_dtype", _i32), ("num_heads", _i32), ("num_kv_heads", _i32),
+        ("head_dim", _i32), ("rotary_dim", _i32), ("num_axes", _i32), ("interleaved", _i32),
+        ("sections", _i32 * 4),
+    ]  # fmt: skip
+
+
+class WindowArgs(ctypes.Structure):
+    """``pkv_window`` (include/pkv.h)."""
+
+    _fields_ = [
+        ("out", _ptr), ("queries", _ptr), ("query_token_stride", _i64), ("query_positions", _ptr),
+        ("query_seq", _ptr), ("num_queries", _i64), ("key_cache", _ptr), ("value_cache", _ptr),
+        ("num_blocks", _i64), ("block_tables", _ptr), ("context_lens", _ptr), ("workspace", _ptr),
+        ("workspace_bytes", _i64), ("q_dtype", _i32), ("kv_dtype", _i32), ("block_size", _i32),
+        ("block_table_stride", _i32), ("num_seqs", _i32), ("num_heads", _i32), ("num_kv_heads", _i32),
+        ("head_dim", _i32), ("window", _i32), ("sinks", _i32), ("max_context_len", _i32),
+        ("max_query_len", _i32), ("num_splits", _i32), ("scale", ctypes.c_float),
+    ]  # fmt: skip
+
+
+class SampleArgs(ctypes.Structure):
+    """``pkv_sample`` (include/pkv.h)."""
+
+    _fields_ = [
+        ("token_ids", _ptr), ("logits", _ptr), ("row_stride", _i64), ("num_rows", _i64), ("vocab_size", _i64),
+        ("uniforms", _ptr), ("temperatures", _ptr), ("top_ks", _ptr), ("top_ps", _ptr), ("min_ps", _ptr),
+        ("workspace", _ptr), ("workspace_bytes", _i64), ("dtype", _i32), ("temperature", ctypes.c_float),
+        ("top_k", _i32), ("top_p", ctypes.c_float), ("min_p", ctypes.c_float),
+    ]  # fmt: skip
+
+
 def _declare(lib: ctypes.CDLL) -> None:
     lib.pkv_init.argtypes = [_c_int]
     lib.pkv_init.restype = _c_int
@@ -326,6 +373,20 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.pkv_sequence_metadata.restype = _c_int
     lib.pkv_linear_forward.argtypes = [_ptr, _c_int, _ptr]  # args, device, stream
     lib.pkv_linear_forward.restype = _c_int
+    lib.pkv_rope_append_axes.argtypes = [ctypes.POINTER(RopeAxesArgs), _c_int, _ptr]  # args, device, stream
+    lib.pkv_rope_append_axes.restype = _c_int
+    lib.pkv_window_splits.argtypes = [
+        _i64, _i32, _i32, _i32, _i32, _i32, _i32,  # queries, heads, kv heads, window, sinks, max context, max query len
+    ]
+    lib.pkv_window_splits.restype = _i32
+    lib.pkv_window_workspace_bytes.argtypes = [_i64, _i32, _i32, _i32]  # queries, heads, head_dim, splits
+    lib.pkv_window_workspace_bytes.restype = _i64
+    lib.pkv_window_attention.argtypes = [ctypes.POINTER(WindowArgs), _c_int, _ptr]  # args, device, stream
+    lib.pkv_window_attention.restype = _c_int
+    lib.pkv_sample_workspace_bytes.argtypes = [_i64, _i64]  # rows, vocab
+    lib.pkv_sample_workspace_bytes.restype = _i64
+    lib.pkv_sample_tokens.argtypes = [ctypes.POINTER(SampleArgs), _c_int, _ptr]  # args, device, stream
+    lib.pkv_sample_tokens.restype = _c_int
 
 
 def library() -> ctypes.CDLL:

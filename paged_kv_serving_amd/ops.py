@@ -8,6 +8,7 @@ the tensors' device). Nothing here computes on the CPU: a missing library raises
 
 from __future__ import annotations
 
+import ctypes
 from dataclasses import dataclass
 
 import numpy as np
@@ -29,6 +30,7 @@ __all__ = [
     "kv_dtype_size",
     "merge_rows_for",
     "paged_attention_ragged",
+    "paged_attention_window",
     "BatchPlan",
     "batch_hints",
     "NativePlanner",
@@ -39,8 +41,11 @@ __all__ = [
     "upload_batch_plan",
     "rms_norm",
     "rope_append",
+    "rope_append_axes",
+    "sample_tokens",
     "silu_mul",
     "upload_plan",
+    "window_workspace_bytes",
 ]
 
 #: Rows per MFMA tile (4 wavefronts x 16 queries).
@@ -194,6 +199,107 @@ def rope_append(
     return out
 
 
+#: Position axes :func:`rope_append_axes` can take.
+MAX_ROPE_AXES = 4
+
+
+def rope_append_axes(
+    key_pool: torch.Tensor,
+    value_pool: torch.Tensor,
+    queries: torch.Tensor,
+    keys: torch.Tensor,
+    values: torch.Tensor,
+    positions: torch.Tensor,
+    cos_table: torch.Tensor,
+    sin_table: torch.Tensor,
+    slot_mapping: torch.Tensor,
+    *,
+    sections: tuple[int, ...] | None = None,
+    interleaved: bool = False,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """:func:`rope_append` for grouped heads, float32 or bfloat16 activations and positions of one
+    to four axes (time, height, width of an image or video token); returns the rotated queries.
+
+    ``queries [T, heads, head_dim]``, ``keys``/``values [T, kv_heads, head_dim]``: float32 or
+    bfloat16 (all three alike), token-strided views allowed. ``key_pool``/``value_pool``: contiguous,
+    trailing dims ``kv_heads, head_dim``, float32 or bfloat16. ``positions``: int64 ``[T]``, or
+    ``[axes, T]`` with ``sections``, the number of frequencies each axis turns (together
+    ``cos_table.shape[1]``): axis 0's frequencies come first, then axis 1's and so on, or with
+    ``interleaved`` one of each axis in turn, as long as its section lasts, and axis 0's then.
+    ``cos_table``/``sin_table``: float32 ``[rows, rotary_dim / 2]``; the dimensions of a head from
+    ``rotary_dim`` on are copied. The rotation is float32, each product and sum rounded on its own,
+    and the results are rounded once to their tensors' types. ``out`` may be ``queries`` itself.
+
+    A token whose slot lies outside the pool (padding: -1) writes no pool row; one with a position
+    outside the tables is skipped entirely.
+    """
+    device = _device_index(key_pool, value_pool, queries, keys, values, positions, cos_table, sin_table, slot_mapping)
+    if key_pool.shape != value_pool.shape or key_pool.dtype != value_pool.dtype:
+        raise ValueError("key and value pools must have the same shape and dtype")
+    if not (key_pool.is_contiguous() and value_pool.is_contiguous()):
+        raise ValueError("pools must be contiguous")
+    if queries.dim() != 3 or keys.dim() != 3 or keys.shape != values.shape:
+        raise ValueError("queries must be [T, heads, head_dim], keys and values [T, kv_heads, head_dim]")
+    tokens, heads, dim = queries.shape
+    kv_heads = keys.shape[1]
+    if keys.shape[0] != tokens or keys.shape[2] != dim:
+        raise ValueError("queries, keys and values disagree on (tokens, head_dim)")
+    if heads < 1 or kv_heads < 1:
+        raise ValueError("queries and keys need at least one head")
+    if key_pool.dim() < 3 or tuple(key_pool.shape[-2:]) != (kv_heads, dim):
+        raise ValueError("pool rows and keys disagree on (kv_heads, head_dim)")
+    io_code = kv_dtype_code(queries.dtype)
+    if keys.dtype != queries.dtype or values.dtype != queries.dtype:
+        raise ValueError("queries, keys and values must have the same dtype")
+    if cos_table.dtype != torch.float32 or sin_table.dtype != torch.float32:
+        raise ValueError("the rope tables must be float32")
+    if cos_table.shape != sin_table.shape or cos_table.dim() != 2 or not 1 <= cos_table.shape[1] <= dim // 2:
+        raise ValueError("rope tables must both be [rows, rotary_dim / 2] with rotary_dim at most head_dim")
+    if not (cos_table.is_contiguous() and sin_table.is_contiguous()):
+        raise ValueError("rope tables must be contiguous")
+    half = cos_table.shape[1]
+    if sections is None:
+        if positions.dim() != 1:
+            raise ValueError("positions of several axes need sections")
+        sections, axis_stride = (half,), 0
+    else:
+        sections = tuple(int(n) for n in sections)
+        if not 1 <= len(sections) <= MAX_ROPE_AXES:
+            raise ValueError(f"sections must name 1 to {MAX_ROPE_AXES} axes")
+        if min(sections) < 0 or sum(sections) != half:
+            raise ValueError("sections must be non-negative and add up to rotary_dim / 2")
+        if interleaved and any(n and a + len(sections) * (n - 1) >= half for a, n in enumerate(sections) if a):
+            raise ValueError("interleaved sections: an axis has more frequencies than its turns")
+        if positions.dim() != 2 or positions.shape[0] != len(sections):
+            raise ValueError("positions must be [axes, T] with one row for each section")
+        axis_stride = positions.stride(0) if len(sections) > 1 else 0
+    if positions.dtype != torch.int64 or positions.shape[-1] != tokens or (tokens > 1 and positions.stride(-1) != 1):
+        raise ValueError("positions must be int64 with one entry per token, adjacent in memory")
+    if slot_mapping.dtype != torch.int64 or slot_mapping.shape != (tokens,) or not slot_mapping.is_contiguous():
+        raise ValueError("slot_mapping must be contiguous int64 with one entry per token")
+    q_stride = _rows_contiguous(queries, "queries")
+    k_stride = _rows_contiguous(keys, "keys")
+    v_stride = _rows_contiguous(values, "values")
+    if out is None:
+        out = torch.empty((tokens, heads, dim), dtype=queries.dtype, device=queries.device)
+    elif out.shape != queries.shape or out.dtype != queries.dtype or out.device != queries.device:
+        raise ValueError("out must match queries")
+    out_stride = _rows_contiguous(out, "out")
+    if tokens == 0:
+        return out
+    args = _native.RopeAxesArgs(
+        out.data_ptr(), queries.data_ptr(), keys.data_ptr(), values.data_ptr(), out_stride, q_stride, k_stride,
+        v_stride, positions.data_ptr(), axis_stride, cos_table.data_ptr(), sin_table.data_ptr(), cos_table.shape[0],
+        key_pool.data_ptr(), value_pool.data_ptr(), key_pool.numel() // (kv_heads * dim), slot_mapping.data_ptr(),
+        tokens, io_code, kv_dtype_code(key_pool.dtype), heads, kv_heads, dim, 2 * half, len(sections),
+        int(interleaved), (ctypes.c_int32 * MAX_ROPE_AXES)(*sections),
+    )  # fmt: skip
+    rc = _native.library().pkv_rope_append_axes(args, device, _stream(device))
+    _native.check(rc, "pkv_rope_append_axes")
+    return out
+
+
 def _rows_2d(tensor: torch.Tensor, name: str, width: int) -> int:
     """Row stride (elements) of a float32 ``[rows, >= width]`` tensor with contiguous rows."""
     if tensor.dim() != 2 or tensor.dtype != torch.float32 or tensor.shape[1] < width:
@@ -280,6 +386,80 @@ def greedy_tokens(logits: torch.Tensor, out: torch.Tensor | None = None) -> torc
         out.data_ptr(), logits.data_ptr(), stride, rows, vocab, device, _stream(device)
     )
     _native.check(rc, "pkv_greedy_tokens")
+    return out
+
+
+def _row_setting(value, name: str, rows: int, dtype: torch.dtype, logits: torch.Tensor):
+    """``(pointer or None, scalar)`` of a sampling setting: one number, or one for each row."""
+    if not isinstance(value, torch.Tensor):
+        return None, value
+    if value.dtype != dtype or value.shape != (rows,) or not value.is_contiguous() or value.device != logits.device:
+        raise ValueError(f"{name} must be a number or contiguous {str(dtype)[6:]} with one entry per row")
+    return value.data_ptr(), 0
+
+
+def sample_tokens(
+    logits: torch.Tensor,
+    uniforms: torch.Tensor,
+    *,
+    temperature: float | torch.Tensor = 1.0,
+    top_k: int | torch.Tensor = 0,
+    top_p: float | torch.Tensor = 1.0,
+    min_p: float | torch.Tensor = 0.0,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """One token id for each row of ``logits [rows, vocab]`` (float32 or bfloat16), drawn on the
+    device with the given ``uniforms`` (float32 ``[rows]`` in [0, 1)); int32 ``[rows]``.
+
+    With weights ``exp((logit - max) / temperature)`` and the tokens in order of falling logits (equal
+    ones in order of their ids), the kept tokens are, in this order, the first ``top_k`` (0: all), of
+    those the ones with a weight of at least ``min_p`` (0: all), and of those the shortest beginning
+    with at least ``top_p`` of their mass (1: all). The token is the first of them whose cumulative mass
+    exceeds ``uniform`` times theirs. Each setting is a number or a tensor with one entry per row
+    (float32; ``top_k`` int32). ``temperature`` 0 takes :func:`greedy_tokens`'s token, and so does a
+    row with a NaN or without any logit above -inf; -inf is never drawn, and +inf logits share the
+    whole mass. The same inputs give the same tokens, whatever the batch.
+
+    Extends the reference's per-row draw (sampling.py:56-74) to batches on the device.
+    """
+    device = _device_index(logits, uniforms)
+    if logits.dim() != 2 or logits.dtype not in _DTYPE_CODES:
+        raise ValueError("logits must be float32 or bfloat16 of shape (rows, vocab)")
+    rows, vocab = logits.shape
+    if vocab < 1:
+        raise ValueError("logits need at least one column")
+    if uniforms.dtype != torch.float32 or uniforms.shape != (rows,) or not uniforms.is_contiguous():
+        raise ValueError("uniforms must be contiguous float32 with one entry per row")
+    temperatures, temperature = _row_setting(temperature, "temperature", rows, torch.float32, logits)
+    top_ks, top_k = _row_setting(top_k, "top_k", rows, torch.int32, logits)
+    top_ps, top_p = _row_setting(top_p, "top_p", rows, torch.float32, logits)
+    min_ps, min_p = _row_setting(min_p, "min_p", rows, torch.float32, logits)
+    if temperatures is None and not temperature >= 0:
+        raise ValueError("temperature must be >= 0")
+    if top_ks is None and top_k < 0:
+        raise ValueError("top_k must be >= 0")
+    if top_ps is None and not 0 < top_p <= 1:
+        raise ValueError("top_p must be in (0, 1]")
+    if min_ps is None and not 0 <= min_p <= 1:
+        raise ValueError("min_p must be in [0, 1]")
+    if vocab > 1 and logits.stride(1) != 1:
+        logits = logits.contiguous()
+    if out is None:
+        out = torch.empty(rows, dtype=torch.int32, device=logits.device)
+    elif out.shape != (rows,) or out.dtype != torch.int32 or not out.is_contiguous() or out.device != logits.device:
+        raise ValueError("out must be a contiguous int32 tensor with one entry per row")
+    if rows == 0:
+        return out
+    lib = _native.library()
+    need = lib.pkv_sample_workspace_bytes(rows, vocab)
+    workspace = torch.empty(need, dtype=torch.uint8, device=logits.device) if need else None
+    args = _native.SampleArgs(
+        out.data_ptr(), logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, rows, vocab, uniforms.data_ptr(),
+        temperatures, top_ks, top_ps, min_ps, workspace.data_ptr() if need else None, need,
+        _DTYPE_CODES[logits.dtype], temperature, min(top_k, 0x7FFFFFFF), top_p, min_p,
+    )  # fmt: skip
+    rc = lib.pkv_sample_tokens(args, device, _stream(device))
+    _native.check(rc, "pkv_sample_tokens")
     return out
 
 
@@ -1224,3 +1404,127 @@ def paged_attention_ragged(
     )  # fmt: skip
     _native.check(rc, "pkv_paged_attention")
     return out
+
+
+#: Query heads per key head :func:`paged_attention_window` can take.
+MAX_WINDOW_GROUP = 64
+#: Workgroups that can share a row's keys in :func:`paged_attention_window`.
+MAX_WINDOW_SPLITS = 64
+_INT32_MAX = 0x7FFFFFFF
+
+
+def paged_attention_window(
+    queries: torch.Tensor,
+    query_positions: torch.Tensor,
+    query_seq: torch.Tensor,
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    block_tables: torch.Tensor,
+    context_lens: torch.Tensor,
+    scale: float,
+    *,
+    window: int,
+    sinks: int = 0,
+    max_context_len: int,
+    max_query_len: int | None = None,
+    num_splits: int = 0,
+    out: torch.Tensor | None = None,
+    workspace: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Causal paged attention with a sliding window and sinks, for grouped heads: a row at position
+    p sees the keys ``j < min(context_len, p + 1)`` with ``j > p - window`` or ``j < sinks``.
+
+    ``queries``: float32 or bfloat16 ``[T, heads, head_dim]`` (token-strided views allowed, 16-byte
+    aligned rows); ``key_cache``/``value_cache``: one layer's pools ``[num_blocks, block_size,
+    kv_heads, head_dim]``, bfloat16, or float32 under float32 queries; query head h reads key head ``h
+    // (heads // kv_heads)``. ``query_positions``, ``query_seq``: int32 ``[T]``; ``block_tables``: int32
+    ``[S, max_blocks]``; ``context_lens``: int32 ``[S]``; ``max_context_len`` bounds every context
+    length. A row whose ``query_seq`` lies outside ``[0, S)`` is padding: its output row is left as it
+    was. ``window`` of at least the context is plain causal attention.
+
+    ``max_query_len`` (default: T) bounds how many rows one sequence has next to each other: 1 for
+    a decode batch. With ``num_splits`` (default: the library's choice) it only decides how the call
+    runs. ``workspace``: float32 scratch of :func:`window_workspace_bytes` bytes, allocated when None.
+    Returns ``[T, heads, head_dim]`` of the queries' dtype. The call needs no plan and no host
+    reading of the batch, so it can be captured into a graph whose batch changes from replay to
+    replay (within T, S, ``max_context_len`` and ``max_query_len``).
+    """
+    device = _device_index(queries, query_positions, query_seq, key_cache, value_cache, block_tables, context_lens)
+    q_code = kv_dtype_code(queries.dtype)
+    stride = _rows_contiguous(queries, "queries")
+    num_queries, heads, dim = queries.shape
+    if key_cache.shape != value_cache.shape or key_cache.dtype != value_cache.dtype:
+        raise ValueError("key and value caches must have the same shape and dtype")
+    if key_cache.dim() != 4 or key_cache.shape[3] != dim:
+        raise ValueError("caches must have shape (num_blocks, block_size, kv_heads, head_dim)")
+    if not (key_cache.is_contiguous() and value_cache.is_contiguous()):
+        raise ValueError("caches must be contiguous")
+    num_blocks, block_size, kv_heads, _ = key_cache.shape
+    if kv_heads < 1 or heads < 1 or heads % kv_heads:
+        raise ValueError("heads must be a multiple of kv_heads")
+    if heads // kv_heads > MAX_WINDOW_GROUP:
+        raise ValueError(f"at most {MAX_WINDOW_GROUP} query heads per key head")
+    kv_code = kv_dtype_code(key_cache.dtype)
+    if key_cache.dtype == torch.float32 and queries.dtype != torch.float32:
+        raise ValueError("float32 caches need float32 queries")
+    for name, tensor in (("query_positions", query_positions), ("query_seq", query_seq)):
+        if tensor.dtype != torch.int32 or tensor.shape != (num_queries,) or not tensor.is_contiguous():
+            raise ValueError(f"{name} must be contiguous int32 with one entry per query")
+    if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or not block_tables.is_contiguous():
+        raise ValueError("block_tables must be contiguous int32 of shape (num_seqs, max_blocks)")
+    num_seqs = block_tables.shape[0]
+    if context_lens.dtype != torch.int32 or context_lens.shape != (num_seqs,) or not context_lens.is_contiguous():
+        raise ValueError("context_lens must be contiguous int32 with one entry per sequence")
+    if not 0 <= max_context_len <= _INT32_MAX or block_tables.shape[1] * block_size < max_context_len:
+        raise ValueError("block_tables are too narrow for max_context_len")
+    if window < 1 or sinks < 0:
+        raise ValueError("window must be >= 1 and sinks >= 0")
+    if max_query_len is not None and max_query_len < 0:
+        raise ValueError("max_query_len must be >= 0")
+    if not 0 <= num_splits <= MAX_WINDOW_SPLITS:
+        raise ValueError(f"num_splits must be in [0, {MAX_WINDOW_SPLITS}]")
+    if out is None:
+        out = torch.empty((num_queries, heads, dim), dtype=queries.dtype, device=queries.device)
+    elif out.shape != queries.shape or out.dtype != queries.dtype or out.device != queries.device:
+        raise ValueError("out must match queries")
+    elif not out.is_contiguous():
+        raise ValueError("out must be contiguous")
+    if num_queries == 0:
+        return out
+    window, sinks = min(window, _INT32_MAX), min(sinks, _INT32_MAX)
+    rows = num_queries if max_query_len is None else min(max_query_len, _INT32_MAX)
+    lib = _native.library()
+    splits = num_splits or lib.pkv_window_splits(num_queries, heads, kv_heads, window, sinks, max_context_len, rows)
+    need = lib.pkv_window_workspace_bytes(num_queries, heads, dim, splits)
+    if need:
+        if workspace is None:
+            workspace = torch.empty(need // 4, dtype=torch.float32, device=queries.device)
+        elif workspace.device != queries.device or not workspace.is_contiguous():
+            raise ValueError("workspace must be contiguous and on the queries' device")
+        elif workspace.numel() * workspace.element_size() < need:
+            raise ValueError(f"workspace must hold {need} bytes")
+    args = _native.WindowArgs(
+        out.data_ptr(), queries.data_ptr(), stride, query_positions.data_ptr(), query_seq.data_ptr(), num_queries,
+        key_cache.data_ptr(), value_cache.data_ptr(), num_blocks, block_tables.data_ptr(), context_lens.data_ptr(),
+        workspace.data_ptr() if need else None, need, q_code, kv_code, block_size, block_tables.shape[1], num_seqs,
+        heads, kv_heads, dim, window, sinks, max_context_len, rows, splits, float(scale),
+    )  # fmt: skip
+    rc = lib.pkv_window_attention(args, device, _stream(device))
+    _native.check(rc, "pkv_window_attention")
+    return out
+
+
+def window_workspace_bytes(
+    num_queries: int, heads: int, kv_heads: int, head_dim: int, *, window: int, sinks: int = 0,
+    max_context_len: int, max_query_len: int | None = None, num_splits: int = 0,
+) -> int:  # fmt: skip
+    """Bytes of float32 workspace :func:`paged_attention_window` needs for these sizes."""
+    lib = _native.library()
+    rows = num_queries if max_query_len is None else max_query_len
+    splits = num_splits or lib.pkv_window_splits(
+        num_queries, heads, kv_heads, min(window, _INT32_MAX), min(sinks, _INT32_MAX), max_context_len, min(rows, _INT32_MAX)
+    )
+    need = lib.pkv_window_workspace_bytes(num_queries, heads, head_dim, splits)
+    if splits < 1 or need < 0:
+        raise ValueError("invalid window workspace query")
+    return int(need)

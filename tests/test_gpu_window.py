@@ -1,0 +1,350 @@
+"""paged_attention_window against the float64 definition, at the sizes and masks where it can go wrong."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from oracle.window import window_attention
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [("float32", "float32"), ("float32", "bfloat16"), ("bfloat16", "bfloat16")]
+
+
+def make(runs, heads, kv_heads, dim, block, io, kv, seed=0, scale_k=1.0):
+    """A batch of ``runs`` = (rows, context) per sequence, each run's rows at its last positions."""
+    import torch
+
+    rng = np.random.default_rng(seed)
+    gen = torch.Generator().manual_seed(seed)
+    contexts = np.asarray([c for _, c in runs], np.int32)
+    used = -(-contexts // block)
+    blocks = int(used.sum()) + 3
+    ids = rng.permutation(blocks)
+    tables = np.full((len(runs), max(1, int(used.max())) + 2), -7, np.int32)  # past the used entries: anything
+    at = 0
+    for s, n in enumerate(used):
+        tables[s, :n] = ids[at : at + n]
+        at += n
+    seqs = np.repeat(np.arange(len(runs)), [r for r, _ in runs]).astype(np.int32)
+    positions = np.concatenate([np.arange(c - r, c) for r, c in runs]).astype(np.int32)
+    io, kv = getattr(torch, io), getattr(torch, kv)
+    return {
+        "q": torch.randn((seqs.size, heads, dim), generator=gen).to(io),
+        "k": (scale_k * torch.randn((blocks, block, kv_heads, dim), generator=gen)).to(kv),
+        "v": torch.randn((blocks, block, kv_heads, dim), generator=gen).to(kv),
+        "positions": positions, "seqs": seqs, "tables": tables, "contexts": contexts, "scale": dim**-0.5,
+    }  # fmt: skip
+
+
+def call(device, d, window, sinks, **more):
+    import torch
+
+    from paged_kv_serving_amd import ops
+
+    put = lambda x: (x if isinstance(x, torch.Tensor) else torch.from_numpy(x)).to(device)  # noqa: E731
+    more.setdefault("max_context_len", int(max(1, d["contexts"].max())))
+    return ops.paged_attention_window(put(d["q"]), put(d["positions"]), put(d["seqs"]), put(d["k"]), put(d["v"]), put(d["tables"]), put(d["contexts"]),
+                                      d["scale"], window=window, sinks=sinks, **more)  # fmt: skip
+
+
+def bound(d, want, size):
+    """Of |out - want|. A score is a sum of dim products in float32: off by at most (dim + 4) 2^-24 of
+    scale * sum |q k|, and bfloat16 pieces leave out 2^-24 of a product. That moves a weight by twice
+    as much, relatively; weights are rounded to 2^-17 at most where the output is bfloat16, sums of n
+    terms to n 2^-24; the output is a mean of values, rounded once to its type."""
+    import torch
+
+    keys = int(d["contexts"].max())
+    values = d["v"].float()
+    most = values[torch.isfinite(values)].abs().max().item()
+    scores = (d["q"].shape[2] + 8) * 2.0**-24 * size[..., None]
+    off = most * (2 * np.expm1(2 * scores) + (keys + 16) * 2.0**-24)
+    if d["q"].dtype == torch.bfloat16:
+        off = off + most * 2.0**-16 + np.abs(want) * 2.0**-8
+    return off
+
+
+def check(device, d, window, sinks, **more):
+    got = call(device, d, window, sinks, **more).float().cpu().numpy().astype(np.float64)
+    want, size = window_attention(d["q"].float().numpy(), d["positions"], d["seqs"], d["k"].float().numpy(), d["v"].float().numpy(), d["tables"],
+                                  d["contexts"], d["scale"], window, sinks)  # fmt: skip
+    rows = ~np.isnan(want).all((1, 2))
+    off = np.abs(got - want)[rows]
+    assert (off <= bound(d, want, size)[rows]).all(), f"worst {off.max()} at {np.unravel_index(off.argmax(), off.shape)}"
+    return got
+
+
+@pytest.mark.parametrize("io,kv", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,dim", [(1, 1, 32), (4, 4, 64), (8, 2, 128), (14, 2, 64), (3, 1, 256), (64, 1, 32), (40, 2, 64)])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (16, 0), (33, 4), (1000, 3)])
+def test_decode_rows(device, io, kv, heads, kv_heads, dim, window, sinks):
+    d = make([(1, 1), (1, 5), (1, 33), (1, 100), (1, 257)], heads, kv_heads, dim, 16, io, kv, seed=heads + dim)
+    check(device, d, window, sinks, max_query_len=1)
+    check(device, d, window, sinks)
+
+
+@pytest.mark.parametrize("io,kv", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,dim", [(2, 2, 32), (4, 4, 64), (8, 2, 128), (7, 1, 64), (2, 1, 256), (64, 1, 32)])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (24, 0), (64, 5), (1000, 2)])
+def test_prompt_chunks(device, io, kv, heads, kv_heads, dim, window, sinks):
+    d = make([(70, 70), (33, 150), (9, 9), (130, 131)], heads, kv_heads, dim, 16, io, kv, seed=heads + dim)
+    check(device, d, window, sinks)
+
+
+@pytest.mark.parametrize("io,kv", TYPES)
+@pytest.mark.parametrize("block", [1, 3, 16, 64, 200])
+def test_mixed_batches_and_block_sizes(device, io, kv, block):
+    d = make([(1, 300), (45, 90), (1, 64), (3, 65), (1, 1), (2, 2), (80, 333), (1, 17)], 8, 2, 64, block, io, kv, seed=block)
+    for window, sinks in ((50, 0), (50, 7), (400, 0)):
+        check(device, d, window, sinks)
+
+
+@pytest.mark.parametrize("io,kv", TYPES)
+@pytest.mark.parametrize("splits", [1, 2, 3, 7, 64])
+def test_splits_agree_with_the_definition(device, io, kv, splits):
+    d = make([(1, 700), (1, 3), (40, 500), (1, 129)], 8, 2, 128, 16, io, kv, seed=splits)
+    for window, sinks in ((1, 2), (90, 4), (5000, 0)):
+        check(device, d, window, sinks, num_splits=splits)
+
+
+@pytest.mark.parametrize("sinks", [0, 1, 30, 31, 32, 33, 64, 100, 10_000])
+def test_sinks_meet_the_window(device, sinks):
+    """Sinks below, next to, inside and past the window, where no key may count twice."""
+    d = make([(1, 96), (1, 64), (40, 96), (1, 32)], 4, 2, 64, 16, "float32", "float32", seed=1)
+    check(device, d, 32, sinks)
+
+
+def test_rows_that_see_nothing_are_zeros(device):
+    import torch
+
+    for io, kv in TYPES:
+        d = make([(1, 40), (1, 20), (30, 60)], 4, 2, 64, 16, io, kv)
+        d["positions"][0] = -1
+        d["contexts"][1] = 0
+        d["positions"][5:9] = -5  # rows of a run too
+        got = check(device, d, 8, 2)
+        assert not got[0].any() and not got[1].any() and not got[5:9].any() and got[2].any()
+        assert torch.isfinite(torch.from_numpy(got)).all()
+
+
+def test_positions_past_the_context_and_a_smaller_limit(device):
+    """A row behind its context: the window goes by its position; max_context_len cuts every context."""
+    d = make([(1, 50), (20, 70)], 4, 2, 64, 16, "float32", "float32")
+    d["positions"][0] = 55
+    check(device, d, 20, 3)
+    d["positions"][0] = 400  # its window lies past the context: only sinks are left
+    check(device, d, 20, 3)
+    got = check(device, d, 20, 0)
+    assert not got[0].any()
+    d["contexts"] = np.minimum(d["contexts"], 37).astype(np.int32)
+    want = check(device, d, 20, 3)
+    d["contexts"] = np.asarray([50, 70], np.int32)
+    np.testing.assert_array_equal(call(device, d, 20, 3, max_context_len=37).cpu().numpy(), want.astype(np.float32))
+
+
+@pytest.mark.parametrize("io,kv", TYPES)
+def test_rows_in_any_order(device, io, kv):
+    """Rows of sequences interleaved and out of order, a run with a gap, one sequence twice."""
+    d = make([(20, 90), (1, 40), (30, 200)], 4, 2, 64, 16, io, kv)
+    order = np.random.default_rng(3).permutation(51)
+    order = np.concatenate([order, np.arange(8, 20), np.arange(50, 20, -1)])
+    d["q"], d["positions"], d["seqs"] = d["q"][order], d["positions"][order], d["seqs"][order]
+    check(device, d, 25, 3)
+
+
+@pytest.mark.parametrize("io,kv", TYPES)
+def test_padding_rows_are_left_as_they_were(device, io, kv):
+    import torch
+
+    d = make([(1, 40), (30, 60), (1, 30)], 4, 2, 64, 16, io, kv)
+    d["seqs"][10:14], d["seqs"][-1], d["seqs"][0] = -1, 3, 2**31 - 1
+    for splits in (1, 4):
+        out = torch.full((32, 4, 64), 5.0, dtype=d["q"].dtype, device=device)
+        check(device, d, 16, 2, out=out, num_splits=splits)
+        kept = out.float().cpu().numpy()
+        assert (kept[10:14] == 5.0).all() and (kept[-1] == 5.0).all() and (kept[0] == 5.0).all()
+
+
+@pytest.mark.parametrize("io,kv", TYPES)
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_bad_values_in_hidden_places_reach_no_output(device, io, kv, bad):
+    """Keys and values that no row may see, in blocks that are read: before the window, behind it, in
+    blocks of the pool that no table names, and, within a run, those that only other rows see."""
+    d = make([(1, 100), (40, 100)], 4, 2, 64, 16, io, kv)
+    clean = call(device, d, 24, 3).float().cpu()
+    flat = lambda s, j: (d["tables"][s, j // 16], j % 16)  # noqa: E731
+    for s, hidden in ((0, (3, 40, 75)), (1, (3, 20, 36))):  # between the sinks and the first row's window
+        for j in hidden:
+            d["k"][flat(s, j)] = bad
+            d["v"][flat(s, j)] = bad
+    unused = [b for b in range(d["k"].shape[0]) if b not in set(d["tables"][d["tables"] >= 0].tolist())]
+    d["k"][unused] = bad
+    d["v"][unused] = bad
+    # The last block of a sequence has slots past its context.
+    d["k"][d["tables"][0, 6], 4:] = bad
+    d["v"][d["tables"][0, 6], 4:] = bad
+    got = call(device, d, 24, 3).float().cpu()
+    assert (got == clean).all()
+    # A value in the middle of the run: rows before it and rows a window behind it do not see it.
+    j = 70
+    d["v"][flat(1, j)] = bad
+    got = call(device, d, 24, 3).float().cpu()
+    pos = d["positions"]
+    sees = (d["seqs"] == 1) & (pos >= j) & (pos < j + 24)
+    off = (got - clean).abs()[~sees]
+    step = 2.0**-8 if d["q"].dtype != d["q"].float().dtype else 2.0**-20
+    assert (off <= step * (1 + clean.abs()[~sees])).all()
+    assert not np.isfinite(got[sees].numpy()).all((1, 2)).any()
+
+
+@pytest.mark.parametrize("io,kv", TYPES)
+def test_blocks_outside_the_pool_are_skipped(device, io, kv):
+    d = make([(1, 100), (40, 100), (1, 20)], 4, 2, 64, 16, io, kv)
+    d["tables"][0, 3], d["tables"][1, 2], d["tables"][1, 5], d["tables"][2, :2] = -1, 10**6, -5, 2**31 - 1
+    got = check(device, d, 60, 3)
+    assert not got[-1].any()  # nothing left to see
+    check(device, d, 60, 3, num_splits=3)
+
+
+@pytest.mark.parametrize("io,kv", TYPES)
+def test_large_scores_do_not_overflow(device, io, kv):
+    d = make([(1, 120), (40, 120)], 4, 2, 64, 16, io, kv, scale_k=300.0)
+    got = call(device, d, 50, 2).float().cpu().numpy()
+    assert np.isfinite(got).all()
+    d = make([(1, 120), (40, 120)], 4, 2, 64, 16, io, kv, scale_k=0.0)
+    check(device, d, 50, 2)
+
+
+def test_queries_with_a_token_stride_and_many_rows(device):
+    import torch
+
+    d = make([(1, 30)] * 70, 8, 2, 64, 16, "bfloat16", "bfloat16")
+    fused = torch.randn((70, 12, 64)).to(torch.bfloat16)
+    d["q"] = fused[:, :8]
+    want = check(device, d, 12, 1)
+    got = call(device, {**d, "q": fused.to(device)[:, :8]}, 12, 1)
+    np.testing.assert_array_equal(got.float().cpu().numpy(), want.astype(np.float32))
+
+
+def test_results_do_not_depend_on_the_hints(device):
+    """Decode rows: the same bits with any max_query_len; a run: as near as the definition asks."""
+    d = make([(1, 90), (1, 30), (50, 200)], 8, 2, 64, 16, "bfloat16", "bfloat16")
+    for hint in (1, 2, 50, 10_000):
+        check(device, d, 40, 2, max_query_len=hint, num_splits=1)
+
+
+def test_twice_the_same_bits(device):
+    for io, kv in TYPES:
+        d = make([(1, 900), (77, 400), (1, 30)], 8, 2, 64, 16, io, kv)
+        first = call(device, d, 300, 4, num_splits=5)
+        assert (first == call(device, d, 300, 4, num_splits=5)).all()
+
+
+def test_offsets_past_32_bits(device):
+    """A pool of more than 2^32 elements: rows in its last blocks."""
+    import torch
+
+    from paged_kv_serving_amd import ops
+
+    heads, dim, block = 8, 128, 16
+    blocks = (1 << 32) // (heads * dim * block) + 64
+    k = torch.empty((blocks, block, heads, dim), dtype=torch.bfloat16, device=device)
+    v = torch.empty((blocks, block, heads, dim), dtype=torch.bfloat16, device=device)
+    d = make([(1, 100), (30, 90)], 16, heads, dim, block, "bfloat16", "bfloat16")
+    used = d["k"].shape[0]
+    k[-used:], v[-used:] = d["k"].to(device), d["v"].to(device)
+    want = call(device, d, 40, 3)
+    tables = torch.from_numpy(np.where(d["tables"] >= 0, d["tables"] + blocks - used, -1).astype(np.int32)).to(device)
+    got = ops.paged_attention_window(d["q"].to(device), torch.from_numpy(d["positions"]).to(device), torch.from_numpy(d["seqs"]).to(device), k, v, tables,
+                                     torch.from_numpy(d["contexts"]).to(device), d["scale"], window=40, sinks=3, max_context_len=100)  # fmt: skip
+    assert torch.equal(got, want)
+
+
+def test_captured_and_replayed_with_another_batch(device):
+    """One graph, batches of another composition: the call reads the batch on the device alone."""
+    import torch
+
+    from paged_kv_serving_amd import ops
+
+    runs = [[(1, 300), (40, 200), (1, 50), (20, 90)], [(30, 222), (1, 10), (30, 290), (1, 1)], [(1, 5), (1, 6), (1, 7), (59, 300)]]
+    cases = [make(r, 8, 2, 64, 16, "bfloat16", "bfloat16", seed=i) for i, r in enumerate(runs)]
+    width = -(-300 // 16)
+    blocks = max(c["k"].shape[0] for c in cases)
+    buf = {
+        "q": torch.zeros((62, 8, 64), dtype=torch.bfloat16, device=device), "k": torch.zeros((blocks, 16, 2, 64), dtype=torch.bfloat16, device=device),
+        "v": torch.zeros((blocks, 16, 2, 64), dtype=torch.bfloat16, device=device), "positions": torch.zeros(62, dtype=torch.int32, device=device),
+        "seqs": torch.full((62,), -1, dtype=torch.int32, device=device), "tables": torch.zeros((4, width), dtype=torch.int32, device=device),
+        "contexts": torch.zeros(4, dtype=torch.int32, device=device),
+    }  # fmt: skip
+    out = torch.zeros((62, 8, 64), dtype=torch.bfloat16, device=device)
+    need = ops.window_workspace_bytes(62, 8, 2, 64, window=64, sinks=3, max_context_len=300, num_splits=3)
+    workspace = torch.empty(max(1, need // 4), device=device)
+
+    def run():
+        ops.paged_attention_window(buf["q"], buf["positions"], buf["seqs"], buf["k"], buf["v"], buf["tables"], buf["contexts"], 0.125, window=64, sinks=3,
+                                   max_context_len=300, num_splits=3, out=out, workspace=workspace)  # fmt: skip
+
+    run()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    for d in cases * 2:
+        for name in ("q", "k", "v"):
+            buf[name][: d[name].shape[0]].copy_(d[name])
+        for name in ("positions", "seqs", "contexts"):
+            buf[name].copy_(torch.from_numpy(d[name]))
+        buf["tables"].zero_()
+        cols = min(width, d["tables"].shape[1])
+        buf["tables"][:, :cols].copy_(torch.from_numpy(d["tables"][:, :cols]))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, call(device, d, 64, 3, num_splits=3, max_context_len=300))
+
+
+def test_two_calls_at_once(device):
+    """Calls on two streams, each with a workspace of its own."""
+    import torch
+
+    batches = [make([(1, 800), (60, 500)], 8, 2, 64, 16, "bfloat16", "bfloat16", seed=s) for s in (1, 2)]
+    want = [call(device, d, 300, 4, num_splits=4) for d in batches]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for d, stream in zip(batches, streams):
+        with torch.cuda.stream(stream):
+            got.append(call(device, d, 300, 4, num_splits=4))
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+def test_no_rows_no_context_and_refusals(device):
+    import torch
+
+    from paged_kv_serving_amd import ops
+
+    d = make([(1, 20), (3, 30)], 4, 2, 64, 16, "float32", "float32")
+    empty = {**d, "q": d["q"][:0], "positions": d["positions"][:0], "seqs": d["seqs"][:0]}
+    assert call(device, empty, 4, 0).shape == (0, 4, 64)
+    assert not call(device, {**d, "contexts": np.zeros(2, np.int32)}, 4, 0, max_context_len=0).any()
+    bad = [
+        ({}, {"window": 0}), ({}, {"sinks": -1}), ({}, {"num_splits": 65}), ({}, {"num_splits": -1}), ({}, {"max_query_len": -1}), ({}, {"max_context_len": 10_000}),
+        ({}, {"out": torch.zeros((4, 4, 64), device=device, dtype=torch.bfloat16)}), ({}, {"num_splits": 2, "workspace": torch.zeros(4, device=device)}),
+        ({}, {"num_splits": 2, "workspace": torch.zeros(10**6)}),
+        ({"q": d["q"].half()}, {}), ({"q": d["q"].bfloat16()}, {}), ({"q": d["q"][:, :3]}, {}), ({"k": d["k"].bfloat16()}, {}), ({"seqs": d["seqs"].astype(np.int64)}, {}),
+        ({"positions": d["positions"][:2]}, {}), ({"tables": d["tables"].astype(np.int64)}, {}), ({"contexts": d["contexts"][:1]}, {}),
+        ({"q": d["q"].transpose(0, 1)}, {}), ({"k": d["k"][0], "v": d["v"][0]}, {}),
+    ]  # fmt: skip
+    for change, more in bad:
+        more = {"window": 4, "sinks": 0, **more}
+        with pytest.raises(ValueError):
+            call(device, {**d, **change}, **more)
+    big = make([(1, 20)], 65, 1, 32, 16, "float32", "float32")
+    with pytest.raises(ValueError):
+        call(device, big, 4, 0)
+    odd = make([(1, 20)], 2, 1, 48, 16, "float32", "float32")
+    with pytest.raises(Exception, match="unsupported|implemented|shape"):
+        call(device, odd, 4, 0)
+    assert ops.window_workspace_bytes(4, 4, 2, 64, window=4, max_context_len=30, num_splits=1) == 0
