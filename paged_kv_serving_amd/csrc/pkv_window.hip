@@ -7,6 +7,8 @@
 // output's type.
 #include <math.h>
 
+#include <algorithm>
+
 #include "pkv_common.h"
 
 namespace pkv {
@@ -14,6 +16,16 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / kWave;
+constexpr int kTileQueries = 128;  // (row, head) pairs of a tile
+constexpr int kMinRun = PKV_WINDOW_MIN_RUN;
+
+typedef float floatx2 __attribute__((ext_vector_type(2)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 struct Window {
   void* out;
@@ -30,6 +42,10 @@ struct Window {
   float* workspace;
   int32_t block_size, table_stride, num_seqs, num_heads, num_kv_heads, group;
   int32_t window, sinks, max_context, splits;
+  int32_t subgroups;       // of up to 16 query heads of a group
+  int32_t tile_rows;       // rows of a tile: the aligned blocks of rows that runs lie in
+  int32_t tiled;           // whether the tile pass computes the runs
+  int32_t rows_per_group;  // rows of a row pass workgroup, one after the other
   float scale_log2;  // scale * log2(e): scores are kept in base 2
 };
 
@@ -38,11 +54,35 @@ __device__ __forceinline__ float load_one(const uint16_t* p) { return __uint_as_
 __device__ __forceinline__ void store_one(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store_one(uint16_t* p, float v) { *p = static_cast<uint16_t>(f32_to_bf16_bits(v)); }
 
+// N adjacent values of an output row.
+template <typename T, int N>
+__device__ __forceinline__ void store_row(T* p, const float (&v)[N]) {
+  if constexpr (sizeof(T) == 4 && N % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) *reinterpret_cast<f32x4*>(p + i) = f32x4{v[i], v[i + 1], v[i + 2], v[i + 3]};
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) p[i] = v[i];
+  } else {
+    uint32_t w[N / 2];
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) w[i] = f32_to_bf16_bits(v[2 * i]) | (f32_to_bf16_bits(v[2 * i + 1]) << 16);
+    if constexpr (N == 8) {
+      *reinterpret_cast<u32x4*>(p) = u32x4{w[0], w[1], w[2], w[3]};
+    } else if constexpr (N == 4) {
+      *reinterpret_cast<u32x2*>(p) = u32x2{w[0], w[1]};
+    } else {
+      *reinterpret_cast<uint32_t*>(p) = w[0];
+    }
+  }
+}
+
 // The keys a row sees: [0, sinks) and [begin, end), or nothing.
 struct Span {
   int32_t sinks, begin, end;
   __device__ __forceinline__ int32_t count() const { return sinks + end - begin; }
   __device__ __forceinline__ int32_t key(int32_t i) const { return i < sinks ? i : begin + (i - sinks); }
+  __device__ __forceinline__ bool sees(int32_t key) const { return key < end && (key >= begin || key < sinks); }
 };
 
 __device__ __forceinline__ Span span_of(const Window& a, int32_t seq, int32_t pos) {
@@ -55,73 +95,510 @@ __device__ __forceinline__ Span span_of(const Window& a, int32_t seq, int32_t po
   return s;
 }
 
-// Element offset of a key's row of one head in the pools; -1 in a block outside the pool.
-__device__ __forceinline__ int64_t row_of(const Window& a, const int32_t* table, int32_t key, int32_t kv_head, int d) {
-  const int32_t page = key / a.block_size;
-  const int64_t block = table[page];
+// Slot (block * block_size + offset) of a key; -1 in a block outside the pool.
+__device__ __forceinline__ int32_t slot_of(const Window& a, const int32_t* table, int32_t key) {
+  const uint32_t page = static_cast<uint32_t>(key) / static_cast<uint32_t>(a.block_size);
+  const int32_t block = table[page];
   if (block < 0 || block >= a.num_blocks) return -1;
-  return ((block * a.block_size + (key - page * a.block_size)) * a.num_kv_heads + kv_head) * d;
+  return block * a.block_size + (key - static_cast<int32_t>(page) * a.block_size);
 }
 
-// One wavefront per (row, head), 64 keys at a time: a lane scores one key, then owns dimensions.
+// Element offset of a slot's row of one head in the pools.
+__device__ __forceinline__ int64_t row_of(const Window& a, int32_t slot, int32_t kv_head, int d) {
+  return (static_cast<int64_t>(slot) * a.num_kv_heads + kv_head) * d;
+}
+
+// A row's split results in the workspace: maxima, sums, then the unnormalised outputs.
+__device__ __forceinline__ int64_t split_index(const Window& a, int64_t t, int32_t head, int32_t split) {
+  return (t * a.num_heads + head) * a.splits + split;
+}
+__device__ __forceinline__ float* split_acc(const Window& a, int64_t index, int d) {
+  return a.workspace + 2 * a.num_queries * a.num_heads * a.splits + index * d;
+}
+__device__ __forceinline__ void store_split_sums(const Window& a, int64_t index, float top, float sum) {
+  a.workspace[index] = top;
+  a.workspace[a.num_queries * a.num_heads * a.splits + index] = sum;
+}
+
+// The maximum / sum over the four lanes {n, n + 16, n + 32, n + 48}, in each of them.
+__device__ __forceinline__ float column_max(float x) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float column_sum(float x) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// Three bfloat16 pieces of pairs of floats, each the next 8 significant bits rounded to nearest:
+// their sum is the float. What is not finite is its first piece alone.
+__device__ __forceinline__ uint32_t take_piece(float& x0, float& x1) {
+  const uint32_t pair = __builtin_bit_cast(uint32_t, __builtin_convertvector((floatx2{x0, x1}), bf16x2));
+  const float h0 = bf16_lo(pair), h1 = bf16_hi(pair);
+  x0 = fabsf(h0) < INFINITY ? x0 - h0 : 0.f;
+  x1 = fabsf(h1) < INFINITY ? x1 - h1 : 0.f;
+  return pair;
+}
+
+// ---------------------------------------------------------------------------------------------
+// One (row, head) over items [first, last) of a span, by the definition: a wavefront, 64 keys at a
+// time; a lane scores one key, then owns dimensions. For rows that the matrix products cannot
+// serve: an infinity or NaN does not survive being cut into pieces, and 0 * inf is not 0.
+// ---------------------------------------------------------------------------------------------
 template <typename QT, typename KVT, int D>
-__global__ __launch_bounds__(kThreads) void plain_kernel(const Window a) {
+__device__ __attribute__((noinline)) void exact_row(const Window& a, int64_t t, int32_t head, int32_t seq, Span own, Span keys,
+                                                    int32_t first, int32_t last, int32_t split) {
   constexpr int kOwn = (D + kWave - 1) / kWave;
   const int lane = threadIdx.x & (kWave - 1);
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * kWaves + threadIdx.x / kWave;
-  const int64_t t = item / a.num_heads;
-  if (t >= a.num_queries) return;
-  const int32_t head = static_cast<int32_t>(item - t * a.num_heads);
-  const int32_t seq = a.seqs[t];
-  if (seq < 0 || seq >= a.num_seqs) return;
   const int32_t kv_head = head / a.group;
   const int32_t* table = a.tables + static_cast<int64_t>(seq) * a.table_stride;
-  const Span span = span_of(a, seq, a.positions[t]);
   const QT* q = static_cast<const QT*>(a.queries) + t * a.query_stride + static_cast<int64_t>(head) * D;
   float top = -INFINITY, sum = 0.f, acc[kOwn] = {};
-  for (int32_t first = 0; first < span.count(); first += kWave) {
-    const bool live = first + lane < span.count();
-    const int64_t row = live ? row_of(a, table, span.key(first + lane), kv_head, D) : -1;
+  for (int32_t at = first; at < last; at += kWave) {
+    const int32_t key = at + lane < last ? keys.key(at + lane) : -1;
+    const int32_t slot = key >= 0 && own.sees(key) ? slot_of(a, table, key) : -1;
     float score = -INFINITY;
-    if (row >= 0) {
-      const KVT* k = static_cast<const KVT*>(a.keys) + row;
+    if (slot >= 0) {
+      const KVT* k = static_cast<const KVT*>(a.keys) + row_of(a, slot, kv_head, D);
       score = 0.f;
       for (int d = 0; d < D; ++d) score += load_one(q + d) * load_one(k + d);
       score *= a.scale_log2;
     }
+    const uint64_t seen = __ballot(slot >= 0);
+    if (seen == 0) continue;
+    // A maximum that keeps NaN: a visible NaN score makes the row NaN.
     float next = score;
     for (int m = kWave / 2; m > 0; m >>= 1) next = fmaxf(next, __shfl_xor(next, m));
     next = fmaxf(top, next);
-    if (next == -INFINITY) continue;
-    const float keep = exp2f(top - next);
-    const float p = row >= 0 ? exp2f(score - next) : 0.f;
+    const float from = next == -INFINITY ? 0.f : next;
+    const float keep = exp2f(top - from);
+    const float p = slot >= 0 ? exp2f(score - from) : 0.f;
     float all = p;
     for (int m = kWave / 2; m > 0; m >>= 1) all += __shfl_xor(all, m);
     sum = sum * keep + all;
     top = next;
     for (int e = 0; e < kOwn; ++e) acc[e] *= keep;
     for (int j = 0; j < kWave; ++j) {
+      if (!((seen >> j) & 1)) continue;
       const float pj = __shfl(p, j);
-      const int64_t rj = __shfl(static_cast<long long>(row), j);
-      if (rj < 0) continue;
+      const KVT* v = static_cast<const KVT*>(a.values) + row_of(a, __shfl(slot, j), kv_head, D);
       for (int e = 0; e < kOwn; ++e) {
         const int d = e * kWave + lane;
-        if (d < D) acc[e] += pj * load_one(static_cast<const KVT*>(a.values) + rj + d);
+        if (d < D) acc[e] += pj * load_one(v + d);
       }
     }
   }
-  QT* out = static_cast<QT*>(a.out) + (t * a.num_heads + head) * D;
+  if (a.splits == 1) {
+    QT* out = static_cast<QT*>(a.out) + (t * a.num_heads + head) * D;
+    for (int e = 0; e < kOwn; ++e) {
+      const int d = e * kWave + lane;
+      if (d < D) store_one(out + d, sum == 0.f ? 0.f : acc[e] / sum);
+    }
+    return;
+  }
+  const int64_t index = split_index(a, t, head, split);
+  if (lane == 0) store_split_sums(a, index, top, sum);
   for (int e = 0; e < kOwn; ++e) {
     const int d = e * kWave + lane;
-    if (d < D) store_one(out + d, sum == 0.f ? 0.f : acc[e] / sum);
+    if (d < D) split_acc(a, index, D)[d] = acc[e];
   }
 }
 
+// ---------------------------------------------------------------------------------------------
+// Rows by themselves (decode): one workgroup per (row, key head, split) and up to 16 of the query
+// heads that share the key head. The row's keys are handed to the four wavefronts kKeys at a time.
+// With lane l = (c = l / 16, n = l % 16):
+//
+//   S^T = K Q^T    16 keys x 16 heads per product, K straight from the pool as the left operand: lane
+//                  (c, n) loads 16 bytes of key n's row. bfloat16 keys: v_mfma_f32_16x16x32_bf16, the
+//                  lane's 8 dimensions are its 8 terms (float32 queries in three pieces); float32 keys:
+//                  v_mfma_f32_16x16x4_f32, its 4 dimensions are 4 steps. Register r of the result is
+//                  the score of key 4c + r for head n.
+//   O^T = V^T P^T  v_mfma_f32_16x16x4_f32, step r taking keys 4c + r of the lane groups c: P is the
+//                  lane's own register r, and V comes straight from the pool too: lane (c, i) loads
+//                  kVWidth adjacent values of key 4c + r and uses them in as many products.
+//
+// So nothing is staged: every key and value row goes from the pool to the registers that multiply it,
+// in float32 throughout, and all heads of a group share one read of it. The loads of the next keys are
+// issued before the present ones are used.
+// ---------------------------------------------------------------------------------------------
 template <typename QT, typename KVT, int D>
-int launch(const Window& a, hipStream_t stream) {
-  const int64_t groups = (a.num_queries * a.num_heads + kWaves - 1) / kWaves;
-  if (groups > 0x7fffffff) return PKV_EUNSUPPORTED;
-  hipLaunchKernelGGL((plain_kernel<QT, KVT, D>), dim3(static_cast<uint32_t>(groups)), dim3(kThreads), 0, stream, a);
+struct RowShape {
+  static constexpr bool kBf16 = sizeof(KVT) == 2;
+  static constexpr int kPieces = kBf16 ? (sizeof(QT) == 4 ? 3 : 1) : 1;
+  static constexpr int kBlocks = kBf16 && D <= 128 ? 2 : 1;  // 16-key blocks per round
+  static constexpr int kKeys = 16 * kBlocks;
+  static constexpr int kKLoads = kBf16 ? D / 32 : D / 16;    // 16-byte loads of a key row per lane
+  static constexpr int kPerLane = D / 16;                    // values of a value row per lane
+  static constexpr int kVWidth = kPerLane < 16 / int(sizeof(KVT)) ? kPerLane : 16 / int(sizeof(KVT));
+  static constexpr int kVLoads = kPerLane / kVWidth;
+  static constexpr int kVWords = kVWidth * int(sizeof(KVT)) / 4;
+  static constexpr int kQRegs = kBf16 ? 4 * kKLoads * kPieces : D / 4;
+};
+
+template <int N>
+struct Words {
+  uint32_t w[N];
+};
+
+template <int N>
+__device__ __forceinline__ Words<N> load_words(const void* p) {
+  Words<N> x;
+  if constexpr (N == 4) {
+    const u32x4 v = __builtin_nontemporal_load(static_cast<const u32x4*>(p));
+    x.w[0] = v.x, x.w[1] = v.y, x.w[2] = v.z, x.w[3] = v.w;
+  } else if constexpr (N == 2) {
+    const u32x2 v = __builtin_nontemporal_load(static_cast<const u32x2*>(p));
+    x.w[0] = v.x, x.w[1] = v.y;
+  } else {
+    x.w[0] = __builtin_nontemporal_load(static_cast<const uint32_t*>(p));
+  }
+  return x;
+}
+
+// Whether row t lies in a run that the tile pass computes: kMinRun rows or more of one sequence next
+// to each other inside one of the aligned blocks of rows that the tile pass goes by.
+__device__ __forceinline__ bool in_run(const Window& a, int64_t t, int32_t seq) {
+  const int64_t begin = t / a.tile_rows * a.tile_rows;
+  const int64_t end = min(begin + a.tile_rows, a.num_queries);
+  int length = 1;
+  for (int64_t i = t - 1; i >= begin && length < kMinRun && a.seqs[i] == seq; --i) ++length;
+  for (int64_t i = t + 1; i < end && length < kMinRun && a.seqs[i] == seq; ++i) ++length;
+  return length >= kMinRun;
+}
+
+template <typename QT, typename KVT, int D>
+__global__ __launch_bounds__(kThreads) void row_kernel(const Window a) {
+  using S = RowShape<QT, KVT, D>;
+  constexpr int kTiles = D / 16;  // output tiles of 16 dimensions
+  __shared__ float s_acc[2][kTiles * 4 * kWave];
+  __shared__ float s_top[kWaves][kWave], s_sum[kWaves][kWave];
+  __shared__ int s_redo;
+  const int lane = threadIdx.x & (kWave - 1), c = lane / 16, n = lane % 16;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  uint32_t item = blockIdx.x;
+  const int32_t kv_head = item % static_cast<uint32_t>(a.num_kv_heads);
+  item /= static_cast<uint32_t>(a.num_kv_heads);
+  const int32_t sub = item % static_cast<uint32_t>(a.subgroups);
+  item /= static_cast<uint32_t>(a.subgroups);
+  const int32_t split = item % static_cast<uint32_t>(a.splits);
+  const int64_t row0 = static_cast<int64_t>(item / static_cast<uint32_t>(a.splits)) * a.rows_per_group;
+  const int32_t heads = min(16, a.group - sub * 16);
+  const int32_t head0 = kv_head * a.group + sub * 16;
+  const auto* keys = static_cast<const char*>(a.keys);
+  const auto* values = static_cast<const char*>(a.values);
+  const int64_t row_bytes = static_cast<int64_t>(a.num_kv_heads) * D * sizeof(KVT);
+  const int64_t k_at = (static_cast<int64_t>(kv_head) * D + (S::kBf16 ? 8 : 4) * c) * sizeof(KVT);
+  const int64_t v_at = (static_cast<int64_t>(kv_head) * D + S::kVWidth * n) * sizeof(KVT);
+
+  for (int64_t t = row0; t < min(row0 + a.rows_per_group, a.num_queries); ++t) {
+    const int32_t seq = a.seqs[t];
+    if (seq < 0 || seq >= a.num_seqs || (a.tiled && in_run(a, t, seq))) continue;
+    const int32_t* table = a.tables + static_cast<int64_t>(seq) * a.table_stride;
+    const Span span = span_of(a, seq, a.positions[t]);
+    const int32_t count = span.count();
+    const int32_t rounds = (count + S::kKeys - 1) / S::kKeys;
+    const int32_t first = static_cast<int32_t>(static_cast<int64_t>(rounds) * split / a.splits);
+    const int32_t last = static_cast<int32_t>(static_cast<int64_t>(rounds) * (split + 1) / a.splits);
+
+    // The queries, the right operand of S^T: lane (c, n) holds its c's dimensions of head n.
+    uint32_t qr[S::kQRegs];
+    {
+      const QT* q = static_cast<const QT*>(a.queries) + t * a.query_stride + static_cast<int64_t>(head0 + min(n, heads - 1)) * D;
+      if constexpr (S::kBf16 && sizeof(QT) == 2) {
+#pragma unroll
+        for (int u = 0; u < S::kKLoads; ++u) {
+          const u32x4 x = *reinterpret_cast<const u32x4*>(q + 32 * u + 8 * c);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) qr[4 * u + e] = x[e];
+        }
+      } else if constexpr (S::kBf16) {
+#pragma unroll
+        for (int u = 0; u < S::kKLoads; ++u) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float x0 = q[32 * u + 8 * c + 2 * e] * a.scale_log2, x1 = q[32 * u + 8 * c + 2 * e + 1] * a.scale_log2;
+#pragma unroll
+            for (int p = 0; p < 3; ++p) qr[4 * (p * S::kKLoads + u) + e] = take_piece(x0, x1);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int u = 0; u < S::kKLoads; ++u) {
+          const f32x4 x = *reinterpret_cast<const f32x4*>(q + 16 * u + 4 * c);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) qr[4 * u + e] = __float_as_uint(x[e] * a.scale_log2);
+        }
+      }
+    }
+
+    floatx4 o[kTiles];
+#pragma unroll
+    for (int b = 0; b < kTiles; ++b) o[b] = floatx4{0.f, 0.f, 0.f, 0.f};
+    float top = -INFINITY, sum = 0.f;
+
+    // Slot of the key that this lane looks up for a round (lanes past kKeys repeat).
+    auto look_up = [&](int32_t round) {
+      const int32_t i = round * S::kKeys + lane % S::kKeys;
+      return round < last && i < count ? slot_of(a, table, span.key(i)) : -1;
+    };
+    Words<4> kx[S::kBlocks][S::kKLoads];
+    Words<S::kVWords> vx[S::kBlocks][4][S::kVLoads];
+    auto load_keys = [&](int32_t slot) {
+#pragma unroll
+      for (int j = 0; j < S::kBlocks; ++j) {
+        const char* p = keys + max(__shfl(slot, 16 * j + n), 0) * row_bytes + k_at;
+#pragma unroll
+        for (int u = 0; u < S::kKLoads; ++u) kx[j][u] = load_words<4>(p + u * 64);
+      }
+    };
+    auto load_values = [&](int32_t slot) {
+#pragma unroll
+      for (int j = 0; j < S::kBlocks; ++j) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const char* p = values + max(__shfl(slot, 16 * j + 4 * c + r), 0) * row_bytes + v_at;
+#pragma unroll
+          for (int g = 0; g < S::kVLoads; ++g) vx[j][r][g] = load_words<S::kVWords>(p + g * 16 * S::kVWidth * int(sizeof(KVT)));
+        }
+      }
+    };
+
+    constexpr uint64_t kAll = S::kKeys == 32 ? 0xffffffffull : 0xffffull;
+    int32_t round = first + wave;
+    int32_t slot = look_up(round);
+    uint32_t live = static_cast<uint32_t>(__ballot(slot >= 0) & kAll);  // the round's keys that count
+    if (live != 0) {
+      load_keys(slot);
+      load_values(slot);
+    }
+    int32_t slot_next = look_up(round + kWaves);
+    for (; round < last; round += kWaves) {
+      const uint32_t live_next = static_cast<uint32_t>(__ballot(slot_next >= 0) & kAll);
+      floatx4 st[S::kBlocks];
+      if (live != 0) {
+#pragma unroll
+        for (int j = 0; j < S::kBlocks; ++j) {
+          st[j] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int u = 0; u < S::kKLoads; ++u) {
+            if constexpr (S::kBf16) {
+#pragma unroll
+              for (int p = S::kPieces - 1; p >= 0; --p) {  // the smallest pieces first
+                const uint32_t* q = qr + 4 * (p * S::kKLoads + u);
+                st[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kx[j][u]),
+                                                                __builtin_bit_cast(bf16x8, (u32x4{q[0], q[1], q[2], q[3]})), st[j], 0, 0, 0);
+              }
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                st[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kx[j][u].w[e]), __uint_as_float(qr[4 * u + e]), st[j], 0, 0, 0);
+              }
+            }
+          }
+        }
+      }
+      if (live_next != 0) load_keys(slot_next);
+      if (live != 0) {
+        float most = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < S::kBlocks; ++j) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            if constexpr (sizeof(QT) == 2) st[j][r] *= a.scale_log2;
+            if (live != kAll && !((live >> (16 * j + 4 * c + r)) & 1)) st[j][r] = -INFINITY;
+            most = fmaxf(most, st[j][r]);
+          }
+        }
+        most = column_max(most);
+        if (__ballot(most > top) != 0) {
+          const float next = fmaxf(top, most);
+          const float keep = next == -INFINITY ? 1.f : fast_exp2(top - next);
+          sum *= keep;
+#pragma unroll
+          for (int b = 0; b < kTiles; ++b) o[b] *= keep;
+          top = next;
+        }
+        const float from = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int j = 0; j < S::kBlocks; ++j) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            st[j][r] = fast_exp2(st[j][r] - from);
+            sum += st[j][r];
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < S::kBlocks; ++j) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            if (live != kAll && !((live >> (16 * j + 4 * c + r)) & 1)) {  // 0 * inf is not 0
+#pragma unroll
+              for (int g = 0; g < S::kVLoads; ++g) {
+#pragma unroll
+                for (int w = 0; w < S::kVWords; ++w) vx[j][r][g].w[w] = 0;
+              }
+            }
+#pragma unroll
+            for (int g = 0; g < S::kVLoads; ++g) {
+#pragma unroll
+              for (int e = 0; e < S::kVWidth; ++e) {
+                float v;
+                if constexpr (S::kBf16) {
+                  v = e % 2 ? bf16_hi(vx[j][r][g].w[e / 2]) : bf16_lo(vx[j][r][g].w[e / 2]);
+                } else {
+                  v = __uint_as_float(vx[j][r][g].w[e]);
+                }
+                o[g * S::kVWidth + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, st[j][r], o[g * S::kVWidth + e], 0, 0, 0);
+              }
+            }
+          }
+        }
+      }
+      if (live_next != 0) load_values(slot_next);
+      live = live_next;
+      slot_next = look_up(round + 2 * kWaves);
+    }
+    sum = column_sum(sum);
+
+    // The four wavefronts' results, lane by lane: every wavefront holds the same places.
+    __syncthreads();  // the row before has been read
+    s_top[wave][lane] = top;
+    s_sum[wave][lane] = sum;
+    __syncthreads();
+    float all = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) all = fmaxf(all, s_top[w][lane]);
+    const float base = all == -INFINITY ? 0.f : all;
+    const float mine = fast_exp2(top - base);
+#pragma unroll
+    for (int b = 0; b < kTiles; ++b) o[b] *= mine;
+    sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) sum += s_sum[w][lane] * fast_exp2(s_top[w][lane] - base);
+#pragma unroll
+    for (int half = kWaves / 2; half > 0; half /= 2) {
+      if (wave >= half && wave < 2 * half) {
+#pragma unroll
+        for (int b = 0; b < kTiles; ++b) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s_acc[wave - half][(b * 4 + r) * kWave + lane] = o[b][r];
+        }
+      }
+      __syncthreads();
+      if (wave < half) {
+#pragma unroll
+        for (int b = 0; b < kTiles; ++b) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) o[b][r] += s_acc[wave][(b * 4 + r) * kWave + lane];
+        }
+      }
+      __syncthreads();
+    }
+    if constexpr (S::kPieces > 1) {  // what is not finite is computed again from whole numbers
+      if (wave == 0) {
+        bool bad = false;
+#pragma unroll
+        for (int b = 0; b < kTiles; ++b) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) bad = bad || !(fabsf(o[b][r]) < INFINITY);
+        }
+        const uint64_t any = __ballot((bad || !(fabsf(sum) < INFINITY)) && n < heads);
+        if (lane == 0) s_redo = any != 0;
+      }
+      __syncthreads();
+      if (s_redo) {
+        for (int g = wave; g < heads; g += kWaves) {
+          exact_row<QT, KVT, D>(a, t, head0 + g, seq, span, span, min(first * S::kKeys, count), min(last * S::kKeys, count), split);
+        }
+        continue;
+      }
+    }
+    if (wave != 0 || n >= heads) continue;
+    // Register r of output tile (g, e) is dimension 16 kVWidth g + kVWidth (4c + r) + e of head n.
+    const int64_t out_row = t * a.num_heads + head0 + n;
+    if (a.splits == 1) {
+      const float scale = sum == 0.f ? 0.f : 1.f / sum;
+      QT* out = static_cast<QT*>(a.out) + out_row * D;
+#pragma unroll
+      for (int g = 0; g < S::kVLoads; ++g) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          float x[S::kVWidth];
+#pragma unroll
+          for (int e = 0; e < S::kVWidth; ++e) x[e] = sum == 0.f ? 0.f : o[g * S::kVWidth + e][r] * scale;
+          store_row<QT, S::kVWidth>(out + 16 * S::kVWidth * g + S::kVWidth * (4 * c + r), x);
+        }
+      }
+    } else {
+      const int64_t index = split_index(a, t, head0 + n, split);
+      if (c == 0) store_split_sums(a, index, all, sum);
+      if (sum == 0.f) continue;
+#pragma unroll
+      for (int g = 0; g < S::kVLoads; ++g) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          float x[S::kVWidth];
+#pragma unroll
+          for (int e = 0; e < S::kVWidth; ++e) x[e] = o[g * S::kVWidth + e][r];
+          store_row<float, S::kVWidth>(split_acc(a, index, D) + 16 * S::kVWidth * g + S::kVWidth * (4 * c + r), x);
+        }
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Joins the splits of every row and head: D / 4 threads each, four dimensions a thread.
+// ---------------------------------------------------------------------------------------------
+template <typename QT, int D>
+__global__ __launch_bounds__(kThreads) void join_kernel(const Window a) {
+  constexpr int kPer = D / 4;
+  const int64_t item = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / kPer;
+  const int d = threadIdx.x % kPer * 4;
+  const int64_t t = item / a.num_heads;
+  if (t >= a.num_queries) return;
+  const int32_t seq = a.seqs[t];
+  if (seq < 0 || seq >= a.num_seqs) return;
+  const int64_t index = item * a.splits;
+  const float* tops = a.workspace + index;
+  const float* sums = a.workspace + a.num_queries * a.num_heads * a.splits + index;
+  float top = -INFINITY;
+  for (int p = 0; p < a.splits; ++p) top = fmaxf(top, tops[p]);
+  const float from = top == -INFINITY ? 0.f : top;
+  float sum = 0.f;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int p = 0; p < a.splits; ++p) {
+    const float part = sums[p];
+    if (part == 0.f) continue;  // no key in this split: its output may hold anything
+    const float weight = exp2f(tops[p] - from);
+    sum += part * weight;
+    acc += *reinterpret_cast<const f32x4*>(split_acc(a, index + p, D) + d) * weight;
+  }
+  float x[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] = sum == 0.f ? 0.f : acc[e] / sum;
+  store_row<QT, 4>(static_cast<QT*>(a.out) + item * D + d, x);
+}
+
+template <typename QT, typename KVT, int D>
+int launch(Window a, hipStream_t stream) {
+  a.subgroups = (a.group + 15) / 16;
+  a.tile_rows = kTileQueries / a.group;
+  a.tiled = 0;
+  a.rows_per_group = 1;
+  const int64_t row_groups = (a.num_queries + a.rows_per_group - 1) / a.rows_per_group;
+  const int64_t groups = row_groups * a.num_kv_heads * a.subgroups * a.splits;
+  const int64_t joins = (a.num_queries * a.num_heads * (D / 4) + kThreads - 1) / kThreads;
+  if (groups > 0x7fffffff || joins > 0x7fffffff) return PKV_EUNSUPPORTED;
+  hipLaunchKernelGGL((row_kernel<QT, KVT, D>), dim3(static_cast<uint32_t>(groups)), dim3(kThreads), 0, stream, a);
+  if (a.splits > 1) {
+    hipLaunchKernelGGL((join_kernel<QT, D>), dim3(static_cast<uint32_t>(joins)), dim3(kThreads), 0, stream, a);
+  }
   return check_launch();
 }
 
@@ -145,7 +622,10 @@ extern "C" int32_t pkv_window_splits(int64_t num_queries, int32_t num_heads, int
       sinks < 0 || max_context_len < 0 || max_query_len < 0) {
     return PKV_EINVAL;
   }
-  return 1;
+  const int64_t longest = std::min<int64_t>(max_context_len, static_cast<int64_t>(window) + sinks);
+  const int64_t groups = std::max<int64_t>(1, num_queries * num_kv_heads * ((num_heads / num_kv_heads + 15) / 16));
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(PKV_WINDOW_MAX_SPLITS, longest / 128));
+  return static_cast<int32_t>(std::min<int64_t>(most, (768 + groups - 1) / groups));
 }
 
 extern "C" int64_t pkv_window_workspace_bytes(int64_t num_queries, int32_t num_heads, int32_t head_dim, int32_t num_splits) {
@@ -170,6 +650,7 @@ extern "C" int pkv_window_attention(const pkv_window* args, int device, void* st
   if (g.q_dtype == PKV_BF16 && g.kv_dtype == PKV_F32) return PKV_EUNSUPPORTED;
   if (g.head_dim != 32 && g.head_dim != 64 && g.head_dim != 128 && g.head_dim != 256) return PKV_EUNSUPPORTED;
   if (g.num_heads / g.num_kv_heads > PKV_WINDOW_MAX_GROUP) return PKV_EUNSUPPORTED;
+  if (g.num_blocks * g.block_size > 0x7fffffff) return PKV_EUNSUPPORTED;  // slots are 32-bit
   if (g.num_queries == 0) return PKV_OK;
   if (!g.out || !g.queries || !g.query_positions || !g.query_seq || !g.key_cache || !g.value_cache || !g.block_tables ||
       !g.context_lens) {
