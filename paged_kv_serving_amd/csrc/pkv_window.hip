@@ -18,10 +18,13 @@ constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / kWave;
 constexpr int kTileQueries = 128;  // (row, head) pairs of a tile
 constexpr int kMinRun = PKV_WINDOW_MIN_RUN;
+constexpr float kLazyLog2 = 8.f;
 
 typedef float floatx2 __attribute__((ext_vector_type(2)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef float floatx16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short short4v __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -47,6 +50,10 @@ struct Window {
   int32_t tiled;           // whether the tile pass computes the runs
   int32_t rows_per_group;  // rows of a row pass workgroup, one after the other
   float scale_log2;  // scale * log2(e): scores are kept in base 2
+  float given_scale;  // the same before the next two
+  // A negative scale of bfloat16 queries turns their signs instead, so that the largest product is the
+  // largest score; a zero one clears them, so that a hidden key's -inf stays what it is.
+  uint32_t keep, flip;
 };
 
 __device__ __forceinline__ float load_one(const float* p) { return *p; }
@@ -78,10 +85,25 @@ __device__ __forceinline__ void store_row(T* p, const float (&v)[N]) {
 }
 
 // The keys a row sees: [0, sinks) and [begin, end), or nothing.
+__device__ __forceinline__ uint32_t bits_between(int32_t low, int32_t high) {  // of [low, high) in 0 .. 31
+  low = max(low, 0);
+  high = min(high, 32);
+  return low < high ? (0xffffffffu >> (32 - (high - low))) << low : 0u;
+}
+
 struct Span {
   int32_t sinks, begin, end;
   __device__ __forceinline__ int32_t count() const { return sinks + end - begin; }
   __device__ __forceinline__ int32_t key(int32_t i) const { return i < sinks ? i : begin + (i - sinks); }
+  // Which of items at .. at + 31 of a span of more rows this row sees.
+  __device__ __forceinline__ uint32_t seen_of(const Span& all, int32_t at) const {
+    const int32_t first = all.begin - all.sinks + at;  // the key of item `at`, were it past the sinks
+    const uint32_t window = bits_between(begin - first, end - first) | bits_between(-first, sinks - first);
+    if (at >= all.sinks) return window;
+    const uint32_t early = bits_between(begin - at, end - at) | bits_between(-at, sinks - at);
+    const uint32_t which = bits_between(0, all.sinks - at);
+    return (early & which) | (window & ~which);
+  }
   __device__ __forceinline__ bool sees(int32_t key) const { return key < end && (key >= begin || key < sinks); }
 };
 
@@ -150,7 +172,7 @@ __device__ __forceinline__ uint32_t take_piece(float& x0, float& x1) {
 // serve: an infinity or NaN does not survive being cut into pieces, and 0 * inf is not 0.
 // ---------------------------------------------------------------------------------------------
 template <typename QT, typename KVT, int D>
-__device__ __attribute__((noinline)) void exact_row(const Window& a, int64_t t, int32_t head, int32_t seq, Span own, Span keys,
+__device__ __forceinline__ void exact_row(const Window& a, int64_t t, int32_t head, int32_t seq, Span own, Span keys,
                                                     int32_t first, int32_t last, int32_t split) {
   constexpr int kOwn = (D + kWave - 1) / kWave;
   const int lane = threadIdx.x & (kWave - 1);
@@ -166,7 +188,7 @@ __device__ __attribute__((noinline)) void exact_row(const Window& a, int64_t t, 
       const KVT* k = static_cast<const KVT*>(a.keys) + row_of(a, slot, kv_head, D);
       score = 0.f;
       for (int d = 0; d < D; ++d) score += load_one(q + d) * load_one(k + d);
-      score *= a.scale_log2;
+      score *= a.given_scale;
     }
     const uint64_t seen = __ballot(slot >= 0);
     if (seen == 0) continue;
@@ -314,7 +336,7 @@ __global__ __launch_bounds__(kThreads) void row_kernel(const Window a) {
         for (int u = 0; u < S::kKLoads; ++u) {
           const u32x4 x = *reinterpret_cast<const u32x4*>(q + 32 * u + 8 * c);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) qr[4 * u + e] = x[e];
+          for (int e = 0; e < 4; ++e) qr[4 * u + e] = (x[e] & a.keep) ^ a.flip;
         }
       } else if constexpr (S::kBf16) {
 #pragma unroll
@@ -410,7 +432,7 @@ __global__ __launch_bounds__(kThreads) void row_kernel(const Window a) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             if constexpr (sizeof(QT) == 2) st[j][r] *= a.scale_log2;
-            if (live != kAll && !((live >> (16 * j + 4 * c + r)) & 1)) st[j][r] = -INFINITY;
+            st[j][r] = (live >> (16 * j + 4 * c + r)) & 1 ? st[j][r] : -INFINITY;
             most = fmaxf(most, st[j][r]);
           }
         }
@@ -553,6 +575,380 @@ __global__ __launch_bounds__(kThreads) void row_kernel(const Window a) {
 }
 
 // ---------------------------------------------------------------------------------------------
+// Runs of rows (prompt chunks): one workgroup per (aligned block of rows, key head, split), whose
+// kTileQueries = 128 queries are the block's rows times the heads that share the key head, 32 to a
+// wavefront. Packing the heads keeps the rows of a tile close together, so a tile reads little more
+// than one row's window, and serves every head of the group from one copy of the keys.
+//
+// With lane l = (c = l / 32, n = l % 32) and v_mfma_f32_32x32x16_bf16:
+//   S^T = K Q^T    32 keys x 32 queries per product chain; K from LDS, 16 bytes of key n's row per lane,
+//                  Q from registers. Register r holds the score of key 8 (r / 4) + 4c + r % 4.
+//   O^T = V^T P^T  step s takes 16 keys, element e of lane group c being key 16 s + 8 (e / 4) + 4 c + e % 4:
+//                  the P operand is the lane's own registers 8 s + e, rounded to pieces, and V is read
+//                  transposed (ds_read_b64_tr_b16), four keys of one dimension at a time.
+// Float32 operands are cut into three bfloat16 pieces, whose products (the 3 or 6 largest of them) add
+// up to the float32 product within one float32 rounding. bfloat16 queries and keys are one piece; their
+// weights P are two, 2^-17 of a weight: one piece (2^-9) would add as much error as the output's rounding.
+//
+// Keys and values are staged kKeys at a time in two LDS buffers: while one is used, the next tile's rows
+// are in flight to registers and the slots of the one after are looked up.
+// ---------------------------------------------------------------------------------------------
+template <typename QT, typename KVT, int D>
+struct TileShape {
+  static constexpr int kQPieces = sizeof(QT) == 4 ? 3 : 1;
+  static constexpr int kKvPieces = sizeof(KVT) == 4 ? 3 : 1;
+  static constexpr int kPPieces = sizeof(QT) == 4 ? 3 : 2;
+  static constexpr int kKeys = (sizeof(KVT) == 2 && D <= 128) || D == 32 ? 64 : 32;
+  static constexpr int kChunks = D / 8;                                // 16-byte chunks of a bfloat16 row
+  static constexpr int kPlane = kKeys * D;                             // elements of one piece of a staged tile
+  static constexpr int kStaged = kKeys * kChunks / kThreads;           // chunks of a tile per thread, K and V each
+  static constexpr int kLds = 2 * 2 * kKvPieces * kPlane * 2;          // bytes: two buffers of K and V
+  static constexpr int kWaves = kLds <= 81920 && sizeof(QT) == 2 && D <= 128 ? 2 : 1;  // per SIMD
+  static constexpr bool kFits = kLds <= 160 * 1024 - 2048 && !(sizeof(QT) == 4 && D > 128);
+};
+
+// The products of pieces i of one operand and j of the other that are computed: i + j <= 2.
+__device__ __forceinline__ constexpr bool counted(int i, int j) { return i + j <= 2; }
+
+__device__ __forceinline__ floatx16 mfma32(const u32x4& a, const u32x4& b, const floatx16& c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// Pieces without the guard: what is not finite turns into NaN, which the tile pass looks for at its end.
+__device__ __forceinline__ uint32_t cut_piece(float& x0, float& x1) {
+  const uint32_t pair = __builtin_bit_cast(uint32_t, __builtin_convertvector((floatx2{x0, x1}), bf16x2));
+  x0 -= bf16_lo(pair);
+  x1 -= bf16_hi(pair);
+  return pair;
+}
+
+// Chunks of a staged row are permuted so that the lanes of a read lie in different banks: the key
+// operand reads one chunk of 32 rows, the value operand two neighbouring ones of four rows.
+template <int D>
+__device__ __forceinline__ int key_chunk(int row, int chunk) {
+  return D >= 64 ? chunk ^ (row & 7) : chunk ^ ((row >> 1) & 3);
+}
+template <int D>
+__device__ __forceinline__ int value_chunk(int row, int chunk) {
+  return D >= 64 ? chunk ^ (2 * (row & 3)) : chunk;
+}
+
+__device__ __forceinline__ short4v read_transposed(const uint16_t* p) {
+  typedef __attribute__((address_space(3))) short4v* lds_ptr;
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p));
+}
+
+__device__ __forceinline__ int32_t wave_min(int32_t x) {
+  for (int m = kWave / 2; m > 0; m >>= 1) x = min(x, __shfl_xor(x, m));
+  return __builtin_amdgcn_readfirstlane(x);
+}
+__device__ __forceinline__ int32_t wave_max(int32_t x) {
+  for (int m = kWave / 2; m > 0; m >>= 1) x = max(x, __shfl_xor(x, m));
+  return __builtin_amdgcn_readfirstlane(x);
+}
+
+template <typename QT, typename KVT, int D>
+__global__ __launch_bounds__(kThreads, (TileShape<QT, KVT, D>::kWaves)) void tile_kernel(const Window a) {
+  using S = TileShape<QT, KVT, D>;
+  constexpr int kBlocks = D / 32;       // output tiles of 32 dimensions
+  constexpr int kSteps = D / 16;        // steps of a score product
+  constexpr int kSub = S::kKeys / 32;   // 32-key blocks of a staged tile
+  extern __shared__ __align__(16) uint16_t s_kv[];  // [buffer][K, V][piece][key][D]
+  __shared__ int32_t s_slot[3][S::kKeys];
+  __shared__ uint64_t s_live[3];
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), c = lane / 32, n = lane % 32;
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  uint32_t item = blockIdx.x;
+  const int32_t kv_head = item % static_cast<uint32_t>(a.num_kv_heads);
+  item /= static_cast<uint32_t>(a.num_kv_heads);
+  const int32_t split = item % static_cast<uint32_t>(a.splits);
+  const int64_t block0 = static_cast<int64_t>(item / static_cast<uint32_t>(a.splits)) * a.tile_rows;
+  const int64_t block1 = min(block0 + a.tile_rows, a.num_queries);
+  const KVT* keys = static_cast<const KVT*>(a.keys);
+  const KVT* values = static_cast<const KVT*>(a.values);
+  auto plane = [&](int buffer, int which, int piece) {
+    return s_kv + ((buffer * 2 + which) * S::kKvPieces + piece) * S::kPlane;
+  };
+
+  for (int64_t run0 = block0, run1; run0 < block1; run0 = run1) {
+    const int32_t seq = a.seqs[run0];
+    for (run1 = run0 + 1; run1 < block1 && a.seqs[run1] == seq;) ++run1;
+    if (run1 - run0 < kMinRun || seq < 0 || seq >= a.num_seqs) continue;
+    const int32_t* table = a.tables + static_cast<int64_t>(seq) * a.table_stride;
+    const int32_t rows = static_cast<int32_t>(run1 - run0);
+
+    // The keys that any row sees: the sinks, then [begin, end).
+    Span all{0, INT32_MAX, 0};
+    for (int32_t i = lane; i < rows; i += kWave) {
+      const Span one = span_of(a, seq, a.positions[run0 + i]);
+      if (one.count() > 0) all.begin = min(all.begin, one.begin), all.end = max(all.end, one.end);
+    }
+    all.begin = wave_min(all.begin);
+    all.end = wave_max(all.end);
+    all.begin = min(all.begin, all.end);  // no row sees any: nothing
+    all.sinks = min(a.sinks, all.begin);
+    const int32_t count = all.count();
+    const int32_t tiles = (count + S::kKeys - 1) / S::kKeys;
+    const int32_t first = static_cast<int32_t>(static_cast<int64_t>(tiles) * split / a.splits);
+    const int32_t last = static_cast<int32_t>(static_cast<int64_t>(tiles) * (split + 1) / a.splits);
+
+    // This lane's query: column n of its wavefront.
+    const int32_t m = wave * 32 + n;
+    const int32_t local = m / a.group;
+    const bool active = local < rows;
+    const int64_t t = run0 + min(local, rows - 1);
+    const int32_t head = kv_head * a.group + (m - local * a.group);
+    const Span own = span_of(a, seq, a.positions[t]);
+    // Keys [wave_begin, wave_end) and sinks are all that this wavefront's rows see; every one of them
+    // sees [full_begin, full_end).
+    const bool sees = active && own.count() > 0;
+    const int32_t wave_begin = wave_min(sees ? own.begin : INT32_MAX);
+    const int32_t wave_end = wave_max(sees ? own.end : 0);
+    const int32_t wave_sinks = wave_max(sees ? own.sinks : 0);
+    const int32_t full_begin = wave_max(!active ? 0 : sees ? own.begin : INT32_MAX);
+    const int32_t full_end = wave_min(!active ? INT32_MAX : own.end);
+
+    // The queries, the right operand of S^T: lane (c, n) holds dimensions 16 s + 8 c of query n.
+    u32x4 qr[S::kQPieces][kSteps];
+    {
+      const QT* q = static_cast<const QT*>(a.queries) + t * a.query_stride + static_cast<int64_t>(head) * D + 8 * c;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        if constexpr (sizeof(QT) == 2) {
+          qr[0][s] = (*reinterpret_cast<const u32x4*>(q + 16 * s) & a.keep) ^ a.flip;
+        } else {
+          f32x4 x[2] = {*reinterpret_cast<const f32x4*>(q + 16 * s), *reinterpret_cast<const f32x4*>(q + 16 * s + 4)};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float x0 = x[e / 2][e % 2 * 2] * a.scale_log2, x1 = x[e / 2][e % 2 * 2 + 1] * a.scale_log2;
+#pragma unroll
+            for (int p = 0; p < S::kQPieces; ++p) qr[p][s][e] = cut_piece(x0, x1);
+          }
+        }
+      }
+    }
+
+    floatx16 o[kBlocks];
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[b][r] = 0.f;
+    }
+    float top = -INFINITY, sum = 0.f;
+
+    // Staging. Slots of a tile by the first wavefront, rows by all.
+    auto look_up = [&](int32_t tile) {
+      const int32_t i = tile * S::kKeys + tid;
+      return tid < S::kKeys && tile < last && i < count ? slot_of(a, table, all.key(i)) : -1;
+    };
+    auto keep_slots = [&](int32_t tile, int32_t slot) {
+      if (wave == 0) {
+        const uint64_t live = __ballot(slot >= 0);
+        if (tid < S::kKeys) s_slot[tile % 3][tid] = slot;
+        if (tid == 0) s_live[tile % 3] = live;
+      }
+    };
+    constexpr int kWide = sizeof(KVT) / 2;  // 16-byte loads of a chunk
+    u32x4 kx[S::kStaged][kWide], vx[S::kStaged][kWide];
+    auto load = [&](int32_t tile) {
+#pragma unroll
+      for (int i = 0; i < S::kStaged; ++i) {
+        const int at = tid + i * kThreads, row = at / S::kChunks, chunk = at % S::kChunks;
+        const int32_t slot = s_slot[tile % 3][row];
+        const int64_t from = row_of(a, slot, kv_head, D) + chunk * 8;
+#pragma unroll
+        for (int w = 0; w < kWide; ++w) {
+          kx[i][w] = slot >= 0 ? *reinterpret_cast<const u32x4*>(keys + from + w * 4) : u32x4{0, 0, 0, 0};
+          vx[i][w] = slot >= 0 ? *reinterpret_cast<const u32x4*>(values + from + w * 4) : u32x4{0, 0, 0, 0};
+        }
+      }
+    };
+    auto put = [&](int buffer, int which, int i, const u32x4 (&x)[kWide]) {
+      const int at = tid + i * kThreads, row = at / S::kChunks, chunk = at % S::kChunks;
+      const int to = row * D + 8 * (which == 0 ? key_chunk<D>(row, chunk) : value_chunk<D>(row, chunk));
+      if constexpr (kWide == 1) {
+        *reinterpret_cast<u32x4*>(plane(buffer, which, 0) + to) = x[0];
+      } else {
+        u32x4 piece[3];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float x0 = __uint_as_float(x[e / 2][e % 2 * 2]), x1 = __uint_as_float(x[e / 2][e % 2 * 2 + 1]);
+#pragma unroll
+          for (int p = 0; p < 3; ++p) piece[p][e] = cut_piece(x0, x1);
+        }
+#pragma unroll
+        for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x4*>(plane(buffer, which, p) + to) = piece[p];
+      }
+    };
+    auto stage = [&](int buffer) {
+#pragma unroll
+      for (int i = 0; i < S::kStaged; ++i) {
+        put(buffer, 0, i, kx[i]);
+        put(buffer, 1, i, vx[i]);
+      }
+    };
+
+    __syncthreads();  // the run before is done with LDS
+    keep_slots(first, look_up(first));
+    keep_slots(first + 1, look_up(first + 1));
+    __syncthreads();
+    if (first < last) {
+      load(first);
+      stage(0);
+    }
+    __syncthreads();
+    for (int32_t tile = first; tile < last; ++tile) {
+      const int buffer = (tile - first) & 1;
+      if (tile + 1 < last) load(tile + 1);
+      const int32_t slot_ahead = look_up(tile + 2);
+      const uint64_t tile_live = s_live[tile % 3];
+#pragma unroll
+      for (int j = 0; j < kSub; ++j) {
+        const int32_t at = tile * S::kKeys + 32 * j;  // the block's first item of the span
+        if (at >= count) break;
+        const int32_t key0 = all.key(at), key1 = all.key(min(at + 31, count - 1));
+        if (key0 >= wave_end || (key0 >= wave_sinks && key1 < wave_begin)) continue;
+        const uint32_t live = static_cast<uint32_t>(tile_live >> (32 * j));
+        floatx16 st;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) st[r] = 0.f;
+        const uint16_t* kp = plane(buffer, 0, 0) + (32 * j + n) * D;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+          u32x4 k[S::kKvPieces];
+#pragma unroll
+          for (int p = 0; p < S::kKvPieces; ++p) {
+            k[p] = *reinterpret_cast<const u32x4*>(kp + p * S::kPlane + 8 * key_chunk<D>(32 * j + n, 2 * s + c));
+          }
+#pragma unroll
+          for (int p = S::kKvPieces - 1; p >= 0; --p) {
+#pragma unroll
+            for (int q = S::kQPieces - 1; q >= 0; --q) {
+              if (counted(p, q)) st = mfma32(k[p], qr[q][s], st);
+            }
+          }
+        }
+        // Scores are kept as they are, times scale (bfloat16) or already scaled (float32).
+        const float scale = sizeof(QT) == 2 ? a.scale_log2 : 1.f;
+        if (!(key0 >= full_begin && key1 < full_end && key0 >= all.sinks && live == 0xffffffffu)) {
+          const uint32_t seen = (own.seen_of(all, at) & live) >> (4 * c);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) st[r] = (seen >> (8 * (r / 4) + r % 4)) & 1 ? st[r] : -INFINITY;
+        }
+        float most = fmaxf(st[0], st[1]);
+#pragma unroll
+        for (int r = 2; r < 16; ++r) most = fmaxf(most, st[r]);
+        {
+          const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(most), __float_as_uint(most), false, false);
+          most = fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1])) * scale;
+        }
+        // The reference of the exponentials is raised only when a score passes it by 2^8: weights then
+        // stay below 2^8, and the outputs are seldom rescaled.
+        if (__ballot(most > top + kLazyLog2) != 0) {
+          const float next = fmaxf(top, most);
+          const float keep = next == -INFINITY ? 1.f : fast_exp2(top - next);
+          sum *= keep;
+#pragma unroll
+          for (int b = 0; b < kBlocks; ++b) o[b] *= keep;
+          top = next;
+        }
+        const float from = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          st[r] = fast_exp2(__builtin_fmaf(st[r], scale, -from));
+          sum += st[r];
+        }
+        u32x4 pr[S::kPPieces][2];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float x0 = st[8 * s + 2 * e], x1 = st[8 * s + 2 * e + 1];
+#pragma unroll
+            for (int p = 0; p < S::kPPieces; ++p) pr[p][s][e] = cut_piece(x0, x1);
+          }
+        }
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          // Keys 16 s + 4 c .. + 3 and 8 more on; this lane reads row i / 4 of its 16 lanes' block.
+          const int row = 32 * j + 16 * s + 4 * c + (lane % 16) / 4;
+          const int part = (lane / 16 % 2) * 16 + lane % 4 * 4;  // its dimension within 32
+#pragma unroll
+          for (int b = 0; b < kBlocks; ++b) {
+            const int chunk = (32 * b + part) / 8, rest = part % 8;
+            u32x4 v[S::kKvPieces];
+#pragma unroll
+            for (int p = 0; p < S::kKvPieces; ++p) {
+              const uint16_t* vp = plane(buffer, 1, p);
+              const auto lo = __builtin_bit_cast(u32x2, read_transposed(vp + row * D + 8 * value_chunk<D>(row, chunk) + rest));
+              const auto hi = __builtin_bit_cast(u32x2, read_transposed(vp + (row + 8) * D + 8 * value_chunk<D>(row + 8, chunk) + rest));
+              v[p] = u32x4{lo.x, lo.y, hi.x, hi.y};
+            }
+#pragma unroll
+            for (int p = S::kKvPieces - 1; p >= 0; --p) {
+#pragma unroll
+              for (int q = S::kPPieces - 1; q >= 0; --q) {
+                if (counted(p, q)) o[b] = mfma32(v[p], pr[q][s], o[b]);
+              }
+            }
+          }
+        }
+      }
+      if (tile + 1 < last) stage(buffer ^ 1);
+      keep_slots(tile + 2, slot_ahead);
+      __syncthreads();
+    }
+    {
+      const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
+      sum = __uint_as_float(both[0]) + __uint_as_float(both[1]);
+    }
+
+    bool bad = !(fabsf(sum) < INFINITY);
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) bad = bad || !(fabsf(o[b][r]) < INFINITY);
+    }
+    const uint64_t wrong = __ballot(bad && active);
+    const uint32_t again = static_cast<uint32_t>(wrong) | static_cast<uint32_t>(wrong >> 32);
+    if (active && !((again >> n) & 1)) {
+      // Register r of output tile b is dimension 32 b + 8 (r / 4) + 4 c + r % 4 of query n.
+      const int64_t out_row = t * a.num_heads + head;
+      const int64_t index = split_index(a, t, head, split);
+      if (a.splits > 1 && c == 0) store_split_sums(a, index, top, sum);
+      const float divide = sum == 0.f ? 0.f : 1.f / sum;
+      if (a.splits == 1 || sum != 0.f) {
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) {
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            float x[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = a.splits == 1 ? o[b][4 * g + e] * divide : o[b][4 * g + e];
+            const int d = 32 * b + 8 * g + 4 * c;
+            if (a.splits == 1) {
+              store_row<QT, 4>(static_cast<QT*>(a.out) + out_row * D + d, x);
+            } else {
+              store_row<float, 4>(split_acc(a, index, D) + d, x);
+            }
+          }
+        }
+      }
+    }
+    for (uint32_t left = again; left != 0; left &= left - 1) {
+      const int col = __builtin_ctz(left);
+      Span one;
+      one.sinks = __shfl(own.sinks, col);
+      one.begin = __shfl(own.begin, col);
+      one.end = __shfl(own.end, col);
+      const int32_t which = wave * 32 + col, row = which / a.group;
+      exact_row<QT, KVT, D>(a, run0 + row, kv_head * a.group + (which - row * a.group), seq, one, all, min(first * S::kKeys, count),
+                            min(last * S::kKeys, count), split);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
 // Joins the splits of every row and head: D / 4 threads each, four dimensions a thread.
 // ---------------------------------------------------------------------------------------------
 template <typename QT, int D>
@@ -586,15 +982,27 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const Window a) {
 }
 
 template <typename QT, typename KVT, int D>
-int launch(Window a, hipStream_t stream) {
+int launch(Window a, bool runs, hipStream_t stream) {
+  using S = TileShape<QT, KVT, D>;
   a.subgroups = (a.group + 15) / 16;
   a.tile_rows = kTileQueries / a.group;
-  a.tiled = 0;
-  a.rows_per_group = 1;
+  a.tiled = S::kFits && runs;
+  // Where most rows belong to the tile pass, few workgroups find that out.
+  a.rows_per_group = a.tiled && a.num_queries > 512 ? 8 : 1;
   const int64_t row_groups = (a.num_queries + a.rows_per_group - 1) / a.rows_per_group;
   const int64_t groups = row_groups * a.num_kv_heads * a.subgroups * a.splits;
+  const int64_t tiles = (a.num_queries + a.tile_rows - 1) / a.tile_rows * a.num_kv_heads * a.splits;
   const int64_t joins = (a.num_queries * a.num_heads * (D / 4) + kThreads - 1) / kThreads;
-  if (groups > 0x7fffffff || joins > 0x7fffffff) return PKV_EUNSUPPORTED;
+  if (groups > 0x7fffffff || joins > 0x7fffffff || tiles > 0x7fffffff) return PKV_EUNSUPPORTED;
+  if constexpr (S::kFits) {
+    if (a.tiled) {
+      if (hipFuncSetAttribute(reinterpret_cast<const void*>(tile_kernel<QT, KVT, D>), hipFuncAttributeMaxDynamicSharedMemorySize,
+                              S::kLds) != hipSuccess) {
+        return PKV_EHIP;
+      }
+      hipLaunchKernelGGL((tile_kernel<QT, KVT, D>), dim3(static_cast<uint32_t>(tiles)), dim3(kThreads), S::kLds, stream, a);
+    }
+  }
   hipLaunchKernelGGL((row_kernel<QT, KVT, D>), dim3(static_cast<uint32_t>(groups)), dim3(kThreads), 0, stream, a);
   if (a.splits > 1) {
     hipLaunchKernelGGL((join_kernel<QT, D>), dim3(static_cast<uint32_t>(joins)), dim3(kThreads), 0, stream, a);
@@ -603,12 +1011,12 @@ int launch(Window a, hipStream_t stream) {
 }
 
 template <typename QT, typename KVT>
-int dispatch(const Window& a, int32_t head_dim, hipStream_t stream) {
+int dispatch(const Window& a, int32_t head_dim, bool runs, hipStream_t stream) {
   switch (head_dim) {
-    case 32: return launch<QT, KVT, 32>(a, stream);
-    case 64: return launch<QT, KVT, 64>(a, stream);
-    case 128: return launch<QT, KVT, 128>(a, stream);
-    case 256: return launch<QT, KVT, 256>(a, stream);
+    case 32: return launch<QT, KVT, 32>(a, runs, stream);
+    case 64: return launch<QT, KVT, 64>(a, runs, stream);
+    case 128: return launch<QT, KVT, 128>(a, runs, stream);
+    case 256: return launch<QT, KVT, 256>(a, runs, stream);
     default: return PKV_EUNSUPPORTED;
   }
 }
@@ -623,9 +1031,13 @@ extern "C" int32_t pkv_window_splits(int64_t num_queries, int32_t num_heads, int
     return PKV_EINVAL;
   }
   const int64_t longest = std::min<int64_t>(max_context_len, static_cast<int64_t>(window) + sinks);
-  const int64_t groups = std::max<int64_t>(1, num_queries * num_kv_heads * ((num_heads / num_kv_heads + 15) / 16));
+  const int32_t group = num_heads / num_kv_heads;
+  if (group > PKV_WINDOW_MAX_GROUP) return PKV_EINVAL;
+  const bool runs = max_query_len >= pkv::kMinRun;
+  const int64_t rows = runs ? pkv::kTileQueries / group : 1;
+  const int64_t groups = (num_queries + rows - 1) / rows * num_kv_heads * (runs ? 1 : (group + 15) / 16);
   const int64_t most = std::max<int64_t>(1, std::min<int64_t>(PKV_WINDOW_MAX_SPLITS, longest / 128));
-  return static_cast<int32_t>(std::min<int64_t>(most, (768 + groups - 1) / groups));
+  return static_cast<int32_t>(std::min<int64_t>(most, (512 + groups - 1) / std::max<int64_t>(1, groups)));
 }
 
 extern "C" int64_t pkv_window_workspace_bytes(int64_t num_queries, int32_t num_heads, int32_t head_dim, int32_t num_splits) {
@@ -691,9 +1103,17 @@ extern "C" int pkv_window_attention(const pkv_window* args, int device, void* st
   a.max_context = g.max_context_len;
   a.splits = splits;
   a.scale_log2 = g.scale * 1.44269504088896340736f;
+  a.given_scale = a.scale_log2;
+  const bool runs = g.max_query_len >= kMinRun;
   DeviceGuard guard(device);
   if (!guard.ok()) return PKV_EHIP;
   auto s = static_cast<hipStream_t>(stream);
-  if (g.q_dtype == PKV_BF16) return dispatch<uint16_t, uint16_t>(a, g.head_dim, s);
-  return g.kv_dtype == PKV_F32 ? dispatch<float, float>(a, g.head_dim, s) : dispatch<float, uint16_t>(a, g.head_dim, s);
+  if (g.q_dtype == PKV_BF16) {
+    a.flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;
+    a.keep = a.scale_log2 == 0.f ? 0u : 0xffffffffu;
+    a.scale_log2 = a.scale_log2 == 0.f ? 1.f : std::fabs(a.scale_log2);
+    return dispatch<uint16_t, uint16_t>(a, g.head_dim, runs, s);
+  }
+  return g.kv_dtype == PKV_F32 ? dispatch<float, float>(a, g.head_dim, runs, s)
+                               : dispatch<float, uint16_t>(a, g.head_dim, runs, s);
 }
