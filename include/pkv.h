@@ -649,8 +649,9 @@ typedef struct pkv_window {
 int32_t pkv_window_splits(int64_t num_queries, int32_t num_heads, int32_t num_kv_heads, int32_t window,
                           int32_t sinks, int32_t max_context_len, int32_t max_query_len);
 
-/* Bytes of workspace for `num_splits` splits (0 for one). Host-only. */
-int64_t pkv_window_workspace_bytes(int64_t num_queries, int32_t num_heads, int32_t head_dim, int32_t num_splits);
+/* Bytes of workspace for `num_splits` splits (0 for one split and a max_query_len of at most 1). Host-only. */
+int64_t pkv_window_workspace_bytes(int64_t num_queries, int32_t num_heads, int32_t head_dim, int32_t max_query_len,
+                                   int32_t num_splits);
 
 int pkv_window_attention(const pkv_window* args, int device, void* stream);
 

@@ -379,7 +379,7 @@ def _declare(lib: ctypes.CDLL) -> None:
         _i64, _i32, _i32, _i32, _i32, _i32, _i32,  # queries, heads, kv heads, window, sinks, max context, max query len
     ]
     lib.pkv_window_splits.restype = _i32
-    lib.pkv_window_workspace_bytes.argtypes = [_i64, _i32, _i32, _i32]  # queries, heads, head_dim, splits
+    lib.pkv_window_workspace_bytes.argtypes = [_i64, _i32, _i32, _i32, _i32]  # queries, heads, head_dim, max query len, splits
     lib.pkv_window_workspace_bytes.restype = _i64
     lib.pkv_window_attention.argtypes = [ctypes.POINTER(WindowArgs), _c_int, _ptr]  # args, device, stream
     lib.pkv_window_attention.restype = _c_int

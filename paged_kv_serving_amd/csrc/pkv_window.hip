@@ -19,6 +19,9 @@ constexpr int kWaves = kThreads / kWave;
 constexpr int kTileQueries = 128;  // (row, head) pairs of a tile
 constexpr int kMinRun = PKV_WINDOW_MIN_RUN;
 constexpr float kLazyLog2 = 8.f;
+#ifndef PKV_PP
+#define PKV_PP 2
+#endif
 
 typedef float floatx2 __attribute__((ext_vector_type(2)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
@@ -48,7 +51,8 @@ struct Window {
   int32_t subgroups;       // of up to 16 query heads of a group
   int32_t tile_rows;       // rows of a tile: the aligned blocks of rows that runs lie in
   int32_t tiled;           // whether the tile pass computes the runs
-  int32_t rows_per_group;  // rows of a row pass workgroup, one after the other
+  int32_t min_run;         // rows of one sequence next to each other that a tile takes
+  int32_t* list;           // the rows that no tile takes (list_rows); NULL without tiles
   float scale_log2;  // scale * log2(e): scores are kept in base 2
   float given_scale;  // the same before the next two
   // A negative scale of bfloat16 queries turns their signs instead, so that the largest product is the
@@ -282,15 +286,42 @@ __device__ __forceinline__ Words<N> load_words(const void* p) {
   return x;
 }
 
-// Whether row t lies in a run that the tile pass computes: kMinRun rows or more of one sequence next
-// to each other inside one of the aligned blocks of rows that the tile pass goes by.
-__device__ __forceinline__ bool in_run(const Window& a, int64_t t, int32_t seq) {
-  const int64_t begin = t / a.tile_rows * a.tile_rows;
-  const int64_t end = min(begin + a.tile_rows, a.num_queries);
-  int length = 1;
-  for (int64_t i = t - 1; i >= begin && length < kMinRun && a.seqs[i] == seq; --i) ++length;
-  for (int64_t i = t + 1; i < end && length < kMinRun && a.seqs[i] == seq; ++i) ++length;
-  return length >= kMinRun;
+// The rows that no tile computes, in order: list[0] is their number. A tile takes the runs of a.min_run
+// rows or more of one sequence next to each other inside an aligned block of a.tile_rows rows; rows
+// outside every sequence are left out. One workgroup writes it.
+__device__ __forceinline__ void list_rows(const Window& a) {
+  __shared__ int32_t s_count[kWaves];
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  int32_t found = 0;
+  for (int64_t start = 0; start < a.num_queries; start += kThreads) {
+    const int64_t t = start + threadIdx.x;
+    bool listed = false;
+    if (t < a.num_queries) {
+      const int32_t seq = a.seqs[t];
+      const int64_t begin = t / a.tile_rows * a.tile_rows;
+      const int64_t end = min(begin + a.tile_rows, a.num_queries);
+      bool left = true, right = true;
+      int32_t length = 1;
+#pragma unroll
+      for (int i = 1; i < kMinRun; ++i) {
+        left = left && t - i >= begin && a.seqs[max(t - i, begin)] == seq;
+        right = right && t + i < end && a.seqs[min(t + i, end - 1)] == seq;
+        length += (left ? 1 : 0) + (right ? 1 : 0);
+      }
+      listed = seq >= 0 && seq < a.num_seqs && length < a.min_run;
+    }
+    const uint64_t ballot = __ballot(listed);
+    if (lane == 0) s_count[wave] = __popcll(ballot);
+    __syncthreads();
+    int32_t at = found + __popcll(ballot & ((1ull << lane) - 1));
+    for (int w = 0; w < kWaves; ++w) {
+      at += w < wave ? s_count[w] : 0;
+      found += s_count[w];
+    }
+    if (listed) a.list[1 + at] = static_cast<int32_t>(t);
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) a.list[0] = found;
 }
 
 template <typename QT, typename KVT, int D>
@@ -302,24 +333,27 @@ __global__ __launch_bounds__(kThreads) void row_kernel(const Window a) {
   __shared__ int s_redo;
   const int lane = threadIdx.x & (kWave - 1), c = lane / 16, n = lane % 16;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  uint32_t item = blockIdx.x;
-  const int32_t kv_head = item % static_cast<uint32_t>(a.num_kv_heads);
-  item /= static_cast<uint32_t>(a.num_kv_heads);
-  const int32_t sub = item % static_cast<uint32_t>(a.subgroups);
-  item /= static_cast<uint32_t>(a.subgroups);
-  const int32_t split = item % static_cast<uint32_t>(a.splits);
-  const int64_t row0 = static_cast<int64_t>(item / static_cast<uint32_t>(a.splits)) * a.rows_per_group;
-  const int32_t heads = min(16, a.group - sub * 16);
-  const int32_t head0 = kv_head * a.group + sub * 16;
-  const auto* keys = static_cast<const char*>(a.keys);
-  const auto* values = static_cast<const char*>(a.values);
-  const int64_t row_bytes = static_cast<int64_t>(a.num_kv_heads) * D * sizeof(KVT);
-  const int64_t k_at = (static_cast<int64_t>(kv_head) * D + (S::kBf16 ? 8 : 4) * c) * sizeof(KVT);
-  const int64_t v_at = (static_cast<int64_t>(kv_head) * D + S::kVWidth * n) * sizeof(KVT);
-
-  for (int64_t t = row0; t < min(row0 + a.rows_per_group, a.num_queries); ++t) {
+  // Items: heads fastest, so that one XCD has its share of the heads of every row.
+  const int64_t rows = a.tiled ? a.list[0] : a.num_queries;
+  const int64_t items = rows * a.splits * a.subgroups * a.num_kv_heads;
+  for (int64_t next = blockIdx.x; next < items; next += gridDim.x) {
+    uint32_t item = static_cast<uint32_t>(next);
+    const int32_t kv_head = item % static_cast<uint32_t>(a.num_kv_heads);
+    item /= static_cast<uint32_t>(a.num_kv_heads);
+    const int32_t sub = item % static_cast<uint32_t>(a.subgroups);
+    item /= static_cast<uint32_t>(a.subgroups);
+    const int32_t split = item % static_cast<uint32_t>(a.splits);
+    item /= static_cast<uint32_t>(a.splits);
+    const int64_t t = a.tiled ? a.list[1 + item] : static_cast<int64_t>(item);
+    const int32_t heads = min(16, a.group - sub * 16);
+    const int32_t head0 = kv_head * a.group + sub * 16;
+    const auto* keys = static_cast<const char*>(a.keys);
+    const auto* values = static_cast<const char*>(a.values);
+    const int64_t row_bytes = static_cast<int64_t>(a.num_kv_heads) * D * sizeof(KVT);
+    const int64_t k_at = (static_cast<int64_t>(kv_head) * D + (S::kBf16 ? 8 : 4) * c) * sizeof(KVT);
+    const int64_t v_at = (static_cast<int64_t>(kv_head) * D + S::kVWidth * n) * sizeof(KVT);
     const int32_t seq = a.seqs[t];
-    if (seq < 0 || seq >= a.num_seqs || (a.tiled && in_run(a, t, seq))) continue;
+    if (seq < 0 || seq >= a.num_seqs) continue;
     const int32_t* table = a.tables + static_cast<int64_t>(seq) * a.table_stride;
     const Span span = span_of(a, seq, a.positions[t]);
     const int32_t count = span.count();
@@ -597,7 +631,7 @@ template <typename QT, typename KVT, int D>
 struct TileShape {
   static constexpr int kQPieces = sizeof(QT) == 4 ? 3 : 1;
   static constexpr int kKvPieces = sizeof(KVT) == 4 ? 3 : 1;
-  static constexpr int kPPieces = sizeof(QT) == 4 ? 3 : 2;
+  static constexpr int kPPieces = sizeof(QT) == 4 ? 3 : PKV_PP;
   static constexpr int kKeys = (sizeof(KVT) == 2 && D <= 128) || D == 32 ? 64 : 32;
   static constexpr int kChunks = D / 8;                                // 16-byte chunks of a bfloat16 row
   static constexpr int kPlane = kKeys * D;                             // elements of one piece of a staged tile
@@ -658,7 +692,11 @@ __global__ __launch_bounds__(kThreads, (TileShape<QT, KVT, D>::kWaves)) void til
   __shared__ uint64_t s_live[3];
   const int tid = threadIdx.x, lane = tid & (kWave - 1), c = lane / 32, n = lane % 32;
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-  uint32_t item = blockIdx.x;
+  if (blockIdx.x == 0) {  // for the row pass, which comes next
+    list_rows(a);
+    return;
+  }
+  uint32_t item = blockIdx.x - 1;
   const int32_t kv_head = item % static_cast<uint32_t>(a.num_kv_heads);
   item /= static_cast<uint32_t>(a.num_kv_heads);
   const int32_t split = item % static_cast<uint32_t>(a.splits);
@@ -673,7 +711,7 @@ __global__ __launch_bounds__(kThreads, (TileShape<QT, KVT, D>::kWaves)) void til
   for (int64_t run0 = block0, run1; run0 < block1; run0 = run1) {
     const int32_t seq = a.seqs[run0];
     for (run1 = run0 + 1; run1 < block1 && a.seqs[run1] == seq;) ++run1;
-    if (run1 - run0 < kMinRun || seq < 0 || seq >= a.num_seqs) continue;
+    if (run1 - run0 < a.min_run || seq < 0 || seq >= a.num_seqs) continue;
     const int32_t* table = a.tables + static_cast<int64_t>(seq) * a.table_stride;
     const int32_t rows = static_cast<int32_t>(run1 - run0);
 
@@ -982,25 +1020,25 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const Window a) {
 }
 
 template <typename QT, typename KVT, int D>
-int launch(Window a, bool runs, hipStream_t stream) {
+int launch(Window a, hipStream_t stream) {
   using S = TileShape<QT, KVT, D>;
   a.subgroups = (a.group + 15) / 16;
   a.tile_rows = kTileQueries / a.group;
-  a.tiled = S::kFits && runs;
-  // Where most rows belong to the tile pass, few workgroups find that out.
-  a.rows_per_group = a.tiled && a.num_queries > 512 ? 8 : 1;
-  const int64_t row_groups = (a.num_queries + a.rows_per_group - 1) / a.rows_per_group;
-  const int64_t groups = row_groups * a.num_kv_heads * a.subgroups * a.splits;
+  a.min_run = std::min(kMinRun, a.tile_rows);
+  a.tiled = S::kFits && a.list;
+  const int64_t items = a.num_queries * a.num_kv_heads * a.subgroups * a.splits;
+  // Beside tiles the number of rows is known on the device only.
+  const int64_t groups = a.tiled ? std::min<int64_t>(items, 1024) : items;
   const int64_t tiles = (a.num_queries + a.tile_rows - 1) / a.tile_rows * a.num_kv_heads * a.splits;
   const int64_t joins = (a.num_queries * a.num_heads * (D / 4) + kThreads - 1) / kThreads;
-  if (groups > 0x7fffffff || joins > 0x7fffffff || tiles > 0x7fffffff) return PKV_EUNSUPPORTED;
+  if (items > 0x7fffffff || joins > 0x7fffffff || tiles >= 0x7fffffff) return PKV_EUNSUPPORTED;
   if constexpr (S::kFits) {
     if (a.tiled) {
       if (hipFuncSetAttribute(reinterpret_cast<const void*>(tile_kernel<QT, KVT, D>), hipFuncAttributeMaxDynamicSharedMemorySize,
                               S::kLds) != hipSuccess) {
         return PKV_EHIP;
       }
-      hipLaunchKernelGGL((tile_kernel<QT, KVT, D>), dim3(static_cast<uint32_t>(tiles)), dim3(kThreads), S::kLds, stream, a);
+      hipLaunchKernelGGL((tile_kernel<QT, KVT, D>), dim3(static_cast<uint32_t>(tiles + 1)), dim3(kThreads), S::kLds, stream, a);
     }
   }
   hipLaunchKernelGGL((row_kernel<QT, KVT, D>), dim3(static_cast<uint32_t>(groups)), dim3(kThreads), 0, stream, a);
@@ -1011,16 +1049,25 @@ int launch(Window a, bool runs, hipStream_t stream) {
 }
 
 template <typename QT, typename KVT>
-int dispatch(const Window& a, int32_t head_dim, bool runs, hipStream_t stream) {
+int dispatch(const Window& a, int32_t head_dim, hipStream_t stream) {
   switch (head_dim) {
-    case 32: return launch<QT, KVT, 32>(a, runs, stream);
-    case 64: return launch<QT, KVT, 64>(a, runs, stream);
-    case 128: return launch<QT, KVT, 128>(a, runs, stream);
-    case 256: return launch<QT, KVT, 256>(a, runs, stream);
+    case 32: return launch<QT, KVT, 32>(a, stream);
+    case 64: return launch<QT, KVT, 64>(a, stream);
+    case 128: return launch<QT, KVT, 128>(a, stream);
+    case 256: return launch<QT, KVT, 256>(a, stream);
     default: return PKV_EUNSUPPORTED;
   }
 }
 
+}  // namespace
+}  // namespace pkv
+
+namespace pkv {
+namespace {
+// Whether a call has tiles, and so a list of the rows outside them at the end of its workspace (kept
+// for every call that may have them: the workspace's size does not go by the heads' grouping).
+bool has_runs(int32_t max_query_len, int32_t group) { return max_query_len >= std::min(kMinRun, kTileQueries / group); }
+int64_t list_bytes(int64_t num_queries) { return (num_queries + 4) / 4 * 16; }
 }  // namespace
 }  // namespace pkv
 
@@ -1033,19 +1080,20 @@ extern "C" int32_t pkv_window_splits(int64_t num_queries, int32_t num_heads, int
   const int64_t longest = std::min<int64_t>(max_context_len, static_cast<int64_t>(window) + sinks);
   const int32_t group = num_heads / num_kv_heads;
   if (group > PKV_WINDOW_MAX_GROUP) return PKV_EINVAL;
-  const bool runs = max_query_len >= pkv::kMinRun;
+  const bool runs = pkv::has_runs(max_query_len, group);
   const int64_t rows = runs ? pkv::kTileQueries / group : 1;
   const int64_t groups = (num_queries + rows - 1) / rows * num_kv_heads * (runs ? 1 : (group + 15) / 16);
   const int64_t most = std::max<int64_t>(1, std::min<int64_t>(PKV_WINDOW_MAX_SPLITS, longest / 128));
   return static_cast<int32_t>(std::min<int64_t>(most, (512 + groups - 1) / std::max<int64_t>(1, groups)));
 }
 
-extern "C" int64_t pkv_window_workspace_bytes(int64_t num_queries, int32_t num_heads, int32_t head_dim, int32_t num_splits) {
-  if (num_queries < 0 || num_heads < 1 || head_dim < 1 || num_splits < 1 || num_splits > PKV_WINDOW_MAX_SPLITS) {
+extern "C" int64_t pkv_window_workspace_bytes(int64_t num_queries, int32_t num_heads, int32_t head_dim, int32_t max_query_len,
+                                              int32_t num_splits) {
+  if (num_queries < 0 || num_heads < 1 || head_dim < 1 || max_query_len < 0 || num_splits < 1 || num_splits > PKV_WINDOW_MAX_SPLITS) {
     return PKV_EINVAL;
   }
-  if (num_splits == 1) return 0;
-  return num_queries * num_heads * num_splits * (head_dim + 2) * static_cast<int64_t>(sizeof(float));
+  const int64_t parts = num_splits == 1 ? 0 : num_queries * num_heads * num_splits * (head_dim + 2) * static_cast<int64_t>(sizeof(float));
+  return (parts + 15) / 16 * 16 + (max_query_len > 1 ? pkv::list_bytes(num_queries) : 0);
 }
 
 extern "C" int pkv_window_attention(const pkv_window* args, int device, void* stream) {
@@ -1077,7 +1125,8 @@ extern "C" int pkv_window_attention(const pkv_window* args, int device, void* st
   const int32_t splits = g.num_splits > 0 ? g.num_splits
                                           : pkv_window_splits(g.num_queries, g.num_heads, g.num_kv_heads, g.window, g.sinks,
                                                               g.max_context_len, g.max_query_len);
-  const int64_t need = pkv_window_workspace_bytes(g.num_queries, g.num_heads, g.head_dim, splits);
+  const int64_t need = pkv_window_workspace_bytes(g.num_queries, g.num_heads, g.head_dim, g.max_query_len, splits);
+  const bool runs = has_runs(g.max_query_len, g.num_heads / g.num_kv_heads);
   if (need > 0 && (!g.workspace || !aligned16(g.workspace) || g.workspace_bytes < need)) return PKV_EINVAL;
   Window a{};
   a.out = g.out;
@@ -1104,7 +1153,7 @@ extern "C" int pkv_window_attention(const pkv_window* args, int device, void* st
   a.splits = splits;
   a.scale_log2 = g.scale * 1.44269504088896340736f;
   a.given_scale = a.scale_log2;
-  const bool runs = g.max_query_len >= kMinRun;
+  if (runs) a.list = reinterpret_cast<int32_t*>(reinterpret_cast<char*>(g.workspace) + need - list_bytes(g.num_queries));
   DeviceGuard guard(device);
   if (!guard.ok()) return PKV_EHIP;
   auto s = static_cast<hipStream_t>(stream);
@@ -1112,8 +1161,8 @@ extern "C" int pkv_window_attention(const pkv_window* args, int device, void* st
     a.flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;
     a.keep = a.scale_log2 == 0.f ? 0u : 0xffffffffu;
     a.scale_log2 = a.scale_log2 == 0.f ? 1.f : std::fabs(a.scale_log2);
-    return dispatch<uint16_t, uint16_t>(a, g.head_dim, runs, s);
+    return dispatch<uint16_t, uint16_t>(a, g.head_dim, s);
   }
-  return g.kv_dtype == PKV_F32 ? dispatch<float, float>(a, g.head_dim, runs, s)
-                               : dispatch<float, uint16_t>(a, g.head_dim, runs, s);
+  return g.kv_dtype == PKV_F32 ? dispatch<float, float>(a, g.head_dim, s)
+                               : dispatch<float, uint16_t>(a, g.head_dim, s);
 }

@@ -1495,7 +1495,7 @@ def paged_attention_window(
     rows = num_queries if max_query_len is None else min(max_query_len, _INT32_MAX)
     lib = _native.library()
     splits = num_splits or lib.pkv_window_splits(num_queries, heads, kv_heads, window, sinks, max_context_len, rows)
-    need = lib.pkv_window_workspace_bytes(num_queries, heads, dim, splits)
+    need = lib.pkv_window_workspace_bytes(num_queries, heads, dim, rows, splits)
     if need:
         if workspace is None:
             workspace = torch.empty(need // 4, dtype=torch.float32, device=queries.device)
@@ -1524,7 +1524,7 @@ def window_workspace_bytes(
     splits = num_splits or lib.pkv_window_splits(
         num_queries, heads, kv_heads, min(window, _INT32_MAX), min(sinks, _INT32_MAX), max_context_len, min(rows, _INT32_MAX)
     )
-    need = lib.pkv_window_workspace_bytes(num_queries, heads, head_dim, splits)
+    need = lib.pkv_window_workspace_bytes(num_queries, heads, head_dim, min(rows, _INT32_MAX), splits)
     if splits < 1 or need < 0:
         raise ValueError("invalid window workspace query")
     return int(need)

@@ -347,4 +347,4 @@ def test_no_rows_no_context_and_refusals(device):
     odd = make([(1, 20)], 2, 1, 48, 16, "float32", "float32")
     with pytest.raises(Exception, match="unsupported|implemented|shape"):
         call(device, odd, 4, 0)
-    assert ops.window_workspace_bytes(4, 4, 2, 64, window=4, max_context_len=30, num_splits=1) == 0
+    assert ops.window_workspace_bytes(4, 4, 2, 64, window=4, max_context_len=30, max_query_len=1, num_splits=1) == 0
