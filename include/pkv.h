@@ -666,7 +666,7 @@ int pkv_window_attention(const pkv_window* args, int device, void* stream);
  *     the first top_k tokens (all with top_k <= 0), of those the tokens with w >= min_p,
  *     of those the shortest beginning with a mass of at least top_p of theirs (all with top_p >= 1),
  *     and the first token whose cumulative mass exceeds uniform * the mass of what is kept.
- * Weights are 64-bit fixed-point numbers of PKV_SAMPLE_BITS fractional bits (fewer from 2^18
+ * Weights are 64-bit fixed-point numbers of PKV_SAMPLE_BITS fractional bits (fewer from 2^17
  * tokens on, so that no sum overflows), rounded from double precision, and their sums are exact: a
  * result does not depend on how a row is spread over the GPU.
  *

@@ -5,9 +5,11 @@
 //     W[i] = round(2^46 exp((logit[i] - max) / T))
 // each step is the same question, "which token is the first whose cumulative mass (or count) reaches
 // X?": X = top_k in counts gives the mass M of the first cut; X = ceil(top_p * M) gives the kept mass
-// S; X = floor(uniform * S) + 1 gives the token. Nothing is sorted: a histogram of the masses over
-// bins that fall with the logit finds the token's bin, and only that bin's tokens are compared with
-// each other. Integer sums make the result independent of the order of the atomics.
+// S; X = floor(uniform * S) + 1 gives the token. A row is never sorted as a whole:
+//   - Where top-k or min-p leave at most kList tokens, those are listed and put in order in LDS.
+//   - Otherwise a histogram of the masses over bins of 1/128 octave finds the bin that holds the answer,
+//     and only that bin's tokens are compared with each other.
+// Integer sums make the result independent of the order of the atomics.
 #include <math.h>
 
 #include "pkv_common.h"
@@ -17,11 +19,11 @@ namespace {
 
 constexpr int kThreads = 1024;
 constexpr int kWaves = kThreads / kWave;
-constexpr int kBins = 4096;
+constexpr int kPerOctave = 128;                    // bins, and entries of the table of powers
+constexpr int kBins = 48 * kPerOctave;             // 2^-47.5 * 2^46 < 1/2: later bins weigh nothing
 constexpr int kBinsPerThread = kBins / kThreads;
-constexpr int kList = 2048;      // tokens of one bin that are compared in LDS
-constexpr float kReach = 33.f;   // exp(-33) * 2^46 < 1/2: a token this many temperatures down weighs 0
-constexpr uint32_t kNoBin = 0xffffffffu;
+constexpr int kList = 1024;                        // tokens that are compared with each other in LDS
+constexpr int kPivotTopK = 512;                    // up to here top-k rows are listed
 
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 
@@ -54,17 +56,16 @@ __device__ __forceinline__ float float_of(uint32_t key) {
 }
 
 // f(value, index) for every element of a row, each by some thread of the workgroup: the 16-byte
-// aligned body in vectors, what lies before and after it one element per thread.
-template <typename T, typename F>
+// aligned body in vectors, kLoads of them in flight per thread, what lies before and after it one
+// element per thread.
+template <int kLoads, typename T, typename F>
 __device__ __forceinline__ void for_each(const T* x, int32_t n, F f) {
   constexpr int kVec = 16 / sizeof(T);
   const int32_t before = static_cast<int32_t>(((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T));
   const int32_t head = before < n ? before : n;
   const u32x4* body = reinterpret_cast<const u32x4*>(x + head);
   const int32_t vectors = (n - head) / kVec;
-  for (int32_t q = threadIdx.x; q < vectors; q += kThreads) {
-    const u32x4 raw = body[q];
-    const int32_t i = head + q * kVec;
+  auto use = [&](const u32x4& raw, int32_t i) {
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
       if constexpr (sizeof(T) == 4) {
@@ -74,7 +75,16 @@ __device__ __forceinline__ void for_each(const T* x, int32_t n, F f) {
         f(bf16_hi(raw[w]), i + 2 * w + 1);
       }
     }
+  };
+  int32_t q = threadIdx.x;
+  for (; q + (kLoads - 1) * kThreads < vectors; q += kLoads * kThreads) {
+    u32x4 raw[kLoads];
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) raw[u] = body[q + u * kThreads];
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) use(raw[u], head + (q + u * kThreads) * kVec);
   }
+  for (; q < vectors; q += kThreads) use(body[q], head + q * kVec);
   const int32_t tail = head + vectors * kVec;
   const int32_t t = threadIdx.x;
   if (t < head + (n - tail)) {
@@ -83,40 +93,70 @@ __device__ __forceinline__ void for_each(const T* x, int32_t n, F f) {
   }
 }
 
-// What the weights of one row go by.
-struct Row {
-  float top;     // the largest logit
-  float scale;   // bins per unit of logit
-  double inv_t;
-  double one;
-  double min_p;
-};
-
-__device__ __forceinline__ uint32_t bin_of(const Row& r, float x) {
-  if (x == r.top) return 0;
-  const float at = (r.top - x) * r.scale;  // falls with x: each step rounds monotonically
-  return at < static_cast<float>(kBins - 1) ? static_cast<uint32_t>(at) : kBins - 1;
-}
-
-__device__ __forceinline__ uint64_t weight_of(const Row& r, float x) {
-  const double d = x == r.top ? 0.0 : static_cast<double>(x) - static_cast<double>(r.top);
-  if (!(d > -INFINITY)) return 0;
-  const double w = exp(d * r.inv_t);
-  return w >= r.min_p ? static_cast<uint64_t>(__double2ull_rn(w * r.one)) : 0;
-}
-
 struct Shared {
   uint64_t mass[kBins + 1];   // exclusive sums over the bins before, once summed up
   uint32_t count[kBins + 1];
   uint64_t list_mass[kList];
+  uint64_t order_mass[kList];
   uint32_t list_key[kList];
   int32_t list_index[kList];
+  int32_t order_index[kList];
+  double power[kPerOctave];   // 2^(j / kPerOctave)
   uint64_t sum[kWaves];
   uint32_t waves[kWaves];
   uint64_t base_mass, found_mass;
   uint32_t base_count, bin, listed;
   int32_t found;
 };
+
+// What the weights of one row go by.
+struct Row {
+  float top;        // the largest logit
+  double rate;      // bins per unit of logit: kPerOctave * log2(e) / T
+  double one;       // 2^(fractional bits)
+  double least;     // min_p * one
+  const double* power;
+};
+
+// A token's distance from the top in bins, a number <= 0 (NaN for -inf logits under an infinite T).
+__device__ __forceinline__ double depth_of(const Row& r, float x) {
+  return x == r.top ? 0.0 : (static_cast<double>(x) - static_cast<double>(r.top)) * r.rate;
+}
+
+__device__ __forceinline__ int32_t bin_of_depth(double z) {  // falls with the logit: each step rounds monotonically
+  return z > -static_cast<double>(kBins) ? -static_cast<int32_t>(rint(z)) : kBins;
+}
+
+// The weight of a token at depth z, in bin -n: 2^(z / 128) = 2^(n >> 7) * power[n & 127] * 2^((z - n) / 128), the
+// last factor, of |z - n| <= 1/2, by its series: the first term left out is below 2^-52.
+__device__ __forceinline__ uint64_t weight_of_depth(const Row& r, double z, int32_t bin) {
+  if (bin >= kBins) return 0;
+  const int32_t n = -bin;
+  const double t = (z + bin) * (0.69314718055994530942 / kPerOctave);
+  const double tail = t + t * t * (0.5 + t * (1.0 / 6 + t * (1.0 / 24 + t * (1.0 / 120))));
+  const double base = r.power[n & (kPerOctave - 1)];
+  const double w = ldexp(base + base * tail, n >> 7) * r.one;
+  // Adding 2^52 rounds to a whole number, to nearest, in the low bits.
+  return w >= r.least ? __double_as_longlong(w + 0x1p52) & 0xfffffffffffffll : 0;
+}
+
+__device__ __forceinline__ uint64_t weight_of(const Row& r, float x) {
+  const double z = depth_of(r, x);
+  return weight_of_depth(r, z, bin_of_depth(z));
+}
+
+// A logit that lies no higher than any of bin `bin`'s: what is below it need not be looked at. The
+// margin covers the rounding of the quotient and of the difference to float32.
+__device__ __forceinline__ float floor_of_bin(const Row& r, int32_t bin) {
+  const double x = static_cast<double>(r.top) - (bin + 0.5) / r.rate;
+  const float low = static_cast<float>(x - (fabs(x) + fabs(static_cast<double>(r.top))) * 0x1p-22);
+  return low == low ? low : -INFINITY;
+}
+__device__ __forceinline__ float ceiling_of_bin(const Row& r, int32_t bin) {
+  const double x = static_cast<double>(r.top) - (bin - 0.5) / r.rate;
+  const float high = static_cast<float>(x + (fabs(x) + fabs(static_cast<double>(r.top))) * 0x1p-22);
+  return high == high ? high : INFINITY;
+}
 
 __device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int mask) {
   const uint32_t lo = __shfl_xor(static_cast<uint32_t>(v), mask);
@@ -178,7 +218,7 @@ struct Place {
 // The first token of the order whose cumulative count (by_count) or mass reaches `target`, which
 // the row's totals reach. Every thread gets the answer.
 template <typename T>
-__device__ Place locate(Shared& s, const Row& r, const T* x, int32_t vocab, bool by_count, uint64_t target) {
+__device__ __forceinline__ Place locate(Shared& s, const Row& r, const T* x, int32_t vocab, bool by_count, uint64_t target) {
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kBinsPerThread; ++i) {
@@ -193,17 +233,25 @@ __device__ Place locate(Shared& s, const Row& r, const T* x, int32_t vocab, bool
   }
   if (threadIdx.x == 0) s.listed = 0;
   __syncthreads();
-  const uint32_t bin = s.bin;
+  const int32_t bin = s.bin;
   uint64_t base_mass = s.base_mass;
   uint32_t base_count = s.base_count;
+  const float floor = floor_of_bin(r, bin), ceiling = ceiling_of_bin(r, bin);
   uint32_t low = 0, high = 0xffffffffu;  // keys still in question
-  auto collect = [&]() {
-    for_each(x, vocab, [&](float v, int32_t i) {
-      if (bin_of(r, v) != bin) return;
+  // f(value, index, key, weight) for the bin's tokens with keys of [from, to].
+  auto tokens = [&](uint32_t from, uint32_t to, auto f) {
+    for_each<4>(x, vocab, [&](float v, int32_t i) {
+      if (!(v >= floor && v <= ceiling)) return;
+      const double z = depth_of(r, v);
+      if (bin_of_depth(z) != bin) return;
       const uint32_t key = key_of(v);
-      if (key < low || key > high) return;
-      const uint64_t w = weight_of(r, v);
-      if (w == 0) return;
+      if (key < from || key > to) return;
+      const uint64_t w = weight_of_depth(r, z, bin);
+      if (w != 0) f(i, key, w);
+    });
+  };
+  auto collect = [&]() {
+    tokens(low, high, [&](int32_t i, uint32_t key, uint64_t w) {
       const uint32_t at = atomicAdd(&s.listed, 1u);
       if (at < kList) {
         s.list_key[at] = key;
@@ -220,13 +268,9 @@ __device__ Place locate(Shared& s, const Row& r, const T* x, int32_t vocab, bool
     while (listed > kList && low < high) {
       const uint32_t mid = low + (high - low) / 2 + 1;
       uint64_t mass = 0, count = 0;
-      for_each(x, vocab, [&](float v, int32_t) {
-        if (bin_of(r, v) != bin) return;
-        const uint32_t key = key_of(v);
-        if (key < mid || key > high) return;
-        const uint64_t w = weight_of(r, v);
+      tokens(mid, high, [&](int32_t, uint32_t, uint64_t w) {
         mass += w;
-        count += w != 0;
+        ++count;
       });
       mass = block_sum(s, mass);
       count = block_sum(s, count);
@@ -268,9 +312,9 @@ __device__ Place locate(Shared& s, const Row& r, const T* x, int32_t vocab, bool
     collect();
     listed = s.listed;
   }
-  for (uint32_t i = threadIdx.x; i < listed; i += kThreads) {
-    const uint32_t key = s.list_key[i];
-    const int32_t index = s.list_index[i];
+  if (threadIdx.x < listed) {
+    const uint32_t key = s.list_key[threadIdx.x];
+    const int32_t index = s.list_index[threadIdx.x];
     uint64_t mass = base_mass, count = base_count;
     for (uint32_t j = 0; j < listed; ++j) {
       const uint32_t other = s.list_key[j];
@@ -279,7 +323,7 @@ __device__ Place locate(Shared& s, const Row& r, const T* x, int32_t vocab, bool
         ++count;
       }
     }
-    const uint64_t upto = mass + s.list_mass[i];
+    const uint64_t upto = mass + s.list_mass[threadIdx.x];
     if (by_count ? count + 1 == target : mass < target && target <= upto) {
       s.found = index;
       s.found_mass = upto;
@@ -287,6 +331,62 @@ __device__ Place locate(Shared& s, const Row& r, const T* x, int32_t vocab, bool
   }
   __syncthreads();
   return {s.found_mass, s.found};
+}
+
+// The mass that top_p keeps of `mass` is the cumulative one of the first token to reach this.
+__device__ __forceinline__ uint64_t nucleus(float top_p, uint64_t mass) {
+  const double want = top_p > 0.f ? ceil(static_cast<double>(top_p) * static_cast<double>(mass)) : 1.0;
+  const uint64_t target = static_cast<uint64_t>(want);
+  return target < 1 ? 1 : target < mass ? target : mass;
+}
+
+// The token is the first whose cumulative mass reaches this.
+__device__ __forceinline__ uint64_t place_of(float u, uint64_t mass) {
+  const uint64_t at = u > 0.f ? static_cast<uint64_t>(static_cast<double>(u) * static_cast<double>(mass)) : 0;
+  return at < mass ? at + 1 : mass;
+}
+
+// The whole row's answer from the `listed` <= kList tokens of its list, which hold every token that the
+// cuts can keep: one token per thread, put in order by counting, then summed up along the order.
+__device__ __forceinline__ int32_t from_list(Shared& s, const Row& r, uint32_t listed, int32_t top_k, float top_p, float u) {
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  const bool mine = threadIdx.x < listed;
+  if (mine) {
+    const uint32_t key = s.list_key[threadIdx.x];
+    const int32_t index = s.list_index[threadIdx.x];
+    uint32_t rank = 0;
+    for (uint32_t j = 0; j < listed; ++j) {
+      const uint32_t other = s.list_key[j];
+      rank += other > key || (other == key && s.list_index[j] < index);
+    }
+    s.order_mass[rank] = weight_of(r, float_of(key));
+    s.order_index[rank] = index;
+  }
+  __syncthreads();
+  const bool kept = mine && (top_k <= 0 || threadIdx.x < static_cast<uint32_t>(top_k));
+  const uint64_t own = kept ? s.order_mass[threadIdx.x] : 0;
+  uint64_t upto = own;
+  for (int d = 1; d < kWave; d <<= 1) {
+    const uint64_t other = shfl_up64(upto, d);
+    if (lane >= d) upto += other;
+  }
+  if (lane == kWave - 1) s.sum[wave] = upto;
+  __syncthreads();
+  uint64_t mass = 0;
+  for (int w = 0; w < kWaves; ++w) {
+    upto += w < wave ? s.sum[w] : 0;
+    mass += s.sum[w];
+  }
+  if (!(top_p >= 1.f)) {
+    const uint64_t target = nucleus(top_p, mass);
+    if (own != 0 && upto - own < target && target <= upto) s.found_mass = upto;
+    __syncthreads();
+    mass = s.found_mass;
+  }
+  const uint64_t target = place_of(u, mass);
+  if (own != 0 && upto - own < target && target <= upto) s.found = s.order_index[threadIdx.x];
+  __syncthreads();
+  return s.found;
 }
 
 // One workgroup per row.
@@ -300,77 +400,116 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const Args a) {
   const int32_t top_k = a.top_ks ? a.top_ks[row] : a.top_k;
   const float top_p = a.top_ps ? a.top_ps[row] : a.top_p;
   const float min_p = a.min_ps ? a.min_ps[row] : a.min_p;
+  const float u = a.uniforms[row];
+  if (threadIdx.x < kPerOctave) s.power[threadIdx.x] = exp2(threadIdx.x * (1.0 / kPerOctave));
 
-  // The greedy token (the first NaN, else the first of the largest), and the smallest finite logit.
-  // A NaN counts as the largest key.
-  uint64_t best = 0;  // key, then the complement of the index
-  float least = INFINITY;
-  for_each(x, a.vocab, [&](float v, int32_t i) {
-    const uint32_t key = isnan(v) ? 0xffffffffu : key_of(v);
-    const uint64_t mine = (static_cast<uint64_t>(key) << 32) | (0xffffffffu - static_cast<uint32_t>(i));
-    best = mine > best ? mine : best;
-    if (v > -INFINITY && v < least) least = v;
+  float most = -INFINITY;
+  bool odd = false;
+  for_each<4>(x, a.vocab, [&](float v, int32_t) {
+    most = fmaxf(most, v);
+    odd = odd || v != v;
   });
-  for (int m = kWave / 2; m > 0; m >>= 1) {
-    const uint64_t other = shfl_xor64(best, m);
-    best = other > best ? other : best;
-    least = fminf(least, __shfl_xor(least, m));
-  }
-  if (lane == 0) {
-    s.sum[wave] = best;
-    s.waves[wave] = __float_as_uint(least);
-  }
-  __syncthreads();
-  for (int w = 0; w < kWaves; ++w) {
-    best = s.sum[w] > best ? s.sum[w] : best;
-    least = fminf(least, __uint_as_float(s.waves[w]));
-  }
-  const uint32_t top_key = static_cast<uint32_t>(best >> 32);
-  const int32_t greedy = static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(best));
-  const bool drawn = temperature > 0.f && top_key != 0xffffffffu && top_key > key_of(-INFINITY);
-  if (!drawn) {
-    if (threadIdx.x == 0) a.out[row] = greedy;
+  float top = most;
+  for (int m = kWave / 2; m > 0; m >>= 1) top = fmaxf(top, __shfl_xor(top, m));
+  if (lane == 0) s.waves[wave] = __float_as_uint(top);
+  const bool any_odd = __syncthreads_or(odd);
+  for (int w = 0; w < kWaves; ++w) top = fmaxf(top, __uint_as_float(s.waves[w]));
+  if (any_odd || top == -INFINITY || !(temperature > 0.f)) {  // the greedy token: the first NaN, else the first of the largest
+    if (threadIdx.x == 0) s.found = a.vocab;
+    __syncthreads();
+    int32_t first = a.vocab;
+    for_each<4>(x, a.vocab, [&](float v, int32_t i) {
+      if (any_odd ? v != v : v == top) first = min(first, i);
+    });
+    if (first < a.vocab) atomicMin(&s.found, first);
+    __syncthreads();
+    if (threadIdx.x == 0) a.out[row] = s.found;
     return;
   }
 
   Row r;
-  r.top = float_of(top_key);
-  r.inv_t = 1.0 / static_cast<double>(temperature);
+  r.top = top;
+  r.rate = kPerOctave * 1.44269504088896340736 / static_cast<double>(temperature);
   r.one = a.one;
-  r.min_p = min_p > 0.f ? fmin(static_cast<double>(min_p), 1.0) : 0.0;
-  const float range = fminf(r.top - least, kReach * temperature);
-  r.scale = range > 0.f ? fminf(kBins / range, 1e30f) : 0.f;
-
+  r.least = min_p > 0.f ? fmin(static_cast<double>(min_p), 1.0) * a.one : 0.0;
+  r.power = s.power;
   const bool counting = top_k > 0;
   for (int i = threadIdx.x; i <= kBins; i += kThreads) {
     s.mass[i] = 0;
     s.count[i] = 0;
   }
+  if (threadIdx.x == 0) {
+    s.listed = 0;
+    s.bin = kBins;
+  }
   __syncthreads();
-  for_each(x, a.vocab, [&](float v, int32_t) {
-    const uint64_t w = weight_of(r, v);
+
+  // The bins that the kept tokens lie in, where the settings bound them beforehand: min-p by its weight;
+  // top-k by the threads' largest tokens, of which there are top_k in the bins up to the pivot's.
+  int32_t last = kBins - 1;
+  if (min_p > 0.f) {
+    const double deep = ceil(-log2(fmin(static_cast<double>(min_p), 1.0)) * kPerOctave) + 1.0;
+    last = deep < last ? static_cast<int32_t>(deep) : last;
+  }
+  if (counting && top_k <= kPivotTopK) {
+    const int32_t bin = bin_of_depth(depth_of(r, most));
+    if (bin < kBins) atomicAdd(&s.count[bin], 1u);
+    __syncthreads();
+    scan_bins(s, s.count);
+#pragma unroll
+    for (int i = 0; i < kBinsPerThread; ++i) {
+      const int b = threadIdx.x * kBinsPerThread + i;
+      if (s.count[b] < static_cast<uint32_t>(top_k) && static_cast<uint32_t>(top_k) <= s.count[b + 1]) s.bin = b;
+    }
+    __syncthreads();
+    last = min(last, static_cast<int32_t>(s.bin));
+    for (int i = threadIdx.x; i <= kBins; i += kThreads) s.count[i] = 0;
+  }
+  const float floor = floor_of_bin(r, last);
+  if (last < kBins - 1 || a.vocab <= kList) {
+    for_each<4>(x, a.vocab, [&](float v, int32_t i) {
+      if (!(v >= floor) || bin_of_depth(depth_of(r, v)) > last) return;
+      const uint32_t slot = atomicAdd(&s.listed, 1u);
+      if (slot < kList) {
+        s.list_key[slot] = key_of(v);
+        s.list_index[slot] = i;
+      }
+    });
+    __syncthreads();
+    const uint32_t listed = s.listed;
+    if (listed <= kList) {
+      const int32_t token = from_list(s, r, listed, top_k, top_p, u);
+      if (threadIdx.x == 0) a.out[row] = token;
+      return;
+    }
+  }
+  __syncthreads();
+
+  for_each<2>(x, a.vocab, [&](float v, int32_t) {
+    if (!(v >= floor)) return;
+    const double z = depth_of(r, v);
+    const int32_t bin = bin_of_depth(z);
+    const uint64_t w = weight_of_depth(r, z, bin);
     if (w == 0) return;
-    const uint32_t b = bin_of(r, v);
-    atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[b]), static_cast<unsigned long long>(w));
-    if (counting) atomicAdd(&s.count[b], 1u);
+    atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[bin]), static_cast<unsigned long long>(w));
+    if (counting) atomicAdd(&s.count[bin], 1u);
   });
   __syncthreads();
   scan_bins(s, s.mass);
   if (counting) scan_bins(s, s.count);
 
+  // Three times the same search: the end of top-k, of top-p, and the draw.
   uint64_t mass = s.mass[kBins];
-  if (counting && s.count[kBins] > static_cast<uint32_t>(top_k)) mass = locate(s, r, x, a.vocab, true, top_k).mass;
-  if (!(top_p >= 1.f)) {
-    const double want = top_p > 0.f ? ceil(static_cast<double>(top_p) * static_cast<double>(mass)) : 1.0;
-    uint64_t target = static_cast<uint64_t>(want);
-    target = target < 1 ? 1 : target;
-    mass = locate(s, r, x, a.vocab, false, target < mass ? target : mass).mass;
+  const bool cut = counting && s.count[kBins] > static_cast<uint32_t>(top_k);
+  int32_t token = 0;
+  for (int step = 0; step < 3; ++step) {
+    if ((step == 0 && !cut) || (step == 1 && top_p >= 1.f)) continue;
+    const uint64_t target = step == 0 ? static_cast<uint64_t>(top_k) : step == 1 ? nucleus(top_p, mass) : place_of(u, mass);
+    const Place place = locate(s, r, x, a.vocab, step == 0, target);
+    mass = place.mass;
+    token = place.index;
   }
-  const float u = a.uniforms[row];
-  uint64_t at = u > 0.f ? static_cast<uint64_t>(static_cast<double>(u) * static_cast<double>(mass)) : 0;
-  at = at < mass ? at : mass - 1;
-  const Place place = locate(s, r, x, a.vocab, false, at + 1);
-  if (threadIdx.x == 0) a.out[row] = place.index;
+  if (threadIdx.x == 0) a.out[row] = token;
 }
 
 }  // namespace
