@@ -17,6 +17,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxAxes = 4;
+constexpr int kHeads = 2;  // heads of one thread
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
@@ -105,9 +106,9 @@ struct RopeAxes {
   int32_t num_axes, interleaved;
   int32_t ends[kMaxAxes];  // frequencies of axes 0..a (their sections' running sum)
   int32_t sections[kMaxAxes];
-  // Work units of one token, kVec elements (a rotated unit: kVec pairs) each, in this order.
-  int32_t rot_per_head, rest_per_head, rot_units, rest_units, units;
-  int32_t tokens_per_group, groups_per_token;  // one of the two is 1
+  // A token's work: `chunks` pieces of a head (turned ones, kVec pairs each, then copied ones of kVec
+  // elements) times `sets` sets of up to kHeads of the query, key and value heads.
+  int32_t turned, chunks, sets;
 };
 
 // The axis that turns frequency i: contiguous sections, or one frequency of each axis in turn until
@@ -123,126 +124,108 @@ __device__ __forceinline__ int axis_of(const RopeAxes& a, int i) {
   return axis;
 }
 
-// One work unit per thread. A token's units are spread over whole workgroups, or several tokens
-// share one where a token has fewer units than a workgroup has threads.
+// One thread per (token, set of kHeads heads, piece of a head): the heads of a set share their table
+// entries, and their loads are all in flight before the first is used. Heads of one set are a number of sets
+// apart, so that the threads of a wavefront read neighbouring heads. The values' heads are copied by the
+// threads of the same pieces.
 template <typename IoT, typename PoolT, int kVec>
 __global__ __launch_bounds__(kThreads) void rope_axes_kernel(const RopeAxes a) {
-  int64_t token;
-  uint32_t unit;
-  if (a.tokens_per_group > 1) {
-    const uint32_t local = threadIdx.x / static_cast<uint32_t>(a.units);
-    unit = threadIdx.x - local * a.units;
-    token = static_cast<int64_t>(blockIdx.x) * a.tokens_per_group + local;
-    if (local >= static_cast<uint32_t>(a.tokens_per_group)) return;
-  } else {
-    const uint32_t group = blockIdx.x / static_cast<uint32_t>(a.groups_per_token);
-    token = group;
-    unit = (blockIdx.x - group * a.groups_per_token) * kThreads + threadIdx.x;
+  const uint32_t item = blockIdx.x * static_cast<uint32_t>(kThreads) + threadIdx.x;
+  const uint32_t rest = item / static_cast<uint32_t>(a.chunks);
+  const int chunk = item - rest * a.chunks;
+  const uint32_t token = rest / static_cast<uint32_t>(a.sets);
+  const int set = rest - token * a.sets;
+  if (token >= a.num_tokens) return;
+  const int64_t t = token;
+  const bool pair = chunk < a.turned;
+  const int i = pair ? chunk * kVec : 2 * a.half + (chunk - a.turned) * kVec;  // dimension of the (lower) piece
+  const int heads = a.num_heads + 2 * a.num_kv_heads;
+
+  float lo[kHeads][kVec], hi[kHeads][kVec];
+#pragma unroll
+  for (int h = 0; h < kHeads; ++h) {
+    const int head = set + h * a.sets;
+    if (head >= heads) break;
+    const int kv = head - a.num_heads;
+    const IoT* src = kv < 0 ? static_cast<const IoT*>(a.queries) + t * a.q_stride + static_cast<int64_t>(head) * a.head_dim
+                     : kv < a.num_kv_heads
+                         ? static_cast<const IoT*>(a.keys) + t * a.k_stride + static_cast<int64_t>(kv) * a.head_dim
+                         : static_cast<const IoT*>(a.values) + t * a.v_stride + static_cast<int64_t>(kv - a.num_kv_heads) * a.head_dim;
+    load_vec<IoT, kVec>(src + i, lo[h]);
+    if (pair) load_vec<IoT, kVec>(src + i + a.half, hi[h]);
   }
-  if (token >= a.num_tokens || unit >= static_cast<uint32_t>(a.units)) return;
 
   int64_t pos[kMaxAxes];
   bool inside = true;
 #pragma unroll
   for (int n = 0; n < kMaxAxes; ++n) {
-    pos[n] = n < a.num_axes ? a.positions[n * a.axis_stride + token] : 0;
-    inside = inside && (n >= a.num_axes || (pos[n] >= 0 && pos[n] < a.table_rows));
+    pos[n] = n < a.num_axes ? a.positions[n * a.axis_stride + t] : 0;
+    inside = inside && pos[n] >= 0 && (n >= a.num_axes || pos[n] < a.table_rows);
   }
-  const int64_t slot = a.slots[token];
+  const int64_t slot = a.slots[t];
   const bool stored = slot >= 0 && slot < a.num_slots;
   if (!inside) return;
 
-  const int D = a.head_dim;
-  const int64_t pool_row = slot * a.num_kv_heads * static_cast<int64_t>(D);
-  const auto* values = static_cast<const IoT*>(a.values);
-  if (unit >= static_cast<uint32_t>(a.rot_units + a.rest_units)) {  // a piece of the value row
-    if (!stored) return;
-    const int at = (unit - a.rot_units - a.rest_units) * kVec;
-    float v[kVec];
-    load_vec<IoT, kVec>(values + token * a.v_stride + at, v);
-    store_vec<PoolT, kVec>(static_cast<PoolT*>(a.value_pool) + pool_row + at, v);
-    return;
-  }
-  const bool turned = unit < static_cast<uint32_t>(a.rot_units);
-  const uint32_t within = turned ? unit : unit - a.rot_units;
-  const uint32_t per_head = turned ? a.rot_per_head : a.rest_per_head;
-  const int head = within / per_head;
-  const int i = (within - head * per_head) * kVec;
-  const bool key = head >= a.num_heads;
-  if (key && !stored) return;
-  const int at = (key ? head - a.num_heads : head) * D + (turned ? i : 2 * a.half + i);
-  const IoT* src = key ? static_cast<const IoT*>(a.keys) + token * a.k_stride + at
-                       : static_cast<const IoT*>(a.queries) + token * a.q_stride + at;
-  IoT* rotated = static_cast<IoT*>(a.rotated) + token * a.rotated_stride + at;
-  PoolT* pool = static_cast<PoolT*>(a.key_pool) + pool_row + at;
-  float lo[kVec];
-  load_vec<IoT, kVec>(src, lo);
-  if (!turned) {
-    if (key) {
-      store_vec<PoolT, kVec>(pool, lo);
+  float c[kVec], s[kVec];
+  if (pair) {
+    auto row_of = [&](int n) { return n == 0 ? pos[0] : n == 1 ? pos[1] : n == 2 ? pos[2] : pos[3]; };
+    const int axis = axis_of(a, i);
+    if (a.num_axes == 1 || (!a.interleaved && axis == axis_of(a, i + kVec - 1))) {
+      const int64_t row = row_of(axis) * a.half + i;
+      load_table<kVec>(a.cos_table + row, c);
+      load_table<kVec>(a.sin_table + row, s);
     } else {
-      store_vec<IoT, kVec>(rotated, lo);
-    }
-    return;
-  }
-  float hi[kVec], c[kVec], s[kVec];
-  load_vec<IoT, kVec>(src + a.half, hi);
-  const int axis = axis_of(a, i);
-  bool uniform = a.num_axes == 1 || (!a.interleaved && axis == axis_of(a, i + kVec - 1));
-  auto row_of = [&](int n) { return n == 0 ? pos[0] : n == 1 ? pos[1] : n == 2 ? pos[2] : pos[3]; };
-  if (uniform) {
-    const int64_t row = row_of(axis) * a.half + i;
-    load_table<kVec>(a.cos_table + row, c);
-    load_table<kVec>(a.sin_table + row, s);
-  } else {
 #pragma unroll
-    for (int e = 0; e < kVec; ++e) {
-      const int64_t row = row_of(axis_of(a, i + e)) * a.half + i + e;
-      c[e] = a.cos_table[row];
-      s[e] = a.sin_table[row];
+      for (int e = 0; e < kVec; ++e) {
+        const int64_t row = row_of(axis_of(a, i + e)) * a.half + i + e;
+        c[e] = a.cos_table[row];
+        s[e] = a.sin_table[row];
+      }
     }
   }
-  {
+  const int64_t pool_row = slot * a.num_kv_heads * static_cast<int64_t>(a.head_dim);
+#pragma unroll
+  for (int h = 0; h < kHeads; ++h) {
+    const int head = set + h * a.sets;
+    if (head >= heads) break;
+    const int kv = head - a.num_heads;
+    if (pair && kv < a.num_kv_heads) {
 #pragma clang fp contract(off)
 #pragma unroll
-    for (int e = 0; e < kVec; ++e) {
-      const float ac = lo[e] * c[e];
-      const float bs = hi[e] * s[e];
-      const float bc = hi[e] * c[e];
-      const float as = lo[e] * s[e];
-      lo[e] = ac - bs;
-      hi[e] = bc + as;
+      for (int e = 0; e < kVec; ++e) {
+        const float ac = lo[h][e] * c[e];
+        const float bs = hi[h][e] * s[e];
+        const float bc = hi[h][e] * c[e];
+        const float as = lo[h][e] * s[e];
+        lo[h][e] = ac - bs;
+        hi[h][e] = bc + as;
+      }
     }
-  }
-  // The rotated queries may overwrite the queries in place: this thread has read both its pieces.
-  if (key) {
-    store_vec<PoolT, kVec>(pool, lo);
-    store_vec<PoolT, kVec>(pool + a.half, hi);
-  } else {
-    store_vec<IoT, kVec>(rotated, lo);
-    store_vec<IoT, kVec>(rotated + a.half, hi);
+    // The rotated queries may overwrite the queries in place: this thread has read its pieces of them.
+    if (kv < 0) {
+      IoT* to = static_cast<IoT*>(a.rotated) + t * a.rotated_stride + static_cast<int64_t>(head) * a.head_dim + i;
+      store_vec<IoT, kVec>(to, lo[h]);
+      if (pair) store_vec<IoT, kVec>(to + a.half, hi[h]);
+    } else if (stored) {
+      const bool key = kv < a.num_kv_heads;
+      PoolT* to = static_cast<PoolT*>(key ? a.key_pool : a.value_pool) + pool_row +
+                  static_cast<int64_t>(key ? kv : kv - a.num_kv_heads) * a.head_dim + i;
+      store_vec<PoolT, kVec>(to, lo[h]);
+      if (pair) store_vec<PoolT, kVec>(to + a.half, hi[h]);
+    }
   }
 }
 
 template <typename IoT, typename PoolT, int kVec>
 int launch(RopeAxes a, hipStream_t stream) {
-  const int64_t heads = a.num_heads + a.num_kv_heads;
-  a.rot_per_head = a.half / kVec;
-  a.rest_per_head = (a.head_dim - 2 * a.half) / kVec;
-  const int64_t rot = heads * a.rot_per_head;
-  const int64_t rest = heads * a.rest_per_head;
-  const int64_t units = rot + rest + static_cast<int64_t>(a.num_kv_heads) * a.head_dim / kVec;
-  if (units > 0x3fffffff) return PKV_EUNSUPPORTED;
-  a.rot_units = static_cast<int32_t>(rot);
-  a.rest_units = static_cast<int32_t>(rest);
-  a.units = static_cast<int32_t>(units);
-  a.tokens_per_group = units < kThreads ? static_cast<int32_t>(kThreads / units) : 1;
-  a.groups_per_token = static_cast<int32_t>((units + kThreads - 1) / kThreads);
-  const int64_t groups = a.tokens_per_group > 1 ? (a.num_tokens + a.tokens_per_group - 1) / a.tokens_per_group
-                                                : a.num_tokens * a.groups_per_token;
-  if (groups > 0x7fffffff) return PKV_EUNSUPPORTED;
-  hipLaunchKernelGGL((rope_axes_kernel<IoT, PoolT, kVec>), dim3(static_cast<uint32_t>(groups)), dim3(kThreads), 0,
-                     stream, a);
+  const int64_t heads = a.num_heads + 2 * static_cast<int64_t>(a.num_kv_heads);
+  a.turned = a.half / kVec;
+  a.chunks = a.turned + (a.head_dim - 2 * a.half) / kVec;
+  a.sets = static_cast<int32_t>((heads + kHeads - 1) / kHeads);
+  const int64_t items = a.num_tokens * a.chunks * a.sets;
+  if (heads > 0x3fffffff || a.num_tokens > 0x7fffffff || items > 0xffff0000ll) return PKV_EUNSUPPORTED;
+  hipLaunchKernelGGL((rope_axes_kernel<IoT, PoolT, kVec>), dim3(static_cast<uint32_t>((items + kThreads - 1) / kThreads)), dim3(kThreads),
+                     0, stream, a);
   return check_launch();
 }
 

@@ -22,7 +22,8 @@ constexpr int kWaves = kThreads / kWave;
 constexpr int kPerOctave = 128;                    // bins, and entries of the table of powers
 constexpr int kBins = 48 * kPerOctave;             // 2^-47.5 * 2^46 < 1/2: later bins weigh nothing
 constexpr int kBinsPerThread = kBins / kThreads;
-constexpr int kList = 1024;                        // tokens that are compared with each other in LDS
+constexpr int kList = 1024;                        // tokens of one bin that are compared with each other
+constexpr int kFew = 512;                          // tokens that are put in order instead of counted in bins
 constexpr int kPivotTopK = 512;                    // up to here top-k rows are listed
 
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
@@ -94,14 +95,13 @@ __device__ __forceinline__ void for_each(const T* x, int32_t n, F f) {
 }
 
 struct Shared {
-  uint64_t mass[kBins + 1];   // exclusive sums over the bins before, once summed up
-  uint32_t count[kBins + 1];
-  uint64_t list_mass[kList];
-  uint64_t order_mass[kList];
-  uint32_t list_key[kList];
-  int32_t list_index[kList];
-  int32_t order_index[kList];
-  double power[kPerOctave];   // 2^(j / kPerOctave)
+  uint64_t mass[kBins + 2];   // exclusive sums over the bins before, once summed up
+  uint32_t count[kBins + 2];
+  __align__(16) uint64_t list[kList];       // tokens as order_of gives them
+  __align__(16) uint64_t list_mass[kList];
+  uint64_t before[kList];     // of each token of the list: the mass, and the number, that come before it
+  uint32_t rank[kList];
+  double power[kPerOctave];   // 2^(j / kPerOctave) * 2^(fractional bits)
   uint64_t sum[kWaves];
   uint32_t waves[kWaves];
   uint64_t base_mass, found_mass;
@@ -109,53 +109,59 @@ struct Shared {
   int32_t found;
 };
 
-// What the weights of one row go by.
+// What the weights of one row go by. Its largest logit is finite here.
 struct Row {
-  float top;        // the largest logit
+  float top;
   double rate;      // bins per unit of logit: kPerOctave * log2(e) / T
-  double one;       // 2^(fractional bits)
-  double least;     // min_p * one
+  double least;     // min_p * 2^(fractional bits)
   const double* power;
 };
 
-// A token's distance from the top in bins, a number <= 0 (NaN for -inf logits under an infinite T).
-__device__ __forceinline__ double depth_of(const Row& r, float x) {
-  return x == r.top ? 0.0 : (static_cast<double>(x) - static_cast<double>(r.top)) * r.rate;
-}
+struct Weight {
+  int32_t bin;
+  uint64_t mass;
+};
 
-__device__ __forceinline__ int32_t bin_of_depth(double z) {  // falls with the logit: each step rounds monotonically
-  return z > -static_cast<double>(kBins) ? -static_cast<int32_t>(rint(z)) : kBins;
-}
-
-// The weight of a token at depth z, in bin -n: 2^(z / 128) = 2^(n >> 7) * power[n & 127] * 2^((z - n) / 128), the
-// last factor, of |z - n| <= 1/2, by its series: the first term left out is below 2^-52.
-__device__ __forceinline__ uint64_t weight_of_depth(const Row& r, double z, int32_t bin) {
-  if (bin >= kBins) return 0;
-  const int32_t n = -bin;
-  const double t = (z + bin) * (0.69314718055994530942 / kPerOctave);
-  const double tail = t + t * t * (0.5 + t * (1.0 / 6 + t * (1.0 / 24 + t * (1.0 / 120))));
+// The bin and weight of a finite logit; what lies below the bins weighs 0. Its depth z below the top in bins is
+// n + f with a whole number n <= 0 and |f| <= 1/2, and its weight is
+//     2^(z / 128) = 2^(n >> 7) * power[n & 127] * 2^(f / 128),
+// the last factor by its series (the first term left out is below 2^-49) and the first added to the
+// exponent. Each step to n rounds monotonically: bins fall with the logit. Adding 2^52 * 1.5 or 2^52 leaves
+// a number rounded to a whole one in the low bits.
+template <bool kMin>
+__device__ __forceinline__ Weight weigh(const Row& r, float x) {
+  const double z = fmax((static_cast<double>(x) - static_cast<double>(r.top)) * r.rate, -(kBins + 1.0));
+  const double whole = z + 0x1.8p52;
+  const int32_t n = __double2loint(whole);
+  const double f = z - (whole - 0x1.8p52);
+  constexpr double kStep = 0.69314718055994530942 / kPerOctave;
+  const double series =
+      kStep + f * (kStep * kStep / 2 + f * (kStep * kStep * kStep / 6 + f * (kStep * kStep * kStep * kStep / 24)));
   const double base = r.power[n & (kPerOctave - 1)];
-  const double w = ldexp(base + base * tail, n >> 7) * r.one;
-  // Adding 2^52 rounds to a whole number, to nearest, in the low bits.
-  return w >= r.least ? __double_as_longlong(w + 0x1p52) & 0xfffffffffffffll : 0;
-}
-
-__device__ __forceinline__ uint64_t weight_of(const Row& r, float x) {
-  const double z = depth_of(r, x);
-  return weight_of_depth(r, z, bin_of_depth(z));
+  const double close = base + base * f * series;
+  const double w = __hiloint2double(__double2hiint(close) + (n >> 7) * (1 << 20), __double2loint(close));
+  const double in_place = w + 0x1p52;
+  uint64_t mass = (static_cast<uint64_t>(__double2hiint(in_place) & 0xfffff) << 32) | static_cast<uint32_t>(__double2loint(in_place));
+  if constexpr (kMin) mass = w >= r.least ? mass : 0;
+  return {-n, mass};
 }
 
 // A logit that lies no higher than any of bin `bin`'s: what is below it need not be looked at. The
 // margin covers the rounding of the quotient and of the difference to float32.
 __device__ __forceinline__ float floor_of_bin(const Row& r, int32_t bin) {
   const double x = static_cast<double>(r.top) - (bin + 0.5) / r.rate;
-  const float low = static_cast<float>(x - (fabs(x) + fabs(static_cast<double>(r.top))) * 0x1p-22);
-  return low == low ? low : -INFINITY;
+  const double low = x - (fabs(x) + fabs(static_cast<double>(r.top))) * 0x1p-22;
+  return low >= -3.4028234663852886e38 ? static_cast<float>(low) : -3.4028234663852886e38f;
 }
 __device__ __forceinline__ float ceiling_of_bin(const Row& r, int32_t bin) {
   const double x = static_cast<double>(r.top) - (bin - 0.5) / r.rate;
-  const float high = static_cast<float>(x + (fabs(x) + fabs(static_cast<double>(r.top))) * 0x1p-22);
-  return high == high ? high : INFINITY;
+  const double high = x + (fabs(x) + fabs(static_cast<double>(r.top))) * 0x1p-22;
+  return high <= 3.4028234663852886e38 ? static_cast<float>(high) : 3.4028234663852886e38f;
+}
+
+// Tokens as numbers whose larger one comes first.
+__device__ __forceinline__ uint64_t order_of(uint32_t key, int32_t index) {
+  return (static_cast<uint64_t>(key) << 32) | (0xffffffffu - static_cast<uint32_t>(index));
 }
 
 __device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int mask) {
@@ -210,6 +216,75 @@ __device__ void scan_bins(Shared& s, V* values) {
   __syncthreads();
 }
 
+// For each of the list's `listed` tokens how many tokens (kMass: what mass too) come before it in the
+// list: all pairs, the threads of a token sharing the others among them.
+template <bool kMass>
+__device__ __forceinline__ void rank_list(Shared& s, uint32_t listed) {
+  uint32_t slots = kWave;
+  while (slots < listed) slots *= 2;
+  const uint32_t mine = threadIdx.x & (slots - 1), part = threadIdx.x / slots, parts = kThreads / slots;
+  const uint32_t each = ((listed + parts - 1) / parts + 3) / 4 * 4;
+  if (threadIdx.x < listed) {
+    s.rank[threadIdx.x] = 0;
+    if constexpr (kMass) s.before[threadIdx.x] = 0;
+  }
+  __syncthreads();
+  if (mine < listed) {
+    const uint64_t own = s.list[mine];
+    uint64_t mass = 0;
+    uint32_t count = 0;
+    const uint32_t end = min((part + 1) * each, listed);
+    uint32_t j = part * each;
+    for (; j + 4 <= end; j += 4) {
+      uint64_t other[4], weight[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) other[e] = s.list[j + e];
+      if constexpr (kMass) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) weight[e] = s.list_mass[j + e];
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        count += other[e] > own;
+        if constexpr (kMass) mass += other[e] > own ? weight[e] : 0;
+      }
+    }
+    for (; j < end; ++j) {
+      count += s.list[j] > own;
+      if constexpr (kMass) mass += s.list[j] > own ? s.list_mass[j] : 0;
+    }
+    if (count) atomicAdd(&s.rank[mine], count);
+    if constexpr (kMass) {
+      if (mass) atomicAdd(reinterpret_cast<unsigned long long*>(&s.before[mine]), static_cast<unsigned long long>(mass));
+    }
+  }
+  __syncthreads();
+}
+
+// The `rank`-th token, from 0, of those with this key, along their ids (there is one).
+template <typename T>
+__device__ __forceinline__ int32_t nth_of_key(Shared& s, const T* x, int32_t vocab, uint32_t key, uint64_t rank) {
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  __syncthreads();
+  for (int64_t start = 0; start < vocab; start += kThreads) {
+    const int64_t i = start + threadIdx.x;
+    const bool match = i < vocab && key_of(to_float(x[i])) == key;
+    const uint64_t ballot = __ballot(match);
+    if (lane == 0) s.waves[wave] = __popcll(ballot);
+    __syncthreads();
+    uint32_t before = __popcll(ballot & ((1ull << lane) - 1)), all = 0;
+    for (int w = 0; w < kWaves; ++w) {
+      before += w < wave ? s.waves[w] : 0;
+      all += s.waves[w];
+    }
+    if (match && before == rank) s.found = static_cast<int32_t>(i);
+    __syncthreads();
+    if (rank < all) break;
+    rank -= all;
+  }
+  return s.found;
+}
+
 struct Place {
   uint64_t mass;  // cumulative, the token's own included
   int32_t index;
@@ -242,20 +317,16 @@ __device__ __forceinline__ Place locate(Shared& s, const Row& r, const T* x, int
   auto tokens = [&](uint32_t from, uint32_t to, auto f) {
     for_each<4>(x, vocab, [&](float v, int32_t i) {
       if (!(v >= floor && v <= ceiling)) return;
-      const double z = depth_of(r, v);
-      if (bin_of_depth(z) != bin) return;
+      const Weight w = weigh<true>(r, v);
       const uint32_t key = key_of(v);
-      if (key < from || key > to) return;
-      const uint64_t w = weight_of_depth(r, z, bin);
-      if (w != 0) f(i, key, w);
+      if (w.bin == bin && key >= from && key <= to && w.mass != 0) f(i, key, w.mass);
     });
   };
   auto collect = [&]() {
     tokens(low, high, [&](int32_t i, uint32_t key, uint64_t w) {
       const uint32_t at = atomicAdd(&s.listed, 1u);
       if (at < kList) {
-        s.list_key[at] = key;
-        s.list_index[at] = i;
+        s.list[at] = order_of(key, i);
         s.list_mass[at] = w;
       }
     });
@@ -285,47 +356,21 @@ __device__ __forceinline__ Place locate(Shared& s, const Row& r, const T* x, int
       }
     }
     if (listed > kList) {  // equal logits: the one that far along their ids
-      const uint64_t w = weight_of(r, float_of(low));
-      uint64_t rank = by_count ? target - base_count - 1 : (target - base_mass - 1) / w;
-      const uint64_t mass = base_mass + (rank + 1) * w;
-      const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-      for (int64_t start = 0; start < vocab; start += kThreads) {
-        const int64_t i = start + threadIdx.x;
-        const bool match = i < vocab && key_of(to_float(x[i])) == low;
-        const uint64_t ballot = __ballot(match);
-        if (lane == 0) s.waves[wave] = __popcll(ballot);
-        __syncthreads();
-        uint32_t before = __popcll(ballot & ((1ull << lane) - 1)), all = 0;
-        for (int w2 = 0; w2 < kWaves; ++w2) {
-          before += w2 < wave ? s.waves[w2] : 0;
-          all += s.waves[w2];
-        }
-        if (match && before == rank) s.found = static_cast<int32_t>(i);
-        __syncthreads();
-        if (rank < all) break;
-        rank -= all;
-      }
-      return {mass, s.found};
+      const uint64_t w = weigh<true>(r, float_of(low)).mass;
+      const uint64_t rank = by_count ? target - base_count - 1 : (target - base_mass - 1) / w;
+      return {base_mass + (rank + 1) * w, nth_of_key(s, x, vocab, low, rank)};
     }
     if (threadIdx.x == 0) s.listed = 0;
     __syncthreads();
     collect();
     listed = s.listed;
   }
+  rank_list<true>(s, listed);
   if (threadIdx.x < listed) {
-    const uint32_t key = s.list_key[threadIdx.x];
-    const int32_t index = s.list_index[threadIdx.x];
-    uint64_t mass = base_mass, count = base_count;
-    for (uint32_t j = 0; j < listed; ++j) {
-      const uint32_t other = s.list_key[j];
-      if (other > key || (other == key && s.list_index[j] < index)) {
-        mass += s.list_mass[j];
-        ++count;
-      }
-    }
-    const uint64_t upto = mass + s.list_mass[threadIdx.x];
-    if (by_count ? count + 1 == target : mass < target && target <= upto) {
-      s.found = index;
+    const uint64_t before = base_mass + s.before[threadIdx.x];
+    const uint64_t upto = before + s.list_mass[threadIdx.x];
+    if (by_count ? base_count + s.rank[threadIdx.x] + 1 == target : before < target && target <= upto) {
+      s.found = static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(s.list[threadIdx.x]));
       s.found_mass = upto;
     }
   }
@@ -346,25 +391,16 @@ __device__ __forceinline__ uint64_t place_of(float u, uint64_t mass) {
   return at < mass ? at + 1 : mass;
 }
 
-// The whole row's answer from the `listed` <= kList tokens of its list, which hold every token that the
-// cuts can keep: one token per thread, put in order by counting, then summed up along the order.
+// The whole row's answer from the `listed` <= kFew tokens of its list, which hold every token that the
+// cuts can keep: put in order by counting, then summed up along the order, a token per thread.
 __device__ __forceinline__ int32_t from_list(Shared& s, const Row& r, uint32_t listed, int32_t top_k, float top_p, float u) {
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-  const bool mine = threadIdx.x < listed;
-  if (mine) {
-    const uint32_t key = s.list_key[threadIdx.x];
-    const int32_t index = s.list_index[threadIdx.x];
-    uint32_t rank = 0;
-    for (uint32_t j = 0; j < listed; ++j) {
-      const uint32_t other = s.list_key[j];
-      rank += other > key || (other == key && s.list_index[j] < index);
-    }
-    s.order_mass[rank] = weight_of(r, float_of(key));
-    s.order_index[rank] = index;
-  }
+  rank_list<false>(s, listed);
+  if (threadIdx.x < listed) s.before[s.rank[threadIdx.x]] = s.list[threadIdx.x];
   __syncthreads();
-  const bool kept = mine && (top_k <= 0 || threadIdx.x < static_cast<uint32_t>(top_k));
-  const uint64_t own = kept ? s.order_mass[threadIdx.x] : 0;
+  const bool kept = threadIdx.x < listed && (top_k <= 0 || threadIdx.x < static_cast<uint32_t>(top_k));
+  const uint64_t token = kept ? s.before[threadIdx.x] : 0;
+  const uint64_t own = kept ? weigh<true>(r, float_of(static_cast<uint32_t>(token >> 32))).mass : 0;
   uint64_t upto = own;
   for (int d = 1; d < kWave; d <<= 1) {
     const uint64_t other = shfl_up64(upto, d);
@@ -384,9 +420,47 @@ __device__ __forceinline__ int32_t from_list(Shared& s, const Row& r, uint32_t l
     mass = s.found_mass;
   }
   const uint64_t target = place_of(u, mass);
-  if (own != 0 && upto - own < target && target <= upto) s.found = s.order_index[threadIdx.x];
+  if (own != 0 && upto - own < target && target <= upto) s.found = static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(token));
   __syncthreads();
   return s.found;
+}
+
+// The answer by a histogram of the masses (and counts) of the tokens from `floor` on.
+template <typename T>
+__device__ __forceinline__ int32_t from_bins(Shared& s, const Row& r, const T* x, int32_t vocab, float floor, int32_t top_k, float top_p,
+                                             float u) {
+  const bool counting = top_k > 0;
+  if (counting || r.least > 0.0) {
+    for_each<2>(x, vocab, [&](float v, int32_t) {
+      if (!(v >= floor)) return;
+      const Weight w = weigh<true>(r, v);
+      if (w.mass == 0) return;
+      atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[w.bin]), static_cast<unsigned long long>(w.mass));
+      if (counting) atomicAdd(&s.count[w.bin], 1u);
+    });
+  } else {
+    for_each<2>(x, vocab, [&](float v, int32_t) {
+      if (!(v >= floor)) return;
+      const Weight w = weigh<false>(r, v);
+      atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[w.bin]), static_cast<unsigned long long>(w.mass));
+    });
+  }
+  __syncthreads();
+  scan_bins(s, s.mass);
+  if (counting) scan_bins(s, s.count);
+
+  // Three times the same search: the end of top-k, of top-p, and the draw.
+  uint64_t mass = s.mass[kBins];
+  const bool cut = counting && s.count[kBins] > static_cast<uint32_t>(top_k);
+  int32_t token = 0;
+  for (int step = 0; step < 3; ++step) {
+    if ((step == 0 && !cut) || (step == 1 && top_p >= 1.f)) continue;
+    const uint64_t target = step == 0 ? static_cast<uint64_t>(top_k) : step == 1 ? nucleus(top_p, mass) : place_of(u, mass);
+    const Place place = locate(s, r, x, vocab, step == 0, target);
+    mass = place.mass;
+    token = place.index;
+  }
+  return token;
 }
 
 // One workgroup per row.
@@ -401,11 +475,10 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const Args a) {
   const float top_p = a.top_ps ? a.top_ps[row] : a.top_p;
   const float min_p = a.min_ps ? a.min_ps[row] : a.min_p;
   const float u = a.uniforms[row];
-  if (threadIdx.x < kPerOctave) s.power[threadIdx.x] = exp2(threadIdx.x * (1.0 / kPerOctave));
 
   float most = -INFINITY;
   bool odd = false;
-  for_each<4>(x, a.vocab, [&](float v, int32_t) {
+  for_each<8>(x, a.vocab, [&](float v, int32_t) {
     most = fmaxf(most, v);
     odd = odd || v != v;
   });
@@ -426,15 +499,24 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const Args a) {
     if (threadIdx.x == 0) a.out[row] = s.found;
     return;
   }
+  if (top == INFINITY) {  // equal weights for the tokens of +inf, nothing for others
+    uint64_t count = 0;
+    for_each<4>(x, a.vocab, [&](float v, int32_t) { count += v == top; });
+    count = block_sum(s, count);
+    if (top_k > 0) count = min(count, static_cast<uint64_t>(top_k));
+    if (!(top_p >= 1.f)) count = nucleus(top_p, count);
+    const int32_t token = nth_of_key(s, x, a.vocab, key_of(top), place_of(u, count) - 1);
+    if (threadIdx.x == 0) a.out[row] = token;
+    return;
+  }
 
   Row r;
   r.top = top;
-  r.rate = kPerOctave * 1.44269504088896340736 / static_cast<double>(temperature);
-  r.one = a.one;
+  r.rate = fmax(kPerOctave * 1.44269504088896340736 / static_cast<double>(temperature), 1e-300);  // T may be infinite
   r.least = min_p > 0.f ? fmin(static_cast<double>(min_p), 1.0) * a.one : 0.0;
   r.power = s.power;
-  const bool counting = top_k > 0;
-  for (int i = threadIdx.x; i <= kBins; i += kThreads) {
+  if (threadIdx.x < kPerOctave) s.power[threadIdx.x] = exp2(threadIdx.x * (1.0 / kPerOctave)) * a.one;
+  for (int i = threadIdx.x; i < kBins + 2; i += kThreads) {
     s.mass[i] = 0;
     s.count[i] = 0;
   }
@@ -446,14 +528,17 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const Args a) {
 
   // The bins that the kept tokens lie in, where the settings bound them beforehand: min-p by its weight;
   // top-k by the threads' largest tokens, of which there are top_k in the bins up to the pivot's.
+  const float lowest = floor_of_bin(r, kBins - 1);
   int32_t last = kBins - 1;
   if (min_p > 0.f) {
     const double deep = ceil(-log2(fmin(static_cast<double>(min_p), 1.0)) * kPerOctave) + 1.0;
     last = deep < last ? static_cast<int32_t>(deep) : last;
   }
-  if (counting && top_k <= kPivotTopK) {
-    const int32_t bin = bin_of_depth(depth_of(r, most));
-    if (bin < kBins) atomicAdd(&s.count[bin], 1u);
+  if (top_k > 0 && top_k <= kPivotTopK) {
+    if (most >= lowest) {
+      const int32_t bin = weigh<false>(r, most).bin;
+      if (bin < kBins) atomicAdd(&s.count[bin], 1u);
+    }
     __syncthreads();
     scan_bins(s, s.count);
 #pragma unroll
@@ -463,52 +548,25 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const Args a) {
     }
     __syncthreads();
     last = min(last, static_cast<int32_t>(s.bin));
-    for (int i = threadIdx.x; i <= kBins; i += kThreads) s.count[i] = 0;
+    for (int i = threadIdx.x; i < kBins + 2; i += kThreads) s.count[i] = 0;
   }
   const float floor = floor_of_bin(r, last);
-  if (last < kBins - 1 || a.vocab <= kList) {
-    for_each<4>(x, a.vocab, [&](float v, int32_t i) {
-      if (!(v >= floor) || bin_of_depth(depth_of(r, v)) > last) return;
+  if (last < kBins - 1 || a.vocab <= kFew) {
+    for_each<8>(x, a.vocab, [&](float v, int32_t i) {
+      if (!(v >= floor)) return;
       const uint32_t slot = atomicAdd(&s.listed, 1u);
-      if (slot < kList) {
-        s.list_key[slot] = key_of(v);
-        s.list_index[slot] = i;
-      }
+      if (slot < kFew) s.list[slot] = order_of(key_of(v), i);
     });
     __syncthreads();
     const uint32_t listed = s.listed;
-    if (listed <= kList) {
+    if (listed <= kFew) {
       const int32_t token = from_list(s, r, listed, top_k, top_p, u);
       if (threadIdx.x == 0) a.out[row] = token;
       return;
     }
   }
   __syncthreads();
-
-  for_each<2>(x, a.vocab, [&](float v, int32_t) {
-    if (!(v >= floor)) return;
-    const double z = depth_of(r, v);
-    const int32_t bin = bin_of_depth(z);
-    const uint64_t w = weight_of_depth(r, z, bin);
-    if (w == 0) return;
-    atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[bin]), static_cast<unsigned long long>(w));
-    if (counting) atomicAdd(&s.count[bin], 1u);
-  });
-  __syncthreads();
-  scan_bins(s, s.mass);
-  if (counting) scan_bins(s, s.count);
-
-  // Three times the same search: the end of top-k, of top-p, and the draw.
-  uint64_t mass = s.mass[kBins];
-  const bool cut = counting && s.count[kBins] > static_cast<uint32_t>(top_k);
-  int32_t token = 0;
-  for (int step = 0; step < 3; ++step) {
-    if ((step == 0 && !cut) || (step == 1 && top_p >= 1.f)) continue;
-    const uint64_t target = step == 0 ? static_cast<uint64_t>(top_k) : step == 1 ? nucleus(top_p, mass) : place_of(u, mass);
-    const Place place = locate(s, r, x, a.vocab, step == 0, target);
-    mass = place.mass;
-    token = place.index;
-  }
+  const int32_t token = from_bins(s, r, x, a.vocab, floor, top_k, top_p, u);
   if (threadIdx.x == 0) a.out[row] = token;
 }
 
