@@ -679,7 +679,6 @@ int pkv_window_attention(const pkv_window* args, int device, void* stream);
  *                 token; a min_p above 1 does too, one of 0 or below (or NaN) keeps all.
  * A token of -inf is never drawn; tokens of +inf share the whole mass. A row with a NaN, or with
  * nothing above -inf, yields its greedy token.
- *   workspace   : scratch of pkv_sample_workspace_bytes(...) bytes, 16-byte aligned (NULL when 0).
  */
 #define PKV_SAMPLE_BITS 46
 
@@ -694,17 +693,12 @@ typedef struct pkv_sample {
   const int32_t* top_ks;
   const float* top_ps;
   const float* min_ps;
-  void* workspace;
-  int64_t workspace_bytes;
   int32_t dtype;
   float temperature;
   int32_t top_k;
   float top_p;
   float min_p;
 } pkv_sample;
-
-/* Bytes of workspace pkv_sample_tokens needs. Host-only. */
-int64_t pkv_sample_workspace_bytes(int64_t num_rows, int64_t vocab_size);
 
 int pkv_sample_tokens(const pkv_sample* args, int device, void* stream);
 

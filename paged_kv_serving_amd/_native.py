@@ -99,7 +99,6 @@ EXPORTED_SYMBOLS = (
     "pkv_window_splits",
     "pkv_window_workspace_bytes",
     "pkv_window_attention",
-    "pkv_sample_workspace_bytes",
     "pkv_sample_tokens",
 )
 
@@ -192,7 +191,8 @@ _BOUND = False
 def bound_host():
     """:func:`host` with the library's entry points bound into it (``_pkvhost.bind``), so its
     ``plan``, ``paged_attention``, ``paged_attention_append``, ``copy_blocks``, ``rms_norm``,
-    ``silu_mul``, ``rope_append``, ``append``, ``forward`` and ``CopyQueue.flush`` call ``libpkv.so``
+    ``silu_mul``, ``rope_append``, ``append``, ``rope_append_axes``, ``window_workspace``,
+    ``window_attention``, ``sample_tokens``, ``forward`` and ``CopyQueue.flush`` call ``libpkv.so``
     directly, and ``stage``, ``forward``, ``CopyQueue.flush`` and ``event_create`` call the
     ``hipMemcpyAsync`` / ``hipGetDevice`` / ``hipSetDevice`` / ``hipEvent*`` functions of the HIP
     runtime ``libpkv.so`` is linked against (looked up through the library's handle, so they are
@@ -212,7 +212,10 @@ def bound_host():
                          address(lib.hipGetDevice), address(lib.hipSetDevice),
                          address(lib.hipEventCreateWithFlags), address(lib.hipEventRecord),
                          address(lib.hipEventSynchronize), address(lib.hipEventDestroy),
-                         address(lib.pkv_append), address(lib.pkv_linear_forward))  # fmt: skip
+                         address(lib.pkv_append), address(lib.pkv_linear_forward),
+                         address(lib.pkv_rope_append_axes), address(lib.pkv_window_splits),
+                         address(lib.pkv_window_workspace_bytes), address(lib.pkv_window_attention),
+                         address(lib.pkv_sample_tokens))  # fmt: skip
                 _BOUND = True
     return ext
 
@@ -224,46 +227,6 @@ _c_int = ctypes.c_int
 _i32 = ctypes.c_int32
 _i64 = ctypes.c_int64
 _ptr = ctypes.c_void_p
-
-
-class RopeAxesArgs(ctypes.Structure):
-    """``pkv_rope_axes`` (include/pkv.h)."""
-
-    _fields_ = [
-        ("rotated_queries", _ptr), ("queries", _ptr), ("keys", _ptr), ("values", _ptr),
-        ("rotated_token_stride", _i64), ("query_token_stride", _i64), ("key_token_stride", _i64),
-        ("value_token_stride", _i64), ("positions", _ptr), ("position_axis_stride", _i64),
-        ("cos_table", _ptr), ("sin_table", _ptr), ("table_rows", _i64), ("key_pool", _ptr),
-        ("value_pool", _ptr), ("num_slots", _i64), ("slot_mapping", _ptr), ("num_tokens", _i64),
-        ("io_dtype", _i32), ("pool_dtype", _i32), ("num_heads", _i32), ("num_kv_heads", _i32),
-        ("head_dim", _i32), ("rotary_dim", _i32), ("num_axes", _i32), ("interleaved", _i32),
-        ("sections", _i32 * 4),
-    ]  # fmt: skip
-
-
-class WindowArgs(ctypes.Structure):
-    """``pkv_window`` (include/pkv.h)."""
-
-    _fields_ = [
-        ("out", _ptr), ("queries", _ptr), ("query_token_stride", _i64), ("query_positions", _ptr),
-        ("query_seq", _ptr), ("num_queries", _i64), ("key_cache", _ptr), ("value_cache", _ptr),
-        ("num_blocks", _i64), ("block_tables", _ptr), ("context_lens", _ptr), ("workspace", _ptr),
-        ("workspace_bytes", _i64), ("q_dtype", _i32), ("kv_dtype", _i32), ("block_size", _i32),
-        ("block_table_stride", _i32), ("num_seqs", _i32), ("num_heads", _i32), ("num_kv_heads", _i32),
-        ("head_dim", _i32), ("window", _i32), ("sinks", _i32), ("max_context_len", _i32),
-        ("max_query_len", _i32), ("num_splits", _i32), ("scale", ctypes.c_float),
-    ]  # fmt: skip
-
-
-class SampleArgs(ctypes.Structure):
-    """``pkv_sample`` (include/pkv.h)."""
-
-    _fields_ = [
-        ("token_ids", _ptr), ("logits", _ptr), ("row_stride", _i64), ("num_rows", _i64), ("vocab_size", _i64),
-        ("uniforms", _ptr), ("temperatures", _ptr), ("top_ks", _ptr), ("top_ps", _ptr), ("min_ps", _ptr),
-        ("workspace", _ptr), ("workspace_bytes", _i64), ("dtype", _i32), ("temperature", ctypes.c_float),
-        ("top_k", _i32), ("top_p", ctypes.c_float), ("min_p", ctypes.c_float),
-    ]  # fmt: skip
 
 
 def _declare(lib: ctypes.CDLL) -> None:
@@ -373,7 +336,7 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.pkv_sequence_metadata.restype = _c_int
     lib.pkv_linear_forward.argtypes = [_ptr, _c_int, _ptr]  # args, device, stream
     lib.pkv_linear_forward.restype = _c_int
-    lib.pkv_rope_append_axes.argtypes = [ctypes.POINTER(RopeAxesArgs), _c_int, _ptr]  # args, device, stream
+    lib.pkv_rope_append_axes.argtypes = [_ptr, _c_int, _ptr]  # args, device, stream
     lib.pkv_rope_append_axes.restype = _c_int
     lib.pkv_window_splits.argtypes = [
         _i64, _i32, _i32, _i32, _i32, _i32, _i32,  # queries, heads, kv heads, window, sinks, max context, max query len
@@ -381,11 +344,9 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.pkv_window_splits.restype = _i32
     lib.pkv_window_workspace_bytes.argtypes = [_i64, _i32, _i32, _i32, _i32]  # queries, heads, head_dim, max query len, splits
     lib.pkv_window_workspace_bytes.restype = _i64
-    lib.pkv_window_attention.argtypes = [ctypes.POINTER(WindowArgs), _c_int, _ptr]  # args, device, stream
+    lib.pkv_window_attention.argtypes = [_ptr, _c_int, _ptr]  # args, device, stream
     lib.pkv_window_attention.restype = _c_int
-    lib.pkv_sample_workspace_bytes.argtypes = [_i64, _i64]  # rows, vocab
-    lib.pkv_sample_workspace_bytes.restype = _i64
-    lib.pkv_sample_tokens.argtypes = [ctypes.POINTER(SampleArgs), _c_int, _ptr]  # args, device, stream
+    lib.pkv_sample_tokens.argtypes = [_ptr, _c_int, _ptr]  # args, device, stream
     lib.pkv_sample_tokens.restype = _c_int
 
 

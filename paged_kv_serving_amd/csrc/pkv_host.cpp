@@ -58,7 +58,8 @@
 //       tens of thousands of blocks); it is left all zero.
 //   bind(plan_batch, paged_attention, paged_attention_append, copy_blocks, rms_norm, silu_mul,
 //        rope_append, memcpy_async[, gather_rows, greedy_tokens, get_device, set_device,
-//        event_create, event_record, event_synchronize, event_destroy, append, linear_forward])
+//        event_create, event_record, event_synchronize, event_destroy, append, linear_forward,
+//        rope_append_axes, window_splits, window_workspace_bytes, window_attention, sample_tokens])
 //       Takes the addresses of those libpkv.so entry points (include/pkv.h), so the calls below
 //       reach the library without ctypes' per-argument conversions, and of hipMemcpyAsync,
 //       hipGetDevice, hipSetDevice and hipEventCreateWithFlags / Record / Synchronize / Destroy
@@ -90,9 +91,14 @@
 //        kv_dtype, partition_size, min_tile_rows, rows, tiles, merge, counts, launch) -> int
 //       pkv_plan_batch on NumPy buffers; returns its PKV_* code.
 //   paged_attention(...), paged_attention_append(...), copy_blocks(...), rms_norm(...),
-//   silu_mul(...), rope_append(...), append(...) -> int
+//   silu_mul(...), rope_append(...), append(...), rope_append_axes(...), window_attention(...),
+//   sample_tokens(...) -> int
 //       The entry points of the same names, with every pointer, stream and handle passed as a
-//       Python int (0 for NULL) in the order of their C declarations; returns the PKV_* code.
+//       Python int (0 for NULL) in the order of their C declarations (the last three: of the
+//       fields of their argument structs, then device and stream); returns the PKV_* code.
+//   window_workspace(queries, heads, kv_heads, head_dim, window, sinks, max_context_len,
+//        max_query_len, splits) -> (splits, bytes)
+//       pkv_window_splits where `splits` is 0, and pkv_window_workspace_bytes.
 //
 // Buffers are NumPy arrays passed through the buffer protocol (C-contiguous, of the stated
 // element type; writable where written); nothing here allocates Python-visible memory besides
@@ -838,6 +844,11 @@ decltype(&pkv_append) g_append = nullptr;
 decltype(&pkv_gather_rows) g_gather_rows = nullptr;
 decltype(&pkv_linear_forward) g_linear = nullptr;  // optional: null takes the library products
 decltype(&pkv_greedy_tokens) g_greedy_tokens = nullptr;
+decltype(&pkv_rope_append_axes) g_rope_axes = nullptr;
+decltype(&pkv_window_splits) g_window_splits = nullptr;
+decltype(&pkv_window_workspace_bytes) g_window_bytes = nullptr;
+decltype(&pkv_window_attention) g_window = nullptr;
+decltype(&pkv_sample_tokens) g_sample = nullptr;
 // hipGetDevice / hipSetDevice of the same runtime, by their C signatures.
 using GetDeviceFn = int (*)(int* device);
 using SetDeviceFn = int (*)(int device);
@@ -894,9 +905,11 @@ PyObject* bind(PyObject*, PyObject* args) {
   unsigned long long plan, attention, attention_append, copy, norm, gate, rope, memcpy_async;
   unsigned long long gather_rows = 0, greedy = 0, get_device = 0, set_device = 0;
   unsigned long long event_create = 0, event_record = 0, event_synchronize = 0, event_destroy = 0, append = 0, linear = 0;
-  if (!PyArg_ParseTuple(args, "KKKKKKKK|KKKKKKKKKK", &plan, &attention, &attention_append, &copy, &norm, &gate, &rope,
+  unsigned long long rope_axes = 0, window_splits = 0, window_bytes = 0, window = 0, sample = 0;
+  if (!PyArg_ParseTuple(args, "KKKKKKKK|KKKKKKKKKKKKKKK", &plan, &attention, &attention_append, &copy, &norm, &gate, &rope,
                         &memcpy_async, &gather_rows, &greedy, &get_device, &set_device, &event_create,
-                        &event_record, &event_synchronize, &event_destroy, &append, &linear)) {
+                        &event_record, &event_synchronize, &event_destroy, &append, &linear, &rope_axes, &window_splits,
+                        &window_bytes, &window, &sample)) {
     return nullptr;
   }
   if (plan == 0 || attention == 0 || attention_append == 0 || copy == 0 || norm == 0 || gate == 0 || rope == 0 ||
@@ -923,6 +936,11 @@ PyObject* bind(PyObject*, PyObject* args) {
   g_event_destroy = reinterpret_cast<EventFn>(static_cast<uintptr_t>(event_destroy));
   g_append = reinterpret_cast<decltype(g_append)>(static_cast<uintptr_t>(append));
   g_linear = reinterpret_cast<decltype(g_linear)>(static_cast<uintptr_t>(linear));
+  g_rope_axes = reinterpret_cast<decltype(g_rope_axes)>(static_cast<uintptr_t>(rope_axes));
+  g_window_splits = reinterpret_cast<decltype(g_window_splits)>(static_cast<uintptr_t>(window_splits));
+  g_window_bytes = reinterpret_cast<decltype(g_window_bytes)>(static_cast<uintptr_t>(window_bytes));
+  g_window = reinterpret_cast<decltype(g_window)>(static_cast<uintptr_t>(window));
+  g_sample = reinterpret_cast<decltype(g_sample)>(static_cast<uintptr_t>(sample));
   Py_RETURN_NONE;
 }
 
@@ -1379,6 +1397,110 @@ PyObject* silu_mul(PyObject*, PyObject* args) {
   return PyLong_FromLong(rc);
 }
 
+// Positional arguments, read in order. `ok` turns false, with the exception set, at the first that is not
+// a number of its kind (or too few or many are given).
+struct Reader {
+  PyObject* const* args;
+  Py_ssize_t count;
+  Py_ssize_t at = 0;
+  bool ok = true;
+
+  PyObject* next() {
+    if (ok && at < count) return args[at++];
+    ok = false;
+    return nullptr;
+  }
+  template <typename T>
+  void operator()(T*& out) {
+    PyObject* o = next();
+    if (o == nullptr) return;
+    out = ptr<T>(PyLong_AsUnsignedLongLong(o));
+    if (PyErr_Occurred()) ok = false;
+  }
+  void operator()(int64_t& out) {
+    PyObject* o = next();
+    if (o == nullptr) return;
+    out = PyLong_AsLongLong(o);
+    if (out == -1 && PyErr_Occurred()) ok = false;
+  }
+  void operator()(int32_t& out) {
+    int64_t wide = 0;
+    (*this)(wide);
+    if (!ok) return;
+    out = static_cast<int32_t>(wide);
+    if (out != wide) {
+      PyErr_SetString(PyExc_OverflowError, "an argument does not fit 32 bits");
+      ok = false;
+    }
+  }
+  void operator()(float& out) {
+    PyObject* o = next();
+    if (o == nullptr) return;
+    const double wide = PyFloat_AsDouble(o);
+    if (wide == -1.0 && PyErr_Occurred()) ok = false;
+    out = static_cast<float>(wide);
+  }
+  bool done() {
+    if (ok && at == count) return true;
+    if (!PyErr_Occurred()) PyErr_SetString(PyExc_TypeError, "wrong number of arguments");
+    return false;
+  }
+};
+
+PyObject* rope_append_axes(PyObject*, PyObject* const* args, Py_ssize_t count) {
+  pkv_rope_axes a{};
+  int32_t device = 0;
+  void* stream = nullptr;
+  Reader r{args, count};
+  r(a.rotated_queries), r(a.queries), r(a.keys), r(a.values);
+  r(a.rotated_token_stride), r(a.query_token_stride), r(a.key_token_stride), r(a.value_token_stride);
+  r(a.positions), r(a.position_axis_stride), r(a.cos_table), r(a.sin_table), r(a.table_rows), r(a.key_pool), r(a.value_pool);
+  r(a.num_slots), r(a.slot_mapping), r(a.num_tokens), r(a.io_dtype), r(a.pool_dtype), r(a.num_heads), r(a.num_kv_heads);
+  r(a.head_dim), r(a.rotary_dim), r(a.num_axes), r(a.interleaved);
+  for (int32_t& n : a.sections) r(n);
+  r(device), r(stream);
+  if (!r.done() || !bound(reinterpret_cast<const void*>(g_rope_axes))) return nullptr;
+  return PyLong_FromLong(g_rope_axes(&a, device, stream));
+}
+
+PyObject* window_workspace(PyObject*, PyObject* const* args, Py_ssize_t count) {
+  int64_t queries = 0;
+  int32_t heads = 0, kv_heads = 0, dim = 0, window = 0, sinks = 0, context = 0, rows = 0, splits = 0;
+  Reader r{args, count};
+  r(queries), r(heads), r(kv_heads), r(dim), r(window), r(sinks), r(context), r(rows), r(splits);
+  if (!r.done() || !bound(reinterpret_cast<const void*>(g_window_splits)) || !bound(reinterpret_cast<const void*>(g_window_bytes))) {
+    return nullptr;
+  }
+  if (splits == 0) splits = g_window_splits(queries, heads, kv_heads, window, sinks, context, rows);
+  return Py_BuildValue("iL", splits, static_cast<long long>(g_window_bytes(queries, heads, dim, rows, splits)));
+}
+
+PyObject* window_attention(PyObject*, PyObject* const* args, Py_ssize_t count) {
+  pkv_window a{};
+  int32_t device = 0;
+  void* stream = nullptr;
+  Reader r{args, count};
+  r(a.out), r(a.queries), r(a.query_token_stride), r(a.query_positions), r(a.query_seq), r(a.num_queries), r(a.key_cache);
+  r(a.value_cache), r(a.num_blocks), r(a.block_tables), r(a.context_lens), r(a.workspace), r(a.workspace_bytes);
+  r(a.q_dtype), r(a.kv_dtype), r(a.block_size), r(a.block_table_stride), r(a.num_seqs), r(a.num_heads), r(a.num_kv_heads);
+  r(a.head_dim), r(a.window), r(a.sinks), r(a.max_context_len), r(a.max_query_len), r(a.num_splits), r(a.scale);
+  r(device), r(stream);
+  if (!r.done() || !bound(reinterpret_cast<const void*>(g_window))) return nullptr;
+  return PyLong_FromLong(g_window(&a, device, stream));
+}
+
+PyObject* sample_tokens(PyObject*, PyObject* const* args, Py_ssize_t count) {
+  pkv_sample a{};
+  int32_t device = 0;
+  void* stream = nullptr;
+  Reader r{args, count};
+  r(a.token_ids), r(a.logits), r(a.row_stride), r(a.num_rows), r(a.vocab_size), r(a.uniforms), r(a.temperatures), r(a.top_ks);
+  r(a.top_ps), r(a.min_ps), r(a.dtype), r(a.temperature), r(a.top_k), r(a.top_p), r(a.min_p);
+  r(device), r(stream);
+  if (!r.done() || !bound(reinterpret_cast<const void*>(g_sample))) return nullptr;
+  return PyLong_FromLong(g_sample(&a, device, stream));
+}
+
 PyObject* append(PyObject*, PyObject* args) {
   unsigned long long kp, vp, k, v, slots, stream;
   long long nslots, k_stride, v_stride, tokens;
@@ -1740,6 +1862,14 @@ PyMethodDef kMethods[] = {
     {"silu_mul", silu_mul, METH_VARARGS, "pkv_silu_mul with integer pointers."},
     {"rope_append", rope_append, METH_VARARGS, "pkv_rope_append with integer pointers."},
     {"append", append, METH_VARARGS, "pkv_append with integer pointers."},
+    {"rope_append_axes", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(rope_append_axes)), METH_FASTCALL,
+     "pkv_rope_append_axes with integer pointers."},
+    {"window_workspace", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(window_workspace)), METH_FASTCALL,
+     "The splits and the workspace bytes of a windowed attention call."},
+    {"window_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(window_attention)), METH_FASTCALL,
+     "pkv_window_attention with integer pointers."},
+    {"sample_tokens", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(sample_tokens)), METH_FASTCALL,
+     "pkv_sample_tokens with integer pointers."},
     {"stage", stage, METH_VARARGS, "Pack a call's metadata into pinned memory and copy it to the device."},
     {"forward", forward, METH_VARARGS, "One iteration's forward pass: rocBLAS products and the library's kernels."},
     {"event_create", event_create, METH_VARARGS, "A timing-free HIP event on a device, as an integer handle."},

@@ -573,11 +573,6 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const Args a) {
 }  // namespace
 }  // namespace pkv
 
-extern "C" int64_t pkv_sample_workspace_bytes(int64_t num_rows, int64_t vocab_size) {
-  if (num_rows < 0 || vocab_size < 1) return PKV_EINVAL;
-  return 0;
-}
-
 extern "C" int pkv_sample_tokens(const pkv_sample* args, int device, void* stream) {
   using namespace pkv;
   if (!args) return PKV_EINVAL;

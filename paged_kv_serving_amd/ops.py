@@ -8,7 +8,6 @@ the tensors' device). Nothing here computes on the CPU: a missing library raises
 
 from __future__ import annotations
 
-import ctypes
 from dataclasses import dataclass
 
 import numpy as np
@@ -54,6 +53,7 @@ TILE_ROWS = 64
 #: row-streaming pass reads a sequence's keys once per row, the tile pass once per 64 rows.
 MIN_TILE_ROWS = 8
 
+_INT32_MAX = 0x7FFFFFFF
 _DTYPE_CODES = {torch.float32: _native.PKV_F32, torch.bfloat16: _native.PKV_BF16}
 
 
@@ -79,6 +79,18 @@ def _stream(device: int) -> int:
     """The raw handle of ``device``'s current stream (torch's own accessor, without building a
     Stream object)."""
     return torch._C._cuda_getCurrentRawStream(device)
+
+
+_HOST = None
+
+
+def _host():
+    """The host extension with the library's entry points bound into it (``_native.bound_host``),
+    without looking for its file at every call."""
+    global _HOST
+    if _HOST is None or not _native._BOUND:
+        _HOST = _native.bound_host()
+    return _HOST
 
 
 def _rows_contiguous(tensor: torch.Tensor, name: str) -> int:
@@ -288,14 +300,13 @@ def rope_append_axes(
     out_stride = _rows_contiguous(out, "out")
     if tokens == 0:
         return out
-    args = _native.RopeAxesArgs(
+    rc = _host().rope_append_axes(
         out.data_ptr(), queries.data_ptr(), keys.data_ptr(), values.data_ptr(), out_stride, q_stride, k_stride,
         v_stride, positions.data_ptr(), axis_stride, cos_table.data_ptr(), sin_table.data_ptr(), cos_table.shape[0],
         key_pool.data_ptr(), value_pool.data_ptr(), key_pool.numel() // (kv_heads * dim), slot_mapping.data_ptr(),
         tokens, io_code, kv_dtype_code(key_pool.dtype), heads, kv_heads, dim, 2 * half, len(sections),
-        int(interleaved), (ctypes.c_int32 * MAX_ROPE_AXES)(*sections),
+        1 if interleaved else 0, *sections, *(0,) * (MAX_ROPE_AXES - len(sections)), device, _stream(device),
     )  # fmt: skip
-    rc = _native.library().pkv_rope_append_axes(args, device, _stream(device))
     _native.check(rc, "pkv_rope_append_axes")
     return out
 
@@ -390,9 +401,9 @@ def greedy_tokens(logits: torch.Tensor, out: torch.Tensor | None = None) -> torc
 
 
 def _row_setting(value, name: str, rows: int, dtype: torch.dtype, logits: torch.Tensor):
-    """``(pointer or None, scalar)`` of a sampling setting: one number, or one for each row."""
+    """``(address or 0, scalar)`` of a sampling setting: one number, or one for each row."""
     if not isinstance(value, torch.Tensor):
-        return None, value
+        return 0, value
     if value.dtype != dtype or value.shape != (rows,) or not value.is_contiguous() or value.device != logits.device:
         raise ValueError(f"{name} must be a number or contiguous {str(dtype)[6:]} with one entry per row")
     return value.data_ptr(), 0
@@ -434,13 +445,13 @@ def sample_tokens(
     top_ks, top_k = _row_setting(top_k, "top_k", rows, torch.int32, logits)
     top_ps, top_p = _row_setting(top_p, "top_p", rows, torch.float32, logits)
     min_ps, min_p = _row_setting(min_p, "min_p", rows, torch.float32, logits)
-    if temperatures is None and not temperature >= 0:
+    if not temperatures and not temperature >= 0:
         raise ValueError("temperature must be >= 0")
-    if top_ks is None and top_k < 0:
+    if not top_ks and top_k < 0:
         raise ValueError("top_k must be >= 0")
-    if top_ps is None and not 0 < top_p <= 1:
+    if not top_ps and not 0 < top_p <= 1:
         raise ValueError("top_p must be in (0, 1]")
-    if min_ps is None and not 0 <= min_p <= 1:
+    if not min_ps and not 0 <= min_p <= 1:
         raise ValueError("min_p must be in [0, 1]")
     if vocab > 1 and logits.stride(1) != 1:
         logits = logits.contiguous()
@@ -450,15 +461,11 @@ def sample_tokens(
         raise ValueError("out must be a contiguous int32 tensor with one entry per row")
     if rows == 0:
         return out
-    lib = _native.library()
-    need = lib.pkv_sample_workspace_bytes(rows, vocab)
-    workspace = torch.empty(need, dtype=torch.uint8, device=logits.device) if need else None
-    args = _native.SampleArgs(
+    rc = _host().sample_tokens(
         out.data_ptr(), logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, rows, vocab, uniforms.data_ptr(),
-        temperatures, top_ks, top_ps, min_ps, workspace.data_ptr() if need else None, need,
-        _DTYPE_CODES[logits.dtype], temperature, min(top_k, 0x7FFFFFFF), top_p, min_p,
+        temperatures, top_ks, top_ps, min_ps, _DTYPE_CODES[logits.dtype], temperature, min(top_k, _INT32_MAX),
+        top_p, min_p, device, _stream(device),
     )  # fmt: skip
-    rc = lib.pkv_sample_tokens(args, device, _stream(device))
     _native.check(rc, "pkv_sample_tokens")
     return out
 
@@ -1410,9 +1417,6 @@ def paged_attention_ragged(
 MAX_WINDOW_GROUP = 64
 #: Workgroups that can share a row's keys in :func:`paged_attention_window`.
 MAX_WINDOW_SPLITS = 64
-_INT32_MAX = 0x7FFFFFFF
-
-
 def paged_attention_window(
     queries: torch.Tensor,
     query_positions: torch.Tensor,
@@ -1493,9 +1497,8 @@ def paged_attention_window(
         return out
     window, sinks = min(window, _INT32_MAX), min(sinks, _INT32_MAX)
     rows = num_queries if max_query_len is None else min(max_query_len, _INT32_MAX)
-    lib = _native.library()
-    splits = num_splits or lib.pkv_window_splits(num_queries, heads, kv_heads, window, sinks, max_context_len, rows)
-    need = lib.pkv_window_workspace_bytes(num_queries, heads, dim, rows, splits)
+    host = _host()
+    splits, need = host.window_workspace(num_queries, heads, kv_heads, dim, window, sinks, max_context_len, rows, num_splits)
     if need:
         if workspace is None:
             workspace = torch.empty(need // 4, dtype=torch.float32, device=queries.device)
@@ -1503,13 +1506,12 @@ def paged_attention_window(
             raise ValueError("workspace must be contiguous and on the queries' device")
         elif workspace.numel() * workspace.element_size() < need:
             raise ValueError(f"workspace must hold {need} bytes")
-    args = _native.WindowArgs(
+    rc = host.window_attention(
         out.data_ptr(), queries.data_ptr(), stride, query_positions.data_ptr(), query_seq.data_ptr(), num_queries,
         key_cache.data_ptr(), value_cache.data_ptr(), num_blocks, block_tables.data_ptr(), context_lens.data_ptr(),
-        workspace.data_ptr() if need else None, need, q_code, kv_code, block_size, block_tables.shape[1], num_seqs,
-        heads, kv_heads, dim, window, sinks, max_context_len, rows, splits, float(scale),
+        workspace.data_ptr() if need else 0, need, q_code, kv_code, block_size, block_tables.shape[1], num_seqs,
+        heads, kv_heads, dim, window, sinks, max_context_len, rows, splits, scale, device, _stream(device),
     )  # fmt: skip
-    rc = lib.pkv_window_attention(args, device, _stream(device))
     _native.check(rc, "pkv_window_attention")
     return out
 
@@ -1519,12 +1521,11 @@ def window_workspace_bytes(
     max_context_len: int, max_query_len: int | None = None, num_splits: int = 0,
 ) -> int:  # fmt: skip
     """Bytes of float32 workspace :func:`paged_attention_window` needs for these sizes."""
-    lib = _native.library()
     rows = num_queries if max_query_len is None else max_query_len
-    splits = num_splits or lib.pkv_window_splits(
-        num_queries, heads, kv_heads, min(window, _INT32_MAX), min(sinks, _INT32_MAX), max_context_len, min(rows, _INT32_MAX)
-    )
-    need = lib.pkv_window_workspace_bytes(num_queries, heads, head_dim, min(rows, _INT32_MAX), splits)
+    splits, need = _host().window_workspace(
+        num_queries, heads, kv_heads, head_dim, min(window, _INT32_MAX), min(sinks, _INT32_MAX), max_context_len,
+        min(rows, _INT32_MAX), num_splits,
+    )  # fmt: skip
     if splits < 1 or need < 0:
         raise ValueError("invalid window workspace query")
     return int(need)
