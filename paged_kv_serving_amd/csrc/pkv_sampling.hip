@@ -24,7 +24,8 @@ constexpr int kBins = 48 * kPerOctave;             // 2^-47.5 * 2^46 < 1/2: late
 constexpr int kBinsPerThread = kBins / kThreads;
 constexpr int kList = 1024;                        // tokens of one bin that are compared with each other
 constexpr int kFew = 512;                          // tokens that are put in order instead of counted in bins
-constexpr int kPivotTopK = 512;                    // up to here top-k rows are listed
+constexpr int kCrowded = 960;                      // threads (of kThreads) that meet a token that the cuts may keep
+constexpr int kKept = 4096;                        // tokens that are kept in LDS instead of read again
 
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 
@@ -94,18 +95,42 @@ __device__ __forceinline__ void for_each(const T* x, int32_t n, F f) {
   }
 }
 
+// Where a row's tokens come from: the row, or (kept >= 0) the tokens kept in LDS.
+template <typename T>
+struct Source {
+  const T* x;
+  int32_t vocab;
+  const uint64_t* list;
+  int32_t kept;
+
+  template <int kLoads, typename F>
+  __device__ __forceinline__ void each(F f) const {
+    if (kept < 0) {
+      for_each<kLoads>(x, vocab, f);
+      return;
+    }
+#pragma unroll 1
+    for (int32_t i = threadIdx.x; i < kept; i += kThreads) {
+      const uint64_t token = list[i];
+      f(float_of(static_cast<uint32_t>(token >> 32)), static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(token)));
+    }
+  }
+};
+
 struct Shared {
+  __align__(16) uint64_t kept[kKept];       // tokens as order_of gives them: all that the cuts can keep
   uint64_t mass[kBins + 2];   // exclusive sums over the bins before, once summed up
   uint32_t count[kBins + 2];
-  __align__(16) uint64_t list[kList];       // tokens as order_of gives them
+  __align__(16) uint64_t list[kList];       // and those that are compared with each other
   __align__(16) uint64_t list_mass[kList];
   uint64_t before[kList];     // of each token of the list: the mass, and the number, that come before it
   uint32_t rank[kList];
   double power[kPerOctave];   // 2^(j / kPerOctave) * 2^(fractional bits)
-  uint64_t sum[kWaves];
-  uint32_t waves[kWaves];
-  uint64_t base_mass, found_mass;
-  uint32_t base_count, bin, listed;
+  __align__(16) uint64_t sum[kWaves];
+  __align__(16) float tops[kWaves];
+  __align__(16) uint32_t waves[kWaves];
+  uint64_t found_mass;
+  uint32_t listed;
   int32_t found;
 };
 
@@ -164,62 +189,107 @@ __device__ __forceinline__ uint64_t order_of(uint32_t key, int32_t index) {
   return (static_cast<uint64_t>(key) << 32) | (0xffffffffu - static_cast<uint32_t>(index));
 }
 
-__device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int mask) {
-  const uint32_t lo = __shfl_xor(static_cast<uint32_t>(v), mask);
-  const uint32_t hi = __shfl_xor(static_cast<uint32_t>(v >> 32), mask);
+// v of the lane that DPP control kCtrl names, where it has one within the rows of kRows, else 0.
+template <int kCtrl, int kRows>
+__device__ __forceinline__ uint64_t dpp64(uint64_t v) {
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(static_cast<uint32_t>(v)), kCtrl, kRows, 0xf, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(static_cast<uint32_t>(v >> 32)), kCtrl, kRows, 0xf, false);
   return (static_cast<uint64_t>(hi) << 32) | lo;
 }
 
-__device__ __forceinline__ uint64_t shfl_up64(uint64_t v, int delta) {
-  const uint32_t lo = __shfl_up(static_cast<uint32_t>(v), delta);
-  const uint32_t hi = __shfl_up(static_cast<uint32_t>(v >> 32), delta);
-  return (static_cast<uint64_t>(hi) << 32) | lo;
+// The inclusive sum over the wavefront's lanes before and this one: within rows of 16 lanes, then the
+// last lane of a row on to the next row, and of the second on to the third and fourth.
+__device__ __forceinline__ uint64_t wave_scan(uint64_t v) {
+  v += dpp64<0x111, 0xf>(v);
+  v += dpp64<0x112, 0xf>(v);
+  v += dpp64<0x114, 0xf>(v);
+  v += dpp64<0x118, 0xf>(v);
+  v += dpp64<0x142, 0xa>(v);
+  v += dpp64<0x143, 0xc>(v);
+  return v;
 }
 
-__device__ uint64_t block_sum(Shared& s, uint64_t v) {
-  for (int m = kWave / 2; m > 0; m >>= 1) v += shfl_xor64(v, m);
-  __syncthreads();
-  if ((threadIdx.x & (kWave - 1)) == 0) s.sum[threadIdx.x / kWave] = v;
-  __syncthreads();
-  uint64_t total = 0;
-  for (int w = 0; w < kWaves; ++w) total += s.sum[w];
-  return total;
+__device__ __forceinline__ void add64(uint64_t* to, uint64_t v) {
+  atomicAdd(reinterpret_cast<unsigned long long*>(to), static_cast<unsigned long long>(v));
 }
 
-// Replaces values[0 .. kBins) by their exclusive sums, values[kBins] by the total.
-template <typename V>
-__device__ void scan_bins(Shared& s, V* values) {
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+// The inclusive sum of v over the threads before and this one, and the sum over all.
+struct Scan {
+  uint64_t upto, all;
+};
+__device__ __forceinline__ Scan scan_threads(Shared& s, uint64_t v) {
+  const int wave = threadIdx.x / kWave;
+  Scan r{wave_scan(v), 0};
+  __syncthreads();
+  if ((threadIdx.x & (kWave - 1)) == kWave - 1) s.sum[wave] = r.upto;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    const uint64_t sum = s.sum[w];
+    r.upto += w < wave ? sum : 0;
+    r.all += sum;
+  }
+  return r;
+}
+
+__device__ __forceinline__ uint64_t block_sum(Shared& s, uint64_t v) { return scan_threads(s, v).all; }
+
+__device__ __forceinline__ float block_max(Shared& s, float v) {
+#pragma unroll
+  for (int m = kWave / 2; m > 0; m >>= 1) v = fmaxf(v, __shfl_xor(v, m));
+  __syncthreads();
+  if ((threadIdx.x & (kWave - 1)) == 0) s.tops[threadIdx.x / kWave] = v;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) v = fmaxf(v, s.tops[w]);
+  return v;
+}
+
+// Replaces values[0 .. kBins) by the exclusive sums of of(value, bin), values[kBins] by their total.
+template <typename V, typename F>
+__device__ __forceinline__ void scan_bins(Shared& s, V* values, F of) {
+  V* at = values + threadIdx.x * kBinsPerThread;
   V own[kBinsPerThread];
-  V sum = 0;
+  uint64_t sum = 0;
+#pragma unroll
+  for (int i = 0; i < kBinsPerThread; ++i) own[i] = at[i];
 #pragma unroll
   for (int i = 0; i < kBinsPerThread; ++i) {
-    own[i] = values[threadIdx.x * kBinsPerThread + i];
+    own[i] = of(own[i], threadIdx.x * kBinsPerThread + i);
     sum += own[i];
   }
-  uint64_t upto = sum;
-  for (int d = 1; d < kWave; d <<= 1) {
-    const uint64_t other = shfl_up64(upto, d);
-    if (lane >= d) upto += other;
-  }
-  __syncthreads();
-  if (lane == kWave - 1) s.sum[wave] = upto;
-  __syncthreads();
-  uint64_t before = upto - sum;
-  for (int w = 0; w < wave; ++w) before += s.sum[w];
+  const Scan scan = scan_threads(s, sum);
+  uint64_t before = scan.upto - sum;
 #pragma unroll
   for (int i = 0; i < kBinsPerThread; ++i) {
-    values[threadIdx.x * kBinsPerThread + i] = static_cast<V>(before);
+    at[i] = static_cast<V>(before);
     before += own[i];
   }
-  if (threadIdx.x == kThreads - 1) values[kBins] = static_cast<V>(before);
+  if (threadIdx.x == 0) values[kBins] = static_cast<V>(scan.all);
   __syncthreads();
 }
 
-// For each of the list's `listed` tokens how many tokens (kMass: what mass too) come before it in the
-// list: all pairs, the threads of a token sharing the others among them.
+// The bin b with sums[b] < target <= sums[b + 1]: there is one. Every wavefront looks for it, 64 places at a time.
+template <typename V>
+__device__ __forceinline__ int32_t bin_reaching(const V* sums, uint64_t target) {
+  constexpr int kFar = kBins / kWave, kNear = (kFar + kWave - 1) / kWave;
+  static_assert(kFar * kWave == kBins, "whole steps");
+  const int lane = threadIdx.x & (kWave - 1);
+  const int32_t far = (__popcll(__ballot(sums[lane * kFar] < target)) - 1) * kFar;
+  int32_t at = far;
+#pragma unroll
+  for (int i = kNear - 1; i >= 0; --i) {
+    const int32_t first = far + i * kWave, n = min(kWave, kFar - i * kWave);
+    const int below = __popcll(__ballot(lane < n && sums[first + min(lane, n - 1)] < target));
+    if (below > 0 && at == far) at = first + below - 1;
+  }
+  return __builtin_amdgcn_readfirstlane(at);
+}
+
+// For each of the `listed` tokens of `list` how many of them (kMass: what mass too) come before it:
+// all pairs, the threads of a token sharing the others among them.
 template <bool kMass>
-__device__ __forceinline__ void rank_list(Shared& s, uint32_t listed) {
+__device__ __forceinline__ void rank_list(Shared& s, const uint64_t* list, uint32_t listed) {
   uint32_t slots = kWave;
   while (slots < listed) slots *= 2;
   const uint32_t mine = threadIdx.x & (slots - 1), part = threadIdx.x / slots, parts = kThreads / slots;
@@ -230,7 +300,7 @@ __device__ __forceinline__ void rank_list(Shared& s, uint32_t listed) {
   }
   __syncthreads();
   if (mine < listed) {
-    const uint64_t own = s.list[mine];
+    const uint64_t own = list[mine];
     uint64_t mass = 0;
     uint32_t count = 0;
     const uint32_t end = min((part + 1) * each, listed);
@@ -238,7 +308,7 @@ __device__ __forceinline__ void rank_list(Shared& s, uint32_t listed) {
     for (; j + 4 <= end; j += 4) {
       uint64_t other[4], weight[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) other[e] = s.list[j + e];
+      for (int e = 0; e < 4; ++e) other[e] = list[j + e];
       if constexpr (kMass) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) weight[e] = s.list_mass[j + e];
@@ -250,8 +320,8 @@ __device__ __forceinline__ void rank_list(Shared& s, uint32_t listed) {
       }
     }
     for (; j < end; ++j) {
-      count += s.list[j] > own;
-      if constexpr (kMass) mass += s.list[j] > own ? s.list_mass[j] : 0;
+      count += list[j] > own;
+      if constexpr (kMass) mass += list[j] > own ? s.list_mass[j] : 0;
     }
     if (count) atomicAdd(&s.rank[mine], count);
     if constexpr (kMass) {
@@ -293,29 +363,18 @@ struct Place {
 // The first token of the order whose cumulative count (by_count) or mass reaches `target`, which
 // the row's totals reach. Every thread gets the answer.
 template <typename T>
-__device__ __forceinline__ Place locate(Shared& s, const Row& r, const T* x, int32_t vocab, bool by_count, uint64_t target) {
+__device__ __forceinline__ Place locate(Shared& s, const Row& r, const Source<T>& source, bool by_count, uint64_t target) {
   __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kBinsPerThread; ++i) {
-    const int b = threadIdx.x * kBinsPerThread + i;
-    const uint64_t lo = by_count ? s.count[b] : s.mass[b];
-    const uint64_t hi = by_count ? s.count[b + 1] : s.mass[b + 1];
-    if (lo < target && target <= hi) {
-      s.bin = b;
-      s.base_mass = s.mass[b];
-      s.base_count = s.count[b];
-    }
-  }
   if (threadIdx.x == 0) s.listed = 0;
   __syncthreads();
-  const int32_t bin = s.bin;
-  uint64_t base_mass = s.base_mass;
-  uint32_t base_count = s.base_count;
+  const int32_t bin = by_count ? bin_reaching(s.count, target) : bin_reaching(s.mass, target);
+  uint64_t base_mass = s.mass[bin];
+  uint32_t base_count = by_count ? s.count[bin] : 0;
   const float floor = floor_of_bin(r, bin), ceiling = ceiling_of_bin(r, bin);
   uint32_t low = 0, high = 0xffffffffu;  // keys still in question
   // f(value, index, key, weight) for the bin's tokens with keys of [from, to].
   auto tokens = [&](uint32_t from, uint32_t to, auto f) {
-    for_each<4>(x, vocab, [&](float v, int32_t i) {
+    source.template each<4>([&](float v, int32_t i) {
       if (!(v >= floor && v <= ceiling)) return;
       const Weight w = weigh<true>(r, v);
       const uint32_t key = key_of(v);
@@ -358,14 +417,14 @@ __device__ __forceinline__ Place locate(Shared& s, const Row& r, const T* x, int
     if (listed > kList) {  // equal logits: the one that far along their ids
       const uint64_t w = weigh<true>(r, float_of(low)).mass;
       const uint64_t rank = by_count ? target - base_count - 1 : (target - base_mass - 1) / w;
-      return {base_mass + (rank + 1) * w, nth_of_key(s, x, vocab, low, rank)};
+      return {base_mass + (rank + 1) * w, nth_of_key(s, source.x, source.vocab, low, rank)};
     }
     if (threadIdx.x == 0) s.listed = 0;
     __syncthreads();
     collect();
     listed = s.listed;
   }
-  rank_list<true>(s, listed);
+  rank_list<true>(s, s.list, listed);
   if (threadIdx.x < listed) {
     const uint64_t before = base_mass + s.before[threadIdx.x];
     const uint64_t upto = before + s.list_mass[threadIdx.x];
@@ -394,25 +453,15 @@ __device__ __forceinline__ uint64_t place_of(float u, uint64_t mass) {
 // The whole row's answer from the `listed` <= kFew tokens of its list, which hold every token that the
 // cuts can keep: put in order by counting, then summed up along the order, a token per thread.
 __device__ __forceinline__ int32_t from_list(Shared& s, const Row& r, uint32_t listed, int32_t top_k, float top_p, float u) {
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-  rank_list<false>(s, listed);
-  if (threadIdx.x < listed) s.before[s.rank[threadIdx.x]] = s.list[threadIdx.x];
+  rank_list<false>(s, s.kept, listed);
+  if (threadIdx.x < listed) s.before[s.rank[threadIdx.x]] = s.kept[threadIdx.x];
   __syncthreads();
   const bool kept = threadIdx.x < listed && (top_k <= 0 || threadIdx.x < static_cast<uint32_t>(top_k));
   const uint64_t token = kept ? s.before[threadIdx.x] : 0;
   const uint64_t own = kept ? weigh<true>(r, float_of(static_cast<uint32_t>(token >> 32))).mass : 0;
-  uint64_t upto = own;
-  for (int d = 1; d < kWave; d <<= 1) {
-    const uint64_t other = shfl_up64(upto, d);
-    if (lane >= d) upto += other;
-  }
-  if (lane == kWave - 1) s.sum[wave] = upto;
-  __syncthreads();
-  uint64_t mass = 0;
-  for (int w = 0; w < kWaves; ++w) {
-    upto += w < wave ? s.sum[w] : 0;
-    mass += s.sum[w];
-  }
+  const Scan scan = scan_threads(s, own);
+  const uint64_t upto = scan.upto;
+  uint64_t mass = scan.all;
   if (!(top_p >= 1.f)) {
     const uint64_t target = nucleus(top_p, mass);
     if (own != 0 && upto - own < target && target <= upto) s.found_mass = upto;
@@ -427,11 +476,11 @@ __device__ __forceinline__ int32_t from_list(Shared& s, const Row& r, uint32_t l
 
 // The answer by a histogram of the masses (and counts) of the tokens from `floor` on.
 template <typename T>
-__device__ __forceinline__ int32_t from_bins(Shared& s, const Row& r, const T* x, int32_t vocab, float floor, int32_t top_k, float top_p,
+__device__ __forceinline__ int32_t from_bins(Shared& s, const Row& r, const Source<T>& source, float floor, int32_t top_k, float top_p,
                                              float u) {
   const bool counting = top_k > 0;
   if (counting || r.least > 0.0) {
-    for_each<2>(x, vocab, [&](float v, int32_t) {
+    source.template each<2>([&](float v, int32_t) {
       if (!(v >= floor)) return;
       const Weight w = weigh<true>(r, v);
       if (w.mass == 0) return;
@@ -439,15 +488,15 @@ __device__ __forceinline__ int32_t from_bins(Shared& s, const Row& r, const T* x
       if (counting) atomicAdd(&s.count[w.bin], 1u);
     });
   } else {
-    for_each<2>(x, vocab, [&](float v, int32_t) {
+    source.template each<2>([&](float v, int32_t) {
       if (!(v >= floor)) return;
       const Weight w = weigh<false>(r, v);
       atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[w.bin]), static_cast<unsigned long long>(w.mass));
     });
   }
   __syncthreads();
-  scan_bins(s, s.mass);
-  if (counting) scan_bins(s, s.count);
+  scan_bins(s, s.mass, [](uint64_t mass, int) { return mass; });
+  if (counting) scan_bins(s, s.count, [](uint32_t count, int) { return count; });
 
   // Three times the same search: the end of top-k, of top-p, and the draw.
   uint64_t mass = s.mass[kBins];
@@ -456,7 +505,7 @@ __device__ __forceinline__ int32_t from_bins(Shared& s, const Row& r, const T* x
   for (int step = 0; step < 3; ++step) {
     if ((step == 0 && !cut) || (step == 1 && top_p >= 1.f)) continue;
     const uint64_t target = step == 0 ? static_cast<uint64_t>(top_k) : step == 1 ? nucleus(top_p, mass) : place_of(u, mass);
-    const Place place = locate(s, r, x, vocab, step == 0, target);
+    const Place place = locate(s, r, source, step == 0, target);
     mass = place.mass;
     token = place.index;
   }
@@ -469,7 +518,6 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const Args a) {
   __shared__ Shared s;
   const int64_t row = blockIdx.x;
   const T* x = static_cast<const T*>(a.logits) + row * a.row_stride;
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   const float temperature = a.temperatures ? a.temperatures[row] : a.temperature;
   const int32_t top_k = a.top_ks ? a.top_ks[row] : a.top_k;
   const float top_p = a.top_ps ? a.top_ps[row] : a.top_p;
@@ -482,11 +530,8 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const Args a) {
     most = fmaxf(most, v);
     odd = odd || v != v;
   });
-  float top = most;
-  for (int m = kWave / 2; m > 0; m >>= 1) top = fmaxf(top, __shfl_xor(top, m));
-  if (lane == 0) s.waves[wave] = __float_as_uint(top);
   const bool any_odd = __syncthreads_or(odd);
-  for (int w = 0; w < kWaves; ++w) top = fmaxf(top, __uint_as_float(s.waves[w]));
+  const float top = block_max(s, most);
   if (any_odd || top == -INFINITY || !(temperature > 0.f)) {  // the greedy token: the first NaN, else the first of the largest
     if (threadIdx.x == 0) s.found = a.vocab;
     __syncthreads();
@@ -520,10 +565,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const Args a) {
     s.mass[i] = 0;
     s.count[i] = 0;
   }
-  if (threadIdx.x == 0) {
-    s.listed = 0;
-    s.bin = kBins;
-  }
+  if (threadIdx.x == 0) s.listed = 0;
   __syncthreads();
 
   // The bins that the kept tokens lie in, where the settings bound them beforehand: min-p by its weight;
@@ -534,39 +576,39 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const Args a) {
     const double deep = ceil(-log2(fmin(static_cast<double>(min_p), 1.0)) * kPerOctave) + 1.0;
     last = deep < last ? static_cast<int32_t>(deep) : last;
   }
-  if (top_k > 0 && top_k <= kPivotTopK) {
+  if (top_k > 0 && top_k <= kThreads) {
     if (most >= lowest) {
       const int32_t bin = weigh<false>(r, most).bin;
       if (bin < kBins) atomicAdd(&s.count[bin], 1u);
     }
     __syncthreads();
-    scan_bins(s, s.count);
-#pragma unroll
-    for (int i = 0; i < kBinsPerThread; ++i) {
-      const int b = threadIdx.x * kBinsPerThread + i;
-      if (s.count[b] < static_cast<uint32_t>(top_k) && static_cast<uint32_t>(top_k) <= s.count[b + 1]) s.bin = b;
-    }
+    scan_bins(s, s.count, [](uint32_t count, int) { return count; });
+    if (s.count[kBins] >= static_cast<uint32_t>(top_k)) last = min(last, bin_reaching(s.count, top_k));
     __syncthreads();
-    last = min(last, static_cast<int32_t>(s.bin));
     for (int i = threadIdx.x; i < kBins + 2; i += kThreads) s.count[i] = 0;
   }
   const float floor = floor_of_bin(r, last);
-  if (last < kBins - 1 || a.vocab <= kFew) {
+  Source<T> source{x, a.vocab, s.kept, -1};
+  // Were m of the 1024 threads to meet a token from the floor on, some -1024 ln(1 - m / 1024) tokens lie there:
+  // 2840 for kCrowded threads, so that the list seldom overflows.
+  const int32_t meet = __syncthreads_count(most >= floor);
+  if (a.vocab <= kFew || (last < kBins - 1 && meet <= kCrowded)) {
     for_each<8>(x, a.vocab, [&](float v, int32_t i) {
       if (!(v >= floor)) return;
       const uint32_t slot = atomicAdd(&s.listed, 1u);
-      if (slot < kFew) s.list[slot] = order_of(key_of(v), i);
+      if (slot < kKept) s.kept[slot] = order_of(key_of(v), i);
     });
     __syncthreads();
-    const uint32_t listed = s.listed;
-    if (listed <= kFew) {
-      const int32_t token = from_list(s, r, listed, top_k, top_p, u);
+    const uint32_t kept = s.listed;
+    if (kept <= kFew) {
+      const int32_t token = from_list(s, r, kept, top_k, top_p, u);
       if (threadIdx.x == 0) a.out[row] = token;
       return;
     }
+    if (kept <= kKept) source.kept = kept;
   }
   __syncthreads();
-  const int32_t token = from_bins(s, r, x, a.vocab, floor, top_k, top_p, u);
+  const int32_t token = from_bins(s, r, source, floor, top_k, top_p, u);
   if (threadIdx.x == 0) a.out[row] = token;
 }
 
