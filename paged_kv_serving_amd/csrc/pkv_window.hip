@@ -250,7 +250,8 @@ __device__ __forceinline__ void exact_row(const Window& a, int64_t t, int32_t he
 //
 // So nothing is staged: every key and value row goes from the pool to the registers that multiply it,
 // in float32 throughout, and all heads of a group share one read of it. The loads of the next keys are
-// issued before the present ones are used.
+// issued before the present ones are used (a second set of registers for the values, so that they too
+// are a whole round ahead, measured 3 to 5% slower).
 // ---------------------------------------------------------------------------------------------
 template <typename QT, typename KVT, int D>
 struct RowShape {
@@ -324,22 +325,24 @@ __device__ __forceinline__ void list_rows(const Window& a) {
   if (threadIdx.x == 0) a.list[0] = found;
 }
 
-template <typename QT, typename KVT, int D>
-__global__ __launch_bounds__(kThreads) void row_kernel(const Window a) {
+template <typename QT, typename KVT, int D, int kRowWaves, int kPair>
+__global__ __launch_bounds__(kRowWaves * kPair * kWave) void row_kernel(const Window a) {
   using S = RowShape<QT, KVT, D>;
   constexpr int kTiles = D / 16;  // output tiles of 16 dimensions
-  __shared__ float s_acc[2][kTiles * 4 * kWave];
-  __shared__ float s_top[kWaves][kWave], s_sum[kWaves][kWave];
-  __shared__ int s_redo;
+  __shared__ float s_acc[kPair][kRowWaves / 2][kTiles * 4 * kWave];
+  __shared__ float s_top[kPair][kRowWaves][kWave], s_sum[kPair][kRowWaves][kWave];
+  __shared__ int s_redo[kPair];
   const int lane = threadIdx.x & (kWave - 1), c = lane / 16, n = lane % 16;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int side = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave % kPair);  // which key head of the pair
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave / kPair);
+  const uint32_t head_groups = a.num_kv_heads / kPair;
   // Items: heads fastest, so that one XCD has its share of the heads of every row.
   const int64_t rows = a.tiled ? a.list[0] : a.num_queries;
-  const int64_t items = rows * a.splits * a.subgroups * a.num_kv_heads;
+  const int64_t items = rows * a.splits * a.subgroups * head_groups;
   for (int64_t next = blockIdx.x; next < items; next += gridDim.x) {
     uint32_t item = static_cast<uint32_t>(next);
-    const int32_t kv_head = item % static_cast<uint32_t>(a.num_kv_heads);
-    item /= static_cast<uint32_t>(a.num_kv_heads);
+    const int32_t kv_head = item % head_groups * kPair + side;
+    item /= head_groups;
     const int32_t sub = item % static_cast<uint32_t>(a.subgroups);
     item /= static_cast<uint32_t>(a.subgroups);
     const int32_t split = item % static_cast<uint32_t>(a.splits);
@@ -432,8 +435,8 @@ __global__ __launch_bounds__(kThreads) void row_kernel(const Window a) {
       load_keys(slot);
       load_values(slot);
     }
-    int32_t slot_next = look_up(round + kWaves);
-    for (; round < last; round += kWaves) {
+    int32_t slot_next = look_up(round + kRowWaves);
+    for (; round < last; round += kRowWaves) {
       const uint32_t live_next = static_cast<uint32_t>(__ballot(slot_next >= 0) & kAll);
       floatx4 st[S::kBlocks];
       if (live != 0) {
@@ -517,32 +520,32 @@ __global__ __launch_bounds__(kThreads) void row_kernel(const Window a) {
       }
       if (live_next != 0) load_values(slot_next);
       live = live_next;
-      slot_next = look_up(round + 2 * kWaves);
+      slot_next = look_up(round + 2 * kRowWaves);
     }
     sum = column_sum(sum);
 
     // The four wavefronts' results, lane by lane: every wavefront holds the same places.
     __syncthreads();  // the row before has been read
-    s_top[wave][lane] = top;
-    s_sum[wave][lane] = sum;
+    s_top[side][wave][lane] = top;
+    s_sum[side][wave][lane] = sum;
     __syncthreads();
     float all = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) all = fmaxf(all, s_top[w][lane]);
+    for (int w = 0; w < kRowWaves; ++w) all = fmaxf(all, s_top[side][w][lane]);
     const float base = all == -INFINITY ? 0.f : all;
     const float mine = fast_exp2(top - base);
 #pragma unroll
     for (int b = 0; b < kTiles; ++b) o[b] *= mine;
     sum = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) sum += s_sum[w][lane] * fast_exp2(s_top[w][lane] - base);
+    for (int w = 0; w < kRowWaves; ++w) sum += s_sum[side][w][lane] * fast_exp2(s_top[side][w][lane] - base);
 #pragma unroll
-    for (int half = kWaves / 2; half > 0; half /= 2) {
+    for (int half = kRowWaves / 2; half > 0; half /= 2) {
       if (wave >= half && wave < 2 * half) {
 #pragma unroll
         for (int b = 0; b < kTiles; ++b) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r) s_acc[wave - half][(b * 4 + r) * kWave + lane] = o[b][r];
+          for (int r = 0; r < 4; ++r) s_acc[side][wave - half][(b * 4 + r) * kWave + lane] = o[b][r];
         }
       }
       __syncthreads();
@@ -550,7 +553,7 @@ __global__ __launch_bounds__(kThreads) void row_kernel(const Window a) {
 #pragma unroll
         for (int b = 0; b < kTiles; ++b) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r) o[b][r] += s_acc[wave][(b * 4 + r) * kWave + lane];
+          for (int r = 0; r < 4; ++r) o[b][r] += s_acc[side][wave][(b * 4 + r) * kWave + lane];
         }
       }
       __syncthreads();
@@ -564,11 +567,11 @@ __global__ __launch_bounds__(kThreads) void row_kernel(const Window a) {
           for (int r = 0; r < 4; ++r) bad = bad || !(fabsf(o[b][r]) < INFINITY);
         }
         const uint64_t any = __ballot((bad || !(fabsf(sum) < INFINITY)) && n < heads);
-        if (lane == 0) s_redo = any != 0;
+        if (lane == 0) s_redo[side] = any != 0;
       }
       __syncthreads();
-      if (s_redo) {
-        for (int g = wave; g < heads; g += kWaves) {
+      if (s_redo[side]) {
+        for (int g = wave; g < heads; g += kRowWaves) {
           exact_row<QT, KVT, D>(a, t, head0 + g, seq, span, span, min(first * S::kKeys, count), min(last * S::kKeys, count), split);
         }
         continue;
@@ -1041,7 +1044,22 @@ int launch(Window a, hipStream_t stream) {
       hipLaunchKernelGGL((tile_kernel<QT, KVT, D>), dim3(static_cast<uint32_t>(tiles + 1)), dim3(kThreads), S::kLds, stream, a);
     }
   }
-  hipLaunchKernelGGL((row_kernel<QT, KVT, D>), dim3(static_cast<uint32_t>(groups)), dim3(kThreads), 0, stream, a);
+  // Few workgroups are of eight wavefronts (1 row, 2 key heads x 64, 516 keys: 11.4 -> 10.3 us; 4 x 4100 keys, 8
+  // splits: 28.4 -> 26.7; 64 rows 203 -> 208). Where there are many and a key row is short, one of eight serves two
+  // neighbouring key heads, and so reads twice as much next to each other. head_dim 256 needs the registers of four.
+  constexpr bool kShort = D * sizeof(KVT) <= 256;
+  const bool wide = D <= 128 && groups <= 256 && !a.tiled;
+  const bool pair = kShort && !wide && a.num_kv_heads % 2 == 0;
+  const auto start = [&](auto kernel, int64_t count, int waves) {
+    hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(count)), dim3(waves * kWave), 0, stream, a);
+  };
+  if constexpr (D <= 128) {
+    if (wide) start(row_kernel<QT, KVT, D, 8, 1>, groups, 8);
+  }
+  if constexpr (kShort) {
+    if (pair) start(row_kernel<QT, KVT, D, 4, 2>, a.tiled ? groups : groups / 2, 8);
+  }
+  if (!wide && !pair) start(row_kernel<QT, KVT, D, 4, 1>, groups, 4);
   if (a.splits > 1) {
     hipLaunchKernelGGL((join_kernel<QT, D>), dim3(static_cast<uint32_t>(joins)), dim3(kThreads), 0, stream, a);
   }
@@ -1083,8 +1101,12 @@ extern "C" int32_t pkv_window_splits(int64_t num_queries, int32_t num_heads, int
   const bool runs = pkv::has_runs(max_query_len, group);
   const int64_t rows = runs ? pkv::kTileQueries / group : 1;
   const int64_t groups = (num_queries + rows - 1) / rows * num_kv_heads * (runs ? 1 : (group + 15) / 16);
-  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(PKV_WINDOW_MAX_SPLITS, longest / 128));
-  return static_cast<int32_t>(std::min<int64_t>(most, (512 + groups - 1) / std::max<int64_t>(1, groups)));
+  // Tiles: two workgroups for every CU, 128 keys to a split at least. Rows: one workgroup of eight
+  // wavefronts for every CU, 512 keys to a split (1 row, 8 key heads x 128, 4100 keys, bfloat16: 62, 39, 27, 22, 24 us
+  // with 1, 2, 4, 8, 16 splits; 4 rows 78, 49, 33, 27, 38; 16 rows 92, 59, 67, 82, 111).
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(PKV_WINDOW_MAX_SPLITS, longest / (runs ? 128 : 512)));
+  const int64_t want = runs ? (512 + groups - 1) / std::max<int64_t>(1, groups) : 256 / std::max<int64_t>(1, groups);
+  return static_cast<int32_t>(std::max<int64_t>(1, std::min(most, want)));
 }
 
 extern "C" int64_t pkv_window_workspace_bytes(int64_t num_queries, int32_t num_heads, int32_t head_dim, int32_t max_query_len,

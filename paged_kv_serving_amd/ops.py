@@ -75,6 +75,17 @@ def _device_index(*tensors: torch.Tensor) -> int:
     return device.index if device.index is not None else torch.cuda.current_device()
 
 
+def _one_device(*tensors: torch.Tensor) -> int:
+    """:func:`_device_index` by the tensors' device ordinals (-1: not on a HIP device)."""
+    device = tensors[0].get_device()
+    if device < 0 or tensors[0].device.type != "cuda":
+        raise ValueError("the KV data path runs on a HIP device; got a tensor on " + str(tensors[0].device))
+    for tensor in tensors:
+        if tensor.get_device() != device:
+            raise ValueError("all tensors must be on the same device")
+    return device
+
+
 def _stream(device: int) -> int:
     """The raw handle of ``device``'s current stream (torch's own accessor, without building a
     Stream object)."""
@@ -101,6 +112,14 @@ def _rows_contiguous(tensor: torch.Tensor, name: str) -> int:
     if tensor.stride(2) != 1 or (heads > 1 and tensor.stride(1) != dim):
         raise ValueError(f"{name}: each token's (heads, head_dim) block must be contiguous")
     return tensor.stride(0) if tensor.shape[0] > 1 else heads * dim
+
+
+def _token_stride(tensor: torch.Tensor, tokens: int, heads: int, dim: int, name: str) -> int:
+    """:func:`_rows_contiguous` of a tensor known to be ``[tokens, heads, dim]``."""
+    token, head, element = tensor.stride()
+    if element != 1 or (head != dim and heads > 1):
+        raise ValueError(f"{name}: each token's (heads, head_dim) block must be contiguous")
+    return token if tokens > 1 else heads * dim
 
 
 def append_kv(
@@ -246,66 +265,73 @@ def rope_append_axes(
     A token whose slot lies outside the pool (padding: -1) writes no pool row; one with a position
     outside the tables is skipped entirely.
     """
-    device = _device_index(key_pool, value_pool, queries, keys, values, positions, cos_table, sin_table, slot_mapping)
-    if key_pool.shape != value_pool.shape or key_pool.dtype != value_pool.dtype:
+    device = _one_device(key_pool, value_pool, queries, keys, values, positions, cos_table, sin_table, slot_mapping)
+    io, kv, pool, shape, kv_shape = queries.dtype, key_pool.dtype, key_pool.shape, queries.shape, keys.shape
+    io_code, kv_code = kv_dtype_code(io), kv_dtype_code(kv)
+    if value_pool.shape != pool or value_pool.dtype != kv:
         raise ValueError("key and value pools must have the same shape and dtype")
     if not (key_pool.is_contiguous() and value_pool.is_contiguous()):
         raise ValueError("pools must be contiguous")
-    if queries.dim() != 3 or keys.dim() != 3 or keys.shape != values.shape:
+    if len(shape) != 3 or len(kv_shape) != 3 or values.shape != kv_shape:
         raise ValueError("queries must be [T, heads, head_dim], keys and values [T, kv_heads, head_dim]")
-    tokens, heads, dim = queries.shape
-    kv_heads = keys.shape[1]
-    if keys.shape[0] != tokens or keys.shape[2] != dim:
+    tokens, heads, dim = shape
+    kv_tokens, kv_heads, kv_dim = kv_shape
+    if kv_tokens != tokens or kv_dim != dim:
         raise ValueError("queries, keys and values disagree on (tokens, head_dim)")
     if heads < 1 or kv_heads < 1:
         raise ValueError("queries and keys need at least one head")
-    if key_pool.dim() < 3 or tuple(key_pool.shape[-2:]) != (kv_heads, dim):
+    if len(pool) < 3 or pool[-1] != dim or pool[-2] != kv_heads:
         raise ValueError("pool rows and keys disagree on (kv_heads, head_dim)")
-    io_code = kv_dtype_code(queries.dtype)
-    if keys.dtype != queries.dtype or values.dtype != queries.dtype:
+    if keys.dtype != io or values.dtype != io:
         raise ValueError("queries, keys and values must have the same dtype")
+    table = cos_table.shape
     if cos_table.dtype != torch.float32 or sin_table.dtype != torch.float32:
         raise ValueError("the rope tables must be float32")
-    if cos_table.shape != sin_table.shape or cos_table.dim() != 2 or not 1 <= cos_table.shape[1] <= dim // 2:
+    if sin_table.shape != table or len(table) != 2 or not 1 <= table[1] <= dim // 2:
         raise ValueError("rope tables must both be [rows, rotary_dim / 2] with rotary_dim at most head_dim")
     if not (cos_table.is_contiguous() and sin_table.is_contiguous()):
         raise ValueError("rope tables must be contiguous")
-    half = cos_table.shape[1]
+    rows, half = table
+    where = positions.shape
     if sections is None:
-        if positions.dim() != 1:
+        if len(where) != 1:
             raise ValueError("positions of several axes need sections")
-        sections, axis_stride = (half,), 0
+        axes, axis_stride, each = 1, 0, (half, 0, 0, 0)
     else:
-        sections = tuple(int(n) for n in sections)
-        if not 1 <= len(sections) <= MAX_ROPE_AXES:
+        each = tuple(int(n) for n in sections)
+        axes = len(each)
+        if not 1 <= axes <= MAX_ROPE_AXES:
             raise ValueError(f"sections must name 1 to {MAX_ROPE_AXES} axes")
-        if min(sections) < 0 or sum(sections) != half:
+        if min(each) < 0 or sum(each) != half:
             raise ValueError("sections must be non-negative and add up to rotary_dim / 2")
-        if interleaved and any(n and a + len(sections) * (n - 1) >= half for a, n in enumerate(sections) if a):
+        if interleaved and any(n and a + axes * (n - 1) >= half for a, n in enumerate(each) if a):
             raise ValueError("interleaved sections: an axis has more frequencies than its turns")
-        if positions.dim() != 2 or positions.shape[0] != len(sections):
+        if len(where) != 2 or where[0] != axes:
             raise ValueError("positions must be [axes, T] with one row for each section")
-        axis_stride = positions.stride(0) if len(sections) > 1 else 0
-    if positions.dtype != torch.int64 or positions.shape[-1] != tokens or (tokens > 1 and positions.stride(-1) != 1):
+        axis_stride = positions.stride(0) if axes > 1 else 0
+        each += (0,) * (MAX_ROPE_AXES - axes)
+    if positions.dtype != torch.int64 or where[-1] != tokens or (tokens > 1 and positions.stride(-1) != 1):
         raise ValueError("positions must be int64 with one entry per token, adjacent in memory")
     if slot_mapping.dtype != torch.int64 or slot_mapping.shape != (tokens,) or not slot_mapping.is_contiguous():
         raise ValueError("slot_mapping must be contiguous int64 with one entry per token")
-    q_stride = _rows_contiguous(queries, "queries")
-    k_stride = _rows_contiguous(keys, "keys")
-    v_stride = _rows_contiguous(values, "values")
+    q_stride = _token_stride(queries, tokens, heads, dim, "queries")
+    k_stride = _token_stride(keys, tokens, kv_heads, dim, "keys")
+    v_stride = _token_stride(values, tokens, kv_heads, dim, "values")
     if out is None:
-        out = torch.empty((tokens, heads, dim), dtype=queries.dtype, device=queries.device)
-    elif out.shape != queries.shape or out.dtype != queries.dtype or out.device != queries.device:
+        out = queries.new_empty(shape)
+        out_stride = heads * dim
+    elif out.shape != shape or out.dtype != io or out.device != queries.device:
         raise ValueError("out must match queries")
-    out_stride = _rows_contiguous(out, "out")
+    else:
+        out_stride = _token_stride(out, tokens, heads, dim, "out")
     if tokens == 0:
         return out
     rc = _host().rope_append_axes(
         out.data_ptr(), queries.data_ptr(), keys.data_ptr(), values.data_ptr(), out_stride, q_stride, k_stride,
-        v_stride, positions.data_ptr(), axis_stride, cos_table.data_ptr(), sin_table.data_ptr(), cos_table.shape[0],
+        v_stride, positions.data_ptr(), axis_stride, cos_table.data_ptr(), sin_table.data_ptr(), rows,
         key_pool.data_ptr(), value_pool.data_ptr(), key_pool.numel() // (kv_heads * dim), slot_mapping.data_ptr(),
-        tokens, io_code, kv_dtype_code(key_pool.dtype), heads, kv_heads, dim, 2 * half, len(sections),
-        1 if interleaved else 0, *sections, *(0,) * (MAX_ROPE_AXES - len(sections)), device, _stream(device),
+        tokens, io_code, kv_code, heads, kv_heads, dim, 2 * half, axes, 1 if interleaved else 0, *each, device,
+        _stream(device),
     )  # fmt: skip
     _native.check(rc, "pkv_rope_append_axes")
     return out
@@ -433,7 +459,7 @@ def sample_tokens(
 
     Extends the reference's per-row draw (sampling.py:56-74) to batches on the device.
     """
-    device = _device_index(logits, uniforms)
+    device = _one_device(logits, uniforms)
     if logits.dim() != 2 or logits.dtype not in _DTYPE_CODES:
         raise ValueError("logits must be float32 or bfloat16 of shape (rows, vocab)")
     rows, vocab = logits.shape
@@ -456,7 +482,7 @@ def sample_tokens(
     if vocab > 1 and logits.stride(1) != 1:
         logits = logits.contiguous()
     if out is None:
-        out = torch.empty(rows, dtype=torch.int32, device=logits.device)
+        out = uniforms.new_empty((rows,), dtype=torch.int32)
     elif out.shape != (rows,) or out.dtype != torch.int32 or not out.is_contiguous() or out.device != logits.device:
         raise ValueError("out must be a contiguous int32 tensor with one entry per row")
     if rows == 0:
@@ -1453,33 +1479,36 @@ def paged_attention_window(
     reading of the batch, so it can be captured into a graph whose batch changes from replay to
     replay (within T, S, ``max_context_len`` and ``max_query_len``).
     """
-    device = _device_index(queries, query_positions, query_seq, key_cache, value_cache, block_tables, context_lens)
-    q_code = kv_dtype_code(queries.dtype)
-    stride = _rows_contiguous(queries, "queries")
-    num_queries, heads, dim = queries.shape
-    if key_cache.shape != value_cache.shape or key_cache.dtype != value_cache.dtype:
+    device = _one_device(queries, query_positions, query_seq, key_cache, value_cache, block_tables, context_lens)
+    io, kv, shape, cache = queries.dtype, key_cache.dtype, queries.shape, key_cache.shape
+    q_code, kv_code = kv_dtype_code(io), kv_dtype_code(kv)
+    if len(shape) != 3:
+        raise ValueError("queries must have shape (tokens, heads, head_dim)")
+    num_queries, heads, dim = shape
+    if value_cache.shape != cache or value_cache.dtype != kv:
         raise ValueError("key and value caches must have the same shape and dtype")
-    if key_cache.dim() != 4 or key_cache.shape[3] != dim:
+    if len(cache) != 4 or cache[3] != dim:
         raise ValueError("caches must have shape (num_blocks, block_size, kv_heads, head_dim)")
     if not (key_cache.is_contiguous() and value_cache.is_contiguous()):
         raise ValueError("caches must be contiguous")
-    num_blocks, block_size, kv_heads, _ = key_cache.shape
+    num_blocks, block_size, kv_heads, _ = cache
     if kv_heads < 1 or heads < 1 or heads % kv_heads:
         raise ValueError("heads must be a multiple of kv_heads")
     if heads // kv_heads > MAX_WINDOW_GROUP:
         raise ValueError(f"at most {MAX_WINDOW_GROUP} query heads per key head")
-    kv_code = kv_dtype_code(key_cache.dtype)
-    if key_cache.dtype == torch.float32 and queries.dtype != torch.float32:
+    if kv == torch.float32 and io != torch.float32:
         raise ValueError("float32 caches need float32 queries")
+    stride = _token_stride(queries, num_queries, heads, dim, "queries")
     for name, tensor in (("query_positions", query_positions), ("query_seq", query_seq)):
         if tensor.dtype != torch.int32 or tensor.shape != (num_queries,) or not tensor.is_contiguous():
             raise ValueError(f"{name} must be contiguous int32 with one entry per query")
-    if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or not block_tables.is_contiguous():
+    tables = block_tables.shape
+    if block_tables.dtype != torch.int32 or len(tables) != 2 or not block_tables.is_contiguous():
         raise ValueError("block_tables must be contiguous int32 of shape (num_seqs, max_blocks)")
-    num_seqs = block_tables.shape[0]
+    num_seqs, table_stride = tables
     if context_lens.dtype != torch.int32 or context_lens.shape != (num_seqs,) or not context_lens.is_contiguous():
         raise ValueError("context_lens must be contiguous int32 with one entry per sequence")
-    if not 0 <= max_context_len <= _INT32_MAX or block_tables.shape[1] * block_size < max_context_len:
+    if not 0 <= max_context_len <= _INT32_MAX or table_stride * block_size < max_context_len:
         raise ValueError("block_tables are too narrow for max_context_len")
     if window < 1 or sinks < 0:
         raise ValueError("window must be >= 1 and sinks >= 0")
@@ -1488,8 +1517,8 @@ def paged_attention_window(
     if not 0 <= num_splits <= MAX_WINDOW_SPLITS:
         raise ValueError(f"num_splits must be in [0, {MAX_WINDOW_SPLITS}]")
     if out is None:
-        out = torch.empty((num_queries, heads, dim), dtype=queries.dtype, device=queries.device)
-    elif out.shape != queries.shape or out.dtype != queries.dtype or out.device != queries.device:
+        out = queries.new_empty(shape)
+    elif out.shape != shape or out.dtype != io or out.device != queries.device:
         raise ValueError("out must match queries")
     elif not out.is_contiguous():
         raise ValueError("out must be contiguous")
@@ -1501,7 +1530,7 @@ def paged_attention_window(
     splits, need = host.window_workspace(num_queries, heads, kv_heads, dim, window, sinks, max_context_len, rows, num_splits)
     if need:
         if workspace is None:
-            workspace = torch.empty(need // 4, dtype=torch.float32, device=queries.device)
+            workspace = context_lens.new_empty((need // 4,))  # no values yet: four bytes an entry
         elif workspace.device != queries.device or not workspace.is_contiguous():
             raise ValueError("workspace must be contiguous and on the queries' device")
         elif workspace.numel() * workspace.element_size() < need:
@@ -1509,7 +1538,7 @@ def paged_attention_window(
     rc = host.window_attention(
         out.data_ptr(), queries.data_ptr(), stride, query_positions.data_ptr(), query_seq.data_ptr(), num_queries,
         key_cache.data_ptr(), value_cache.data_ptr(), num_blocks, block_tables.data_ptr(), context_lens.data_ptr(),
-        workspace.data_ptr() if need else 0, need, q_code, kv_code, block_size, block_tables.shape[1], num_seqs,
+        workspace.data_ptr() if need else 0, need, q_code, kv_code, block_size, table_stride, num_seqs,
         heads, kv_heads, dim, window, sinks, max_context_len, rows, splits, scale, device, _stream(device),
     )  # fmt: skip
     _native.check(rc, "pkv_window_attention")
