@@ -675,6 +675,16 @@ __device__ __forceinline__ short4v read_transposed(const uint16_t* p) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p));
 }
 
+// What a tile's rows in no block of the pool are read from.
+__device__ const u32x4 kZeros = {0, 0, 0, 0};
+
+// 16 bytes per lane from global memory to LDS: `to`, the same in every lane, is the first lane's place.
+__device__ __forceinline__ void load_to_lds(const void* from, uint16_t* to) {
+  typedef const __attribute__((address_space(1))) void* global_ptr;
+  typedef __attribute__((address_space(3))) void* lds_ptr;
+  __builtin_amdgcn_global_load_lds((global_ptr)(from), (lds_ptr)(to), 16, 0, 0);
+}
+
 __device__ __forceinline__ int32_t wave_min(int32_t x) {
   for (int m = kWave / 2; m > 0; m >>= 1) x = min(x, __shfl_xor(x, m));
   return __builtin_amdgcn_readfirstlane(x);
@@ -707,6 +717,7 @@ __global__ __launch_bounds__(kThreads, (TileShape<QT, KVT, D>::kWaves)) void til
   const int64_t block1 = min(block0 + a.tile_rows, a.num_queries);
   const KVT* keys = static_cast<const KVT*>(a.keys);
   const KVT* values = static_cast<const KVT*>(a.values);
+  const void* zeros = &kZeros;
   auto plane = [&](int buffer, int which, int piece) {
     return s_kv + ((buffer * 2 + which) * S::kKvPieces + piece) * S::kPlane;
   };
@@ -791,41 +802,50 @@ __global__ __launch_bounds__(kThreads, (TileShape<QT, KVT, D>::kWaves)) void til
     };
     constexpr int kWide = sizeof(KVT) / 2;  // 16-byte loads of a chunk
     u32x4 kx[S::kStaged][kWide], vx[S::kStaged][kWide];
-    auto load = [&](int32_t tile) {
+    auto load = [&](int32_t tile, int buffer) {
 #pragma unroll
       for (int i = 0; i < S::kStaged; ++i) {
         const int at = tid + i * kThreads, row = at / S::kChunks, chunk = at % S::kChunks;
         const int32_t slot = s_slot[tile % 3][row];
-        const int64_t from = row_of(a, slot, kv_head, D) + chunk * 8;
+        const int64_t from = row_of(a, slot, kv_head, D);
+        if constexpr (kWide == 1) {
+          // Straight to LDS, where a wavefront's 64 chunks lie one after the other: the permutation is made
+          // by which chunk of the row a lane fetches (it is its own inverse).
+          const void* k = slot >= 0 ? static_cast<const void*>(keys + from + 8 * key_chunk<D>(row, chunk)) : zeros;
+          const void* v = slot >= 0 ? static_cast<const void*>(values + from + 8 * value_chunk<D>(row, chunk)) : zeros;
+          load_to_lds(k, plane(buffer, 0, 0) + 8 * (wave * kWave + i * kThreads));
+          load_to_lds(v, plane(buffer, 1, 0) + 8 * (wave * kWave + i * kThreads));
+        } else {
 #pragma unroll
-        for (int w = 0; w < kWide; ++w) {
-          kx[i][w] = slot >= 0 ? *reinterpret_cast<const u32x4*>(keys + from + w * 4) : u32x4{0, 0, 0, 0};
-          vx[i][w] = slot >= 0 ? *reinterpret_cast<const u32x4*>(values + from + w * 4) : u32x4{0, 0, 0, 0};
+          for (int w = 0; w < kWide; ++w) {
+            kx[i][w] = slot >= 0 ? *reinterpret_cast<const u32x4*>(keys + from + chunk * 8 + w * 4) : u32x4{0, 0, 0, 0};
+            vx[i][w] = slot >= 0 ? *reinterpret_cast<const u32x4*>(values + from + chunk * 8 + w * 4) : u32x4{0, 0, 0, 0};
+          }
         }
       }
     };
     auto put = [&](int buffer, int which, int i, const u32x4 (&x)[kWide]) {
       const int at = tid + i * kThreads, row = at / S::kChunks, chunk = at % S::kChunks;
       const int to = row * D + 8 * (which == 0 ? key_chunk<D>(row, chunk) : value_chunk<D>(row, chunk));
-      if constexpr (kWide == 1) {
-        *reinterpret_cast<u32x4*>(plane(buffer, which, 0) + to) = x[0];
-      } else {
-        u32x4 piece[3];
+      u32x4 piece[3];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float x0 = __uint_as_float(x[e / 2][e % 2 * 2]), x1 = __uint_as_float(x[e / 2][e % 2 * 2 + 1]);
+      for (int e = 0; e < 4; ++e) {
+        float x0 = __uint_as_float(x[e / 2][e % 2 * 2]), x1 = __uint_as_float(x[e / 2][e % 2 * 2 + 1]);
 #pragma unroll
-          for (int p = 0; p < 3; ++p) piece[p][e] = cut_piece(x0, x1);
-        }
-#pragma unroll
-        for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x4*>(plane(buffer, which, p) + to) = piece[p];
+        for (int p = 0; p < 3; ++p) piece[p][e] = cut_piece(x0, x1);
       }
+#pragma unroll
+      for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x4*>(plane(buffer, which, p) + to) = piece[p];
     };
     auto stage = [&](int buffer) {
+      if constexpr (kWide == 1) {
+        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wavefront's loads to LDS have arrived
+      } else {
 #pragma unroll
-      for (int i = 0; i < S::kStaged; ++i) {
-        put(buffer, 0, i, kx[i]);
-        put(buffer, 1, i, vx[i]);
+        for (int i = 0; i < S::kStaged; ++i) {
+          put(buffer, 0, i, kx[i]);
+          put(buffer, 1, i, vx[i]);
+        }
       }
     };
 
@@ -834,51 +854,60 @@ __global__ __launch_bounds__(kThreads, (TileShape<QT, KVT, D>::kWaves)) void til
     keep_slots(first + 1, look_up(first + 1));
     __syncthreads();
     if (first < last) {
-      load(first);
+      load(first, 0);
       stage(0);
     }
     __syncthreads();
     for (int32_t tile = first; tile < last; ++tile) {
       const int buffer = (tile - first) & 1;
-      if (tile + 1 < last) load(tile + 1);
+      if (tile + 1 < last) load(tile + 1, buffer ^ 1);
       const int32_t slot_ahead = look_up(tile + 2);
       const uint64_t tile_live = s_live[tile % 3];
+      // The tile's 32-key blocks one after the other through the scores, together through the softmax.
+      floatx16 st[kSub];
+      bool any = false;
 #pragma unroll
       for (int j = 0; j < kSub; ++j) {
         const int32_t at = tile * S::kKeys + 32 * j;  // the block's first item of the span
-        if (at >= count) break;
         const int32_t key0 = all.key(at), key1 = all.key(min(at + 31, count - 1));
-        if (key0 >= wave_end || (key0 >= wave_sinks && key1 < wave_begin)) continue;
+        const bool needed = at < count && key0 < wave_end && (key0 < wave_sinks || key1 >= wave_begin);
         const uint32_t live = static_cast<uint32_t>(tile_live >> (32 * j));
-        floatx16 st;
+        any = any || needed;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) st[r] = 0.f;
-        const uint16_t* kp = plane(buffer, 0, 0) + (32 * j + n) * D;
+        for (int r = 0; r < 16; ++r) st[j][r] = needed ? 0.f : -INFINITY;
+        if (needed) {
+          const uint16_t* kp = plane(buffer, 0, 0) + (32 * j + n) * D;
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-          u32x4 k[S::kKvPieces];
+          for (int s = 0; s < kSteps; ++s) {
+            u32x4 k[S::kKvPieces];
 #pragma unroll
-          for (int p = 0; p < S::kKvPieces; ++p) {
-            k[p] = *reinterpret_cast<const u32x4*>(kp + p * S::kPlane + 8 * key_chunk<D>(32 * j + n, 2 * s + c));
-          }
+            for (int p = 0; p < S::kKvPieces; ++p) {
+              k[p] = *reinterpret_cast<const u32x4*>(kp + p * S::kPlane + 8 * key_chunk<D>(32 * j + n, 2 * s + c));
+            }
 #pragma unroll
-          for (int p = S::kKvPieces - 1; p >= 0; --p) {
+            for (int p = S::kKvPieces - 1; p >= 0; --p) {
 #pragma unroll
-            for (int q = S::kQPieces - 1; q >= 0; --q) {
-              if (counted(p, q)) st = mfma32(k[p], qr[q][s], st);
+              for (int q = S::kQPieces - 1; q >= 0; --q) {
+                if (counted(p, q)) st[j] = mfma32(k[p], qr[q][s], st[j]);
+              }
             }
           }
+          if (!(key0 >= full_begin && key1 < full_end && key0 >= all.sinks && live == 0xffffffffu)) {
+            const uint32_t seen = (own.seen_of(all, at) & live) >> (4 * c);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) st[j][r] = (seen >> (8 * (r / 4) + r % 4)) & 1 ? st[j][r] : -INFINITY;
+          }
         }
+      }
+      if (any) {
         // Scores are kept as they are, times scale (bfloat16) or already scaled (float32).
         const float scale = sizeof(QT) == 2 ? a.scale_log2 : 1.f;
-        if (!(key0 >= full_begin && key1 < full_end && key0 >= all.sinks && live == 0xffffffffu)) {
-          const uint32_t seen = (own.seen_of(all, at) & live) >> (4 * c);
+        float most = -INFINITY;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) st[r] = (seen >> (8 * (r / 4) + r % 4)) & 1 ? st[r] : -INFINITY;
+        for (int j = 0; j < kSub; ++j) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) most = fmaxf(most, st[j][r]);
         }
-        float most = fmaxf(st[0], st[1]);
-#pragma unroll
-        for (int r = 2; r < 16; ++r) most = fmaxf(most, st[r]);
         {
           const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(most), __float_as_uint(most), false, false);
           most = fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1])) * scale;
@@ -895,41 +924,41 @@ __global__ __launch_bounds__(kThreads, (TileShape<QT, KVT, D>::kWaves)) void til
         }
         const float from = top == -INFINITY ? 0.f : top;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          st[r] = fast_exp2(__builtin_fmaf(st[r], scale, -from));
-          sum += st[r];
-        }
-        u32x4 pr[S::kPPieces][2];
+        for (int j = 0; j < kSub; ++j) {
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float x0 = st[8 * s + 2 * e], x1 = st[8 * s + 2 * e + 1];
-#pragma unroll
-            for (int p = 0; p < S::kPPieces; ++p) pr[p][s][e] = cut_piece(x0, x1);
+          for (int r = 0; r < 16; ++r) {
+            st[j][r] = fast_exp2(__builtin_fmaf(st[j][r], scale, -from));
+            sum += st[j][r];
           }
-        }
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          // Keys 16 s + 4 c .. + 3 and 8 more on; this lane reads row i / 4 of its 16 lanes' block.
-          const int row = 32 * j + 16 * s + 4 * c + (lane % 16) / 4;
-          const int part = (lane / 16 % 2) * 16 + lane % 4 * 4;  // its dimension within 32
+          for (int s = 0; s < 2; ++s) {
+            u32x4 pr[S::kPPieces];
 #pragma unroll
-          for (int b = 0; b < kBlocks; ++b) {
-            const int chunk = (32 * b + part) / 8, rest = part % 8;
-            u32x4 v[S::kKvPieces];
+            for (int e = 0; e < 4; ++e) {
+              float x0 = st[j][8 * s + 2 * e], x1 = st[j][8 * s + 2 * e + 1];
 #pragma unroll
-            for (int p = 0; p < S::kKvPieces; ++p) {
-              const uint16_t* vp = plane(buffer, 1, p);
-              const auto lo = __builtin_bit_cast(u32x2, read_transposed(vp + row * D + 8 * value_chunk<D>(row, chunk) + rest));
-              const auto hi = __builtin_bit_cast(u32x2, read_transposed(vp + (row + 8) * D + 8 * value_chunk<D>(row + 8, chunk) + rest));
-              v[p] = u32x4{lo.x, lo.y, hi.x, hi.y};
+              for (int p = 0; p < S::kPPieces; ++p) pr[p][e] = cut_piece(x0, x1);
             }
+            // Keys 16 s + 4 c .. + 3 and 8 more on; this lane reads row i / 4 of its 16 lanes' block.
+            const int row = 32 * j + 16 * s + 4 * c + (lane % 16) / 4;
+            const int part = (lane / 16 % 2) * 16 + lane % 4 * 4;  // its dimension within 32
 #pragma unroll
-            for (int p = S::kKvPieces - 1; p >= 0; --p) {
+            for (int b = 0; b < kBlocks; ++b) {
+              const int chunk = (32 * b + part) / 8, rest = part % 8;
+              u32x4 v[S::kKvPieces];
 #pragma unroll
-              for (int q = S::kPPieces - 1; q >= 0; --q) {
-                if (counted(p, q)) o[b] = mfma32(v[p], pr[q][s], o[b]);
+              for (int p = 0; p < S::kKvPieces; ++p) {
+                const uint16_t* vp = plane(buffer, 1, p);
+                const auto lo = __builtin_bit_cast(u32x2, read_transposed(vp + row * D + 8 * value_chunk<D>(row, chunk) + rest));
+                const auto hi = __builtin_bit_cast(u32x2, read_transposed(vp + (row + 8) * D + 8 * value_chunk<D>(row + 8, chunk) + rest));
+                v[p] = u32x4{lo.x, lo.y, hi.x, hi.y};
+              }
+#pragma unroll
+              for (int p = S::kKvPieces - 1; p >= 0; --p) {
+#pragma unroll
+                for (int q = S::kPPieces - 1; q >= 0; --q) {
+                  if (counted(p, q)) o[b] = mfma32(v[p], pr[q], o[b]);
+                }
               }
             }
           }
@@ -1049,7 +1078,7 @@ int launch(Window a, hipStream_t stream) {
   // neighbouring key heads, and so reads twice as much next to each other. head_dim 256 needs the registers of four.
   constexpr bool kShort = D * sizeof(KVT) <= 256;
   const bool wide = D <= 128 && groups <= 256 && !a.tiled;
-  const bool pair = kShort && !wide && a.num_kv_heads % 2 == 0;
+  const bool pair = kShort && groups >= 512 && a.num_kv_heads % 2 == 0;
   const auto start = [&](auto kernel, int64_t count, int waves) {
     hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(count)), dim3(waves * kWave), 0, stream, a);
   };
