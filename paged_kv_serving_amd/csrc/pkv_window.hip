@@ -19,15 +19,11 @@ constexpr int kWaves = kThreads / kWave;
 constexpr int kTileQueries = 128;  // (row, head) pairs of a tile
 constexpr int kMinRun = PKV_WINDOW_MIN_RUN;
 constexpr float kLazyLog2 = 8.f;
-#ifndef PKV_PP
-#define PKV_PP 2
-#endif
 
 typedef float floatx2 __attribute__((ext_vector_type(2)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef short short4v __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -628,13 +624,14 @@ __global__ __launch_bounds__(kRowWaves * kPair * kWave) void row_kernel(const Wi
 // weights P are two, 2^-17 of a weight: one piece (2^-9) would add as much error as the output's rounding.
 //
 // Keys and values are staged kKeys at a time in two LDS buffers: while one is used, the next tile's rows
-// are in flight to registers and the slots of the one after are looked up.
+// are in flight (bfloat16 pools: straight to LDS; float32 pools: to registers, cut on their way to LDS) and
+// the slots of the one after are looked up.
 // ---------------------------------------------------------------------------------------------
 template <typename QT, typename KVT, int D>
 struct TileShape {
   static constexpr int kQPieces = sizeof(QT) == 4 ? 3 : 1;
   static constexpr int kKvPieces = sizeof(KVT) == 4 ? 3 : 1;
-  static constexpr int kPPieces = sizeof(QT) == 4 ? 3 : PKV_PP;
+  static constexpr int kPPieces = sizeof(QT) == 4 ? 3 : 2;
   static constexpr int kKeys = (sizeof(KVT) == 2 && D <= 128) || D == 32 ? 64 : 32;
   static constexpr int kChunks = D / 8;                                // 16-byte chunks of a bfloat16 row
   static constexpr int kPlane = kKeys * D;                             // elements of one piece of a staged tile
@@ -670,13 +667,47 @@ __device__ __forceinline__ int value_chunk(int row, int chunk) {
   return D >= 64 ? chunk ^ (2 * (row & 3)) : chunk;
 }
 
-__device__ __forceinline__ short4v read_transposed(const uint16_t* p) {
-  typedef __attribute__((address_space(3))) short4v* lds_ptr;
-  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p));
+// The value operands of one step for `N` output tiles: of each, four keys of a lane's dimension from `lo` and
+// four from 8 rows on. The reads of a step are issued together and waited for once, in one block: as separate
+// ones the compiler waits for each, and for the next tile's rows on their way to LDS besides, which it takes
+// for the same memory. Output tiles b and b + 2 lie 128 bytes apart; even and odd ones have their own address.
+template <int N, int kRowBytes>
+__device__ __forceinline__ void read_values(uint32_t even, uint32_t odd, u32x4 (&v)[N]) {
+  u32x2 lo[N], hi[N];
+  if constexpr (N == 1) {
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %2\n\tds_read_b64_tr_b16 %1, %2 offset:%3\n\ts_waitcnt lgkmcnt(0)"
+        : "=&v"(lo[0]), "=&v"(hi[0])
+        : "v"(even), "i"(8 * kRowBytes)
+        : "memory");
+  } else if constexpr (N == 2) {
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %4\n\tds_read_b64_tr_b16 %1, %4 offset:%6\n\t"
+        "ds_read_b64_tr_b16 %2, %5\n\tds_read_b64_tr_b16 %3, %5 offset:%6\n\ts_waitcnt lgkmcnt(0)"
+        : "=&v"(lo[0]), "=&v"(hi[0]), "=&v"(lo[1]), "=&v"(hi[1])
+        : "v"(even), "v"(odd), "i"(8 * kRowBytes)
+        : "memory");
+  } else {
+    static_assert(N == 4, "one, two or four output tiles at a time");
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%10\n\t"
+        "ds_read_b64_tr_b16 %2, %9\n\tds_read_b64_tr_b16 %3, %9 offset:%10\n\t"
+        "ds_read_b64_tr_b16 %4, %8 offset:128\n\tds_read_b64_tr_b16 %5, %8 offset:%11\n\t"
+        "ds_read_b64_tr_b16 %6, %9 offset:128\n\tds_read_b64_tr_b16 %7, %9 offset:%11\n\ts_waitcnt lgkmcnt(0)"
+        : "=&v"(lo[0]), "=&v"(hi[0]), "=&v"(lo[1]), "=&v"(hi[1]), "=&v"(lo[2]), "=&v"(hi[2]), "=&v"(lo[3]), "=&v"(hi[3])
+        : "v"(even), "v"(odd), "i"(8 * kRowBytes), "i"(8 * kRowBytes + 128)
+        : "memory");
+  }
+#pragma unroll
+  for (int b = 0; b < N; ++b) v[b] = u32x4{lo[b].x, lo[b].y, hi[b].x, hi[b].y};
 }
 
 // What a tile's rows in no block of the pool are read from.
 __device__ const u32x4 kZeros = {0, 0, 0, 0};
+
+__device__ __forceinline__ uint32_t lds_address(const uint16_t* p) {
+  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) uint16_t*)(p)));
+}
 
 // 16 bytes per lane from global memory to LDS: `to`, the same in every lane, is the first lane's place.
 __device__ __forceinline__ void load_to_lds(const void* from, uint16_t* to) {
@@ -700,6 +731,10 @@ __global__ __launch_bounds__(kThreads, (TileShape<QT, KVT, D>::kWaves)) void til
   constexpr int kBlocks = D / 32;       // output tiles of 32 dimensions
   constexpr int kSteps = D / 16;        // steps of a score product
   constexpr int kSub = S::kKeys / 32;   // 32-key blocks of a staged tile
+  // Steps whose keys are read together: one at a time the compiler waits for each read before its product
+  // (8 sequences of 512 tokens in bfloat16: 141 us, and 137 by fours).
+  constexpr int kAhead = S::kKvPieces > 1 || kSteps < 4 ? 2 : 4;
+  constexpr int kTogether = kBlocks < 4 ? kBlocks : 4;  // output tiles whose values are read together
   extern __shared__ __align__(16) uint16_t s_kv[];  // [buffer][K, V][piece][key][D]
   __shared__ int32_t s_slot[3][S::kKeys];
   __shared__ uint64_t s_live[3];
@@ -788,13 +823,25 @@ __global__ __launch_bounds__(kThreads, (TileShape<QT, KVT, D>::kWaves)) void til
     }
     float top = -INFINITY, sum = 0.f;
 
-    // Staging. Slots of a tile by the first wavefront, rows by all.
+    // Staging. Slots of a tile by the first wavefront, rows by all. A tile's table entries are loaded long
+    // before they are used, and before the rows that are loaded in between: loads arrive in order.
+    struct Entry {
+      int32_t key, block;
+    };
     auto look_up = [&](int32_t tile) {
       const int32_t i = tile * S::kKeys + tid;
-      return tid < S::kKeys && tile < last && i < count ? slot_of(a, table, all.key(i)) : -1;
+      Entry e{-1, -1};
+      if (tid < S::kKeys && tile < last && i < count) {
+        e.key = all.key(i);
+        e.block = table[static_cast<uint32_t>(e.key) / static_cast<uint32_t>(a.block_size)];
+      }
+      return e;
     };
-    auto keep_slots = [&](int32_t tile, int32_t slot) {
+    auto keep_slots = [&](int32_t tile, const Entry& e) {
       if (wave == 0) {
+        const int32_t slot = e.block < 0 || e.block >= a.num_blocks
+                                 ? -1
+                                 : e.block * a.block_size + static_cast<int32_t>(static_cast<uint32_t>(e.key) % static_cast<uint32_t>(a.block_size));
         const uint64_t live = __ballot(slot >= 0);
         if (tid < S::kKeys) s_slot[tile % 3][tid] = slot;
         if (tid == 0) s_live[tile % 3] = live;
@@ -860,8 +907,8 @@ __global__ __launch_bounds__(kThreads, (TileShape<QT, KVT, D>::kWaves)) void til
     __syncthreads();
     for (int32_t tile = first; tile < last; ++tile) {
       const int buffer = (tile - first) & 1;
+      const Entry ahead = look_up(tile + 2);
       if (tile + 1 < last) load(tile + 1, buffer ^ 1);
-      const int32_t slot_ahead = look_up(tile + 2);
       const uint64_t tile_live = s_live[tile % 3];
       // The tile's 32-key blocks one after the other through the scores, together through the softmax.
       floatx16 st[kSub];
@@ -878,17 +925,24 @@ __global__ __launch_bounds__(kThreads, (TileShape<QT, KVT, D>::kWaves)) void til
         if (needed) {
           const uint16_t* kp = plane(buffer, 0, 0) + (32 * j + n) * D;
 #pragma unroll
-          for (int s = 0; s < kSteps; ++s) {
-            u32x4 k[S::kKvPieces];
+          for (int s0 = 0; s0 < kSteps; s0 += kAhead) {
+            u32x4 k[kAhead][S::kKvPieces];
 #pragma unroll
-            for (int p = 0; p < S::kKvPieces; ++p) {
-              k[p] = *reinterpret_cast<const u32x4*>(kp + p * S::kPlane + 8 * key_chunk<D>(32 * j + n, 2 * s + c));
+            for (int s = 0; s < kAhead; ++s) {
+#pragma unroll
+              for (int p = 0; p < S::kKvPieces; ++p) {
+                k[s][p] = *reinterpret_cast<const u32x4*>(kp + p * S::kPlane + 8 * key_chunk<D>(32 * j + n, 2 * (s0 + s) + c));
+              }
             }
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int p = S::kKvPieces - 1; p >= 0; --p) {
+            for (int s = 0; s < kAhead; ++s) {
 #pragma unroll
-              for (int q = S::kQPieces - 1; q >= 0; --q) {
-                if (counted(p, q)) st[j] = mfma32(k[p], qr[q][s], st[j]);
+              for (int p = S::kKvPieces - 1; p >= 0; --p) {
+#pragma unroll
+                for (int q = S::kQPieces - 1; q >= 0; --q) {
+                  if (counted(p, q)) st[j] = mfma32(k[s][p], qr[q][s0 + s], st[j]);
+                }
               }
             }
           }
@@ -943,21 +997,23 @@ __global__ __launch_bounds__(kThreads, (TileShape<QT, KVT, D>::kWaves)) void til
             const int row = 32 * j + 16 * s + 4 * c + (lane % 16) / 4;
             const int part = (lane / 16 % 2) * 16 + lane % 4 * 4;  // its dimension within 32
 #pragma unroll
-            for (int b = 0; b < kBlocks; ++b) {
-              const int chunk = (32 * b + part) / 8, rest = part % 8;
-              u32x4 v[S::kKvPieces];
+            for (int b0 = 0; b0 < kBlocks; b0 += kTogether) {
+              u32x4 v[S::kKvPieces][kTogether];
 #pragma unroll
               for (int p = 0; p < S::kKvPieces; ++p) {
-                const uint16_t* vp = plane(buffer, 1, p);
-                const auto lo = __builtin_bit_cast(u32x2, read_transposed(vp + row * D + 8 * value_chunk<D>(row, chunk) + rest));
-                const auto hi = __builtin_bit_cast(u32x2, read_transposed(vp + (row + 8) * D + 8 * value_chunk<D>(row + 8, chunk) + rest));
-                v[p] = u32x4{lo.x, lo.y, hi.x, hi.y};
+                const auto at = [&](int b) {
+                  return lds_address(plane(buffer, 1, p) + row * D + 8 * value_chunk<D>(row, 4 * b + part / 8) + part % 8);
+                };
+                read_values<kTogether, 2 * D>(at(b0), kTogether > 1 ? at(b0 + 1) : 0, v[p]);
               }
 #pragma unroll
-              for (int p = S::kKvPieces - 1; p >= 0; --p) {
+              for (int b = 0; b < kTogether; ++b) {
 #pragma unroll
-                for (int q = S::kPPieces - 1; q >= 0; --q) {
-                  if (counted(p, q)) o[b] = mfma32(v[p], pr[q], o[b]);
+                for (int p = S::kKvPieces - 1; p >= 0; --p) {
+#pragma unroll
+                  for (int q = S::kPPieces - 1; q >= 0; --q) {
+                    if (counted(p, q)) o[b0 + b] = mfma32(v[p][b], pr[q], o[b0 + b]);
+                  }
                 }
               }
             }
@@ -965,7 +1021,7 @@ __global__ __launch_bounds__(kThreads, (TileShape<QT, KVT, D>::kWaves)) void til
         }
       }
       if (tile + 1 < last) stage(buffer ^ 1);
-      keep_slots(tile + 2, slot_ahead);
+      keep_slots(tile + 2, ahead);
       __syncthreads();
     }
     {
