@@ -608,12 +608,15 @@ int pkv_rope_append_axes(const pkv_rope_axes* args, int device, void* stream);
  * Rows of one sequence need not lie next to each other, nor in order. A row that sees no key gets
  * zeros. Block ids outside [0, num_blocks) at a visible position are skipped, as in
  * pkv_paged_attention. Supported: head_dim 32, 64, 128, 256; float32 queries over float32 or bfloat16
- * pools, bfloat16 queries over bfloat16 pools; up to PKV_WINDOW_MAX_GROUP query heads per key head.
+ * pools, bfloat16 queries over bfloat16 pools; up to PKV_WINDOW_MAX_GROUP query heads per key head;
+ * fewer than 2^31 slots, and a max_context_len of up to PKV_WINDOW_MAX_CONTEXT. `out` and `workspace`
+ * must not overlap an input, and calls that may run at the same time need workspaces of their own.
  * Scores, softmax and sums are float32; a bfloat16 output is rounded once.
  */
 #define PKV_WINDOW_MAX_GROUP 64
 #define PKV_WINDOW_MAX_SPLITS 64
 #define PKV_WINDOW_MIN_RUN 4
+#define PKV_WINDOW_MAX_CONTEXT (1 << 30)
 
 typedef struct pkv_window {
   void* out;

@@ -135,7 +135,7 @@ __device__ __forceinline__ int64_t split_index(const Window& a, int64_t t, int32
   return (t * a.num_heads + head) * a.splits + split;
 }
 __device__ __forceinline__ float* split_acc(const Window& a, int64_t index, int d) {
-  return a.workspace + 2 * a.num_queries * a.num_heads * a.splits + index * d;
+  return a.workspace + (2 * a.num_queries * a.num_heads * a.splits + 3) / 4 * 4 + index * d;  // 16-byte aligned
 }
 __device__ __forceinline__ void store_split_sums(const Window& a, int64_t index, float top, float sum) {
   a.workspace[index] = top;
@@ -1217,7 +1217,8 @@ extern "C" int pkv_window_attention(const pkv_window* args, int device, void* st
   if (g.q_dtype == PKV_BF16 && g.kv_dtype == PKV_F32) return PKV_EUNSUPPORTED;
   if (g.head_dim != 32 && g.head_dim != 64 && g.head_dim != 128 && g.head_dim != 256) return PKV_EUNSUPPORTED;
   if (g.num_heads / g.num_kv_heads > PKV_WINDOW_MAX_GROUP) return PKV_EUNSUPPORTED;
-  if (g.num_blocks * g.block_size > 0x7fffffff) return PKV_EUNSUPPORTED;  // slots are 32-bit
+  // Slots, and a span's items some tiles past its end, are 32-bit.
+  if (g.num_blocks > 0x7fffffff / g.block_size || g.max_context_len > PKV_WINDOW_MAX_CONTEXT) return PKV_EUNSUPPORTED;
   if (g.num_queries == 0) return PKV_OK;
   if (!g.out || !g.queries || !g.query_positions || !g.query_seq || !g.key_cache || !g.value_cache || !g.block_tables ||
       !g.context_lens) {

@@ -479,7 +479,7 @@ def sample_tokens(
         raise ValueError("top_p must be in (0, 1]")
     if not min_ps and not 0 <= min_p <= 1:
         raise ValueError("min_p must be in [0, 1]")
-    if vocab > 1 and logits.stride(1) != 1:
+    if (vocab > 1 and logits.stride(1) != 1) or (rows > 1 and logits.stride(0) < vocab):
         logits = logits.contiguous()
     if out is None:
         out = uniforms.new_empty((rows,), dtype=torch.int32)
@@ -1474,10 +1474,11 @@ def paged_attention_window(
 
     ``max_query_len`` (default: T) bounds how many rows one sequence has next to each other: 1 for
     a decode batch. With ``num_splits`` (default: the library's choice) it only decides how the call
-    runs. ``workspace``: float32 scratch of :func:`window_workspace_bytes` bytes, allocated when None.
-    Returns ``[T, heads, head_dim]`` of the queries' dtype. The call needs no plan and no host
-    reading of the batch, so it can be captured into a graph whose batch changes from replay to
-    replay (within T, S, ``max_context_len`` and ``max_query_len``).
+    runs. ``workspace``: float32 scratch of :func:`window_workspace_bytes` bytes, allocated when None;
+    calls that may run at the same time need their own. ``out`` must not overlap an input. Returns
+    ``[T, heads, head_dim]`` of the queries' dtype. The call needs no plan and no host reading of the
+    batch, so it can be captured into a graph whose batch changes from replay to replay (within T, S,
+    ``max_context_len`` and ``max_query_len``).
     """
     device = _one_device(queries, query_positions, query_seq, key_cache, value_cache, block_tables, context_lens)
     io, kv, shape, cache = queries.dtype, key_cache.dtype, queries.shape, key_cache.shape

@@ -269,3 +269,9 @@ def test_refusals(device):
     for logits, uniforms in ((x.half(), u), (x[0], u), (x, u[:1]), (x, u.double()), (x[:, :0], u), (x.cpu(), u), (x, u.cpu())):
         with pytest.raises(ValueError):
             ops.sample_tokens(logits, uniforms)
+
+
+def test_one_row_expanded_over_the_batch(device):
+    logits, _ = make(1, 300, 8)
+    uniforms = np.linspace(0, 0.99, 7, dtype=np.float32)
+    assert draw(device, logits.to(device).expand(7, 300), uniforms).tolist() == expect(logits.expand(7, 300), uniforms).tolist()
