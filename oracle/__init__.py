@@ -14,6 +14,8 @@ Modules:
     model      -- the fp32 decoder math and the cache-free recompute (model.py:43-288)
     runner     -- slots, append, copy-on-write and the paged forward (runner.py:95-227)
     bf16       -- round-to-nearest-even float32 -> bfloat16 for the bf16-KV tolerance oracle
+    window     -- attention with a sliding window and sinks for grouped heads, axes of rotary frequencies
+    sampling   -- a token by temperature, top-k, min-p, top-p and a given uniform (sampling.py:56-74)
 
 Each function is pinned (closed forms, invariants, brute force on tiny inputs, planted mistakes)
 by ``tests/test_oracle_*.py``.
