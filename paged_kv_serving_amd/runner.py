@@ -49,6 +49,8 @@ DEFAULT_TILE_BLOCKS = 8
 
 _NO_ROWS = np.zeros(0, dtype=np.int64)  # no logits rows (read only)
 _NO_ROWS.flags.writeable = False
+_NO_PLAN = np.zeros(0, dtype=np.int32)  # no plan rows, tiles or merges (read only)
+_NO_PLAN.flags.writeable = False
 
 
 @dataclass(frozen=True, slots=True)
@@ -498,6 +500,50 @@ class ModelRunner:
         picked = tokens.cpu().numpy()
         return {name: int(picked[i]) for i, name in enumerate(names)}
 
+    def execute_sampled(
+        self, batch: ExecutionBatch, uniforms, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0
+    ) -> dict[str, int]:
+        """:meth:`execute` followed by :func:`ops.sample_tokens` on the device: a token id for each
+        logits row, one int32 per row copied to the host (reference sampling.py:56-74).
+
+        ``uniforms``: one number in [0, 1) per entry that asks for logits, in batch order, from the
+        caller's generator. Each setting is a number or a sequence with one entry per such row."""
+        rows = sum(entry.logits_index is not None for entry in batch.entries)
+        drawn = np.asarray(uniforms, dtype=np.float64)
+        if drawn.shape != (rows,):
+            raise ValueError(f"uniforms must have one entry per logits row ({rows})")
+        if not ((drawn >= 0) & (drawn < 1)).all():
+            raise ValueError("uniforms must be in [0, 1)")
+        # What rounds up to one is the largest float32 below it.
+        parts = [np.minimum(drawn.astype(np.float32), np.nextafter(np.float32(1), np.float32(0)))]
+        settings = {"temperature": temperature, "top_k": top_k, "top_p": top_p, "min_p": min_p}
+        at = {}
+        for name, value in settings.items():
+            array = np.asarray(value)
+            if name == "top_k" and array.dtype.kind not in "iu":
+                raise ValueError("top_k must be whole numbers")
+            low = {"temperature": array >= 0, "top_k": array >= 0, "top_p": array > 0, "min_p": array >= 0}[name]
+            if not (low & (array <= (1 if name in ("top_p", "min_p") else np.inf))).all():
+                raise ValueError(f"{name} is out of range")
+            if array.ndim == 0:
+                settings[name] = array.item()
+                continue
+            if array.shape != (rows,):
+                raise ValueError(f"{name} must be a number or have one entry per logits row ({rows})")
+            at[name] = len(parts)
+            if name == "top_k":
+                parts.append(np.minimum(array, np.iinfo(np.int32).max).astype(np.int32).view(np.float32))
+            else:
+                parts.append(array.astype(np.float32))
+        names, logits = self._forward(batch)
+        if not names:
+            return {}
+        sent = torch.from_numpy(np.stack(parts)).to(self.device)  # one copy
+        for name, part in at.items():
+            settings[name] = sent[part].view(torch.int32) if name == "top_k" else sent[part]
+        picked = ops.sample_tokens(logits, sent[0], **settings).cpu().numpy()
+        return {name: int(picked[i]) for i, name in enumerate(names)}
+
     def _gather(self, entries):
         """One C++ walk over the entries (``_pkvhost.gather``): token ids, positions and slots
         (batch order, int64), per-entry lengths, context lengths (int32) and flat logits rows (-1:
@@ -522,11 +568,12 @@ class ModelRunner:
         return (tokens[:total], positions[:total], slots[:total], lengths[:count], contexts[:count],
                 logits[:count], (problem, entry, position))  # fmt: skip
 
-    def _prepare(self, batch: ExecutionBatch, *, logits: bool = True) -> _Step | None:
+    def _prepare(self, batch: ExecutionBatch, *, logits: bool = True, plan: bool = True) -> _Step | None:
         """Everything one iteration needs on the device before its first kernel: validation in
         the reference's order and with its messages, slots, the block-table arena update, the
         attention plan, and one asynchronous copy of all of it (None for an empty batch). Without
-        ``logits`` (attend, which computes none) no logits rows are listed."""
+        ``logits`` (attend, which computes none) no logits rows are listed; without ``plan``
+        (windowed attention, which needs none) rows stay in batch order and none is made."""
         entries = batch.entries
         if not entries:
             return None
@@ -571,7 +618,7 @@ class ModelRunner:
         # batch where two decode entries start in the same block can have such entries; the
         # order is read from the arena's rows, which hold every table as int32 by now.
         order = None
-        if repeats:
+        if repeats and plan:
             if self._order.size < len(entries):
                 self._order = np.zeros(max(len(entries), 2 * self._order.size), np.int64)
             if self._host.prefix_order_rows(
@@ -601,11 +648,16 @@ class ModelRunner:
         contexts_by_row[rows] = context
         query_seq = rows if total == len(entries) else np.repeat(rows, lengths)
         query_pos = positions.astype(np.int32)
-        plan_rows, plan_tiles, merge, partition, flags = self._planner.plan_views(
-            query_seq, query_pos, self._tables.host, contexts_by_row, self.block_size, config.n_heads,
-            config.head_dim, self.partition_size, kv_dtype=self._keys.dtype,
-        )  # fmt: skip
-        self._last_plan = (plan_rows, plan_tiles, partition, flags, merge)
+        if plan:
+            plan_rows, plan_tiles, merge, partition, flags = self._planner.plan_views(
+                query_seq, query_pos, self._tables.host, contexts_by_row, self.block_size, config.n_heads,
+                config.head_dim, self.partition_size, kv_dtype=self._keys.dtype,
+            )  # fmt: skip
+            self._last_plan = (plan_rows, plan_tiles, partition, flags, merge)
+        else:
+            plan_rows = plan_tiles = merge = _NO_PLAN
+            partition = flags = 0
+            self._last_plan = None
         parts64 = [tokens, rope_positions, slots, update.index, wanted]
         parts32 = [query_pos, query_seq, contexts_by_row, update.values, plan_rows.ravel(), plan_tiles.ravel(), merge]
         if token_order is not None:  # attend's caller rows, and its slots in batch order
@@ -629,7 +681,7 @@ class ModelRunner:
         # path. Tiles may stay: only the row pass appends, so no tile may cover a row's new
         # position, which exclusive_writes also checks (a decode batch's tiles are shared-prefix
         # tiles, and a written block that one row alone reads lies past every shared prefix).
-        decode_only = len(entries) == total and self._host.exclusive_writes(
+        decode_only = plan and len(entries) == total and self._host.exclusive_writes(
             rows, context, self._tables.host, self.block_size, self._marks, plan_tiles, partition
         )  # fmt: skip
         return _Step(
@@ -692,18 +744,25 @@ class ModelRunner:
 
     def attend(
         self, batch: ExecutionBatch, queries: torch.Tensor, keys: torch.Tensor, values: torch.Tensor,
-        *, layer: int = 0, out: torch.Tensor | None = None,
+        *, layer: int = 0, window: int | None = None, sinks: int = 0, out: torch.Tensor | None = None,
     ) -> torch.Tensor:  # fmt: skip
         """The KV data path of one layer for caller-computed projections: the batch's keys and
         values (float32 ``[T, heads, head_dim]``, rotated already, in batch token order) are
         written at its slots and every query attends over its entry's block table
         (reference runner.py:184-212 for one layer). Returns float32 ``[T, heads, head_dim]`` in
         batch order, on the device (asynchronous). A decode batch (one token per entry, at its
-        last position) appends inside the attention call."""
+        last position) appends inside the attention call.
+
+        With ``window`` (and ``sinks``) a query at position p sees only the keys ``j > p - window`` or
+        ``j < sinks`` of those (:func:`ops.paged_attention_window`), after the append."""
         config = self.model.config
         if not 0 <= layer < config.n_layers:
             raise IndexError(f"layer {layer} is outside the model's {config.n_layers} layers")
-        step = self._prepare(batch, logits=False)
+        if window is None and sinks:
+            raise ValueError("sinks need a window")
+        if window is not None and (window < 1 or sinks < 0):
+            raise ValueError("window must be >= 1 and sinks >= 0")
+        step = self._prepare(batch, logits=False, plan=window is None)  # batch order without a plan
         total = 0 if step is None else step.total
         shape = (total, config.n_heads, config.head_dim)
         if out is None:
@@ -731,8 +790,22 @@ class ModelRunner:
                 self._device_index, ops._stream(self._device_index),
             )  # fmt: skip
             _native.check(rc, "pkv_append")
-            self._attention(step, layer, queries, out)
+            if window is None:
+                self._attention(step, layer, queries, out)
+            else:
+                self._window_attention(step, layer, queries, out, window, sinks)
         return out
+
+    def _window_attention(self, step: _Step, layer: int, queries, out, window: int, sinks: int) -> None:
+        """:func:`ops.paged_attention_window` of the step's rows, which are in batch order."""
+        staging, tables = step.staging, self._tables.tables
+        ops.paged_attention_window(
+            queries, staging.tensor(step.qpos_at, step.total, torch.int32),
+            staging.tensor(step.qseq_at, step.total, torch.int32), self._keys[layer], self._values[layer], tables,
+            staging.tensor(step.contexts_at, tables.shape[0], torch.int32), float(self.model.attention_scale),
+            window=window, sinks=sinks, max_context_len=step.max_context,
+            max_query_len=max(entry.num_tokens for entry in step.entries), out=out,
+        )  # fmt: skip
 
     def _forward(self, batch: ExecutionBatch, *, greedy: bool = False):
         """The forward pass of one iteration: (seq ids of the entries that ask for logits, in
