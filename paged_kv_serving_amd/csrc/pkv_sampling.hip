@@ -450,6 +450,59 @@ __device__ __forceinline__ uint64_t place_of(float u, uint64_t mass) {
   return at < mass ? at + 1 : mass;
 }
 
+// The end of top-p and the draw from one pass over the tokens; -1 where they do not fit the list. `mass` is
+// what top-k leaves. The nucleus ends in bin `edge`, with a mass between `target` and `most`, and so the draw
+// falls into one of the bins [first, last] (one or two as a rule), none of them behind the edge's. One pass
+// less: 256 rows of 128256 tokens with top_p 93 -> 77 us, 2 rows of 1000 11.2 -> 10.2.
+template <typename T>
+__device__ __forceinline__ int32_t nucleus_and_draw(Shared& s, const Row& r, const Source<T>& source, uint64_t target, uint64_t mass,
+                                                    float u) {
+  __syncthreads();
+  if (threadIdx.x == 0) s.listed = 0;
+  __syncthreads();
+  const int32_t edge = bin_reaching(s.mass, target);
+  const uint64_t most = min(s.mass[edge + 1], mass);
+  const int32_t first = bin_reaching(s.mass, place_of(u, target)), last = bin_reaching(s.mass, place_of(u, most));
+  // No token weighs less than 2^(-1 / 256) of its bin's middle, so masses say how many they are at most.
+  const auto tokens_of = [&](int32_t from, int32_t to) {
+    return static_cast<float>(s.mass[to + 1] - s.mass[from]) * exp2f((to + 0.5f) * (1.f / kPerOctave)) / static_cast<float>(r.power[0]);
+  };
+  if (tokens_of(first, last) + (edge > last ? tokens_of(edge, edge) : 0.f) > kList) return -1;
+  const float floor = floor_of_bin(r, edge), ceiling = ceiling_of_bin(r, edge);
+  const float draw_floor = floor_of_bin(r, last), draw_ceiling = ceiling_of_bin(r, first);
+  source.template each<4>([&](float v, int32_t i) {
+    if (!((v >= floor && v <= ceiling) || (v >= draw_floor && v <= draw_ceiling))) return;
+    const uint32_t at = atomicAdd(&s.listed, 1u);
+    if (at < kList) s.list[at] = order_of(key_of(v), i);
+  });
+  __syncthreads();
+  const uint32_t listed = s.listed;
+  if (listed > kList) return -1;
+  // Between a bin's bounds lie some tokens of the bins beside it: these turn into one behind all others.
+  Weight own{-1, 0};
+  if (threadIdx.x < listed) {
+    own = weigh<true>(r, float_of(static_cast<uint32_t>(s.list[threadIdx.x] >> 32)));
+    if (own.bin != edge && (own.bin < first || own.bin > last)) own.mass = 0;
+    if (own.mass == 0) s.list[threadIdx.x] = 0;
+    s.list_mass[threadIdx.x] = own.mass;
+  }
+  __syncthreads();
+  rank_list<true>(s, s.list, listed);
+  // Cumulative masses: of what is not in the list, the bins before the first come before the draw's tokens,
+  // those between them and the edge's before the edge's too.
+  uint64_t before = 0;
+  if (own.mass != 0) {
+    before = s.before[threadIdx.x] + s.mass[first];
+    if (own.bin > last) before += s.mass[edge] - s.mass[last + 1];
+    if (before < target && target <= before + own.mass) s.found_mass = before + own.mass;
+  }
+  __syncthreads();
+  const uint64_t place = place_of(u, s.found_mass);
+  if (before < place && place <= before + own.mass) s.found = static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(s.list[threadIdx.x]));
+  __syncthreads();
+  return s.found;
+}
+
 // The whole row's answer from the `listed` <= kFew tokens of its list, which hold every token that the
 // cuts can keep: put in order by counting, then summed up along the order, a token per thread.
 __device__ __forceinline__ int32_t from_list(Shared& s, const Row& r, uint32_t listed, int32_t top_k, float top_p, float u) {
@@ -498,13 +551,17 @@ __device__ __forceinline__ int32_t from_bins(Shared& s, const Row& r, const Sour
   scan_bins(s, s.mass, [](uint64_t mass, int) { return mass; });
   if (counting) scan_bins(s, s.count, [](uint32_t count, int) { return count; });
 
-  // Three times the same search: the end of top-k, of top-p, and the draw.
+  // The end of top-k, then that of top-p and the draw: together, or where that fails one after the other.
   uint64_t mass = s.mass[kBins];
-  const bool cut = counting && s.count[kBins] > static_cast<uint32_t>(top_k);
-  int32_t token = 0;
+  const bool cut = counting && s.count[kBins] > static_cast<uint32_t>(top_k), nuclear = !(top_p >= 1.f);
+  int32_t token = -1;
   for (int step = 0; step < 3; ++step) {
-    if ((step == 0 && !cut) || (step == 1 && top_p >= 1.f)) continue;
+    if ((step == 0 && !cut) || (step == 1 && !nuclear)) continue;
     const uint64_t target = step == 0 ? static_cast<uint64_t>(top_k) : step == 1 ? nucleus(top_p, mass) : place_of(u, mass);
+    if (step == 1) {
+      token = nucleus_and_draw(s, r, source, target, mass, u);
+      if (token >= 0) break;
+    }
     const Place place = locate(s, r, source, step == 0, target);
     mass = place.mass;
     token = place.index;

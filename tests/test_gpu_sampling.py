@@ -275,3 +275,14 @@ def test_one_row_expanded_over_the_batch(device):
     logits, _ = make(1, 300, 8)
     uniforms = np.linspace(0, 0.99, 7, dtype=np.float32)
     assert draw(device, logits.to(device).expand(7, 300), uniforms).tolist() == expect(logits.expand(7, 300), uniforms).tolist()
+
+
+@pytest.mark.parametrize("spread", [0.3, 1.0, 3.0, 12.0])
+@pytest.mark.parametrize("more", [{}, {"top_k": 6000}, {"min_p": 1e-4}], ids=str)
+def test_the_nucleus_end_and_the_draw_wherever_they_lie(device, more, spread):
+    """From the draw in front of everything to the draw of the nucleus's last token."""
+    settings = [(u, p) for u in (0.0, 0.02, 0.5, 0.97, np.nextafter(np.float32(1), np.float32(0))) for p in (0.02, 0.5, 0.9, 0.9999)]
+    logits, _ = make(len(settings), 20011, 77, spread)
+    uniforms = np.asarray([u for u, _ in settings], np.float32)
+    more = {**more, "top_p": np.asarray([p for _, p in settings], np.float32)}
+    assert draw(device, logits, uniforms, **more).tolist() == expect(logits, uniforms, **more).tolist()
