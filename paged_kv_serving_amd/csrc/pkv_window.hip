@@ -46,9 +46,10 @@ struct Window {
   int32_t window, sinks, max_context, splits;
   int32_t subgroups;       // of up to 16 query heads of a group
   int32_t tile_rows;       // rows of a tile: the aligned blocks of rows that runs lie in
+  uint32_t tile_items;     // workgroups with tiles; the others have rows
   int32_t tiled;           // whether the tile pass computes the runs
   int32_t min_run;         // rows of one sequence next to each other that a tile takes
-  int32_t* list;           // the rows that no tile takes (list_rows); NULL without tiles
+  int32_t* list;           // the rows that no tile takes (list_kernel); NULL without tiles
   float scale_log2;  // scale * log2(e): scores are kept in base 2
   float given_scale;  // the same before the next two
   // A negative scale of bfloat16 queries turns their signs instead, so that the largest product is the
@@ -285,12 +286,14 @@ __device__ __forceinline__ Words<N> load_words(const void* p) {
 
 // The rows that no tile computes, in order: list[0] is their number. A tile takes the runs of a.min_run
 // rows or more of one sequence next to each other inside an aligned block of a.tile_rows rows; rows
-// outside every sequence are left out. One workgroup writes it.
-__device__ __forceinline__ void list_rows(const Window& a) {
-  __shared__ int32_t s_count[kWaves];
+// outside every sequence are left out. One workgroup, 4 us for 4096 rows: a workgroup per possible row
+// that finds out for itself took 48 us of a prefill of 8 x 512 rows.
+constexpr int kListThreads = 1024;
+__global__ __launch_bounds__(kListThreads) void list_kernel(const Window a) {
+  __shared__ int32_t s_count[kListThreads / kWave];
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   int32_t found = 0;
-  for (int64_t start = 0; start < a.num_queries; start += kThreads) {
+  for (int64_t start = 0; start < a.num_queries; start += kListThreads) {
     const int64_t t = start + threadIdx.x;
     bool listed = false;
     if (t < a.num_queries) {
@@ -311,7 +314,7 @@ __device__ __forceinline__ void list_rows(const Window& a) {
     if (lane == 0) s_count[wave] = __popcll(ballot);
     __syncthreads();
     int32_t at = found + __popcll(ballot & ((1ull << lane) - 1));
-    for (int w = 0; w < kWaves; ++w) {
+    for (int w = 0; w < kListThreads / kWave; ++w) {
       at += w < wave ? s_count[w] : 0;
       found += s_count[w];
     }
@@ -321,13 +324,23 @@ __device__ __forceinline__ void list_rows(const Window& a) {
   if (threadIdx.x == 0) a.list[0] = found;
 }
 
+// What a workgroup of the row pass keeps in LDS.
+template <int D, int kRowWaves, int kPair>
+struct RowScratch {
+  float acc[kPair][kRowWaves / 2][D / 16 * 4 * kWave];
+  float top[kPair][kRowWaves][kWave], sum[kPair][kRowWaves][kWave];
+  int redo[kPair];
+};
+
+// The items of workgroup `block` of `blocks`.
 template <typename QT, typename KVT, int D, int kRowWaves, int kPair>
-__global__ __launch_bounds__(kRowWaves * kPair * kWave) void row_kernel(const Window a) {
+__device__ __forceinline__ void row_pass(const Window& a, RowScratch<D, kRowWaves, kPair>& shared, uint32_t block, uint32_t blocks) {
   using S = RowShape<QT, KVT, D>;
   constexpr int kTiles = D / 16;  // output tiles of 16 dimensions
-  __shared__ float s_acc[kPair][kRowWaves / 2][kTiles * 4 * kWave];
-  __shared__ float s_top[kPair][kRowWaves][kWave], s_sum[kPair][kRowWaves][kWave];
-  __shared__ int s_redo[kPair];
+  auto& s_acc = shared.acc;
+  auto& s_top = shared.top;
+  auto& s_sum = shared.sum;
+  auto& s_redo = shared.redo;
   const int lane = threadIdx.x & (kWave - 1), c = lane / 16, n = lane % 16;
   const int side = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave % kPair);  // which key head of the pair
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave / kPair);
@@ -335,7 +348,7 @@ __global__ __launch_bounds__(kRowWaves * kPair * kWave) void row_kernel(const Wi
   // Items: heads fastest, so that one XCD has its share of the heads of every row.
   const int64_t rows = a.tiled ? a.list[0] : a.num_queries;
   const int64_t items = rows * a.splits * a.subgroups * head_groups;
-  for (int64_t next = blockIdx.x; next < items; next += gridDim.x) {
+  for (int64_t next = block; next < items; next += blocks) {
     uint32_t item = static_cast<uint32_t>(next);
     const int32_t kv_head = item % head_groups * kPair + side;
     item /= head_groups;
@@ -607,6 +620,12 @@ __global__ __launch_bounds__(kRowWaves * kPair * kWave) void row_kernel(const Wi
   }
 }
 
+template <typename QT, typename KVT, int D, int kRowWaves, int kPair>
+__global__ __launch_bounds__(kRowWaves * kPair * kWave) void row_kernel(const Window a) {
+  __shared__ RowScratch<D, kRowWaves, kPair> shared;
+  row_pass<QT, KVT, D, kRowWaves, kPair>(a, shared, blockIdx.x, gridDim.x);
+}
+
 // ---------------------------------------------------------------------------------------------
 // Runs of rows (prompt chunks): one workgroup per (aligned block of rows, key head, split), whose
 // kTileQueries = 128 queries are the block's rows times the heads that share the key head, 32 to a
@@ -740,11 +759,16 @@ __global__ __launch_bounds__(kThreads, (TileShape<QT, KVT, D>::kWaves)) void til
   __shared__ uint64_t s_live[3];
   const int tid = threadIdx.x, lane = tid & (kWave - 1), c = lane / 32, n = lane % 32;
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-  if (blockIdx.x == 0) {  // for the row pass, which comes next
-    list_rows(a);
+  // The rows outside the runs in the same launch, before bfloat16's tiles and behind float32's, which take
+  // longer (24 rows of up to 4000 keys beside 2 x 301, 16 heads x 64, float32: in a launch of their own 70 us,
+  // before the tiles 63, behind them 52; 64 of up to 8000 beside 512, 32/8 heads x 128, bfloat16: 243, 236, 267).
+  constexpr bool kRowsFirst = sizeof(QT) == 2;
+  const uint32_t row_blocks = gridDim.x - a.tile_items, before = kRowsFirst ? row_blocks : a.tile_items;
+  if ((blockIdx.x < before) == kRowsFirst) {
+    row_pass<QT, KVT, D, kWaves, 1>(a, *reinterpret_cast<RowScratch<D, kWaves, 1>*>(s_kv), blockIdx.x - (kRowsFirst ? 0 : before), row_blocks);
     return;
   }
-  uint32_t item = blockIdx.x - 1;
+  uint32_t item = blockIdx.x - (kRowsFirst ? before : 0);
   const int32_t kv_head = item % static_cast<uint32_t>(a.num_kv_heads);
   item /= static_cast<uint32_t>(a.num_kv_heads);
   const int32_t split = item % static_cast<uint32_t>(a.splits);
@@ -1115,25 +1139,33 @@ int launch(Window a, hipStream_t stream) {
   a.min_run = std::min(kMinRun, a.tile_rows);
   a.tiled = S::kFits && a.list;
   const int64_t items = a.num_queries * a.num_kv_heads * a.subgroups * a.splits;
-  // Beside tiles the number of rows is known on the device only.
-  const int64_t groups = a.tiled ? std::min<int64_t>(items, 1024) : items;
+  // Beside tiles the number of rows is known on the device only: two workgroups for every CU share them.
+  const int64_t groups = a.tiled ? std::min<int64_t>(items, 512) : items;
   const int64_t tiles = (a.num_queries + a.tile_rows - 1) / a.tile_rows * a.num_kv_heads * a.splits;
   const int64_t joins = (a.num_queries * a.num_heads * (D / 4) + kThreads - 1) / kThreads;
   if (items > 0x7fffffff || joins > 0x7fffffff || tiles >= 0x7fffffff) return PKV_EUNSUPPORTED;
+  const auto join = [&]() {
+    if (a.splits > 1) hipLaunchKernelGGL((join_kernel<QT, D>), dim3(static_cast<uint32_t>(joins)), dim3(kThreads), 0, stream, a);
+  };
   if constexpr (S::kFits) {
     if (a.tiled) {
+      static_assert(sizeof(RowScratch<D, kWaves, 1>) <= S::kLds, "the row pass's part fits");
       if (hipFuncSetAttribute(reinterpret_cast<const void*>(tile_kernel<QT, KVT, D>), hipFuncAttributeMaxDynamicSharedMemorySize,
                               S::kLds) != hipSuccess) {
         return PKV_EHIP;
       }
-      hipLaunchKernelGGL((tile_kernel<QT, KVT, D>), dim3(static_cast<uint32_t>(tiles + 1)), dim3(kThreads), S::kLds, stream, a);
+      a.tile_items = static_cast<uint32_t>(tiles);
+      hipLaunchKernelGGL(list_kernel, dim3(1), dim3(kListThreads), 0, stream, a);
+      hipLaunchKernelGGL((tile_kernel<QT, KVT, D>), dim3(static_cast<uint32_t>(tiles + groups)), dim3(kThreads), S::kLds, stream, a);
+      join();
+      return check_launch();
     }
   }
   // Few workgroups are of eight wavefronts (1 row, 2 key heads x 64, 516 keys: 11.4 -> 10.3 us; 4 x 4100 keys, 8
   // splits: 28.4 -> 26.7; 64 rows 203 -> 208). Where there are many and a key row is short, one of eight serves two
   // neighbouring key heads, and so reads twice as much next to each other. head_dim 256 needs the registers of four.
   constexpr bool kShort = D * sizeof(KVT) <= 256;
-  const bool wide = D <= 128 && groups <= 256 && !a.tiled;
+  const bool wide = D <= 128 && groups <= 256;
   const bool pair = kShort && groups >= 512 && a.num_kv_heads % 2 == 0;
   const auto start = [&](auto kernel, int64_t count, int waves) {
     hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(count)), dim3(waves * kWave), 0, stream, a);
@@ -1142,12 +1174,10 @@ int launch(Window a, hipStream_t stream) {
     if (wide) start(row_kernel<QT, KVT, D, 8, 1>, groups, 8);
   }
   if constexpr (kShort) {
-    if (pair) start(row_kernel<QT, KVT, D, 4, 2>, a.tiled ? groups : groups / 2, 8);
+    if (pair) start(row_kernel<QT, KVT, D, 4, 2>, groups / 2, 8);
   }
   if (!wide && !pair) start(row_kernel<QT, KVT, D, 4, 1>, groups, 4);
-  if (a.splits > 1) {
-    hipLaunchKernelGGL((join_kernel<QT, D>), dim3(static_cast<uint32_t>(joins)), dim3(kThreads), 0, stream, a);
-  }
+  join();
   return check_launch();
 }
 
