@@ -680,7 +680,7 @@ int pkv_window_attention(const pkv_window* args, int device, void* stream);
  *                 name is given, one for each row (float32, top_k int32). A temperature of 0 or below
  *                 (or NaN) takes the greedy token. A top_p of 0 or below (or NaN) keeps the first
  *                 token; a min_p above 1 does too, one of 0 or below (or NaN) keeps all.
- * A token of -inf is never drawn; tokens of +inf share the whole mass. A row with a NaN, or with
+ * Up to 2^22 - 1 rows. A token of -inf is never drawn; tokens of +inf share the whole mass. A row with a NaN, or with
  * nothing above -inf, yields its greedy token.
  */
 #define PKV_SAMPLE_BITS 46

@@ -8,8 +8,11 @@
 //     out[j] = x[j] for j >= R
 // in float32, each product and sum rounded on its own, and one rounding to the output's type.
 //
-// Bound: HBM, every q, k, v element read once and written once. The tables are read once per token
-// from the caches: the heads of a token lie in one workgroup or in neighbouring ones.
+// Bound: HBM, every q, k, v element read once and written once; the tables come from the caches. Two
+// heads per thread share their table entries and have four loads in flight, and what is read once goes past
+// the caches. 4216 tokens of 32 + 2 * 32 heads x 128 in float32, 417 MB: 63 us, 6.6 TB/s, where the pools lie
+// in the caches, 82 us, 5.1 TB/s, with other tensors each time (a copy of 4 GiB: 4.8 TB/s). 16384 tokens of
+// 32 + 2 * 4 heads x 128 in bfloat16 with three axes, 345 MB: 67 us, 5.1 TB/s. 4 tokens: 4.0 us, a launch.
 #include "pkv_common.h"
 
 namespace pkv {

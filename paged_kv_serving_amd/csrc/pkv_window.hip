@@ -249,6 +249,11 @@ __device__ __forceinline__ void exact_row(const Window& a, int64_t t, int32_t he
 // in float32 throughout, and all heads of a group share one read of it. The loads of the next keys are
 // issued before the present ones are used (a second set of registers for the values, so that they too
 // are a whole round ahead, measured 3 to 5% slower).
+//
+// Bound: HBM. 64 rows with contexts of 2048 to 16384 and a window of 4096, 32 heads on 8 x 128, bfloat16, 1.1 GB:
+// 180 us, 6.0 TB/s; contexts of 512 to 4096 and a window of 1024, 32 x 128 heads in float32, 2.2 GB: 345 us, 6.3
+// TB/s (only reading one head's rows at a time in that pattern: 5.4).
+// One row of 2 key heads x 64 and 516 keys: 10.3 us, the latency of a few dependent loads.
 // ---------------------------------------------------------------------------------------------
 template <typename QT, typename KVT, int D>
 struct RowShape {
@@ -647,6 +652,11 @@ __global__ __launch_bounds__(kRowWaves * kPair * kWave) void row_kernel(const Wi
 // Keys and values are staged kKeys at a time in two LDS buffers: while one is used, the next tile's rows
 // are in flight (bfloat16 pools: straight to LDS; float32 pools: to registers, cut on their way to LDS) and
 // the slots of the one after are looked up.
+//
+// Bound: latency. 8 x 512 rows behind 2048 others, window 1024, 32 heads on 8 x 128, bfloat16: 137 us, 500 TFLOP/s of visible
+// products (1390 in a large library product); the matrix units are busy 27% of it, vector instructions
+// issue in 29% and LDS works in 20%, at two wavefronts per SIMD. One piece of P instead of two
+// was 9% faster.
 // ---------------------------------------------------------------------------------------------
 template <typename QT, typename KVT, int D>
 struct TileShape {
@@ -762,8 +772,8 @@ __global__ __launch_bounds__(kThreads, (TileShape<QT, KVT, D>::kWaves)) void til
   const int tid = threadIdx.x, lane = tid & (kWave - 1), c = lane / 32, n = lane % 32;
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   // The rows outside the runs in the same launch, before bfloat16's tiles and behind float32's, which take
-  // longer (24 rows of up to 4000 keys beside 2 x 301, 16 heads x 64, float32: in a launch of their own 70 us,
-  // before the tiles 63, behind them 52; 64 of up to 8000 beside 512, 32/8 heads x 128, bfloat16: 243, 236, 267).
+  // longer (24 rows beside 2 x 301, window 500, 16 heads x 64, float32 over bfloat16: in a launch of their own 70
+  // us, before the tiles 63, behind them 52; 64 of up to 4096 keys beside 512, 32/8 heads x 128, bfloat16: 243, 236, 267).
   constexpr bool kRowsFirst = sizeof(QT) == 2;
   const uint32_t row_blocks = gridDim.x - a.tile_items, before = kRowsFirst ? row_blocks : a.tile_items;
   if ((blockIdx.x < before) == kRowsFirst) {
@@ -1101,7 +1111,8 @@ __global__ __launch_bounds__(kThreads, (TileShape<QT, KVT, D>::kWaves)) void til
 }
 
 // ---------------------------------------------------------------------------------------------
-// Joins the splits of every row and head: D / 4 threads each, four dimensions a thread.
+// Joins the splits of every row and head: D / 4 threads each, four dimensions a thread. 5.1 us for 626 rows of
+// 16 heads x 64 in 2 to 3 splits, of which a launch is 2.
 // ---------------------------------------------------------------------------------------------
 template <typename QT, int D>
 __global__ __launch_bounds__(kThreads) void join_kernel(const Window a) {
@@ -1145,7 +1156,8 @@ int launch(Window a, hipStream_t stream) {
   const int64_t groups = a.tiled ? std::min<int64_t>(items, 512) : items;
   const int64_t tiles = (a.num_queries + a.tile_rows - 1) / a.tile_rows * a.num_kv_heads * a.splits;
   const int64_t joins = (a.num_queries * a.num_heads * (D / 4) + kThreads - 1) / kThreads;
-  if (items > 0x7fffffff || joins > 0x7fffffff || tiles >= 0x7fffffff) return PKV_EUNSUPPORTED;
+  constexpr int64_t kMost = 0xffffffffll / (2 * kThreads);  // workgroups whose threads, up to 512 each, 32 bits count
+  if (groups > kMost || joins > kMost || tiles > kMost - 512 || items > 0x7fffffff) return PKV_EUNSUPPORTED;
   const auto join = [&]() {
     if (a.splits > 1) hipLaunchKernelGGL((join_kernel<QT, D>), dim3(static_cast<uint32_t>(joins)), dim3(kThreads), 0, stream, a);
   };

@@ -1443,6 +1443,10 @@ def paged_attention_ragged(
 MAX_WINDOW_GROUP = 64
 #: Workgroups that can share a row's keys in :func:`paged_attention_window`.
 MAX_WINDOW_SPLITS = 64
+#: Head sizes it takes.
+WINDOW_HEAD_DIMS = (32, 64, 128, 256)
+
+
 def paged_attention_window(
     queries: torch.Tensor,
     query_positions: torch.Tensor,
@@ -1499,6 +1503,8 @@ def paged_attention_window(
         raise ValueError(f"at most {MAX_WINDOW_GROUP} query heads per key head")
     if kv == torch.float32 and io != torch.float32:
         raise ValueError("float32 caches need float32 queries")
+    if dim not in WINDOW_HEAD_DIMS:
+        raise ValueError(f"unsupported head_dim {dim}: it must be one of {WINDOW_HEAD_DIMS}")
     stride = _token_stride(queries, num_queries, heads, dim, "queries")
     for name, tensor in (("query_positions", query_positions), ("query_seq", query_seq)):
         if tensor.dtype != torch.int32 or tensor.shape != (num_queries,) or not tensor.is_contiguous():

@@ -762,6 +762,8 @@ class ModelRunner:
             raise ValueError("sinks need a window")
         if window is not None and (window < 1 or sinks < 0):
             raise ValueError("window must be >= 1 and sinks >= 0")
+        if window is not None and config.head_dim not in ops.WINDOW_HEAD_DIMS:  # before anything is appended
+            raise ValueError(f"a window needs a head_dim of {ops.WINDOW_HEAD_DIMS}")
         step = self._prepare(batch, logits=False, plan=window is None)  # batch order without a plan
         total = 0 if step is None else step.total
         shape = (total, config.n_heads, config.head_dim)

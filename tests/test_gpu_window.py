@@ -348,3 +348,13 @@ def test_no_rows_no_context_and_refusals(device):
     with pytest.raises(Exception, match="unsupported|implemented|shape"):
         call(device, odd, 4, 0)
     assert ops.window_workspace_bytes(4, 4, 2, 64, window=4, max_context_len=30, max_query_len=1, num_splits=1) == 0
+
+
+@pytest.mark.parametrize("io,kv", TYPES)
+@pytest.mark.parametrize("splits", [0, 3])
+def test_more_rows_beside_a_run_than_workgroups(device, io, kv, splits):
+    """Rows outside the runs share a fixed number of workgroups: here each has several."""
+    runs = [(1, 5 + 7 * i % 90) for i in range(180)]
+    runs[60:60] = [(30, 130)]
+    check(device, make(runs, 8, 8, 64, 16, io, kv, seed=12), 40, 2, num_splits=splits)
+    check(device, make([(30, 130), *runs], 16, 8, 32, 16, io, kv, seed=13), 40, 2, num_splits=splits, max_query_len=30)

@@ -207,6 +207,12 @@ def test_attend_refuses_a_window_that_is_none(device, model) -> None:
     for more in ({"sinks": 2}, {"window": 0}, {"window": 4, "sinks": -1}):
         with pytest.raises(ValueError, match="window"):
             runner.attend(batch, rows, rows, rows, **more)
+    narrow = ModelConfig(**{**MODEL, "n_heads": 4})  # head_dim 16
+    other = ModelRunner(LanguageModel(narrow, random_weights(narrow, seed=1)), num_blocks=4, block_size=8, device=device)
+    ones = torch.ones((3, 4, 16), device=device)
+    with pytest.raises(ValueError, match="head_dim"):
+        other.attend(batch, ones, ones, ones, window=4)
+    assert not other.key_cache.any()  # refused before the append
     assert runner.attend(ExecutionBatch(()), rows[:0], rows[:0], rows[:0], window=3).shape == (0, 2, 32)
 
 

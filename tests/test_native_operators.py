@@ -92,7 +92,7 @@ def test_window_refusals(lib, changes, code) -> None:
 @pytest.mark.parametrize("changes,code", [
     ({"num_rows": -1}, EINVAL), ({"vocab_size": 0}, EINVAL), ({"vocab_size": 1 << 31, "row_stride": 1 << 31}, EINVAL),
     ({"row_stride": 99}, EINVAL), ({"dtype": 2}, EINVAL), ({"token_ids": None}, EINVAL), ({"logits": None}, EINVAL),
-    ({"uniforms": None}, EINVAL), ({"num_rows": 1 << 31}, EUNSUPPORTED),
+    ({"uniforms": None}, EINVAL), ({"num_rows": 1 << 31}, EUNSUPPORTED), ({"num_rows": 1 << 22}, EUNSUPPORTED),
 ], ids=str)  # fmt: skip
 def test_sampling_refusals(lib, changes, code) -> None:
     assert refused(lib.pkv_sample_tokens, structure("pkv_sample"), SAMPLE, **changes) == code
