@@ -96,6 +96,8 @@
 //       The entry points of the same names, with every pointer, stream and handle passed as a
 //       Python int (0 for NULL) in the order of their C declarations (the last three: of the
 //       fields of their argument structs, then device and stream); returns the PKV_* code.
+//   one_device(*tensors) -> int
+//       The ordinal that get_device() of all of them gives (-1: on no device, or not on one).
 //   window_workspace(queries, heads, kv_heads, head_dim, window, sinks, max_context_len,
 //        max_query_len, splits) -> (splits, bytes)
 //       pkv_window_splits where `splits` is 0, and pkv_window_workspace_bytes.
@@ -1447,6 +1449,23 @@ struct Reader {
   }
 };
 
+PyObject* s_get_device;
+
+// The ordinal that get_device() of every argument gives, or -1 where they differ.
+PyObject* one_device(PyObject*, PyObject* const* args, Py_ssize_t count) {
+  long device = -1;
+  for (Py_ssize_t i = 0; i < count; ++i) {
+    PyObject* found = PyObject_CallMethodNoArgs(args[i], s_get_device);
+    if (found == nullptr) return nullptr;
+    const long one = PyLong_AsLong(found);
+    Py_DECREF(found);
+    if (one == -1 && PyErr_Occurred()) return nullptr;
+    if (i == 0) device = one;
+    if (one != device) return PyLong_FromLong(-1);
+  }
+  return PyLong_FromLong(device);
+}
+
 PyObject* rope_append_axes(PyObject*, PyObject* const* args, Py_ssize_t count) {
   pkv_rope_axes a{};
   int32_t device = 0;
@@ -1862,6 +1881,8 @@ PyMethodDef kMethods[] = {
     {"silu_mul", silu_mul, METH_VARARGS, "pkv_silu_mul with integer pointers."},
     {"rope_append", rope_append, METH_VARARGS, "pkv_rope_append with integer pointers."},
     {"append", append, METH_VARARGS, "pkv_append with integer pointers."},
+    {"one_device", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(one_device)), METH_FASTCALL,
+     "The ordinal of the tensors' device, or -1 where they lie on different ones or none."},
     {"rope_append_axes", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(rope_append_axes)), METH_FASTCALL,
      "pkv_rope_append_axes with integer pointers."},
     {"window_workspace", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(window_workspace)), METH_FASTCALL,
@@ -1888,6 +1909,7 @@ PyMODINIT_FUNC PyInit__pkvhost(void) {
   s_positions = PyUnicode_InternFromString("positions");
   s_block_table = PyUnicode_InternFromString("block_table");
   s_logits_index = PyUnicode_InternFromString("logits_index");
+  s_get_device = PyUnicode_InternFromString("get_device");
   kCopyQueueType.tp_basicsize = sizeof(CopyQueue);
   kCopyQueueType.tp_flags = Py_TPFLAGS_DEFAULT;
   kCopyQueueType.tp_doc = "CopyQueue(num_blocks): queued copy-on-write block copies, flushed as batched launches.";

@@ -76,13 +76,13 @@ def _device_index(*tensors: torch.Tensor) -> int:
 
 
 def _one_device(*tensors: torch.Tensor) -> int:
-    """:func:`_device_index` by the tensors' device ordinals (-1: not on a HIP device)."""
-    device = tensors[0].get_device()
-    if device < 0 or tensors[0].device.type != "cuda":
-        raise ValueError("the KV data path runs on a HIP device; got a tensor on " + str(tensors[0].device))
-    for tensor in tensors:
-        if tensor.get_device() != device:
-            raise ValueError("all tensors must be on the same device")
+    """:func:`_device_index`, by one call of the host extension."""
+    device = _host().one_device(*tensors)
+    if device < 0:
+        for tensor in tensors:
+            if tensor.device.type != "cuda":
+                raise ValueError("the KV data path runs on a HIP device; got a tensor on " + str(tensor.device))
+        raise ValueError("all tensors must be on the same device")
     return device
 
 
@@ -318,7 +318,7 @@ def rope_append_axes(
     k_stride = _token_stride(keys, tokens, kv_heads, dim, "keys")
     v_stride = _token_stride(values, tokens, kv_heads, dim, "values")
     if out is None:
-        out = queries.new_empty(shape)
+        out = torch.empty_like(queries, memory_format=torch.contiguous_format)
         out_stride = heads * dim
     elif out.shape != shape or out.dtype != io or out.device != queries.device:
         raise ValueError("out must match queries")
@@ -1524,7 +1524,7 @@ def paged_attention_window(
     if not 0 <= num_splits <= MAX_WINDOW_SPLITS:
         raise ValueError(f"num_splits must be in [0, {MAX_WINDOW_SPLITS}]")
     if out is None:
-        out = queries.new_empty(shape)
+        out = torch.empty_like(queries, memory_format=torch.contiguous_format)
     elif out.shape != shape or out.dtype != io or out.device != queries.device:
         raise ValueError("out must match queries")
     elif not out.is_contiguous():
