@@ -13,9 +13,10 @@
 //
 // One workgroup of 1024 threads per row, so that nothing is joined outside LDS: a pass for the largest
 // logit, then a pass for the list, or one for the histogram and one or two for the bins. Bound: at 256 rows of
-// 128256, 131 MB a pass, the passes' reads (5.9 TB/s of caches) and, in the histogram, the issue of some 33
-// instructions per token (27 us of a pass's 22 us of reading): 46 us with top-k, 76 us plain, 78 us with top-p. At few
-// rows the workgroup's own latencies: 1 row of 32000 with top-p 20.9 us, 64 rows of 50257 with top-k 50 and top-p 13.8 us.
+// 128256, 131 MB a pass, the passes' reads (5.9 TB/s of caches) and, in the histogram, the issue of some 26
+// instructions per token (23 us a row by itself, where a pass's reading for all rows is 22): 44 us with top-k, 70 us plain and with top-p. At few
+// rows the workgroup's own latencies: 1 row of 32000 with top-p 17.2 us (the largest 2.7, histogram 6, sums 1.3, bins
+// and tokens 5.5, a launch 1.7), 64 rows of 50257 with top-k 50 and top-p 12.6 us.
 // Keeping a thread's first 16 to 64 values in registers for the later passes made 256 rows 3 to 8% faster and
 // short rows 7 to 60% slower (longer code, fetched anew by every launch): not kept.
 #include <math.h>
@@ -65,25 +66,29 @@ __device__ __forceinline__ float float_of(uint32_t key) {
   return __uint_as_float(key ^ ((key >> 31) ? 0x80000000u : 0xffffffffu));
 }
 
-// f(value, index) for every element of a row, each by some thread of the workgroup: the 16-byte
-// aligned body in vectors, kLoads of them in flight per thread, what lies before and after it one
-// element per thread.
-template <int kLoads, typename T, typename F>
-__device__ __forceinline__ void for_each(const T* x, int32_t n, F f) {
+// f(value, index) for every element of a row with test(value), each by some thread of the workgroup: the
+// 16-byte aligned body in vectors, kLoads of them in flight per thread, what lies before and after it one
+// element per thread. Where tests are seldom true, a vector's are made together before any branch (a pass
+// for the tokens of some bins over 1 row of 128256: 12.6 -> 7.2 us).
+template <int kLoads, typename T, typename P, typename F>
+__device__ __forceinline__ void for_each_if(const T* x, int32_t n, P test, F f) {
   constexpr int kVec = 16 / sizeof(T);
   const int32_t before = static_cast<int32_t>(((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T));
   const int32_t head = before < n ? before : n;
   const u32x4* body = reinterpret_cast<const u32x4*>(x + head);
   const int32_t vectors = (n - head) / kVec;
   auto use = [&](const u32x4& raw, int32_t i) {
+    float v[kVec];
+    bool any = false;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      if constexpr (sizeof(T) == 4) {
-        f(__uint_as_float(raw[w]), i + w);
-      } else {
-        f(bf16_lo(raw[w]), i + 2 * w);
-        f(bf16_hi(raw[w]), i + 2 * w + 1);
-      }
+    for (int e = 0; e < kVec; ++e) {
+      v[e] = sizeof(T) == 4 ? __uint_as_float(raw[e * 4 / kVec]) : e % 2 == 0 ? bf16_lo(raw[e * 4 / kVec]) : bf16_hi(raw[e * 4 / kVec]);
+      any |= test(v[e]);
+    }
+    if (!any) return;
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) {
+      if (test(v[e])) f(v[e], i + e);
     }
   };
   int32_t q = threadIdx.x;
@@ -99,8 +104,13 @@ __device__ __forceinline__ void for_each(const T* x, int32_t n, F f) {
   const int32_t t = threadIdx.x;
   if (t < head + (n - tail)) {
     const int32_t i = t < head ? t : tail + (t - head);
-    f(to_float(x[i]), i);
+    if (test(to_float(x[i]))) f(to_float(x[i]), i);
   }
+}
+
+template <int kLoads, typename T, typename F>
+__device__ __forceinline__ void for_each(const T* x, int32_t n, F f) {
+  for_each_if<kLoads>(x, n, [](float) { return true; }, f);
 }
 
 // Where a row's tokens come from: the row, or (kept >= 0) the tokens kept in LDS.
@@ -111,16 +121,17 @@ struct Source {
   const uint64_t* list;
   int32_t kept;
 
-  template <int kLoads, typename F>
-  __device__ __forceinline__ void each(F f) const {
+  template <int kLoads, typename P, typename F>
+  __device__ __forceinline__ void each_if(P test, F f) const {
     if (kept < 0) {
-      for_each<kLoads>(x, vocab, f);
+      for_each_if<kLoads>(x, vocab, test, f);
       return;
     }
 #pragma unroll 1
     for (int32_t i = threadIdx.x; i < kept; i += kThreads) {
       const uint64_t token = list[i];
-      f(float_of(static_cast<uint32_t>(token >> 32)), static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(token)));
+      const float v = float_of(static_cast<uint32_t>(token >> 32));
+      if (test(v)) f(v, static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(token)));
     }
   }
 };
@@ -146,14 +157,27 @@ struct Shared {
 struct Row {
   float top;
   double rate;      // bins per unit of logit: kPerOctave * log2(e) / T
+  double step;      // and units of logit per bin, for the bins' bounds
   double least;     // min_p * 2^(fractional bits)
   const double* power;
+  double series[4];  // of 2^(f / kPerOctave) - 1 in f, kept in registers
 };
+
+// a * b + c, not in place: the coefficients stay where they are.
+__device__ __forceinline__ double fma_apart(double a, double b, double c) {
+  double d;
+  asm("v_fma_f64 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));
+  return d;
+}
 
 struct Weight {
   int32_t bin;
   uint64_t mass;
 };
+
+__device__ __forceinline__ uint64_t* mass_of_bin(uint64_t* masses, int32_t bin) {  // an index in one instruction
+  return reinterpret_cast<uint64_t*>(reinterpret_cast<char*>(masses) + __mul24(-bin, -8));
+}
 
 // The bin and weight of a finite logit; what lies below the bins weighs 0. Its depth z below the top in bins is
 // n + f with a whole number n <= 0 and |f| <= 1/2, and its weight is
@@ -167,12 +191,10 @@ __device__ __forceinline__ Weight weigh(const Row& r, float x) {
   const double whole = z + 0x1.8p52;
   const int32_t n = __double2loint(whole);
   const double f = z - (whole - 0x1.8p52);
-  constexpr double kStep = 0.69314718055994530942 / kPerOctave;
-  const double series =
-      kStep + f * (kStep * kStep / 2 + f * (kStep * kStep * kStep / 6 + f * (kStep * kStep * kStep * kStep / 24)));
+  const double series = fma_apart(f, fma_apart(f, fma_apart(f, r.series[3], r.series[2]), r.series[1]), r.series[0]);
   const double base = r.power[n & (kPerOctave - 1)];
   const double close = base + base * f * series;
-  const double w = __hiloint2double(__double2hiint(close) + (n >> 7) * (1 << 20), __double2loint(close));
+  const double w = __builtin_ldexp(close, n >> 7);
   const double in_place = w + 0x1p52;
   uint64_t mass = (static_cast<uint64_t>(__double2hiint(in_place) & 0xfffff) << 32) | static_cast<uint32_t>(__double2loint(in_place));
   if constexpr (kMin) mass = w >= r.least ? mass : 0;
@@ -180,14 +202,14 @@ __device__ __forceinline__ Weight weigh(const Row& r, float x) {
 }
 
 // A logit that lies no higher than any of bin `bin`'s: what is below it need not be looked at. The
-// margin covers the rounding of the quotient and of the difference to float32.
+// margin covers the rounding of the product and of the difference to float32.
 __device__ __forceinline__ float floor_of_bin(const Row& r, int32_t bin) {
-  const double x = static_cast<double>(r.top) - (bin + 0.5) / r.rate;
+  const double x = static_cast<double>(r.top) - (bin + 0.5) * r.step;
   const double low = x - (fabs(x) + fabs(static_cast<double>(r.top))) * 0x1p-22;
   return low >= -3.4028234663852886e38 ? static_cast<float>(low) : -3.4028234663852886e38f;
 }
 __device__ __forceinline__ float ceiling_of_bin(const Row& r, int32_t bin) {
-  const double x = static_cast<double>(r.top) - (bin - 0.5) / r.rate;
+  const double x = static_cast<double>(r.top) - (bin - 0.5) * r.step;
   const double high = x + (fabs(x) + fabs(static_cast<double>(r.top))) * 0x1p-22;
   return high <= 3.4028234663852886e38 ? static_cast<float>(high) : 3.4028234663852886e38f;
 }
@@ -242,15 +264,21 @@ __device__ __forceinline__ Scan scan_threads(Shared& s, uint64_t v) {
 
 __device__ __forceinline__ uint64_t block_sum(Shared& s, uint64_t v) { return scan_threads(s, v).all; }
 
-__device__ __forceinline__ float block_max(Shared& s, float v) {
+// The largest v of all threads, or NaN where `odd` is true in any.
+__device__ __forceinline__ float block_max(Shared& s, float v, bool odd) {
 #pragma unroll
   for (int m = kWave / 2; m > 0; m >>= 1) v = fmaxf(v, __shfl_xor(v, m));
-  __syncthreads();
+  if (__ballot(odd) != 0) v = __uint_as_float(0x7fc00000u);
   if ((threadIdx.x & (kWave - 1)) == 0) s.tops[threadIdx.x / kWave] = v;
   __syncthreads();
+  bool any = false;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) v = fmaxf(v, s.tops[w]);
-  return v;
+  for (int w = 0; w < kWaves; ++w) {
+    const float top = s.tops[w];
+    any = any || top != top;
+    v = fmaxf(v, top);
+  }
+  return any ? __uint_as_float(0x7fc00000u) : v;
 }
 
 // Replaces values[0 .. kBins) by the exclusive sums of of(value, bin), values[kBins] by their total.
@@ -280,15 +308,15 @@ __device__ __forceinline__ void scan_bins(Shared& s, V* values, F of) {
 // The bin b with sums[b] < target <= sums[b + 1]: there is one. Every wavefront looks for it, 64 places at a time.
 template <typename V>
 __device__ __forceinline__ int32_t bin_reaching(const V* sums, uint64_t target) {
-  constexpr int kFar = kBins / kWave, kNear = (kFar + kWave - 1) / kWave;
-  static_assert(kFar * kWave == kBins, "whole steps");
+  constexpr int kFar = kBins / kWave | 1, kNear = (kFar + kWave - 1) / kWave;  // odd: each lane in a bank of its own
+  static_assert(kFar * kWave >= kBins, "every bin");
   const int lane = threadIdx.x & (kWave - 1);
-  const int32_t far = (__popcll(__ballot(sums[lane * kFar] < target)) - 1) * kFar;
+  const int32_t far = (__popcll(__ballot(sums[min(lane * kFar, kBins)] < target)) - 1) * kFar;
   int32_t at = far;
 #pragma unroll
   for (int i = kNear - 1; i >= 0; --i) {
     const int32_t first = far + i * kWave, n = min(kWave, kFar - i * kWave);
-    const int below = __popcll(__ballot(lane < n && sums[first + min(lane, n - 1)] < target));
+    const int below = __popcll(__ballot(lane < n && sums[min(first + min(lane, n - 1), kBins)] < target));
     if (below > 0 && at == far) at = first + below - 1;
   }
   return __builtin_amdgcn_readfirstlane(at);
@@ -382,8 +410,7 @@ __device__ __forceinline__ Place locate(Shared& s, const Row& r, const Source<T>
   uint32_t low = 0, high = 0xffffffffu;  // keys still in question
   // f(value, index, key, weight) for the bin's tokens with keys of [from, to].
   auto tokens = [&](uint32_t from, uint32_t to, auto f) {
-    source.template each<4>([&](float v, int32_t i) {
-      if (!(v >= floor && v <= ceiling)) return;
+    source.template each_if<4>([&](float v) { return (v >= floor) & (v <= ceiling); }, [&](float v, int32_t i) {
       const Weight w = weigh<true>(r, v);
       const uint32_t key = key_of(v);
       if (w.bin == bin && key >= from && key <= to && w.mass != 0) f(i, key, w.mass);
@@ -478,8 +505,8 @@ __device__ __forceinline__ int32_t nucleus_and_draw(Shared& s, const Row& r, con
   if (tokens_of(first, last) + (edge > last ? tokens_of(edge, edge) : 0.f) > kList) return -1;
   const float floor = floor_of_bin(r, edge), ceiling = ceiling_of_bin(r, edge);
   const float draw_floor = floor_of_bin(r, last), draw_ceiling = ceiling_of_bin(r, first);
-  source.template each<4>([&](float v, int32_t i) {
-    if (!((v >= floor && v <= ceiling) || (v >= draw_floor && v <= draw_ceiling))) return;
+  const auto near = [&](float v) { return (v >= floor) & (v <= ceiling) | (v >= draw_floor) & (v <= draw_ceiling); };
+  source.template each_if<4>(near, [&](float v, int32_t i) {
     const uint32_t at = atomicAdd(&s.listed, 1u);
     if (at < kList) s.list[at] = order_of(key_of(v), i);
   });
@@ -540,19 +567,20 @@ template <typename T>
 __device__ __forceinline__ int32_t from_bins(Shared& s, const Row& r, const Source<T>& source, float floor, int32_t top_k, float top_p,
                                              float u) {
   const bool counting = top_k > 0;
+  const auto every = [](float) { return true; };  // most tokens lie above the floor: tests together cost 5% here
   if (counting || r.least > 0.0) {
-    source.template each<2>([&](float v, int32_t) {
+    source.template each_if<2>(every, [&](float v, int32_t) {
       if (!(v >= floor)) return;
       const Weight w = weigh<true>(r, v);
       if (w.mass == 0) return;
-      atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[w.bin]), static_cast<unsigned long long>(w.mass));
+      add64(mass_of_bin(s.mass, w.bin), w.mass);
       if (counting) atomicAdd(&s.count[w.bin], 1u);
     });
   } else {
-    source.template each<2>([&](float v, int32_t) {
+    source.template each_if<2>(every, [&](float v, int32_t) {
       if (!(v >= floor)) return;
       const Weight w = weigh<false>(r, v);
-      atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[w.bin]), static_cast<unsigned long long>(w.mass));
+      add64(mass_of_bin(s.mass, w.bin), w.mass);
     });
   }
   __syncthreads();
@@ -589,14 +617,22 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const Args a) {
   const float min_p = a.min_ps ? a.min_ps[row] : a.min_p;
   const float u = a.uniforms[row];
 
+  // LDS is made ready while the row arrives.
+  if (threadIdx.x < kPerOctave) s.power[threadIdx.x] = exp2(threadIdx.x * (1.0 / kPerOctave)) * a.one;
+  for (int i = threadIdx.x; i < kBins + 2; i += kThreads) {
+    s.mass[i] = 0;
+    s.count[i] = 0;
+  }
+  if (threadIdx.x == 0) s.listed = 0;
+
   float most = -INFINITY;
   bool odd = false;
   for_each<8>(x, a.vocab, [&](float v, int32_t) {
     most = fmaxf(most, v);
     odd = odd || v != v;
   });
-  const bool any_odd = __syncthreads_or(odd);
-  const float top = block_max(s, most);
+  const float top = block_max(s, most, odd);
+  const bool any_odd = top != top;
   if (any_odd || top == -INFINITY || !(temperature > 0.f)) {  // the greedy token: the first NaN, else the first of the largest
     if (threadIdx.x == 0) s.found = a.vocab;
     __syncthreads();
@@ -623,15 +659,16 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const Args a) {
   Row r;
   r.top = top;
   r.rate = fmax(kPerOctave * 1.44269504088896340736 / static_cast<double>(temperature), 1e-300);  // T may be infinite
+  r.step = 1.0 / r.rate;
   r.least = min_p > 0.f ? fmin(static_cast<double>(min_p), 1.0) * a.one : 0.0;
   r.power = s.power;
-  if (threadIdx.x < kPerOctave) s.power[threadIdx.x] = exp2(threadIdx.x * (1.0 / kPerOctave)) * a.one;
-  for (int i = threadIdx.x; i < kBins + 2; i += kThreads) {
-    s.mass[i] = 0;
-    s.count[i] = 0;
-  }
-  if (threadIdx.x == 0) s.listed = 0;
-  __syncthreads();
+  constexpr double kStep = 0.69314718055994530942 / kPerOctave;
+  r.series[0] = kStep;
+  r.series[1] = kStep * kStep / 2;
+  r.series[2] = kStep * kStep * kStep / 6;
+  r.series[3] = kStep * kStep * kStep * kStep / 24;
+#pragma unroll
+  for (double& c : r.series) asm volatile("" : "+v"(c));
 
   // The bins that the kept tokens lie in, where the settings bound them beforehand: min-p by its weight;
   // top-k by the threads' largest tokens, of which there are top_k in the bins up to the pivot's.
@@ -656,10 +693,8 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const Args a) {
   Source<T> source{x, a.vocab, s.kept, -1};
   // Were m of the 1024 threads to meet a token from the floor on, some -1024 ln(1 - m / 1024) tokens lie there:
   // 2840 for kCrowded threads, so that the list seldom overflows.
-  const int32_t meet = __syncthreads_count(most >= floor);
-  if (a.vocab <= kFew || (last < kBins - 1 && meet <= kCrowded)) {
-    for_each<8>(x, a.vocab, [&](float v, int32_t i) {
-      if (!(v >= floor)) return;
+  if (a.vocab <= kFew || (last < kBins - 1 && __syncthreads_count(most >= floor) <= kCrowded)) {
+    for_each_if<8>(x, a.vocab, [&](float v) { return v >= floor; }, [&](float v, int32_t i) {
       const uint32_t slot = atomicAdd(&s.listed, 1u);
       if (slot < kKept) s.kept[slot] = order_of(key_of(v), i);
     });
