@@ -167,6 +167,14 @@ __device__ __forceinline__ uint32_t take_piece(float& x0, float& x1) {
   return pair;
 }
 
+// Pieces without the guard: what is not finite turns into NaN, which its user looks for at the end.
+__device__ __forceinline__ uint32_t cut_piece(float& x0, float& x1) {
+  const uint32_t pair = __builtin_bit_cast(uint32_t, __builtin_convertvector((floatx2{x0, x1}), bf16x2));
+  x0 -= bf16_lo(pair);
+  x1 -= bf16_hi(pair);
+  return pair;
+}
+
 // ---------------------------------------------------------------------------------------------
 // One (row, head) over items [first, last) of a span, by the definition: a wavefront, 64 keys at a
 // time; a lane scores one key, then owns dimensions. For rows that the matrix products cannot
@@ -241,24 +249,28 @@ __device__ __forceinline__ void exact_row(const Window& a, int64_t t, int32_t he
 //                  lane's 8 dimensions are its 8 terms (float32 queries in three pieces); float32 keys:
 //                  v_mfma_f32_16x16x4_f32, its 4 dimensions are 4 steps. Register r of the result is
 //                  the score of key 4c + r for head n.
-//   O^T = V^T P^T  v_mfma_f32_16x16x4_f32, step r taking keys 4c + r of the lane groups c: P is the
-//                  lane's own register r, and V comes straight from the pool too: lane (c, i) loads
-//                  kVWidth adjacent values of key 4c + r and uses them in as many products.
+//   O^T = V^T P^T  V comes straight from the pool too: lane (c, i) loads kVWidth adjacent values of keys 4c + r
+//                  and uses each in a product of its own. float32: v_mfma_f32_16x16x4_f32, step r taking keys
+//                  4c + r of the lane groups c, P being the lane's own register r. bfloat16:
+//                  v_mfma_f32_16x16x32_bf16 with the lane's eight keys of two blocks as its terms, P cut into two
+//                  pieces (2^-17 of a weight; under float32 queries three): an eighth of the float32 steps'
+//                  time, which one row felt (2 key heads x 64, 516 keys: 10.4 -> 8.8 us).
 //
 // So nothing is staged: every key and value row goes from the pool to the registers that multiply it,
-// in float32 throughout, and all heads of a group share one read of it. The loads of the next keys are
+// and all heads of a group share one read of it. The loads of the next keys are
 // issued before the present ones are used (a second set of registers for the values, so that they too
 // are a whole round ahead, measured 3 to 5% slower).
 //
 // Bound: HBM. 64 rows with contexts of 2048 to 16384 and a window of 4096, 32 heads on 8 x 128, bfloat16, 1.1 GB:
 // 180 us, 6.0 TB/s; contexts of 512 to 4096 and a window of 1024, 32 x 128 heads in float32, 2.2 GB: 345 us, 6.3
 // TB/s (only reading one head's rows at a time in that pattern: 5.4).
-// One row of 2 key heads x 64 and 516 keys: 10.3 us, the latency of a few dependent loads.
+// One row of 2 key heads x 64 and 516 keys: 8.8 us, the latency of a few dependent loads.
 // ---------------------------------------------------------------------------------------------
 template <typename QT, typename KVT, int D>
 struct RowShape {
   static constexpr bool kBf16 = sizeof(KVT) == 2;
   static constexpr int kPieces = kBf16 ? (sizeof(QT) == 4 ? 3 : 1) : 1;
+  static constexpr int kPPieces = sizeof(QT) == 4 ? 3 : 2;   // of the weights, over bfloat16 values
   static constexpr int kBlocks = kBf16 && D <= 128 ? 2 : 1;  // 16-key blocks per round
   static constexpr int kKeys = 16 * kBlocks;
   static constexpr int kKLoads = kBf16 ? D / 32 : D / 16;    // 16-byte loads of a key row per lane
@@ -518,17 +530,47 @@ __device__ __forceinline__ void row_pass(const Window& a, RowScratch<D, kRowWave
                 for (int w = 0; w < S::kVWords; ++w) vx[j][r][g].w[w] = 0;
               }
             }
+            if constexpr (!S::kBf16) {
 #pragma unroll
-            for (int g = 0; g < S::kVLoads; ++g) {
+              for (int g = 0; g < S::kVLoads; ++g) {
 #pragma unroll
-              for (int e = 0; e < S::kVWidth; ++e) {
-                float v;
-                if constexpr (S::kBf16) {
-                  v = e % 2 ? bf16_hi(vx[j][r][g].w[e / 2]) : bf16_lo(vx[j][r][g].w[e / 2]);
-                } else {
-                  v = __uint_as_float(vx[j][r][g].w[e]);
+                for (int e = 0; e < S::kVWidth; ++e) {
+                  o[g * S::kVWidth + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vx[j][r][g].w[e]), st[j][r],
+                                                                               o[g * S::kVWidth + e], 0, 0, 0);
                 }
-                o[g * S::kVWidth + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, st[j][r], o[g * S::kVWidth + e], 0, 0, 0);
+              }
+            }
+          }
+        }
+        if constexpr (S::kBf16) {
+          // Term 4j + r of a lane's eight is key 16j + 4c + r: of the weights its own registers, of a dimension
+          // the eight values of it that it has loaded.
+          u32x4 pr[S::kPPieces] = {};
+#pragma unroll
+          for (int j = 0; j < S::kBlocks; ++j) {
+#pragma unroll
+            for (int r = 0; r < 4; r += 2) {
+              float x0 = st[j][r], x1 = st[j][r + 1];
+#pragma unroll
+              for (int p = 0; p < S::kPPieces; ++p) pr[p][2 * j + r / 2] = cut_piece(x0, x1);
+            }
+          }
+#pragma unroll
+          for (int g = 0; g < S::kVLoads; ++g) {
+#pragma unroll
+            for (int e = 0; e < S::kVWidth; ++e) {
+              u32x4 v = {};
+#pragma unroll
+              for (int j = 0; j < S::kBlocks; ++j) {
+#pragma unroll
+                for (int r = 0; r < 4; r += 2) {
+                  v[2 * j + r / 2] = __builtin_amdgcn_perm(vx[j][r + 1][g].w[e / 2], vx[j][r][g].w[e / 2], e % 2 ? 0x07060302 : 0x05040100);
+                }
+              }
+#pragma unroll
+              for (int p = S::kPPieces - 1; p >= 0; --p) {
+                o[g * S::kVWidth + e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                    __builtin_bit_cast(bf16x8, v), __builtin_bit_cast(bf16x8, pr[p]), o[g * S::kVWidth + e], 0, 0, 0);
               }
             }
           }
@@ -574,7 +616,7 @@ __device__ __forceinline__ void row_pass(const Window& a, RowScratch<D, kRowWave
       }
       __syncthreads();
     }
-    if constexpr (S::kPieces > 1) {  // what is not finite is computed again from whole numbers
+    if constexpr (S::kBf16) {  // what is not finite is computed again from whole numbers
       if (wave == 0) {
         bool bad = false;
 #pragma unroll
@@ -677,14 +719,6 @@ __device__ __forceinline__ constexpr bool counted(int i, int j) { return i + j <
 
 __device__ __forceinline__ floatx16 mfma32(const u32x4& a, const u32x4& b, const floatx16& c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
-
-// Pieces without the guard: what is not finite turns into NaN, which the tile pass looks for at its end.
-__device__ __forceinline__ uint32_t cut_piece(float& x0, float& x1) {
-  const uint32_t pair = __builtin_bit_cast(uint32_t, __builtin_convertvector((floatx2{x0, x1}), bf16x2));
-  x0 -= bf16_lo(pair);
-  x1 -= bf16_hi(pair);
-  return pair;
 }
 
 // Chunks of a staged row are permuted so that the lanes of a read lie in different banks: the key
