@@ -1209,16 +1209,19 @@ int launch(Window a, hipStream_t stream) {
       return check_launch();
     }
   }
-  // Few workgroups are of eight wavefronts (1 row, 2 key heads x 64, 516 keys: 11.4 -> 10.3 us; 4 x 4100 keys, 8
-  // splits: 28.4 -> 26.7; 64 rows 203 -> 208). Where there are many and a key row is short, one of eight serves two
-  // neighbouring key heads, and so reads twice as much next to each other. head_dim 256 needs the registers of four.
+  // Few workgroups are of eight wavefronts (1 row, 2 key heads x 64, 516 keys: 9.1 -> 8.8 us; 24 rows of 1024 keys, 8 x
+  // 64, float32: 34 -> 27; 64 rows of 4100 keys 203 -> 208). head_dim 256 needs the registers of four, and so do float32
+  // queries of head_dim 128 over bfloat16 keys (8 rows of 1024 keys, 32/8 heads: 20.4 us, 21.9 with eight). Where there
+  // are many and a key row is short, one of eight serves two neighbouring key heads, and so reads twice as much next to
+  // each other.
   constexpr bool kShort = D * sizeof(KVT) <= 256;
-  const bool wide = D <= 128 && groups <= 256;
+  constexpr bool kWide = D < 128 || (D == 128 && sizeof(QT) == sizeof(KVT));
+  const bool wide = kWide && groups <= 256;
   const bool pair = kShort && groups >= 512 && a.num_kv_heads % 2 == 0;
   const auto start = [&](auto kernel, int64_t count, int waves) {
     hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(count)), dim3(waves * kWave), 0, stream, a);
   };
-  if constexpr (D <= 128) {
+  if constexpr (kWide) {
     if (wide) start(row_kernel<QT, KVT, D, 8, 1>, groups, 8);
   }
   if constexpr (kShort) {
@@ -1265,10 +1268,15 @@ extern "C" int32_t pkv_window_splits(int64_t num_queries, int32_t num_heads, int
   const int64_t rows = runs ? pkv::kTileQueries / group : 1;
   const int64_t groups = (num_queries + rows - 1) / rows * num_kv_heads * (runs ? 1 : (group + 15) / 16);
   // Tiles: two workgroups for every CU, 128 keys to a split at least. Rows: one workgroup of eight
-  // wavefronts for every CU, 512 keys to a split (1 row, 8 key heads x 128, 4100 keys, bfloat16: 62, 39, 27, 22, 24 us
-  // with 1, 2, 4, 8, 16 splits; 4 rows 78, 49, 33, 27, 38; 16 rows 92, 59, 67, 82, 111).
+  // wavefronts for every CU, 512 keys to a split (1 row, 8 key heads x 128, 4100 keys, bfloat16: 44, 29, 21, 20, 23 us
+  // with 1, 2, 4, 8, 16 splits; 4 rows 69, 46, 31, 25, 27; 16 rows 89, 57, 52, 60, 75).
   const int64_t most = std::max<int64_t>(1, std::min<int64_t>(PKV_WINDOW_MAX_SPLITS, longest / (runs ? 128 : 512)));
-  const int64_t want = runs ? (512 + groups - 1) / std::max<int64_t>(1, groups) : 256 / std::max<int64_t>(1, groups);
+  int64_t want = runs ? (512 + groups - 1) / std::max<int64_t>(1, groups) : 256 / std::max<int64_t>(1, groups);
+  // More workgroups than CUs, which would leave many of them idle at the end: up to four splits of 1024 keys (8 key heads x
+  // 128, 4100 keys, one split and four: 36 rows 171 and 134 us, in float32 295 and 214; 68 rows 298 and 232, 479 and
+  // 376; 56 rows, seven eighths of two rounds, 191 and 190, with 2050 keys x 64 61 and 67).
+  const int64_t round = (groups + 255) / 256 * 256;
+  if (!runs && groups > 256 && groups * 20 < round * 17) want = std::min<int64_t>(4, longest / 1024);
   return static_cast<int32_t>(std::max<int64_t>(1, std::min(most, want)));
 }
 

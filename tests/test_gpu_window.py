@@ -358,3 +358,25 @@ def test_more_rows_beside_a_run_than_workgroups(device, io, kv, splits):
     runs[60:60] = [(30, 130)]
     check(device, make(runs, 8, 8, 64, 16, io, kv, seed=12), 40, 2, num_splits=splits)
     check(device, make([(30, 130), *runs], 16, 8, 32, 16, io, kv, seed=13), 40, 2, num_splits=splits, max_query_len=30)
+
+
+@pytest.mark.parametrize("io,kv", TYPES)
+@pytest.mark.parametrize("dim", [32, 128, 256])
+@pytest.mark.parametrize("splits", [1, 3])
+def test_an_infinite_value_that_rows_see_stays_in_its_dimension(device, io, kv, dim, splits):
+    d = make([(1, 60), (20, 60)], 4, 2, dim, 16, io, kv, seed=4)
+    clean = call(device, d, 100, 0, num_splits=splits).float().cpu()
+    for s in (0, 1):
+        d["v"][d["tables"][s, 1], 3, 0, 5] = float("inf")  # key 19 of key head 0
+        d["v"][d["tables"][s, 1], 4, 1, 7] = -float("inf")
+    got = call(device, d, 100, 0, num_splits=splits).float().cpu()
+    assert (got[:, :2, 5] == float("inf")).all() and (got[:, 2:, 7] == -float("inf")).all()
+    want = clean.clone()
+    want[:, :2, 5] = float("inf")
+    want[:, 2:, 7] = -float("inf")
+    finite = want.abs() < float("inf")
+    # Both are within the bound of the same number: these rows may be computed another way.
+    _, size = window_attention(d["q"].float().numpy(), d["positions"], d["seqs"], d["k"].float().numpy(), np.zeros(d["v"].shape),
+                               d["tables"], d["contexts"], d["scale"], 100, 0)  # fmt: skip
+    off = np.broadcast_to(2 * bound(d, want.double().numpy(), size), finite.shape)
+    assert ((got - want).abs()[finite].numpy() <= off[finite.numpy()]).all()

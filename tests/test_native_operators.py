@@ -121,6 +121,8 @@ def test_window_splits_follow_the_work(lib) -> None:
     splits = lib.pkv_window_splits  # queries, heads, kv_heads, window, sinks, context, rows of a run
     assert splits(1, 64, 8, 4096, 4, 32768, 1) == 8  # few rows: 512 keys to a split
     assert splits(256, 64, 8, 4096, 4, 32768, 1) == 1  # enough rows
+    assert splits(36, 64, 8, 4096, 4, 32768, 1) == 4  # 288 workgroups would leave 224 of 512 places idle
+    assert splits(36, 64, 8, 2048, 0, 32768, 1) == 2 and splits(36, 64, 8, 512, 0, 32768, 1) == 1
     assert splits(1, 64, 8, 100, 0, 32768, 1) == splits(1, 64, 8, 4096, 4, 100, 1) == 1  # few keys
     assert splits(1, 1, 1, 1 << 20, 0, 1 << 20, 1) == 64  # no more than the most
     assert splits(512, 8, 8, 4096, 0, 4096, 512) > splits(8192, 8, 8, 4096, 0, 4096, 512) >= 1
