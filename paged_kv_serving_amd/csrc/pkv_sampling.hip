@@ -13,8 +13,8 @@
 //
 // One workgroup of 1024 threads per row, so that nothing is joined outside LDS: a pass for the largest
 // logit, then a pass for the list, or one for the histogram and one or two for the bins. Bound: at 256 rows of
-// 128256, 131 MB a pass, the passes' reads (5.9 TB/s of caches) and, in the histogram, the issue of some 26
-// instructions per token (23 us for a row by itself; reading all of them once takes 22): 44 us with top-k, 70 us plain
+// 128256, 131 MB a pass, the passes' reads (5.9 TB/s of caches) and, in the histogram, the issue of some 24
+// vector instructions per token (23 us for a row by itself; reading all rows once takes 22): 44 us with top-k, 70 plain
 // and with top-p. At few rows the workgroup's own latencies: 1 row of 32000 with top-p 17.2 us (the largest 2.7,
 // histogram 6, sums 1.3, bins and tokens 5.5, a launch 1.7), 64 rows of 50257 with top-k 50 and top-p 12.6 us.
 // Keeping a thread's first 16 to 64 values in registers for the later passes made 256 rows 3 to 8% faster and

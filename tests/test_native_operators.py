@@ -130,3 +130,22 @@ def test_window_splits_follow_the_work(lib) -> None:
     for bad in ((-1, 8, 8, 1, 0, 1, 1), (1, 8, 0, 1, 0, 1, 1), (1, 7, 2, 1, 0, 1, 1), (1, 8, 8, 0, 0, 1, 1),
                 (1, 8, 8, 1, -1, 1, 1), (1, 8, 8, 1, 0, -1, 1), (1, 8, 8, 1, 0, 1, -1), (1, 65, 1, 1, 0, 1, 1)):  # fmt: skip
         assert splits(*bad) == EINVAL
+
+
+def test_tensors_off_the_device_are_refused_by_name(lib) -> None:
+    import torch
+
+    from paged_kv_serving_amd import ops
+
+    f, i32, i64 = torch.zeros(1, 2, 32), torch.zeros(1, dtype=torch.int32), torch.zeros(1, dtype=torch.int64)
+    pool, table = torch.zeros(4, 8, 2, 32), torch.zeros(1, 4, dtype=torch.int32)
+    with pytest.raises(ValueError, match="HIP device"):
+        ops.rope_append_axes(pool, pool, f, f, f, i64, torch.zeros(4, 16), torch.zeros(4, 16), i64)
+    with pytest.raises(ValueError, match="HIP device"):
+        ops.paged_attention_window(f, i32, i32, pool, pool, table, i32, 1.0, window=4, max_context_len=8)
+    with pytest.raises(ValueError, match="HIP device"):
+        ops.sample_tokens(torch.zeros(1, 9), torch.zeros(1))
+    host = _native.bound_host()
+    assert host.one_device(f, i32) == host.one_device() == -1
+    with pytest.raises(AttributeError):
+        host.one_device(3)
