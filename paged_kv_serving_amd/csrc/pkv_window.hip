@@ -1306,10 +1306,12 @@ extern "C" int32_t pkv_window_splits(int64_t num_queries, int32_t num_heads, int
   const bool runs = pkv::has_runs(max_query_len, group);
   const int64_t rows = runs ? pkv::kTileQueries / group : 1;
   const int64_t groups = (num_queries + rows - 1) / rows * num_kv_heads * (runs ? 1 : (group + 15) / 16);
-  // Tiles: two workgroups for every CU, 128 keys to a split at least. Rows: one workgroup of eight
-  // wavefronts for every CU, 512 keys to a split (1 row, 8 key heads x 128, 4100 keys, bfloat16: 44, 29, 21, 20, 23 us
-  // with 1, 2, 4, 8, 16 splits; 4 rows 69, 46, 31, 25, 27; 16 rows 89, 57, 52, 60, 75).
-  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(PKV_WINDOW_MAX_SPLITS, longest / (runs ? 128 : 512)));
+  // Tiles: two workgroups for every CU, 128 keys to a split at least. Rows: one workgroup of eight wavefronts for
+  // every CU, 256 keys to a split, and one split below 1024 keys, which saves a launch. 8 key heads x 128, bfloat16,
+  // with 1, 2, 4, 8, 16 splits: 1 row of 4096 keys 63, 38, 24, 18, 16 us, 4 rows 73, 44, 28, 21, 22, 16 rows 85, 56,
+  // 51, 57, 69; 8 rows of 1024 keys 24, 18, 15, 15, 23; 1 row of 512 keys 12.4, 12.2, 11.3, 11.2, 12.3.
+  const int64_t fewest = runs ? 128 : longest < 1024 ? 1024 : 256;
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(PKV_WINDOW_MAX_SPLITS, longest / fewest));
   int64_t want = runs ? (512 + groups - 1) / std::max<int64_t>(1, groups) : 256 / std::max<int64_t>(1, groups);
   // More workgroups than CUs, which would leave many of them idle at the end: up to four splits of 1024 keys (8 key heads x
   // 128, 4100 keys, one split and four: 36 rows 171 and 134 us, in float32 295 and 214; 68 rows 298 and 232, 479 and

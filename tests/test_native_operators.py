@@ -119,7 +119,8 @@ def test_window_workspace_holds_every_split_and_the_row_list(lib) -> None:
 
 def test_window_splits_follow_the_work(lib) -> None:
     splits = lib.pkv_window_splits  # queries, heads, kv_heads, window, sinks, context, rows of a run
-    assert splits(1, 64, 8, 4096, 4, 32768, 1) == 8  # few rows: 512 keys to a split
+    assert splits(1, 64, 8, 4096, 4, 32768, 1) == 16  # few rows: 256 keys to a split
+    assert splits(1, 64, 8, 1000, 4, 32768, 1) == 1  # but few keys are not split
     assert splits(256, 64, 8, 4096, 4, 32768, 1) == 1  # enough rows
     assert splits(36, 64, 8, 4096, 4, 32768, 1) == 4  # 288 workgroups would leave 224 of 512 places idle
     assert splits(36, 64, 8, 2048, 0, 32768, 1) == 2 and splits(36, 64, 8, 512, 0, 32768, 1) == 1
