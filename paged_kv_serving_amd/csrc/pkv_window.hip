@@ -696,7 +696,7 @@ __global__ __launch_bounds__(kRowWaves * kPair * kWave) void row_kernel(const Wi
 // are in flight (bfloat16 pools: straight to LDS; float32 pools: to registers, cut on their way to LDS) and
 // the slots of the one after are looked up.
 //
-// Bound: latency. 8 x 512 rows behind 2048 others, window 1024, 32 heads on 8 x 128, bfloat16: 132 us, 520 TFLOP/s of visible
+// Bound: latency. 8 x 512 rows behind 2048 others, window 1024, 32 heads on 8 x 128, bfloat16: 130 us, 530 TFLOP/s of visible
 // products (1390 in a large library product); the matrix units are busy 27% of it, vector instructions
 // issue in 29% and LDS works in 20%, at two wavefronts per SIMD. One piece of P instead of two
 // was 9% faster.
