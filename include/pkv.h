@@ -611,7 +611,8 @@ int pkv_rope_append_axes(const pkv_rope_axes* args, int device, void* stream);
  * pools, bfloat16 queries over bfloat16 pools; up to PKV_WINDOW_MAX_GROUP query heads per key head;
  * fewer than 2^31 slots, and a max_context_len of up to PKV_WINDOW_MAX_CONTEXT. `out` and `workspace`
  * must not overlap an input, and calls that may run at the same time need workspaces of their own.
- * Scores, softmax and sums are float32; a bfloat16 output is rounded once.
+ * Scores, softmax and sums are float32; a bfloat16 output is rounded once. Where bfloat16 rows are computed
+ * together, their values are multiplied by weights of 16 bits (off by up to 2^-17 of a weight).
  */
 #define PKV_WINDOW_MAX_GROUP 64
 #define PKV_WINDOW_MAX_SPLITS 64

@@ -4,7 +4,7 @@
 // j > p - window or j < sinks:
 //     out = sum_j exp(s_j) v_j / sum_j exp(s_j),  s_j = scale * q . k_j
 // with an online softmax (running maximum and sum), everything in float32 and one rounding to the
-// output's type.
+// output's type, but for the weights that a bfloat16 tile multiplies its values by (16 bits, at tile_kernel).
 #include <math.h>
 
 #include <algorithm>
@@ -253,9 +253,10 @@ __device__ __forceinline__ void exact_row(const Window& a, int64_t t, int32_t he
 //   O^T = V^T P^T  V comes straight from the pool too: lane (c, i) loads kVWidth adjacent values of keys 4c + r
 //                  and uses each in a product of its own. float32: v_mfma_f32_16x16x4_f32, step r taking keys
 //                  4c + r of the lane groups c, P being the lane's own register r. bfloat16:
-//                  v_mfma_f32_16x16x32_bf16 with the lane's eight keys of two blocks as its terms, P cut into two
-//                  pieces (2^-17 of a weight; under float32 queries three): an eighth of the float32 steps'
-//                  time, which one row felt (2 key heads x 64, 516 keys: 10.4 -> 8.8 us).
+//                  v_mfma_f32_16x16x32_bf16 with the lane's eight keys of two blocks as its terms, P cut into three
+//                  pieces, which hold all its bits: 3/16 of the float32 steps' time, which one row felt (2 key
+//                  heads x 64, 516 keys: 10.4 -> 9.5 us). Two pieces leave out 2^-17 of a weight and took 8.8 us there
+//                  and the same elsewhere (64 rows of up to 4100 keys, 32/8 heads x 128: 181 us with either).
 //
 // So nothing is staged: every key and value row goes from the pool to the registers that multiply it,
 // and all heads of a group share one read of it. The loads of the next keys are
@@ -265,13 +266,13 @@ __device__ __forceinline__ void exact_row(const Window& a, int64_t t, int32_t he
 // Bound: HBM. 64 rows with contexts of 2048 to 16384 and a window of 4096, 32 heads on 8 x 128, bfloat16, 1.1 GB:
 // 180 us, 6.0 TB/s; contexts of 512 to 4096 and a window of 1024, 32 x 128 heads in float32, 2.2 GB: 345 us, 6.3
 // TB/s (only reading one head's rows at a time in that pattern: 5.4).
-// One row of 2 key heads x 64 and 516 keys: 8.8 us, the latency of a few dependent loads.
+// One row of 2 key heads x 64 and 516 keys: 9.5 us, the latency of a few dependent loads.
 // ---------------------------------------------------------------------------------------------
 template <typename QT, typename KVT, int D>
 struct RowShape {
   static constexpr bool kBf16 = sizeof(KVT) == 2;
   static constexpr int kPieces = kBf16 ? (sizeof(QT) == 4 ? 3 : 1) : 1;
-  static constexpr int kPPieces = sizeof(QT) == 4 ? 3 : 2;   // of the weights, over bfloat16 values
+  static constexpr int kPPieces = 3;                         // of the weights, over bfloat16 values
   static constexpr int kBlocks = kBf16 && D <= 128 ? 2 : 1;  // 16-key blocks per round
   static constexpr int kKeys = 16 * kBlocks;
   static constexpr int kKLoads = kBf16 ? D / 32 : D / 16;    // 16-byte loads of a key row per lane
@@ -690,7 +691,9 @@ __global__ __launch_bounds__(kRowWaves * kPair * kWave) void row_kernel(const Wi
 //                  transposed (ds_read_b64_tr_b16), four keys of one dimension at a time.
 // Float32 operands are cut into three bfloat16 pieces, whose products (the 3 or 6 largest of them) add
 // up to the float32 product within one float32 rounding. bfloat16 queries and keys are one piece; their
-// weights P are two, 2^-17 of a weight: one piece (2^-9) would add as much error as the output's rounding.
+// weights P are two, 16 bits, off by 2^-17 of a weight: 2^-8 of the output's own rounding, which one piece
+// would double. Three pieces would keep every bit and cost 16% (8 x 512 rows: 126 -> 147 us, 14% x 64, 13% x 256).
+// Their sum is taken of the float32 weights.
 //
 // Keys and values are staged kKeys at a time in two LDS buffers: while one is used, the next tile's rows
 // are in flight (bfloat16 pools: straight to LDS; float32 pools: to registers, cut on their way to LDS) and

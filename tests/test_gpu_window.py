@@ -380,3 +380,45 @@ def test_an_infinite_value_that_rows_see_stays_in_its_dimension(device, io, kv, 
                                d["tables"], d["contexts"], d["scale"], 100, 0)  # fmt: skip
     off = np.broadcast_to(2 * bound(d, want.double().numpy(), size), finite.shape)
     assert ((got - want).abs()[finite].numpy() <= off[finite.numpy()]).all()
+
+
+def cancelling_pairs(weight: float, count: int) -> np.ndarray:
+    """``count`` pairs of bfloat16 values (v1, v2) with the smallest |v1 + weight v2| there are: a mean of
+    such values shows what its weights have lost, next to which its own rounding is nothing."""
+    grid = np.arange(128, 256) / 128.0  # one binade of bfloat16
+    sums = np.abs(np.concatenate([grid[:, None] - weight * grid * f for f in (1.0, 2.0, 4.0)], 1))
+    first, second = np.unravel_index(np.argsort(sums, axis=None)[:count], sums.shape)
+    return np.stack([grid[first], -np.concatenate([grid, 2 * grid, 4 * grid])[second]])
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(1, 1, 32), (4, 2, 64), (2, 2, 128), (8, 1, 256)])
+@pytest.mark.parametrize("seqs", [3, 600])
+@pytest.mark.parametrize("splits", [1, 2])
+def test_the_weights_of_a_bfloat16_row_keep_the_bits_of_a_float32(device, heads, kv_heads, dim, seqs, splits):
+    """Two keys that differ in one dimension, with weights 1 and w, and values that cancel. Scores have one
+    product, exact in float32; scaling it, the step to base 2 and the difference to the largest are at most
+    five roundings of numbers below 2, so with the exponential's own (2^-23) the weight is off by less than
+    12 2^-24 of itself; the products' sums, the joins' and the division by at most 12 2^-24 of their terms."""
+    import torch
+
+    rng = np.random.default_rng(dim + seqs)
+    scores = np.round(rng.uniform(0.05, 1.2, seqs) * 128) / 128  # bfloat16 and exact
+    q, k, v = np.zeros((seqs, heads, dim)), np.zeros((seqs, 2, kv_heads, dim)), np.zeros((seqs, 2, kv_heads, dim))
+    q[:, :, 5] = 1.0
+    k[:, 1, :, 5] = -scores[:, None]
+    weights = np.exp(-scores)
+    for s in range(seqs):
+        v[s] = cancelling_pairs(weights[s], dim)[:, None, :]
+    d = {
+        **{name: torch.from_numpy(x).to(torch.bfloat16) for name, x in (("q", q), ("k", k), ("v", v))},
+        "positions": np.ones(seqs, np.int32), "seqs": np.arange(seqs, dtype=np.int32), "scale": 1.0,
+        "tables": np.arange(seqs, dtype=np.int32)[:, None], "contexts": np.full(seqs, 2, np.int32),
+    }  # fmt: skip
+    for name, x in (("q", q), ("k", k), ("v", v)):
+        assert (d[name].double().numpy() == x).all()
+    got = call(device, d, 2, 0, max_query_len=1, num_splits=splits).double().cpu().numpy()
+    first, second = v[:, 0, :1], weights[:, None, None] * v[:, 1, :1]  # [seqs, 1, dim]
+    total = 1 + weights[:, None, None]
+    want = (first + second) / total
+    off = (12 * np.abs(second) + 12 * (np.abs(first) + np.abs(second))) * 2.0**-24 / total + np.abs(want) * 2.0**-8
+    assert (np.abs(got - want) <= off).all(), (np.abs(got - want) / off).max()
