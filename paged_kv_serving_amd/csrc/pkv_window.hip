@@ -1218,7 +1218,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const Window a) {
   float x[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) x[e] = sum == 0.f ? 0.f : acc[e] / sum;
-  store_row<QT, 4>(static_cast<QT*>(a.out) + item * D + d, x);
+  store_row<QT, 4>(static_cast<QT*>(a.out) + static_cast<int64_t>(item) * D + d, x);  // up to 2^33 elements
 }
 
 template <typename QT, typename KVT, int D>

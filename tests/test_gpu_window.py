@@ -422,3 +422,32 @@ def test_the_weights_of_a_bfloat16_row_keep_the_bits_of_a_float32(device, heads,
     want = (first + second) / total
     off = (12 * np.abs(second) + 12 * (np.abs(first) + np.abs(second))) * 2.0**-24 / total + np.abs(want) * 2.0**-8
     assert (np.abs(got - want) <= off).all(), (np.abs(got - want) / off).max()
+
+
+def test_outputs_past_32_bits(device):
+    """More than 2^32 output elements in one split call. Every score is zero, so a row's output is the mean of
+    the values up to its position: whole weights, whose float32 sums of 64 terms, join and division are off by
+    at most (64 + 16) 2^-24 of the largest value, and one rounding to bfloat16."""
+    import torch
+
+    from paged_kv_serving_amd import ops
+
+    heads, dim, keys = 64, 256, 64
+    rows = (1 << 32) // (heads * dim) + 77
+    gen = torch.Generator().manual_seed(5)
+    k, v = (torch.randn((4, 16, 1, dim), generator=gen).to(torch.bfloat16).to(device) for _ in range(2))
+    positions = torch.arange(rows, dtype=torch.int32, device=device) * 7 % keys
+    zero = torch.zeros(rows, dtype=torch.int32, device=device)
+    queries = torch.zeros((rows, heads, dim), dtype=torch.bfloat16, device=device)
+    out = torch.full_like(queries, float("nan"))
+    ops.paged_attention_window(queries, positions, zero, k, v, torch.arange(4, dtype=torch.int32, device=device)[None], torch.full_like(zero[:1], keys),
+                               0.1, window=keys, max_context_len=keys, max_query_len=1, num_splits=2, out=out)  # fmt: skip
+    del queries
+    values = v.double().view(keys, dim)
+    means = values.cumsum(0) / torch.arange(1, keys + 1, device=device)[:, None]
+    off = (keys + 16) * 2.0**-24 * values.abs().max() + means.abs() * 2.0**-8
+    low, high = (means - off).float(), (means + off).float()
+    for start in range(0, rows, 1 << 14):
+        part = out[start : start + (1 << 14)].float()
+        at = positions[start : start + (1 << 14)].long()
+        assert ((part >= low[at][:, None]) & (part <= high[at][:, None])).all(), start
