@@ -520,7 +520,7 @@ class ModelRunner:
         at = {}
         for name, value in settings.items():
             array = np.asarray(value)
-            if name == "top_k" and array.dtype.kind not in "iu":
+            if name == "top_k" and array.size and array.dtype.kind not in "iu":  # no entries: no type
                 raise ValueError("top_k must be whole numbers")
             low = {"temperature": array >= 0, "top_k": array >= 0, "top_p": array > 0, "min_p": array >= 0}[name]
             if not (low & (array <= (1 if name in ("top_p", "min_p") else np.inf))).all():

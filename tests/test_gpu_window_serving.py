@@ -254,3 +254,11 @@ def test_execute_sampled_refusals_and_edges(device, model) -> None:
     assert runner.execute_sampled(ExecutionBatch(()), []) == {}
     quiet = ExecutionBatch((entry("a", 3, 5, (1,), rng, want=False),))
     assert runner.execute_sampled(quiet, []) == {}
+
+
+def test_a_sampled_step_without_logits_rows_appends_its_keys_and_values(device, model) -> None:
+    runner, other = (ModelRunner(model, num_blocks=4, block_size=8, device=device) for _ in range(2))
+    batch = ExecutionBatch((entry("a", 0, 11, (1, 3), np.random.default_rng(6), want=False),))
+    assert runner.execute_sampled(batch, [], temperature=[], top_k=[], top_p=[], min_p=[]) == {} == other.execute(batch)
+    assert runner.key_cache[:, 1].any() and runner.value_cache[:, 3, :3].any()
+    assert torch.equal(runner.key_cache, other.key_cache) and torch.equal(runner.value_cache, other.value_cache)

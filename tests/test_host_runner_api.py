@@ -40,3 +40,22 @@ def test_batch_entry_and_execution_batch_keep_the_reference_interface() -> None:
     for twin in (pickle.loads(pickle.dumps(batch)), copy.deepcopy(batch), copy.copy(batch)):
         assert twin == batch and hash(twin) == hash(batch)
     assert dataclasses.replace(decode, positions=(41,)).context_len == 42
+
+
+@pytest.mark.parametrize("settings", [
+    {}, {"top_k": []}, {"temperature": [], "top_k": [], "top_p": [], "min_p": []}, {"top_k": 5, "temperature": []},
+], ids=str)  # fmt: skip
+def test_a_sampled_step_without_logits_rows_takes_empty_settings_and_runs(settings) -> None:
+    """Chunks of unfinished prompts ask for no logits: lists with one entry per such row are empty, and the
+    step still runs, for its keys and values."""
+    from paged_kv_serving_amd.runner import ExecutionBatch, ModelRunner
+
+    ran = []
+    runner = object.__new__(ModelRunner)  # the settings are read before anything of the device
+    runner._forward = lambda batch: (ran.append(batch), ([], None))[1]
+    batch = ExecutionBatch((BatchEntry("a", (5, 6), (0, 1), (3,)),))
+    assert runner.execute_sampled(batch, [], **settings) == {} and ran == [batch]
+    for wrong in ({"top_k": [1]}, {"temperature": [1.0]}, {"top_k": 1.5}):
+        with pytest.raises(ValueError, match=next(iter(wrong))):
+            runner.execute_sampled(batch, [], **wrong)
+    assert len(ran) == 1
