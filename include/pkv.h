@@ -602,8 +602,8 @@ int pkv_rope_append_axes(const pkv_rope_axes* args, int device, void* stream);
  *                     how the call runs, never its result; rows of one sequence lying next to each
  *                     other are computed together from PKV_WINDOW_MIN_RUN on.
  *   num_splits      : workgroups that share a row's keys, 1 to PKV_WINDOW_MAX_SPLITS, or 0 for the
- *                     library's choice (pkv_window_splits).
- *   workspace       : float32 scratch of pkv_window_workspace_bytes(...) bytes, 16-byte aligned (may be
+ *                     library's choice.
+ *   workspace       : float32 scratch of the bytes that pkv_window_sizes gives, 16-byte aligned (may be
  *                     NULL when that is 0). Nothing in it needs to start at zero.
  * Rows of one sequence need not lie next to each other, nor in order. A row that sees no key gets
  * zeros. Block ids outside [0, num_blocks) at a visible position are skipped, as in
@@ -649,7 +649,14 @@ typedef struct pkv_window {
   float scale;
 } pkv_window;
 
-/* Splits the library chooses for a call with num_splits 0 (1 where nothing is split). Host-only. */
+/* The splits of a call (num_splits, or where that is 0 the library's choice) and its bytes of workspace. Host-only. */
+int32_t pkv_window_sizes(int64_t num_queries, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t q_dtype,
+                         int32_t window, int32_t sinks, int32_t max_context_len, int32_t max_query_len, int32_t num_splits,
+                         int64_t* workspace_bytes);
+
+/* The same in two steps, for all but float32 queries of head_dim 256: these have no rows that are computed
+ * together, so their splits are chosen as for as many rows by themselves and their workspace holds no list of rows.
+ * Splits the library chooses for a call with num_splits 0 (1 where nothing is split). Host-only. */
 int32_t pkv_window_splits(int64_t num_queries, int32_t num_heads, int32_t num_kv_heads, int32_t window,
                           int32_t sinks, int32_t max_context_len, int32_t max_query_len);
 

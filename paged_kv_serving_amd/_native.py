@@ -96,6 +96,7 @@ EXPORTED_SYMBOLS = (
     "pkv_sequence_metadata",
     "pkv_linear_forward",
     "pkv_rope_append_axes",
+    "pkv_window_sizes",
     "pkv_window_splits",
     "pkv_window_workspace_bytes",
     "pkv_window_attention",
@@ -213,9 +214,8 @@ def bound_host():
                          address(lib.hipEventCreateWithFlags), address(lib.hipEventRecord),
                          address(lib.hipEventSynchronize), address(lib.hipEventDestroy),
                          address(lib.pkv_append), address(lib.pkv_linear_forward),
-                         address(lib.pkv_rope_append_axes), address(lib.pkv_window_splits),
-                         address(lib.pkv_window_workspace_bytes), address(lib.pkv_window_attention),
-                         address(lib.pkv_sample_tokens))  # fmt: skip
+                         address(lib.pkv_rope_append_axes), address(lib.pkv_window_sizes),
+                         address(lib.pkv_window_attention), address(lib.pkv_sample_tokens))  # fmt: skip
                 _BOUND = True
     return ext
 
@@ -338,6 +338,11 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.pkv_linear_forward.restype = _c_int
     lib.pkv_rope_append_axes.argtypes = [_ptr, _c_int, _ptr]  # args, device, stream
     lib.pkv_rope_append_axes.restype = _c_int
+    lib.pkv_window_sizes.argtypes = [
+        _i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32,  # queries, heads, kv heads, head_dim, q dtype, window,
+        _ptr,  # sinks, max context, max query len, splits; int64* of the bytes
+    ]
+    lib.pkv_window_sizes.restype = _i32
     lib.pkv_window_splits.argtypes = [
         _i64, _i32, _i32, _i32, _i32, _i32, _i32,  # queries, heads, kv heads, window, sinks, max context, max query len
     ]

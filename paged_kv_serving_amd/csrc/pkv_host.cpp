@@ -59,7 +59,7 @@
 //   bind(plan_batch, paged_attention, paged_attention_append, copy_blocks, rms_norm, silu_mul,
 //        rope_append, memcpy_async[, gather_rows, greedy_tokens, get_device, set_device,
 //        event_create, event_record, event_synchronize, event_destroy, append, linear_forward,
-//        rope_append_axes, window_splits, window_workspace_bytes, window_attention, sample_tokens])
+//        rope_append_axes, window_sizes, window_attention, sample_tokens])
 //       Takes the addresses of those libpkv.so entry points (include/pkv.h), so the calls below
 //       reach the library without ctypes' per-argument conversions, and of hipMemcpyAsync,
 //       hipGetDevice, hipSetDevice and hipEventCreateWithFlags / Record / Synchronize / Destroy
@@ -98,9 +98,9 @@
 //       fields of their argument structs, then device and stream); returns the PKV_* code.
 //   one_device(*tensors) -> int
 //       The ordinal that get_device() of all of them gives (-1: on no device, or not on one).
-//   window_workspace(queries, heads, kv_heads, head_dim, window, sinks, max_context_len,
+//   window_workspace(queries, heads, kv_heads, head_dim, q_dtype, window, sinks, max_context_len,
 //        max_query_len, splits) -> (splits, bytes)
-//       pkv_window_splits where `splits` is 0, and pkv_window_workspace_bytes.
+//       pkv_window_sizes.
 //
 // Buffers are NumPy arrays passed through the buffer protocol (C-contiguous, of the stated
 // element type; writable where written); nothing here allocates Python-visible memory besides
@@ -847,8 +847,7 @@ decltype(&pkv_gather_rows) g_gather_rows = nullptr;
 decltype(&pkv_linear_forward) g_linear = nullptr;  // optional: null takes the library products
 decltype(&pkv_greedy_tokens) g_greedy_tokens = nullptr;
 decltype(&pkv_rope_append_axes) g_rope_axes = nullptr;
-decltype(&pkv_window_splits) g_window_splits = nullptr;
-decltype(&pkv_window_workspace_bytes) g_window_bytes = nullptr;
+decltype(&pkv_window_sizes) g_window_sizes = nullptr;
 decltype(&pkv_window_attention) g_window = nullptr;
 decltype(&pkv_sample_tokens) g_sample = nullptr;
 // hipGetDevice / hipSetDevice of the same runtime, by their C signatures.
@@ -907,11 +906,11 @@ PyObject* bind(PyObject*, PyObject* args) {
   unsigned long long plan, attention, attention_append, copy, norm, gate, rope, memcpy_async;
   unsigned long long gather_rows = 0, greedy = 0, get_device = 0, set_device = 0;
   unsigned long long event_create = 0, event_record = 0, event_synchronize = 0, event_destroy = 0, append = 0, linear = 0;
-  unsigned long long rope_axes = 0, window_splits = 0, window_bytes = 0, window = 0, sample = 0;
-  if (!PyArg_ParseTuple(args, "KKKKKKKK|KKKKKKKKKKKKKKK", &plan, &attention, &attention_append, &copy, &norm, &gate, &rope,
+  unsigned long long rope_axes = 0, window_sizes = 0, window = 0, sample = 0;
+  if (!PyArg_ParseTuple(args, "KKKKKKKK|KKKKKKKKKKKKKK", &plan, &attention, &attention_append, &copy, &norm, &gate, &rope,
                         &memcpy_async, &gather_rows, &greedy, &get_device, &set_device, &event_create,
-                        &event_record, &event_synchronize, &event_destroy, &append, &linear, &rope_axes, &window_splits,
-                        &window_bytes, &window, &sample)) {
+                        &event_record, &event_synchronize, &event_destroy, &append, &linear, &rope_axes, &window_sizes,
+                        &window, &sample)) {
     return nullptr;
   }
   if (plan == 0 || attention == 0 || attention_append == 0 || copy == 0 || norm == 0 || gate == 0 || rope == 0 ||
@@ -939,8 +938,7 @@ PyObject* bind(PyObject*, PyObject* args) {
   g_append = reinterpret_cast<decltype(g_append)>(static_cast<uintptr_t>(append));
   g_linear = reinterpret_cast<decltype(g_linear)>(static_cast<uintptr_t>(linear));
   g_rope_axes = reinterpret_cast<decltype(g_rope_axes)>(static_cast<uintptr_t>(rope_axes));
-  g_window_splits = reinterpret_cast<decltype(g_window_splits)>(static_cast<uintptr_t>(window_splits));
-  g_window_bytes = reinterpret_cast<decltype(g_window_bytes)>(static_cast<uintptr_t>(window_bytes));
+  g_window_sizes = reinterpret_cast<decltype(g_window_sizes)>(static_cast<uintptr_t>(window_sizes));
   g_window = reinterpret_cast<decltype(g_window)>(static_cast<uintptr_t>(window));
   g_sample = reinterpret_cast<decltype(g_sample)>(static_cast<uintptr_t>(sample));
   Py_RETURN_NONE;
@@ -1483,15 +1481,13 @@ PyObject* rope_append_axes(PyObject*, PyObject* const* args, Py_ssize_t count) {
 }
 
 PyObject* window_workspace(PyObject*, PyObject* const* args, Py_ssize_t count) {
-  int64_t queries = 0;
-  int32_t heads = 0, kv_heads = 0, dim = 0, window = 0, sinks = 0, context = 0, rows = 0, splits = 0;
+  int64_t queries = 0, bytes = -1;
+  int32_t heads = 0, kv_heads = 0, dim = 0, q_dtype = 0, window = 0, sinks = 0, context = 0, rows = 0, splits = 0;
   Reader r{args, count};
-  r(queries), r(heads), r(kv_heads), r(dim), r(window), r(sinks), r(context), r(rows), r(splits);
-  if (!r.done() || !bound(reinterpret_cast<const void*>(g_window_splits)) || !bound(reinterpret_cast<const void*>(g_window_bytes))) {
-    return nullptr;
-  }
-  if (splits == 0) splits = g_window_splits(queries, heads, kv_heads, window, sinks, context, rows);
-  return Py_BuildValue("iL", splits, static_cast<long long>(g_window_bytes(queries, heads, dim, rows, splits)));
+  r(queries), r(heads), r(kv_heads), r(dim), r(q_dtype), r(window), r(sinks), r(context), r(rows), r(splits);
+  if (!r.done() || !bound(reinterpret_cast<const void*>(g_window_sizes))) return nullptr;
+  splits = g_window_sizes(queries, heads, kv_heads, dim, q_dtype, window, sinks, context, rows, splits, &bytes);
+  return Py_BuildValue("iL", splits, static_cast<long long>(bytes));
 }
 
 PyObject* window_attention(PyObject*, PyObject* const* args, Py_ssize_t count) {

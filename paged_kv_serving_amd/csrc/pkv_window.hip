@@ -704,6 +704,10 @@ __global__ __launch_bounds__(kRowWaves * kPair * kWave) void row_kernel(const Wi
 // issue in 29% and LDS works in 20%, at two wavefronts per SIMD. One piece of P instead of two
 // was 9% faster.
 // ---------------------------------------------------------------------------------------------
+// float32 queries of head_dim 256 have no tiles (their pieces do not fit the registers, nor float32 pools' LDS): their
+// rows go by themselves.
+constexpr bool tiles_of(int q_size, int head_dim) { return q_size == 2 || head_dim <= 128; }
+
 template <typename QT, typename KVT, int D>
 struct TileShape {
   static constexpr int kQPieces = sizeof(QT) == 4 ? 3 : 1;
@@ -715,7 +719,8 @@ struct TileShape {
   static constexpr int kStaged = kKeys * kChunks / kThreads;           // chunks of a tile per thread, K and V each
   static constexpr int kLds = 2 * 2 * kKvPieces * kPlane * 2;          // bytes: two buffers of K and V
   static constexpr int kWaves = kLds <= 81920 && sizeof(QT) == 2 && D <= 128 ? 2 : 1;  // per SIMD
-  static constexpr bool kFits = kLds <= 160 * 1024 - 2048 && !(sizeof(QT) == 4 && D > 128);
+  static constexpr bool kFits = tiles_of(sizeof(QT), D);
+  static_assert(!kFits || kLds <= 160 * 1024 - 2048, "a tile's buffers, slots and live bits fit LDS");
 };
 
 // The products of pieces i of one operand and j of the other that are computed: i + j <= 2.
@@ -1227,7 +1232,7 @@ int launch(Window a, hipStream_t stream) {
   a.subgroups = (a.group + 15) / 16;
   a.tile_rows = kTileQueries / a.group;
   a.min_run = std::min(kMinRun, a.tile_rows);
-  a.tiled = S::kFits && a.list;
+  a.tiled = S::kFits && a.list;  // no list without tiles
   const int64_t items = a.num_queries * a.num_kv_heads * a.subgroups * a.splits;
   // Beside tiles the number of rows is known on the device only: two workgroups for every CU share them.
   const int64_t groups = a.tiled ? std::min<int64_t>(items, 512) : items;
@@ -1295,11 +1300,9 @@ namespace {
 // for every call that may have them: the workspace's size does not go by the heads' grouping).
 bool has_runs(int32_t max_query_len, int32_t group) { return max_query_len >= std::min(kMinRun, kTileQueries / group); }
 int64_t list_bytes(int64_t num_queries) { return (num_queries + 4) / 4 * 16; }
-}  // namespace
-}  // namespace pkv
 
-extern "C" int32_t pkv_window_splits(int64_t num_queries, int32_t num_heads, int32_t num_kv_heads, int32_t window,
-                                     int32_t sinks, int32_t max_context_len, int32_t max_query_len) {
+int32_t choose_splits(int64_t num_queries, int32_t num_heads, int32_t num_kv_heads, int32_t window, int32_t sinks,
+                      int32_t max_context_len, int32_t max_query_len, bool tiles) {
   if (num_queries < 0 || num_kv_heads < 1 || num_heads < num_kv_heads || num_heads % num_kv_heads != 0 || window < 1 ||
       sinks < 0 || max_context_len < 0 || max_query_len < 0) {
     return PKV_EINVAL;
@@ -1307,14 +1310,17 @@ extern "C" int32_t pkv_window_splits(int64_t num_queries, int32_t num_heads, int
   const int64_t longest = std::min<int64_t>(max_context_len, static_cast<int64_t>(window) + sinks);
   const int32_t group = num_heads / num_kv_heads;
   if (group > PKV_WINDOW_MAX_GROUP) return PKV_EINVAL;
-  const bool runs = pkv::has_runs(max_query_len, group);
-  const int64_t rows = runs ? pkv::kTileQueries / group : 1;
+  const bool runs = tiles && has_runs(max_query_len, group);
+  const int64_t rows = runs ? kTileQueries / group : 1;
   const int64_t groups = (num_queries + rows - 1) / rows * num_kv_heads * (runs ? 1 : (group + 15) / 16);
   // Tiles: two workgroups for every CU, 128 keys to a split at least. Rows: one workgroup of eight wavefronts for
   // every CU, 256 keys to a split, and one split below 1024 keys, which saves a launch. 8 key heads x 128, bfloat16,
   // with 1, 2, 4, 8, 16 splits: 1 row of 4096 keys 63, 38, 24, 18, 16 us, 4 rows 73, 44, 28, 21, 22, 16 rows 85, 56,
   // 51, 57, 69; 8 rows of 1024 keys 24, 18, 15, 15, 23; 1 row of 512 keys 12.4, 12.2, 11.3, 11.2, 12.3.
-  const int64_t fewest = runs ? 128 : longest < 1024 ? 1024 : 256;
+  // Rows without tiles have long key rows and four wavefronts: 128 keys to a split. Float32, 2 key heads x 256, with 1, 2, 4,
+  // 8, 16 splits: 5 rows of 2000 keys 116, 61, 36, 25, 20, of 300 keys 23.2, 19.6, 16.1, 13.9, 14.5, 512 rows of some 1450
+  // keys 265, 314, 397, 561, 858 (11 splits, as of tiles: 695; over bfloat16 168 and 600).
+  const int64_t fewest = runs || !tiles ? 128 : longest < 1024 ? 1024 : 256;
   const int64_t most = std::max<int64_t>(1, std::min<int64_t>(PKV_WINDOW_MAX_SPLITS, longest / fewest));
   int64_t want = runs ? (512 + groups - 1) / std::max<int64_t>(1, groups) : 256 / std::max<int64_t>(1, groups);
   // More workgroups than CUs, which would leave many of them idle at the end: up to four splits of 1024 keys (8 key heads x
@@ -1324,6 +1330,13 @@ extern "C" int32_t pkv_window_splits(int64_t num_queries, int32_t num_heads, int
   if (!runs && groups > 256 && groups * 20 < round * 17) want = std::min<int64_t>(4, longest / 1024);
   return static_cast<int32_t>(std::max<int64_t>(1, std::min(most, want)));
 }
+}  // namespace
+}  // namespace pkv
+
+extern "C" int32_t pkv_window_splits(int64_t num_queries, int32_t num_heads, int32_t num_kv_heads, int32_t window,
+                                     int32_t sinks, int32_t max_context_len, int32_t max_query_len) {
+  return pkv::choose_splits(num_queries, num_heads, num_kv_heads, window, sinks, max_context_len, max_query_len, true);
+}
 
 extern "C" int64_t pkv_window_workspace_bytes(int64_t num_queries, int32_t num_heads, int32_t head_dim, int32_t max_query_len,
                                               int32_t num_splits) {
@@ -1332,6 +1345,23 @@ extern "C" int64_t pkv_window_workspace_bytes(int64_t num_queries, int32_t num_h
   }
   const int64_t parts = num_splits == 1 ? 0 : num_queries * num_heads * num_splits * (head_dim + 2) * static_cast<int64_t>(sizeof(float));
   return (parts + 15) / 16 * 16 + (max_query_len > 1 ? pkv::list_bytes(num_queries) : 0);
+}
+
+extern "C" int32_t pkv_window_sizes(int64_t num_queries, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                    int32_t q_dtype, int32_t window, int32_t sinks, int32_t max_context_len,
+                                    int32_t max_query_len, int32_t num_splits, int64_t* workspace_bytes) {
+  const int size = pkv::dtype_size(static_cast<pkv_dtype>(q_dtype));
+  if (size == 0 || !workspace_bytes || num_splits < 0) return PKV_EINVAL;
+  const bool tiles = pkv::tiles_of(size, head_dim);
+  const int32_t splits = num_splits > 0 ? num_splits
+                                        : pkv::choose_splits(num_queries, num_heads, num_kv_heads, window, sinks, max_context_len,
+                                                             max_query_len, tiles);
+  if (splits < 1) return PKV_EINVAL;
+  // Without tiles there is no list of the rows outside them.
+  const int64_t need = pkv_window_workspace_bytes(num_queries, num_heads, head_dim, tiles ? max_query_len : 0, splits);
+  if (need < 0) return PKV_EINVAL;
+  *workspace_bytes = need;
+  return splits;
 }
 
 extern "C" int pkv_window_attention(const pkv_window* args, int device, void* stream) {
@@ -1361,11 +1391,12 @@ extern "C" int pkv_window_attention(const pkv_window* args, int device, void* st
       !aligned16(g.key_cache) || !aligned16(g.value_cache)) {
     return PKV_EINVAL;
   }
-  const int32_t splits = g.num_splits > 0 ? g.num_splits
-                                          : pkv_window_splits(g.num_queries, g.num_heads, g.num_kv_heads, g.window, g.sinks,
-                                                              g.max_context_len, g.max_query_len);
-  const int64_t need = pkv_window_workspace_bytes(g.num_queries, g.num_heads, g.head_dim, g.max_query_len, splits);
-  const bool runs = has_runs(g.max_query_len, g.num_heads / g.num_kv_heads);
+  const bool tiles = tiles_of(dtype_size(static_cast<pkv_dtype>(g.q_dtype)), g.head_dim);
+  const bool runs = tiles && has_runs(g.max_query_len, g.num_heads / g.num_kv_heads);
+  int64_t need = 0;
+  const int32_t splits = pkv_window_sizes(g.num_queries, g.num_heads, g.num_kv_heads, g.head_dim, g.q_dtype, g.window, g.sinks,
+                                          g.max_context_len, g.max_query_len, g.num_splits, &need);
+  if (splits < 1) return PKV_EINVAL;
   if (need > 0 && (!g.workspace || !aligned16(g.workspace) || g.workspace_bytes < need)) return PKV_EINVAL;
   Window a{};
   a.out = g.out;

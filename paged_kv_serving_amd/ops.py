@@ -1535,7 +1535,7 @@ def paged_attention_window(
     window, sinks = min(window, _INT32_MAX), min(sinks, _INT32_MAX)
     rows = num_queries if max_query_len is None else min(max_query_len, _INT32_MAX)
     host = _host()
-    splits, need = host.window_workspace(num_queries, heads, kv_heads, dim, window, sinks, max_context_len, rows, num_splits)
+    splits, need = host.window_workspace(num_queries, heads, kv_heads, dim, q_code, window, sinks, max_context_len, rows, num_splits)
     if need:
         if workspace is None:
             workspace = context_lens.new_empty((need // 4,))  # no values yet: four bytes an entry
@@ -1557,12 +1557,15 @@ def window_workspace_bytes(
     num_queries: int, heads: int, kv_heads: int, head_dim: int, *, window: int, sinks: int = 0,
     max_context_len: int, max_query_len: int | None = None, num_splits: int = 0,
 ) -> int:  # fmt: skip
-    """Bytes of float32 workspace :func:`paged_attention_window` needs for these sizes."""
+    """Bytes of float32 workspace :func:`paged_attention_window` needs for these sizes, whatever its types."""
     rows = num_queries if max_query_len is None else max_query_len
-    splits, need = _host().window_workspace(
-        num_queries, heads, kv_heads, head_dim, min(window, _INT32_MAX), min(sinks, _INT32_MAX), max_context_len,
-        min(rows, _INT32_MAX), num_splits,
-    )  # fmt: skip
-    if splits < 1 or need < 0:
+    sizes = [
+        _host().window_workspace(
+            num_queries, heads, kv_heads, head_dim, code, min(window, _INT32_MAX), min(sinks, _INT32_MAX),
+            max_context_len, min(rows, _INT32_MAX), num_splits,
+        )
+        for code in _DTYPE_CODES.values()
+    ]  # fmt: skip
+    if any(splits < 1 or need < 0 for splits, need in sizes):
         raise ValueError("invalid window workspace query")
-    return int(need)
+    return max(need for _, need in sizes)

@@ -451,3 +451,14 @@ def test_outputs_past_32_bits(device):
         part = out[start : start + (1 << 14)].float()
         at = positions[start : start + (1 << 14)].long()
         assert ((part >= low[at][:, None]) & (part <= high[at][:, None])).all(), start
+
+
+@pytest.mark.parametrize("kv", ["float32", "bfloat16"])
+def test_float32_rows_of_256_need_no_list_of_rows(device, kv):
+    """Rows that no tile computes together: a run needs no workspace of its own."""
+    import torch
+
+    d = make([(60, 300), (1, 40), (20, 20)], 6, 2, 256, 16, "float32", kv)
+    check(device, d, 100, 3, num_splits=1, workspace=torch.empty(0, device=device))
+    check(device, d, 100, 3, num_splits=2, workspace=torch.empty(81 * 6 * 2 * 258, device=device))
+    check(device, d, 5000, 3)

@@ -150,3 +150,37 @@ def test_tensors_off_the_device_are_refused_by_name(lib) -> None:
     assert host.one_device(f, i32) == host.one_device() == -1
     with pytest.raises(AttributeError):
         host.one_device(3)
+
+
+def test_float32_rows_of_256_are_split_as_rows_by_themselves(lib) -> None:
+    """No tile computes them together, so the splits are those of so many rows, and no list of rows is kept."""
+    host = _native.bound_host()
+    sizes = lambda rows, dim, dtype, splits=0, n=512: host.window_workspace(n, 8, 2, dim, dtype, 4096, 0, 2512, rows, splits)  # noqa: E731
+    assert sizes(512, 256, 0) == sizes(1, 256, 0) == (1, 0)  # 1024 workgroups of one row each fill the CUs
+    assert sizes(512, 256, 1)[0] == sizes(512, 128, 0)[0] == lib.pkv_window_splits(512, 8, 2, 4096, 0, 2512, 512) == 16
+    assert sizes(512, 256, 0, 3) == (3, 512 * 8 * 3 * 258 * 4)
+    assert sizes(5, 256, 0, n=5)[0] == 19  # few of them: 128 keys to a split
+    for dim, dtype in ((32, 0), (64, 1), (128, 0), (128, 1), (256, 1)):
+        for rows, splits in ((1, 0), (512, 0), (512, 5)):
+            got = sizes(rows, dim, dtype, splits)
+            assert got[0] == (splits or lib.pkv_window_splits(512, 8, 2, 4096, 0, 2512, rows))
+            assert got[1] == lib.pkv_window_workspace_bytes(512, 8, dim, rows, got[0])
+    bytes_out = ctypes.c_int64()
+    for changes in ({0: -1}, {1: 7}, {2: 0}, {3: 0}, {4: 2}, {5: 0}, {6: -1}, {7: -1}, {8: -1}, {9: -1}, {9: 65}, {10: None}):
+        args = [512, 8, 2, 256, 0, 4096, 0, 2512, 512, 0, ctypes.byref(bytes_out)]
+        for place, value in changes.items():
+            args[place] = value
+        assert lib.pkv_window_sizes(*args) == EINVAL, changes
+
+
+def test_workspace_bytes_serve_every_type(lib) -> None:
+    from paged_kv_serving_amd import ops
+
+    host = _native.bound_host()
+    for rows, heads, kv_heads in ((512, 8, 2), (30, 45, 1), (700, 45, 1), (1, 8, 8)):
+        for dim in (128, 256):
+            need = ops.window_workspace_bytes(rows, heads, kv_heads, dim, window=9000, max_context_len=8192)
+            each = [host.window_workspace(rows, heads, kv_heads, dim, code, 9000, 0, 8192, rows, 0)[1] for code in (0, 1)]
+            assert need == max(each)
+    with pytest.raises(ValueError):
+        ops.window_workspace_bytes(3, 5, 2, 64, window=9, max_context_len=8)
