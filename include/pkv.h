@@ -599,8 +599,9 @@ int pkv_rope_append_axes(const pkv_rope_axes* args, int device, void* stream);
  *                     max_context_len (checked).
  *   context_lens    : int32 [num_seqs]; visible lengths are clamped to max_context_len.
  *   max_query_len   : an upper bound of the rows that one sequence has next to each other. It chooses
- *                     how the call runs, never its result; rows of one sequence lying next to each
- *                     other are computed together from PKV_WINDOW_MIN_RUN on.
+ *                     how the call runs, and with that the roundings of its result, but not what it
+ *                     computes; rows of one sequence lying next to each other are computed together
+ *                     from PKV_WINDOW_MIN_RUN on (two or three where a tile of 128 queries has room for no more).
  *   num_splits      : workgroups that share a row's keys, 1 to PKV_WINDOW_MAX_SPLITS, or 0 for the
  *                     library's choice.
  *   workspace       : float32 scratch of the bytes that pkv_window_sizes gives, 16-byte aligned (may be

@@ -1477,11 +1477,12 @@ def paged_attention_window(
     was. ``window`` of at least the context is plain causal attention.
 
     ``max_query_len`` (default: T) bounds how many rows one sequence has next to each other: 1 for
-    a decode batch. With ``num_splits`` (default: the library's choice) it only decides how the call
-    runs. ``workspace``: float32 scratch of :func:`window_workspace_bytes` bytes, allocated when None;
+    a decode batch. With ``num_splits`` (default: the library's choice) it decides how the call
+    runs, which changes its result by roundings alone: scores, softmax and sums are float32 and the result
+    is rounded once, but runs of bfloat16 rows multiply their values by weights of 16 bits.
+    ``workspace``: float32 scratch of :func:`window_workspace_bytes` bytes, allocated when None;
     calls that may run at the same time need their own. ``out`` must not overlap an input. Returns
-    ``[T, heads, head_dim]`` of the queries' dtype: scores, softmax and sums are float32 and the result is
-    rounded once, but runs of bfloat16 rows multiply their values by weights of 16 bits. The call needs no plan and no host reading of the
+    ``[T, heads, head_dim]`` of the queries' dtype. The call needs no plan and no host reading of the
     batch, so it can be captured into a graph whose batch changes from replay to replay (within T, S,
     ``max_context_len`` and ``max_query_len``).
     """

@@ -462,3 +462,17 @@ def test_float32_rows_of_256_need_no_list_of_rows(device, kv):
     check(device, d, 100, 3, num_splits=1, workspace=torch.empty(0, device=device))
     check(device, d, 100, 3, num_splits=2, workspace=torch.empty(81 * 6 * 2 * 258, device=device))
     check(device, d, 5000, 3)
+
+
+@pytest.mark.parametrize("io,kv", TYPES)
+@pytest.mark.parametrize("heads,least", [(2, 4), (8, 4), (128, 2)])
+@pytest.mark.parametrize("splits", [0, 1, 3])
+def test_hints_choose_between_two_ways_to_run(device, io, kv, heads, least, splits):
+    """Below the shortest run that is computed together any max_query_len gives the same bits, and so does any from
+    it on; the two ways agree within the roundings of both."""
+    d = make([(1, 90), (1, 30), (50, 200), (3, 70)], heads, 2, 64, 16, io, kv, seed=heads)
+    below = [check(device, d, 40, 2, max_query_len=hint, num_splits=splits) for hint in range(least)]
+    above = [check(device, d, 40, 2, max_query_len=hint, num_splits=splits) for hint in (least, 50, 10_000)]
+    for same in (below, above):
+        for other in same[1:]:
+            np.testing.assert_array_equal(other, same[0])
