@@ -476,3 +476,51 @@ def test_hints_choose_between_two_ways_to_run(device, io, kv, heads, least, spli
     for same in (below, above):
         for other in same[1:]:
             np.testing.assert_array_equal(other, same[0])
+
+
+@pytest.mark.parametrize("io,kv", TYPES)
+def test_large_scores_keep_the_definition(device, io, kv):
+    """Scores of hundreds: within the bound, which their size widens to a part of the values."""
+    d = make([(1, 120), (40, 120)], 4, 2, 64, 16, io, kv, scale_k=300.0)
+    check(device, d, 50, 2)
+    check(device, d, 50, 2, num_splits=3)
+
+
+@pytest.mark.parametrize("io,kv", TYPES)
+@pytest.mark.parametrize("dim", [32, 128, 256])
+@pytest.mark.parametrize("splits", [1, 3])
+@pytest.mark.parametrize("key", [0, 61, 99])
+def test_a_key_far_above_the_others_is_the_output(device, io, kv, dim, splits, key):
+    """A score thousands above all others leaves these weights of 0, so the output is that key's value: exactly in
+    bfloat16, whose rounding hides the float32 ones; in float32 within those of a product, a reciprocal, another
+    product and, joined, two more."""
+    import torch
+
+    d = make([(1, 100), (30, 100), (1, 100)], 4, 2, dim, 16, io, kv, seed=key + dim)
+    d["positions"] = np.full(32, 99, np.int32)
+    axis = torch.zeros(dim)
+    axis[3] = 1.0
+    d["q"] = (d["q"].float() + 40 * axis).to(d["q"].dtype)
+    for s in range(3):
+        d["k"][d["tables"][s, key // 16], key % 16] = 400.0 * (dim / 32) ** 0.5 * axis
+    got = check(device, d, 200, 0, num_splits=splits)
+    want = np.stack([d["v"][d["tables"][s, key // 16], key % 16].double().numpy().repeat(2, 0) for s in d["seqs"]])
+    off = 0.0 if io == "bfloat16" else 8 * 2.0**-24 * np.abs(want)
+    assert (np.abs(got - want) <= off).all()
+
+
+@pytest.mark.parametrize("io,kv", TYPES)
+@pytest.mark.parametrize("dim", [32, 128, 256])
+@pytest.mark.parametrize("scale", [-0.2, 0.0, -0.0, 1e-30, -1e-30])
+def test_negative_and_vanishing_scales(device, io, kv, dim, scale):
+    """A negative scale turns the order of the scores, one of zero makes them all equal, and neither lets a hidden
+    key in: what is hidden holds infinities here."""
+    d = {**make([(1, 100), (40, 100), (1, 30), (1, 1)], 4, 2, dim, 16, io, kv, seed=dim), "scale": scale}
+    clean = call(device, d, 24, 3).float().cpu()
+    for s, hidden in ((0, (3, 40, 75)), (1, (3, 20, 36))):
+        for j in hidden:
+            d["k"][d["tables"][s, j // 16], j % 16] = float("inf")
+    for splits in (0, 3):
+        got = check(device, d, 24, 3, num_splits=splits)
+        if splits == 0:
+            np.testing.assert_array_equal(got, clean.numpy())
