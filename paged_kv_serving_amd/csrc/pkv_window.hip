@@ -86,13 +86,14 @@ __device__ __forceinline__ void store_row(T* p, const float (&v)[N]) {
   }
 }
 
-// The keys a row sees: [0, sinks) and [begin, end), or nothing.
-__device__ __forceinline__ uint32_t bits_between(int32_t low, int32_t high) {  // of [low, high) in 0 .. 31
+// Bits low .. high - 1 of a word, as far as it has them.
+__device__ __forceinline__ uint32_t bits_between(int32_t low, int32_t high) {
   low = max(low, 0);
   high = min(high, 32);
   return low < high ? (0xffffffffu >> (32 - (high - low))) << low : 0u;
 }
 
+// The keys a row sees: [0, sinks) and [begin, end), or nothing.
 struct Span {
   int32_t sinks, begin, end;
   __device__ __forceinline__ int32_t count() const { return sinks + end - begin; }
@@ -202,7 +203,7 @@ __device__ __forceinline__ void exact_row(const Window& a, int64_t t, int32_t he
     }
     const uint64_t seen = __ballot(slot >= 0);
     if (seen == 0) continue;
-    // A maximum that keeps NaN: a visible NaN score makes the row NaN.
+    // The maximum leaves a NaN out; a visible NaN score makes the row NaN by its weight.
     float next = score;
     for (int m = kWave / 2; m > 0; m >>= 1) next = fmaxf(next, __shfl_xor(next, m));
     next = fmaxf(top, next);
@@ -242,7 +243,7 @@ __device__ __forceinline__ void exact_row(const Window& a, int64_t t, int32_t he
 
 // ---------------------------------------------------------------------------------------------
 // Rows by themselves (decode): one workgroup per (row, key head, split) and up to 16 of the query
-// heads that share the key head. The row's keys are handed to the four wavefronts kKeys at a time.
+// heads that share the key head. The row's keys are handed to the wavefronts, four or eight, kKeys at a time.
 // With lane l = (c = l / 16, n = l % 16):
 //
 //   S^T = K Q^T    16 keys x 16 heads per product, K straight from the pool as the left operand: lane
@@ -584,7 +585,7 @@ __device__ __forceinline__ void row_pass(const Window& a, RowScratch<D, kRowWave
     }
     sum = column_sum(sum);
 
-    // The four wavefronts' results, lane by lane: every wavefront holds the same places.
+    // The wavefronts' results, lane by lane: every wavefront holds the same places.
     __syncthreads();  // the row before has been read
     s_top[side][wave][lane] = top;
     s_sum[side][wave][lane] = sum;
