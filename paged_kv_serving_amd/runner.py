@@ -32,6 +32,7 @@ before the append and attention of the step that scheduled them.
 from __future__ import annotations
 
 import hashlib
+import operator
 from dataclasses import dataclass
 
 import numpy as np
@@ -754,16 +755,23 @@ class ModelRunner:
         last position) appends inside the attention call.
 
         With ``window`` (and ``sinks``) a query at position p sees only the keys ``j > p - window`` or
-        ``j < sinks`` of those (:func:`ops.paged_attention_window`), after the append."""
+        ``j < sinks`` of those (:func:`ops.paged_attention_window`), after the append; ``out`` is 16-byte
+        aligned then."""
         config = self.model.config
         if not 0 <= layer < config.n_layers:
             raise IndexError(f"layer {layer} is outside the model's {config.n_layers} layers")
         if window is None and sinks:
             raise ValueError("sinks need a window")
-        if window is not None and (window < 1 or sinks < 0):
-            raise ValueError("window must be >= 1 and sinks >= 0")
-        if window is not None and config.head_dim not in ops.WINDOW_HEAD_DIMS:  # before anything is appended
-            raise ValueError(f"a window needs a head_dim of {ops.WINDOW_HEAD_DIMS}")
+        if window is not None:  # what the attention would refuse, before anything is appended
+            window, sinks = operator.index(window), operator.index(sinks)
+            if window < 1 or sinks < 0:
+                raise ValueError("window must be >= 1 and sinks >= 0")
+            if config.head_dim not in ops.WINDOW_HEAD_DIMS:
+                raise ValueError(f"a window needs a head_dim of {ops.WINDOW_HEAD_DIMS}")
+            if out is not None and out.data_ptr() % 16:
+                raise ValueError("out must be 16-byte aligned under a window")
+            if queries.data_ptr() % 16:
+                queries = queries.clone()
         step = self._prepare(batch, logits=False, plan=window is None)  # batch order without a plan
         total = 0 if step is None else step.total
         shape = (total, config.n_heads, config.head_dim)

@@ -262,3 +262,27 @@ def test_a_sampled_step_without_logits_rows_appends_its_keys_and_values(device, 
     assert runner.execute_sampled(batch, [], temperature=[], top_k=[], top_p=[], min_p=[]) == {} == other.execute(batch)
     assert runner.key_cache[:, 1].any() and runner.value_cache[:, 3, :3].any()
     assert torch.equal(runner.key_cache, other.key_cache) and torch.equal(runner.value_cache, other.value_cache)
+
+
+def test_attend_refuses_before_it_appends(device, model) -> None:
+    """What the windowed attention would refuse after the append is refused before it."""
+    runner = ModelRunner(model, num_blocks=4, block_size=8, device=device)
+    batch = ExecutionBatch((entry("a", 0, 3, (1,), np.random.default_rng(0)),))
+    rows = torch.ones((3, 2, 32), device=device)
+    for more in ({"window": 2.5}, {"window": 4, "sinks": 1.0}, {"window": "4"}):
+        with pytest.raises(TypeError):
+            runner.attend(batch, rows, rows, rows, **more)
+    odd = torch.zeros(3 * 2 * 32 + 1, device=device)[1:].view(3, 2, 32)
+    with pytest.raises(ValueError, match="16-byte"):
+        runner.attend(batch, rows, rows, rows, window=4, out=odd)
+    assert not runner.key_cache.any() and not odd.any()
+    assert runner.attend(batch, rows, rows, rows, window=np.int64(4), sinks=np.int32(1)).eq(1).all()
+
+
+def test_attend_with_a_window_takes_queries_at_any_address(device, model) -> None:
+    runner = ModelRunner(model, num_blocks=4, block_size=8, device=device)
+    batch = ExecutionBatch((entry("a", 0, 9, (1, 2), np.random.default_rng(0)),))
+    parts = [torch.randn(9 * 2 * 32 + 1, generator=torch.Generator().manual_seed(n)).to(device)[1:].view(9, 2, 32) for n in range(3)]
+    want = runner.attend(batch, *(part.clone() for part in parts), window=4)
+    runner.reset_cache()
+    assert parts[0].data_ptr() % 16 and torch.equal(runner.attend(batch, *parts, window=4), want)
