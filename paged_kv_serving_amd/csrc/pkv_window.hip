@@ -700,10 +700,12 @@ __global__ __launch_bounds__(kRowWaves * kPair * kWave) void row_kernel(const Wi
 // are in flight (bfloat16 pools: straight to LDS; float32 pools: to registers, cut on their way to LDS) and
 // the slots of the one after are looked up.
 //
-// Bound: latency. 8 x 512 rows behind 2048 others, window 1024, 32 heads on 8 x 128, bfloat16: 130 us, 530 TFLOP/s of visible
-// products (1390 in a large library product); the matrix units are busy 27% of it, vector instructions
-// issue in 29% and LDS works in 20%, at two wavefronts per SIMD. One piece of P instead of two
-// was 9% faster.
+// Bound: latency. 8 x 512 rows behind up to 2048 others, window 1024, bfloat16, 32 heads on 8 x 128: 126 us, 5 of
+// them the list's, 550 TFLOP/s of visible products (1390 in a large library product); x 64 91 us, 16 on 4 x 256 167.
+// Of the first's 304,000 cycles the matrix units are busy in 29%, vector instructions issue in 38% and LDS works in 21%,
+// at two wavefronts per SIMD: a step's values are waited for before its products. Float32 queries over bfloat16
+// 234 us (three products for one), over float32 438 (six, at one wavefront per SIMD). One piece of P instead of two was
+// 9% faster.
 // ---------------------------------------------------------------------------------------------
 // float32 queries of head_dim 256 have no tiles (their pieces do not fit the registers, nor float32 pools' LDS): their
 // rows go by themselves.
@@ -1258,8 +1260,8 @@ int launch(Window a, hipStream_t stream) {
       return check_launch();
     }
   }
-  // Few workgroups are of eight wavefronts (1 row, 2 key heads x 64, 516 keys: 9.1 -> 8.8 us; 24 rows of 1024 keys, 8 x
-  // 64, float32: 34 -> 27; 64 rows of 4100 keys 203 -> 208). head_dim 256 needs the registers of four, and so do float32
+  // Few workgroups are of eight wavefronts (24 rows of 1024 keys, 8 x 64, float32: 34 -> 27 us; 1 row, 2 key heads x 64,
+  // 516 keys, bfloat16: 9.4 and 9.5; 64 rows of 4100 keys 203 -> 208). head_dim 256 needs the registers of four, and so do float32
   // queries of head_dim 128 over bfloat16 keys (8 rows of 1024 keys, 32/8 heads: 20.4 us, 21.9 with eight). Where there
   // are many and a key row is short, one of eight serves two neighbouring key heads, and so reads twice as much next to
   // each other.
