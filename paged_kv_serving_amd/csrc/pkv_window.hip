@@ -315,7 +315,6 @@ __global__ __launch_bounds__(kListThreads) void list_kernel(const Window a) {
   if (threadIdx.x == 0) s_found = 0;
   __syncthreads();
   const int lane = threadIdx.x & (kWave - 1);
-#pragma unroll 2
   for (int64_t start = threadIdx.x - lane; start < a.num_queries; start += kListThreads) {
     const int64_t t = min(start + lane, a.num_queries - 1);
     const int32_t seq = a.seqs[t];
@@ -1261,10 +1260,10 @@ int launch(Window a, hipStream_t stream) {
     }
   }
   // Few workgroups are of eight wavefronts (24 rows of 1024 keys, 8 x 64, float32: 34 -> 27 us; 1 row, 2 key heads x 64,
-  // 516 keys, bfloat16: 9.4 and 9.5; 64 rows of 4100 keys 203 -> 208). head_dim 256 needs the registers of four, and so do float32
-  // queries of head_dim 128 over bfloat16 keys (8 rows of 1024 keys, 32/8 heads: 20.4 us, 21.9 with eight). Where there
-  // are many and a key row is short, one of eight serves two neighbouring key heads, and so reads twice as much next to
-  // each other.
+  // 516 keys, bfloat16: 9.4 and 9.5; 64 rows of 4100 keys 203 -> 208). head_dim 256 needs the registers of four, and so do
+  // float32 queries of head_dim 128 over bfloat16 keys (8 rows of 1024 keys, 32/8 heads: 20.4 us, 21.9 with eight). Where
+  // there are many and a key row is short, one of eight serves two neighbouring key heads, and so reads twice as much next
+  // to each other.
   constexpr bool kShort = D * sizeof(KVT) <= 256;
   constexpr bool kWide = D < 128 || (D == 128 && sizeof(QT) == sizeof(KVT));
   const bool wide = kWide && groups <= 256;
