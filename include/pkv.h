@@ -714,6 +714,90 @@ typedef struct pkv_sample {
 
 int pkv_sample_tokens(const pkv_sample* args, int device, void* stream);
 
+/*
+ * The append to a cache held in 8 bits: e4m3 codes (4 exponent and 3 mantissa bits, up to 448, the "fn" form without
+ * infinities) with a scale for each block of tokens and head, a power of two. A cached value is its code times its
+ * block's scale, which bfloat16 holds exactly.
+ *     scale[block, head] = the smallest power of two s >= 2^-100 with |x| <= 448 s for the tokens x that the call
+ *                          writes to the block, or what the block's scale is already, where that is more and the
+ *                          block has tokens before them
+ *     pool[slot, head]   = e4m3(x / scale), to nearest, ties to even
+ * and, where a block's scale grows, the codes of its tokens before the first that the call writes: e4m3(code * old / new),
+ * exact but for codes that fall below 2^-6. A block is filled in the order of its places: what lies behind the first place
+ * that a call writes, and in a block that is written from its first place on its old scale, counts as gone.
+ *
+ * No counterpart in the reference, whose cache is float32 (src/paged_kv_serving/engine/runner.py:112-114, 195-196).
+ *
+ *   key_pool, value_pool     : e4m3 [num_blocks, block_size, num_kv_heads, head_dim], 16-byte aligned.
+ *   key_scales, value_scales : float32 [num_blocks, num_kv_heads].
+ *   keys, values             : src_dtype rows [num_kv_heads, head_dim] with token strides.
+ *   slot_mapping             : int64 [num_tokens]; a slot outside the pool (padding: -1) is skipped.
+ * The tokens of one block have to stand next to each other in the call, as a batch's slots do; where they do not, or where a
+ * slot is named twice, that block's contents and scales are unspecified. A value that is not finite becomes NaN and counts
+ * nothing for the scale. The same inputs give the same bits. Supported: head_dim 32, 64, 128, 256, fewer than 2^31 slots.
+ */
+typedef struct pkv_e4m3_append {
+  void* key_pool;
+  void* value_pool;
+  float* key_scales;
+  float* value_scales;
+  const void* keys;
+  const void* values;
+  int64_t key_token_stride;
+  int64_t value_token_stride;
+  const int64_t* slot_mapping;
+  int64_t num_tokens;
+  int64_t num_blocks;
+  int32_t src_dtype;
+  int32_t block_size;
+  int32_t num_kv_heads;
+  int32_t head_dim;
+} pkv_e4m3_append;
+
+int pkv_append_e4m3(const pkv_e4m3_append* args, int device, void* stream);
+
+/*
+ * pkv_window_attention over a cache held in 8 bits, as pkv_append_e4m3 writes it.
+ *
+ *   key_cache, value_cache   : e4m3 codes [num_blocks, block_size, num_kv_heads, head_dim], 16-byte aligned.
+ *   key_scales, value_scales : float32 [num_blocks, num_kv_heads], powers of two from 2^-100 to 2^120. Of another
+ *                              number its exponent alone counts.
+ * All else is pkv_window's: a window of INT32_MAX is plain causal attention, and pkv_window_sizes gives the splits and the
+ * workspace. Queries are float32 or bfloat16. A NaN code (127, 255) is a NaN to the rows that see it.
+ */
+typedef struct pkv_e4m3_attention {
+  void* out;
+  const void* queries;
+  int64_t query_token_stride;
+  const int32_t* query_positions;
+  const int32_t* query_seq;
+  int64_t num_queries;
+  const void* key_cache;
+  const void* value_cache;
+  const float* key_scales;
+  const float* value_scales;
+  int64_t num_blocks;
+  const int32_t* block_tables;
+  const int32_t* context_lens;
+  float* workspace;
+  int64_t workspace_bytes;
+  int32_t q_dtype;
+  int32_t block_size;
+  int32_t block_table_stride;
+  int32_t num_seqs;
+  int32_t num_heads;
+  int32_t num_kv_heads;
+  int32_t head_dim;
+  int32_t window;
+  int32_t sinks;
+  int32_t max_context_len;
+  int32_t max_query_len;
+  int32_t num_splits;
+  float scale;
+} pkv_e4m3_attention;
+
+int pkv_attention_e4m3(const pkv_e4m3_attention* args, int device, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

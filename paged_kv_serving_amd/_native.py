@@ -39,7 +39,7 @@ LIB_PATH = PACKAGE_DIR / "libpkv.so"
 SOURCES = (
     CSRC / "pkv_copy.hip", CSRC / "pkv_rope.hip", CSRC / "pkv_attention.hip", CSRC / "pkv_sample.hip",
     CSRC / "pkv_plan.hip", CSRC / "pkv_model.hip", CSRC / "pkv_linear.hip", CSRC / "pkv_rope_axes.hip",
-    CSRC / "pkv_window.hip", CSRC / "pkv_sampling.hip",
+    CSRC / "pkv_window.hip", CSRC / "pkv_sampling.hip", CSRC / "pkv_e4m3.hip",
 )
 
 # gfx950 only. Packed-FP32 VALU instructions are disabled: the code relies on scalar fp32 FMA.
@@ -101,6 +101,8 @@ EXPORTED_SYMBOLS = (
     "pkv_window_workspace_bytes",
     "pkv_window_attention",
     "pkv_sample_tokens",
+    "pkv_append_e4m3",
+    "pkv_attention_e4m3",
 )
 
 
@@ -193,8 +195,8 @@ def bound_host():
     """:func:`host` with the library's entry points bound into it (``_pkvhost.bind``), so its
     ``plan``, ``paged_attention``, ``paged_attention_append``, ``copy_blocks``, ``rms_norm``,
     ``silu_mul``, ``rope_append``, ``append``, ``rope_append_axes``, ``window_workspace``,
-    ``window_attention``, ``sample_tokens``, ``forward`` and ``CopyQueue.flush`` call ``libpkv.so``
-    directly, and ``stage``, ``forward``, ``CopyQueue.flush`` and ``event_create`` call the
+    ``window_attention``, ``sample_tokens``, ``append_e4m3``, ``attention_e4m3``, ``forward`` and
+    ``CopyQueue.flush`` call ``libpkv.so`` directly, and ``stage``, ``forward``, ``CopyQueue.flush`` and ``event_create`` call the
     ``hipMemcpyAsync`` / ``hipGetDevice`` / ``hipSetDevice`` / ``hipEvent*`` functions of the HIP
     runtime ``libpkv.so`` is linked against (looked up through the library's handle, so they are
     that runtime's). Binding loads the library (it must be built)."""
@@ -215,7 +217,8 @@ def bound_host():
                          address(lib.hipEventSynchronize), address(lib.hipEventDestroy),
                          address(lib.pkv_append), address(lib.pkv_linear_forward),
                          address(lib.pkv_rope_append_axes), address(lib.pkv_window_sizes),
-                         address(lib.pkv_window_attention), address(lib.pkv_sample_tokens))  # fmt: skip
+                         address(lib.pkv_window_attention), address(lib.pkv_sample_tokens),
+                         address(lib.pkv_append_e4m3), address(lib.pkv_attention_e4m3))  # fmt: skip
                 _BOUND = True
     return ext
 
@@ -353,6 +356,10 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.pkv_window_attention.restype = _c_int
     lib.pkv_sample_tokens.argtypes = [_ptr, _c_int, _ptr]  # args, device, stream
     lib.pkv_sample_tokens.restype = _c_int
+    lib.pkv_append_e4m3.argtypes = [_ptr, _c_int, _ptr]  # args, device, stream
+    lib.pkv_append_e4m3.restype = _c_int
+    lib.pkv_attention_e4m3.argtypes = [_ptr, _c_int, _ptr]  # args, device, stream
+    lib.pkv_attention_e4m3.restype = _c_int
 
 
 def library() -> ctypes.CDLL:

@@ -1,0 +1,239 @@
+// The append to a paged cache of 8-bit floats (e4m3: 4 exponent and 3 mantissa bits, up to 448) with a power of two as
+// the scale of each block of tokens and head: a value is its code times its block's scale.
+#include "pkv_common.h"
+
+namespace pkv {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kHeld = 16;           // tokens whose values a wavefront holds between their maximum and their codes
+constexpr int kLowExponent = -100;  // of a scale: far above where code times scale would leave bfloat16's normal numbers
+
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+struct Append {
+  uint8_t* pool[2];  // keys, values
+  float* scales[2];
+  const void* source[2];
+  int64_t stride[2];
+  int32_t aligned[2];  // 16-byte loads of the source rows
+  const int64_t* slots;
+  int64_t tokens;
+  int32_t num_slots, block_size, kv_heads, window;
+};
+
+// Eight adjacent values of a source row.
+struct Eight {
+  float v[8];
+};
+__device__ __forceinline__ Eight load_eight(const float* p, bool aligned) {
+  Eight x;
+  if (aligned) {
+    const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x.v[i] = a[i], x.v[4 + i] = b[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x.v[i] = p[i];
+  }
+  return x;
+}
+__device__ __forceinline__ Eight load_eight(const uint16_t* p, bool aligned) {
+  Eight x;
+  if (aligned) {
+    const u32x4 a = *reinterpret_cast<const u32x4*>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x.v[2 * i] = bf16_lo(a[i]), x.v[2 * i + 1] = bf16_hi(a[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x.v[i] = __uint_as_float(static_cast<uint32_t>(p[i]) << 16);
+  }
+  return x;
+}
+
+// The codes of eight values times a power of two, rounded to nearest, ties to even. What is not finite becomes NaN.
+__device__ __forceinline__ u32x2 codes_of(const float (&v)[8], float times) {
+  u32x2 w;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    int x = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i] * times, v[4 * i + 1] * times, 0, false);
+    w[i] = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i + 2] * times, v[4 * i + 3] * times, x, true);
+  }
+  return w;
+}
+
+// The smallest power of two s of at least 2^kLowExponent with `most` <= 448 s = 1.75 * 2^8 s.
+__device__ __forceinline__ float scale_for(float most) {
+  const uint32_t bits = __float_as_uint(most);
+  const int exponent = static_cast<int>(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return __uint_as_float(static_cast<uint32_t>(max(exponent, kLowExponent) + 127) << 23);
+}
+
+// The block of a slot, -1 outside the pool.
+__device__ __forceinline__ int32_t block_of(const Append& a, int64_t slot) {
+  return slot < 0 || slot >= a.num_slots ? -1 : static_cast<int32_t>(static_cast<uint32_t>(slot) / static_cast<uint32_t>(a.block_size));
+}
+
+// ---------------------------------------------------------------------------------------------
+// A wavefront has the tokens of one block that stand next to each other in the call (a run), of one head, keys or
+// values: D / 8 lanes to a row. Their largest magnitude gives the scale; where the block has tokens before them and
+// its scale has to grow, their codes are multiplied by the ratio of the scales, a power of two, which is exact but
+// for codes that fall below 2^-6. No two wavefronts write the same block and head, so nothing waits for another.
+// Tokens' values are read once and held in registers (kHeld of them; longer runs are read twice, the second time
+// from the caches).
+// ---------------------------------------------------------------------------------------------
+template <typename T, int D>
+__device__ void append_run(const Append& a, int which, int32_t head, int64_t t0, int32_t block) {
+  constexpr int kLanes = D / 8, kRows = kWave / kLanes, kSteps = kHeld / kRows;
+  const int lane = threadIdx.x & (kWave - 1), row = lane / kLanes, d = lane % kLanes * 8;
+  const bool aligned = a.aligned[which];
+  const T* source = static_cast<const T*>(a.source[which]) + static_cast<int64_t>(head) * D + d;
+  uint8_t* pool = a.pool[which] + static_cast<int64_t>(head) * D + d;
+  const int64_t row_bytes = static_cast<int64_t>(a.kv_heads) * D;
+  float* scale_at = a.scales[which] + static_cast<int64_t>(block) * a.kv_heads + head;
+  const float held_scale = *scale_at;
+
+  // The run, and the first place of the block that it writes.
+  int64_t end = t0;
+  int64_t low = INT64_MAX;
+  for (;;) {
+    const int64_t t = end + lane;
+    const int64_t slot = t < a.tokens ? a.slots[t] : -1;
+    const uint64_t other = ~__ballot(block_of(a, slot) == block);
+    const int count = other == 0 ? kWave : __builtin_ctzll(other);
+    if (lane < count) low = min(low, slot);
+    end += count;
+    if (count < kWave) break;
+  }
+  for (int m = kWave / 2; m > 0; m >>= 1) low = min(low, static_cast<int64_t>(__shfl_xor(static_cast<long long>(low), m)));
+  const int64_t block0 = static_cast<int64_t>(block) * a.block_size;
+  const int32_t before = static_cast<int32_t>(low - block0);  // tokens that the block keeps
+
+  Eight x[kSteps];
+  float most = 0.f;
+  const auto load = [&](int64_t from) {
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      const int64_t t = min(from + i * kRows + row, end - 1);  // rows past the run repeat its last
+      x[i] = load_eight(source + t * a.stride[which], aligned);
+    }
+  };
+  for (int64_t from = t0; from < end; from += kHeld) {
+    load(from);
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float size = fabsf(x[i].v[e]);
+        most = fmaxf(most, size < INFINITY ? size : 0.f);
+      }
+    }
+  }
+  for (int m = kWave / 2; m > 0; m >>= 1) most = fmaxf(most, __shfl_xor(most, m));
+  float scale = scale_for(most);
+  if (before > 0) {
+    scale = fmaxf(scale, held_scale);
+    if (scale != held_scale) {
+      const float ratio = held_scale / scale;
+      for (int32_t r = row; r < before; r += kRows) {
+        u32x2* p = reinterpret_cast<u32x2*>(pool + (block0 + r) * row_bytes);
+        const u32x2 w = *p;
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          v[4 * i] = __builtin_amdgcn_cvt_f32_fp8(w[i], 0), v[4 * i + 1] = __builtin_amdgcn_cvt_f32_fp8(w[i], 1);
+          v[4 * i + 2] = __builtin_amdgcn_cvt_f32_fp8(w[i], 2), v[4 * i + 3] = __builtin_amdgcn_cvt_f32_fp8(w[i], 3);
+        }
+        *p = codes_of(v, ratio);
+      }
+    }
+  }
+  const float times = 1.f / scale;
+  for (int64_t from = t0; from < end; from += kHeld) {
+    if (end - t0 > kHeld) load(from);
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      const int64_t t = from + i * kRows + row;
+      if (t < end) *reinterpret_cast<u32x2*>(pool + a.slots[t] * row_bytes) = codes_of(x[i].v, times);
+    }
+  }
+  if (lane == 0) *scale_at = scale;
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads) void append_kernel(const Append a) {
+  // Items: keys and values of a head, heads, then windows of tokens, whose runs' first tokens a wavefront looks for.
+  const uint32_t item = __builtin_amdgcn_readfirstlane(blockIdx.x * (kThreads / kWave) + threadIdx.x / kWave);
+  const uint32_t columns = 2 * static_cast<uint32_t>(a.kv_heads);
+  const int which = item & 1;
+  const int32_t head = static_cast<int32_t>(item % columns / 2);
+  const int64_t t0 = static_cast<int64_t>(item / columns) * a.window;
+  if (t0 >= a.tokens) return;
+  const int lane = threadIdx.x & (kWave - 1);
+  const int64_t t = t0 + lane;
+  const bool mine = lane < a.window && t < a.tokens;
+  const int32_t block = mine ? block_of(a, a.slots[t]) : -1;
+  const int32_t last = mine && t > 0 ? block_of(a, a.slots[t - 1]) : -1;
+  for (uint64_t starts = __ballot(block >= 0 && block != last); starts != 0; starts &= starts - 1) {
+    const int at = __builtin_ctzll(starts);
+    append_run<T, D>(a, which, head, t0 + at, __builtin_amdgcn_readfirstlane(__shfl(block, at)));
+  }
+}
+
+int64_t groups_of(const Append& a) {
+  const int64_t items = (a.tokens + a.window - 1) / a.window * 2 * a.kv_heads;
+  return (items + kThreads / kWave - 1) / (kThreads / kWave);
+}
+
+template <typename T>
+int dispatch(const Append& a, int32_t head_dim, hipStream_t stream) {
+  const int64_t groups = groups_of(a);
+  const dim3 grid(static_cast<uint32_t>(groups)), block(kThreads);
+  switch (head_dim) {
+    case 32: hipLaunchKernelGGL((append_kernel<T, 32>), grid, block, 0, stream, a); break;
+    case 64: hipLaunchKernelGGL((append_kernel<T, 64>), grid, block, 0, stream, a); break;
+    case 128: hipLaunchKernelGGL((append_kernel<T, 128>), grid, block, 0, stream, a); break;
+    case 256: hipLaunchKernelGGL((append_kernel<T, 256>), grid, block, 0, stream, a); break;
+    default: return PKV_EUNSUPPORTED;
+  }
+  return check_launch();
+}
+
+}  // namespace
+}  // namespace pkv
+
+extern "C" int pkv_append_e4m3(const pkv_e4m3_append* args, int device, void* stream) {
+  using namespace pkv;
+  if (!args) return PKV_EINVAL;
+  const pkv_e4m3_append& g = *args;
+  if (g.num_tokens < 0 || g.num_blocks < 0 || g.block_size < 1 || g.num_kv_heads < 1) return PKV_EINVAL;
+  if (g.src_dtype != PKV_F32 && g.src_dtype != PKV_BF16) return PKV_EINVAL;
+  if (g.head_dim != 32 && g.head_dim != 64 && g.head_dim != 128 && g.head_dim != 256) return PKV_EUNSUPPORTED;
+  if (g.num_blocks > 0x7fffffff / g.block_size || g.num_kv_heads > (1 << 20) || g.num_tokens > 0x7fffffff) return PKV_EUNSUPPORTED;
+  if (g.num_tokens == 0) return PKV_OK;
+  if (!g.key_pool || !g.value_pool || !g.key_scales || !g.value_scales || !g.keys || !g.values || !g.slot_mapping) return PKV_EINVAL;
+  const int64_t row = static_cast<int64_t>(g.num_kv_heads) * g.head_dim;
+  if (g.key_token_stride < row || g.value_token_stride < row) return PKV_EINVAL;
+  const int size = dtype_size(static_cast<pkv_dtype>(g.src_dtype));
+  const auto aligned8 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0; };
+  if (!aligned8(g.key_pool) || !aligned8(g.value_pool)) return PKV_EINVAL;
+  Append a{};
+  a.pool[0] = static_cast<uint8_t*>(g.key_pool), a.pool[1] = static_cast<uint8_t*>(g.value_pool);
+  a.scales[0] = g.key_scales, a.scales[1] = g.value_scales;
+  a.source[0] = g.keys, a.source[1] = g.values;
+  a.stride[0] = g.key_token_stride, a.stride[1] = g.value_token_stride;
+  for (int i = 0; i < 2; ++i) a.aligned[i] = aligned16(a.source[i]) && a.stride[i] * size % 16 == 0;
+  a.slots = g.slot_mapping;
+  a.tokens = g.num_tokens;
+  a.num_slots = static_cast<int32_t>(g.num_blocks * g.block_size);
+  a.block_size = g.block_size;
+  a.kv_heads = g.num_kv_heads;
+  a.window = g.num_tokens * g.num_kv_heads <= 8192 ? 1 : 16;
+  if (groups_of(a) > 0x7fffffff / kThreads) return PKV_EUNSUPPORTED;
+  DeviceGuard guard(device);
+  if (!guard.ok()) return PKV_EHIP;
+  const auto s = static_cast<hipStream_t>(stream);
+  return g.src_dtype == PKV_F32 ? dispatch<float>(a, g.head_dim, s) : dispatch<uint16_t>(a, g.head_dim, s);
+}

@@ -59,7 +59,7 @@
 //   bind(plan_batch, paged_attention, paged_attention_append, copy_blocks, rms_norm, silu_mul,
 //        rope_append, memcpy_async[, gather_rows, greedy_tokens, get_device, set_device,
 //        event_create, event_record, event_synchronize, event_destroy, append, linear_forward,
-//        rope_append_axes, window_sizes, window_attention, sample_tokens])
+//        rope_append_axes, window_sizes, window_attention, sample_tokens, append_e4m3, attention_e4m3])
 //       Takes the addresses of those libpkv.so entry points (include/pkv.h), so the calls below
 //       reach the library without ctypes' per-argument conversions, and of hipMemcpyAsync,
 //       hipGetDevice, hipSetDevice and hipEventCreateWithFlags / Record / Synchronize / Destroy
@@ -92,7 +92,7 @@
 //       pkv_plan_batch on NumPy buffers; returns its PKV_* code.
 //   paged_attention(...), paged_attention_append(...), copy_blocks(...), rms_norm(...),
 //   silu_mul(...), rope_append(...), append(...), rope_append_axes(...), window_attention(...),
-//   sample_tokens(...) -> int
+//   sample_tokens(...), append_e4m3(...), attention_e4m3(...) -> int
 //       The entry points of the same names, with every pointer, stream and handle passed as a
 //       Python int (0 for NULL) in the order of their C declarations (the last three: of the
 //       fields of their argument structs, then device and stream); returns the PKV_* code.
@@ -850,6 +850,8 @@ decltype(&pkv_rope_append_axes) g_rope_axes = nullptr;
 decltype(&pkv_window_sizes) g_window_sizes = nullptr;
 decltype(&pkv_window_attention) g_window = nullptr;
 decltype(&pkv_sample_tokens) g_sample = nullptr;
+decltype(&pkv_append_e4m3) g_append_e4m3 = nullptr;
+decltype(&pkv_attention_e4m3) g_attention_e4m3 = nullptr;
 // hipGetDevice / hipSetDevice of the same runtime, by their C signatures.
 using GetDeviceFn = int (*)(int* device);
 using SetDeviceFn = int (*)(int device);
@@ -907,10 +909,11 @@ PyObject* bind(PyObject*, PyObject* args) {
   unsigned long long gather_rows = 0, greedy = 0, get_device = 0, set_device = 0;
   unsigned long long event_create = 0, event_record = 0, event_synchronize = 0, event_destroy = 0, append = 0, linear = 0;
   unsigned long long rope_axes = 0, window_sizes = 0, window = 0, sample = 0;
-  if (!PyArg_ParseTuple(args, "KKKKKKKK|KKKKKKKKKKKKKK", &plan, &attention, &attention_append, &copy, &norm, &gate, &rope,
+  unsigned long long append_codes = 0, attention_codes = 0;
+  if (!PyArg_ParseTuple(args, "KKKKKKKK|KKKKKKKKKKKKKKKK", &plan, &attention, &attention_append, &copy, &norm, &gate, &rope,
                         &memcpy_async, &gather_rows, &greedy, &get_device, &set_device, &event_create,
                         &event_record, &event_synchronize, &event_destroy, &append, &linear, &rope_axes, &window_sizes,
-                        &window, &sample)) {
+                        &window, &sample, &append_codes, &attention_codes)) {
     return nullptr;
   }
   if (plan == 0 || attention == 0 || attention_append == 0 || copy == 0 || norm == 0 || gate == 0 || rope == 0 ||
@@ -941,6 +944,8 @@ PyObject* bind(PyObject*, PyObject* args) {
   g_window_sizes = reinterpret_cast<decltype(g_window_sizes)>(static_cast<uintptr_t>(window_sizes));
   g_window = reinterpret_cast<decltype(g_window)>(static_cast<uintptr_t>(window));
   g_sample = reinterpret_cast<decltype(g_sample)>(static_cast<uintptr_t>(sample));
+  g_append_e4m3 = reinterpret_cast<decltype(g_append_e4m3)>(static_cast<uintptr_t>(append_codes));
+  g_attention_e4m3 = reinterpret_cast<decltype(g_attention_e4m3)>(static_cast<uintptr_t>(attention_codes));
   Py_RETURN_NONE;
 }
 
@@ -1516,6 +1521,34 @@ PyObject* sample_tokens(PyObject*, PyObject* const* args, Py_ssize_t count) {
   return PyLong_FromLong(g_sample(&a, device, stream));
 }
 
+PyObject* append_e4m3(PyObject*, PyObject* const* args, Py_ssize_t count) {
+  pkv_e4m3_append a{};
+  int32_t device = 0;
+  void* stream = nullptr;
+  Reader r{args, count};
+  r(a.key_pool), r(a.value_pool), r(a.key_scales), r(a.value_scales), r(a.keys), r(a.values), r(a.key_token_stride);
+  r(a.value_token_stride), r(a.slot_mapping), r(a.num_tokens), r(a.num_blocks), r(a.src_dtype), r(a.block_size);
+  r(a.num_kv_heads), r(a.head_dim);
+  r(device), r(stream);
+  if (!r.done() || !bound(reinterpret_cast<const void*>(g_append_e4m3))) return nullptr;
+  return PyLong_FromLong(g_append_e4m3(&a, device, stream));
+}
+
+PyObject* attention_e4m3(PyObject*, PyObject* const* args, Py_ssize_t count) {
+  pkv_e4m3_attention a{};
+  int32_t device = 0;
+  void* stream = nullptr;
+  Reader r{args, count};
+  r(a.out), r(a.queries), r(a.query_token_stride), r(a.query_positions), r(a.query_seq), r(a.num_queries), r(a.key_cache);
+  r(a.value_cache), r(a.key_scales), r(a.value_scales), r(a.num_blocks), r(a.block_tables), r(a.context_lens);
+  r(a.workspace), r(a.workspace_bytes), r(a.q_dtype), r(a.block_size), r(a.block_table_stride), r(a.num_seqs);
+  r(a.num_heads), r(a.num_kv_heads), r(a.head_dim), r(a.window), r(a.sinks), r(a.max_context_len), r(a.max_query_len);
+  r(a.num_splits), r(a.scale);
+  r(device), r(stream);
+  if (!r.done() || !bound(reinterpret_cast<const void*>(g_attention_e4m3))) return nullptr;
+  return PyLong_FromLong(g_attention_e4m3(&a, device, stream));
+}
+
 PyObject* append(PyObject*, PyObject* args) {
   unsigned long long kp, vp, k, v, slots, stream;
   long long nslots, k_stride, v_stride, tokens;
@@ -1887,6 +1920,10 @@ PyMethodDef kMethods[] = {
      "pkv_window_attention with integer pointers."},
     {"sample_tokens", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(sample_tokens)), METH_FASTCALL,
      "pkv_sample_tokens with integer pointers."},
+    {"append_e4m3", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(append_e4m3)), METH_FASTCALL,
+     "pkv_append_e4m3 with integer pointers."},
+    {"attention_e4m3", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(attention_e4m3)), METH_FASTCALL,
+     "pkv_attention_e4m3 with integer pointers."},
     {"stage", stage, METH_VARARGS, "Pack a call's metadata into pinned memory and copy it to the device."},
     {"forward", forward, METH_VARARGS, "One iteration's forward pass: rocBLAS products and the library's kernels."},
     {"event_create", event_create, METH_VARARGS, "A timing-free HIP event on a device, as an integer handle."},

@@ -5,6 +5,10 @@
 //     out = sum_j exp(s_j) v_j / sum_j exp(s_j),  s_j = scale * q . k_j
 // with an online softmax (running maximum and sum), everything in float32 and one rounding to the
 // output's type, but for the weights that a bfloat16 tile multiplies its values by (16 bits, at tile_kernel).
+//
+// A cache may hold e4m3 codes with a power of two as the scale of each block and head. A code times such a scale is a
+// bfloat16 number, so codes are widened on their way into the bfloat16 products, the scale being the conversion
+// instruction's own operand, and all else is as over a bfloat16 cache.
 #include <math.h>
 
 #include <algorithm>
@@ -56,10 +60,13 @@ struct Window {
   // A negative scale of bfloat16 queries turns their signs instead, so that the largest product is the
   // largest score; a zero one clears them, so that a hidden key's -inf stays what it is.
   uint32_t keep, flip;
+  const float* key_scales;  // of e4m3 codes, [num_blocks, num_kv_heads]; else NULL
+  const float* value_scales;
 };
 
 __device__ __forceinline__ float load_one(const float* p) { return *p; }
 __device__ __forceinline__ float load_one(const uint16_t* p) { return __uint_as_float(static_cast<uint32_t>(*p) << 16); }
+__device__ __forceinline__ float load_one(const uint8_t* p) { return __builtin_amdgcn_cvt_f32_fp8(*p, 0); }
 __device__ __forceinline__ void store_one(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store_one(uint16_t* p, float v) { *p = static_cast<uint16_t>(f32_to_bf16_bits(v)); }
 
@@ -76,11 +83,13 @@ __device__ __forceinline__ void store_row(T* p, const float (&v)[N]) {
     uint32_t w[N / 2];
 #pragma unroll
     for (int i = 0; i < N / 2; ++i) w[i] = f32_to_bf16_bits(v[2 * i]) | (f32_to_bf16_bits(v[2 * i + 1]) << 16);
-    if constexpr (N == 8) {
-      *reinterpret_cast<u32x4*>(p) = u32x4{w[0], w[1], w[2], w[3]};
+    if constexpr (N % 8 == 0) {
+#pragma unroll
+      for (int i = 0; i < N / 2; i += 4) *reinterpret_cast<u32x4*>(p + 2 * i) = u32x4{w[i], w[i + 1], w[i + 2], w[i + 3]};
     } else if constexpr (N == 4) {
       *reinterpret_cast<u32x2*>(p) = u32x2{w[0], w[1]};
     } else {
+      static_assert(N == 2, "two, four, or groups of eight");
       *reinterpret_cast<uint32_t*>(p) = w[0];
     }
   }
@@ -126,6 +135,17 @@ __device__ __forceinline__ int32_t slot_of(const Window& a, const int32_t* table
   const int32_t block = table[page];
   if (block < 0 || block >= a.num_blocks) return -1;
   return block * a.block_size + (key - static_cast<int32_t>(page) * a.block_size);
+}
+
+// Where the scale of a slot's block of one head lies.
+__device__ __forceinline__ int64_t scale_of(const Window& a, int32_t slot, int32_t kv_head) {
+  return static_cast<int64_t>(static_cast<uint32_t>(slot) / static_cast<uint32_t>(a.block_size)) * a.num_kv_heads + kv_head;
+}
+
+// Codes 0 and 1 of a word, or 2 and 3, as bfloat16 numbers times a power of two.
+template <int kHalf>
+__device__ __forceinline__ uint32_t widen(uint32_t codes, float scale) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, kHalf != 0));
 }
 
 // Element offset of a slot's row of one head in the pools.
@@ -200,6 +220,7 @@ __device__ __forceinline__ void exact_row(const Window& a, int64_t t, int32_t he
       score = 0.f;
       for (int d = 0; d < D; ++d) score += load_one(q + d) * load_one(k + d);
       score *= a.given_scale;
+      if constexpr (sizeof(KVT) == 1) score *= a.key_scales[scale_of(a, slot, kv_head)];
     }
     const uint64_t seen = __ballot(slot >= 0);
     if (seen == 0) continue;
@@ -217,8 +238,10 @@ __device__ __forceinline__ void exact_row(const Window& a, int64_t t, int32_t he
     for (int e = 0; e < kOwn; ++e) acc[e] *= keep;
     for (int j = 0; j < kWave; ++j) {
       if (!((seen >> j) & 1)) continue;
-      const float pj = __shfl(p, j);
-      const KVT* v = static_cast<const KVT*>(a.values) + row_of(a, __shfl(slot, j), kv_head, D);
+      float pj = __shfl(p, j);
+      const int32_t from_slot = __shfl(slot, j);
+      const KVT* v = static_cast<const KVT*>(a.values) + row_of(a, from_slot, kv_head, D);
+      if constexpr (sizeof(KVT) == 1) pj *= a.value_scales[scale_of(a, from_slot, kv_head)];
       for (int e = 0; e < kOwn; ++e) {
         const int d = e * kWave + lane;
         if (d < D) acc[e] += pj * load_one(v + d);
@@ -271,17 +294,22 @@ __device__ __forceinline__ void exact_row(const Window& a, int64_t t, int32_t he
 // ---------------------------------------------------------------------------------------------
 template <typename QT, typename KVT, int D>
 struct RowShape {
-  static constexpr bool kBf16 = sizeof(KVT) == 2;
+  static constexpr bool kCodes = sizeof(KVT) == 1;  // e4m3, widened to bfloat16
+  static constexpr bool kBf16 = sizeof(KVT) <= 2;   // the products
   static constexpr int kPieces = kBf16 ? (sizeof(QT) == 4 ? 3 : 1) : 1;
   static constexpr int kPPieces = 3;                         // of the weights, over bfloat16 values
   static constexpr int kBlocks = kBf16 && D <= 128 ? 2 : 1;  // 16-key blocks per round
   static constexpr int kKeys = 16 * kBlocks;
-  static constexpr int kKLoads = kBf16 ? D / 32 : D / 16;    // 16-byte loads of a key row per lane
+  static constexpr int kKSteps = D / 32;                     // products of 32 dimensions
+  static constexpr int kKWidth = kCodes && D == 32 ? 8 : 16;  // bytes of a load of a key row per lane
+  static constexpr int kKLoads = D * int(sizeof(KVT)) / (4 * kKWidth);
   static constexpr int kPerLane = D / 16;                    // values of a value row per lane
   static constexpr int kVWidth = kPerLane < 16 / int(sizeof(KVT)) ? kPerLane : 16 / int(sizeof(KVT));
   static constexpr int kVLoads = kPerLane / kVWidth;
-  static constexpr int kVWords = kVWidth * int(sizeof(KVT)) / 4;
-  static constexpr int kQRegs = kBf16 ? 4 * kKLoads * kPieces : D / 4;
+  static constexpr int kVWords = (kVWidth * int(sizeof(KVT)) + 3) / 4;
+  static constexpr int kQRegs = kBf16 ? 4 * kKSteps * kPieces : D / 4;
+  // The first of the 8 dimensions that lane group c has of step u.
+  __device__ static constexpr int dims(int u, int c) { return kCodes && D > 32 ? 64 * (u / 2) + 16 * c + 8 * (u % 2) : 32 * u + 8 * c; }
 };
 
 template <int N>
@@ -383,7 +411,7 @@ __device__ __forceinline__ void row_pass(const Window& a, RowScratch<D, kRowWave
     const auto* keys = static_cast<const char*>(a.keys);
     const auto* values = static_cast<const char*>(a.values);
     const int64_t row_bytes = static_cast<int64_t>(a.num_kv_heads) * D * sizeof(KVT);
-    const int64_t k_at = (static_cast<int64_t>(kv_head) * D + (S::kBf16 ? 8 : 4) * c) * sizeof(KVT);
+    const int64_t k_at = (static_cast<int64_t>(kv_head) * D + S::kKWidth / int(sizeof(KVT)) * c) * sizeof(KVT);
     const int64_t v_at = (static_cast<int64_t>(kv_head) * D + S::kVWidth * n) * sizeof(KVT);
     const int32_t seq = a.seqs[t];
     if (seq < 0 || seq >= a.num_seqs) continue;
@@ -400,19 +428,19 @@ __device__ __forceinline__ void row_pass(const Window& a, RowScratch<D, kRowWave
       const QT* q = static_cast<const QT*>(a.queries) + t * a.query_stride + static_cast<int64_t>(head0 + min(n, heads - 1)) * D;
       if constexpr (S::kBf16 && sizeof(QT) == 2) {
 #pragma unroll
-        for (int u = 0; u < S::kKLoads; ++u) {
-          const u32x4 x = *reinterpret_cast<const u32x4*>(q + 32 * u + 8 * c);
+        for (int u = 0; u < S::kKSteps; ++u) {
+          const u32x4 x = *reinterpret_cast<const u32x4*>(q + S::dims(u, c));
 #pragma unroll
           for (int e = 0; e < 4; ++e) qr[4 * u + e] = (x[e] & a.keep) ^ a.flip;
         }
       } else if constexpr (S::kBf16) {
 #pragma unroll
-        for (int u = 0; u < S::kKLoads; ++u) {
+        for (int u = 0; u < S::kKSteps; ++u) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            float x0 = q[32 * u + 8 * c + 2 * e] * a.scale_log2, x1 = q[32 * u + 8 * c + 2 * e + 1] * a.scale_log2;
+            float x0 = q[S::dims(u, c) + 2 * e] * a.scale_log2, x1 = q[S::dims(u, c) + 2 * e + 1] * a.scale_log2;
 #pragma unroll
-            for (int p = 0; p < 3; ++p) qr[4 * (p * S::kKLoads + u) + e] = take_piece(x0, x1);
+            for (int p = 0; p < 3; ++p) qr[4 * (p * S::kKSteps + u) + e] = take_piece(x0, x1);
           }
         }
       } else {
@@ -435,14 +463,24 @@ __device__ __forceinline__ void row_pass(const Window& a, RowScratch<D, kRowWave
       const int32_t i = round * S::kKeys + lane % S::kKeys;
       return round < last && i < count ? slot_of(a, table, span.key(i)) : -1;
     };
-    Words<4> kx[S::kBlocks][S::kKLoads];
+    // Of codes also the scales of that key's block, for its key and its value.
+    float key_scale = 1.f, value_scale = 1.f;  // of the round whose rows are loaded
+    auto look_up_scales = [&](int32_t slot) {
+      if constexpr (S::kCodes) {
+        const bool known = slot >= 0;  // elsewhere 1: code 0 times a NaN is not 0
+        const int64_t at = known ? scale_of(a, slot, kv_head) : 0;
+        key_scale = known ? a.key_scales[at] : 1.f;
+        value_scale = known ? a.value_scales[at] : 1.f;
+      }
+    };
+    Words<S::kKWidth / 4> kx[S::kBlocks][S::kKLoads];
     Words<S::kVWords> vx[S::kBlocks][4][S::kVLoads];
     auto load_keys = [&](int32_t slot) {
 #pragma unroll
       for (int j = 0; j < S::kBlocks; ++j) {
         const char* p = keys + max(__shfl(slot, 16 * j + n), 0) * row_bytes + k_at;
 #pragma unroll
-        for (int u = 0; u < S::kKLoads; ++u) kx[j][u] = load_words<4>(p + u * 64);
+        for (int u = 0; u < S::kKLoads; ++u) kx[j][u] = load_words<S::kKWidth / 4>(p + u * 4 * S::kKWidth);
       }
     };
     auto load_values = [&](int32_t slot) {
@@ -452,7 +490,13 @@ __device__ __forceinline__ void row_pass(const Window& a, RowScratch<D, kRowWave
         for (int r = 0; r < 4; ++r) {
           const char* p = values + max(__shfl(slot, 16 * j + 4 * c + r), 0) * row_bytes + v_at;
 #pragma unroll
-          for (int g = 0; g < S::kVLoads; ++g) vx[j][r][g] = load_words<S::kVWords>(p + g * 16 * S::kVWidth * int(sizeof(KVT)));
+          for (int g = 0; g < S::kVLoads; ++g) {
+            if constexpr (S::kVWidth * sizeof(KVT) == 2) {
+              vx[j][r][g].w[0] = __builtin_nontemporal_load(reinterpret_cast<const uint16_t*>(p));
+            } else {
+              vx[j][r][g] = load_words<S::kVWords>(p + g * 16 * S::kVWidth * int(sizeof(KVT)));
+            }
+          }
         }
       }
     };
@@ -462,6 +506,7 @@ __device__ __forceinline__ void row_pass(const Window& a, RowScratch<D, kRowWave
     int32_t slot = look_up(round);
     uint32_t live = static_cast<uint32_t>(__ballot(slot >= 0) & kAll);  // the round's keys that count
     if (live != 0) {
+      look_up_scales(slot);
       load_keys(slot);
       load_values(slot);
     }
@@ -473,16 +518,27 @@ __device__ __forceinline__ void row_pass(const Window& a, RowScratch<D, kRowWave
 #pragma unroll
         for (int j = 0; j < S::kBlocks; ++j) {
           st[j] = floatx4{0.f, 0.f, 0.f, 0.f};
+          if constexpr (S::kBf16) {
+            const float scale = S::kCodes ? __shfl(key_scale, 16 * j + n) : 1.f;  // of this lane's key
 #pragma unroll
-          for (int u = 0; u < S::kKLoads; ++u) {
-            if constexpr (S::kBf16) {
+            for (int u = 0; u < S::kKSteps; ++u) {
+              u32x4 k;
+              if constexpr (S::kCodes) {
+                const uint32_t* w = kx[j][D == 32 ? 0 : u / 2].w + (D == 32 ? 0 : u % 2 * 2);
+                k = u32x4{widen<0>(w[0], scale), widen<1>(w[0], scale), widen<0>(w[1], scale), widen<1>(w[1], scale)};
+              } else {
+                k = __builtin_bit_cast(u32x4, kx[j][u]);
+              }
 #pragma unroll
               for (int p = S::kPieces - 1; p >= 0; --p) {  // the smallest pieces first
-                const uint32_t* q = qr + 4 * (p * S::kKLoads + u);
-                st[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kx[j][u]),
+                const uint32_t* q = qr + 4 * (p * S::kKSteps + u);
+                st[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k),
                                                                 __builtin_bit_cast(bf16x8, (u32x4{q[0], q[1], q[2], q[3]})), st[j], 0, 0, 0);
               }
-            } else {
+            }
+          } else {
+#pragma unroll
+            for (int u = 0; u < S::kKLoads; ++u) {
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 st[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kx[j][u].w[e]), __uint_as_float(qr[4 * u + e]), st[j], 0, 0, 0);
@@ -491,7 +547,11 @@ __device__ __forceinline__ void row_pass(const Window& a, RowScratch<D, kRowWave
           }
         }
       }
-      if (live_next != 0) load_keys(slot_next);
+      const float values_by = value_scale;  // the present round's, before the next one's are looked up
+      if (live_next != 0) {
+        look_up_scales(slot_next);
+        load_keys(slot_next);
+      }
       if (live != 0) {
         float most = -INFINITY;
 #pragma unroll
@@ -557,6 +617,28 @@ __device__ __forceinline__ void row_pass(const Window& a, RowScratch<D, kRowWave
               for (int p = 0; p < S::kPPieces; ++p) pr[p][2 * j + r / 2] = cut_piece(x0, x1);
             }
           }
+          // Pairs of a key's values in bfloat16.
+          constexpr int kPairs = S::kVWidth / 2;
+          uint32_t wide[S::kBlocks][4][S::kVLoads][kPairs];
+#pragma unroll
+          for (int j = 0; j < S::kBlocks; ++j) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const float scale = S::kCodes ? __shfl(values_by, 16 * j + 4 * c + r) : 1.f;
+#pragma unroll
+              for (int g = 0; g < S::kVLoads; ++g) {
+#pragma unroll
+                for (int w = 0; w < kPairs; ++w) {
+                  if constexpr (!S::kCodes) {
+                    wide[j][r][g][w] = vx[j][r][g].w[w];
+                  } else {
+                    const uint32_t codes = vx[j][r][g].w[w / 2];
+                    wide[j][r][g][w] = w % 2 ? widen<1>(codes, scale) : widen<0>(codes, scale);
+                  }
+                }
+              }
+            }
+          }
 #pragma unroll
           for (int g = 0; g < S::kVLoads; ++g) {
 #pragma unroll
@@ -566,7 +648,7 @@ __device__ __forceinline__ void row_pass(const Window& a, RowScratch<D, kRowWave
               for (int j = 0; j < S::kBlocks; ++j) {
 #pragma unroll
                 for (int r = 0; r < 4; r += 2) {
-                  v[2 * j + r / 2] = __builtin_amdgcn_perm(vx[j][r + 1][g].w[e / 2], vx[j][r][g].w[e / 2], e % 2 ? 0x07060302 : 0x05040100);
+                  v[2 * j + r / 2] = __builtin_amdgcn_perm(wide[j][r + 1][g][e / 2], wide[j][r][g][e / 2], e % 2 ? 0x07060302 : 0x05040100);
                 }
               }
 #pragma unroll
@@ -715,7 +797,7 @@ struct TileShape {
   static constexpr int kQPieces = sizeof(QT) == 4 ? 3 : 1;
   static constexpr int kKvPieces = sizeof(KVT) == 4 ? 3 : 1;
   static constexpr int kPPieces = sizeof(QT) == 4 ? 3 : 2;
-  static constexpr int kKeys = (sizeof(KVT) == 2 && D <= 128) || D == 32 ? 64 : 32;
+  static constexpr int kKeys = (sizeof(KVT) <= 2 && D <= 128) || D == 32 ? 64 : 32;
   static constexpr int kChunks = D / 8;                                // 16-byte chunks of a bfloat16 row
   static constexpr int kPlane = kKeys * D;                             // elements of one piece of a staged tile
   static constexpr int kStaged = kKeys * kChunks / kThreads;           // chunks of a tile per thread, K and V each
@@ -952,15 +1034,28 @@ __global__ __launch_bounds__(kThreads, (TileShape<QT, KVT, D>::kWaves)) void til
         if (tid == 0) s_live[tile % 3] = live;
       }
     };
+    constexpr bool kCodes = sizeof(KVT) == 1;
     constexpr int kWide = sizeof(KVT) / 2;  // 16-byte loads of a chunk
-    u32x4 kx[S::kStaged][kWide], vx[S::kStaged][kWide];
+    u32x4 kx[S::kStaged][kWide ? kWide : 1], vx[S::kStaged][kWide ? kWide : 1];
+    u32x2 kc[kCodes ? S::kStaged : 1], vc[kCodes ? S::kStaged : 1];  // eight codes each, and their scales
+    float ks[kCodes ? S::kStaged : 1], vs[kCodes ? S::kStaged : 1];
     auto load = [&](int32_t tile, int buffer) {
 #pragma unroll
       for (int i = 0; i < S::kStaged; ++i) {
         const int at = tid + i * kThreads, row = at / S::kChunks, chunk = at % S::kChunks;
         const int32_t slot = s_slot[tile % 3][row];
         const int64_t from = row_of(a, slot, kv_head, D);
-        if constexpr (kWide == 1) {
+        if constexpr (kCodes) {
+          kc[i] = vc[i] = u32x2{0, 0};
+          ks[i] = vs[i] = 1.f;
+          if (slot >= 0) {
+            const int64_t at = scale_of(a, slot, kv_head);
+            ks[i] = a.key_scales[at];
+            vs[i] = a.value_scales[at];
+            kc[i] = *reinterpret_cast<const u32x2*>(keys + from + 8 * chunk);
+            vc[i] = *reinterpret_cast<const u32x2*>(values + from + 8 * chunk);
+          }
+        } else if constexpr (kWide == 1) {
           // Straight to LDS, where a wavefront's 64 chunks lie one after the other: the permutation is made
           // by which chunk of the row a lane fetches (it is its own inverse).
           const void* k = slot >= 0 ? static_cast<const void*>(keys + from + 8 * key_chunk<D>(row, chunk)) : zeros;
@@ -976,9 +1071,16 @@ __global__ __launch_bounds__(kThreads, (TileShape<QT, KVT, D>::kWaves)) void til
         }
       }
     };
-    auto put = [&](int buffer, int which, int i, const u32x4 (&x)[kWide]) {
+    auto place = [&](int which, int i) {  // of a staged chunk in its plane
       const int at = tid + i * kThreads, row = at / S::kChunks, chunk = at % S::kChunks;
-      const int to = row * D + 8 * (which == 0 ? key_chunk<D>(row, chunk) : value_chunk<D>(row, chunk));
+      return row * D + 8 * (which == 0 ? key_chunk<D>(row, chunk) : value_chunk<D>(row, chunk));
+    };
+    auto put_codes = [&](int buffer, int which, int i, const u32x2& x, float scale) {
+      *reinterpret_cast<u32x4*>(plane(buffer, which, 0) + place(which, i)) =
+          u32x4{widen<0>(x.x, scale), widen<1>(x.x, scale), widen<0>(x.y, scale), widen<1>(x.y, scale)};
+    };
+    auto put = [&](int buffer, int which, int i, const u32x4 (&x)[kWide ? kWide : 1]) {
+      const int to = place(which, i);
       u32x4 piece[3];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -992,6 +1094,12 @@ __global__ __launch_bounds__(kThreads, (TileShape<QT, KVT, D>::kWaves)) void til
     auto stage = [&](int buffer) {
       if constexpr (kWide == 1) {
         __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wavefront's loads to LDS have arrived
+      } else if constexpr (kCodes) {
+#pragma unroll
+        for (int i = 0; i < S::kStaged; ++i) {
+          put_codes(buffer, 0, i, kc[i], ks[i]);
+          put_codes(buffer, 1, i, vc[i], vs[i]);
+        }
       } else {
 #pragma unroll
         for (int i = 0; i < S::kStaged; ++i) {
@@ -1264,8 +1372,8 @@ int launch(Window a, hipStream_t stream) {
   // float32 queries of head_dim 128 over bfloat16 keys (8 rows of 1024 keys, 32/8 heads: 20.4 us, 21.9 with eight). Where
   // there are many and a key row is short, one of eight serves two neighbouring key heads, and so reads twice as much next
   // to each other.
-  constexpr bool kShort = D * sizeof(KVT) <= 256;
-  constexpr bool kWide = D < 128 || (D == 128 && sizeof(QT) == sizeof(KVT));
+  constexpr bool kShort = D * sizeof(KVT) <= 256 && D <= 128;
+  constexpr bool kWide = D < 128 || (D == 128 && (sizeof(QT) == sizeof(KVT) || (sizeof(QT) == 2 && sizeof(KVT) == 1)));
   const bool wide = kWide && groups <= 256;
   const bool pair = kShort && groups >= 512 && a.num_kv_heads % 2 == 0;
   const auto start = [&](auto kernel, int64_t count, int waves) {
@@ -1366,25 +1474,26 @@ extern "C" int32_t pkv_window_sizes(int64_t num_queries, int32_t num_heads, int3
   return splits;
 }
 
-extern "C" int pkv_window_attention(const pkv_window* args, int device, void* stream) {
-  using namespace pkv;
-  if (!args) return PKV_EINVAL;
-  const pkv_window& g = *args;
+namespace pkv {
+namespace {
+// pkv_window_attention, and with scales pkv_attention_e4m3, whose pools hold codes (kv_dtype is not looked at then).
+int attention(const pkv_window& g, const float* key_scales, const float* value_scales, bool codes, int device, void* stream) {
   if (g.num_queries < 0 || g.num_heads < 1 || g.num_kv_heads < 1 || g.num_heads % g.num_kv_heads != 0 || g.num_seqs < 0 ||
       g.num_blocks < 0 || g.block_size < 1 || g.block_table_stride < 0 || g.window < 1 || g.sinks < 0 ||
       g.max_context_len < 0 || g.max_query_len < 0 || g.num_splits < 0 || g.num_splits > PKV_WINDOW_MAX_SPLITS) {
     return PKV_EINVAL;
   }
   if (static_cast<int64_t>(g.block_table_stride) * g.block_size < g.max_context_len) return PKV_EINVAL;
-  if ((g.q_dtype != PKV_F32 && g.q_dtype != PKV_BF16) || (g.kv_dtype != PKV_F32 && g.kv_dtype != PKV_BF16)) return PKV_EINVAL;
-  if (g.q_dtype == PKV_BF16 && g.kv_dtype == PKV_F32) return PKV_EUNSUPPORTED;
+  if (g.q_dtype != PKV_F32 && g.q_dtype != PKV_BF16) return PKV_EINVAL;
+  if (!codes && g.kv_dtype != PKV_F32 && g.kv_dtype != PKV_BF16) return PKV_EINVAL;
+  if (!codes && g.q_dtype == PKV_BF16 && g.kv_dtype == PKV_F32) return PKV_EUNSUPPORTED;
   if (g.head_dim != 32 && g.head_dim != 64 && g.head_dim != 128 && g.head_dim != 256) return PKV_EUNSUPPORTED;
   if (g.num_heads / g.num_kv_heads > PKV_WINDOW_MAX_GROUP) return PKV_EUNSUPPORTED;
   // Slots, and a span's items some tiles past its end, are 32-bit.
   if (g.num_blocks > 0x7fffffff / g.block_size || g.max_context_len > PKV_WINDOW_MAX_CONTEXT) return PKV_EUNSUPPORTED;
   if (g.num_queries == 0) return PKV_OK;
   if (!g.out || !g.queries || !g.query_positions || !g.query_seq || !g.key_cache || !g.value_cache || !g.block_tables ||
-      !g.context_lens) {
+      !g.context_lens || (codes && (!key_scales || !value_scales))) {
     return PKV_EINVAL;
   }
   const int64_t row = static_cast<int64_t>(g.num_heads) * g.head_dim;
@@ -1409,6 +1518,8 @@ extern "C" int pkv_window_attention(const pkv_window* args, int device, void* st
   a.num_queries = g.num_queries;
   a.keys = g.key_cache;
   a.values = g.value_cache;
+  a.key_scales = key_scales;
+  a.value_scales = value_scales;
   a.num_blocks = g.num_blocks;
   a.tables = g.block_tables;
   a.contexts = g.context_lens;
@@ -1433,8 +1544,48 @@ extern "C" int pkv_window_attention(const pkv_window* args, int device, void* st
     a.flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;
     a.keep = a.scale_log2 == 0.f ? 0u : 0xffffffffu;
     a.scale_log2 = a.scale_log2 == 0.f ? 1.f : std::fabs(a.scale_log2);
-    return dispatch<uint16_t, uint16_t>(a, g.head_dim, s);
+    return codes ? dispatch<uint16_t, uint8_t>(a, g.head_dim, s) : dispatch<uint16_t, uint16_t>(a, g.head_dim, s);
   }
+  if (codes) return dispatch<float, uint8_t>(a, g.head_dim, s);
   return g.kv_dtype == PKV_F32 ? dispatch<float, float>(a, g.head_dim, s)
                                : dispatch<float, uint16_t>(a, g.head_dim, s);
+}
+}  // namespace
+}  // namespace pkv
+
+extern "C" int pkv_window_attention(const pkv_window* args, int device, void* stream) {
+  return args ? pkv::attention(*args, nullptr, nullptr, false, device, stream) : PKV_EINVAL;
+}
+
+extern "C" int pkv_attention_e4m3(const pkv_e4m3_attention* args, int device, void* stream) {
+  if (!args) return PKV_EINVAL;
+  const pkv_e4m3_attention& g = *args;
+  pkv_window w{};
+  w.out = g.out;
+  w.queries = g.queries;
+  w.query_token_stride = g.query_token_stride;
+  w.query_positions = g.query_positions;
+  w.query_seq = g.query_seq;
+  w.num_queries = g.num_queries;
+  w.key_cache = g.key_cache;
+  w.value_cache = g.value_cache;
+  w.num_blocks = g.num_blocks;
+  w.block_tables = g.block_tables;
+  w.context_lens = g.context_lens;
+  w.workspace = g.workspace;
+  w.workspace_bytes = g.workspace_bytes;
+  w.q_dtype = g.q_dtype;
+  w.block_size = g.block_size;
+  w.block_table_stride = g.block_table_stride;
+  w.num_seqs = g.num_seqs;
+  w.num_heads = g.num_heads;
+  w.num_kv_heads = g.num_kv_heads;
+  w.head_dim = g.head_dim;
+  w.window = g.window;
+  w.sinks = g.sinks;
+  w.max_context_len = g.max_context_len;
+  w.max_query_len = g.max_query_len;
+  w.num_splits = g.num_splits;
+  w.scale = g.scale;
+  return pkv::attention(w, g.key_scales, g.value_scales, true, device, stream);
 }

@@ -20,6 +20,7 @@ __all__ = [
     "MIN_TILE_ROWS",
     "TILE_ROWS",
     "append_kv",
+    "append_kv_e4m3",
     "attention_workspace_bytes",
     "copy_blocks",
     "expand_rows",
@@ -28,6 +29,7 @@ __all__ = [
     "kv_dtype_code",
     "kv_dtype_size",
     "merge_rows_for",
+    "paged_attention_e4m3",
     "paged_attention_ragged",
     "paged_attention_window",
     "BatchPlan",
@@ -161,6 +163,72 @@ def append_kv(
         device, _stream(device),
     )  # fmt: skip
     _native.check(rc, "pkv_append")
+
+
+def _e4m3_pools(keys: torch.Tensor, values: torch.Tensor, key_scales: torch.Tensor, value_scales: torch.Tensor):
+    """The shape of one layer's e4m3 pools, after checking them and their scales."""
+    shape = keys.shape
+    if keys.dtype != torch.float8_e4m3fn or values.dtype != torch.float8_e4m3fn:
+        raise ValueError("the pools must be float8_e4m3fn")
+    if len(shape) != 4 or values.shape != shape:
+        raise ValueError("key and value pools must both be [num_blocks, block_size, kv_heads, head_dim]")
+    if not (keys.is_contiguous() and values.is_contiguous()):
+        raise ValueError("pools must be contiguous")
+    scales = (shape[0], shape[2])
+    for name, tensor in (("key_scales", key_scales), ("value_scales", value_scales)):
+        if tensor.dtype != torch.float32 or tensor.shape != scales or not tensor.is_contiguous():
+            raise ValueError(f"{name} must be contiguous float32 of shape (num_blocks, kv_heads)")
+    return shape
+
+
+def append_kv_e4m3(
+    key_pool: torch.Tensor,
+    value_pool: torch.Tensor,
+    key_scales: torch.Tensor,
+    value_scales: torch.Tensor,
+    keys: torch.Tensor,
+    values: torch.Tensor,
+    slot_mapping: torch.Tensor,
+) -> None:
+    """:func:`append_kv` to one layer's cache held in 8 bits, for :func:`paged_attention_e4m3`.
+
+    ``key_pool``/``value_pool``: contiguous float8_e4m3fn ``[num_blocks, block_size, kv_heads, head_dim]``;
+    ``key_scales``/``value_scales``: contiguous float32 ``[num_blocks, kv_heads]``, powers of two. A cached value is
+    its code times its block's scale. ``keys``/``values``: ``[T, kv_heads, head_dim]`` float32 or bfloat16 (both
+    alike), token-strided views allowed. ``slot_mapping``: int64 ``[T]``; a slot outside the pool (padding: -1) is
+    skipped.
+
+    A block's scale is the smallest power of two, 2^-100 at least, that keeps the largest magnitude written to the
+    block within the format (448 times the scale). Where a later call brings larger values, the scale grows and the
+    codes of the tokens before them are scaled down, exactly but for those that fall below 2^-6. A block is filled in the
+    order of its places: tokens behind the first place that a call writes count as gone, and a block written from its
+    first place begins anew. The tokens of one block have to stand next to each other in the call, as a batch's do, and no
+    slot may be named twice; otherwise that block's contents are unspecified. What is not finite becomes NaN and counts
+    nothing for the scale.
+    """
+    device = _one_device(key_pool, value_pool, key_scales, value_scales, keys, values, slot_mapping)
+    num_blocks, block_size, kv_heads, dim = _e4m3_pools(key_pool, value_pool, key_scales, value_scales)
+    shape = keys.shape
+    if len(shape) != 3 or values.shape != shape or values.dtype != keys.dtype:
+        raise ValueError("keys and values must both be [T, kv_heads, head_dim] of the same dtype")
+    tokens = shape[0]
+    if shape[1] != kv_heads or shape[2] != dim:
+        raise ValueError("pool rows and keys disagree on (kv_heads, head_dim)")
+    code = kv_dtype_code(keys.dtype)
+    if dim not in WINDOW_HEAD_DIMS:
+        raise ValueError(f"unsupported head_dim {dim}: it must be one of {WINDOW_HEAD_DIMS}")
+    if slot_mapping.dtype != torch.int64 or slot_mapping.shape != (tokens,) or not slot_mapping.is_contiguous():
+        raise ValueError("slot_mapping must be contiguous int64 with one entry per token")
+    k_stride = _token_stride(keys, tokens, kv_heads, dim, "keys")
+    v_stride = _token_stride(values, tokens, kv_heads, dim, "values")
+    if tokens == 0:
+        return
+    rc = _host().append_e4m3(
+        key_pool.data_ptr(), value_pool.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(), keys.data_ptr(),
+        values.data_ptr(), k_stride, v_stride, slot_mapping.data_ptr(), tokens, num_blocks, code, block_size, kv_heads,
+        dim, device, _stream(device),
+    )  # fmt: skip
+    _native.check(rc, "pkv_append_e4m3")
 
 
 def rope_append(
@@ -1487,13 +1555,66 @@ def paged_attention_window(
     ``max_context_len`` and ``max_query_len``).
     """
     device = _one_device(queries, query_positions, query_seq, key_cache, value_cache, block_tables, context_lens)
-    io, kv, shape, cache = queries.dtype, key_cache.dtype, queries.shape, key_cache.shape
-    q_code, kv_code = kv_dtype_code(io), kv_dtype_code(kv)
+    kv = key_cache.dtype
+    kv_code = kv_dtype_code(kv)
+    if value_cache.shape != key_cache.shape or value_cache.dtype != kv:
+        raise ValueError("key and value caches must have the same shape and dtype")
+    if kv == torch.float32 and queries.dtype == torch.bfloat16:
+        raise ValueError("float32 caches need float32 queries")
+    return _windowed(device, queries, query_positions, query_seq, key_cache, value_cache, None, None, kv_code, block_tables, context_lens,
+                     scale, window, sinks, max_context_len, max_query_len, num_splits, out, workspace)  # fmt: skip
+
+
+def paged_attention_e4m3(
+    queries: torch.Tensor,
+    query_positions: torch.Tensor,
+    query_seq: torch.Tensor,
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    key_scales: torch.Tensor,
+    value_scales: torch.Tensor,
+    block_tables: torch.Tensor,
+    context_lens: torch.Tensor,
+    scale: float,
+    *,
+    window: int | None = None,
+    sinks: int = 0,
+    max_context_len: int,
+    max_query_len: int | None = None,
+    num_splits: int = 0,
+    out: torch.Tensor | None = None,
+    workspace: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Causal paged attention for grouped heads over a cache held in 8 bits, as :func:`append_kv_e4m3` writes it:
+    :func:`paged_attention_window` with every argument and rule of its, except for the cache and that ``window`` may be
+    None (and is, unless given): every key up to the row's own position is seen then.
+
+    ``key_cache``/``value_cache``: contiguous float8_e4m3fn ``[num_blocks, block_size, kv_heads, head_dim]``;
+    ``key_scales``/``value_scales``: contiguous float32 ``[num_blocks, kv_heads]``, powers of two (of another number its
+    power of two alone counts). Codes are widened to bfloat16, which holds a code times its scale exactly, on their way
+    into the products. Queries are float32 or bfloat16. The workspace is :func:`window_workspace_bytes`'s, for a
+    ``window`` of ``max_context_len`` where there is none.
+    """
+    device = _one_device(queries, query_positions, query_seq, key_cache, value_cache, key_scales, value_scales, block_tables, context_lens)
+    _e4m3_pools(key_cache, value_cache, key_scales, value_scales)
+    if window is None:
+        if sinks:
+            raise ValueError("sinks need a window")
+        window = _INT32_MAX
+    return _windowed(device, queries, query_positions, query_seq, key_cache, value_cache, key_scales, value_scales, None, block_tables,
+                     context_lens, scale, window, sinks, max_context_len, max_query_len, num_splits, out, workspace)  # fmt: skip
+
+
+def _windowed(
+    device, queries, query_positions, query_seq, key_cache, value_cache, key_scales, value_scales, kv_code, block_tables, context_lens,
+    scale, window, sinks, max_context_len, max_query_len, num_splits, out, workspace,
+) -> torch.Tensor:  # fmt: skip
+    """The two functions above, after they have looked at their caches' types. ``kv_code`` None: e4m3 codes."""
+    io, shape, cache = queries.dtype, queries.shape, key_cache.shape
+    q_code = kv_dtype_code(io)
     if len(shape) != 3:
         raise ValueError("queries must have shape (tokens, heads, head_dim)")
     num_queries, heads, dim = shape
-    if value_cache.shape != cache or value_cache.dtype != kv:
-        raise ValueError("key and value caches must have the same shape and dtype")
     if len(cache) != 4 or cache[3] != dim:
         raise ValueError("caches must have shape (num_blocks, block_size, kv_heads, head_dim)")
     if not (key_cache.is_contiguous() and value_cache.is_contiguous()):
@@ -1503,8 +1624,6 @@ def paged_attention_window(
         raise ValueError("heads must be a multiple of kv_heads")
     if heads // kv_heads > MAX_WINDOW_GROUP:
         raise ValueError(f"at most {MAX_WINDOW_GROUP} query heads per key head")
-    if kv == torch.float32 and io != torch.float32:
-        raise ValueError("float32 caches need float32 queries")
     if dim not in WINDOW_HEAD_DIMS:
         raise ValueError(f"unsupported head_dim {dim}: it must be one of {WINDOW_HEAD_DIMS}")
     stride = _token_stride(queries, num_queries, heads, dim, "queries")
@@ -1544,13 +1663,16 @@ def paged_attention_window(
             raise ValueError("workspace must be contiguous and on the queries' device")
         elif workspace.numel() * workspace.element_size() < need:
             raise ValueError(f"workspace must hold {need} bytes")
-    rc = host.window_attention(
-        out.data_ptr(), queries.data_ptr(), stride, query_positions.data_ptr(), query_seq.data_ptr(), num_queries,
-        key_cache.data_ptr(), value_cache.data_ptr(), num_blocks, block_tables.data_ptr(), context_lens.data_ptr(),
-        workspace.data_ptr() if need else 0, need, q_code, kv_code, block_size, table_stride, num_seqs,
-        heads, kv_heads, dim, window, sinks, max_context_len, rows, splits, scale, device, _stream(device),
-    )  # fmt: skip
-    _native.check(rc, "pkv_window_attention")
+    before = (out.data_ptr(), queries.data_ptr(), stride, query_positions.data_ptr(), query_seq.data_ptr(), num_queries,
+              key_cache.data_ptr(), value_cache.data_ptr())  # fmt: skip
+    middle = (num_blocks, block_tables.data_ptr(), context_lens.data_ptr(), workspace.data_ptr() if need else 0, need, q_code)
+    after = (block_size, table_stride, num_seqs, heads, kv_heads, dim, window, sinks, max_context_len, rows, splits, scale,
+             device, _stream(device))  # fmt: skip
+    if kv_code is None:
+        rc = host.attention_e4m3(*before, key_scales.data_ptr(), value_scales.data_ptr(), *middle, *after)
+    else:
+        rc = host.window_attention(*before, *middle, kv_code, *after)
+    _native.check(rc, "pkv_attention_e4m3" if kv_code is None else "pkv_window_attention")
     return out
 
 
