@@ -798,6 +798,147 @@ typedef struct pkv_e4m3_attention {
 
 int pkv_attention_e4m3(const pkv_e4m3_attention* args, int device, void* stream);
 
+/*
+ * The metadata of a serving step on the device, from its requests' lengths: which request and position each row is, the
+ * slot its key and value go to, and the requests' block tables, extended from a list of free blocks. With it a captured step
+ * serves requests that grow from replay to replay without the host.
+ *
+ * Does on the device what src/paged_kv_serving/engine/runner.py:149-159 and :184-212 (slots and rows of a batch) and
+ * kvcache.py (the blocks of a request) do on the host, without sharing: every block is its request's own.
+ *
+ *   query_lens, context_lens : int32 [num_seqs]: the tokens that request i runs in this step (0: none), and its tokens
+ *                              after the step, these among them.
+ *   block_tables             : int32 [num_seqs, table_stride], in and out. With B = block_size, request i has
+ *                              ceil((context - query) / B) blocks; what it needs for more, up to ceil(context / B), is
+ *                              written behind them.
+ *   free_blocks, next_free   : int32 [num_free], and where in it the next free block stands (int32 [1], or NULL for 0;
+ *                              taken as within [0, num_free]). Requests take their blocks in order.
+ *   query_seq, query_positions, positions, slot_mapping : int32, int32, int64, int64 [num_rows], output. Row r's request and
+ *                              position (once in each type that the other calls take) and its slot (-1 where a table entry
+ *                              is negative). Rows are the requests' in order; those behind the last are padding: request -1,
+ *                              position 0, slot -1.
+ *   query_starts             : int32 [num_seqs + 1], output: the first row of each request, then the number of rows, each
+ *                              num_rows at most.
+ *   context_lens_out         : int32 [num_seqs], output: the context lengths that the step's attention sees. Not the input.
+ *   next_free_out            : int32 [1], output: next_free behind the blocks that were taken. Not the input.
+ * A request is not served, and changes nothing, where the blocks needed up to and with it (by requests not refused for the other
+ * reasons) are more than are free and it needs any, where its rows pass num_rows, where its table is too narrow, or where
+ * its context is shorter than its query: its rows are padding then, and its context length out is context - query (0 where that
+ * is negative). A negative query length is 0. No memset or synchronisation: the call may be captured. Up to
+ * PKV_STEP_MAX_ROWS rows, 2^29 free blocks, tables of fewer than 2^31 tokens.
+ */
+#define PKV_STEP_MAX_ROWS (1 << 21)
+
+typedef struct pkv_step {
+  const int32_t* query_lens;
+  const int32_t* context_lens;
+  int32_t* block_tables;
+  const int32_t* free_blocks;
+  const int32_t* next_free;
+  int32_t* query_seq;
+  int32_t* query_positions;
+  int64_t* positions;
+  int64_t* slot_mapping;
+  int32_t* query_starts;
+  int32_t* context_lens_out;
+  int32_t* next_free_out;
+  int64_t num_rows;
+  int32_t num_seqs;
+  int32_t table_stride;
+  int32_t num_free;
+  int32_t block_size;
+} pkv_step;
+
+int pkv_step_metadata(const pkv_step* args, int device, void* stream);
+
+/*
+ * Beam search: the best continuations of each group of num_beams beams over the whole vocabulary.
+ *     score(b, v) = scores[b] + (logits[b, v] - log sum_u exp(logits[b, u]))
+ * in double precision (exponentials, their sums and the logarithm within 2^-40 of themselves), rounded once to float32 at the
+ * end. Of a group's continuations with a score above -inf, the `count` of the highest scores, in falling order; equal
+ * scores in order of their beams, and within a beam of falling logits, then of rising tokens. Where there are fewer, the rest are
+ * (-inf, beam 0, end_token).
+ * A beam whose score is not finite has no continuation, nor has one whose row's sum is not finite or zero (a NaN or +inf, or
+ * nothing above -inf). A beam that `finished` marks has one: end_token at its own score; its row is not looked at.
+ *
+ * No counterpart in the reference, which samples one sequence (src/paged_kv_serving/engine/sampling.py:28-74).
+ *
+ *   best_scores, best_beams, best_tokens : float32, int32, int32 [num_groups, count], output. A beam's number is its place
+ *                 in its group.
+ *   logits      : rows of vocab_size values of `dtype`, row r at element r * row_stride, beam b of group g being row
+ *                 g * num_beams + b.
+ *   scores      : float32 [num_groups * num_beams].
+ *   finished    : one byte for each row (0: goes on), or NULL.
+ *   workspace   : scratch of pkv_beam_workspace_bytes bytes, 16-byte aligned; calls that may run at the same time need
+ *                 their own. Nothing in it needs to start at zero.
+ * Up to PKV_BEAM_MAX beams and PKV_BEAM_MAX_COUNT continuations, which a group must have (count <= num_beams * vocab_size), up
+ * to 2^20 rows. The same inputs give the same bits, whatever the batch.
+ */
+#define PKV_BEAM_MAX 64
+#define PKV_BEAM_MAX_COUNT 128
+
+typedef struct pkv_beam {
+  float* best_scores;
+  int32_t* best_beams;
+  int32_t* best_tokens;
+  const void* logits;
+  int64_t row_stride;
+  int64_t num_groups;
+  int64_t vocab_size;
+  const float* scores;
+  const uint8_t* finished;
+  void* workspace;
+  int64_t workspace_bytes;
+  int32_t dtype;
+  int32_t num_beams;
+  int32_t count;
+  int32_t end_token;
+} pkv_beam;
+
+/* Bytes of workspace of a selection. Host-only. */
+int64_t pkv_beam_workspace_bytes(int64_t num_groups, int32_t num_beams, int64_t vocab_size, int32_t count);
+
+int pkv_beam_select(const pkv_beam* args, int device, void* stream);
+
+/*
+ * Beam search: block tables and cached states of the beams that go on. Child c of group g goes on from row
+ * parents[g, c] of its group, at a context of context_lens[g] tokens, full = context / block_size of whose blocks are full:
+ *     new_tables[g, c, j] = block_tables[g, parent, j]  for j < full;  block_tables[g, c, j]  for j behind the context's blocks
+ * Full blocks are shared from then on. The last, partly filled block (where context is no multiple of block_size) stays
+ * with its parent's first child; the n-th of the other children takes over the last block of the n-th row that no child
+ * names, and its parent's last block is copied there, in every state. So a group needs no block beyond its own, and no copy
+ * reads a block that another writes, provided that a group's last blocks are the rows' own (as when every row appends to a
+ * block of its own; rows that start from one prompt have to be given a last block each, which need not hold anything).
+ *
+ * No counterpart in the reference, whose copy-on-write (src/paged_kv_serving/engine/runner.py:128-133) is the host's.
+ *
+ *   new_tables, block_tables : int32 [num_groups * num_beams, table_stride]; the output must not be the input.
+ *   parents                  : int32 [num_groups, num_beams]; one outside [0, num_beams) is the row itself.
+ *   context_lens             : int32 [num_groups]; one whose blocks the table does not hold counts as the table's.
+ *   states                   : up to PKV_BEAM_STATES tensors [num_layers, num_blocks, block_bytes], with layers
+ *                              layer_bytes apart. A block outside [0, num_blocks) is not read or written.
+ */
+#define PKV_BEAM_STATES 8
+
+typedef struct pkv_reorder {
+  int32_t* new_tables;
+  const int32_t* block_tables;
+  const int32_t* parents;
+  const int32_t* context_lens;
+  int64_t num_groups;
+  int64_t num_blocks;
+  void* states[PKV_BEAM_STATES];
+  int64_t block_bytes[PKV_BEAM_STATES];
+  int64_t layer_bytes[PKV_BEAM_STATES];
+  int32_t num_layers[PKV_BEAM_STATES];
+  int32_t num_states;
+  int32_t num_beams;
+  int32_t table_stride;
+  int32_t block_size;
+} pkv_reorder;
+
+int pkv_beam_reorder(const pkv_reorder* args, int device, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

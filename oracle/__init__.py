@@ -16,6 +16,8 @@ Modules:
     bf16       -- round-to-nearest-even float32 -> bfloat16 for the bf16-KV tolerance oracle
     window     -- attention with a sliding window and sinks for grouped heads, axes of rotary frequencies
     e4m3       -- a cache of 8-bit floats with a scale for each block and head, its append
+    step       -- a step's rows, positions, slots and block tables from its requests' lengths
+    beam       -- the best continuations of a group of beams, and what becomes of its rows' blocks
     sampling   -- a token by temperature, top-k, min-p, top-p and a given uniform (sampling.py:56-74)
 
 Each function is pinned (closed forms, invariants, brute force on tiny inputs, planted mistakes)

@@ -40,6 +40,7 @@ SOURCES = (
     CSRC / "pkv_copy.hip", CSRC / "pkv_rope.hip", CSRC / "pkv_attention.hip", CSRC / "pkv_sample.hip",
     CSRC / "pkv_plan.hip", CSRC / "pkv_model.hip", CSRC / "pkv_linear.hip", CSRC / "pkv_rope_axes.hip",
     CSRC / "pkv_window.hip", CSRC / "pkv_sampling.hip", CSRC / "pkv_e4m3.hip",
+    CSRC / "pkv_step.hip", CSRC / "pkv_beam.hip",
 )
 
 # gfx950 only. Packed-FP32 VALU instructions are disabled: the code relies on scalar fp32 FMA.
@@ -103,6 +104,10 @@ EXPORTED_SYMBOLS = (
     "pkv_sample_tokens",
     "pkv_append_e4m3",
     "pkv_attention_e4m3",
+    "pkv_step_metadata",
+    "pkv_beam_workspace_bytes",
+    "pkv_beam_select",
+    "pkv_beam_reorder",
 )
 
 
@@ -195,8 +200,8 @@ def bound_host():
     """:func:`host` with the library's entry points bound into it (``_pkvhost.bind``), so its
     ``plan``, ``paged_attention``, ``paged_attention_append``, ``copy_blocks``, ``rms_norm``,
     ``silu_mul``, ``rope_append``, ``append``, ``rope_append_axes``, ``window_workspace``,
-    ``window_attention``, ``sample_tokens``, ``append_e4m3``, ``attention_e4m3``, ``forward`` and
-    ``CopyQueue.flush`` call ``libpkv.so`` directly, and ``stage``, ``forward``, ``CopyQueue.flush`` and ``event_create`` call the
+    ``window_attention``, ``sample_tokens``, ``append_e4m3``, ``attention_e4m3``, ``step_metadata``,
+    ``beam_workspace``, ``beam_select``, ``beam_reorder``, ``forward`` and ``CopyQueue.flush`` call ``libpkv.so`` directly, and ``stage``, ``forward``, ``CopyQueue.flush`` and ``event_create`` call the
     ``hipMemcpyAsync`` / ``hipGetDevice`` / ``hipSetDevice`` / ``hipEvent*`` functions of the HIP
     runtime ``libpkv.so`` is linked against (looked up through the library's handle, so they are
     that runtime's). Binding loads the library (it must be built)."""
@@ -218,7 +223,9 @@ def bound_host():
                          address(lib.pkv_append), address(lib.pkv_linear_forward),
                          address(lib.pkv_rope_append_axes), address(lib.pkv_window_sizes),
                          address(lib.pkv_window_attention), address(lib.pkv_sample_tokens),
-                         address(lib.pkv_append_e4m3), address(lib.pkv_attention_e4m3))  # fmt: skip
+                         address(lib.pkv_append_e4m3), address(lib.pkv_attention_e4m3),
+                         address(lib.pkv_step_metadata), address(lib.pkv_beam_workspace_bytes),
+                         address(lib.pkv_beam_select), address(lib.pkv_beam_reorder))  # fmt: skip
                 _BOUND = True
     return ext
 
@@ -360,6 +367,14 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.pkv_append_e4m3.restype = _c_int
     lib.pkv_attention_e4m3.argtypes = [_ptr, _c_int, _ptr]  # args, device, stream
     lib.pkv_attention_e4m3.restype = _c_int
+    lib.pkv_step_metadata.argtypes = [_ptr, _c_int, _ptr]  # args, device, stream
+    lib.pkv_step_metadata.restype = _c_int
+    lib.pkv_beam_workspace_bytes.argtypes = [_i64, _i32, _i64, _i32]  # groups, beams, vocabulary, count
+    lib.pkv_beam_workspace_bytes.restype = _i64
+    lib.pkv_beam_select.argtypes = [_ptr, _c_int, _ptr]  # args, device, stream
+    lib.pkv_beam_select.restype = _c_int
+    lib.pkv_beam_reorder.argtypes = [_ptr, _c_int, _ptr]  # args, device, stream
+    lib.pkv_beam_reorder.restype = _c_int
 
 
 def library() -> ctypes.CDLL:

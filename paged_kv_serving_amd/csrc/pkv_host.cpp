@@ -59,7 +59,8 @@
 //   bind(plan_batch, paged_attention, paged_attention_append, copy_blocks, rms_norm, silu_mul,
 //        rope_append, memcpy_async[, gather_rows, greedy_tokens, get_device, set_device,
 //        event_create, event_record, event_synchronize, event_destroy, append, linear_forward,
-//        rope_append_axes, window_sizes, window_attention, sample_tokens, append_e4m3, attention_e4m3])
+//        rope_append_axes, window_sizes, window_attention, sample_tokens, append_e4m3, attention_e4m3,
+//        step_metadata, beam_workspace_bytes, beam_select, beam_reorder])
 //       Takes the addresses of those libpkv.so entry points (include/pkv.h), so the calls below
 //       reach the library without ctypes' per-argument conversions, and of hipMemcpyAsync,
 //       hipGetDevice, hipSetDevice and hipEventCreateWithFlags / Record / Synchronize / Destroy
@@ -92,7 +93,8 @@
 //       pkv_plan_batch on NumPy buffers; returns its PKV_* code.
 //   paged_attention(...), paged_attention_append(...), copy_blocks(...), rms_norm(...),
 //   silu_mul(...), rope_append(...), append(...), rope_append_axes(...), window_attention(...),
-//   sample_tokens(...), append_e4m3(...), attention_e4m3(...) -> int
+//   sample_tokens(...), append_e4m3(...), attention_e4m3(...), step_metadata(...), beam_select(...),
+//   beam_reorder(...) -> int
 //       The entry points of the same names, with every pointer, stream and handle passed as a
 //       Python int (0 for NULL) in the order of their C declarations (the last three: of the
 //       fields of their argument structs, then device and stream); returns the PKV_* code.
@@ -852,6 +854,10 @@ decltype(&pkv_window_attention) g_window = nullptr;
 decltype(&pkv_sample_tokens) g_sample = nullptr;
 decltype(&pkv_append_e4m3) g_append_e4m3 = nullptr;
 decltype(&pkv_attention_e4m3) g_attention_e4m3 = nullptr;
+decltype(&pkv_step_metadata) g_step = nullptr;
+decltype(&pkv_beam_workspace_bytes) g_beam_bytes = nullptr;
+decltype(&pkv_beam_select) g_beam_select = nullptr;
+decltype(&pkv_beam_reorder) g_beam_reorder = nullptr;
 // hipGetDevice / hipSetDevice of the same runtime, by their C signatures.
 using GetDeviceFn = int (*)(int* device);
 using SetDeviceFn = int (*)(int device);
@@ -910,10 +916,11 @@ PyObject* bind(PyObject*, PyObject* args) {
   unsigned long long event_create = 0, event_record = 0, event_synchronize = 0, event_destroy = 0, append = 0, linear = 0;
   unsigned long long rope_axes = 0, window_sizes = 0, window = 0, sample = 0;
   unsigned long long append_codes = 0, attention_codes = 0;
-  if (!PyArg_ParseTuple(args, "KKKKKKKK|KKKKKKKKKKKKKKKK", &plan, &attention, &attention_append, &copy, &norm, &gate, &rope,
+  unsigned long long step = 0, beam_bytes = 0, beam_best = 0, beam_move = 0;
+  if (!PyArg_ParseTuple(args, "KKKKKKKK|KKKKKKKKKKKKKKKKKKKK", &plan, &attention, &attention_append, &copy, &norm, &gate, &rope,
                         &memcpy_async, &gather_rows, &greedy, &get_device, &set_device, &event_create,
                         &event_record, &event_synchronize, &event_destroy, &append, &linear, &rope_axes, &window_sizes,
-                        &window, &sample, &append_codes, &attention_codes)) {
+                        &window, &sample, &append_codes, &attention_codes, &step, &beam_bytes, &beam_best, &beam_move)) {
     return nullptr;
   }
   if (plan == 0 || attention == 0 || attention_append == 0 || copy == 0 || norm == 0 || gate == 0 || rope == 0 ||
@@ -946,6 +953,10 @@ PyObject* bind(PyObject*, PyObject* args) {
   g_sample = reinterpret_cast<decltype(g_sample)>(static_cast<uintptr_t>(sample));
   g_append_e4m3 = reinterpret_cast<decltype(g_append_e4m3)>(static_cast<uintptr_t>(append_codes));
   g_attention_e4m3 = reinterpret_cast<decltype(g_attention_e4m3)>(static_cast<uintptr_t>(attention_codes));
+  g_step = reinterpret_cast<decltype(g_step)>(static_cast<uintptr_t>(step));
+  g_beam_bytes = reinterpret_cast<decltype(g_beam_bytes)>(static_cast<uintptr_t>(beam_bytes));
+  g_beam_select = reinterpret_cast<decltype(g_beam_select)>(static_cast<uintptr_t>(beam_best));
+  g_beam_reorder = reinterpret_cast<decltype(g_beam_reorder)>(static_cast<uintptr_t>(beam_move));
   Py_RETURN_NONE;
 }
 
@@ -1549,6 +1560,55 @@ PyObject* attention_e4m3(PyObject*, PyObject* const* args, Py_ssize_t count) {
   return PyLong_FromLong(g_attention_e4m3(&a, device, stream));
 }
 
+PyObject* step_metadata(PyObject*, PyObject* const* args, Py_ssize_t count) {
+  pkv_step a{};
+  int32_t device = 0;
+  void* stream = nullptr;
+  Reader r{args, count};
+  r(a.query_lens), r(a.context_lens), r(a.block_tables), r(a.free_blocks), r(a.next_free), r(a.query_seq), r(a.query_positions);
+  r(a.positions), r(a.slot_mapping), r(a.query_starts), r(a.context_lens_out), r(a.next_free_out), r(a.num_rows), r(a.num_seqs);
+  r(a.table_stride), r(a.num_free), r(a.block_size);
+  r(device), r(stream);
+  if (!r.done() || !bound(reinterpret_cast<const void*>(g_step))) return nullptr;
+  return PyLong_FromLong(g_step(&a, device, stream));
+}
+
+PyObject* beam_workspace(PyObject*, PyObject* const* args, Py_ssize_t count) {
+  int64_t groups = 0, vocab = 0;
+  int32_t beams = 0, best = 0;
+  Reader r{args, count};
+  r(groups), r(beams), r(vocab), r(best);
+  if (!r.done() || !bound(reinterpret_cast<const void*>(g_beam_bytes))) return nullptr;
+  return PyLong_FromLongLong(g_beam_bytes(groups, beams, vocab, best));
+}
+
+PyObject* beam_select(PyObject*, PyObject* const* args, Py_ssize_t count) {
+  pkv_beam a{};
+  int32_t device = 0;
+  void* stream = nullptr;
+  Reader r{args, count};
+  r(a.best_scores), r(a.best_beams), r(a.best_tokens), r(a.logits), r(a.row_stride), r(a.num_groups), r(a.vocab_size), r(a.scores);
+  r(a.finished), r(a.workspace), r(a.workspace_bytes), r(a.dtype), r(a.num_beams), r(a.count), r(a.end_token);
+  r(device), r(stream);
+  if (!r.done() || !bound(reinterpret_cast<const void*>(g_beam_select))) return nullptr;
+  return PyLong_FromLong(g_beam_select(&a, device, stream));
+}
+
+// The fields in order, the states last: address, bytes of a block, bytes of a layer and layers of each.
+PyObject* beam_reorder(PyObject*, PyObject* const* args, Py_ssize_t count) {
+  pkv_reorder a{};
+  int32_t device = 0;
+  void* stream = nullptr;
+  Reader r{args, count};
+  r(a.new_tables), r(a.block_tables), r(a.parents), r(a.context_lens), r(a.num_groups), r(a.num_blocks), r(a.num_beams);
+  r(a.table_stride), r(a.block_size), r(device), r(stream), r(a.num_states);
+  for (int32_t s = 0; r.ok && s < a.num_states && s < PKV_BEAM_STATES; ++s) {
+    r(a.states[s]), r(a.block_bytes[s]), r(a.layer_bytes[s]), r(a.num_layers[s]);
+  }
+  if (!r.done() || !bound(reinterpret_cast<const void*>(g_beam_reorder))) return nullptr;
+  return PyLong_FromLong(g_beam_reorder(&a, device, stream));
+}
+
 PyObject* append(PyObject*, PyObject* args) {
   unsigned long long kp, vp, k, v, slots, stream;
   long long nslots, k_stride, v_stride, tokens;
@@ -1924,6 +1984,14 @@ PyMethodDef kMethods[] = {
      "pkv_append_e4m3 with integer pointers."},
     {"attention_e4m3", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(attention_e4m3)), METH_FASTCALL,
      "pkv_attention_e4m3 with integer pointers."},
+    {"step_metadata", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(step_metadata)), METH_FASTCALL,
+     "pkv_step_metadata with integer pointers."},
+    {"beam_workspace", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(beam_workspace)), METH_FASTCALL,
+     "pkv_beam_workspace_bytes."},
+    {"beam_select", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(beam_select)), METH_FASTCALL,
+     "pkv_beam_select with integer pointers."},
+    {"beam_reorder", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(beam_reorder)), METH_FASTCALL,
+     "pkv_beam_reorder with integer pointers."},
     {"stage", stage, METH_VARARGS, "Pack a call's metadata into pinned memory and copy it to the device."},
     {"forward", forward, METH_VARARGS, "One iteration's forward pass: rocBLAS products and the library's kernels."},
     {"event_create", event_create, METH_VARARGS, "A timing-free HIP event on a device, as an integer handle."},

@@ -1,0 +1,141 @@
+// The metadata of a serving step from its requests' lengths, on the device.
+#include <algorithm>
+
+#include "pkv_common.h"
+
+namespace pkv {
+namespace {
+
+constexpr int kThreads = 512;  // requests of a chunk, rows of a workgroup
+constexpr int kWaves = kThreads / kWave;
+constexpr int32_t kMostFree = 1 << 29;  // with PKV_STEP_MAX_ROWS no sum passes 32 bits
+
+// The sums of a thread's and all earlier threads' values, of the low and the high halves at once (no half overflows).
+__device__ __forceinline__ uint64_t inclusive_sums(uint64_t x, uint64_t* s_wave) {
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+#pragma unroll
+  for (int m = 1; m < kWave; m *= 2) {
+    const uint64_t other = __shfl_up(static_cast<unsigned long long>(x), m);
+    if (lane >= m) x += other;
+  }
+  if (lane == kWave - 1) s_wave[wave] = x;
+  __syncthreads();
+  uint64_t before = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) before += w < wave ? s_wave[w] : 0;
+  return x + before;
+}
+
+// ---------------------------------------------------------------------------------------------
+// With q and c of request i its query and context lengths, blocks of B tokens: it has held = ceil((c - q) / B) blocks
+// and needs ceil(c / B) - held more; its rows are [sum of q before i, + q). Every workgroup sums all requests' rows and
+// needs by itself, kThreads requests at a time, which costs less than a launch of its own for the sums, and finds the
+// requests of its own rows by bisection. A new block's table entry is written by the row at its first place, which lies
+// among the call's rows; no row reads an entry that another writes. The first workgroup writes what is one value a request.
+// Bound: latency (a few dependent loads and the sums).
+// ---------------------------------------------------------------------------------------------
+__global__ __launch_bounds__(kThreads) void step_kernel(const pkv_step a) {
+  __shared__ uint64_t s_wave[2][kWaves];
+  __shared__ int32_t s_end[kThreads], s_start[kThreads], s_held[kThreads], s_fresh[kThreads];
+  __shared__ int32_t s_need, s_most[kWaves];
+  const int tid = threadIdx.x;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kThreads + tid;
+  const int32_t limit = static_cast<int32_t>(a.num_rows) + 1;  // sums of rows stop counting here
+  const int32_t next_free = a.next_free ? min(max(*a.next_free, 0), a.num_free) : 0;
+  const int32_t available = a.num_free - next_free;
+  const int32_t block = a.block_size;
+  int32_t rows_before = 0, need_before = 0, most = 0;
+  int32_t seq = -1, position = 0;
+  int64_t slot = -1;
+  for (int32_t first = 0; first < a.num_seqs; first += kThreads) {
+    const int32_t i = first + tid;
+    int32_t q = 0, c = 0;
+    if (i < a.num_seqs) q = max(a.query_lens[i], 0), c = a.context_lens[i];
+    const bool fits = c >= q && c <= static_cast<int64_t>(a.table_stride) * block;
+    const int32_t start = c >= q ? c - q : 0;
+    const int32_t held = fits ? static_cast<int32_t>((static_cast<uint32_t>(start) + block - 1) / block) : 0;
+    const int32_t need = fits ? static_cast<int32_t>((static_cast<uint32_t>(c) + block - 1) / block) - held : 0;
+    // A request with more rows than there are gets none, and neither does any behind it: their needs do not matter.
+    const uint64_t sums = inclusive_sums(static_cast<uint64_t>(min(need, limit)) << 32 | static_cast<uint32_t>(min(q, limit)),
+                                   s_wave[first / kThreads % 2]);
+    const int32_t end = min(rows_before + static_cast<int32_t>(static_cast<uint32_t>(sums)), limit);
+    const int32_t taken = need_before + static_cast<int32_t>(sums >> 32);
+    const bool served = fits && end < limit && (need == 0 || taken <= available);
+    s_end[tid] = end;
+    s_start[tid] = start;
+    s_held[tid] = served ? held : -1;
+    s_fresh[tid] = next_free + taken - need - held;  // of the list, for table column 0
+    if (served && need > 0) most = taken;
+    if (tid == kThreads - 1) s_need = min(taken, kMostFree);
+    if (blockIdx.x == 0 && i < a.num_seqs) {
+      a.query_starts[i + 1] = min(end, limit - 1);
+      a.context_lens_out[i] = served ? c : start;
+    }
+    __syncthreads();
+    const int32_t last = min(kThreads, a.num_seqs - first) - 1;
+    if (row >= rows_before && row < s_end[last] && row < a.num_rows) {
+      int32_t low = 0, high = last;  // the first request whose end lies behind the row
+      while (low < high) {
+        const int32_t middle = (low + high) / 2;
+        if (s_end[middle] > row) high = middle; else low = middle + 1;
+      }
+      const int32_t begins = low == 0 ? rows_before : s_end[low - 1];
+      if (s_held[low] >= 0) {
+        seq = first + low;
+        position = s_start[low] + static_cast<int32_t>(row - begins);
+        const int32_t page = static_cast<int32_t>(static_cast<uint32_t>(position) / static_cast<uint32_t>(block));
+        const int32_t place = position - page * block;
+        int32_t* entry_at = a.block_tables + static_cast<int64_t>(seq) * a.table_stride + page;
+        int32_t entry;
+        if (page >= s_held[low]) {
+          entry = a.free_blocks[s_fresh[low] + page];
+          if (place == 0) *entry_at = entry;
+        } else {
+          entry = *entry_at;
+        }
+        if (entry >= 0) slot = static_cast<int64_t>(entry) * block + place;
+      }
+    }
+    rows_before = s_end[kThreads - 1];  // threads past the requests hold the last one's sum
+    need_before = s_need;
+    // The next chunk writes these places behind the barrier in its sums.
+  }
+  if (row < a.num_rows) {
+    a.query_seq[row] = seq;
+    a.query_positions[row] = position;
+    a.positions[row] = position;
+    a.slot_mapping[row] = slot;
+  }
+  if (blockIdx.x != 0) return;
+  for (int m = kWave / 2; m > 0; m >>= 1) most = max(most, __shfl_xor(most, m));
+  __syncthreads();
+  if (tid % kWave == 0) s_most[tid / kWave] = most;
+  __syncthreads();
+  if (tid == 0) {
+    for (int w = 1; w < kWaves; ++w) most = max(most, s_most[w]);
+    a.query_starts[0] = 0;
+    *a.next_free_out = next_free + most;
+  }
+}
+
+}  // namespace
+}  // namespace pkv
+
+extern "C" int pkv_step_metadata(const pkv_step* args, int device, void* stream) {
+  using namespace pkv;
+  if (!args) return PKV_EINVAL;
+  const pkv_step& g = *args;
+  if (g.num_seqs < 0 || g.num_rows < 0 || g.num_free < 0 || g.table_stride < 0 || g.block_size < 1) return PKV_EINVAL;
+  if (g.num_rows > PKV_STEP_MAX_ROWS || g.num_free > kMostFree) return PKV_EUNSUPPORTED;
+  if (static_cast<int64_t>(g.table_stride) * g.block_size > 0x7fffffff) return PKV_EUNSUPPORTED;
+  if (!g.query_starts || !g.next_free_out) return PKV_EINVAL;
+  if (g.num_seqs > 0 && (!g.query_lens || !g.context_lens || !g.context_lens_out || (!g.block_tables && g.table_stride > 0))) return PKV_EINVAL;
+  if (g.num_rows > 0 && (!g.query_seq || !g.query_positions || !g.positions || !g.slot_mapping)) return PKV_EINVAL;
+  if (g.num_free > 0 && !g.free_blocks) return PKV_EINVAL;
+  if (g.next_free == g.next_free_out || (g.num_seqs > 0 && g.context_lens == g.context_lens_out)) return PKV_EINVAL;
+  DeviceGuard guard(device);
+  if (!guard.ok()) return PKV_EHIP;
+  const uint32_t groups = static_cast<uint32_t>(std::max<int64_t>(1, (g.num_rows + kThreads - 1) / kThreads));
+  hipLaunchKernelGGL(step_kernel, dim3(groups), dim3(kThreads), 0, static_cast<hipStream_t>(stream), g);
+  return check_launch();
+}

@@ -9,6 +9,7 @@ the tensors' device). Nothing here computes on the CPU: a missing library raises
 from __future__ import annotations
 
 from dataclasses import dataclass
+from typing import NamedTuple
 
 import numpy as np
 import torch
@@ -22,6 +23,10 @@ __all__ = [
     "append_kv",
     "append_kv_e4m3",
     "attention_workspace_bytes",
+    "BeamChoice",
+    "beam_reorder",
+    "beam_select",
+    "beam_workspace_bytes",
     "copy_blocks",
     "expand_rows",
     "greedy_tokens",
@@ -45,6 +50,8 @@ __all__ = [
     "rope_append_axes",
     "sample_tokens",
     "silu_mul",
+    "step_metadata",
+    "StepMetadata",
     "upload_plan",
     "window_workspace_bytes",
 ]
@@ -561,6 +568,243 @@ def sample_tokens(
         top_p, min_p, device, _stream(device),
     )  # fmt: skip
     _native.check(rc, "pkv_sample_tokens")
+    return out
+
+
+#: Rows of a step that :func:`step_metadata` can take.
+MAX_STEP_ROWS = 1 << 21
+
+#: Beams of a group, and continuations of it, that :func:`beam_select` can take, and states of :func:`beam_reorder`.
+MAX_BEAMS, MAX_BEAM_COUNT, MAX_BEAM_STATES = 64, 128, 8
+
+
+class BeamChoice(NamedTuple):
+    """What :func:`beam_select` chose, each ``[groups, count]``: float32 scores, int32 beams and int32 tokens."""
+
+    scores: torch.Tensor
+    beams: torch.Tensor
+    tokens: torch.Tensor
+
+
+def beam_workspace_bytes(num_groups: int, num_beams: int, vocab_size: int, count: int) -> int:
+    """Bytes of workspace :func:`beam_select` needs for these sizes."""
+    need = _host().beam_workspace(num_groups, num_beams, vocab_size, count)
+    if need < 0:
+        raise ValueError(f"unsupported beam search: up to {MAX_BEAMS} beams, {MAX_BEAM_COUNT} continuations, 2^20 rows and 2^25 logits of a group")
+    return need
+
+
+def beam_select(
+    logits: torch.Tensor,
+    scores: torch.Tensor,
+    *,
+    num_beams: int,
+    count: int | None = None,
+    finished: torch.Tensor | None = None,
+    end_token: int = 0,
+    out: BeamChoice | None = None,
+    workspace: torch.Tensor | None = None,
+) -> BeamChoice:
+    """The ``count`` (default: ``num_beams``) best continuations of each group of ``num_beams`` beams, on the device.
+
+    ``logits``: float32 or bfloat16 ``[groups * num_beams, vocab]``, a group's beams next to each other; ``scores``:
+    float32 with one entry per row, the beams' so far (-inf: a beam that does not count). A continuation's score is its
+    beam's plus the logarithm of its token's softmax, in double precision, rounded to float32 at the end. Continuations come in
+    falling order of their scores; equal ones in order of their beams, and of one beam in order of falling logits, then rising
+    tokens. Scores of -inf are no continuations: where a group has fewer than ``count``, the rest are (-inf, beam 0, ``end_token``).
+    A row with a NaN, a logit of +inf or none above -inf has no continuation. ``finished`` (bool, one entry per row) marks beams
+    that have ended: such a beam has one, ``end_token`` at its own score. ``beams`` are places in the group, as
+    :func:`beam_reorder` takes them.
+
+    ``workspace``: scratch of :func:`beam_workspace_bytes` bytes, allocated when None; calls that may run at the same time
+    need their own. The same inputs give the same bits, whatever the batch.
+    """
+    device = _one_device(logits, scores) if finished is None else _one_device(logits, scores, finished)
+    if logits.dim() != 2 or logits.dtype not in _DTYPE_CODES:
+        raise ValueError("logits must be float32 or bfloat16 of shape (rows, vocab)")
+    rows, vocab = logits.shape
+    if vocab < 1:
+        raise ValueError("logits need at least one column")
+    if num_beams < 1 or rows % num_beams:
+        raise ValueError("rows must be a multiple of num_beams")
+    groups, count = rows // num_beams, num_beams if count is None else count
+    if not 1 <= count <= num_beams * vocab:
+        raise ValueError("count must be at least 1 and at most num_beams * vocab")
+    if scores.dtype != torch.float32 or scores.numel() != rows or not scores.is_contiguous():
+        raise ValueError("scores must be contiguous float32 with one entry per row")
+    if finished is not None and (finished.dtype != torch.bool or finished.numel() != rows or not finished.is_contiguous()):
+        raise ValueError("finished must be contiguous bool with one entry per row")
+    if not 0 <= end_token <= _INT32_MAX:
+        raise ValueError("end_token must be a token id")
+    need = beam_workspace_bytes(groups, num_beams, vocab, count)
+    if (vocab > 1 and logits.stride(1) != 1) or (rows > 1 and logits.stride(0) < vocab):
+        logits = logits.contiguous()
+    shape = (groups, count)
+    if out is None:
+        best = scores.new_empty((3, *shape))
+        out = BeamChoice(best[0], *best[1:].view(torch.int32).unbind(0))
+    else:
+        for name, tensor, dtype in zip(out._fields, out, (torch.float32, torch.int32, torch.int32)):
+            if tensor.shape != shape or tensor.dtype != dtype or not tensor.is_contiguous() or tensor.device != logits.device:
+                raise ValueError(f"out.{name} must be contiguous {str(dtype)[6:]} of shape (groups, count)")
+    if groups == 0:
+        return out
+    if workspace is None:
+        workspace = scores.new_empty((need // 4,))
+    elif workspace.device != logits.device or not workspace.is_contiguous() or workspace.numel() * workspace.element_size() < need:
+        raise ValueError(f"workspace must be contiguous, on the logits' device, and hold {need} bytes")
+    rc = _host().beam_select(
+        out.scores.data_ptr(), out.beams.data_ptr(), out.tokens.data_ptr(), logits.data_ptr(), logits.stride(0) if rows > 1 else vocab,
+        groups, vocab, scores.data_ptr(), 0 if finished is None else finished.data_ptr(), workspace.data_ptr(), need,
+        _DTYPE_CODES[logits.dtype], num_beams, count, end_token, device, _stream(device),
+    )  # fmt: skip
+    _native.check(rc, "pkv_beam_select")
+    return out
+
+
+def beam_reorder(
+    block_tables: torch.Tensor,
+    parents: torch.Tensor,
+    context_lens: torch.Tensor,
+    states: list[torch.Tensor] | tuple[torch.Tensor, ...],
+    *,
+    block_size: int,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Block tables and cached states of the beams that go on; returns the new tables.
+
+    ``block_tables``: int32 ``[groups * num_beams, max_blocks]``; ``parents``: int32 ``[groups, num_beams]``, the row of its
+    group that each child goes on from (:func:`beam_select`'s ``beams``); ``context_lens``: int32 ``[groups]``, the tokens
+    that a group's rows have cached; ``states``: up to 8 contiguous tensors ``[layers, num_blocks, ...]`` of any dtype (key
+    and value pools, their scales), changed in place. A child's row of the new tables names its parent's full
+    blocks, which the two share from then on; behind the context's blocks it names its own row's. The last, partly filled block
+    stays with its parent's first child, and each other child takes over that of a row that no child names, into which
+    its parent's is copied in every state: a group needs no block beyond its own. For that, the last blocks of a group's rows
+    have to be the rows' own. Beams that start from one prompt are given a last block each and ``parents`` of zero, the
+    prompt's row being the first.
+
+    ``out``: where the new tables go (a new tensor when None); it must not be ``block_tables``.
+    """
+    device = _one_device(block_tables, parents, context_lens, *states)
+    if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or not block_tables.is_contiguous():
+        raise ValueError("block_tables must be contiguous int32 of shape (groups * num_beams, max_blocks)")
+    if parents.dtype != torch.int32 or parents.dim() != 2 or not parents.is_contiguous():
+        raise ValueError("parents must be contiguous int32 of shape (groups, num_beams)")
+    groups, beams = parents.shape
+    rows, width = block_tables.shape
+    if not 1 <= beams <= MAX_BEAMS or rows != groups * beams:
+        raise ValueError(f"block_tables must have a row for each of 1 to {MAX_BEAMS} beams of every group")
+    if context_lens.dtype != torch.int32 or context_lens.shape != (groups,) or not context_lens.is_contiguous():
+        raise ValueError("context_lens must be contiguous int32 with one entry per group")
+    if block_size < 1:
+        raise ValueError("block_size must be >= 1")
+    if len(states) > MAX_BEAM_STATES:
+        raise ValueError(f"at most {MAX_BEAM_STATES} states")
+    num_blocks = states[0].shape[1] if states and states[0].dim() > 1 else 0
+    moved = []
+    for state in states:
+        shape = state.shape
+        if len(shape) < 2 or shape[1] != num_blocks or not state.is_contiguous():
+            raise ValueError("states must be contiguous [layers, num_blocks, ...] of one number of blocks")
+        layer = state[0].numel() * state.element_size() if shape[0] else 0
+        moved += (state.data_ptr(), layer // num_blocks if num_blocks else 0, layer, shape[0])
+    if out is None:
+        out = torch.empty_like(block_tables)
+    elif out.shape != block_tables.shape or out.dtype != torch.int32 or not out.is_contiguous() or out.device != block_tables.device:
+        raise ValueError("out must match block_tables")
+    elif out.data_ptr() == block_tables.data_ptr():
+        raise ValueError("out must not be block_tables")
+    if groups == 0:
+        return out
+    rc = _host().beam_reorder(
+        out.data_ptr(), block_tables.data_ptr(), parents.data_ptr(), context_lens.data_ptr(), groups, num_blocks, beams, width,
+        block_size, device, _stream(device), len(states), *moved,
+    )  # fmt: skip
+    _native.check(rc, "pkv_beam_reorder")
+    return out
+
+
+class StepMetadata(NamedTuple):
+    """A step's rows and requests on the device (:func:`step_metadata`): int32 ``query_seq`` and ``query_positions``, int64
+    ``positions`` and ``slot_mapping`` (one entry per row), int32 ``query_starts [S + 1]``, ``context_lens [S]`` and
+    ``next_free [1]``."""
+
+    query_seq: torch.Tensor
+    query_positions: torch.Tensor
+    positions: torch.Tensor
+    slot_mapping: torch.Tensor
+    query_starts: torch.Tensor
+    context_lens: torch.Tensor
+    next_free: torch.Tensor
+
+
+def step_metadata(
+    query_lens: torch.Tensor,
+    context_lens: torch.Tensor,
+    block_tables: torch.Tensor,
+    free_blocks: torch.Tensor,
+    next_free: torch.Tensor | None = None,
+    *,
+    block_size: int,
+    num_rows: int,
+    out: StepMetadata | None = None,
+) -> StepMetadata:
+    """What the data path's calls take of a step, from its requests' lengths, without the host: the rows' requests, positions
+    and slots, and ``block_tables`` extended in place from a list of free blocks.
+
+    ``query_lens``, ``context_lens``: int32 ``[S]``, the tokens that request i runs in this step (0: none), and its tokens
+    after the step, these among them; ``block_tables``: int32 ``[S, max_blocks]``, whose row i names the ``ceil((context -
+    query) / block_size)`` blocks that the request has, and then also those it needs for more; ``free_blocks``: int32
+    ``[F]``, taken in order from place ``next_free`` on (int32 ``[1]``; None: 0). Rows are the requests' in order, ``num_rows``
+    of them; those behind the last request's are padding (``query_seq`` and ``slot_mapping`` -1, positions 0), which
+    :func:`paged_attention_window`, :func:`paged_attention_e4m3` and the appends leave out. ``query_starts`` are the requests' first rows and
+    the end of the last; ``context_lens`` (of the result) is what the step's attention sees, and its ``next_free`` what the
+    next step starts from.
+
+    A request that cannot be served changes nothing, has padding rows and its context without this step's tokens: where the
+    free blocks do not suffice for the requests up to and with it, and it needs any; where its rows pass ``num_rows``, its table is
+    too narrow, or its context shorter than its query. ``out``: an earlier result to write to; it must not hold
+    ``context_lens`` or ``next_free`` given here. The call can be captured into a graph, whose requests then grow from replay to
+    replay.
+    """
+    device = _one_device(query_lens, context_lens, block_tables, free_blocks) if next_free is None else _one_device(
+        query_lens, context_lens, block_tables, free_blocks, next_free)  # fmt: skip
+    if query_lens.dtype != torch.int32 or query_lens.dim() != 1 or not query_lens.is_contiguous():
+        raise ValueError("query_lens must be contiguous int32 with one entry per request")
+    seqs = query_lens.shape[0]
+    if context_lens.dtype != torch.int32 or context_lens.shape != (seqs,) or not context_lens.is_contiguous():
+        raise ValueError("context_lens must be contiguous int32 with one entry per request")
+    if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or block_tables.shape[0] != seqs or not block_tables.is_contiguous():
+        raise ValueError("block_tables must be contiguous int32 of shape (num_seqs, max_blocks)")
+    if free_blocks.dtype != torch.int32 or free_blocks.dim() != 1 or not free_blocks.is_contiguous():
+        raise ValueError("free_blocks must be contiguous int32 of one dimension")
+    if next_free is not None and (next_free.dtype != torch.int32 or next_free.numel() != 1):
+        raise ValueError("next_free must be one int32")
+    width = block_tables.shape[1]
+    if block_size < 1 or width * block_size > _INT32_MAX:
+        raise ValueError("block_size must be >= 1, and a table's tokens fewer than 2^31")
+    if not 0 <= num_rows <= MAX_STEP_ROWS:
+        raise ValueError(f"num_rows must be in [0, {MAX_STEP_ROWS}]")
+    if out is None:
+        wide = query_lens.new_empty((2, num_rows), dtype=torch.int64)
+        seq, position, starts, contexts, following = query_lens.new_empty((2 * num_rows + 2 * seqs + 2,)).split((num_rows, num_rows, seqs + 1, seqs, 1))
+        out = StepMetadata(seq, position, *wide.unbind(0), starts, contexts, following)
+    else:
+        sizes, wide = (num_rows, num_rows, num_rows, num_rows, seqs + 1, seqs, 1), ("positions", "slot_mapping")
+        for name, tensor, size in zip(out._fields, out, sizes):
+            dtype = torch.int64 if name in wide else torch.int32
+            if tensor.dtype != dtype or tensor.shape != (size,) or not tensor.is_contiguous() or tensor.device != query_lens.device:
+                raise ValueError(f"out.{name} must be contiguous {str(dtype)[6:]} with {size} entries")
+        if (next_free is not None and out.next_free.data_ptr() == next_free.data_ptr()) or (
+            seqs and out.context_lens.data_ptr() == context_lens.data_ptr()
+        ):
+            raise ValueError("out must not hold the call's own context_lens or next_free")
+    rc = _host().step_metadata(
+        query_lens.data_ptr(), context_lens.data_ptr(), block_tables.data_ptr(), free_blocks.data_ptr(),
+        0 if next_free is None else next_free.data_ptr(), *(tensor.data_ptr() for tensor in out), num_rows, seqs, width,
+        free_blocks.shape[0], block_size, device, _stream(device),
+    )  # fmt: skip
+    _native.check(rc, "pkv_step_metadata")
     return out
 
 
