@@ -762,8 +762,10 @@ int pkv_append_e4m3(const pkv_e4m3_append* args, int device, void* stream);
  *   key_cache, value_cache   : e4m3 codes [num_blocks, block_size, num_kv_heads, head_dim], 16-byte aligned.
  *   key_scales, value_scales : float32 [num_blocks, num_kv_heads], powers of two from 2^-100 to 2^120. Of another
  *                              number its exponent alone counts.
- * All else is pkv_window's: a window of INT32_MAX is plain causal attention, and pkv_window_sizes gives the splits and the
- * workspace. Queries are float32 or bfloat16. A NaN code (127, 255) is a NaN to the rows that see it.
+ * workspace                : of the bytes that pkv_attention_e4m3_workspace_bytes gives.
+ * All else is pkv_window's; a window of INT32_MAX is plain causal attention. With num_splits 0, rows by themselves without a
+ * window over blocks of a multiple of 16 tokens are cut into equal shares of the call's keys, whichever rows these are of, so a
+ * row's result may differ by roundings with what else is in the batch. Queries are float32 or bfloat16. A NaN code (127, 255) is a NaN to the rows that see it.
  */
 typedef struct pkv_e4m3_attention {
   void* out;
@@ -795,6 +797,9 @@ typedef struct pkv_e4m3_attention {
   int32_t num_splits;
   float scale;
 } pkv_e4m3_attention;
+
+/* Bytes of workspace of a call with these sizes (its pointers are not looked at). Host-only. */
+int64_t pkv_attention_e4m3_workspace_bytes(const pkv_e4m3_attention* args);
 
 int pkv_attention_e4m3(const pkv_e4m3_attention* args, int device, void* stream);
 

@@ -103,6 +103,7 @@ EXPORTED_SYMBOLS = (
     "pkv_window_attention",
     "pkv_sample_tokens",
     "pkv_append_e4m3",
+    "pkv_attention_e4m3_workspace_bytes",
     "pkv_attention_e4m3",
     "pkv_step_metadata",
     "pkv_beam_workspace_bytes",
@@ -200,7 +201,7 @@ def bound_host():
     """:func:`host` with the library's entry points bound into it (``_pkvhost.bind``), so its
     ``plan``, ``paged_attention``, ``paged_attention_append``, ``copy_blocks``, ``rms_norm``,
     ``silu_mul``, ``rope_append``, ``append``, ``rope_append_axes``, ``window_workspace``,
-    ``window_attention``, ``sample_tokens``, ``append_e4m3``, ``attention_e4m3``, ``step_metadata``,
+    ``window_attention``, ``sample_tokens``, ``append_e4m3``, ``attention_e4m3_workspace``, ``attention_e4m3``, ``step_metadata``,
     ``beam_workspace``, ``beam_select``, ``beam_reorder``, ``forward`` and ``CopyQueue.flush`` call ``libpkv.so`` directly, and ``stage``, ``forward``, ``CopyQueue.flush`` and ``event_create`` call the
     ``hipMemcpyAsync`` / ``hipGetDevice`` / ``hipSetDevice`` / ``hipEvent*`` functions of the HIP
     runtime ``libpkv.so`` is linked against (looked up through the library's handle, so they are
@@ -223,7 +224,8 @@ def bound_host():
                          address(lib.pkv_append), address(lib.pkv_linear_forward),
                          address(lib.pkv_rope_append_axes), address(lib.pkv_window_sizes),
                          address(lib.pkv_window_attention), address(lib.pkv_sample_tokens),
-                         address(lib.pkv_append_e4m3), address(lib.pkv_attention_e4m3),
+                         address(lib.pkv_append_e4m3), address(lib.pkv_attention_e4m3_workspace_bytes),
+                         address(lib.pkv_attention_e4m3),
                          address(lib.pkv_step_metadata), address(lib.pkv_beam_workspace_bytes),
                          address(lib.pkv_beam_select), address(lib.pkv_beam_reorder))  # fmt: skip
                 _BOUND = True
@@ -365,6 +367,8 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.pkv_sample_tokens.restype = _c_int
     lib.pkv_append_e4m3.argtypes = [_ptr, _c_int, _ptr]  # args, device, stream
     lib.pkv_append_e4m3.restype = _c_int
+    lib.pkv_attention_e4m3_workspace_bytes.argtypes = [_ptr]  # args
+    lib.pkv_attention_e4m3_workspace_bytes.restype = _i64
     lib.pkv_attention_e4m3.argtypes = [_ptr, _c_int, _ptr]  # args, device, stream
     lib.pkv_attention_e4m3.restype = _c_int
     lib.pkv_step_metadata.argtypes = [_ptr, _c_int, _ptr]  # args, device, stream

@@ -59,7 +59,8 @@
 //   bind(plan_batch, paged_attention, paged_attention_append, copy_blocks, rms_norm, silu_mul,
 //        rope_append, memcpy_async[, gather_rows, greedy_tokens, get_device, set_device,
 //        event_create, event_record, event_synchronize, event_destroy, append, linear_forward,
-//        rope_append_axes, window_sizes, window_attention, sample_tokens, append_e4m3, attention_e4m3,
+//        rope_append_axes, window_sizes, window_attention, sample_tokens, append_e4m3,
+//        attention_e4m3_workspace_bytes, attention_e4m3,
 //        step_metadata, beam_workspace_bytes, beam_select, beam_reorder])
 //       Takes the addresses of those libpkv.so entry points (include/pkv.h), so the calls below
 //       reach the library without ctypes' per-argument conversions, and of hipMemcpyAsync,
@@ -853,6 +854,7 @@ decltype(&pkv_window_sizes) g_window_sizes = nullptr;
 decltype(&pkv_window_attention) g_window = nullptr;
 decltype(&pkv_sample_tokens) g_sample = nullptr;
 decltype(&pkv_append_e4m3) g_append_e4m3 = nullptr;
+decltype(&pkv_attention_e4m3_workspace_bytes) g_e4m3_bytes = nullptr;
 decltype(&pkv_attention_e4m3) g_attention_e4m3 = nullptr;
 decltype(&pkv_step_metadata) g_step = nullptr;
 decltype(&pkv_beam_workspace_bytes) g_beam_bytes = nullptr;
@@ -915,12 +917,12 @@ PyObject* bind(PyObject*, PyObject* args) {
   unsigned long long gather_rows = 0, greedy = 0, get_device = 0, set_device = 0;
   unsigned long long event_create = 0, event_record = 0, event_synchronize = 0, event_destroy = 0, append = 0, linear = 0;
   unsigned long long rope_axes = 0, window_sizes = 0, window = 0, sample = 0;
-  unsigned long long append_codes = 0, attention_codes = 0;
+  unsigned long long append_codes = 0, codes_bytes = 0, attention_codes = 0;
   unsigned long long step = 0, beam_bytes = 0, beam_best = 0, beam_move = 0;
-  if (!PyArg_ParseTuple(args, "KKKKKKKK|KKKKKKKKKKKKKKKKKKKK", &plan, &attention, &attention_append, &copy, &norm, &gate, &rope,
+  if (!PyArg_ParseTuple(args, "KKKKKKKK|KKKKKKKKKKKKKKKKKKKKK", &plan, &attention, &attention_append, &copy, &norm, &gate, &rope,
                         &memcpy_async, &gather_rows, &greedy, &get_device, &set_device, &event_create,
                         &event_record, &event_synchronize, &event_destroy, &append, &linear, &rope_axes, &window_sizes,
-                        &window, &sample, &append_codes, &attention_codes, &step, &beam_bytes, &beam_best, &beam_move)) {
+                        &window, &sample, &append_codes, &codes_bytes, &attention_codes, &step, &beam_bytes, &beam_best, &beam_move)) {
     return nullptr;
   }
   if (plan == 0 || attention == 0 || attention_append == 0 || copy == 0 || norm == 0 || gate == 0 || rope == 0 ||
@@ -952,6 +954,7 @@ PyObject* bind(PyObject*, PyObject* args) {
   g_window = reinterpret_cast<decltype(g_window)>(static_cast<uintptr_t>(window));
   g_sample = reinterpret_cast<decltype(g_sample)>(static_cast<uintptr_t>(sample));
   g_append_e4m3 = reinterpret_cast<decltype(g_append_e4m3)>(static_cast<uintptr_t>(append_codes));
+  g_e4m3_bytes = reinterpret_cast<decltype(g_e4m3_bytes)>(static_cast<uintptr_t>(codes_bytes));
   g_attention_e4m3 = reinterpret_cast<decltype(g_attention_e4m3)>(static_cast<uintptr_t>(attention_codes));
   g_step = reinterpret_cast<decltype(g_step)>(static_cast<uintptr_t>(step));
   g_beam_bytes = reinterpret_cast<decltype(g_beam_bytes)>(static_cast<uintptr_t>(beam_bytes));
@@ -1545,6 +1548,15 @@ PyObject* append_e4m3(PyObject*, PyObject* const* args, Py_ssize_t count) {
   return PyLong_FromLong(g_append_e4m3(&a, device, stream));
 }
 
+PyObject* attention_e4m3_workspace(PyObject*, PyObject* const* args, Py_ssize_t count) {
+  pkv_e4m3_attention a{};
+  Reader r{args, count};
+  r(a.num_queries), r(a.num_blocks), r(a.q_dtype), r(a.block_size), r(a.num_heads), r(a.num_kv_heads), r(a.head_dim), r(a.window);
+  r(a.sinks), r(a.max_context_len), r(a.max_query_len), r(a.num_splits);
+  if (!r.done() || !bound(reinterpret_cast<const void*>(g_e4m3_bytes))) return nullptr;
+  return PyLong_FromLongLong(g_e4m3_bytes(&a));
+}
+
 PyObject* attention_e4m3(PyObject*, PyObject* const* args, Py_ssize_t count) {
   pkv_e4m3_attention a{};
   int32_t device = 0;
@@ -1982,6 +1994,8 @@ PyMethodDef kMethods[] = {
      "pkv_sample_tokens with integer pointers."},
     {"append_e4m3", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(append_e4m3)), METH_FASTCALL,
      "pkv_append_e4m3 with integer pointers."},
+    {"attention_e4m3_workspace", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(attention_e4m3_workspace)), METH_FASTCALL,
+     "pkv_attention_e4m3_workspace_bytes of the sizes."},
     {"attention_e4m3", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(attention_e4m3)), METH_FASTCALL,
      "pkv_attention_e4m3 with integer pointers."},
     {"step_metadata", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(step_metadata)), METH_FASTCALL,

@@ -34,6 +34,8 @@ typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
+struct Stream;
+
 struct Window {
   void* out;
   const void* queries;
@@ -62,6 +64,12 @@ struct Window {
   uint32_t keep, flip;
   const float* key_scales;  // of e4m3 codes, [num_blocks, num_kv_heads]; else NULL
   const float* value_scales;
+  int32_t page_groups;   // 16-key groups of a block, for page_kernel
+  uint32_t page_magic;   // ceil(2^32 / page_groups)
+  Stream* stream;        // for stream_kernel; NULL where a call has splits
+  int32_t stream_groups; // shares
+  int32_t stream_least;  // rounds of a share
+  int64_t stream_places; // of parts in the workspace, two for each share and head
 };
 
 __device__ __forceinline__ float load_one(const float* p) { return *p; }
@@ -157,12 +165,23 @@ __device__ __forceinline__ int64_t row_of(const Window& a, int32_t slot, int32_t
 __device__ __forceinline__ int64_t split_index(const Window& a, int64_t t, int32_t head, int32_t split) {
   return (t * a.num_heads + head) * a.splits + split;
 }
-__device__ __forceinline__ float* split_acc(const Window& a, int64_t index, int d) {
-  return a.workspace + (2 * a.num_queries * a.num_heads * a.splits + 3) / 4 * 4 + index * d;  // 16-byte aligned
+
+// Where a row's result for `heads` heads from `head0` on goes: to the output, or, unnormalised, to the workspace.
+struct Place {
+  bool direct;
+  int64_t index;  // of head0's maximum and sum in the workspace, and of its output
+  int64_t step;   // to the next head's
+  int64_t total;  // of such results, where sums begin
+};
+__device__ __forceinline__ Place split_place(const Window& a, int64_t t, int32_t head0, int32_t split) {
+  return Place{a.splits == 1, split_index(a, t, head0, split), a.splits, a.num_queries * a.num_heads * a.splits};
 }
-__device__ __forceinline__ void store_split_sums(const Window& a, int64_t index, float top, float sum) {
+__device__ __forceinline__ void store_sums(const Window& a, const Place& to, int64_t index, float top, float sum) {
   a.workspace[index] = top;
-  a.workspace[a.num_queries * a.num_heads * a.splits + index] = sum;
+  a.workspace[to.total + index] = sum;
+}
+__device__ __forceinline__ float* acc_of(const Window& a, const Place& to, int64_t index, int d) {
+  return a.workspace + (2 * to.total + 3) / 4 * 4 + index * d;  // 16-byte aligned
 }
 
 // The maximum / sum over the four lanes {n, n + 16, n + 32, n + 48}, in each of them.
@@ -204,7 +223,7 @@ __device__ __forceinline__ uint32_t cut_piece(float& x0, float& x1) {
 // ---------------------------------------------------------------------------------------------
 template <typename QT, typename KVT, int D>
 __device__ __forceinline__ void exact_row(const Window& a, int64_t t, int32_t head, int32_t seq, Span own, Span keys,
-                                                    int32_t first, int32_t last, int32_t split) {
+                                                    int32_t first, int32_t last, const Place& to, int32_t place) {
   constexpr int kOwn = (D + kWave - 1) / kWave;
   const int lane = threadIdx.x & (kWave - 1);
   const int32_t kv_head = head / a.group;
@@ -248,7 +267,7 @@ __device__ __forceinline__ void exact_row(const Window& a, int64_t t, int32_t he
       }
     }
   }
-  if (a.splits == 1) {
+  if (to.direct) {
     QT* out = static_cast<QT*>(a.out) + (t * a.num_heads + head) * D;
     for (int e = 0; e < kOwn; ++e) {
       const int d = e * kWave + lane;
@@ -256,11 +275,11 @@ __device__ __forceinline__ void exact_row(const Window& a, int64_t t, int32_t he
     }
     return;
   }
-  const int64_t index = split_index(a, t, head, split);
-  if (lane == 0) store_split_sums(a, index, top, sum);
+  const int64_t index = to.index + place * to.step;
+  if (lane == 0) store_sums(a, to, index, top, sum);
   for (int e = 0; e < kOwn; ++e) {
     const int d = e * kWave + lane;
-    if (d < D) split_acc(a, index, D)[d] = acc[e];
+    if (d < D) acc_of(a, to, index, D)[d] = acc[e];
   }
 }
 
@@ -381,15 +400,113 @@ struct RowScratch {
   int redo[kPair];
 };
 
-// The items of workgroup `block` of `blocks`.
+// The end of a row's pass: the wavefronts' maxima, sums and outputs `o` joined, and the row's result or its part's stored.
 template <typename QT, typename KVT, int D, int kRowWaves, int kPair>
-__device__ __forceinline__ void row_pass(const Window& a, RowScratch<D, kRowWaves, kPair>& shared, uint32_t block, uint32_t blocks) {
+__device__ __forceinline__ void finish_row(const Window& a, RowScratch<D, kRowWaves, kPair>& shared, floatx4 (&o)[D / 16], float top, float sum,
+                                           int64_t t, int32_t head0, int32_t heads, int32_t seq, const Span& span, int32_t first_item,
+                                           int32_t last_item, const Place& to) {
   using S = RowShape<QT, KVT, D>;
   constexpr int kTiles = D / 16;  // output tiles of 16 dimensions
   auto& s_acc = shared.acc;
   auto& s_top = shared.top;
   auto& s_sum = shared.sum;
   auto& s_redo = shared.redo;
+  const int lane = threadIdx.x & (kWave - 1), c = lane / 16, n = lane % 16;
+  const int side = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave % kPair);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave / kPair);
+  sum = column_sum(sum);
+
+  // The wavefronts' results, lane by lane: every wavefront holds the same places.
+  __syncthreads();  // the row before has been read
+  s_top[side][wave][lane] = top;
+  s_sum[side][wave][lane] = sum;
+  __syncthreads();
+  float all = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < kRowWaves; ++w) all = fmaxf(all, s_top[side][w][lane]);
+  const float base = all == -INFINITY ? 0.f : all;
+  const float mine = fast_exp2(top - base);
+#pragma unroll
+  for (int b = 0; b < kTiles; ++b) o[b] *= mine;
+  sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < kRowWaves; ++w) sum += s_sum[side][w][lane] * fast_exp2(s_top[side][w][lane] - base);
+#pragma unroll
+  for (int half = kRowWaves / 2; half > 0; half /= 2) {
+    if (wave >= half && wave < 2 * half) {
+#pragma unroll
+      for (int b = 0; b < kTiles; ++b) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s_acc[side][wave - half][(b * 4 + r) * kWave + lane] = o[b][r];
+      }
+    }
+    __syncthreads();
+    if (wave < half) {
+#pragma unroll
+      for (int b = 0; b < kTiles; ++b) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[b][r] += s_acc[side][wave][(b * 4 + r) * kWave + lane];
+      }
+    }
+    __syncthreads();
+  }
+  if constexpr (S::kBf16) {  // what is not finite is computed again from whole numbers
+    if (wave == 0) {
+      bool bad = false;
+#pragma unroll
+      for (int b = 0; b < kTiles; ++b) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) bad = bad || !(fabsf(o[b][r]) < INFINITY);
+      }
+      const uint64_t any = __ballot((bad || !(fabsf(sum) < INFINITY)) && n < heads);
+      if (lane == 0) s_redo[side] = any != 0;
+    }
+    __syncthreads();
+    if (s_redo[side]) {
+      for (int g = wave; g < heads; g += kRowWaves) {
+        exact_row<QT, KVT, D>(a, t, head0 + g, seq, span, span, first_item, last_item, to, g);
+      }
+      return;
+    }
+  }
+  if (wave != 0 || n >= heads) return;
+  // Register r of output tile (g, e) is dimension 16 kVWidth g + kVWidth (4c + r) + e of head n.
+  const int64_t out_row = t * a.num_heads + head0 + n;
+  if (to.direct) {
+    const float scale = sum == 0.f ? 0.f : 1.f / sum;
+    QT* out = static_cast<QT*>(a.out) + out_row * D;
+#pragma unroll
+    for (int g = 0; g < S::kVLoads; ++g) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float x[S::kVWidth];
+#pragma unroll
+        for (int e = 0; e < S::kVWidth; ++e) x[e] = sum == 0.f ? 0.f : o[g * S::kVWidth + e][r] * scale;
+        store_row<QT, S::kVWidth>(out + 16 * S::kVWidth * g + S::kVWidth * (4 * c + r), x);
+      }
+    }
+  } else {
+    const int64_t index = to.index + n * to.step;
+    if (c == 0) store_sums(a, to, index, all, sum);
+    if (sum == 0.f) return;
+#pragma unroll
+    for (int g = 0; g < S::kVLoads; ++g) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float x[S::kVWidth];
+#pragma unroll
+        for (int e = 0; e < S::kVWidth; ++e) x[e] = o[g * S::kVWidth + e][r];
+        store_row<float, S::kVWidth>(acc_of(a, to, index, D) + 16 * S::kVWidth * g + S::kVWidth * (4 * c + r), x);
+      }
+    }
+  }
+}
+
+// The items of workgroup `block` of `blocks`.
+template <typename QT, typename KVT, int D, int kRowWaves, int kPair>
+__device__ __forceinline__ void row_pass(const Window& a, RowScratch<D, kRowWaves, kPair>& shared, uint32_t block, uint32_t blocks) {
+  using S = RowShape<QT, KVT, D>;
+  constexpr int kTiles = D / 16;  // output tiles of 16 dimensions
   const int lane = threadIdx.x & (kWave - 1), c = lane / 16, n = lane % 16;
   const int side = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave % kPair);  // which key head of the pair
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave / kPair);
@@ -664,92 +781,8 @@ __device__ __forceinline__ void row_pass(const Window& a, RowScratch<D, kRowWave
       live = live_next;
       slot_next = look_up(round + 2 * kRowWaves);
     }
-    sum = column_sum(sum);
-
-    // The wavefronts' results, lane by lane: every wavefront holds the same places.
-    __syncthreads();  // the row before has been read
-    s_top[side][wave][lane] = top;
-    s_sum[side][wave][lane] = sum;
-    __syncthreads();
-    float all = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < kRowWaves; ++w) all = fmaxf(all, s_top[side][w][lane]);
-    const float base = all == -INFINITY ? 0.f : all;
-    const float mine = fast_exp2(top - base);
-#pragma unroll
-    for (int b = 0; b < kTiles; ++b) o[b] *= mine;
-    sum = 0.f;
-#pragma unroll
-    for (int w = 0; w < kRowWaves; ++w) sum += s_sum[side][w][lane] * fast_exp2(s_top[side][w][lane] - base);
-#pragma unroll
-    for (int half = kRowWaves / 2; half > 0; half /= 2) {
-      if (wave >= half && wave < 2 * half) {
-#pragma unroll
-        for (int b = 0; b < kTiles; ++b) {
-#pragma unroll
-          for (int r = 0; r < 4; ++r) s_acc[side][wave - half][(b * 4 + r) * kWave + lane] = o[b][r];
-        }
-      }
-      __syncthreads();
-      if (wave < half) {
-#pragma unroll
-        for (int b = 0; b < kTiles; ++b) {
-#pragma unroll
-          for (int r = 0; r < 4; ++r) o[b][r] += s_acc[side][wave][(b * 4 + r) * kWave + lane];
-        }
-      }
-      __syncthreads();
-    }
-    if constexpr (S::kBf16) {  // what is not finite is computed again from whole numbers
-      if (wave == 0) {
-        bool bad = false;
-#pragma unroll
-        for (int b = 0; b < kTiles; ++b) {
-#pragma unroll
-          for (int r = 0; r < 4; ++r) bad = bad || !(fabsf(o[b][r]) < INFINITY);
-        }
-        const uint64_t any = __ballot((bad || !(fabsf(sum) < INFINITY)) && n < heads);
-        if (lane == 0) s_redo[side] = any != 0;
-      }
-      __syncthreads();
-      if (s_redo[side]) {
-        for (int g = wave; g < heads; g += kRowWaves) {
-          exact_row<QT, KVT, D>(a, t, head0 + g, seq, span, span, min(first * S::kKeys, count), min(last * S::kKeys, count), split);
-        }
-        continue;
-      }
-    }
-    if (wave != 0 || n >= heads) continue;
-    // Register r of output tile (g, e) is dimension 16 kVWidth g + kVWidth (4c + r) + e of head n.
-    const int64_t out_row = t * a.num_heads + head0 + n;
-    if (a.splits == 1) {
-      const float scale = sum == 0.f ? 0.f : 1.f / sum;
-      QT* out = static_cast<QT*>(a.out) + out_row * D;
-#pragma unroll
-      for (int g = 0; g < S::kVLoads; ++g) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          float x[S::kVWidth];
-#pragma unroll
-          for (int e = 0; e < S::kVWidth; ++e) x[e] = sum == 0.f ? 0.f : o[g * S::kVWidth + e][r] * scale;
-          store_row<QT, S::kVWidth>(out + 16 * S::kVWidth * g + S::kVWidth * (4 * c + r), x);
-        }
-      }
-    } else {
-      const int64_t index = split_index(a, t, head0 + n, split);
-      if (c == 0) store_split_sums(a, index, all, sum);
-      if (sum == 0.f) continue;
-#pragma unroll
-      for (int g = 0; g < S::kVLoads; ++g) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          float x[S::kVWidth];
-#pragma unroll
-          for (int e = 0; e < S::kVWidth; ++e) x[e] = o[g * S::kVWidth + e][r];
-          store_row<float, S::kVWidth>(split_acc(a, index, D) + 16 * S::kVWidth * g + S::kVWidth * (4 * c + r), x);
-        }
-      }
-    }
+    finish_row<QT, KVT, D, kRowWaves, kPair>(a, shared, o, top, sum, t, head0, heads, seq, span, min(first * S::kKeys, count),
+                                             min(last * S::kKeys, count), split_place(a, t, head0, split));
   }
 }
 
@@ -757,6 +790,409 @@ template <typename QT, typename KVT, int D, int kRowWaves, int kPair>
 __global__ __launch_bounds__(kRowWaves * kPair * kWave) void row_kernel(const Window a) {
   __shared__ RowScratch<D, kRowWaves, kPair> shared;
   row_pass<QT, KVT, D, kRowWaves, kPair>(a, shared, blockIdx.x, gridDim.x);
+}
+
+// ---------------------------------------------------------------------------------------------
+// Rows by themselves over e4m3 codes without a window, where a block's tokens are a multiple of 16: the row pass above with
+// every 16 keys of a product in one block. Their place and scales are the same for the whole wavefront, so addresses and
+// scales are scalars (a wavefront looks 64 groups' up at once), and nothing is exchanged between lanes but the maximum.
+// The codes of two neighbouring keys are interleaved before they are widened, which gives the value operand's pairs at
+// once. The next round's keys are asked for as soon as the present one's are scores, its values when the present ones are used.
+//
+// Bound: HBM. 64 rows of 16384 keys, 32/8 heads x 128, bfloat16 queries, 2.15 GB: 351 us, 6.1 TB/s (a copy of these bytes
+// by the same pieces alone: 6.7; by the general row pass above, which exchanges slots and scales between lanes, 560).
+// ---------------------------------------------------------------------------------------------
+template <typename QT, int D>
+struct PageShape {
+  static constexpr int kBlocks = D <= 128 ? 2 : 1;  // 16-key groups of a round
+  static constexpr int kBatch = kWave / kBlocks;    // rounds whose groups are looked up at once
+};
+
+// Rounds [first, last) of row t's `count` visible keys.
+template <typename QT, int D, int kRowWaves, int kPair>
+__device__ __forceinline__ void page_piece(const Window& a, RowScratch<D, kRowWaves, kPair>& shared, int64_t t, int32_t seq, int32_t count,
+                                           int32_t first, int32_t last, int32_t kv_head, int32_t head0, int32_t heads, const Place& to) {
+  using S = RowShape<QT, uint8_t, D>;
+  using P = PageShape<QT, D>;
+  constexpr int kTiles = D / 16, kKeys = 16 * P::kBlocks, kWords = S::kVWords;
+  const int lane = threadIdx.x & (kWave - 1), c = lane / 16, n = lane % 16;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave / kPair);
+  const int32_t* table = a.tables + static_cast<int64_t>(seq) * a.table_stride;
+  const int32_t mine = (last - first - wave + kRowWaves - 1) / kRowWaves;  // this wavefront's rounds (0 or less: none)
+
+  // The queries, the right operand of S^T: lane (c, n) holds its c's dimensions of head n.
+  uint32_t qr[S::kQRegs];
+  {
+    const QT* q = static_cast<const QT*>(a.queries) + t * a.query_stride + static_cast<int64_t>(head0 + min(n, heads - 1)) * D;
+#pragma unroll
+    for (int u = 0; u < S::kKSteps; ++u) {
+      if constexpr (sizeof(QT) == 2) {
+        const u32x4 x = *reinterpret_cast<const u32x4*>(q + S::dims(u, c));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) qr[4 * u + e] = (x[e] & a.keep) ^ a.flip;
+      } else {
+        const f32x4 x[2] = {*reinterpret_cast<const f32x4*>(q + S::dims(u, c)), *reinterpret_cast<const f32x4*>(q + S::dims(u, c) + 4)};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float x0 = x[e / 2][e % 2 * 2] * a.scale_log2, x1 = x[e / 2][e % 2 * 2 + 1] * a.scale_log2;
+#pragma unroll
+          for (int p = 0; p < 3; ++p) qr[4 * (p * S::kKSteps + u) + e] = take_piece(x0, x1);
+        }
+      }
+    }
+  }
+
+  // Byte offsets of this lane from a group's first row: of its key, and of the first of its four values' keys.
+  const uint32_t row_bytes = static_cast<uint32_t>(a.num_kv_heads) * D;
+  const uint32_t k_at = static_cast<uint32_t>(kv_head) * D + n * row_bytes + S::kKWidth * c;
+  const uint32_t v_at = static_cast<uint32_t>(kv_head) * D + 4 * c * row_bytes + S::kVWidth * n;
+  const char* keys = static_cast<const char*>(a.keys);
+  const char* values = static_cast<const char*>(a.values);
+
+  // A batch: lane l has the slot (-1: in no block) and the scales of group l % kBlocks of this wavefront's l / kBlocks-th round.
+  int32_t slots = -1, looked = -1;
+  float key_scales = 1.f, value_scales = 1.f;
+  const auto look_up = [&](int32_t from) {
+    const int32_t round = first + wave + kRowWaves * (from + lane / P::kBlocks);
+    const uint32_t group = static_cast<uint32_t>(round) * P::kBlocks + lane % P::kBlocks;
+    slots = -1;
+    key_scales = value_scales = 1.f;  // code 0 times a NaN is not 0
+    if (round < last && static_cast<int32_t>(group * 16) < count) {
+      const uint32_t page = a.page_groups == 1 ? group : __umulhi(group, a.page_magic);
+      const int32_t block = table[page];
+      if (block >= 0 && block < a.num_blocks) {
+        slots = block * a.block_size + static_cast<int32_t>(group - page * a.page_groups) * 16;
+        const int64_t at = static_cast<int64_t>(block) * a.num_kv_heads + kv_head;
+        key_scales = a.key_scales[at];
+        value_scales = a.value_scales[at];
+      }
+    }
+  };
+
+  struct Round {
+    Words<S::kKWidth / 4> k[P::kBlocks][S::kKLoads];
+    Words<kWords> v[P::kBlocks][4];
+    float key_scale[P::kBlocks], value_scale[P::kBlocks];
+    int32_t slot[P::kBlocks];
+  };
+  // Fetches behind the last round repeat it: without a branch around them, a wait for values leaves the keys that were
+  // asked for after them in flight.
+  const auto fetch_keys = [&](Round& x, int32_t k) {
+    k = min(k, mine - 1);
+    if (k % P::kBatch == 0 && k != looked) {
+      looked = k;
+      look_up(k);
+      // Arrived before anything else is asked for.
+      asm volatile("" : "+v"(slots), "+v"(key_scales), "+v"(value_scales));
+    }
+#pragma unroll
+    for (int j = 0; j < P::kBlocks; ++j) {
+      const int from = k % P::kBatch * P::kBlocks + j;
+      x.slot[j] = __builtin_amdgcn_readlane(slots, from);
+      x.key_scale[j] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(key_scales), from));
+      x.value_scale[j] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(value_scales), from));
+      const int64_t base = static_cast<int64_t>(max(x.slot[j], 0)) * row_bytes;
+      const char* kp = keys + base;
+#pragma unroll
+      for (int u = 0; u < S::kKLoads; ++u) x.k[j][u] = load_words<S::kKWidth / 4>(kp + (k_at + u * 4 * S::kKWidth));
+    }
+    __builtin_amdgcn_sched_barrier(0);  // loads arrive in order: no value between the keys
+  };
+  const auto fetch_values = [&](Round& x) {
+#pragma unroll
+    for (int j = 0; j < P::kBlocks; ++j) {
+      const char* vp = values + static_cast<int64_t>(max(x.slot[j], 0)) * row_bytes;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        if constexpr (S::kVWidth == 2) {
+          x.v[j][r].w[0] = __builtin_nontemporal_load(reinterpret_cast<const uint16_t*>(vp + (v_at + r * row_bytes)));
+        } else {
+          x.v[j][r] = load_words<kWords>(vp + (v_at + r * row_bytes));
+        }
+      }
+    }
+  };
+
+  floatx4 o[kTiles];
+#pragma unroll
+  for (int b = 0; b < kTiles; ++b) o[b] = floatx4{0.f, 0.f, 0.f, 0.f};
+  float top = -INFINITY, sum = 0.f;
+  const float scale = sizeof(QT) == 2 ? a.scale_log2 : 1.f;  // of the scores
+  const auto use = [&](Round& x, int32_t k, int32_t ahead) {
+    const int32_t key0 = (first + wave + kRowWaves * k) * kKeys;
+    bool whole = key0 + kKeys <= count;
+    floatx4 st[P::kBlocks];
+#pragma unroll
+    for (int j = 0; j < P::kBlocks; ++j) {
+      whole = whole && x.slot[j] >= 0;
+      st[j] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int u = 0; u < S::kKSteps; ++u) {
+        const uint32_t* w = x.k[j][D == 32 ? 0 : u / 2].w + (D == 32 ? 0 : u % 2 * 2);
+        const u32x4 key = {widen<0>(w[0], x.key_scale[j]), widen<1>(w[0], x.key_scale[j]), widen<0>(w[1], x.key_scale[j]),
+                           widen<1>(w[1], x.key_scale[j])};
+#pragma unroll
+        for (int p = S::kPieces - 1; p >= 0; --p) {  // the smallest pieces first
+          const uint32_t* q = qr + 4 * (p * S::kKSteps + u);
+          st[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, key),
+                                                          __builtin_bit_cast(bf16x8, (u32x4{q[0], q[1], q[2], q[3]})), st[j], 0, 0, 0);
+        }
+      }
+    }
+    int32_t slot_now[P::kBlocks];
+    float value_scale_now[P::kBlocks];
+#pragma unroll
+    for (int j = 0; j < P::kBlocks; ++j) slot_now[j] = x.slot[j], value_scale_now[j] = x.value_scale[j];
+    fetch_keys(x, ahead);
+    if (!whole) {
+#pragma unroll
+      for (int j = 0; j < P::kBlocks; ++j) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const bool seen = slot_now[j] >= 0 && key0 + 16 * j + 4 * c + r < count;
+          st[j][r] = seen ? st[j][r] : -INFINITY;
+#pragma unroll
+          for (int w = 0; w < kWords; ++w) x.v[j][r].w[w] = seen ? x.v[j][r].w[w] : 0;  // 0 * inf is not 0
+        }
+      }
+    }
+    float most = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < P::kBlocks; ++j) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) most = fmaxf(most, st[j][r]);
+    }
+    most = column_max(most) * scale;
+    if (__ballot(most > top) != 0) {
+      const float next = fmaxf(top, most);
+      const float keep = next == -INFINITY ? 1.f : fast_exp2(top - next);
+      sum *= keep;
+#pragma unroll
+      for (int b = 0; b < kTiles; ++b) o[b] *= keep;
+      top = next;
+    }
+    const float from = top == -INFINITY ? 0.f : top;
+    // Term 4j + r of a lane's eight is key 16j + 4c + r.
+    u32x4 pr[S::kPPieces] = {};
+#pragma unroll
+    for (int j = 0; j < P::kBlocks; ++j) {
+#pragma unroll
+      for (int r = 0; r < 4; r += 2) {
+        float x0 = fast_exp2(__builtin_fmaf(st[j][r], scale, -from)), x1 = fast_exp2(__builtin_fmaf(st[j][r + 1], scale, -from));
+        sum += x0 + x1;
+#pragma unroll
+        for (int p = 0; p < S::kPPieces; ++p) pr[p][2 * j + r / 2] = cut_piece(x0, x1);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < S::kVWidth; e += 2) {
+      // Two dimensions of a word: pairs of codes of keys r and r + 1, first one dimension's, then the other's.
+      u32x4 v[2] = {};
+#pragma unroll
+      for (int j = 0; j < P::kBlocks; ++j) {
+#pragma unroll
+        for (int r = 0; r < 4; r += 2) {
+          const uint32_t pairs = __builtin_amdgcn_perm(x.v[j][r + 1].w[e / 4], x.v[j][r].w[e / 4], e % 4 ? 0x07030602 : 0x05010400);
+          v[0][2 * j + r / 2] = widen<0>(pairs, value_scale_now[j]);
+          v[1][2 * j + r / 2] = widen<1>(pairs, value_scale_now[j]);
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int p = S::kPPieces - 1; p >= 0; --p) {
+          o[e + h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, v[h]), __builtin_bit_cast(bf16x8, pr[p]), o[e + h], 0, 0, 0);
+        }
+      }
+    }
+  };
+
+  if (mine > 0) {
+    Round x;
+    fetch_keys(x, 0);
+    fetch_values(x);
+    for (int32_t k = 0; k < mine; ++k) {
+      use(x, k, k + 1);
+      fetch_values(x);
+    }
+  }
+  finish_row<QT, uint8_t, D, kRowWaves, kPair>(a, shared, o, top, sum, t, head0, heads, seq, Span{0, 0, count}, min(first * kKeys, count),
+                                               min(last * kKeys, count), to);
+}
+
+// The key head and the first of its query heads that a wavefront serves, of the workgroup's `group` of them.
+struct Heads {
+  int32_t kv_head, head0, count;
+};
+template <int kPair>
+__device__ __forceinline__ Heads heads_of(const Window& a, uint32_t group) {
+  const uint32_t head_groups = a.num_kv_heads / kPair;
+  const int side = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave % kPair);
+  const int32_t kv_head = group % head_groups * kPair + side, sub = group / head_groups;
+  return Heads{kv_head, kv_head * a.group + sub * 16, min(16, a.group - sub * 16)};
+}
+
+// A row or one of its splits to a workgroup.
+template <typename QT, int D, int kRowWaves, int kPair>
+__global__ __launch_bounds__(kRowWaves * kPair * kWave) void page_kernel(const Window a) {
+  constexpr int kKeys = 16 * PageShape<QT, D>::kBlocks;
+  __shared__ RowScratch<D, kRowWaves, kPair> shared;
+  const uint32_t groups = a.num_kv_heads / kPair * a.subgroups;
+  const Heads h = heads_of<kPair>(a, blockIdx.x % groups);
+  const uint32_t item = blockIdx.x / groups;
+  const int32_t split = item % static_cast<uint32_t>(a.splits);
+  const int64_t t = item / static_cast<uint32_t>(a.splits);
+  const int32_t seq = a.seqs[t];
+  if (seq < 0 || seq >= a.num_seqs) return;
+  const int32_t count = span_of(a, seq, a.positions[t]).end;
+  const int32_t rounds = (count + kKeys - 1) / kKeys;
+  const int32_t first = static_cast<int32_t>(static_cast<int64_t>(rounds) * split / a.splits);
+  const int32_t last = static_cast<int32_t>(static_cast<int64_t>(rounds) * (split + 1) / a.splits);
+  page_piece<QT, D, kRowWaves, kPair>(a, shared, t, seq, count, first, last, h.kv_head, h.head0, h.count, split_place(a, t, h.head0, split));
+}
+
+// ---------------------------------------------------------------------------------------------
+// The same with equal shares of the whole call's rounds instead of splits of its rows, whose lengths only the device knows: every
+// workgroup sums all rows' rounds, and takes the rounds from `share` times its number on, through as many rows as they
+// are of. A row that lies in one share is finished there; of the others each share leaves a part in the workspace, at most
+// two (its first row's and its last's), and stream_join_kernel joins them.
+// 64 rows of 2048 to 32768 keys, 32/8 heads x 128, 2.29 GB: 379 us, 6.0 TB/s; in 16 splits of each row 437, in equal pieces of
+// 1024 keys, which all begin and end at the same time, 530. Rows of one length gain nothing and pay for the sums and the join, some
+// 10 us together: calls of up to kStreamKeys keys, and of more rows than LDS has room for the sums of, take splits (16 rows of up
+// to 1024 keys: 16 us, in shares 19).
+// ---------------------------------------------------------------------------------------------
+constexpr int kStreamRows = 1024;
+constexpr int64_t kStreamKeys = 32768;
+
+struct Stream {
+  int32_t share;                    // rounds of a workgroup
+  int32_t before[kStreamRows + 1];  // rounds of the rows before
+};
+
+// The place of a share's part of a row for one head: of its first row, or of its last.
+__device__ __forceinline__ int64_t part_index(const Window& a, int32_t share, bool first, int32_t head) {
+  return (static_cast<int64_t>(share) * 2 + (first ? 0 : 1)) * a.num_heads + head;
+}
+
+template <typename QT, int D, int kRowWaves, int kPair>
+__global__ __launch_bounds__(kRowWaves * kPair * kWave) void stream_kernel(const Window a) {
+  constexpr int kKeys = 16 * PageShape<QT, D>::kBlocks, kCount = kRowWaves * kPair * kWave, kPer = kStreamRows / kCount;
+  __shared__ RowScratch<D, kRowWaves, kPair> shared;
+  __shared__ int32_t s_before[kStreamRows + 1], s_count[kStreamRows], s_seq[kStreamRows], s_wave[kCount / kWave];
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
+  const int32_t rows = static_cast<int32_t>(a.num_queries);
+  // The sums: kPer rows to a thread.
+  int32_t rounds[kPer], all = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int32_t t = tid * kPer + i;
+    int32_t seq = t < rows ? a.seqs[t] : -1, count = 0;
+    if (seq >= 0 && seq < a.num_seqs) count = span_of(a, seq, a.positions[t]).end;
+    s_seq[t] = seq;
+    s_count[t] = count;
+    rounds[i] = (count + kKeys - 1) / kKeys;
+    all += rounds[i];
+  }
+  int32_t sum = all;
+#pragma unroll
+  for (int m = 1; m < kWave; m *= 2) {
+    const int32_t other = __shfl_up(sum, m);
+    if (lane >= m) sum += other;
+  }
+  if (lane == kWave - 1) s_wave[wave] = sum;
+  __syncthreads();
+  int32_t before = sum - all, total = 0;
+#pragma unroll
+  for (int w = 0; w < kCount / kWave; ++w) {
+    before += w < wave ? s_wave[w] : 0;
+    total += s_wave[w];
+  }
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    s_before[tid * kPer + i] = before;
+    before += rounds[i];
+  }
+  if (tid == 0) s_before[kStreamRows] = total;
+  total = __builtin_amdgcn_readfirstlane(total);
+  const int32_t share = max((total + a.stream_groups - 1) / a.stream_groups, a.stream_least);
+  __syncthreads();
+  if (blockIdx.x == 0) {
+    for (int i = tid; i <= rows; i += kCount) a.stream->before[i] = i < rows ? s_before[i] : total;
+    if (tid == 0) a.stream->share = share;
+  }
+  const uint32_t groups = a.num_kv_heads / kPair * a.subgroups;
+  const Heads h = heads_of<kPair>(a, blockIdx.x % groups);
+  const int32_t mine = blockIdx.x / groups;
+  const int32_t begin = min(static_cast<int64_t>(mine) * share, static_cast<int64_t>(total)), end = min(begin + share, total);
+  if (begin >= end) return;
+  int32_t low = 0, high = rows - 1;  // the last row that begins at or before `begin` and has rounds: the one that holds it
+  while (low < high) {
+    const int32_t middle = (low + high + 1) / 2;
+    if (s_before[middle] <= begin) low = middle; else high = middle - 1;
+  }
+  // What comes from LDS is the same in every lane, and in scalars the loops' conditions are too.
+  for (int32_t at = begin, t = __builtin_amdgcn_readfirstlane(low); at < end; ++t) {
+    const int32_t row0 = __builtin_amdgcn_readfirstlane(s_before[t]), row1 = __builtin_amdgcn_readfirstlane(s_before[t + 1]);
+    if (row1 <= at) continue;  // without rounds
+    const int32_t until = min(row1, end);
+    const Place to{row0 >= begin && row1 <= end, part_index(a, mine, row0 <= begin, h.head0), 1, a.stream_places};
+    page_piece<QT, D, kRowWaves, kPair>(a, shared, t, __builtin_amdgcn_readfirstlane(s_seq[t]), __builtin_amdgcn_readfirstlane(s_count[t]), at - row0,
+                                        until - row0, h.kv_head, h.head0, h.count, to);
+    at = until;
+  }
+}
+
+// Joins the parts of the rows that more than one share has, and clears the rows that see nothing: D / 4 threads for each row
+// and head.
+template <typename QT, int D>
+__global__ __launch_bounds__(kThreads) void stream_join_kernel(const Window a) {
+  constexpr int kPer = D / 4, kTogether = 4;
+  const uint32_t item = (blockIdx.x * static_cast<uint32_t>(kThreads) + threadIdx.x) / kPer;
+  const int d = threadIdx.x % kPer * 4;
+  const uint32_t t = item / static_cast<uint32_t>(a.num_heads);
+  if (t >= a.num_queries) return;
+  const int32_t head = item % static_cast<uint32_t>(a.num_heads);
+  const int32_t seq = a.seqs[t], share = a.stream->share, row0 = a.stream->before[t], row1 = a.stream->before[t + 1];
+  if (seq < 0 || seq >= a.num_seqs) return;
+  float x[4] = {0.f, 0.f, 0.f, 0.f};
+  QT* out = static_cast<QT*>(a.out) + static_cast<int64_t>(item) * D + d;
+  if (row0 == row1) {
+    store_row<QT, 4>(out, x);
+    return;
+  }
+  const int32_t from = row0 / share, until = (row1 - 1) / share;
+  if (from == until) return;  // its share has finished it
+  const Place place{false, 0, 1, a.stream_places};
+  float top = -INFINITY, sum = 0.f;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int32_t first = from; first <= until; first += kTogether) {
+    float tp[kTogether], part[kTogether], most = top;
+    f32x4 its[kTogether];
+#pragma unroll
+    for (int i = 0; i < kTogether; ++i) {
+      const int32_t p = min(first + i, until);
+      const int64_t index = part_index(a, p, row0 <= p * share, head);
+      tp[i] = a.workspace[index];
+      part[i] = first + i <= until ? a.workspace[place.total + index] : 0.f;
+      its[i] = *reinterpret_cast<const f32x4*>(acc_of(a, place, index, D) + d);
+    }
+#pragma unroll
+    for (int i = 0; i < kTogether; ++i) most = fmaxf(most, part[i] == 0.f ? -INFINITY : tp[i]);
+    const float base = most == -INFINITY ? 0.f : most, keep = exp2f(top - base);
+    sum *= keep;
+    acc *= keep;
+#pragma unroll
+    for (int i = 0; i < kTogether; ++i) {
+      if (part[i] == 0.f) continue;  // no key in this part: its output may hold anything
+      const float weight = exp2f(tp[i] - base);
+      sum += part[i] * weight;
+      acc += its[i] * weight;
+    }
+    top = most;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] = sum == 0.f ? 0.f : acc[e] / sum;
+  store_row<QT, 4>(out, x);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -1253,8 +1689,8 @@ __global__ __launch_bounds__(kThreads, (TileShape<QT, KVT, D>::kWaves)) void til
     if (active && !((again >> n) & 1)) {
       // Register r of output tile b is dimension 32 b + 8 (r / 4) + 4 c + r % 4 of query n.
       const int64_t out_row = t * a.num_heads + head;
-      const int64_t index = split_index(a, t, head, split);
-      if (a.splits > 1 && c == 0) store_split_sums(a, index, top, sum);
+      const Place to = split_place(a, t, head, split);
+      if (a.splits > 1 && c == 0) store_sums(a, to, to.index, top, sum);
       const float divide = sum == 0.f ? 0.f : 1.f / sum;
       if (a.splits == 1 || sum != 0.f) {
 #pragma unroll
@@ -1268,7 +1704,7 @@ __global__ __launch_bounds__(kThreads, (TileShape<QT, KVT, D>::kWaves)) void til
             if (a.splits == 1) {
               store_row<QT, 4>(static_cast<QT*>(a.out) + out_row * D + d, x);
             } else {
-              store_row<float, 4>(split_acc(a, index, D) + d, x);
+              store_row<float, 4>(acc_of(a, to, to.index, D) + d, x);
             }
           }
         }
@@ -1281,8 +1717,9 @@ __global__ __launch_bounds__(kThreads, (TileShape<QT, KVT, D>::kWaves)) void til
       one.begin = __shfl(own.begin, col);
       one.end = __shfl(own.end, col);
       const int32_t which = wave * 32 + col, row = which / a.group;
-      exact_row<QT, KVT, D>(a, run0 + row, kv_head * a.group + (which - row * a.group), seq, one, all, min(first * S::kKeys, count),
-                            min(last * S::kKeys, count), split);
+      const int32_t its_head = kv_head * a.group + (which - row * a.group);
+      exact_row<QT, KVT, D>(a, run0 + row, its_head, seq, one, all, min(first * S::kKeys, count), min(last * S::kKeys, count),
+                            split_place(a, run0 + row, its_head, split), 0);
     }
   }
 }
@@ -1301,6 +1738,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const Window a) {
   if (t >= a.num_queries) return;
   const int32_t seq = a.seqs[t];
   const int64_t index = static_cast<int64_t>(item) * a.splits;
+  const Place place = split_place(a, 0, 0, 0);
   const float* tops = a.workspace + index;
   const float* sums = a.workspace + a.num_queries * a.num_heads * a.splits + index;
   float top = -INFINITY, sum = 0.f;
@@ -1313,7 +1751,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const Window a) {
       const int p = min(first + i, a.splits - 1);
       tp[i] = tops[p];
       part[i] = first + i < a.splits ? sums[p] : 0.f;
-      out[i] = *reinterpret_cast<const f32x4*>(split_acc(a, index + p, D) + d);
+      out[i] = *reinterpret_cast<const f32x4*>(acc_of(a, place, index + p, D) + d);
     }
 #pragma unroll
     for (int i = 0; i < kTogether; ++i) most = fmaxf(most, tp[i]);
@@ -1334,6 +1772,24 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const Window a) {
 #pragma unroll
   for (int e = 0; e < 4; ++e) x[e] = sum == 0.f ? 0.f : acc[e] / sum;
   store_row<QT, 4>(static_cast<QT*>(a.out) + static_cast<int64_t>(item) * D + d, x);  // up to 2^33 elements
+}
+
+// How stream_kernel serves a call: key heads of a workgroup, and its shares. Rows are read in pieces of D bytes a head, so
+// neighbouring heads together where there is much to read (64 rows of 4096 keys, 8 key heads x 128, in even splits: 94 us with
+// four heads to a workgroup, 103 with two, 123 with one; 1 row 17.0, 14.9, 12.6). One workgroup of eight wavefronts or
+// two of four for every CU.
+struct PageForm {
+  int32_t pair, groups;
+};
+PageForm page_form(int64_t num_queries, int32_t num_kv_heads, int32_t subgroups, int32_t head_dim, int32_t max_context) {
+  const bool much = head_dim <= 128 && num_queries * max_context > 32768;
+  const int32_t pair = much && num_kv_heads % 4 == 0 ? 4 : much && num_kv_heads % 2 == 0 ? 2 : 1;
+  const int64_t columns = static_cast<int64_t>(num_kv_heads) / pair * subgroups;
+  return PageForm{pair, static_cast<int32_t>(std::max<int64_t>(1, (pair == 1 ? 512 : 256) / columns))};
+}
+int64_t stream_bytes(const PageForm& form, int32_t num_heads, int32_t head_dim) {
+  const int64_t places = 2 * static_cast<int64_t>(form.groups) * num_heads;
+  return ((2 * places + 3) / 4 * 4 + places * head_dim) * static_cast<int64_t>(sizeof(float)) + static_cast<int64_t>(sizeof(Stream) + 15) / 16 * 16;
 }
 
 template <typename QT, typename KVT, int D>
@@ -1379,6 +1835,32 @@ int launch(Window a, hipStream_t stream) {
   const auto start = [&](auto kernel, int64_t count, int waves) {
     hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(count)), dim3(waves * kWave), 0, stream, a);
   };
+  if constexpr (sizeof(KVT) == 1) {
+    if (a.page_groups > 0) {
+      a.page_magic = static_cast<uint32_t>(((int64_t{1} << 32) + a.page_groups - 1) / a.page_groups);
+      if (!a.stream) {
+        // Where there are many rows, a workgroup serves four neighbouring key heads and so reads 4 D bytes next to each other
+        // (128 rows of 256 keys, 8 key heads x 128: 17.0 us, a head to a workgroup 21.8; 16 rows 10.4 and 9.0).
+        constexpr bool kFour = D <= 128;
+        if (kFour && a.num_kv_heads % 4 == 0 && groups >= 1024) {
+          if constexpr (kFour) start(page_kernel<QT, D, 2, 4>, groups / 4, 8);
+        } else {
+          start(page_kernel<QT, D, 4, 1>, groups, 4);
+        }
+        join();
+        return check_launch();
+      }
+      const PageForm form = page_form(a.num_queries, a.num_kv_heads, a.subgroups, D, a.max_context);
+      const int64_t shares = static_cast<int64_t>(a.stream_groups) * (a.num_kv_heads / form.pair) * a.subgroups;
+      if constexpr (D <= 128) {
+        if (form.pair == 4) start(stream_kernel<QT, D, 2, 4>, shares, 8);
+        if (form.pair == 2) start(stream_kernel<QT, D, 4, 2>, shares, 8);
+      }
+      if (form.pair == 1) start(stream_kernel<QT, D, 4, 1>, shares, 4);
+      hipLaunchKernelGGL((stream_join_kernel<QT, D>), dim3(static_cast<uint32_t>(joins)), dim3(kThreads), 0, stream, a);
+      return check_launch();
+    }
+  }
   if constexpr (kWide) {
     if (wide) start(row_kernel<QT, KVT, D, 8, 1>, groups, 8);
   }
@@ -1476,6 +1958,39 @@ extern "C" int32_t pkv_window_sizes(int64_t num_queries, int32_t num_heads, int3
 
 namespace pkv {
 namespace {
+// How a call runs: its splits (below 1: refused), its bytes of workspace, and whether it has tiles beside its rows. Over codes:
+// whether page_kernel's 16 keys to a block hold, and whether its rows are cut into equal shares instead of splits.
+struct Plan {
+  int32_t splits = 0;
+  int64_t bytes = 0;
+  bool runs = false, pages = false, stream = false;
+  PageForm form{};
+};
+
+Plan window_plan(const pkv_window& g) {
+  Plan p;
+  p.runs = tiles_of(dtype_size(static_cast<pkv_dtype>(g.q_dtype)), g.head_dim) && has_runs(g.max_query_len, g.num_heads / g.num_kv_heads);
+  p.splits = pkv_window_sizes(g.num_queries, g.num_heads, g.num_kv_heads, g.head_dim, g.q_dtype, g.window, g.sinks, g.max_context_len,
+                              g.max_query_len, g.num_splits, &p.bytes);
+  return p;
+}
+
+Plan codes_plan(const pkv_window& g) {
+  Plan p = window_plan(g);
+  if (p.splits < 1 || p.runs) return p;
+  // page_kernel's offsets within 16 rows are 32-bit, and its reciprocal holds for up to 64 groups to a block.
+  p.pages = g.window == INT32_MAX && g.block_size % 16 == 0 && g.block_size <= 1024 && g.num_blocks > 0 && g.num_kv_heads <= (1 << 18);
+  // A short row is one workgroup's, which saves the join's launch.
+  p.stream = p.pages && g.num_splits == 0 && g.num_queries <= kStreamRows && g.num_queries * g.max_context_len > kStreamKeys;
+  if (p.stream) {
+    const int32_t subgroups = (g.num_heads / g.num_kv_heads + 15) / 16;
+    p.form = page_form(g.num_queries, g.num_kv_heads, subgroups, g.head_dim, g.max_context_len);
+    p.splits = 1;
+    p.bytes = stream_bytes(p.form, g.num_heads, g.head_dim);
+  }
+  return p;
+}
+
 // pkv_window_attention, and with scales pkv_attention_e4m3, whose pools hold codes (kv_dtype is not looked at then).
 int attention(const pkv_window& g, const float* key_scales, const float* value_scales, bool codes, int device, void* stream) {
   if (g.num_queries < 0 || g.num_heads < 1 || g.num_kv_heads < 1 || g.num_heads % g.num_kv_heads != 0 || g.num_seqs < 0 ||
@@ -1502,11 +2017,9 @@ int attention(const pkv_window& g, const float* key_scales, const float* value_s
       !aligned16(g.key_cache) || !aligned16(g.value_cache)) {
     return PKV_EINVAL;
   }
-  const bool tiles = tiles_of(dtype_size(static_cast<pkv_dtype>(g.q_dtype)), g.head_dim);
-  const bool runs = tiles && has_runs(g.max_query_len, g.num_heads / g.num_kv_heads);
-  int64_t need = 0;
-  const int32_t splits = pkv_window_sizes(g.num_queries, g.num_heads, g.num_kv_heads, g.head_dim, g.q_dtype, g.window, g.sinks,
-                                          g.max_context_len, g.max_query_len, g.num_splits, &need);
+  const Plan plan = codes ? codes_plan(g) : window_plan(g);
+  const int32_t splits = plan.splits;
+  const int64_t need = plan.bytes;
   if (splits < 1) return PKV_EINVAL;
   if (need > 0 && (!g.workspace || !aligned16(g.workspace) || g.workspace_bytes < need)) return PKV_EINVAL;
   Window a{};
@@ -1536,7 +2049,14 @@ int attention(const pkv_window& g, const float* key_scales, const float* value_s
   a.splits = splits;
   a.scale_log2 = g.scale * 1.44269504088896340736f;
   a.given_scale = a.scale_log2;
-  if (runs) a.list = reinterpret_cast<int32_t*>(reinterpret_cast<char*>(g.workspace) + need - list_bytes(g.num_queries));
+  if (plan.runs) a.list = reinterpret_cast<int32_t*>(reinterpret_cast<char*>(g.workspace) + need - list_bytes(g.num_queries));
+  if (plan.pages) a.page_groups = g.block_size / 16;
+  if (plan.stream) {
+    a.stream_groups = plan.form.groups;
+    a.stream_least = 8;
+    a.stream_places = 2 * static_cast<int64_t>(a.stream_groups) * g.num_heads;
+    a.stream = reinterpret_cast<Stream*>(reinterpret_cast<char*>(g.workspace) + need - (sizeof(Stream) + 15) / 16 * 16);
+  }
   DeviceGuard guard(device);
   if (!guard.ok()) return PKV_EHIP;
   auto s = static_cast<hipStream_t>(stream);
@@ -1557,9 +2077,9 @@ extern "C" int pkv_window_attention(const pkv_window* args, int device, void* st
   return args ? pkv::attention(*args, nullptr, nullptr, false, device, stream) : PKV_EINVAL;
 }
 
-extern "C" int pkv_attention_e4m3(const pkv_e4m3_attention* args, int device, void* stream) {
-  if (!args) return PKV_EINVAL;
-  const pkv_e4m3_attention& g = *args;
+namespace pkv {
+namespace {
+pkv_window window_of(const pkv_e4m3_attention& g) {
   pkv_window w{};
   w.out = g.out;
   w.queries = g.queries;
@@ -1587,5 +2107,24 @@ extern "C" int pkv_attention_e4m3(const pkv_e4m3_attention* args, int device, vo
   w.max_query_len = g.max_query_len;
   w.num_splits = g.num_splits;
   w.scale = g.scale;
-  return pkv::attention(w, g.key_scales, g.value_scales, true, device, stream);
+  return w;
+}
+}  // namespace
+}  // namespace pkv
+
+extern "C" int64_t pkv_attention_e4m3_workspace_bytes(const pkv_e4m3_attention* args) {
+  if (!args) return PKV_EINVAL;
+  const pkv_e4m3_attention& g = *args;
+  if (g.num_queries < 0 || g.num_heads < 1 || g.num_kv_heads < 1 || g.num_heads % g.num_kv_heads != 0 || g.head_dim < 1 || g.block_size < 1 ||
+      g.window < 1 || g.sinks < 0 || g.max_context_len < 0 || g.max_query_len < 0 || g.num_splits < 0 || g.num_splits > PKV_WINDOW_MAX_SPLITS ||
+      g.num_heads / g.num_kv_heads > PKV_WINDOW_MAX_GROUP) {
+    return PKV_EINVAL;
+  }
+  const pkv::Plan plan = pkv::codes_plan(pkv::window_of(g));
+  return plan.splits < 1 ? PKV_EINVAL : plan.bytes;
+}
+
+extern "C" int pkv_attention_e4m3(const pkv_e4m3_attention* args, int device, void* stream) {
+  if (!args) return PKV_EINVAL;
+  return pkv::attention(pkv::window_of(*args), args->key_scales, args->value_scales, true, device, stream);
 }

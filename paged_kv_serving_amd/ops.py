@@ -37,6 +37,7 @@ __all__ = [
     "paged_attention_e4m3",
     "paged_attention_ragged",
     "paged_attention_window",
+    "e4m3_workspace_bytes",
     "BatchPlan",
     "batch_hints",
     "NativePlanner",
@@ -1836,8 +1837,9 @@ def paged_attention_e4m3(
     ``key_cache``/``value_cache``: contiguous float8_e4m3fn ``[num_blocks, block_size, kv_heads, head_dim]``;
     ``key_scales``/``value_scales``: contiguous float32 ``[num_blocks, kv_heads]``, powers of two (of another number its
     power of two alone counts). Codes are widened to bfloat16, which holds a code times its scale exactly, on their way
-    into the products. Queries are float32 or bfloat16. The workspace is :func:`window_workspace_bytes`'s, for a
-    ``window`` of ``max_context_len`` where there is none.
+    into the products. Queries are float32 or bfloat16. ``workspace`` has :func:`e4m3_workspace_bytes` bytes. Without
+    ``num_splits`` and a window, decode rows over blocks of a multiple of 16 tokens are cut into equal shares of the call's
+    keys, whichever rows these are of: what else is in a batch may change a row's result by roundings.
     """
     device = _one_device(queries, query_positions, query_seq, key_cache, value_cache, key_scales, value_scales, block_tables, context_lens)
     _e4m3_pools(key_cache, value_cache, key_scales, value_scales)
@@ -1899,7 +1901,11 @@ def _windowed(
     window, sinks = min(window, _INT32_MAX), min(sinks, _INT32_MAX)
     rows = num_queries if max_query_len is None else min(max_query_len, _INT32_MAX)
     host = _host()
-    splits, need = host.window_workspace(num_queries, heads, kv_heads, dim, q_code, window, sinks, max_context_len, rows, num_splits)
+    if kv_code is None:
+        splits = num_splits
+        need = host.attention_e4m3_workspace(num_queries, num_blocks, q_code, block_size, heads, kv_heads, dim, window, sinks, max_context_len, rows, splits)
+    else:
+        splits, need = host.window_workspace(num_queries, heads, kv_heads, dim, q_code, window, sinks, max_context_len, rows, num_splits)
     if need:
         if workspace is None:
             workspace = context_lens.new_empty((need // 4,))  # no values yet: four bytes an entry
@@ -1918,6 +1924,24 @@ def _windowed(
         rc = host.window_attention(*before, *middle, kv_code, *after)
     _native.check(rc, "pkv_attention_e4m3" if kv_code is None else "pkv_window_attention")
     return out
+
+
+def e4m3_workspace_bytes(
+    num_queries: int, heads: int, kv_heads: int, head_dim: int, *, block_size: int, window: int | None = None, sinks: int = 0,
+    max_context_len: int, max_query_len: int | None = None, num_splits: int = 0,
+) -> int:  # fmt: skip
+    """Bytes of float32 workspace :func:`paged_attention_e4m3` needs for these sizes, whatever its queries' type."""
+    rows = num_queries if max_query_len is None else max_query_len
+    window = _INT32_MAX if window is None else min(window, _INT32_MAX)
+    needs = [
+        _host().attention_e4m3_workspace(num_queries, blocks, code, block_size, heads, kv_heads, head_dim, window, min(sinks, _INT32_MAX), max_context_len,
+                                         min(rows, _INT32_MAX), num_splits)
+        for code in _DTYPE_CODES.values()
+        for blocks in (0, 1)  # a pool without a block takes another path
+    ]  # fmt: skip
+    if min(needs) < 0:
+        raise ValueError("invalid e4m3 workspace query")
+    return max(needs)
 
 
 def window_workspace_bytes(

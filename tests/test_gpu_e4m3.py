@@ -496,3 +496,127 @@ def test_no_rows_no_context_no_blocks_and_refusals(device):
     for change, more in bad:
         with pytest.raises(ValueError):
             call(device, {**d, **change}, **more)
+
+
+# --- decode rows in equal shares -------------------------------------------------------------------
+
+UNEVEN = [700, 1, 33, 2000, 64, 32, 5, 900, 16, 1200, 31, 300, 2, 17, 450, 100]  # together more than one workgroup's share
+
+
+@pytest.mark.parametrize("io", IO)
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 4, 128), (8, 8, 64), (12, 6, 128), (4, 4, 32), (3, 3, 128), (4, 2, 256), (40, 2, 64), (64, 4, 32)])
+def test_rows_in_equal_shares(device, io, heads, kv_heads, dim):
+    """Rows in one share, in several, and shares of several rows; four, two or one key head to a workgroup."""
+    runs = [(1, c) for c in UNEVEN * 2]
+    check(device, make(runs, heads, kv_heads, dim, 16, io, seed=heads + dim), max_query_len=1)
+
+
+@pytest.mark.parametrize("block", [16, 32, 48, 1024])
+def test_shares_of_other_blocks(device, block):
+    check(device, make([(1, c) for c in UNEVEN * 2], 8, 4, 64, block, "bfloat16", seed=block), max_query_len=1)
+
+
+@pytest.mark.parametrize("io", IO)
+def test_shares_with_rows_that_see_nothing_padding_and_missing_blocks(device, io):
+    import torch
+
+    d = make([(1, c) for c in UNEVEN * 2], 8, 4, 64, 16, io, seed=3)
+    d["contexts"][[0, 5, 6, 31]] = 0
+    d["positions"][9] = -1
+    d["positions"][20] = 100  # fewer keys than its context
+    d["seqs"][[3, 14, 30]] = -1, 32, 2**31 - 1
+    d["tables"][7, 10:20], d["tables"][19, 0], d["tables"][25, -5:] = -1, 10**6, -2
+    out = torch.full(d["q"].shape, 5.0, dtype=d["q"].dtype, device=device)
+    got = check(device, d, max_query_len=1, out=out)
+    assert not got[[0, 5, 6, 9, 31]].any() and (got[[3, 14, 30]] == 5.0).all()
+    d["contexts"][:] = 0
+    assert not call(device, d, max_query_len=1, max_context_len=2000).float().cpu().numpy()[[0, 1, 2]].any()
+
+
+@pytest.mark.parametrize("io", IO)
+def test_shares_with_nan_codes(device, io):
+    d = make([(1, c) for c in UNEVEN * 2], 8, 4, 64, 16, io, seed=4)
+    clean = check(device, d, max_query_len=1)
+    want, size = window_attention(d["q"].float().numpy(), d["positions"], d["seqs"], e4m3.values(d["k"], d["ks"]), e4m3.values(d["v"], d["vs"]),
+                                  d["tables"], d["contexts"], d["scale"], CAUSAL, 0)  # fmt: skip
+    off = bound(d, want, size)
+    for s, j, h, dim in ((3, 1999, 1, 7), (7, 0, 2, 63), (0, 350, 0, 0), (1, 0, 3, 5)):
+        d["v"][d["tables"][s, j // 16], j % 16, h, dim] = np.nan
+    got = call(device, d, max_query_len=1).float().cpu().numpy()
+    for s, h, dim in ((3, 1, 7), (7, 2, 63), (0, 0, 0), (1, 3, 5)):
+        assert np.isnan(got[s, 2 * h : 2 * h + 2, dim]).all()
+        got[s, 2 * h : 2 * h + 2, dim] = clean[s, 2 * h : 2 * h + 2, dim]
+    assert (np.abs(got - clean) <= 2 * off).all()
+
+
+@pytest.mark.parametrize("rows", [1, 2, 1023, 1024, 1025])
+def test_as_many_rows_as_shares_take_and_more(device, rows):
+    d = make([(1, 40 if rows > 2 else 33000)] * rows, 4, 4, 32, 16, "bfloat16", seed=rows)
+    rng = np.random.default_rng(rows)
+    if rows > 2:
+        d["contexts"] = rng.integers(0, 41, rows).astype(np.int32)
+        d["positions"] = (d["contexts"] - 1).astype(np.int32)
+    check(device, d, max_query_len=1, max_context_len=int(max(40, d["contexts"].max())))
+
+
+def test_shares_captured_and_replayed_with_another_batch(device):
+    """One graph and one workspace, batches whose rows and lengths change."""
+    import torch
+
+    from paged_kv_serving_amd import ops
+
+    most, heads, kv_heads, dim = 2000, 8, 4, 64
+    rng = np.random.default_rng(1)
+    cases = [make([(1, int(c)) for c in lengths], heads, kv_heads, dim, 16, "bfloat16", seed=i)
+             for i, lengths in enumerate((UNEVEN * 2, [2000] * 32, rng.integers(1, 2001, 32), [1] * 31 + [1990]))]  # fmt: skip
+    blocks, width = max(c["k"].shape[0] for c in cases), most // 16
+    buf = {
+        "q": torch.zeros((32, heads, dim), dtype=torch.bfloat16, device=device), "tables": torch.zeros((32, width), dtype=torch.int32, device=device),
+        **{name: torch.zeros((blocks, 16, kv_heads, dim), dtype=torch.uint8, device=device) for name in "kv"},
+        **{name: torch.ones((blocks, kv_heads), device=device) for name in ("ks", "vs")},
+        **{name: torch.zeros(32, dtype=torch.int32, device=device) for name in ("positions", "seqs", "contexts")},
+    }  # fmt: skip
+    out = torch.zeros_like(buf["q"])
+    need = ops.e4m3_workspace_bytes(32, heads, kv_heads, dim, block_size=16, max_context_len=most, max_query_len=1)
+    workspace = torch.full((need // 4,), float("nan"), device=device)
+
+    def run():
+        ops.paged_attention_e4m3(buf["q"], buf["positions"], buf["seqs"], buf["k"].view(torch.float8_e4m3fn), buf["v"].view(torch.float8_e4m3fn), buf["ks"],
+                                 buf["vs"], buf["tables"], buf["contexts"], dim**-0.5, max_context_len=most, max_query_len=1, out=out, workspace=workspace)  # fmt: skip
+
+    run()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    for d in cases * 2:
+        for name in "kv":
+            buf[name][: d[name].shape[0]].copy_(codes_of(d[name]).view(torch.uint8))
+            buf[name + "s"][: d[name].shape[0]].copy_(torch.from_numpy(d[name + "s"]))
+        buf["q"].copy_(d["q"])
+        for name in ("positions", "seqs", "contexts"):
+            buf[name].copy_(torch.from_numpy(d[name]))
+        buf["tables"].zero_()
+        cols = min(width, d["tables"].shape[1])
+        buf["tables"][:, :cols].copy_(torch.from_numpy(d["tables"][:, :cols]))
+        graph.replay()
+        torch.cuda.synchronize()
+        wide = {**d, "tables": np.pad(d["tables"], ((0, 0), (0, max(0, width - d["tables"].shape[1]))), constant_values=-7)}
+        assert torch.equal(out, call(device, wide, max_query_len=1, max_context_len=most))
+
+
+def test_the_workspace_that_a_call_needs(device):
+    import torch
+
+    from paged_kv_serving_amd import ops
+
+    d = make([(1, c) for c in UNEVEN * 2], 8, 4, 64, 16, "bfloat16", seed=3)
+    need = ops.e4m3_workspace_bytes(32, 8, 4, 64, block_size=16, max_context_len=2000, max_query_len=1)
+    assert need > 0
+    check(device, d, max_query_len=1, workspace=torch.empty(need // 4, device=device))
+    with pytest.raises(ValueError, match="workspace"):
+        call(device, d, max_query_len=1, workspace=torch.empty(need // 4 - 1, device=device))
+    for more in ({"num_splits": 3}, {"window": 100}, {"max_query_len": 40}, {}):
+        for block in (16, 12):
+            e = make([(1, 700), (1, 5)], 4, 4, 64, block, "float32", seed=1)
+            need = ops.e4m3_workspace_bytes(2, 4, 4, 64, block_size=block, max_context_len=700, **more)
+            check(device, e, workspace=torch.empty(max(1, need // 4), device=device), **more)

@@ -79,6 +79,32 @@ def test_attention_refusals(lib, changes, code) -> None:
     assert refused(lib.pkv_attention_e4m3, structure("pkv_e4m3_attention"), ATTENTION, **changes) == code
 
 
+def test_the_attentions_workspace(lib) -> None:
+    kind = structure("pkv_e4m3_attention")
+
+    def need(**changes) -> int:
+        args = kind()
+        for name, value in {**ATTENTION, "num_splits": 0, "sinks": 0, **changes}.items():
+            setattr(args, name, value)
+        return lib.pkv_attention_e4m3_workspace_bytes(ctypes.addressof(args))
+
+    decode = dict(window=(1 << 31) - 1, max_query_len=1, num_queries=64, max_context_len=32768, num_heads=32, num_kv_heads=8, head_dim=128)
+    shares = need(**decode)
+    assert shares >= 2 * 32 * 130 * 4 * 128 and shares % 16 == 0  # two parts of every head for each of 128 shares
+    assert need(**{**decode, "num_queries": 65}) == shares  # whatever the rows
+    assert need(**decode, num_splits=1) == 0 and need(**{**decode, "max_context_len": 500}) == 0
+    for more in ({"num_splits": 5}, {"block_size": 24}, {"window": 4096}, {"num_blocks": 0}, {"num_queries": 1025}):  # as windowed attention's
+        args = {**ATTENTION, "num_splits": 0, "sinks": 0, **decode, **more}
+        size = ctypes.c_int64()
+        sizes = [args[name] for name in ("num_queries", "num_heads", "num_kv_heads", "head_dim", "q_dtype", "window", "sinks", "max_context_len", "max_query_len",
+                                         "num_splits")]  # fmt: skip
+        assert lib.pkv_window_sizes(*sizes, ctypes.addressof(size)) >= 1
+        assert need(**{**decode, **more}) == size.value
+    for bad in ({"num_queries": -1}, {"num_heads": 7}, {"num_kv_heads": 0}, {"block_size": 0}, {"window": 0}, {"num_splits": 65}, {"q_dtype": 2}, {"num_heads": 130}):
+        assert need(**bad) == EINVAL
+    assert lib.pkv_attention_e4m3_workspace_bytes(None) == EINVAL
+
+
 def test_no_arguments_and_nothing_to_do(lib) -> None:
     for function in (lib.pkv_append_e4m3, lib.pkv_attention_e4m3):
         assert function(None, 0, None) == EINVAL
