@@ -70,6 +70,7 @@ struct Window {
   int32_t stream_groups; // shares
   int32_t stream_least;  // rounds of a share
   int64_t stream_places; // of parts in the workspace, two for each share and head
+  int32_t* order;        // of the aligned blocks of rows, the longest first; NULL: as they come
 };
 
 __device__ __forceinline__ float load_one(const float* p) { return *p; }
@@ -356,9 +357,35 @@ __device__ __forceinline__ Words<N> load_words(const void* p) {
 // outside every sequence are left out. One workgroup of independent wavefronts, 5.0 us for 4096 rows (with
 // barriers for an order 6.3): a workgroup per possible row that finds out for itself took 48 us of a
 // prefill of 8 x 512 rows.
+//
+// kOrder: also the aligned blocks in the order of the keys that their rows see (three rows of a block speak for it), the most first, for
+// as many blocks as the workgroup has threads. The tiles' workgroups then end together: 8 x 512 rows behind up to 2048 others,
+// 32/8 heads x 128 over e4m3 codes, 250 -> 208 us.
 constexpr int kListThreads = 1024;
+template <bool kOrder>
 __global__ __launch_bounds__(kListThreads) void list_kernel(const Window a) {
   __shared__ int32_t s_found;
+  if constexpr (kOrder) {
+    __shared__ int32_t s_keys[kListThreads];
+    const int32_t blocks = static_cast<int32_t>((a.num_queries + a.tile_rows - 1) / a.tile_rows), b = threadIdx.x;
+    int32_t keys = 0;
+    if (b < blocks) {
+      const int64_t begin = static_cast<int64_t>(b) * a.tile_rows, end = min(begin + a.tile_rows, a.num_queries);
+      const int64_t at[3] = {begin, (begin + end) / 2, end - 1};
+#pragma unroll
+      for (int i = 0; i < 3; ++i) {
+        const int32_t seq = a.seqs[at[i]];
+        if (seq >= 0 && seq < a.num_seqs) keys = max(keys, span_of(a, seq, a.positions[at[i]]).count());
+      }
+    }
+    s_keys[b] = keys;
+    __syncthreads();
+    if (b < blocks) {
+      int32_t place = 0;
+      for (int32_t j = 0; j < blocks; ++j) place += s_keys[j] > keys || (s_keys[j] == keys && j < b) ? 1 : 0;
+      a.order[place] = b;
+    }
+  }
   if (threadIdx.x == 0) s_found = 0;
   __syncthreads();
   const int lane = threadIdx.x & (kWave - 1);
@@ -1303,6 +1330,11 @@ __device__ __forceinline__ uint32_t lds_address(const uint16_t* p) {
   return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) uint16_t*)(p)));
 }
 
+// Eight bytes from global memory: of a chosen pointer the compiler no longer knows that it is one into global memory.
+__device__ __forceinline__ u32x2 load_global(const void* from) {
+  return *(const __attribute__((address_space(1))) u32x2*)(from);
+}
+
 // 16 bytes per lane from global memory to LDS: `to`, the same in every lane, is the first lane's place.
 __device__ __forceinline__ void load_to_lds(const void* from, uint16_t* to) {
   typedef const __attribute__((address_space(1))) void* global_ptr;
@@ -1332,6 +1364,7 @@ __global__ __launch_bounds__(kThreads, (TileShape<QT, KVT, D>::kWaves)) void til
   extern __shared__ __align__(16) uint16_t s_kv[];  // [buffer][K, V][piece][key][D]
   __shared__ int32_t s_slot[3][S::kKeys];
   __shared__ uint64_t s_live[3];
+  __shared__ float s_scale[3][2][sizeof(KVT) == 1 ? S::kKeys : 1];  // of codes, for keys and values
   const int tid = threadIdx.x, lane = tid & (kWave - 1), c = lane / 32, n = lane % 32;
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   // The rows outside the runs in the same launch, before bfloat16's tiles and behind float32's, which take
@@ -1348,7 +1381,11 @@ __global__ __launch_bounds__(kThreads, (TileShape<QT, KVT, D>::kWaves)) void til
   const int32_t kv_head = item % static_cast<uint32_t>(a.num_kv_heads);
   item /= static_cast<uint32_t>(a.num_kv_heads);
   const int32_t split = item % static_cast<uint32_t>(a.splits);
-  const int64_t block0 = static_cast<int64_t>(item / static_cast<uint32_t>(a.splits)) * a.tile_rows;
+  int64_t block0 = item / static_cast<uint32_t>(a.splits);
+  if constexpr (sizeof(KVT) == 1) {
+    if (a.order) block0 = a.order[block0];
+  }
+  block0 *= a.tile_rows;
   const int64_t block1 = min(block0 + a.tile_rows, a.num_queries);
   const KVT* keys = static_cast<const KVT*>(a.keys);
   const KVT* values = static_cast<const KVT*>(a.values);
@@ -1470,11 +1507,25 @@ __global__ __launch_bounds__(kThreads, (TileShape<QT, KVT, D>::kWaves)) void til
         if (tid == 0) s_live[tile % 3] = live;
       }
     };
+    // Scales of codes: asked for when a tile's table entries have arrived, one tile after these and one before the rows are put.
     constexpr bool kCodes = sizeof(KVT) == 1;
+    struct Scales {
+      float key, value;
+    };
+    auto look_up_scales = [&](const Entry& e) {
+      Scales s{1.f, 1.f};  // in no block: code 0 times a NaN is not 0
+      if (e.block >= 0 && e.block < a.num_blocks) {
+        const int64_t at = static_cast<int64_t>(e.block) * a.num_kv_heads + kv_head;
+        s = Scales{a.key_scales[at], a.value_scales[at]};
+      }
+      return s;
+    };
+    auto keep_scales = [&](int32_t tile, const Scales& s) {
+      if (tid < S::kKeys) s_scale[tile % 3][0][tid] = s.key, s_scale[tile % 3][1][tid] = s.value;
+    };
     constexpr int kWide = sizeof(KVT) / 2;  // 16-byte loads of a chunk
     u32x4 kx[S::kStaged][kWide ? kWide : 1], vx[S::kStaged][kWide ? kWide : 1];
-    u32x2 kc[kCodes ? S::kStaged : 1], vc[kCodes ? S::kStaged : 1];  // eight codes each, and their scales
-    float ks[kCodes ? S::kStaged : 1], vs[kCodes ? S::kStaged : 1];
+    u32x2 kc[kCodes ? S::kStaged : 1], vc[kCodes ? S::kStaged : 1];  // eight codes each
     auto load = [&](int32_t tile, int buffer) {
 #pragma unroll
       for (int i = 0; i < S::kStaged; ++i) {
@@ -1482,15 +1533,8 @@ __global__ __launch_bounds__(kThreads, (TileShape<QT, KVT, D>::kWaves)) void til
         const int32_t slot = s_slot[tile % 3][row];
         const int64_t from = row_of(a, slot, kv_head, D);
         if constexpr (kCodes) {
-          kc[i] = vc[i] = u32x2{0, 0};
-          ks[i] = vs[i] = 1.f;
-          if (slot >= 0) {
-            const int64_t at = scale_of(a, slot, kv_head);
-            ks[i] = a.key_scales[at];
-            vs[i] = a.value_scales[at];
-            kc[i] = *reinterpret_cast<const u32x2*>(keys + from + 8 * chunk);
-            vc[i] = *reinterpret_cast<const u32x2*>(values + from + 8 * chunk);
-          }
+          kc[i] = load_global(slot >= 0 ? static_cast<const void*>(keys + from + 8 * chunk) : zeros);
+          vc[i] = load_global(slot >= 0 ? static_cast<const void*>(values + from + 8 * chunk) : zeros);
         } else if constexpr (kWide == 1) {
           // Straight to LDS, where a wavefront's 64 chunks lie one after the other: the permutation is made
           // by which chunk of the row a lane fetches (it is its own inverse).
@@ -1527,14 +1571,15 @@ __global__ __launch_bounds__(kThreads, (TileShape<QT, KVT, D>::kWaves)) void til
 #pragma unroll
       for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x4*>(plane(buffer, which, p) + to) = piece[p];
     };
-    auto stage = [&](int buffer) {
+    auto stage = [&](int32_t tile, int buffer) {
       if constexpr (kWide == 1) {
         __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wavefront's loads to LDS have arrived
       } else if constexpr (kCodes) {
 #pragma unroll
         for (int i = 0; i < S::kStaged; ++i) {
-          put_codes(buffer, 0, i, kc[i], ks[i]);
-          put_codes(buffer, 1, i, vc[i], vs[i]);
+          const int row = (tid + i * kThreads) / S::kChunks;
+          put_codes(buffer, 0, i, kc[i], s_scale[tile % 3][0][row]);
+          put_codes(buffer, 1, i, vc[i], s_scale[tile % 3][1][row]);
         }
       } else {
 #pragma unroll
@@ -1546,17 +1591,27 @@ __global__ __launch_bounds__(kThreads, (TileShape<QT, KVT, D>::kWaves)) void til
     };
 
     __syncthreads();  // the run before is done with LDS
-    keep_slots(first, look_up(first));
-    keep_slots(first + 1, look_up(first + 1));
+    Entry waiting{-1, -1};  // of codes: the tile's after the next
+    {
+      const Entry one = look_up(first), two = look_up(first + 1);
+      keep_slots(first, one);
+      keep_slots(first + 1, two);
+      if constexpr (kCodes) {
+        waiting = look_up(first + 2);
+        keep_scales(first, look_up_scales(one));
+        keep_scales(first + 1, look_up_scales(two));
+      }
+    }
     __syncthreads();
     if (first < last) {
       load(first, 0);
-      stage(0);
+      stage(first, 0);
     }
     __syncthreads();
     for (int32_t tile = first; tile < last; ++tile) {
       const int buffer = (tile - first) & 1;
-      const Entry ahead = look_up(tile + 2);
+      const Entry ahead = kCodes ? look_up(tile + 3) : look_up(tile + 2);
+      const Scales scales = kCodes ? look_up_scales(waiting) : Scales{};
       if (tile + 1 < last) load(tile + 1, buffer ^ 1);
       const uint64_t tile_live = s_live[tile % 3];
       // The tile's 32-key blocks one after the other through the scores, together through the softmax.
@@ -1669,8 +1724,14 @@ __global__ __launch_bounds__(kThreads, (TileShape<QT, KVT, D>::kWaves)) void til
           }
         }
       }
-      if (tile + 1 < last) stage(buffer ^ 1);
-      keep_slots(tile + 2, ahead);
+      if (tile + 1 < last) stage(tile + 1, buffer ^ 1);
+      if constexpr (kCodes) {
+        keep_slots(tile + 2, waiting);
+        keep_scales(tile + 2, scales);
+        waiting = ahead;
+      } else {
+        keep_slots(tile + 2, ahead);
+      }
       __syncthreads();
     }
     {
@@ -1817,7 +1878,11 @@ int launch(Window a, hipStream_t stream) {
         return PKV_EHIP;
       }
       a.tile_items = static_cast<uint32_t>(tiles);
-      hipLaunchKernelGGL(list_kernel, dim3(1), dim3(kListThreads), 0, stream, a);
+      if (a.order) {
+        hipLaunchKernelGGL(list_kernel<true>, dim3(1), dim3(kListThreads), 0, stream, a);
+      } else {
+        hipLaunchKernelGGL(list_kernel<false>, dim3(1), dim3(kListThreads), 0, stream, a);
+      }
       hipLaunchKernelGGL((tile_kernel<QT, KVT, D>), dim3(static_cast<uint32_t>(tiles + groups)), dim3(kThreads), S::kLds, stream, a);
       join();
       return check_launch();
@@ -1962,7 +2027,7 @@ namespace {
 // whether page_kernel's 16 keys to a block hold, and whether its rows are cut into equal shares instead of splits.
 struct Plan {
   int32_t splits = 0;
-  int64_t bytes = 0;
+  int64_t bytes = 0, order_bytes = 0;  // the order's are its last
   bool runs = false, pages = false, stream = false;
   PageForm form{};
 };
@@ -1975,9 +2040,32 @@ Plan window_plan(const pkv_window& g) {
   return p;
 }
 
+// The blocks of rows that list_kernel orders, 0 where they are too many.
+int64_t ordered_blocks(int64_t num_queries, int32_t group) {
+  const int64_t rows = kTileQueries / group, blocks = (num_queries + rows - 1) / rows;
+  return blocks <= kListThreads ? blocks : 0;
+}
+
 Plan codes_plan(const pkv_window& g) {
   Plan p = window_plan(g);
-  if (p.splits < 1 || p.runs) return p;
+  if (p.splits < 1) return p;
+  if (p.runs) {
+    const int32_t group = g.num_heads / g.num_kv_heads;
+    if (g.num_splits == 0) {
+      // Tiles of bfloat16 queries are two to a CU, of float32 ones one. Shares of 384 keys at least, of 128 where tiles are few: a part
+      // more of every row is written and joined. 1 x 128 rows of up to 4128 keys, 32/8 heads x 128, float32, with 4, 8, 16 splits:
+      // 46, 39, 53 us; 2 x 301 rows beside 24, 16 heads x 64, window 1000, with 1, 2, 3, 6: 58, 46, 54, 65; 1 x 32 rows of
+      // 1032 keys, 16/2 heads x 64, bfloat16, with 2, 4, 8: 19, 15, 15.
+      const int64_t rows = kTileQueries / group, groups = (g.num_queries + rows - 1) / rows * g.num_kv_heads;
+      const int64_t longest = std::min<int64_t>(g.max_context_len, static_cast<int64_t>(g.window) + g.sinks);
+      const int64_t most = std::min<int64_t>(PKV_WINDOW_MAX_SPLITS, longest / (groups <= 16 ? 128 : 384));
+      p.splits = static_cast<int32_t>(std::max<int64_t>(1, std::min(most, (g.q_dtype == PKV_F32 ? 256 : 512) / groups)));
+      p.bytes = pkv_window_workspace_bytes(g.num_queries, g.num_heads, g.head_dim, g.max_query_len, p.splits);
+    }
+    p.order_bytes = (ordered_blocks(g.num_queries, group) + 3) / 4 * 16;
+    p.bytes += p.order_bytes;
+    return p;
+  }
   // page_kernel's offsets within 16 rows are 32-bit, and its reciprocal holds for up to 64 groups to a block.
   p.pages = g.window == INT32_MAX && g.block_size % 16 == 0 && g.block_size <= 1024 && g.num_blocks > 0 && g.num_kv_heads <= (1 << 18);
   // A short row is one workgroup's, which saves the join's launch.
@@ -2049,7 +2137,8 @@ int attention(const pkv_window& g, const float* key_scales, const float* value_s
   a.splits = splits;
   a.scale_log2 = g.scale * 1.44269504088896340736f;
   a.given_scale = a.scale_log2;
-  if (plan.runs) a.list = reinterpret_cast<int32_t*>(reinterpret_cast<char*>(g.workspace) + need - list_bytes(g.num_queries));
+  if (plan.runs) a.list = reinterpret_cast<int32_t*>(reinterpret_cast<char*>(g.workspace) + need - plan.order_bytes - list_bytes(g.num_queries));
+  if (plan.order_bytes > 0) a.order = reinterpret_cast<int32_t*>(reinterpret_cast<char*>(g.workspace) + need - plan.order_bytes);
   if (plan.pages) a.page_groups = g.block_size / 16;
   if (plan.stream) {
     a.stream_groups = plan.form.groups;
