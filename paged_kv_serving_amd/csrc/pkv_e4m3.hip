@@ -76,13 +76,34 @@ __device__ __forceinline__ int32_t block_of(const Append& a, int64_t slot) {
   return slot < 0 || slot >= a.num_slots ? -1 : static_cast<int32_t>(static_cast<uint32_t>(slot) / static_cast<uint32_t>(a.block_size));
 }
 
+// The codes of a block's first `rows` tokens times `ratio`, a power of two: exact but for codes that fall below 2^-6.
+template <int D>
+__device__ void scale_down(uint8_t* block, int64_t row_bytes, int32_t rows, float ratio) {
+  constexpr int kLanes = D / 8, kRows = kWave / kLanes;
+  const int lane = threadIdx.x & (kWave - 1), row = lane / kLanes, d = lane % kLanes * 8;
+  for (int32_t r = row; r < rows; r += kRows) {
+    u32x2* p = reinterpret_cast<u32x2*>(block + r * row_bytes + d);
+    const u32x2 w = *p;
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      v[4 * i] = __builtin_amdgcn_cvt_f32_fp8(w[i], 0), v[4 * i + 1] = __builtin_amdgcn_cvt_f32_fp8(w[i], 1);
+      v[4 * i + 2] = __builtin_amdgcn_cvt_f32_fp8(w[i], 2), v[4 * i + 3] = __builtin_amdgcn_cvt_f32_fp8(w[i], 3);
+    }
+    *p = codes_of(v, ratio);
+  }
+}
+
+__device__ __forceinline__ float finite_size(float x) {
+  const float size = fabsf(x);
+  return size < INFINITY ? size : 0.f;
+}
+
 // ---------------------------------------------------------------------------------------------
-// A wavefront has the tokens of one block that stand next to each other in the call (a run), of one head, keys or
-// values: D / 8 lanes to a row. Their largest magnitude gives the scale; where the block has tokens before them and
-// its scale has to grow, their codes are multiplied by the ratio of the scales, a power of two, which is exact but
-// for codes that fall below 2^-6. No two wavefronts write the same block and head, so nothing waits for another.
-// Tokens' values are read once and held in registers (kHeld of them; longer runs are read twice, the second time
-// from the caches).
+// The tokens of one block that stand next to each other in the call (a run), of one head, keys or values: D / 8 lanes to a
+// row. Their largest magnitude gives the scale; where the block has tokens before them and its scale has to grow, their
+// codes are scaled down. No two wavefronts write the same block and head, so nothing waits for another. Here a run of more
+// than kHeld tokens, read twice, the second time from the caches.
 // ---------------------------------------------------------------------------------------------
 template <typename T, int D>
 __device__ void append_run(const Append& a, int which, int32_t head, int64_t t0, int32_t block) {
@@ -125,34 +146,18 @@ __device__ void append_run(const Append& a, int which, int32_t head, int64_t t0,
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float size = fabsf(x[i].v[e]);
-        most = fmaxf(most, size < INFINITY ? size : 0.f);
-      }
+      for (int e = 0; e < 8; ++e) most = fmaxf(most, finite_size(x[i].v[e]));
     }
   }
   for (int m = kWave / 2; m > 0; m >>= 1) most = fmaxf(most, __shfl_xor(most, m));
   float scale = scale_for(most);
   if (before > 0) {
     scale = fmaxf(scale, held_scale);
-    if (scale != held_scale) {
-      const float ratio = held_scale / scale;
-      for (int32_t r = row; r < before; r += kRows) {
-        u32x2* p = reinterpret_cast<u32x2*>(pool + (block0 + r) * row_bytes);
-        const u32x2 w = *p;
-        float v[8];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          v[4 * i] = __builtin_amdgcn_cvt_f32_fp8(w[i], 0), v[4 * i + 1] = __builtin_amdgcn_cvt_f32_fp8(w[i], 1);
-          v[4 * i + 2] = __builtin_amdgcn_cvt_f32_fp8(w[i], 2), v[4 * i + 3] = __builtin_amdgcn_cvt_f32_fp8(w[i], 3);
-        }
-        *p = codes_of(v, ratio);
-      }
-    }
+    if (scale != held_scale) scale_down<D>(pool - d + block0 * row_bytes, row_bytes, before, held_scale / scale);
   }
   const float times = 1.f / scale;
   for (int64_t from = t0; from < end; from += kHeld) {
-    if (end - t0 > kHeld) load(from);
+    load(from);
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
       const int64_t t = from + i * kRows + row;
@@ -162,23 +167,111 @@ __device__ void append_run(const Append& a, int which, int32_t head, int64_t t0,
   if (lane == 0) *scale_at = scale;
 }
 
+// Runs within kHeld tokens from t0 on, all at once: lane j < kHeld speaks for token j. `slot` is the lane's (-1: none),
+// `block` its block, `begins` the tokens that are not of the block of the one before, `count` the tokens, which end with a run.
+template <typename T, int D>
+__device__ __forceinline__ void append_runs(const Append& a, int which, int32_t head, int64_t t0, int32_t count, int64_t slot, int32_t block,
+                                            uint32_t begins) {
+  constexpr int kLanes = D / 8, kRows = kWave / kLanes, kSteps = kHeld / kRows;
+  const int lane = threadIdx.x & (kWave - 1), row = lane / kLanes, d = lane % kLanes * 8;
+  const bool aligned = a.aligned[which];
+  const T* source = static_cast<const T*>(a.source[which]) + static_cast<int64_t>(head) * D + d;
+  uint8_t* pool = a.pool[which] + static_cast<int64_t>(head) * D;
+  const int64_t row_bytes = static_cast<int64_t>(a.kv_heads) * D;
+  const bool speaks = lane < count && block >= 0;
+  float* scale_at = a.scales[which] + static_cast<int64_t>(max(block, 0)) * a.kv_heads + head;
+  const float held_scale = speaks ? *scale_at : 0.f;
+
+  Eight x[kSteps];
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) x[i] = load_eight(source + (t0 + min(i * kRows + row, count - 1)) * a.stride[which], aligned);
+  float most = 0.f;  // of this lane's token
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) {
+    float its = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) its = fmaxf(its, finite_size(x[i].v[e]));
+#pragma unroll
+    for (int m = 1; m < kLanes; m *= 2) its = fmaxf(its, __shfl_xor(its, m));
+    const float here = __shfl(its, lane % kRows * kLanes);
+    most = lane / kRows == i ? here : most;
+  }
+  // The run's largest, and its first place in the block.
+  const int32_t place = static_cast<int32_t>(slot - static_cast<int64_t>(block) * a.block_size);
+  int32_t before = place;
+  const uint32_t up_to = (2u << min(lane, kHeld - 1)) - 1;
+  const int begin = 31 - __builtin_clz(begins & up_to), end = begins & ~up_to ? __builtin_ctz(begins & ~up_to) : count;
+  const bool first = speaks && lane == begin;
+#pragma unroll
+  for (int m = 1; m < kHeld; m *= 2) {
+    const float other = __shfl_up(most, m);
+    const int32_t low = __shfl_up(before, m);
+    if (lane - m >= begin) most = fmaxf(most, other), before = min(before, low);
+  }
+  most = __shfl(most, end - 1);
+  before = __shfl(before, end - 1);
+  float scale = scale_for(most);
+  if (before > 0) scale = fmaxf(scale, held_scale);
+  for (uint64_t grown = __ballot(first && before > 0 && scale != held_scale); grown != 0; grown &= grown - 1) {
+    const int j = __builtin_ctzll(grown);
+    const int64_t block0 = static_cast<int64_t>(__builtin_amdgcn_readfirstlane(__shfl(block, j))) * a.block_size;
+    scale_down<D>(pool + block0 * row_bytes, row_bytes, __shfl(before, j), __shfl(held_scale / scale, j));
+  }
+  const float times = 1.f / scale;
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) {
+    const int j = i * kRows + row;
+    const int64_t to = __shfl(static_cast<long long>(speaks ? slot : -1), j);
+    const float by = __shfl(times, j);
+    if (to >= 0) *reinterpret_cast<u32x2*>(pool + to * row_bytes + d) = codes_of(x[i].v, by);
+  }
+  if (first) *scale_at = scale;
+}
+
+// A wavefront has the runs that begin in its window of kHeld tokens, of one head, keys or values. Short ones are taken together, as
+// many as end within kHeld tokens: one after the other, the latency of each (2 us) counted.
+// Bound: HBM for long prompts, latency for single tokens. 16 x 512 tokens of 32 heads x 128, bfloat16, in blocks of 16, 201 MB: 43 us,
+// 4.7 TB/s; 64 single tokens of 8 heads x 128 5 us.
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads) void append_kernel(const Append a) {
-  // Items: keys and values of a head, heads, then windows of tokens, whose runs' first tokens a wavefront looks for.
+  // Items: keys and values of a head, heads, then windows.
   const uint32_t item = __builtin_amdgcn_readfirstlane(blockIdx.x * (kThreads / kWave) + threadIdx.x / kWave);
   const uint32_t columns = 2 * static_cast<uint32_t>(a.kv_heads);
   const int which = item & 1;
   const int32_t head = static_cast<int32_t>(item % columns / 2);
-  const int64_t t0 = static_cast<int64_t>(item / columns) * a.window;
-  if (t0 >= a.tokens) return;
+  const int64_t window = static_cast<int64_t>(item / columns) * a.window, until = min(window + a.window, a.tokens);
+  if (window >= a.tokens) return;
   const int lane = threadIdx.x & (kWave - 1);
-  const int64_t t = t0 + lane;
-  const bool mine = lane < a.window && t < a.tokens;
-  const int32_t block = mine ? block_of(a, a.slots[t]) : -1;
-  const int32_t last = mine && t > 0 ? block_of(a, a.slots[t - 1]) : -1;
-  for (uint64_t starts = __ballot(block >= 0 && block != last); starts != 0; starts &= starts - 1) {
-    const int at = __builtin_ctzll(starts);
-    append_run<T, D>(a, which, head, t0 + at, __builtin_amdgcn_readfirstlane(__shfl(block, at)));
+  for (int64_t t0 = window; t0 < until;) {
+    // Lane j: token t0 + j, its slot and block, and whether it begins a run or ends what stands before it.
+    const int64_t t = t0 + lane;
+    int64_t slot = t < a.tokens ? a.slots[t] : -1;
+    const int64_t last_slot = t > 0 && t <= a.tokens ? a.slots[t - 1] : -1;
+    const int32_t block = block_of(a, slot), last = block_of(a, last_slot);
+    if (block < 0) slot = -1;
+    const uint64_t changes = __ballot(block != last || lane == 0);  // t0 begins a run, or is its window's first token
+    const uint64_t starts = __ballot(block >= 0 && block != last);
+    // The first token in the window that begins a run.
+    const uint64_t inside = until - t0 >= kWave ? ~0ull : (1ull << (until - t0)) - 1;
+    if ((starts & inside) == 0) return;
+    const int first = __builtin_ctzll(starts & inside);
+    if (first > 0) {  // what is before it belongs to another wavefront, or to nobody
+      t0 += first;
+      continue;
+    }
+    // How many tokens from here on end with a run: up to the last change of at most kHeld tokens on (the call's end is one), and
+    // to the first run that the next window's wavefront has.
+    const uint64_t theirs = starts & ~inside;
+    const int most = theirs == 0 ? kHeld : min(kHeld, __builtin_ctzll(theirs));
+    const uint64_t ends = changes & ((2ull << most) - 2);
+    if (ends == 0) {
+      append_run<T, D>(a, which, head, t0, __builtin_amdgcn_readfirstlane(block));
+      t0 += kHeld;  // the next run begins behind
+      continue;
+    }
+    const int count = 63 - __builtin_clzll(ends);
+    append_runs<T, D>(a, which, head, t0, count, slot, block, static_cast<uint32_t>(changes) & ((1u << count) - 1));
+    t0 += count;
   }
 }
 
@@ -230,7 +323,7 @@ extern "C" int pkv_append_e4m3(const pkv_e4m3_append* args, int device, void* st
   a.num_slots = static_cast<int32_t>(g.num_blocks * g.block_size);
   a.block_size = g.block_size;
   a.kv_heads = g.num_kv_heads;
-  a.window = g.num_tokens * g.num_kv_heads <= 8192 ? 1 : 16;
+  a.window = kHeld;
   if (groups_of(a) > 0x7fffffff / kThreads) return PKV_EUNSUPPORTED;
   DeviceGuard guard(device);
   if (!guard.ok()) return PKV_EHIP;
