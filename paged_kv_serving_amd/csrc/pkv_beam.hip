@@ -1,8 +1,10 @@
 // Beam search over a paged cache: the best continuations of a group's beams, and the beams' tables and last blocks moved
 // to the beams that go on.
+#include <float.h>
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "pkv_common.h"
 
@@ -11,12 +13,15 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / kWave;
-constexpr int kCapacity = 1024;  // of a workgroup's list of candidates
+constexpr int kMergeThreads = 512;
+constexpr int kMergeWaves = kMergeThreads / kWave;
+constexpr int kCapacity = 256;  // of a workgroup's list of candidates, PKV_BEAM_MAX_COUNT or more
 constexpr int kMaxLists = 4096;  // of a group: beams times chunks
-constexpr int kStagedKeys = 8192;  // of a group, kept in LDS
 
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef u32x4 u32x4_at4 __attribute__((aligned(4)));  // rows of an odd length start anywhere
+typedef u32x4 u32x4_at2 __attribute__((aligned(2)));
+
 
 // ---------------------------------------------------------------------------------------------
 // Selection. A row is cut into chunks, whose numbers a workgroup holds in registers: the logits are read once.
@@ -34,38 +39,47 @@ __device__ __forceinline__ uint64_t ordered(double x) {
   const uint64_t u = static_cast<uint64_t>(__double_as_longlong(x));
   return u ^ (static_cast<uint64_t>(static_cast<int64_t>(u) >> 63) | (1ull << 63));
 }
+__device__ __forceinline__ double number_of(uint64_t order) {
+  return __longlong_as_double(static_cast<long long>(order >> 63 ? order ^ (1ull << 63) : ~order));
+}
 // A candidate of a row: falling keys are falling logits, and of equal ones rising tokens. No two of a row are alike; 0 is none.
 __device__ __forceinline__ uint64_t key_of(float x, uint32_t token) {
-  return x == -INFINITY ? 0 : static_cast<uint64_t>(ordered(x)) << 32 | static_cast<uint32_t>(~token);
+  return static_cast<uint64_t>(ordered(x + 0.f)) << 32 | static_cast<uint32_t>(~token);  // -0 and 0 are one logit
+}
+__device__ __forceinline__ double logit_of(uint64_t key) { return static_cast<double>(number_of(static_cast<uint32_t>(key >> 32))); }
+
+// The larger of two, NaN where one is.
+__device__ __forceinline__ float maximum(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
+// 2^t in double precision for t <= 0, from 2^-1000 on: 2^k p(t - k), k being the nearest whole number, which adding 1.5 * 2^52
+// leaves in the low bits. p is the interpolation of 2^r at the ten Chebyshev nodes of [-1/2, 1/2], within 2^-45 of it. Additions
+// and products alone: conversions and ldexp run at a fraction of their rate.
+constexpr double kLog2E = 1.4426950408889634;
+__device__ __forceinline__ double exp2_of(double t) {
+  constexpr double kWhole = 6755399441055744.0;
+  t = fmax(t, -1000.0);
+  const double shifted = t + kWhole;
+  const double r = t - (shifted - kWhole);
+  double p = 1.0205905413765595e-07;
+  p = __builtin_fma(p, r, 1.325964524488711e-06);
+  p = __builtin_fma(p, r, 1.5252672924850737e-05);
+  p = __builtin_fma(p, r, 0.0001540343375125101);
+  p = __builtin_fma(p, r, 0.0013333558200794592);
+  p = __builtin_fma(p, r, 0.009618129193934313);
+  p = __builtin_fma(p, r, 0.05550410866465167);
+  p = __builtin_fma(p, r, 0.2402265069564034);
+  p = __builtin_fma(p, r, 0.6931471805599462);
+  p = __builtin_fma(p, r, 1.0000000000000135);
+  const uint64_t bits = static_cast<uint64_t>(__double_as_longlong(p));
+  const uint32_t high = static_cast<uint32_t>(bits >> 32) + (static_cast<uint32_t>(__double_as_longlong(shifted)) << 20);
+  return __longlong_as_double(static_cast<long long>(static_cast<uint64_t>(high) << 32 | static_cast<uint32_t>(bits)));
 }
 
-// e^x for x <= 0 in double precision: 2^k e^r with |r| <= ln 2 / 2 and e^r's series up to r^10 / 10!, which leaves out 2^-42.
-__device__ __forceinline__ double exp_of(double x) {
-  x = x < -1000.0 ? -1000.0 : x;  // 0 from there on; a NaN stays one
-  const double k = __builtin_rint(x * 1.4426950408889634);
-  const double r = __builtin_fma(k, -0.6931471805599453, x);
-  double p = 1.0 / 3628800.0;
-  p = __builtin_fma(p, r, 1.0 / 362880.0);
-  p = __builtin_fma(p, r, 1.0 / 40320.0);
-  p = __builtin_fma(p, r, 1.0 / 5040.0);
-  p = __builtin_fma(p, r, 1.0 / 720.0);
-  p = __builtin_fma(p, r, 1.0 / 120.0);
-  p = __builtin_fma(p, r, 1.0 / 24.0);
-  p = __builtin_fma(p, r, 1.0 / 6.0);
-  p = __builtin_fma(p, r, 0.5);
-  p = __builtin_fma(p, r, 1.0);
-  p = __builtin_fma(p, r, 1.0);
-  return ldexp(p, static_cast<int>(fmax(k, -2000.0)));
-}
-
-// The largest / smallest over aligned groups of lanes, `size` of them (a power of two), in each lane.
-__device__ __forceinline__ uint64_t group_max(uint64_t x, int size) {
-  for (int m = 1; m < size; m *= 2) x = max(x, static_cast<uint64_t>(__shfl_xor(static_cast<unsigned long long>(x), m)));
-  return x;
-}
-__device__ __forceinline__ uint64_t group_min(uint64_t x, int from, int size) {
-  for (int m = from; m < size; m *= 2) x = min(x, static_cast<uint64_t>(__shfl_xor(static_cast<unsigned long long>(x), m)));
-  return x;
+// Lanes of the groups that a workgroup of `threads` makes of its wavefronts' lanes: `count` groups or more, none across wavefronts.
+__device__ __forceinline__ int group_lanes(int threads, int count) {
+  int size = kWave;
+  while (threads / size < count) size /= 2;
+  return size;
 }
 
 struct Select {
@@ -81,17 +95,17 @@ __device__ __forceinline__ bool looked_at(const pkv_beam& g, int64_t row) {
   return fabsf(g.scores[row]) < INFINITY && !(g.finished && g.finished[row]);
 }
 
-// A chunk of a row: its largest logit, the sum of exponentials, its `count` best in order. A thread's largest keys give a
-// number that at least `count` keys reach: the lanes of a wavefront make `count` groups or more, and the smallest of the
-// groups' largest keys is one. The keys that reach it, a few times `count`, are listed, and each one's place is the number of
-// larger ones.
+// A chunk of a row: its largest logit, the sum of exponentials, its `count` best in order. The threads make `count` groups or
+// more, so the smallest of the groups' largest logits is a number that at least `count` logits reach, and few more: 8192 of them
+// and 8 groups list about 20. Each one's place is the number of larger ones. Where too many reach it (128 groups: about 700; equal
+// logits), bisection finds a number that fewer do.
 template <typename T, int kPer>
 __global__ __launch_bounds__(kThreads) void chunk_kernel(const Select a) {
   constexpr int kVec = 16 / sizeof(T), kLoads = kPer / kVec;
-  __shared__ uint64_t s_list[kCapacity], s_reach[kWaves];
-  __shared__ float s_top[kWaves];
+  __shared__ uint64_t s_list[kCapacity];
+  __shared__ float s_top[kWaves], s_reach[kWaves];
   __shared__ double s_sum[kWaves];
-  __shared__ int32_t s_count;
+  __shared__ int32_t s_count, s_part[kWaves];
   const pkv_beam& g = a.g;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
   const int64_t row = blockIdx.x / static_cast<uint32_t>(a.chunks);
@@ -100,21 +114,18 @@ __global__ __launch_bounds__(kThreads) void chunk_kernel(const Select a) {
   const uint32_t vocab = static_cast<uint32_t>(g.vocab_size);
   const uint32_t first = chunk * (kThreads * kPer) + tid * kVec;  // this thread's: kVec numbers every kThreads * kVec
   const T* p = static_cast<const T*>(g.logits) + row * g.row_stride;
-  const bool aligned = (reinterpret_cast<uintptr_t>(p) & 15u) == 0;
+  using Vec = std::conditional_t<sizeof(T) == 4, u32x4_at4, u32x4_at2>;
 
   float x[kPer];
 #pragma unroll
   for (int i = 0; i < kLoads; ++i) {
     const uint32_t at = first + i * (kThreads * kVec);
-    if (aligned && at + kVec <= vocab) {
-      if constexpr (sizeof(T) == 4) {
-        const f32x4 v = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(p + at));
+    if ((chunk + 1) * (kThreads * kPer) <= vocab || at + kVec <= vocab) {
+      const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const Vec*>(p + at));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[i * kVec + e] = v[e];
-      } else {
-        const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p + at));
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[i * kVec + 2 * e] = bf16_lo(v[e]), x[i * kVec + 2 * e + 1] = bf16_hi(v[e]);
+      for (int e = 0; e < 4; ++e) {
+        if constexpr (sizeof(T) == 4) x[i * kVec + e] = __uint_as_float(v[e]);
+        else x[i * kVec + 2 * e] = bf16_lo(v[e]), x[i * kVec + 2 * e + 1] = bf16_hi(v[e]);
       }
     } else {
 #pragma unroll
@@ -129,189 +140,305 @@ __global__ __launch_bounds__(kThreads) void chunk_kernel(const Select a) {
   }
   const auto token = [&](int i) { return first + i / kVec * (kThreads * kVec) + i % kVec; };
 
-  // This thread's largest, of its even and its odd places apart: the lowest token of equal ones.
-  float best[2] = {-INFINITY, -INFINITY};
-  int at[2] = {0, 0};
+  float top = x[0];
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    x[i] += 0.f;  // -0 and 0 are one logit
-    const int side = i % 2;
-    if (x[i] > best[side]) best[side] = x[i], at[side] = i;
+  for (int i = 1; i < kPer; ++i) top = maximum(top, x[i]);
+  const int size = group_lanes(kThreads, g.count);
+  for (int m = 1; m < size; m *= 2) top = maximum(top, __shfl_xor(top, m));
+  float reach = top;
+  for (int m = size; m < kWave; m *= 2) {
+    top = maximum(top, __shfl_xor(top, m));
+    reach = fminf(reach, __shfl_xor(reach, m));
   }
-  uint64_t half[2];
-#pragma unroll
-  for (int s = 0; s < 2; ++s) half[s] = key_of(best[s], token(at[s]));
-  uint64_t reach;
-  if (g.count > kWave) {
-    reach = group_min(min(half[0], half[1]), 1, kWave);
-  } else {
-    int size = kWave;  // lanes of a group
-    while (kWave / size < g.count) size /= 2;
-    reach = group_min(group_max(max(half[0], half[1]), size), size, kWave);
-  }
-  float top = fmaxf(best[0], best[1]);
-  for (int m = kWave / 2; m > 0; m >>= 1) top = fmaxf(top, __shfl_xor(top, m));
   if (lane == 0) s_top[wave] = top, s_reach[wave] = reach;
   if (tid == 0) s_count = 0;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) top = fmaxf(top, s_top[w]), reach = max(reach, s_reach[w]);
+  for (int w = 0; w < kWaves; ++w) top = maximum(top, s_top[w]), reach = fminf(reach, s_reach[w]);
+  reach = fmaxf(reach, -FLT_MAX);  // -inf is no candidate
+  const int64_t index = row * a.chunks + chunk;
+  uint64_t* out = a.keys + index * g.count;
+  if (!(fabsf(top) < INFINITY)) {  // nothing, or a row without continuations
+    if (tid == 0) a.sums[index] = 0.0, a.tops[index] = top;
+    for (int32_t i = tid; i < g.count; i += kThreads) out[i] = 0;
+    return;
+  }
 
-  // A NaN or +inf makes the sum NaN.
   double sum = 0.0;
-  const double from = top == -INFINITY ? 0.0 : static_cast<double>(top);
+  const double from = -kLog2E * static_cast<double>(top);
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) sum += exp_of(static_cast<double>(x[i]) - from);
+  for (int i = 0; i < kPer; ++i) sum += exp2_of(__builtin_fma(kLog2E, static_cast<double>(x[i]), from));
   for (int m = kWave / 2; m > 0; m >>= 1) sum += __shfl_xor(sum, m);
   if (lane == 0) s_sum[wave] = sum;
 
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    const uint64_t key = key_of(x[i], token(i));
-    if (key != 0 && key >= reach) {
+    if (x[i] >= reach) {
       const int32_t place = atomicAdd(&s_count, 1);
-      if (place < kCapacity) s_list[place] = key;
+      if (place < kCapacity) s_list[place] = key_of(x[i], token(i));
     }
   }
   __syncthreads();
-  const int64_t index = row * a.chunks + chunk;
-  uint64_t* out = a.keys + index * g.count;
   if (tid == 0) {
     sum = 0.0;
     for (int w = 0; w < kWaves; ++w) sum += s_sum[w];
     a.sums[index] = sum;
     a.tops[index] = top;
   }
-  const int32_t found = s_count;
-  if (found <= kCapacity) {
-    for (int32_t i = tid; i < found; i += kThreads) {
-      const uint64_t mine = s_list[i];
-      int32_t place = 0;
-      for (int32_t j = 0; j < found; ++j) place += s_list[j] > mine ? 1 : 0;
-      if (place < g.count) out[place] = mine;
+  int32_t found = s_count;
+  if (found > kCapacity) {
+    // How many of the chunk's numbers a condition holds for.
+    const auto number = [&](auto holds) {
+      int32_t n = 0;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) n += __popcll(__ballot(holds(i)));
+      __syncthreads();
+      if (lane == 0) s_part[wave] = n;
+      __syncthreads();
+      n = 0;
+      for (int w = 0; w < kWaves; ++w) n += s_part[w];
+      return n;
+    };
+    // More than the capacity reach `low`, fewer than `count` reach `high`.
+    uint32_t low = ordered(reach), high = ordered(top) + 1;
+    bool fits = false;
+    while (high - low > 1) {
+      const uint32_t middle = low + (high - low) / 2;
+      const float at = number_of(middle);
+      const int32_t n = number([&](int i) { return x[i] >= at; });
+      fits = n >= g.count && n <= kCapacity;
+      if (fits || n > kCapacity) low = middle;
+      else high = middle;
+      if (fits) break;
     }
-    for (int32_t i = found + tid; i < g.count; i += kThreads) out[i] = 0;
-    return;
-  }
-  // Too many reach it (rows of which most logits are -inf in certain places): one after the other.
-  uint64_t last = ~0ull;
-  for (int32_t n = 0; n < g.count; ++n) {
-    uint64_t most = 0;
+    reach = number_of(low);
+    // All that reach it, or all above it and of the equal ones the first tokens.
+    uint32_t last = ~0u;
+    if (!fits) {
+      const int32_t rest = g.count - number([&](int i) { return x[i] > reach; });
+      uint32_t under = chunk * (kThreads * kPer);  // `last` is enough, `under - 1` is not
+      last = under + kThreads * kPer - 1;
+      while (under < last) {
+        const uint32_t middle = under + (last - under) / 2;
+        if (number([&](int i) { return x[i] == reach && token(i) <= middle; }) >= rest) last = middle;
+        else under = middle + 1;
+      }
+    }
+    __syncthreads();
+    if (tid == 0) s_count = 0;
+    __syncthreads();
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const uint64_t key = key_of(x[i], token(i));
-      if (key < last) most = max(most, key);
+      if (x[i] > reach || (x[i] == reach && token(i) <= last)) {
+        const int32_t place = atomicAdd(&s_count, 1);
+        if (place < kCapacity) s_list[place] = key_of(x[i], token(i));
+      }
     }
-    most = group_max(most, kWave);
     __syncthreads();
-    if (lane == 0) s_reach[wave] = most;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) most = max(most, s_reach[w]);
-    if (tid == 0) out[n] = most;
-    last = most;
+    found = min(s_count, kCapacity);
   }
+  for (int32_t i = tid; i < found; i += kThreads) {
+    const uint64_t mine = s_list[i];
+    int32_t place = 0;
+#pragma unroll 8
+    for (int32_t j = 0; j < found; ++j) place += s_list[j] > mine ? 1 : 0;
+    if (place < g.count) out[place] = mine;
+  }
+  for (int32_t i = found + tid; i < g.count; i += kThreads) out[i] = 0;
 }
 
-// A group's chunks: the logarithms of its rows' sums, then one wavefront takes the best of the lists' first candidates `count`
-// times. Lists are a row's chunks, each with falling keys.
-__global__ __launch_bounds__(kThreads) void merge_kernel(const Select a) {
-  extern __shared__ __align__(16) uint64_t s_keys[];  // the lists, where they fit
+// A group: the logarithms of its rows' sums, then the chunks' candidates by score, in the same way. The candidates are numbered
+// through the lists' first ones, then their second ones and so on, and dealt out to the groups of lanes one by one, so that every
+// group has some of the best.
+__global__ __launch_bounds__(kMergeThreads) void merge_kernel(const Select a) {
+  constexpr int kHeld = 4;  // candidates of a thread in registers; what is left of them is read again
   __shared__ double s_norm[PKV_BEAM_MAX], s_score[PKV_BEAM_MAX];
   __shared__ uint8_t s_kind[PKV_BEAM_MAX];  // 0: no continuation, 1: its row's, 2: the end token
-  __shared__ uint8_t s_at[kMaxLists];
+  __shared__ double s_scores[kCapacity];
+  __shared__ uint64_t s_keys[kCapacity];
+  __shared__ uint8_t s_beams[kCapacity];
+  __shared__ int32_t s_places[kCapacity];
+  __shared__ double s_top[kMergeWaves], s_reach[kMergeWaves];
+  __shared__ int32_t s_count, s_part[kMergeWaves];
   const pkv_beam& g = a.g;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
   const int64_t group = blockIdx.x, row0 = group * g.num_beams;
-  const int32_t lists = g.num_beams * a.chunks;
-  const bool staged = static_cast<int64_t>(lists) * g.count <= kStagedKeys;
+  const uint32_t lists = static_cast<uint32_t>(g.num_beams) * a.chunks, total = lists * g.count;
   const uint64_t* keys = a.keys + row0 * a.chunks * g.count;
-  for (int32_t l = tid; l < lists; l += kThreads) s_at[l] = 0;
-  if (staged) {
-    for (int32_t i = tid; i < lists * g.count; i += kThreads) {
-      if (looked_at(g, row0 + i / (a.chunks * g.count))) s_keys[i] = keys[i];
-    }
+  const auto key_at = [&](uint32_t i) { return keys[static_cast<int64_t>(i % lists) * g.count + i / lists]; };
+
+  const int size = group_lanes(kMergeThreads, g.count);
+  const uint32_t groups = kMergeThreads / size, mine = tid / size + groups * (tid % size);  // and every kMergeThreads further on
+
+  uint64_t held[kHeld];  // what a row that is not looked at has here is not used
+#pragma unroll
+  for (int j = 0; j < kHeld; ++j) {
+    const uint32_t i = mine + j * kMergeThreads;
+    held[j] = i < total ? key_at(i) : 0;
   }
-  for (int32_t b = wave; b < g.num_beams; b += kWaves) {
+  for (int32_t b = wave; b < g.num_beams; b += kMergeWaves) {
     const int64_t row = row0 + b;
-    const bool look = looked_at(g, row);
+    const float* tops = a.tops + row * a.chunks;
+    const double* sums = a.sums + row * a.chunks;
+    const float score = g.scores[row];
+    const bool finished = g.finished && g.finished[row];
+    const float top0 = lane < a.chunks ? tops[lane] : -INFINITY;
+    const double sum0 = lane < a.chunks ? sums[lane] : 0.0;
+    float top = top0;
+    for (int32_t c = lane + kWave; c < a.chunks; c += kWave) top = maximum(top, tops[c]);
+    for (int m = kWave / 2; m > 0; m >>= 1) top = maximum(top, __shfl_xor(top, m));
     double sum = 0.0;
-    float top = -INFINITY;
-    if (look) {
-      for (int32_t c = lane; c < a.chunks; c += kWave) top = fmaxf(top, a.tops[row * a.chunks + c]);
-      for (int m = kWave / 2; m > 0; m >>= 1) top = fmaxf(top, __shfl_xor(top, m));
-      for (int32_t c = lane; c < a.chunks; c += kWave) {
-        const float one = a.tops[row * a.chunks + c];
-        const double part = a.sums[row * a.chunks + c];
-        if (part != 0.0) sum += part * exp_of(static_cast<double>(one) - static_cast<double>(top));
-      }
-      for (int m = kWave / 2; m > 0; m >>= 1) sum += __shfl_xor(sum, m);
-    }
+    const auto add = [&](float one, double part) {
+      if (part != 0.0) sum += part * exp2_of(kLog2E * (static_cast<double>(one) - static_cast<double>(top)));
+    };
+    add(top0, sum0);
+    for (int32_t c = lane + kWave; c < a.chunks; c += kWave) add(tops[c], sums[c]);
+    for (int m = kWave / 2; m > 0; m >>= 1) sum += __shfl_xor(sum, m);
     if (lane == 0) {
-      const bool counts = look && sum > 0.0 && sum < INFINITY && fabsf(top) < INFINITY;
-      const float score = g.scores[row];
+      const bool usable = fabsf(score) < INFINITY, counts = usable && !finished && fabsf(top) < INFINITY;
       s_norm[b] = counts ? static_cast<double>(top) + log(sum) : 0.0;
       s_score[b] = score;
-      s_kind[b] = counts ? 1 : (fabsf(score) < INFINITY && g.finished && g.finished[row]) ? 2 : 0;
+      s_kind[b] = counts ? 1 : usable && finished ? 2 : 0;
     }
   }
+  if (tid == 0) s_count = 0;
+  for (int32_t i = tid; i < kCapacity; i += kMergeThreads) s_places[i] = 0;
   __syncthreads();
-  if (wave != 0) return;
 
-  // The first candidate of list l that is left: its key (0: none) and its score.
-  const auto head = [&](int32_t l, uint64_t& key, uint64_t& score) {
-    const int32_t b = l / a.chunks, at = s_at[l], kind = s_kind[b];
-    key = 0;
-    score = 0;
-    if (kind == 2 && l == b * a.chunks && at == 0) {
-      key = 1;
-      score = ordered(s_score[b]);
-    } else if (kind == 1 && at < g.count) {
-      key = staged ? s_keys[l * g.count + at] : keys[static_cast<int64_t>(l) * g.count + at];
-      if (key != 0) score = ordered(s_score[b] + (static_cast<double>(number_of(static_cast<uint32_t>(key >> 32))) - s_norm[b]));
+  const auto beam_of = [&](uint32_t i) { return i % lists / a.chunks; };
+  // The score of candidate i, -inf if it is none; of a beam that has ended, its first one is the end token.
+  const auto score_of = [&](uint32_t i, uint64_t key) {
+    const uint32_t b = beam_of(i);
+    const int32_t kind = s_kind[b];
+    if (kind == 2) return i == b * a.chunks ? s_score[b] : -INFINITY;
+    return kind == 1 && key != 0 ? s_score[b] + (logit_of(key) - s_norm[b]) : -INFINITY;
+  };
+  double scores[kHeld];
+#pragma unroll
+  for (int j = 0; j < kHeld; ++j) {
+    const uint32_t i = mine + j * kMergeThreads;
+    scores[j] = i < total ? score_of(i, held[j]) : -INFINITY;
+  }
+  // f(candidate, key, score) for all of this thread's.
+  const auto each = [&](auto f) {
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) {
+      if (scores[j] > -INFINITY) f(mine + j * kMergeThreads, held[j], scores[j]);
+    }
+    for (uint32_t i = mine + kHeld * kMergeThreads; i < total; i += kMergeThreads) {
+      const uint64_t key = key_at(i);
+      const double score = score_of(i, key);
+      if (score > -INFINITY) f(i, key, score);
     }
   };
-  // The best of this lane's lists. Of equal scores the lower beam's, and in a beam the larger key.
-  int32_t mine = -1;
-  uint64_t key = 0, score = 0;
-  const auto look = [&]() {
-    mine = -1;
-    key = score = 0;
-    for (int32_t l = lane; l < lists; l += kWave) {
-      uint64_t k, s;
-      head(l, k, s);
-      if (k == 0) continue;
-      const bool same = s == score && mine >= 0;
-      if (mine < 0 || s > score || (same && l / a.chunks == mine / a.chunks && k > key)) mine = l, key = k, score = s;
-    }
+
+  double top = -INFINITY;
+  each([&](uint32_t, uint64_t, double score) { top = fmax(top, score); });
+  for (int m = 1; m < size; m *= 2) top = fmax(top, __shfl_xor(top, m));
+  double reach = top;
+  for (int m = size; m < kWave; m *= 2) {
+    top = fmax(top, __shfl_xor(top, m));
+    reach = fmin(reach, __shfl_xor(reach, m));
+  }
+  if (lane == 0) s_top[wave] = top, s_reach[wave] = reach;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kMergeWaves; ++w) top = fmax(top, s_top[w]), reach = fmin(reach, s_reach[w]);
+
+  const auto list = [&](uint32_t i, uint64_t key, double score) {
+    const int32_t place = atomicAdd(&s_count, 1);
+    if (place < kCapacity) s_scores[place] = score, s_keys[place] = key, s_beams[place] = static_cast<uint8_t>(beam_of(i));
   };
-  look();
-  for (int32_t n = 0; n < g.count; ++n) {
-    const int64_t out = group * g.count + n;
-    const uint64_t most = group_max(score, kWave);
-    uint64_t winners = __ballot(mine >= 0 && score == most);
-    if (winners == 0) {  // nothing is left
-      if (lane == 0) g.best_scores[out] = -INFINITY, g.best_beams[out] = 0, g.best_tokens[out] = g.end_token;
-      continue;
+  each([&](uint32_t i, uint64_t key, double score) {
+    if (score >= reach) list(i, key, score);
+  });
+  __syncthreads();
+  int32_t found = s_count;
+  if (found > kCapacity) {
+    const auto number = [&](auto holds) {
+      int32_t n = 0;
+      each([&](uint32_t i, uint64_t key, double score) { n += holds(i, key, score) ? 1 : 0; });
+      for (int m = kWave / 2; m > 0; m >>= 1) n += __shfl_xor(n, m);
+      __syncthreads();
+      if (lane == 0) s_part[wave] = n;
+      __syncthreads();
+      n = 0;
+      for (int w = 0; w < kMergeWaves; ++w) n += s_part[w];
+      return n;
+    };
+    // More than the capacity reach `low`, fewer than `count` reach `high`.
+    uint64_t low = ordered(reach), high = ordered(top) + 1;
+    bool fits = false;
+    while (high - low > 1) {
+      const uint64_t middle = low + (high - low) / 2;
+      const double at = number_of(middle);
+      const int32_t n = number([&](uint32_t, uint64_t, double score) { return score >= at; });
+      fits = n >= g.count && n <= kCapacity;
+      if (fits || n > kCapacity) low = middle;
+      else high = middle;
+      if (fits) break;
     }
-    if (winners & (winners - 1)) {  // equal scores
-      const uint64_t inside = (winners >> lane) & 1 ? ~0ull : 0;
-      // The lower beam, whose lists lower numbers have; then the larger key.
-      const uint64_t beam = group_max(inside & static_cast<uint64_t>(PKV_BEAM_MAX - mine / a.chunks), kWave);
-      const bool there = inside && static_cast<uint64_t>(PKV_BEAM_MAX - mine / a.chunks) == beam;
-      const uint64_t largest = group_max(there ? key : 0, kWave);
-      winners = __ballot(there && key == largest);
+    reach = number_of(low);
+    // All that reach it, or all above it and of the equal ones the first beams', of the last of those the largest keys.
+    uint32_t last = PKV_BEAM_MAX;
+    uint64_t least = 0;
+    if (!fits) {
+      const int32_t rest = g.count - number([&](uint32_t, uint64_t, double score) { return score > reach; });
+      uint32_t under = 0;
+      last = g.num_beams - 1;
+      while (under < last) {
+        const uint32_t middle = under + (last - under) / 2;
+        if (number([&](uint32_t i, uint64_t, double score) { return score == reach && beam_of(i) <= middle; }) >= rest) last = middle;
+        else under = middle + 1;
+      }
+      const int32_t own = rest - number([&](uint32_t i, uint64_t, double score) { return score == reach && beam_of(i) < last; });
+      uint64_t over = ~0ull;  // `least` is low enough, `over + 1` is not
+      while (least < over) {
+        const uint64_t middle = over - (over - least) / 2;
+        const auto holds = [&](uint32_t i, uint64_t key, double score) { return score == reach && beam_of(i) == last && key >= middle; };
+        if (number(holds) >= own) least = middle;
+        else over = middle - 1;
+      }
     }
-    if (lane == __builtin_ctzll(winners)) {
-      const int32_t b = mine / a.chunks;
-      const bool ended = s_kind[b] == 2;
-      const double at = ended ? s_score[b] : s_score[b] + (static_cast<double>(number_of(static_cast<uint32_t>(key >> 32))) - s_norm[b]);
-      g.best_scores[out] = static_cast<float>(at);
-      g.best_beams[out] = b;
-      g.best_tokens[out] = ended ? g.end_token : static_cast<int32_t>(~static_cast<uint32_t>(key));
-      s_at[mine] += 1;
-      look();
+    __syncthreads();
+    if (tid == 0) s_count = 0;
+    __syncthreads();
+    each([&](uint32_t i, uint64_t key, double score) {
+      const uint32_t b = beam_of(i);
+      if (score > reach || (score == reach && (b < last || (b == last && key >= least)))) list(i, key, score);
+    });
+    __syncthreads();
+    found = min(s_count, kCapacity);
+  }
+  // Places. Of equal scores the lower beam's is first, in a beam the larger key. Threads that are left over share a candidate.
+  const int32_t parts = found > 0 ? max(kMergeThreads / found, 1) : 1;
+  for (int32_t w = tid; w < found * parts; w += kMergeThreads) {
+    const int32_t c = w % found, part = w / found;
+    const double score = s_scores[c];
+    const uint64_t key = s_keys[c];
+    const int32_t b = s_beams[c];
+    int32_t place = 0;
+#pragma unroll 4
+    for (int32_t j = found * part / parts; j < found * (part + 1) / parts; ++j) {
+      const double other = s_scores[j];
+      const int32_t beam = s_beams[j];
+      place += other > score || (other == score && (beam < b || (beam == b && s_keys[j] > key))) ? 1 : 0;
     }
+    if (place > 0) atomicAdd(&s_places[c], place);
+  }
+  __syncthreads();
+  const int64_t out = group * g.count;
+  for (int32_t i = tid; i < found; i += kMergeThreads) {
+    const int32_t place = s_places[i], b = s_beams[i];
+    if (place >= g.count) continue;
+    g.best_scores[out + place] = static_cast<float>(s_scores[i]);
+    g.best_beams[out + place] = b;
+    g.best_tokens[out + place] = s_kind[b] == 2 ? g.end_token : static_cast<int32_t>(~static_cast<uint32_t>(s_keys[i]));
+  }
+  for (int32_t i = found + tid; i < g.count; i += kMergeThreads) {
+    g.best_scores[out + i] = -INFINITY;
+    g.best_beams[out + i] = 0;
+    g.best_tokens[out + i] = g.end_token;
   }
 }
 
@@ -407,9 +534,7 @@ int select(Select a, int per, hipStream_t stream) {
   } else {
     hipLaunchKernelGGL((chunk_kernel<T, 32>), chunks, block, 0, stream, a);
   }
-  const int64_t keys = static_cast<int64_t>(a.g.num_beams) * a.chunks * a.g.count;
-  const uint32_t lds = keys <= kStagedKeys ? static_cast<uint32_t>(keys * sizeof(uint64_t)) : 0;
-  hipLaunchKernelGGL(merge_kernel, dim3(static_cast<uint32_t>(a.g.num_groups)), block, lds, stream, a);
+  hipLaunchKernelGGL(merge_kernel, dim3(static_cast<uint32_t>(a.g.num_groups)), dim3(kMergeThreads), 0, stream, a);
   return check_launch();
 }
 
