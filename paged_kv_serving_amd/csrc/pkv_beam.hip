@@ -18,6 +18,7 @@ constexpr int kMergeWaves = kMergeThreads / kWave;
 constexpr int kCapacity = 256;  // of a workgroup's list of candidates, PKV_BEAM_MAX_COUNT or more
 constexpr int kMaxLists = 4096;  // of a group: beams times chunks
 
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef u32x4 u32x4_at4 __attribute__((aligned(4)));  // rows of an odd length start anywhere
 typedef u32x4 u32x4_at2 __attribute__((aligned(2)));
@@ -51,7 +52,7 @@ __device__ __forceinline__ double logit_of(uint64_t key) { return static_cast<do
 // The larger of two, NaN where one is.
 __device__ __forceinline__ float maximum(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
-// 2^t in double precision for t <= 0, from 2^-1000 on: 2^k p(t - k), k being the nearest whole number, which adding 1.5 * 2^52
+// 2^t in double precision for t <= 1000, from 2^-1000 on: 2^k p(t - k), k being the nearest whole number, which adding 1.5 * 2^52
 // leaves in the low bits. p is the interpolation of 2^r at the ten Chebyshev nodes of [-1/2, 1/2], within 2^-45 of it. Additions
 // and products alone: conversions and ldexp run at a fraction of their rate.
 constexpr double kLog2E = 1.4426950408889634;
@@ -70,9 +71,9 @@ __device__ __forceinline__ double exp2_of(double t) {
   p = __builtin_fma(p, r, 0.2402265069564034);
   p = __builtin_fma(p, r, 0.6931471805599462);
   p = __builtin_fma(p, r, 1.0000000000000135);
-  const uint64_t bits = static_cast<uint64_t>(__double_as_longlong(p));
-  const uint32_t high = static_cast<uint32_t>(bits >> 32) + (static_cast<uint32_t>(__double_as_longlong(shifted)) << 20);
-  return __longlong_as_double(static_cast<long long>(static_cast<uint64_t>(high) << 32 | static_cast<uint32_t>(bits)));
+  u32x2 bits = __builtin_bit_cast(u32x2, p);
+  bits[1] += __builtin_bit_cast(u32x2, shifted)[0] << 20;
+  return __builtin_bit_cast(double, bits);
 }
 
 // Lanes of the groups that a workgroup of `threads` makes of its wavefronts' lanes: `count` groups or more, none across wavefronts.
@@ -80,6 +81,13 @@ __device__ __forceinline__ int group_lanes(int threads, int count) {
   int size = kWave;
   while (threads / size < count) size /= 2;
   return size;
+}
+
+// Adjacent lanes, as many as there are for each of `found` candidates, that count the larger ones together.
+__device__ __forceinline__ int shares_of(int threads, int found) {
+  int shares = 1;
+  while (shares < kWave && 2 * shares * found <= threads) shares *= 2;
+  return shares;
 }
 
 struct Select {
@@ -95,17 +103,21 @@ __device__ __forceinline__ bool looked_at(const pkv_beam& g, int64_t row) {
   return fabsf(g.scores[row]) < INFINITY && !(g.finished && g.finished[row]);
 }
 
-// A chunk of a row: its largest logit, the sum of exponentials, its `count` best in order. The threads make `count` groups or
-// more, so the smallest of the groups' largest logits is a number that at least `count` logits reach, and few more: 8192 of them
-// and 8 groups list about 20. Each one's place is the number of larger ones. Where too many reach it (128 groups: about 700; equal
-// logits), bisection finds a number that fewer do.
+// A chunk of a row: its largest logit, the sum of exponentials, its `count` best in order. The lanes of all wavefronts that are
+// alike modulo a power of two make `count` classes or more, so the smallest of the classes' largest logits is a number that at
+// least `count` logits reach, and few more: 8192 of them and 8 classes list about 23. Classes of lanes rather than neighbours:
+// a row's last chunk, which has numbers for the first threads alone, leaves no class empty. Each one's place is the number of
+// larger ones. Where too many reach it (128 classes: about 700; equal logits), bisection finds a number that fewer do.
+// 32 groups of 8 beams over 128256 float32 logits: about 35 us for 115 MB. Bound by the vector units at 22 us of it, the
+// exponentials' 17 operations being two thirds of them, which the reads of 18 us overlap with in part; the kernel takes 21 us
+// without them. Half the bytes (bf16) take the same time.
 template <typename T, int kPer>
 __global__ __launch_bounds__(kThreads) void chunk_kernel(const Select a) {
   constexpr int kVec = 16 / sizeof(T), kLoads = kPer / kVec;
-  __shared__ uint64_t s_list[kCapacity];
-  __shared__ float s_top[kWaves], s_reach[kWaves];
+  __shared__ uint64_t s_list[kWaves][kCapacity];  // a wavefront's own, so that no place needs an atomic
+  __shared__ float s_top[kWaves][kWave];
   __shared__ double s_sum[kWaves];
-  __shared__ int32_t s_count, s_part[kWaves];
+  __shared__ int32_t s_part[kWaves];
   const pkv_beam& g = a.g;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
   const int64_t row = blockIdx.x / static_cast<uint32_t>(a.chunks);
@@ -116,45 +128,65 @@ __global__ __launch_bounds__(kThreads) void chunk_kernel(const Select a) {
   const T* p = static_cast<const T*>(g.logits) + row * g.row_stride;
   using Vec = std::conditional_t<sizeof(T) == 4, u32x4_at4, u32x4_at2>;
 
-  float x[kPer];
-#pragma unroll
-  for (int i = 0; i < kLoads; ++i) {
-    const uint32_t at = first + i * (kThreads * kVec);
-    if ((chunk + 1) * (kThreads * kPer) <= vocab || at + kVec <= vocab) {
-      const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const Vec*>(p + at));
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if constexpr (sizeof(T) == 4) x[i * kVec + e] = __uint_as_float(v[e]);
-        else x[i * kVec + 2 * e] = bf16_lo(v[e]), x[i * kVec + 2 * e + 1] = bf16_hi(v[e]);
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < kVec; ++e) {
-        x[i * kVec + e] = -INFINITY;
-        if (at + e < vocab) {
-          if constexpr (sizeof(T) == 4) x[i * kVec + e] = p[at + e];
-          else x[i * kVec + e] = __uint_as_float(static_cast<uint32_t>(p[at + e]) << 16);
-        }
-      }
-    }
-  }
   const auto token = [&](int i) { return first + i / kVec * (kThreads * kVec) + i % kVec; };
 
-  float top = x[0];
+  // The exponentials are taken as the numbers arrive, against the largest of the thread's first ones: double precision holds those
+  // of numbers 600 above and below it, and where a thread has others it starts again, against its largest.
+  float x[kPer], top, base;
+  double sum = 0.0;
+  const auto add = [&](int i, double from) { sum += exp2_of(__builtin_fma(kLog2E, static_cast<double>(x[i]), from)); };
+  const auto take = [&](auto whole) {
+    u32x4 v[kLoads];
+    if constexpr (whole) {
 #pragma unroll
-  for (int i = 1; i < kPer; ++i) top = maximum(top, x[i]);
-  const int size = group_lanes(kThreads, g.count);
-  for (int m = 1; m < size; m *= 2) top = maximum(top, __shfl_xor(top, m));
-  float reach = top;
-  for (int m = size; m < kWave; m *= 2) {
+      for (int i = 0; i < kLoads; ++i) v[i] = __builtin_nontemporal_load(reinterpret_cast<const Vec*>(p + token(i * kVec)));
+    }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      if constexpr (!whole) {
+        const T one = p[min(token(i), vocab - 1)];
+        if constexpr (sizeof(T) == 4) x[i] = one;
+        else x[i] = __uint_as_float(static_cast<uint32_t>(one) << 16);
+        if (token(i) >= vocab) x[i] = -INFINITY;
+      } else {
+        if constexpr (sizeof(T) == 4) x[i] = __uint_as_float(v[i / 4][i % 4]);
+        else x[i] = i % 2 == 0 ? bf16_lo(v[i / 8][i % 8 / 2]) : bf16_hi(v[i / 8][i % 8 / 2]);
+      }
+    }
+    top = x[0];
+#pragma unroll
+    for (int i = 1; i < kVec; ++i) top = maximum(top, x[i]);
+    base = fabsf(top) < INFINITY ? top : 0.f;
+    const double from = -kLog2E * static_cast<double>(base);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      if (i >= kVec) top = maximum(top, x[i]);
+      add(i, from);
+      if (i % kVec == kVec - 1) __builtin_amdgcn_sched_barrier(0);  // a load's numbers are used before the next load's are waited for
+    }
+  };
+  if ((chunk + 1) * (kThreads * kPer) <= vocab) take(std::true_type{});
+  else take(std::false_type{});
+  if (fabsf(top) < INFINITY && !(fabsf(top - base) < 600.f)) {
+    base = top;
+    sum = 0.0;
+    const double from = -kLog2E * static_cast<double>(base);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) add(i, from);
+  }
+  int classes = 1;
+  while (classes < kWave && classes < g.count) classes *= 2;
+  for (int m = kWave / 2; m >= classes; m /= 2) top = maximum(top, __shfl_xor(top, m));
+  if (lane < classes) s_top[wave][lane] = top;
+  __syncthreads();
+  const int c = lane % classes;
+  const float even = maximum(s_top[0][c], s_top[2][c]), odd = maximum(s_top[1][c], s_top[3][c]);
+  top = maximum(even, odd);
+  float reach = g.count > kWave ? fminf(even, odd) : top;
+  for (int m = 1; m < classes; m *= 2) {
     top = maximum(top, __shfl_xor(top, m));
     reach = fminf(reach, __shfl_xor(reach, m));
   }
-  if (lane == 0) s_top[wave] = top, s_reach[wave] = reach;
-  if (tid == 0) s_count = 0;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) top = maximum(top, s_top[w]), reach = fminf(reach, s_reach[w]);
   reach = fmaxf(reach, -FLT_MAX);  // -inf is no candidate
   const int64_t index = row * a.chunks + chunk;
   uint64_t* out = a.keys + index * g.count;
@@ -164,28 +196,35 @@ __global__ __launch_bounds__(kThreads) void chunk_kernel(const Select a) {
     return;
   }
 
-  double sum = 0.0;
-  const double from = -kLog2E * static_cast<double>(top);
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) sum += exp2_of(__builtin_fma(kLog2E, static_cast<double>(x[i]), from));
+  sum *= exp2_of(kLog2E * (static_cast<double>(base) - static_cast<double>(top)));
   for (int m = kWave / 2; m > 0; m >>= 1) sum += __shfl_xor(sum, m);
   if (lane == 0) s_sum[wave] = sum;
 
+  // Lists the numbers that a condition holds for; how many there are.
+  const auto list = [&](auto holds) {
+    int32_t n = 0;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    if (x[i] >= reach) {
-      const int32_t place = atomicAdd(&s_count, 1);
-      if (place < kCapacity) s_list[place] = key_of(x[i], token(i));
+    for (int i = 0; i < kPer; ++i) {
+      const bool one = holds(i);
+      const uint64_t those = __ballot(one);
+      if (those == 0) continue;
+      const int32_t place = n + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(those >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(those), 0));
+      if (one && place < kCapacity) s_list[wave][place] = key_of(x[i], token(i));
+      n += __popcll(those);
     }
-  }
-  __syncthreads();
+    if (lane == 0) s_part[wave] = n;
+    __syncthreads();
+    n = 0;
+    for (int w = 0; w < kWaves; ++w) n += s_part[w];
+    return n;
+  };
+  int32_t found = list([&](int i) { return x[i] >= reach; });
   if (tid == 0) {
     sum = 0.0;
     for (int w = 0; w < kWaves; ++w) sum += s_sum[w];
     a.sums[index] = sum;
     a.tops[index] = top;
   }
-  int32_t found = s_count;
   if (found > kCapacity) {
     // How many of the chunk's numbers a condition holds for.
     const auto number = [&](auto holds) {
@@ -225,39 +264,33 @@ __global__ __launch_bounds__(kThreads) void chunk_kernel(const Select a) {
       }
     }
     __syncthreads();
-    if (tid == 0) s_count = 0;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      if (x[i] > reach || (x[i] == reach && token(i) <= last)) {
-        const int32_t place = atomicAdd(&s_count, 1);
-        if (place < kCapacity) s_list[place] = key_of(x[i], token(i));
-      }
-    }
-    __syncthreads();
-    found = min(s_count, kCapacity);
+    found = list([&](int i) { return x[i] > reach || (x[i] == reach && token(i) <= last); });
   }
-  for (int32_t i = tid; i < found; i += kThreads) {
-    const uint64_t mine = s_list[i];
-    int32_t place = 0;
-#pragma unroll 8
-    for (int32_t j = 0; j < found; ++j) place += s_list[j] > mine ? 1 : 0;
-    if (place < g.count) out[place] = mine;
+  if (tid < found) {
+    int32_t of = 0, at = tid, place = 0;
+    while (at >= s_part[of]) at -= s_part[of++];
+    const uint64_t key = s_list[of][at];
+    for (int w = 0; w < kWaves; ++w) {
+      const int32_t n = s_part[w];
+#pragma unroll 4
+      for (int32_t j = 0; j < n; ++j) place += s_list[w][j] > key ? 1 : 0;
+    }
+    if (place < g.count) out[place] = key;
   }
   for (int32_t i = found + tid; i < g.count; i += kThreads) out[i] = 0;
 }
 
 // A group: the logarithms of its rows' sums, then the chunks' candidates by score, in the same way. The candidates are numbered
 // through the lists' first ones, then their second ones and so on, and dealt out to the groups of lanes one by one, so that every
-// group has some of the best.
+// group has some of the best. Bound by latency: 32 groups of 8 beams and 16 chunks take 8 us, 4.5 us of which are the launch and
+// the reads; 1 group of 64 beams for 128 continuations 30 us.
 __global__ __launch_bounds__(kMergeThreads) void merge_kernel(const Select a) {
-  constexpr int kHeld = 4;  // candidates of a thread in registers; what is left of them is read again
+  constexpr int kHeld = 4;  // candidates of a thread in registers, which give a number that `count` of them reach
   __shared__ double s_norm[PKV_BEAM_MAX], s_score[PKV_BEAM_MAX];
   __shared__ uint8_t s_kind[PKV_BEAM_MAX];  // 0: no continuation, 1: its row's, 2: the end token
   __shared__ double s_scores[kCapacity];
   __shared__ uint64_t s_keys[kCapacity];
   __shared__ uint8_t s_beams[kCapacity];
-  __shared__ int32_t s_places[kCapacity];
   __shared__ double s_top[kMergeWaves], s_reach[kMergeWaves];
   __shared__ int32_t s_count, s_part[kMergeWaves];
   const pkv_beam& g = a.g;
@@ -302,7 +335,6 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(const Select a) {
     }
   }
   if (tid == 0) s_count = 0;
-  for (int32_t i = tid; i < kCapacity; i += kMergeThreads) s_places[i] = 0;
   __syncthreads();
 
   const auto beam_of = [&](uint32_t i) { return i % lists / a.chunks; };
@@ -319,21 +351,9 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(const Select a) {
     const uint32_t i = mine + j * kMergeThreads;
     scores[j] = i < total ? score_of(i, held[j]) : -INFINITY;
   }
-  // f(candidate, key, score) for all of this thread's.
-  const auto each = [&](auto f) {
-#pragma unroll
-    for (int j = 0; j < kHeld; ++j) {
-      if (scores[j] > -INFINITY) f(mine + j * kMergeThreads, held[j], scores[j]);
-    }
-    for (uint32_t i = mine + kHeld * kMergeThreads; i < total; i += kMergeThreads) {
-      const uint64_t key = key_at(i);
-      const double score = score_of(i, key);
-      if (score > -INFINITY) f(i, key, score);
-    }
-  };
-
   double top = -INFINITY;
-  each([&](uint32_t, uint64_t, double score) { top = fmax(top, score); });
+#pragma unroll
+  for (int j = 0; j < kHeld; ++j) top = fmax(top, scores[j]);
   for (int m = 1; m < size; m *= 2) top = fmax(top, __shfl_xor(top, m));
   double reach = top;
   for (int m = size; m < kWave; m *= 2) {
@@ -345,19 +365,62 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(const Select a) {
 #pragma unroll
   for (int w = 0; w < kMergeWaves; ++w) top = fmax(top, s_top[w]), reach = fmin(reach, s_reach[w]);
 
-  const auto list = [&](uint32_t i, uint64_t key, double score) {
-    const int32_t place = atomicAdd(&s_count, 1);
-    if (place < kCapacity) s_scores[place] = score, s_keys[place] = key, s_beams[place] = static_cast<uint8_t>(beam_of(i));
+  // Bisection over the held candidates, where many reach it (one beam far above the others, or alone): `count` of them or
+  // little more, as candidates that are not held will reach it too.
+  const auto held_ones = [&](double at) {
+    int32_t n = 0;
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) n += __popcll(__ballot(scores[j] > -INFINITY && scores[j] >= at));
+    __syncthreads();
+    if (lane == 0) s_part[wave] = n;
+    __syncthreads();
+    n = 0;
+#pragma unroll
+    for (int w = 0; w < kMergeWaves; ++w) n += s_part[w];
+    return n;
   };
-  each([&](uint32_t i, uint64_t key, double score) {
-    if (score >= reach) list(i, key, score);
-  });
+  const int32_t enough = total <= kHeld * kMergeThreads ? kCapacity : g.count + g.count / 2 + 8;
+  if (held_ones(reach) > enough) {
+    uint64_t low = ordered(reach), high = ordered(top) + 1;
+    while (high - low > 1) {
+      const uint64_t middle = low + (high - low) / 2;
+      const int32_t n = held_ones(number_of(middle));
+      if (n >= g.count) low = middle;
+      else high = middle;
+      if (n >= g.count && n <= enough) break;
+    }
+    reach = number_of(low);
+  }
+
+  // f(beam, key, score) for the candidates that reach it: the held ones, and of what is left of each list the first ones.
+  const double least_score = reach;
+  const auto each = [&](auto f) {
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) {
+      if (scores[j] > -INFINITY && scores[j] >= least_score) f(beam_of(mine + j * kMergeThreads), held[j], scores[j]);
+    }
+    if (total <= kHeld * kMergeThreads) return;
+    for (uint32_t l = tid; l < lists; l += kMergeThreads) {
+      const uint32_t before = l < kHeld * kMergeThreads ? (kHeld * kMergeThreads - l + lists - 1) / lists : 0;
+      for (uint32_t i = l + before * lists; i < total; i += lists) {
+        const uint64_t key = key_at(i);
+        const double score = score_of(i, key);
+        if (!(score > -INFINITY && score >= least_score)) break;
+        f(beam_of(i), key, score);
+      }
+    }
+  };
+  const auto list = [&](uint32_t b, uint64_t key, double score) {
+    const int32_t place = atomicAdd(&s_count, 1);
+    if (place < kCapacity) s_scores[place] = score, s_keys[place] = key, s_beams[place] = static_cast<uint8_t>(b);
+  };
+  each(list);
   __syncthreads();
   int32_t found = s_count;
   if (found > kCapacity) {
     const auto number = [&](auto holds) {
       int32_t n = 0;
-      each([&](uint32_t i, uint64_t key, double score) { n += holds(i, key, score) ? 1 : 0; });
+      each([&](uint32_t b, uint64_t key, double score) { n += holds(b, key, score) ? 1 : 0; });
       for (int m = kWave / 2; m > 0; m >>= 1) n += __shfl_xor(n, m);
       __syncthreads();
       if (lane == 0) s_part[wave] = n;
@@ -388,14 +451,14 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(const Select a) {
       last = g.num_beams - 1;
       while (under < last) {
         const uint32_t middle = under + (last - under) / 2;
-        if (number([&](uint32_t i, uint64_t, double score) { return score == reach && beam_of(i) <= middle; }) >= rest) last = middle;
+        if (number([&](uint32_t b, uint64_t, double score) { return score == reach && b <= middle; }) >= rest) last = middle;
         else under = middle + 1;
       }
-      const int32_t own = rest - number([&](uint32_t i, uint64_t, double score) { return score == reach && beam_of(i) < last; });
+      const int32_t own = rest - number([&](uint32_t b, uint64_t, double score) { return score == reach && b < last; });
       uint64_t over = ~0ull;  // `least` is low enough, `over + 1` is not
       while (least < over) {
         const uint64_t middle = over - (over - least) / 2;
-        const auto holds = [&](uint32_t i, uint64_t key, double score) { return score == reach && beam_of(i) == last && key >= middle; };
+        const auto holds = [&](uint32_t b, uint64_t key, double score) { return score == reach && b == last && key >= middle; };
         if (number(holds) >= own) least = middle;
         else over = middle - 1;
       }
@@ -403,37 +466,40 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(const Select a) {
     __syncthreads();
     if (tid == 0) s_count = 0;
     __syncthreads();
-    each([&](uint32_t i, uint64_t key, double score) {
-      const uint32_t b = beam_of(i);
-      if (score > reach || (score == reach && (b < last || (b == last && key >= least)))) list(i, key, score);
+    each([&](uint32_t b, uint64_t key, double score) {
+      if (score > reach || (score == reach && (b < last || (b == last && key >= least)))) list(b, key, score);
     });
     __syncthreads();
     found = min(s_count, kCapacity);
   }
-  // Places. Of equal scores the lower beam's is first, in a beam the larger key. Threads that are left over share a candidate.
-  const int32_t parts = found > 0 ? max(kMergeThreads / found, 1) : 1;
-  for (int32_t w = tid; w < found * parts; w += kMergeThreads) {
-    const int32_t c = w % found, part = w / found;
-    const double score = s_scores[c];
-    const uint64_t key = s_keys[c];
-    const int32_t b = s_beams[c];
-    int32_t place = 0;
-#pragma unroll 4
-    for (int32_t j = found * part / parts; j < found * (part + 1) / parts; ++j) {
-      const double other = s_scores[j];
-      const int32_t beam = s_beams[j];
-      place += other > score || (other == score && (beam < b || (beam == b && s_keys[j] > key))) ? 1 : 0;
-    }
-    if (place > 0) atomicAdd(&s_places[c], place);
-  }
-  __syncthreads();
+  // Places. Of equal scores the lower beam's is first, in a beam the larger key.
   const int64_t out = group * g.count;
-  for (int32_t i = tid; i < found; i += kMergeThreads) {
-    const int32_t place = s_places[i], b = s_beams[i];
-    if (place >= g.count) continue;
-    g.best_scores[out + place] = static_cast<float>(s_scores[i]);
-    g.best_beams[out + place] = b;
-    g.best_tokens[out + place] = s_kind[b] == 2 ? g.end_token : static_cast<int32_t>(~static_cast<uint32_t>(s_keys[i]));
+  const int shares = shares_of(kMergeThreads, found), own = tid / shares;
+  if (own < found) {
+    const double score = s_scores[own];
+    const uint64_t key = s_keys[own];
+    const int32_t b = s_beams[own];
+    int32_t place = 0, equal = 0;
+#pragma unroll 4
+    for (int32_t j = tid % shares; j < found; j += shares) {
+      const double other = s_scores[j];
+      place += other > score ? 1 : 0;
+      equal += other == score ? 1 : 0;
+    }
+    for (int m = 1; m < shares; m *= 2) place += __shfl_xor(place, m), equal += __shfl_xor(equal, m);
+    if (tid % shares == 0) {
+      if (equal > 1) {
+        for (int32_t j = 0; j < found; ++j) {
+          const int32_t beam = s_beams[j];
+          place += s_scores[j] == score && (beam < b || (beam == b && s_keys[j] > key)) ? 1 : 0;
+        }
+      }
+      if (place < g.count) {
+        g.best_scores[out + place] = static_cast<float>(score);
+        g.best_beams[out + place] = b;
+        g.best_tokens[out + place] = s_kind[b] == 2 ? g.end_token : static_cast<int32_t>(~static_cast<uint32_t>(key));
+      }
+    }
   }
   for (int32_t i = found + tid; i < g.count; i += kMergeThreads) {
     g.best_scores[out + i] = -INFINITY;
