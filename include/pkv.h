@@ -877,7 +877,7 @@ int pkv_step_metadata(const pkv_step* args, int device, void* stream);
  *   workspace   : scratch of pkv_beam_workspace_bytes bytes, 16-byte aligned; calls that may run at the same time need
  *                 their own. Nothing in it needs to start at zero.
  * Up to PKV_BEAM_MAX beams and PKV_BEAM_MAX_COUNT continuations, which a group must have (count <= num_beams * vocab_size), up
- * to 2^20 rows. The same inputs give the same bits, whatever the batch.
+ * to 2^20 rows. The same call gives the same bits.
  */
 #define PKV_BEAM_MAX 64
 #define PKV_BEAM_MAX_COUNT 128

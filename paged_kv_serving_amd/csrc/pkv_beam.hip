@@ -110,9 +110,9 @@ __device__ __forceinline__ bool looked_at(const pkv_beam& g, int64_t row) {
 // larger ones. Where too many reach it (128 classes: about 700; equal logits), bisection finds a number that fewer do.
 // 32 groups of 8 beams over 128256 float32 logits: about 35 us for 115 MB. Bound by the vector units at 22 us of it, the
 // exponentials' 17 operations being two thirds of them, which the reads of 18 us overlap with in part; the kernel takes 21 us
-// without them. Half the bytes (bf16) take the same time.
+// without them. Half the bytes (bf16) take the same time. 7 wavefronts on a SIMD take 1.3 us less than the 5 of 88 registers.
 template <typename T, int kPer>
-__global__ __launch_bounds__(kThreads) void chunk_kernel(const Select a) {
+__global__ __launch_bounds__(kThreads, 7) void chunk_kernel(const Select a) {
   constexpr int kVec = 16 / sizeof(T), kLoads = kPer / kVec;
   __shared__ uint64_t s_list[kWaves][kCapacity];  // a wavefront's own, so that no place needs an atomic
   __shared__ float s_top[kWaves][kWave];

@@ -618,7 +618,7 @@ def beam_select(
     :func:`beam_reorder` takes them.
 
     ``workspace``: scratch of :func:`beam_workspace_bytes` bytes, allocated when None; calls that may run at the same time
-    need their own. The same inputs give the same bits, whatever the batch.
+    need their own. The same call gives the same bits.
     """
     device = _one_device(logits, scores) if finished is None else _one_device(logits, scores, finished)
     if logits.dim() != 2 or logits.dtype not in _DTYPE_CODES:
@@ -642,8 +642,7 @@ def beam_select(
         logits = logits.contiguous()
     shape = (groups, count)
     if out is None:
-        best = scores.new_empty((3, *shape))
-        out = BeamChoice(best[0], *best[1:].view(torch.int32).unbind(0))
+        out = BeamChoice(scores.new_empty(shape), *scores.new_empty((2, groups, count), dtype=torch.int32).unbind(0))
     else:
         for name, tensor, dtype in zip(out._fields, out, (torch.float32, torch.int32, torch.int32)):
             if tensor.shape != shape or tensor.dtype != dtype or not tensor.is_contiguous() or tensor.device != logits.device:
@@ -707,7 +706,7 @@ def beam_reorder(
         shape = state.shape
         if len(shape) < 2 or shape[1] != num_blocks or not state.is_contiguous():
             raise ValueError("states must be contiguous [layers, num_blocks, ...] of one number of blocks")
-        layer = state[0].numel() * state.element_size() if shape[0] else 0
+        layer = state.numel() // shape[0] * state.element_size() if shape[0] else 0
         moved += (state.data_ptr(), layer // num_blocks if num_blocks else 0, layer, shape[0])
     if out is None:
         out = torch.empty_like(block_tables)
@@ -788,7 +787,7 @@ def step_metadata(
         raise ValueError(f"num_rows must be in [0, {MAX_STEP_ROWS}]")
     if out is None:
         wide = query_lens.new_empty((2, num_rows), dtype=torch.int64)
-        seq, position, starts, contexts, following = query_lens.new_empty((2 * num_rows + 2 * seqs + 2,)).split((num_rows, num_rows, seqs + 1, seqs, 1))
+        seq, position, starts, contexts, following = query_lens.new_empty((2 * num_rows + 2 * seqs + 2,)).split_with_sizes((num_rows, num_rows, seqs + 1, seqs, 1))
         out = StepMetadata(seq, position, *wide.unbind(0), starts, contexts, following)
     else:
         sizes, wide = (num_rows, num_rows, num_rows, num_rows, seqs + 1, seqs, 1), ("positions", "slot_mapping")
