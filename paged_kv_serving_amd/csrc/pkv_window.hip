@@ -54,6 +54,7 @@ struct Window {
   int32_t subgroups;       // of up to 16 query heads of a group
   int32_t tile_rows;       // rows of a tile: the aligned blocks of rows that runs lie in
   uint32_t tile_items;     // workgroups with tiles; the others have rows
+  uint32_t run_shares;     // of codes: workgroups that share a tile's runs
   int32_t tiled;           // whether the tile pass computes the runs
   int32_t min_run;         // rows of one sequence next to each other that a tile takes
   int32_t* list;           // the rows that no tile takes (list_kernel); NULL without tiles
@@ -1382,7 +1383,10 @@ __global__ __launch_bounds__(kThreads, (TileShape<QT, KVT, D>::kWaves)) void til
   item /= static_cast<uint32_t>(a.num_kv_heads);
   const int32_t split = item % static_cast<uint32_t>(a.splits);
   int64_t block0 = item / static_cast<uint32_t>(a.splits);
+  uint32_t share = 0;
   if constexpr (sizeof(KVT) == 1) {
+    share = static_cast<uint32_t>(block0) % a.run_shares;
+    block0 = static_cast<uint32_t>(block0) / a.run_shares;
     if (a.order) block0 = a.order[block0];
   }
   block0 *= a.tile_rows;
@@ -1416,7 +1420,11 @@ __global__ __launch_bounds__(kThreads, (TileShape<QT, KVT, D>::kWaves)) void til
     const uint64_t low = static_cast<uint64_t>(bits);
     return low != 0 ? __builtin_ctzll(low) : 64 + __builtin_ctzll(static_cast<uint64_t>(bits >> 64));
   };
+  uint32_t nth = 0;
   for (; runs != 0; runs &= runs - 1) {
+    if constexpr (sizeof(KVT) == 1) {
+      if (nth++ % a.run_shares != share) continue;
+    }
     const int at = first_of(runs);
     const uint128 behind = starts & ~((static_cast<uint128>(2) << at) - 1);
     const int64_t run0 = block0 + at, run1 = behind != 0 ? block0 + first_of(behind) : block1;
@@ -1863,7 +1871,7 @@ int launch(Window a, hipStream_t stream) {
   const int64_t items = a.num_queries * a.num_kv_heads * a.subgroups * a.splits;
   // Beside tiles the number of rows is known on the device only: two workgroups for every CU share them.
   const int64_t groups = a.tiled ? std::min<int64_t>(items, 512) : items;
-  const int64_t tiles = (a.num_queries + a.tile_rows - 1) / a.tile_rows * a.num_kv_heads * a.splits;
+  const int64_t tiles = (a.num_queries + a.tile_rows - 1) / a.tile_rows * a.num_kv_heads * a.splits * std::max(a.run_shares, 1u);
   const int64_t joins = (a.num_queries * a.num_heads * (D / 4) + kThreads - 1) / kThreads;
   constexpr int64_t kMost = 0xffffffffll / (2 * kThreads);  // workgroups whose threads, up to 512 each, 32 bits count
   if (groups > kMost || joins > kMost || tiles > kMost - 512 || items > 0x7fffffff) return PKV_EUNSUPPORTED;
@@ -2028,6 +2036,7 @@ namespace {
 struct Plan {
   int32_t splits = 0;
   int64_t bytes = 0, order_bytes = 0;  // the order's are its last
+  uint32_t run_shares = 1;
   bool runs = false, pages = false, stream = false;
   PageForm form{};
 };
@@ -2055,13 +2064,21 @@ Plan codes_plan(const pkv_window& g) {
       // Tiles of bfloat16 queries are two to a CU, of float32 ones one. Shares of 384 keys at least, of 128 where tiles are few: a part
       // more of every row is written and joined. 1 x 128 rows of up to 4128 keys, 32/8 heads x 128, float32, with 4, 8, 16 splits:
       // 46, 39, 53 us; 2 x 301 rows beside 24, 16 heads x 64, window 1000, with 1, 2, 3, 6: 58, 46, 54, 65; 1 x 32 rows of
-      // 1032 keys, 16/2 heads x 64, bfloat16, with 2, 4, 8: 19, 15, 15.
+      // 1032 keys, 16/2 heads x 64, bfloat16, with 2, 4, 8: 19, 15, 15; 3 x 339 rows of up to 610 keys, 8/1 heads x 64, float32 (64 tiles),
+      // with 1, 2, 4, 8: 49, 39, 34, 34; 1 x 512 rows, 8 heads x 128, bfloat16 (32 tiles): 36, 30, 27, 27; 7 x 130 rows of 226 keys, 16/4
+      // heads x 256 (116 tiles): 51, 51, 62, 94.
       const int64_t rows = kTileQueries / group, groups = (g.num_queries + rows - 1) / rows * g.num_kv_heads;
       const int64_t longest = std::min<int64_t>(g.max_context_len, static_cast<int64_t>(g.window) + g.sinks);
-      const int64_t most = std::min<int64_t>(PKV_WINDOW_MAX_SPLITS, longest / (groups <= 16 ? 128 : 384));
-      p.splits = static_cast<int32_t>(std::max<int64_t>(1, std::min(most, (g.q_dtype == PKV_F32 ? 256 : 512) / groups)));
+      const int64_t most = std::min<int64_t>(PKV_WINDOW_MAX_SPLITS, longest / (groups <= 64 ? 128 : 384));
+      p.splits = static_cast<int32_t>(std::max<int64_t>(1, std::min(most, (g.q_dtype == PKV_F32 || (groups > 16 && groups <= 64) ? 256 : 512) / groups)));
       p.bytes = pkv_window_workspace_bytes(g.num_queries, g.num_heads, g.head_dim, g.max_query_len, p.splits);
     }
+    // A tile's runs one after the other cost their latencies; where tiles are few and runs surely shorter than they are, several
+    // workgroups share them. 6 x 27 rows, 8 heads x 128, bfloat16: 18 us, in one workgroup each 54; 2 x 12 rows of up to 1191
+    // keys, 8/2 heads x 128, float32: 26 us and 42.
+    const int64_t rows = kTileQueries / group, groups = (g.num_queries + rows - 1) / rows * g.num_kv_heads * p.splits;
+    const int64_t longest = g.max_query_len > 0 ? g.max_query_len : g.num_queries;
+    p.run_shares = static_cast<uint32_t>(std::max<int64_t>(1, std::min({int64_t{8}, 256 / groups, (2 * rows + longest - 1) / longest})));
     p.order_bytes = (ordered_blocks(g.num_queries, group) + 3) / 4 * 16;
     p.bytes += p.order_bytes;
     return p;
@@ -2139,6 +2156,7 @@ int attention(const pkv_window& g, const float* key_scales, const float* value_s
   a.given_scale = a.scale_log2;
   if (plan.runs) a.list = reinterpret_cast<int32_t*>(reinterpret_cast<char*>(g.workspace) + need - plan.order_bytes - list_bytes(g.num_queries));
   if (plan.order_bytes > 0) a.order = reinterpret_cast<int32_t*>(reinterpret_cast<char*>(g.workspace) + need - plan.order_bytes);
+  a.run_shares = plan.run_shares;
   if (plan.pages) a.page_groups = g.block_size / 16;
   if (plan.stream) {
     a.stream_groups = plan.form.groups;
