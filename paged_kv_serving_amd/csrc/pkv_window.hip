@@ -1252,8 +1252,8 @@ __global__ __launch_bounds__(kThreads) void stream_join_kernel(const Window a) {
 // 234 us (three products for one), over float32 438 (six, at one wavefront per SIMD). One piece of P instead of two was
 // 9% faster.
 // ---------------------------------------------------------------------------------------------
-// float32 queries of head_dim 256 have no tiles (their pieces do not fit the registers, nor float32 pools' LDS): their
-// rows go by themselves.
+// float32 queries of head_dim 256 have tiles over codes alone (float32 pools' pieces do not fit LDS): over pools their rows go by
+// themselves (codes, 5 x 455 rows behind up to 2055 others, 8 heads: 422 us, by themselves 3277).
 constexpr bool tiles_of(int q_size, int head_dim) { return q_size == 2 || head_dim <= 128; }
 
 template <typename QT, typename KVT, int D>
@@ -1267,7 +1267,7 @@ struct TileShape {
   static constexpr int kStaged = kKeys * kChunks / kThreads;           // chunks of a tile per thread, K and V each
   static constexpr int kLds = 2 * 2 * kKvPieces * kPlane * 2;          // bytes: two buffers of K and V
   static constexpr int kWaves = kLds <= 81920 && sizeof(QT) == 2 && D <= 128 ? 2 : 1;  // per SIMD
-  static constexpr bool kFits = tiles_of(sizeof(QT), D);
+  static constexpr bool kFits = tiles_of(sizeof(QT), D) || sizeof(KVT) == 1;
   static_assert(!kFits || kLds <= 160 * 1024 - 2048, "a tile's buffers, slots and live bits fit LDS");
 };
 
@@ -2058,8 +2058,10 @@ int64_t ordered_blocks(int64_t num_queries, int32_t group) {
 Plan codes_plan(const pkv_window& g) {
   Plan p = window_plan(g);
   if (p.splits < 1) return p;
+  const int32_t group = g.num_heads / g.num_kv_heads;
+  p.runs = has_runs(g.max_query_len, group);
   if (p.runs) {
-    const int32_t group = g.num_heads / g.num_kv_heads;
+    p.bytes = pkv_window_workspace_bytes(g.num_queries, g.num_heads, g.head_dim, g.max_query_len, p.splits);
     if (g.num_splits == 0) {
       // Tiles of bfloat16 queries are two to a CU, of float32 ones one. Shares of 384 keys at least, of 128 where tiles are few: a part
       // more of every row is written and joined. 1 x 128 rows of up to 4128 keys, 32/8 heads x 128, float32, with 4, 8, 16 splits:
