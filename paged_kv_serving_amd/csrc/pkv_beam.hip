@@ -486,19 +486,20 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(const Select a) {
       place += other > score ? 1 : 0;
       equal += other == score ? 1 : 0;
     }
-    for (int m = 1; m < shares; m *= 2) place += __shfl_xor(place, m), equal += __shfl_xor(equal, m);
-    if (tid % shares == 0) {
-      if (equal > 1) {
-        for (int32_t j = 0; j < found; ++j) {
-          const int32_t beam = s_beams[j];
-          place += s_scores[j] == score && (beam < b || (beam == b && s_keys[j] > key)) ? 1 : 0;
-        }
+    for (int m = 1; m < shares; m *= 2) equal += __shfl_xor(equal, m);
+    if (equal > 1) {  // as bfloat16 logits often are
+#pragma unroll 4
+      for (int32_t j = tid % shares; j < found; j += shares) {
+        const int32_t beam = s_beams[j];
+        const bool larger = s_keys[j] > key;
+        place += (s_scores[j] == score) & ((beam < b) | ((beam == b) & larger)) ? 1 : 0;
       }
-      if (place < g.count) {
-        g.best_scores[out + place] = static_cast<float>(score);
-        g.best_beams[out + place] = b;
-        g.best_tokens[out + place] = s_kind[b] == 2 ? g.end_token : static_cast<int32_t>(~static_cast<uint32_t>(key));
-      }
+    }
+    for (int m = 1; m < shares; m *= 2) place += __shfl_xor(place, m);
+    if (tid % shares == 0 && place < g.count) {
+      g.best_scores[out + place] = static_cast<float>(score);
+      g.best_beams[out + place] = b;
+      g.best_tokens[out + place] = s_kind[b] == 2 ? g.end_token : static_cast<int32_t>(~static_cast<uint32_t>(key));
     }
   }
   for (int32_t i = found + tid; i < g.count; i += kMergeThreads) {
@@ -513,23 +514,26 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(const Select a) {
 // copy. Every workgroup finds its group's moves by itself: the parents that earlier children named are a word of bits.
 // Bound: HBM.
 // ---------------------------------------------------------------------------------------------
+constexpr int kTogether = 4;  // units that a thread loads before it stores them
 struct Reorder {
   pkv_reorder g;
   int32_t unit[PKV_BEAM_STATES];  // bytes that are moved together: 16, 4 or 1
+  // Whether every state's block is one batch of a wavefront. The wavefronts then have a state each, and the states' latencies run
+  // at the same time: 18 groups of 16 beams, 22 layers, 1 KB each of keys and values with their scales, 24 us, together 31.
+  bool apart;
 };
 
-template <typename U>
-__device__ __forceinline__ void copy_units(void* to, const void* from, int64_t count) {
-  constexpr int kTogether = 4;
-  for (int64_t i = threadIdx.x; i < count; i += kThreads * kTogether) {
+template <typename U, int kThreadsOf>
+__device__ __forceinline__ void copy_units(void* to, const void* from, int64_t count, int first) {
+  for (int64_t i = first; i < count; i += kThreadsOf * kTogether) {
     U x[kTogether];
 #pragma unroll
     for (int j = 0; j < kTogether; ++j) {
-      if (i + j * kThreads < count) x[j] = static_cast<const U*>(from)[i + j * kThreads];
+      if (i + j * kThreadsOf < count) x[j] = static_cast<const U*>(from)[i + j * kThreadsOf];
     }
 #pragma unroll
     for (int j = 0; j < kTogether; ++j) {
-      if (i + j * kThreads < count) static_cast<U*>(to)[i + j * kThreads] = x[j];
+      if (i + j * kThreadsOf < count) static_cast<U*>(to)[i + j * kThreadsOf] = x[j];
     }
   }
 }
@@ -570,15 +574,22 @@ __global__ __launch_bounds__(kThreads) void reorder_kernel(const Reorder a) {
   const int32_t source = tables[static_cast<int64_t>(parent) * g.table_stride + full];
   const int32_t target = tables[static_cast<int64_t>(keeper) * g.table_stride + full];
   if (source < 0 || source >= g.num_blocks || target < 0 || target >= g.num_blocks || source == target) return;
-  for (int32_t s = 0; s < g.num_states; ++s) {
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  for (int32_t s = a.apart ? wave : 0; s < g.num_states; s += a.apart ? kWaves : 1) {
     if (layer >= g.num_layers[s]) continue;
     char* base = static_cast<char*>(g.states[s]) + layer * g.layer_bytes[s];
     const int64_t bytes = g.block_bytes[s];
     char* to = base + target * bytes;
     const char* from = base + source * bytes;
-    if (a.unit[s] == 16) copy_units<u32x4>(to, from, bytes / 16);
-    else if (a.unit[s] == 4) copy_units<uint32_t>(to, from, bytes / 4);
-    else copy_units<uint8_t>(to, from, bytes);
+    if (a.apart) {
+      if (a.unit[s] == 16) copy_units<u32x4, kWave>(to, from, bytes / 16, lane);
+      else if (a.unit[s] == 4) copy_units<uint32_t, kWave>(to, from, bytes / 4, lane);
+      else copy_units<uint8_t, kWave>(to, from, bytes, lane);
+    } else {
+      if (a.unit[s] == 16) copy_units<u32x4, kThreads>(to, from, bytes / 16, tid);
+      else if (a.unit[s] == 4) copy_units<uint32_t, kThreads>(to, from, bytes / 4, tid);
+      else copy_units<uint8_t, kThreads>(to, from, bytes, tid);
+    }
   }
 }
 
@@ -652,6 +663,7 @@ extern "C" int pkv_beam_reorder(const pkv_reorder* args, int device, void* strea
   if (static_cast<int64_t>(g.table_stride) * g.block_size > 0x7fffffff) return PKV_EUNSUPPORTED;
   Reorder a{};
   a.g = g;
+  a.apart = true;
   int32_t layers = 1;
   for (int s = 0; s < g.num_states; ++s) {
     if (g.num_layers[s] < 0 || g.block_bytes[s] < 0 || g.layer_bytes[s] < 0) return PKV_EINVAL;
@@ -660,6 +672,7 @@ extern "C" int pkv_beam_reorder(const pkv_reorder* args, int device, void* strea
     layers = std::max(layers, g.num_layers[s]);
     const uint64_t bits = reinterpret_cast<uintptr_t>(g.states[s]) | static_cast<uint64_t>(g.block_bytes[s]) | static_cast<uint64_t>(g.layer_bytes[s]);
     a.unit[s] = bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : 1;
+    a.apart = a.apart && g.block_bytes[s] / a.unit[s] <= kWave * kTogether;
   }
   if (g.num_groups > 0x7fffffff / (kThreads * PKV_BEAM_MAX)) return PKV_EUNSUPPORTED;
   if (g.num_groups == 0) return PKV_OK;
