@@ -1079,6 +1079,27 @@ __global__ __launch_bounds__(kRowWaves * kPair * kWave) void page_kernel(const W
   page_piece<QT, D, kRowWaves, kPair>(a, shared, t, seq, count, first, last, h.kv_head, h.head0, h.count, split_place(a, t, h.head0, split));
 }
 
+// The listed rows of a call with tiles, item by item of workgroup `block` of `blocks`. 20 rows of 2481 to 2853 keys beside a run of 10,
+// 32/8 heads x 128, bfloat16, blocks of 16: 39 us, of one token, which the general row pass takes, 51.
+template <typename QT, int D>
+__device__ __forceinline__ void page_pass(const Window& a, RowScratch<D, kWaves, 1>& shared, uint32_t block, uint32_t blocks) {
+  constexpr int kKeys = 16 * PageShape<QT, D>::kBlocks;
+  const uint32_t groups = a.num_kv_heads * a.subgroups;
+  const int64_t items = static_cast<int64_t>(a.list[0]) * a.splits * groups;
+  for (int64_t next = block; next < items; next += blocks) {
+    const uint32_t item = static_cast<uint32_t>(next) / groups;
+    const Heads h = heads_of<1>(a, static_cast<uint32_t>(next) % groups);
+    const int32_t split = item % static_cast<uint32_t>(a.splits);
+    const int64_t t = a.list[1 + item / static_cast<uint32_t>(a.splits)];
+    const int32_t seq = a.seqs[t];
+    const int32_t count = span_of(a, seq, a.positions[t]).end;
+    const int32_t rounds = (count + kKeys - 1) / kKeys;
+    const int32_t first = static_cast<int32_t>(static_cast<int64_t>(rounds) * split / a.splits);
+    const int32_t last = static_cast<int32_t>(static_cast<int64_t>(rounds) * (split + 1) / a.splits);
+    page_piece<QT, D, kWaves, 1>(a, shared, t, seq, count, first, last, h.kv_head, h.head0, h.count, split_place(a, t, h.head0, split));
+  }
+}
+
 // ---------------------------------------------------------------------------------------------
 // The same with equal shares of the whole call's rounds instead of splits of its rows, whose lengths only the device knows: every
 // workgroup sums all rows' rounds, and takes the rounds from `share` times its number on, through as many rows as they
@@ -1375,7 +1396,12 @@ __global__ __launch_bounds__(kThreads, (TileShape<QT, KVT, D>::kWaves)) void til
   constexpr bool kRowsFirst = sizeof(QT) == 2;
   const uint32_t row_blocks = gridDim.x - a.tile_items, before = kRowsFirst ? row_blocks : a.tile_items;
   if ((blockIdx.x < before) == kRowsFirst) {
-    row_pass<QT, KVT, D, kWaves, 1>(a, *reinterpret_cast<RowScratch<D, kWaves, 1>*>(s_kv), blockIdx.x - (kRowsFirst ? 0 : before), row_blocks);
+    auto& scratch = *reinterpret_cast<RowScratch<D, kWaves, 1>*>(s_kv);
+    const uint32_t block = blockIdx.x - (kRowsFirst ? 0 : before);
+    if constexpr (sizeof(KVT) == 1) {
+      if (a.page_groups > 0) return page_pass<QT, D>(a, scratch, block, row_blocks);
+    }
+    row_pass<QT, KVT, D, kWaves, 1>(a, scratch, block, row_blocks);
     return;
   }
   uint32_t item = blockIdx.x - (kRowsFirst ? before : 0);
@@ -1868,6 +1894,7 @@ int launch(Window a, hipStream_t stream) {
   a.tile_rows = kTileQueries / a.group;
   a.min_run = std::min(kMinRun, a.tile_rows);
   a.tiled = S::kFits && a.list;  // no list without tiles
+  if (a.page_groups > 0) a.page_magic = static_cast<uint32_t>(((int64_t{1} << 32) + a.page_groups - 1) / a.page_groups);
   const int64_t items = a.num_queries * a.num_kv_heads * a.subgroups * a.splits;
   // Beside tiles the number of rows is known on the device only: two workgroups for every CU share them.
   const int64_t groups = a.tiled ? std::min<int64_t>(items, 512) : items;
@@ -1910,7 +1937,6 @@ int launch(Window a, hipStream_t stream) {
   };
   if constexpr (sizeof(KVT) == 1) {
     if (a.page_groups > 0) {
-      a.page_magic = static_cast<uint32_t>(((int64_t{1} << 32) + a.page_groups - 1) / a.page_groups);
       if (!a.stream) {
         // Where there are many rows, a workgroup serves four neighbouring key heads and so reads 4 D bytes next to each other
         // (128 rows of 256 keys, 8 key heads x 128: 17.0 us, a head to a workgroup 21.8; 16 rows 10.4 and 9.0).
@@ -2059,6 +2085,8 @@ Plan codes_plan(const pkv_window& g) {
   Plan p = window_plan(g);
   if (p.splits < 1) return p;
   const int32_t group = g.num_heads / g.num_kv_heads;
+  // page_kernel's offsets within 16 rows are 32-bit, and its reciprocal holds for up to 64 groups to a block.
+  p.pages = g.window == INT32_MAX && g.block_size % 16 == 0 && g.block_size <= 1024 && g.num_blocks > 0 && g.num_kv_heads <= (1 << 18);
   p.runs = has_runs(g.max_query_len, group);
   if (p.runs) {
     p.bytes = pkv_window_workspace_bytes(g.num_queries, g.num_heads, g.head_dim, g.max_query_len, p.splits);
@@ -2071,8 +2099,13 @@ Plan codes_plan(const pkv_window& g) {
       // heads x 256 (116 tiles): 51, 51, 62, 94.
       const int64_t rows = kTileQueries / group, groups = (g.num_queries + rows - 1) / rows * g.num_kv_heads;
       const int64_t longest = std::min<int64_t>(g.max_context_len, static_cast<int64_t>(g.window) + g.sinks);
-      const int64_t most = std::min<int64_t>(PKV_WINDOW_MAX_SPLITS, longest / (groups <= 64 ? 128 : 384));
-      p.splits = static_cast<int32_t>(std::max<int64_t>(1, std::min(most, (g.q_dtype == PKV_F32 || (groups > 16 && groups <= 64) ? 256 : 512) / groups)));
+      const int64_t shares = groups <= 64 ? std::min(longest / 128, std::max<int64_t>(8, longest / 1024)) : longest / 384;
+      const int64_t tiles = (g.q_dtype == PKV_F32 || (groups > 16 && groups <= 64) ? 256 : 512) / groups;
+      // The rows by themselves, a sequence each at most, have the tiles' splits, and fill the GPU with fewer. 20 rows of 2481 to 2853 keys
+      // beside a run of 10, 32/8 heads x 128, bfloat16, with 1, 3, 8, 22: 44, 39, 52, 81; 64 rows of 100 to 4000 beside 512, with 1, 3: 104,
+      // 115; 61 of 64 beside a run of 6 with 1503, 16/8 heads x 64, float32, with 1, 3, 8: 65, 33, 48.
+      const int64_t rows_fill = std::max<int64_t>(groups <= 64 ? 3 : 1, 512 / std::max<int64_t>(1, static_cast<int64_t>(g.num_seqs) * g.num_kv_heads));
+      p.splits = static_cast<int32_t>(std::max<int64_t>(1, std::min({int64_t{PKV_WINDOW_MAX_SPLITS}, shares, tiles, rows_fill})));
       p.bytes = pkv_window_workspace_bytes(g.num_queries, g.num_heads, g.head_dim, g.max_query_len, p.splits);
     }
     // A tile's runs one after the other cost their latencies; where tiles are few and runs surely shorter than they are, several
@@ -2085,8 +2118,6 @@ Plan codes_plan(const pkv_window& g) {
     p.bytes += p.order_bytes;
     return p;
   }
-  // page_kernel's offsets within 16 rows are 32-bit, and its reciprocal holds for up to 64 groups to a block.
-  p.pages = g.window == INT32_MAX && g.block_size % 16 == 0 && g.block_size <= 1024 && g.num_blocks > 0 && g.num_kv_heads <= (1 << 18);
   // A short row is one workgroup's, which saves the join's launch.
   p.stream = p.pages && g.num_splits == 0 && g.num_queries <= kStreamRows && g.num_queries * g.max_context_len > kStreamKeys;
   if (p.stream) {
