@@ -858,7 +858,7 @@ int pkv_step_metadata(const pkv_step* args, int device, void* stream);
 
 /*
  * Beam search: the best continuations of each group of num_beams beams over the whole vocabulary.
- *     score(b, v) = scores[b] + (logits[b, v] - log sum_u exp(logits[b, u]))
+ *     score(b, v) = scores[b] + ((logits[b, v] - most(b)) - log sum_u exp(logits[b, u] - most(b))),  most(b) = max_u logits[b, u]
  * in double precision (exponentials, their sums and the logarithm within 2^-40 of themselves), rounded once to float32 at the
  * end. Of a group's continuations with a score above -inf, the `count` of the highest scores, in falling order; equal
  * scores in order of their beams, and within a beam of falling logits, then of rising tokens. Where there are fewer, the rest are

@@ -25,10 +25,10 @@ def select_group(logits, scores, count: int, finished=None, end_token: int = 0) 
         most = row.max()
         if not math.isfinite(most):  # a NaN, +inf, or nothing above -inf
             continue
-        norm = most + math.log(math.fsum(np.exp(row - most)))
+        norm = math.log(math.fsum(np.exp(row - most)))
         # No token outside a row's best `count`, ties by number, can be among the group's.
         order = np.lexsort((np.arange(row.size), -row))[:count]
-        found += [(-(score + (row[token] - norm)), beam, -row[token], int(token)) for token in order if row[token] > -math.inf]
+        found += [(-(score + ((row[token] - most) - norm)), beam, -row[token], int(token)) for token in order if row[token] > -math.inf]
     best = [(-negative, beam, token) for negative, beam, _, token in sorted(found)[:count]]
     return best + [(-math.inf, 0, end_token)] * (count - len(best))
 

@@ -52,15 +52,15 @@ __device__ __forceinline__ double logit_of(uint64_t key) { return static_cast<do
 // The larger of two, NaN where one is.
 __device__ __forceinline__ float maximum(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
-// 2^t in double precision for t <= 1000, from 2^-1000 on: 2^k p(t - k), k being the nearest whole number, which adding 1.5 * 2^52
-// leaves in the low bits. p is the interpolation of 2^r at the ten Chebyshev nodes of [-1/2, 1/2], within 2^-45 of it. Additions
-// and products alone: conversions and ldexp run at a fraction of their rate.
-constexpr double kLog2E = 1.4426950408889634;
-__device__ __forceinline__ double exp2_of(double t) {
-  constexpr double kWhole = 6755399441055744.0;
-  t = fmax(t, -1000.0);
-  const double shifted = t + kWhole;
-  const double r = t - (shifted - kWhole);
+// e^x in double precision for x <= 690, from e^-690 on: 2^k p(x / ln 2 - k), k being the nearest whole number, which adding
+// 1.5 * 2^52 leaves in the low bits. p is the interpolation of 2^r at the ten Chebyshev nodes of [-1/2, 1/2], within 2^-45 of it.
+// Additions and products alone: conversions and ldexp run at a fraction of their rate. Differences come in, not their terms:
+// a product of each with 1 / ln 2 would lose what a difference of large ones keeps.
+__device__ __forceinline__ double exp_of(double x) {
+  constexpr double kWhole = 6755399441055744.0, kLog2E = 1.4426950408889634;
+  x = fmax(x, -690.0);
+  const double shifted = __builtin_fma(kLog2E, x, kWhole);
+  const double r = __builtin_fma(kLog2E, x, kWhole - shifted);
   double p = 1.0205905413765595e-07;
   p = __builtin_fma(p, r, 1.325964524488711e-06);
   p = __builtin_fma(p, r, 1.5252672924850737e-05);
@@ -134,7 +134,7 @@ __global__ __launch_bounds__(kThreads, 7) void chunk_kernel(const Select a) {
   // of numbers 600 above and below it, and where a thread has others it starts again, against its largest.
   float x[kPer], top, base;
   double sum = 0.0;
-  const auto add = [&](int i, double from) { sum += exp2_of(__builtin_fma(kLog2E, static_cast<double>(x[i]), from)); };
+  const auto add = [&](int i, double from) { sum += exp_of(static_cast<double>(x[i]) - from); };
   const auto take = [&](auto whole) {
     u32x4 v[kLoads];
     if constexpr (whole) {
@@ -157,7 +157,7 @@ __global__ __launch_bounds__(kThreads, 7) void chunk_kernel(const Select a) {
 #pragma unroll
     for (int i = 1; i < kVec; ++i) top = maximum(top, x[i]);
     base = fabsf(top) < INFINITY ? top : 0.f;
-    const double from = -kLog2E * static_cast<double>(base);
+    const double from = base;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       if (i >= kVec) top = maximum(top, x[i]);
@@ -170,7 +170,7 @@ __global__ __launch_bounds__(kThreads, 7) void chunk_kernel(const Select a) {
   if (fabsf(top) < INFINITY && !(fabsf(top - base) < 600.f)) {
     base = top;
     sum = 0.0;
-    const double from = -kLog2E * static_cast<double>(base);
+    const double from = base;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) add(i, from);
   }
@@ -196,7 +196,7 @@ __global__ __launch_bounds__(kThreads, 7) void chunk_kernel(const Select a) {
     return;
   }
 
-  sum *= exp2_of(kLog2E * (static_cast<double>(base) - static_cast<double>(top)));
+  sum *= exp_of(static_cast<double>(base) - static_cast<double>(top));
   for (int m = kWave / 2; m > 0; m >>= 1) sum += __shfl_xor(sum, m);
   if (lane == 0) s_sum[wave] = sum;
 
@@ -286,7 +286,7 @@ __global__ __launch_bounds__(kThreads, 7) void chunk_kernel(const Select a) {
 // the reads; 1 group of 64 beams for 128 continuations 30 us.
 __global__ __launch_bounds__(kMergeThreads) void merge_kernel(const Select a) {
   constexpr int kHeld = 4;  // candidates of a thread in registers, which give a number that `count` of them reach
-  __shared__ double s_norm[PKV_BEAM_MAX], s_score[PKV_BEAM_MAX];
+  __shared__ double s_top_logit[PKV_BEAM_MAX], s_log[PKV_BEAM_MAX], s_score[PKV_BEAM_MAX];
   __shared__ uint8_t s_kind[PKV_BEAM_MAX];  // 0: no continuation, 1: its row's, 2: the end token
   __shared__ double s_scores[kCapacity];
   __shared__ uint64_t s_keys[kCapacity];
@@ -322,14 +322,15 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(const Select a) {
     for (int m = kWave / 2; m > 0; m >>= 1) top = maximum(top, __shfl_xor(top, m));
     double sum = 0.0;
     const auto add = [&](float one, double part) {
-      if (part != 0.0) sum += part * exp2_of(kLog2E * (static_cast<double>(one) - static_cast<double>(top)));
+      if (part != 0.0) sum += part * exp_of(static_cast<double>(one) - static_cast<double>(top));
     };
     add(top0, sum0);
     for (int32_t c = lane + kWave; c < a.chunks; c += kWave) add(tops[c], sums[c]);
     for (int m = kWave / 2; m > 0; m >>= 1) sum += __shfl_xor(sum, m);
     if (lane == 0) {
       const bool usable = fabsf(score) < INFINITY, counts = usable && !finished && fabsf(top) < INFINITY;
-      s_norm[b] = counts ? static_cast<double>(top) + log(sum) : 0.0;
+      s_top_logit[b] = top;
+      s_log[b] = counts ? log(sum) : 0.0;
       s_score[b] = score;
       s_kind[b] = counts ? 1 : usable && finished ? 2 : 0;
     }
@@ -343,7 +344,7 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(const Select a) {
     const uint32_t b = beam_of(i);
     const int32_t kind = s_kind[b];
     if (kind == 2) return i == b * a.chunks ? s_score[b] : -INFINITY;
-    return kind == 1 && key != 0 ? s_score[b] + (logit_of(key) - s_norm[b]) : -INFINITY;
+    return kind == 1 && key != 0 ? s_score[b] + ((logit_of(key) - s_top_logit[b]) - s_log[b]) : -INFINITY;
   };
   double scores[kHeld];
 #pragma unroll

@@ -22,9 +22,12 @@ def select(device, logits, scores, beams, count, finished=None, end_token=0, **m
     return ops.beam_select(logits.to(device), torch.as_tensor(np.asarray(scores, np.float32)).to(device), num_beams=beams, count=count, **more)
 
 
-def check(device, logits, scores, beams, count, finished=None, end_token=0, **more):
+def check(device, logits, scores, beams, count, finished=None, end_token=0, near=False, **more):
     """Beams and tokens are the definition's. A score is a number within 2^-36 (1 + |logits|) of the definition's (sums and
-    exponentials to 2^-40, a logarithm, two additions of double numbers), rounded once to float32."""
+    exponentials to 2^-40, a logarithm, two additions of double numbers), rounded once to float32. ``near``: two scores that the
+    definition has within twice 2^-36 (1 + |score|) of each other may come in either order, since each is within that of the exact
+    one (the largest logit is taken from the logit first, which rounds that difference alone): rows with the same sum of
+    exponentials in another order have sums that differ in their last bits."""
     best = select(device, logits, scores, beams, count, finished, end_token, **more)
     got = [x.cpu().numpy() for x in best]
     rows = logits.float().numpy().astype(np.float64)
@@ -32,7 +35,14 @@ def check(device, logits, scores, beams, count, finished=None, end_token=0, **mo
     for g in range(len(rows) // beams):
         at = slice(g * beams, (g + 1) * beams)
         want = select_group(rows[at], scores[at], count, None if finished is None else np.asarray(finished).ravel()[at], end_token)
-        assert [(int(b), int(t)) for b, t in zip(got[1][g], got[2][g])] == [(b, t) for _, b, t in want], f"group {g}"
+        chosen = [(int(b), int(t)) for b, t in zip(got[1][g], got[2][g])]
+        if near:
+            score_of = {(b, t): s for s, b, t in select_group(rows[at], scores[at], 4 * count, None, end_token)}
+            assert len(set(chosen)) == count, f"group {g}"
+            for pair, (score, _, _) in zip(chosen, want):
+                assert abs(score_of[pair] - score) <= 2 * 2.0**-36 * (1 + abs(score)), f"group {g}"
+        else:
+            assert chosen == [(b, t) for _, b, t in want], f"group {g}"
         largest = np.abs(rows[at][np.isfinite(rows[at])]).max(initial=0.0)
         for x, (score, _, _) in zip(got[0][g].astype(np.float64), want):
             assert x == score or abs(x - score) <= 2.0**-24 * abs(score) + 2.0**-36 * (1 + largest), (g, x, score)
@@ -139,6 +149,76 @@ def test_large_and_small_logits_and_far_scores(device):
     row = torch.randn((1, 4000), generator=torch.Generator().manual_seed(5)) * 3
     near = torch.cat([row, row + 1.0, row - 3e-7, row * 1.0000002])
     check(device, near, [-50.0, -50.0, -50.0, -50.0], 4, 16)
+
+
+@pytest.mark.parametrize("io", ["float32", "bfloat16"])
+@pytest.mark.parametrize("count", [8, 100, 128])
+def test_plateaus_at_the_last_place(device, io, count):
+    """More equal logits than a list holds, of which the first tokens are taken: above them nothing, some, or all but one."""
+    import torch
+
+    vocab = 20000
+    logits = torch.zeros((6, vocab), dtype=getattr(torch, io))
+    gen = torch.Generator().manual_seed(count)
+    for row, above in enumerate((0, 3, count // 2, count - 1, count, 5000)):
+        at = torch.randperm(vocab, generator=gen)[:above]
+        logits[row, at] = 1 + torch.arange(above).to(logits.dtype) / 64 if above < 5000 else 1.0
+    logits[2, torch.arange(vocab) % 3 == 0] = -1.0
+    for beams in (1, 3, 6):
+        check(device, logits, np.zeros(6), beams, count)
+
+
+@pytest.mark.parametrize("io", ["float32", "bfloat16"])
+@pytest.mark.parametrize("vocab", [200, 3000, 20000])
+def test_many_beams_of_equal_rows(device, io, vocab):
+    """64 beams with the same candidates at equal scores: more than a list holds, by beams and then tokens."""
+    import torch
+
+    row = torch.randn((1, vocab), generator=torch.Generator().manual_seed(vocab)).to(getattr(torch, io))
+    check(device, row.expand(64, -1).contiguous(), np.full(64, -2.0), 64, 128)
+    check(device, torch.zeros((64, vocab), dtype=row.dtype), np.zeros(64), 64, 128)
+    scores = np.full(64, -1.0)
+    scores[5:] = -math.inf  # five of them count
+    check(device, torch.zeros((64, vocab), dtype=row.dtype), scores, 64, 128)
+
+
+@pytest.mark.parametrize("io", ["float32", "bfloat16"])
+def test_one_beam_far_above_the_others(device, io):
+    logits, _ = rows_of(2, 16, 9000, io, 5)
+    scores = np.full(32, -1000.0)
+    scores[3], scores[16:] = 0.0, -math.inf
+    scores[20] = -7.0
+    for count in (16, 32, 128):
+        check(device, logits, scores, 16, count)
+
+
+@pytest.mark.parametrize("io", ["float32", "bfloat16"])
+def test_logits_further_apart_than_exponents(device, io):
+    """A thread's first logits tell it little of its others: rising and falling rows, masked beginnings, one high logit anywhere."""
+    import torch
+
+    dtype = getattr(torch, io)
+    ramp = torch.arange(9000.0)
+    logits = torch.stack([ramp, -ramp, ramp * 1e34, -ramp * 1e34, torch.full((9000,), 2e38), torch.full((9000,), -2e38), ramp % 2 * 5e3, ramp % 7 * -3e3]).to(dtype)
+    check(device, logits, np.zeros(8), 2, 4, near=True)
+    masked = torch.full((4, 9000), -math.inf, dtype=dtype)
+    for row, (every, value) in enumerate(((16, 3000.0), (32, -3000.0), (8191, 1e30), (8192, -1e30))):
+        masked[row, every - 1 :: every] = value
+    check(device, masked, np.zeros(4), 1, 1)
+    check(device, masked, np.zeros(4), 2, 3)
+    high, _ = rows_of(3, 8, 9000, io, 9)
+    for row in range(24):
+        high[row, row * 373 + 5] = 4000.0 + row
+    check(device, high, np.linspace(0, -1, 24), 8, 8)
+
+
+@pytest.mark.parametrize("io", ["float32", "bfloat16"])
+@pytest.mark.parametrize("vocab", [5, 2048, 9000])
+def test_one_bad_logit_anywhere(device, io, vocab):
+    logits, scores = rows_of(3, 8, vocab, io, vocab)
+    for row in range(0, 24, 2):
+        logits[row, row * 7919 % vocab] = (math.nan, math.inf)[row // 2 % 2]
+    check(device, logits, scores, 8, 8)
 
 
 def test_rows_with_strides_and_given_buffers(device):
@@ -286,6 +366,15 @@ def test_blocks_of_many_sizes_and_alignments(device, size):
         view.copy_(states[0])
         check_reorder(device, tables, parents, contexts, states, 4, given=[view])
         assert not flat[:shift].any() and not flat[shift + states[0].numel() :].any()
+
+
+@pytest.mark.parametrize("sizes", [(64, 4, 16, 1, 1000, 48, 7, 2048), (3, 5), (256, 257), (4096, 4096, 4, 4), (4096, 4112, 4, 4)])
+def test_states_of_different_sizes(device, sizes):
+    """Blocks that a wavefront moves by itself, and one byte more than those."""
+    rng = np.random.default_rng(3)
+    contexts = rng.integers(1, 40, 9)
+    tables, states = beams_of(9, 4, 8, 12, tuple(range(1, len(sizes) + 1)), sizes, contexts, 3)
+    check_reorder(device, tables, rng.integers(0, 4, (9, 4)), contexts, states, 8)
 
 
 def test_a_cache_of_codes_and_scales(device):

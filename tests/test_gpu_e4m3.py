@@ -318,6 +318,26 @@ def test_mixed_batches_and_block_sizes(device, io, block):
 
 
 @pytest.mark.parametrize("io", IO)
+@pytest.mark.parametrize("heads,kv_heads,dim", [(2, 2, 128), (8, 2, 64), (4, 1, 32), (16, 2, 256)])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (7, 2)])
+def test_short_runs_that_share_a_tile(device, io, heads, kv_heads, dim, window, sinks):
+    rng = np.random.default_rng(heads)
+    for most in (4, 5, 9, 27):
+        runs = [(n, n + int(rng.integers(0, 40))) for n in rng.integers(1, most + 1, 12).tolist() + [most] * 3]
+        check(device, make(runs, heads, kv_heads, dim, 16, io, seed=most), window, sinks, max_query_len=most)
+
+
+@pytest.mark.parametrize("io", IO)
+@pytest.mark.parametrize("dim", [32, 64, 128, 256])
+@pytest.mark.parametrize("block", [16, 48])
+def test_whole_pages_beside_runs(device, io, dim, block):
+    """Rows by themselves of every length around a page, beside runs; in some splits they have no key."""
+    runs = [(1, n) for n in (1, 15, 16, 17, 31, 32, 33, 47, 48, 49, 500)] + [(40, 60), (1, 0), (5, 300), (1, 129)]
+    for splits in (0, 1, 5):
+        check(device, make(runs, 6, 2, dim, block, io, seed=block + splits), num_splits=splits)
+
+
+@pytest.mark.parametrize("io", IO)
 @pytest.mark.parametrize("splits", [1, 2, 3, 7, 64])
 def test_splits_agree_with_the_definition(device, io, splits):
     d = make([(1, 700), (1, 3), (40, 500), (1, 129)], 8, 2, 128, 16, io, seed=splits)
