@@ -2104,7 +2104,7 @@ Plan codes_plan(const pkv_window& g) {
       // The rows by themselves, a sequence each at most, have the tiles' splits, and fill the GPU with fewer. 20 rows of 2481 to 2853 keys
       // beside a run of 10, 32/8 heads x 128, bfloat16, with 1, 3, 8, 22: 44, 39, 52, 81; 64 rows of 100 to 4000 beside 512, with 1, 3: 104,
       // 115; 61 of 64 beside a run of 6 with 1503, 16/8 heads x 64, float32, with 1, 3, 8: 65, 33, 48.
-      const int64_t rows_fill = std::max<int64_t>(groups <= 64 ? 3 : 1, 512 / std::max<int64_t>(1, static_cast<int64_t>(g.num_seqs) * g.num_kv_heads));
+      const int64_t rows_fill = std::max(std::min<int64_t>(3, 256 / groups), 512 / std::max<int64_t>(1, static_cast<int64_t>(g.num_seqs) * g.num_kv_heads));
       p.splits = static_cast<int32_t>(std::max<int64_t>(1, std::min({int64_t{PKV_WINDOW_MAX_SPLITS}, shares, tiles, rows_fill})));
       p.bytes = pkv_window_workspace_bytes(g.num_queries, g.num_heads, g.head_dim, g.max_query_len, p.splits);
     }
