@@ -362,12 +362,12 @@ __device__ __forceinline__ Words<N> load_words(const void* p) {
 // kOrder: also the aligned blocks in the order of the keys that their rows see (three rows of a block speak for it), the most first, for
 // as many blocks as the workgroup has threads. The tiles' workgroups then end together: 8 x 512 rows behind up to 2048 others,
 // 32/8 heads x 128 over e4m3 codes, 250 -> 208 us.
-constexpr int kListThreads = 1024;
+constexpr int kListThreads = 1024;  // the order's keys hold a block's number in ten bits
 template <bool kOrder>
 __global__ __launch_bounds__(kListThreads) void list_kernel(const Window a) {
   __shared__ int32_t s_found;
   if constexpr (kOrder) {
-    __shared__ int32_t s_keys[kListThreads];
+    __shared__ __align__(16) uint32_t s_keys[kListThreads];  // keys, then the block's number from behind: no two alike
     const int32_t blocks = static_cast<int32_t>((a.num_queries + a.tile_rows - 1) / a.tile_rows), b = threadIdx.x;
     int32_t keys = 0;
     if (b < blocks) {
@@ -379,16 +379,24 @@ __global__ __launch_bounds__(kListThreads) void list_kernel(const Window a) {
         if (seq >= 0 && seq < a.num_seqs) keys = max(keys, span_of(a, seq, a.positions[at[i]]).count());
       }
     }
-    s_keys[b] = keys;
+    const uint32_t mine = b < blocks ? static_cast<uint32_t>(min(keys, (1 << 22) - 1)) << 10 | (kListThreads - 1 - b) : 0;
+    s_keys[b] = mine;
+    if (threadIdx.x == 0) s_found = 0;
     __syncthreads();
-    if (b < blocks) {
+    if (b < blocks) {  // the other wavefronts go on
       int32_t place = 0;
-      for (int32_t j = 0; j < blocks; ++j) place += s_keys[j] > keys || (s_keys[j] == keys && j < b) ? 1 : 0;
+#pragma unroll 4
+      for (int32_t j = 0; j < blocks; j += 4) {
+        const u32x4 four = *reinterpret_cast<const u32x4*>(s_keys + j);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) place += four[e] > mine ? 1 : 0;
+      }
       a.order[place] = b;
     }
+  } else {
+    if (threadIdx.x == 0) s_found = 0;
+    __syncthreads();
   }
-  if (threadIdx.x == 0) s_found = 0;
-  __syncthreads();
   const int lane = threadIdx.x & (kWave - 1);
   for (int64_t start = threadIdx.x - lane; start < a.num_queries; start += kListThreads) {
     const int64_t t = min(start + lane, a.num_queries - 1);
