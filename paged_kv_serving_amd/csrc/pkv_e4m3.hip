@@ -53,6 +53,39 @@ __device__ __forceinline__ Eight load_eight(const uint16_t* p, bool aligned) {
   return x;
 }
 
+// The same as they are stored, to be held in fewer registers.
+template <typename T>
+struct Stored {
+  u32x4 w[sizeof(T) / 2];
+};
+template <typename T>
+__device__ __forceinline__ Stored<T> load_stored(const T* p, bool aligned) {
+  Stored<T> x;
+  if (aligned) {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) x.w[i] = reinterpret_cast<const u32x4*>(p)[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2 * static_cast<int>(sizeof(T)); ++i) {
+      if constexpr (sizeof(T) == 4) x.w[i / 4][i % 4] = __float_as_uint(p[i]);
+      else x.w[0][i] = p[2 * i] | static_cast<uint32_t>(p[2 * i + 1]) << 16;
+    }
+  }
+  return x;
+}
+__device__ __forceinline__ Eight eight_of(const Stored<float>& s) {
+  Eight x;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x.v[i] = __uint_as_float(s.w[i / 4][i % 4]);
+  return x;
+}
+__device__ __forceinline__ Eight eight_of(const Stored<uint16_t>& s) {
+  Eight x;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x.v[2 * i] = bf16_lo(s.w[0][i]), x.v[2 * i + 1] = bf16_hi(s.w[0][i]);
+  return x;
+}
+
 // The codes of eight values times a power of two, rounded to nearest, ties to even. What is not finite becomes NaN.
 __device__ __forceinline__ u32x2 codes_of(const float (&v)[8], float times) {
   u32x2 w;
@@ -103,9 +136,12 @@ __device__ __forceinline__ float finite_size(float x) {
 // The tokens of one block that stand next to each other in the call (a run), of one head, keys or values: D / 8 lanes to a
 // row. Their largest magnitude gives the scale; where the block has tokens before them and its scale has to grow, their
 // codes are scaled down. No two wavefronts write the same block and head, so nothing waits for another. Here a run of more
-// than kHeld tokens, read twice, the second time from the caches.
+// than kHeld tokens. Where blocks have more, kLong tokens (32 or 64) are held as they are stored, in registers that would cost a kernel of small
+// blocks its wavefronts; longer runs are read twice, the second time from the caches. 16 x 512 tokens of 32 heads x 128,
+// bfloat16, in blocks of 64: 51 us, read twice 66; 8 x 512, float32, in blocks of 32 with kLong 32 and 64: 34 and 53, of 64: 47
+// and 38.
 // ---------------------------------------------------------------------------------------------
-template <typename T, int D>
+template <typename T, int D, int kLong>
 __device__ void append_run(const Append& a, int which, int32_t head, int64_t t0, int32_t block) {
   constexpr int kLanes = D / 8, kRows = kWave / kLanes, kSteps = kHeld / kRows;
   const int lane = threadIdx.x & (kWave - 1), row = lane / kLanes, d = lane % kLanes * 8;
@@ -132,8 +168,41 @@ __device__ void append_run(const Append& a, int which, int32_t head, int64_t t0,
   const int64_t block0 = static_cast<int64_t>(block) * a.block_size;
   const int32_t before = static_cast<int32_t>(low - block0);  // tokens that the block keeps
 
-  Eight x[kSteps];
   float most = 0.f;
+  const auto look = [&](const Eight& one) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) most = fmaxf(most, finite_size(one.v[e]));
+  };
+  float times;
+  const auto settle = [&]() {  // the scale, and the codes of the tokens before
+    for (int m = kWave / 2; m > 0; m >>= 1) most = fmaxf(most, __shfl_xor(most, m));
+    float scale = scale_for(most);
+    if (before > 0) {
+      scale = fmaxf(scale, held_scale);
+      if (scale != held_scale) scale_down<D>(pool - d + block0 * row_bytes, row_bytes, before, held_scale / scale);
+    }
+    times = 1.f / scale;
+    if (lane == 0) *scale_at = scale;
+  };
+  if constexpr (kLong > 0) {
+    constexpr int kAll = kLong / kRows;
+    if (end - t0 <= kAll * kRows) {
+      Stored<T> held[kAll];
+#pragma unroll
+      for (int i = 0; i < kAll; ++i) held[i] = load_stored(source + min(t0 + i * kRows + row, end - 1) * a.stride[which], aligned);
+#pragma unroll
+      for (int i = 0; i < kAll; ++i) look(eight_of(held[i]));
+      settle();
+#pragma unroll
+      for (int i = 0; i < kAll; ++i) {
+        asm volatile("" : "+v"(held[i].w[0]));  // widened again, not kept widened
+        const int64_t t = t0 + i * kRows + row;
+        if (t < end) *reinterpret_cast<u32x2*>(pool + a.slots[t] * row_bytes) = codes_of(eight_of(held[i]).v, times);
+      }
+      return;
+    }
+  }
+  Eight x[kSteps];
   const auto load = [&](int64_t from) {
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
@@ -144,18 +213,9 @@ __device__ void append_run(const Append& a, int which, int32_t head, int64_t t0,
   for (int64_t from = t0; from < end; from += kHeld) {
     load(from);
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) most = fmaxf(most, finite_size(x[i].v[e]));
-    }
+    for (int i = 0; i < kSteps; ++i) look(x[i]);
   }
-  for (int m = kWave / 2; m > 0; m >>= 1) most = fmaxf(most, __shfl_xor(most, m));
-  float scale = scale_for(most);
-  if (before > 0) {
-    scale = fmaxf(scale, held_scale);
-    if (scale != held_scale) scale_down<D>(pool - d + block0 * row_bytes, row_bytes, before, held_scale / scale);
-  }
-  const float times = 1.f / scale;
+  settle();
   for (int64_t from = t0; from < end; from += kHeld) {
     load(from);
 #pragma unroll
@@ -164,7 +224,6 @@ __device__ void append_run(const Append& a, int which, int32_t head, int64_t t0,
       if (t < end) *reinterpret_cast<u32x2*>(pool + a.slots[t] * row_bytes) = codes_of(x[i].v, times);
     }
   }
-  if (lane == 0) *scale_at = scale;
 }
 
 // Runs within kHeld tokens from t0 on, all at once: lane j < kHeld speaks for token j. `slot` is the lane's (-1: none),
@@ -232,7 +291,7 @@ __device__ __forceinline__ void append_runs(const Append& a, int which, int32_t 
 // many as end within kHeld tokens: one after the other, the latency of each (2 us) counted.
 // Bound: HBM for long prompts, latency for single tokens. 16 x 512 tokens of 32 heads x 128, bfloat16, in blocks of 16, 201 MB: 43 us,
 // 4.7 TB/s; 64 single tokens of 8 heads x 128 5 us.
-template <typename T, int D>
+template <typename T, int D, int kLong>
 __global__ __launch_bounds__(kThreads) void append_kernel(const Append a) {
   // Items: keys and values of a head, heads, then windows.
   const uint32_t item = __builtin_amdgcn_readfirstlane(blockIdx.x * (kThreads / kWave) + threadIdx.x / kWave);
@@ -265,7 +324,7 @@ __global__ __launch_bounds__(kThreads) void append_kernel(const Append a) {
     const int most = theirs == 0 ? kHeld : min(kHeld, __builtin_ctzll(theirs));
     const uint64_t ends = changes & ((2ull << most) - 2);
     if (ends == 0) {
-      append_run<T, D>(a, which, head, t0, __builtin_amdgcn_readfirstlane(block));
+      append_run<T, D, kLong>(a, which, head, t0, __builtin_amdgcn_readfirstlane(block));
       t0 += kHeld;  // the next run begins behind
       continue;
     }
@@ -280,15 +339,21 @@ int64_t groups_of(const Append& a) {
   return (items + kThreads / kWave - 1) / (kThreads / kWave);
 }
 
+template <typename T, int D>
+void launch(const Append& a, hipStream_t stream) {
+  const dim3 grid(static_cast<uint32_t>(groups_of(a))), block(kThreads);
+  if (a.block_size <= kHeld) hipLaunchKernelGGL((append_kernel<T, D, 0>), grid, block, 0, stream, a);
+  else if (a.block_size <= 32) hipLaunchKernelGGL((append_kernel<T, D, 32>), grid, block, 0, stream, a);
+  else hipLaunchKernelGGL((append_kernel<T, D, 64>), grid, block, 0, stream, a);
+}
+
 template <typename T>
 int dispatch(const Append& a, int32_t head_dim, hipStream_t stream) {
-  const int64_t groups = groups_of(a);
-  const dim3 grid(static_cast<uint32_t>(groups)), block(kThreads);
   switch (head_dim) {
-    case 32: hipLaunchKernelGGL((append_kernel<T, 32>), grid, block, 0, stream, a); break;
-    case 64: hipLaunchKernelGGL((append_kernel<T, 64>), grid, block, 0, stream, a); break;
-    case 128: hipLaunchKernelGGL((append_kernel<T, 128>), grid, block, 0, stream, a); break;
-    case 256: hipLaunchKernelGGL((append_kernel<T, 256>), grid, block, 0, stream, a); break;
+    case 32: launch<T, 32>(a, stream); break;
+    case 64: launch<T, 64>(a, stream); break;
+    case 128: launch<T, 128>(a, stream); break;
+    case 256: launch<T, 256>(a, stream); break;
     default: return PKV_EUNSUPPORTED;
   }
   return check_launch();

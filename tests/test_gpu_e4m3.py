@@ -88,6 +88,24 @@ def test_appends_of_many_lengths(device, io, dim, block):
 
 
 @pytest.mark.parametrize("io", ["float32", "bfloat16"])
+@pytest.mark.parametrize("dim", [32, 64, 128, 256])
+@pytest.mark.parametrize("block", [17, 32, 64, 65, 200])
+def test_long_runs_of_larger_blocks(device, io, dim, block):
+    """Runs that a wavefront holds, just does not, and reads twice; from rows that are not 16-byte aligned too."""
+    runs = [(n, before) for n in (16, 17, 31, 32, 33, 63, 64, 65, 2 * block + 3) for before in (0, block - 5)] + [(1, 3)] * 4
+    slots, blocks = run_slots(runs, block, dim + block)
+    pools = (*pool_of(blocks, block, 2, dim, 1), *pool_of(blocks, block, 2, dim, 2))
+    keys, values = (tokens_of(slots.size, 2, dim, io, dim + block + i) for i in (0, 1))
+    check_append(device, pools, keys, values, slots)
+    wide = keys.new_zeros((2, slots.size, 2 * dim + 1), device=device)
+    for i, x in enumerate((keys, values)):
+        wide[i, :, 1:] = x.flatten(1)
+    apart = append(device, pools, *(x[:, 1:].unflatten(1, (2, dim)) for x in wide), slots)
+    for a, b in zip(apart, append(device, pools, keys.to(device), values.to(device), slots)):
+        np.testing.assert_array_equal(a, b)
+
+
+@pytest.mark.parametrize("io", ["float32", "bfloat16"])
 def test_many_tokens_and_heads(device, io):
     """More tokens than one wavefront looks at, runs that lie across its window's ends."""
     runs = [(1, b) for b in range(60)] + [(301, 9), (512, 0), (300, 31)] + [(1, b) for b in range(30)]
