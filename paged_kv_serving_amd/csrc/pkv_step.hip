@@ -32,7 +32,7 @@ __device__ __forceinline__ uint64_t inclusive_sums(uint64_t x, uint64_t* s_wave)
 // needs by itself, kThreads requests at a time, which costs less than a launch of its own for the sums, and finds the
 // requests of its own rows by bisection. A new block's table entry is written by the row at its first place, which lies
 // among the call's rows; no row reads an entry that another writes. The first workgroup writes what is one value a request.
-// Bound: latency (a few dependent loads and the sums).
+// Bound: latency (a few dependent loads and the sums). 64 requests of a token 3.9 us, 282 requests with 16,634 rows 4.3.
 // ---------------------------------------------------------------------------------------------
 __global__ __launch_bounds__(kThreads) void step_kernel(const pkv_step a) {
   __shared__ uint64_t s_wave[2][kWaves];
