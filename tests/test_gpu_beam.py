@@ -262,6 +262,39 @@ def test_a_row_does_not_depend_on_the_batch(device):
     assert all(torch.equal(a, b) for a, b in zip(whole, again))
 
 
+def test_two_streams_at_once_and_a_replayed_graph(device):
+    import torch
+
+    from paged_kv_serving_amd import ops
+
+    both = []
+    for seed, (groups, beams, vocab, io) in enumerate(((3, 4, 30000, "float32"), (40, 8, 9001, "bfloat16"))):
+        logits, scores = rows_of(groups, beams, vocab, io, seed)
+        both.append((logits.to(device), torch.as_tensor(scores, dtype=torch.float32).to(device), beams))
+    want = [ops.beam_select(x, s, num_beams=b, count=2 * b) for x, s, b in both]
+    streams = [torch.cuda.Stream(device) for _ in both]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i, (x, s, b) in enumerate(both):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(ops.beam_select(x, s, num_beams=b, count=2 * b))
+    torch.cuda.synchronize()
+    for results, expected in zip(got, want):
+        for result in results:
+            assert all(torch.equal(a, e) for a, e in zip(result, expected))
+    x, s, b = both[0]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = ops.beam_select(x, s, num_beams=b, count=2 * b)
+    for step in range(4):
+        x.copy_(x.roll(step, 1) * (1 + step))
+        s.sub_(float(step))
+        graph.replay()
+        eager = ops.beam_select(x, s, num_beams=b, count=2 * b)
+        assert all(torch.equal(a, e) for a, e in zip(held, eager))
+
+
 def test_select_refusals(device):
     import torch
 

@@ -450,6 +450,79 @@ def test_a_nan_reaches_the_rows_and_dimensions_that_see_it(device, io, splits):
 
 
 @pytest.mark.parametrize("io", IO)
+@pytest.mark.parametrize("dim", [32, 128, 256])
+@pytest.mark.parametrize("splits", [1, 4])
+def test_nan_codes_of_every_head_dim(device, io, dim, splits):
+    """Rows by themselves over whole pages and runs, in one call: hidden NaN codes reach nobody, seen ones those who see them."""
+    d = make([(1, 60), (20, 60), (1, 200), (7, 33)], 6, 2, dim, 16, io, seed=dim)
+    clean = call(device, d, num_splits=splits).float().cpu().numpy()
+    for s, end in ((0, 60), (1, 60), (2, 200), (3, 33)):
+        for name in ("k", "v"):
+            d[name][d["tables"][s, end // 16], end % 16 :] = np.nan
+    np.testing.assert_array_equal(call(device, d, num_splits=splits).float().cpu().numpy(), clean)
+    for s in range(4):
+        d["v"][d["tables"][s, 1], 9, 1, 5] = np.nan  # key 25 of key head 1
+    got = call(device, d, num_splits=splits).float().cpu().numpy()
+    sees = d["positions"] >= 25
+    assert np.isnan(got[sees][:, 3:, 5]).all()
+    want, size = window_attention(d["q"].float().numpy(), d["positions"], d["seqs"], e4m3.values(d["k"], d["ks"]), np.nan_to_num(e4m3.values(d["v"], d["vs"])),
+                                  d["tables"], d["contexts"], d["scale"], CAUSAL, 0)  # fmt: skip
+    off = bound(d, want, size)
+    got[:, 3:, 5] = clean[:, 3:, 5]
+    assert (np.abs(got - clean) <= 2 * off).all()
+
+
+def test_mixed_calls_captured_and_replayed_with_another_batch(device):
+    """Tiles with shared runs, listed rows by pages, the order and the join in a graph whose lengths change between replays."""
+    import torch
+
+    from paged_kv_serving_amd import ops
+
+    for io in IO:
+        batches = [make([(n, n + more) for n, more in runs], 8, 2, 128, 16, io, seed=i) for i, runs in enumerate((
+            [(9, 5), (1, 500), (1, 31), (27, 200), (1, 16), (25, 0)], [(1, 100), (30, 0), (1, 7), (1, 0), (21, 477), (10, 30)], [(10, 0)] * 6))]  # fmt: skip
+        rows, blocks, width = 64, max(b["k"].shape[0] for b in batches), max(b["tables"].shape[1] for b in batches)
+
+        def padded(d):
+            n = d["seqs"].size
+            pool = np.zeros((2, blocks, 16, 2, 128))
+            scales = np.ones((2, blocks, 2), np.float32)
+            for i, name in enumerate(("k", "v")):
+                pool[i, : d[name].shape[0]], scales[i, : d[name].shape[0]] = d[name], d[name + "s"]
+            tables = np.full((6, width), -1, np.int32)
+            tables[:, : d["tables"].shape[1]] = d["tables"]
+            q = torch.zeros((rows, 8, 128), dtype=d["q"].dtype)
+            q[:n] = d["q"]
+            return [q, torch.from_numpy(np.pad(d["positions"], (0, rows - n))), torch.from_numpy(np.pad(d["seqs"], (0, rows - n), constant_values=-1)),
+                    codes_of(pool[0]), codes_of(pool[1]), *map(torch.from_numpy, scales), torch.from_numpy(tables), torch.from_numpy(d["contexts"])]  # fmt: skip
+
+        assert all(b["seqs"].size <= rows for b in batches)
+        held = [x.to(device) for x in padded(batches[0])]
+        out = torch.zeros((rows, 8, 128), dtype=held[0].dtype, device=device)
+
+        def run(result):
+            return ops.paged_attention_e4m3(*held, 128**-0.5, max_context_len=512, max_query_len=30, out=result)
+
+        run(out)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            run(out)
+        for d in batches + batches[::-1]:
+            for a, b in zip(held, padded(d)):
+                a.view(torch.uint8).copy_(b.view(torch.uint8)) if a.dtype == torch.float8_e4m3fn else a.copy_(b)
+            out.fill_(7.0)
+            graph.replay()
+            eager = run(torch.full_like(out, 7.0))
+            assert torch.equal(out, eager)
+            n = d["seqs"].size
+            assert (out[n:] == 7.0).all()  # padding is left as it was
+            want, size = window_attention(d["q"].float().numpy(), d["positions"], d["seqs"], e4m3.values(d["k"], d["ks"]), e4m3.values(d["v"], d["vs"]),
+                                          d["tables"], d["contexts"], d["scale"], CAUSAL, 0)  # fmt: skip
+            assert (np.abs(out[:n].float().cpu().numpy().astype(np.float64) - want) <= bound(d, want, size)).all()
+
+
+@pytest.mark.parametrize("io", IO)
 def test_blocks_outside_the_pool_are_skipped(device, io):
     d = make([(1, 100), (40, 100), (1, 20)], 4, 2, 64, 16, io)
     d["tables"][0, 3], d["tables"][1, 2], d["tables"][1, 5], d["tables"][2, :2] = -1, 10**6, -5, 2**31 - 1
