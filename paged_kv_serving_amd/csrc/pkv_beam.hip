@@ -108,12 +108,12 @@ __device__ __forceinline__ bool looked_at(const pkv_beam& g, int64_t row) {
 // least `count` logits reach, and few more: 8192 of them and 8 classes list about 23. Classes of lanes rather than neighbours:
 // a row's last chunk, which has numbers for the first threads alone, leaves no class empty. Each one's place is the number of
 // larger ones. Where too many reach it (128 classes: about 700; equal logits), bisection finds a number that fewer do.
-// 32 groups of 8 beams over 128256 float32 logits: about 35 us for 115 MB. Bound by the vector units at 22 us of it, the
+// 32 groups of 8 beams over 128256 float32 logits: about 36 us for 115 MB. Bound by the vector units at 22 us of it, the
 // exponentials' 17 operations being two thirds of them, which the reads of 18 us overlap with in part; the kernel takes 21 us
 // without them. Half the bytes (bf16) take the same time. 7 wavefronts on a SIMD take 1.3 us less than the 5 of 88 registers.
 template <typename T, int kPer>
 __global__ __launch_bounds__(kThreads, 7) void chunk_kernel(const Select a) {
-  constexpr int kVec = 16 / sizeof(T), kLoads = kPer / kVec;
+  constexpr int kVec = 16 / sizeof(T), kLoads = kPer / kVec, kAhead = kLoads < 3 ? kLoads : 3;
   __shared__ uint64_t s_list[kWaves][kCapacity];  // a wavefront's own, so that no place needs an atomic
   __shared__ float s_top[kWaves][kWave];
   __shared__ double s_sum[kWaves];
@@ -130,6 +130,8 @@ __global__ __launch_bounds__(kThreads, 7) void chunk_kernel(const Select a) {
 
   const auto token = [&](int i) { return first + i / kVec * (kThreads * kVec) + i % kVec; };
 
+  // A thread asks for four loads at a time: with all eight, every workgroup's numbers arrive at about the same time, when the
+  // vector units have waited long (32 x 8 beams, both kernels: 50 us, with two, four and five loads 46).
   // The exponentials are taken as the numbers arrive, against the largest of the thread's first ones: double precision holds those
   // of numbers 600 above and below it, and where a thread has others it starts again, against its largest.
   float x[kPer], top, base;
@@ -137,32 +139,38 @@ __global__ __launch_bounds__(kThreads, 7) void chunk_kernel(const Select a) {
   const auto add = [&](int i, double from) { sum += exp_of(static_cast<double>(x[i]) - from); };
   const auto take = [&](auto whole) {
     u32x4 v[kLoads];
-    if constexpr (whole) {
+    const auto ask = [&](int i) {
+      if constexpr (whole) v[i] = __builtin_nontemporal_load(reinterpret_cast<const Vec*>(p + token(i * kVec)));
+    };
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) v[i] = __builtin_nontemporal_load(reinterpret_cast<const Vec*>(p + token(i * kVec)));
-    }
+    for (int i = 0; i < kAhead; ++i) ask(i);
+    if constexpr (!whole) {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      if constexpr (!whole) {
+      for (int i = 0; i < kPer; ++i) {
         const T one = p[min(token(i), vocab - 1)];
         if constexpr (sizeof(T) == 4) x[i] = one;
         else x[i] = __uint_as_float(static_cast<uint32_t>(one) << 16);
         if (token(i) >= vocab) x[i] = -INFINITY;
-      } else {
-        if constexpr (sizeof(T) == 4) x[i] = __uint_as_float(v[i / 4][i % 4]);
-        else x[i] = i % 2 == 0 ? bf16_lo(v[i / 8][i % 8 / 2]) : bf16_hi(v[i / 8][i % 8 / 2]);
       }
     }
-    top = x[0];
 #pragma unroll
-    for (int i = 1; i < kVec; ++i) top = maximum(top, x[i]);
-    base = fabsf(top) < INFINITY ? top : 0.f;
-    const double from = base;
+    for (int j = 0; j < kLoads; ++j) {
+      if (j + kAhead < kLoads) ask(j + kAhead);
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (whole) {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      if (i >= kVec) top = maximum(top, x[i]);
-      add(i, from);
-      if (i % kVec == kVec - 1) __builtin_amdgcn_sched_barrier(0);  // a load's numbers are used before the next load's are waited for
+        for (int e = 0; e < kVec; ++e) {
+          if constexpr (sizeof(T) == 4) x[j * kVec + e] = __uint_as_float(v[j][e]);
+          else x[j * kVec + e] = e % 2 == 0 ? bf16_lo(v[j][e / 2]) : bf16_hi(v[j][e / 2]);
+        }
+      }
+#pragma unroll
+      for (int i = j * kVec; i < (j + 1) * kVec; ++i) top = i == 0 ? x[0] : maximum(top, x[i]);
+      if (j == 0) base = fabsf(top) < INFINITY ? top : 0.f;
+      const double from = base;
+#pragma unroll
+      for (int i = j * kVec; i < (j + 1) * kVec; ++i) add(i, from);
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
   if ((chunk + 1) * (kThreads * kPer) <= vocab) take(std::true_type{});
