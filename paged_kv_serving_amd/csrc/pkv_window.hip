@@ -2121,7 +2121,11 @@ Plan codes_plan(const pkv_window& g) {
     // keys, 8/2 heads x 128, float32: 26 us and 42.
     const int64_t rows = kTileQueries / group, groups = (g.num_queries + rows - 1) / rows * g.num_kv_heads * p.splits;
     const int64_t longest = g.max_query_len > 0 ? g.max_query_len : g.num_queries;
-    p.run_shares = static_cast<uint32_t>(std::max<int64_t>(1, std::min({int64_t{8}, 256 / groups, (2 * rows + longest - 1) / longest})));
+    // Of longer runs a tile may still hold the end of one and the start of the next: two workgroups for it, one of them mostly without
+    // any, cost what their look does (7 x 211 rows, 16/8 heads x 32, float32: 25 us, with one 35; 2 x 465 rows beside 15, 8/1 heads x
+    // 128, bfloat16, 240 workgroups: 42 and 34).
+    const int64_t least = g.num_seqs > 1 && groups <= (g.q_dtype == PKV_F32 ? 256 : 192) ? 2 : 1;
+    p.run_shares = static_cast<uint32_t>(std::max(least, std::min({int64_t{8}, 256 / groups, (2 * rows + longest - 1) / longest})));
     p.order_bytes = (ordered_blocks(g.num_queries, group) + 3) / 4 * 16;
     p.bytes += p.order_bytes;
     return p;
