@@ -182,6 +182,9 @@ __global__ __launch_bounds__(kThreads, 7) void chunk_kernel(const Select a) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) add(i, from);
   }
+  // Without a number above -inf (masked, or behind the row's end) a thread adds nothing: its exponentials of -inf are e^-690, and what
+  // they would be multiplied by below, e^-(the chunk's largest), may be anything.
+  const bool counts = top > -INFINITY;
   int classes = 1;
   while (classes < kWave && classes < g.count) classes *= 2;
   for (int m = kWave / 2; m >= classes; m /= 2) top = maximum(top, __shfl_xor(top, m));
@@ -204,7 +207,8 @@ __global__ __launch_bounds__(kThreads, 7) void chunk_kernel(const Select a) {
     return;
   }
 
-  sum *= exp_of(static_cast<double>(base) - static_cast<double>(top));
+  // Of others `base` is their first largest, no more than `top`, or 0 and within 600 of their own: exp_of's range.
+  sum = counts ? sum * exp_of(static_cast<double>(base) - static_cast<double>(top)) : 0.0;
   for (int m = kWave / 2; m > 0; m >>= 1) sum += __shfl_xor(sum, m);
   if (lane == 0) s_sum[wave] = sum;
 

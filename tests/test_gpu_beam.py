@@ -213,6 +213,30 @@ def test_logits_further_apart_than_exponents(device, io):
 
 
 @pytest.mark.parametrize("io", ["float32", "bfloat16"])
+@pytest.mark.parametrize("level", [-600.0, -655.0, -690.0, -700.0, -709.0, -709.8, -711.0, -1000.0, -2110.0, -2120.0, -2130.0, -3549.0, -4970.0])
+def test_rows_far_below_zero(device, io, level):
+    """A thread without a finite logit (behind the vocabulary's end, or masked) adds nothing, wherever the others lie."""
+    import torch
+
+    dtype = getattr(torch, io)
+    for vocab in (200, 1000, 2049, 9001):
+        logits, scores = rows_of(2, 4, vocab, "float32", vocab)
+        check(device, (logits + level).to(dtype), scores, 4, 8)
+        masked = torch.full(logits.shape, -math.inf)
+        for row in range(8):  # some tokens of the row, or a stretch
+            at = torch.arange(vocab) % 37 == row if row % 2 else (torch.arange(vocab) >= 20 * row) & (torch.arange(vocab) < 20 * row + 40)
+            masked[row, at] = logits[row, at] + level
+        check(device, masked.to(dtype), scores, 4, 8)
+    # Ordinary rows, of which one chunk or the last numbers hold such logits alone, with and without masked ones between.
+    for vocab in (2060, 9001):
+        logits, scores = rows_of(2, 4, vocab, "float32", vocab)
+        logits[::2, 2048:] += level
+        logits[1::2, -12:] += level
+        logits[2:4, 2050::3] = -math.inf
+        check(device, logits.to(dtype), scores, 4, 8)
+
+
+@pytest.mark.parametrize("io", ["float32", "bfloat16"])
 @pytest.mark.parametrize("vocab", [5, 2048, 9000])
 def test_one_bad_logit_anywhere(device, io, vocab):
     logits, scores = rows_of(3, 8, vocab, io, vocab)
