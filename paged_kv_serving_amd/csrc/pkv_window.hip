@@ -2097,6 +2097,8 @@ Plan codes_plan(const pkv_window& g) {
   p.pages = g.window == INT32_MAX && g.block_size % 16 == 0 && g.block_size <= 1024 && g.num_blocks > 0 && g.num_kv_heads <= (1 << 18);
   p.runs = has_runs(g.max_query_len, group);
   if (p.runs) {
+    // Tiles of one split: one at least, as a workspace may be asked for without queries.
+    const int64_t rows = kTileQueries / group, groups = std::max<int64_t>(1, (g.num_queries + rows - 1) / rows * g.num_kv_heads);
     p.bytes = pkv_window_workspace_bytes(g.num_queries, g.num_heads, g.head_dim, g.max_query_len, p.splits);
     if (g.num_splits == 0) {
       // Tiles of bfloat16 queries are two to a CU, of float32 ones one. Shares of 384 keys at least, of 128 where tiles are few: a part
@@ -2105,7 +2107,6 @@ Plan codes_plan(const pkv_window& g) {
       // 1032 keys, 16/2 heads x 64, bfloat16, with 2, 4, 8: 19, 15, 15; 3 x 339 rows of up to 610 keys, 8/1 heads x 64, float32 (64 tiles),
       // with 1, 2, 4, 8: 49, 39, 34, 34; 1 x 512 rows, 8 heads x 128, bfloat16 (32 tiles): 36, 30, 27, 27; 7 x 130 rows of 226 keys, 16/4
       // heads x 256 (116 tiles): 51, 51, 62, 94.
-      const int64_t rows = kTileQueries / group, groups = (g.num_queries + rows - 1) / rows * g.num_kv_heads;
       const int64_t longest = std::min<int64_t>(g.max_context_len, static_cast<int64_t>(g.window) + g.sinks);
       const int64_t shares = groups <= 64 ? std::min(longest / 128, std::max<int64_t>(8, longest / 1024)) : longest / 384;
       const int64_t tiles = (g.q_dtype == PKV_F32 || (groups > 16 && groups <= 64) ? 256 : 512) / groups;
@@ -2119,13 +2120,12 @@ Plan codes_plan(const pkv_window& g) {
     // A tile's runs one after the other cost their latencies; where tiles are few and runs surely shorter than they are, several
     // workgroups share them. 6 x 27 rows, 8 heads x 128, bfloat16: 18 us, in one workgroup each 54; 2 x 12 rows of up to 1191
     // keys, 8/2 heads x 128, float32: 26 us and 42.
-    const int64_t rows = kTileQueries / group, groups = (g.num_queries + rows - 1) / rows * g.num_kv_heads * p.splits;
-    const int64_t longest = g.max_query_len > 0 ? g.max_query_len : g.num_queries;
+    const int64_t parts = groups * p.splits, longest = g.max_query_len;
     // Of longer runs a tile may still hold the end of one and the start of the next: two workgroups for it, one of them mostly without
     // any, cost what their look does (7 x 211 rows, 16/8 heads x 32, float32: 25 us, with one 35; 2 x 465 rows beside 15, 8/1 heads x
     // 128, bfloat16, 240 workgroups: 42 and 34).
-    const int64_t least = g.num_seqs > 1 && groups <= (g.q_dtype == PKV_F32 ? 256 : 192) ? 2 : 1;
-    p.run_shares = static_cast<uint32_t>(std::max(least, std::min({int64_t{8}, 256 / groups, (2 * rows + longest - 1) / longest})));
+    const int64_t least = g.num_seqs > 1 && parts <= (g.q_dtype == PKV_F32 ? 256 : 192) ? 2 : 1;
+    p.run_shares = static_cast<uint32_t>(std::max(least, std::min({int64_t{8}, 256 / parts, (2 * rows + longest - 1) / longest})));
     p.order_bytes = (ordered_blocks(g.num_queries, group) + 3) / 4 * 16;
     p.bytes += p.order_bytes;
     return p;

@@ -105,6 +105,25 @@ def test_the_attentions_workspace(lib) -> None:
     assert lib.pkv_attention_e4m3_workspace_bytes(None) == EINVAL
 
 
+@pytest.mark.parametrize("q_dtype", [0, 1])
+@pytest.mark.parametrize("num_splits", [0, 1, 2])
+def test_the_workspace_of_a_call_without_queries(lib, q_dtype, num_splits) -> None:
+    """A plan without rows, whatever their runs would be: what windowed attention needs, and no division by no tiles."""
+    from paged_kv_serving_amd import ops
+
+    kind, size = structure("pkv_e4m3_attention"), ctypes.c_int64()
+    for max_query_len in (0, 1, 4, 512, (1 << 31) - 1):
+        for heads, window, num_seqs in ((8, 100, 0), (64, (1 << 31) - 1, 4), (128, 8, 1)):
+            args = kind()
+            more = dict(num_queries=0, q_dtype=q_dtype, num_splits=num_splits, max_query_len=max_query_len, num_heads=heads, window=window, sinks=0, num_seqs=num_seqs)
+            for name, value in {**ATTENTION, **more}.items():
+                setattr(args, name, value)
+            sizes = (0, heads, 2, 64, q_dtype, window, 0, 160, max_query_len, num_splits)
+            assert lib.pkv_window_sizes(*sizes, ctypes.addressof(size)) >= 1
+            assert lib.pkv_attention_e4m3_workspace_bytes(ctypes.addressof(args)) == size.value
+        assert ops.e4m3_workspace_bytes(0, 8, 2, 64, block_size=16, max_context_len=160, max_query_len=max_query_len, num_splits=num_splits) == size.value
+
+
 def test_no_arguments_and_nothing_to_do(lib) -> None:
     for function in (lib.pkv_append_e4m3, lib.pkv_attention_e4m3):
         assert function(None, 0, None) == EINVAL
