@@ -152,6 +152,9 @@ __device__ __forceinline__ int64_t scale_of(const Window& a, int32_t slot, int32
   return static_cast<int64_t>(static_cast<uint32_t>(slot) / static_cast<uint32_t>(a.block_size)) * a.num_kv_heads + kv_head;
 }
 
+// The power of two that a scale stands for: its exponent, which is all that the conversion below looks at.
+__device__ __forceinline__ float power_of(float scale) { return __uint_as_float(__float_as_uint(scale) & 0x7f800000u); }
+
 // Codes 0 and 1 of a word, or 2 and 3, as bfloat16 numbers times a power of two.
 template <int kHalf>
 __device__ __forceinline__ uint32_t widen(uint32_t codes, float scale) {
@@ -241,7 +244,7 @@ __device__ __forceinline__ void exact_row(const Window& a, int64_t t, int32_t he
       score = 0.f;
       for (int d = 0; d < D; ++d) score += load_one(q + d) * load_one(k + d);
       score *= a.given_scale;
-      if constexpr (sizeof(KVT) == 1) score *= a.key_scales[scale_of(a, slot, kv_head)];
+      if constexpr (sizeof(KVT) == 1) score *= power_of(a.key_scales[scale_of(a, slot, kv_head)]);
     }
     const uint64_t seen = __ballot(slot >= 0);
     if (seen == 0) continue;
@@ -262,7 +265,7 @@ __device__ __forceinline__ void exact_row(const Window& a, int64_t t, int32_t he
       float pj = __shfl(p, j);
       const int32_t from_slot = __shfl(slot, j);
       const KVT* v = static_cast<const KVT*>(a.values) + row_of(a, from_slot, kv_head, D);
-      if constexpr (sizeof(KVT) == 1) pj *= a.value_scales[scale_of(a, from_slot, kv_head)];
+      if constexpr (sizeof(KVT) == 1) pj *= power_of(a.value_scales[scale_of(a, from_slot, kv_head)]);
       for (int e = 0; e < kOwn; ++e) {
         const int d = e * kWave + lane;
         if (d < D) acc[e] += pj * load_one(v + d);

@@ -472,6 +472,28 @@ def test_nan_codes_of_every_head_dim(device, io, dim, splits):
     assert (np.abs(got - clean) <= 2 * off).all()
 
 
+@pytest.mark.parametrize("io", IO)
+@pytest.mark.parametrize("block", [16, 6])
+@pytest.mark.parametrize("bad", [False, True])
+def test_of_a_scale_its_exponent_alone_counts(device, io, block, bad):
+    """Rows by themselves and runs, and both again where a NaN code has them computed by the definition: the same bits as with the
+    scales' powers of two."""
+    import torch
+
+    d = make([(1, 60), (20, 60), (1, 200), (7, 33)], 6, 2, 64, block, io, seed=8)
+    if bad:
+        for s in range(4):
+            d["v"][d["tables"][s, 25 // block], 25 % block, 1, 5] = np.nan
+    clean = {w: call(device, d, *w).float().cpu() for w in ((None, 0), (24, 3))}
+    rng = np.random.default_rng(3)
+    for name in ("ks", "vs"):
+        d[name] = d[name] * rng.choice([1.0, 1.25, 1.5, 1.9375, -1.0, -1.75], d[name].shape)
+    for w, want in clean.items():
+        got = call(device, d, *w).float().cpu()
+        assert torch.equal(got.isnan(), want.isnan()) and bool(want.isnan().any()) == bad
+        assert torch.equal(got.nan_to_num(), want.nan_to_num())
+
+
 def test_mixed_calls_captured_and_replayed_with_another_batch(device):
     """Tiles with shared runs, listed rows by pages, the order and the join in a graph whose lengths change between replays."""
     import torch
