@@ -152,14 +152,14 @@ __device__ __forceinline__ int64_t scale_of(const Window& a, int32_t slot, int32
   return static_cast<int64_t>(static_cast<uint32_t>(slot) / static_cast<uint32_t>(a.block_size)) * a.num_kv_heads + kv_head;
 }
 
-// The power of two that a scale stands for: its exponent, which is all that the conversion below looks at.
-__device__ __forceinline__ float power_of(float scale) { return __uint_as_float(__float_as_uint(scale) & 0x7f800000u); }
-
 // Codes 0 and 1 of a word, or 2 and 3, as bfloat16 numbers times a power of two.
 template <int kHalf>
 __device__ __forceinline__ uint32_t widen(uint32_t codes, float scale) {
   return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, kHalf != 0));
 }
+
+// The power of two that a scale stands for, as the conversion takes it (its exponent; NaN where that is no number's): code 0x38 is 1.
+__device__ __forceinline__ float power_of(float scale) { return bf16_lo(widen<0>(0x38, scale)); }
 
 // Element offset of a slot's row of one head in the pools.
 __device__ __forceinline__ int64_t row_of(const Window& a, int32_t slot, int32_t kv_head, int d) {

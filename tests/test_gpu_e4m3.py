@@ -494,6 +494,23 @@ def test_of_a_scale_its_exponent_alone_counts(device, io, block, bad):
         assert torch.equal(got.nan_to_num(), want.nan_to_num())
 
 
+@pytest.mark.parametrize("io", IO)
+@pytest.mark.parametrize("block", [16, 6])
+@pytest.mark.parametrize("name", ["ks", "vs"])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+def test_scales_that_are_no_numbers_are_nan_to_those_who_see_them(device, io, block, name, bad):
+    d = make([(1, 60), (20, 60), (1, 200), (7, 33)], 6, 2, 64, block, io, seed=6)
+    clean = call(device, d).float().cpu().numpy()
+    for s in range(4):
+        d[name][d["tables"][s, 25 // block], 1] = bad  # key head 1
+    got = call(device, d).float().cpu().numpy()
+    first = 25 // block * block  # of the block's keys
+    sees = d["positions"] >= first
+    assert np.isnan(got[sees][:, 3:]).all()
+    np.testing.assert_array_equal(got[:, :3], clean[:, :3])
+    np.testing.assert_array_equal(got[~sees], clean[~sees])
+
+
 def test_mixed_calls_captured_and_replayed_with_another_batch(device):
     """Tiles with shared runs, listed rows by pages, the order and the join in a graph whose lengths change between replays."""
     import torch
