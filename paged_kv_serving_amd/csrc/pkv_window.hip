@@ -241,10 +241,16 @@ __device__ __forceinline__ void exact_row(const Window& a, int64_t t, int32_t he
     float score = -INFINITY;
     if (slot >= 0) {
       const KVT* k = static_cast<const KVT*>(a.keys) + row_of(a, slot, kv_head, D);
+      // A query times a code may pass float32's range where the key does not: a scale below 1 comes first, one above it last.
+      float by = 1.f, last_by = 1.f;
+      if constexpr (sizeof(KVT) == 1) {
+        by = power_of(a.key_scales[scale_of(a, slot, kv_head)]);
+        if (!(by < 1.f)) last_by = by, by = 1.f;
+      }
       score = 0.f;
-      for (int d = 0; d < D; ++d) score += load_one(q + d) * load_one(k + d);
+      for (int d = 0; d < D; ++d) score += load_one(q + d) * (sizeof(KVT) == 1 ? load_one(k + d) * by : load_one(k + d));
       score *= a.given_scale;
-      if constexpr (sizeof(KVT) == 1) score *= power_of(a.key_scales[scale_of(a, slot, kv_head)]);
+      if constexpr (sizeof(KVT) == 1) score *= last_by;
     }
     const uint64_t seen = __ballot(slot >= 0);
     if (seen == 0) continue;

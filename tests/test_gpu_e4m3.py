@@ -511,6 +511,28 @@ def test_scales_that_are_no_numbers_are_nan_to_those_who_see_them(device, io, bl
     np.testing.assert_array_equal(got[~sees], clean[~sees])
 
 
+@pytest.mark.parametrize("io", IO)
+@pytest.mark.parametrize("block", [16, 6])
+@pytest.mark.parametrize("splits", [1, 3])
+def test_large_queries_over_small_scales_beside_a_nan(device, io, block, splits):
+    """Products of queries and codes pass float32's range, those of queries and keys do not: 2^120 * 2^8 * 8 against 2^31. A row's two
+    largest scores lie 2^16 or more apart here and are off by at most (64 + 8) 2^-24 of their terms' sum, 2^29.5: less than 2^12. So
+    each row is its largest key's value, in any type, and other dimensions' too where one is NaN."""
+    d = make([(1, 60), (20, 60), (1, 200), (7, 33)], 6, 2, 64, block, io, seed=9)
+    d["q"] = d["q"].sign() * 2.0**120
+    d["ks"] = np.full(d["ks"].shape, 2.0**-100)
+    clean = call(device, d, num_splits=splits).float().cpu().numpy()
+    want, _ = window_attention(d["q"].float().numpy(), d["positions"], d["seqs"], e4m3.values(d["k"], d["ks"]), e4m3.values(d["v"], d["vs"]),
+                               d["tables"], d["contexts"], d["scale"], CAUSAL, 0)  # fmt: skip
+    np.testing.assert_array_equal(clean, want)
+    for s in range(4):
+        d["v"][d["tables"][s, 25 // block], 25 % block, 1, 5] = np.nan  # of key head 1
+    got = call(device, d, num_splits=splits).float().cpu().numpy()
+    assert np.isnan(got[d["positions"] >= 25][:, 3:, 5]).all()
+    got[:, 3:, 5] = clean[:, 3:, 5]
+    np.testing.assert_array_equal(got, clean)
+
+
 def test_mixed_calls_captured_and_replayed_with_another_batch(device):
     """Tiles with shared runs, listed rows by pages, the order and the join in a graph whose lengths change between replays."""
     import torch
