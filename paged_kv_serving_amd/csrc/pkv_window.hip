@@ -2139,8 +2139,9 @@ Plan codes_plan(const pkv_window& g) {
     p.bytes += p.order_bytes;
     return p;
   }
-  // A short row is one workgroup's, which saves the join's launch.
-  p.stream = p.pages && g.num_splits == 0 && g.num_queries <= kStreamRows && g.num_queries * g.max_context_len > kStreamKeys;
+  // A short row is one workgroup's, which saves the join's launch. Sums of rounds, of 16 keys at least, are 32-bit.
+  p.stream = p.pages && g.num_splits == 0 && g.num_queries <= kStreamRows && g.num_queries * g.max_context_len > kStreamKeys &&
+             g.num_queries * ((g.max_context_len + int64_t{15}) / 16) < (int64_t{1} << 30);
   if (p.stream) {
     const int32_t subgroups = (g.num_heads / g.num_kv_heads + 15) / 16;
     p.form = page_form(g.num_queries, g.num_kv_heads, subgroups, g.head_dim, g.max_context_len);

@@ -105,6 +105,22 @@ def test_the_attentions_workspace(lib) -> None:
     assert lib.pkv_attention_e4m3_workspace_bytes(None) == EINVAL
 
 
+@pytest.mark.parametrize("num_queries,max_context_len,shared", [
+    (1, 1 << 30, True), (15, 1 << 30, True), (16, 1 << 30, False), (64, (1 << 28) - 16, True), (64, (1 << 28) - 15, False), (64, 1 << 28, False),
+    (1024, (1 << 24) - 16, True), (1024, 1 << 24, False), (1024, 1 << 30, False),
+])  # fmt: skip
+@pytest.mark.parametrize("head_dim", [32, 256])
+def test_rows_whose_rounds_32_bits_do_not_count_are_split_by_themselves(lib, num_queries, max_context_len, shared, head_dim) -> None:
+    """Equal shares are of the sum of all rows' rounds of 16 keys or more, which has to stay below 2^30."""
+    kind, size = structure("pkv_e4m3_attention"), ctypes.c_int64()
+    args = kind()
+    more = dict(num_queries=num_queries, max_context_len=max_context_len, head_dim=head_dim, num_heads=8, window=(1 << 31) - 1, sinks=0, max_query_len=1, num_splits=0)
+    for name, value in {**ATTENTION, **more}.items():
+        setattr(args, name, value)
+    assert lib.pkv_window_sizes(num_queries, 8, 2, head_dim, 0, (1 << 31) - 1, 0, max_context_len, 1, 0, ctypes.addressof(size)) >= 1
+    assert (lib.pkv_attention_e4m3_workspace_bytes(ctypes.addressof(args)) != size.value) == shared
+
+
 @pytest.mark.parametrize("q_dtype", [0, 1])
 @pytest.mark.parametrize("num_splits", [0, 1, 2])
 def test_the_workspace_of_a_call_without_queries(lib, q_dtype, num_splits) -> None:
