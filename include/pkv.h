@@ -917,7 +917,7 @@ int pkv_beam_select(const pkv_beam* args, int device, void* stream);
  *
  * No counterpart in the reference, whose copy-on-write (src/paged_kv_serving/engine/runner.py:128-133) is the host's.
  *
- *   new_tables, block_tables : int32 [num_groups * num_beams, table_stride]; the output must not be the input.
+ *   new_tables, block_tables : int32 [num_groups * num_beams, table_stride]; the output must not share memory with the input.
  *   parents                  : int32 [num_groups, num_beams]; one outside [0, num_beams) is the row itself.
  *   context_lens             : int32 [num_groups]; one whose blocks the table does not hold counts as the table's.
  *   states                   : up to PKV_BEAM_STATES tensors [num_layers, num_blocks, block_bytes], with layers

@@ -691,7 +691,9 @@ extern "C" int pkv_beam_reorder(const pkv_reorder* args, int device, void* strea
   if (g.num_groups > 0x7fffffff / (kThreads * PKV_BEAM_MAX)) return PKV_EUNSUPPORTED;
   if (g.num_groups == 0) return PKV_OK;
   if (!g.parents || !g.context_lens || (g.table_stride > 0 && (!g.new_tables || !g.block_tables))) return PKV_EINVAL;
-  if (g.table_stride > 0 && g.new_tables == g.block_tables) return PKV_EINVAL;
+  // Rows are read while others are written.
+  const int64_t entries = g.num_groups * g.num_beams * g.table_stride;
+  if (entries > 0 && g.new_tables < g.block_tables + entries && g.block_tables < g.new_tables + entries) return PKV_EINVAL;
   DeviceGuard guard(device);
   if (!guard.ok()) return PKV_EHIP;
   hipLaunchKernelGGL(reorder_kernel, dim3(static_cast<uint32_t>(g.num_groups * g.num_beams), static_cast<uint32_t>(layers)), dim3(kThreads), 0,

@@ -683,7 +683,7 @@ def beam_reorder(
     have to be the rows' own. Beams that start from one prompt are given a last block each and ``parents`` of zero, the
     prompt's row being the first.
 
-    ``out``: where the new tables go (a new tensor when None); it must not be ``block_tables``.
+    ``out``: where the new tables go (a new tensor when None); it must not share memory with ``block_tables``.
     """
     device = _one_device(block_tables, parents, context_lens, *states)
     if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or not block_tables.is_contiguous():
@@ -712,8 +712,8 @@ def beam_reorder(
         out = torch.empty_like(block_tables)
     elif out.shape != block_tables.shape or out.dtype != torch.int32 or not out.is_contiguous() or out.device != block_tables.device:
         raise ValueError("out must match block_tables")
-    elif out.data_ptr() == block_tables.data_ptr():
-        raise ValueError("out must not be block_tables")
+    elif abs(out.data_ptr() - block_tables.data_ptr()) < 4 * rows * width:
+        raise ValueError("out must not share memory with block_tables")
     if groups == 0:
         return out
     rc = _host().beam_reorder(

@@ -485,6 +485,24 @@ def test_states_past_32_bit_offsets(device):
     assert torch.equal(state[:, blocks - 1], state[:, blocks - 2]) and state[:, blocks - 1].any(1).all() and not state[:, : blocks - 2].any()
 
 
+def test_new_tables_in_the_memory_of_the_old_ones_are_refused(device):
+    import torch
+
+    from paged_kv_serving_amd import ops
+
+    both = torch.arange(48, dtype=torch.int32, device=device).view(12, 4)
+    parents, contexts = torch.zeros((2, 3), dtype=torch.int32, device=device), torch.tensor([5, 9], dtype=torch.int32, device=device)
+    for first in range(6):
+        there = both[first : first + 6]
+        for old, new in ((both[:6], there), (there, both[:6])):
+            with pytest.raises(ValueError, match="share memory"):
+                ops.beam_reorder(old, parents, contexts, [], block_size=4, out=new)
+    want = ops.beam_reorder(both[:6].clone(), parents, contexts, [], block_size=4)
+    assert torch.equal(ops.beam_reorder(both[:6], parents, contexts, [], block_size=4, out=both[6:]), want)
+    narrow = both.view(-1)[:0].view(6, 0)
+    assert ops.beam_reorder(narrow, parents, contexts, [], block_size=4, out=narrow).shape == (6, 0)
+
+
 def test_reorder_without_states_and_refusals(device):
     import torch
 

@@ -90,6 +90,12 @@ def test_reorder_refusals(lib, changes, code) -> None:
     assert refused(lib.pkv_beam_reorder, structure("pkv_reorder"), REORDER, **changes) == code
 
 
+@pytest.mark.parametrize("away", [-476, -4, 0, 4, 40, 476])
+def test_tables_that_share_memory_are_refused(lib, away) -> None:
+    """3 groups of 4 rows of 10 entries, 480 bytes: no entry of the output may be one of the input."""
+    assert refused(lib.pkv_beam_reorder, structure("pkv_reorder"), REORDER, new_tables=2 * FAKE + away) == EINVAL
+
+
 def test_no_arguments_and_nothing_to_do(lib) -> None:
     for function in (lib.pkv_step_metadata, lib.pkv_beam_select, lib.pkv_beam_reorder):
         assert function(None, 0, None) == EINVAL
