@@ -869,7 +869,7 @@ int pkv_step_metadata(const pkv_step* args, int device, void* stream);
  * No counterpart in the reference, which samples one sequence (src/paged_kv_serving/engine/sampling.py:28-74).
  *
  *   best_scores, best_beams, best_tokens : float32, int32, int32 [num_groups, count], output. A beam's number is its place
- *                 in its group.
+ *                 in its group. best_scores may be scores where count is num_beams, and shares no memory with them otherwise.
  *   logits      : rows of vocab_size values of `dtype`, row r at element r * row_stride, beam b of group g being row
  *                 g * num_beams + b.
  *   scores      : float32 [num_groups * num_beams].

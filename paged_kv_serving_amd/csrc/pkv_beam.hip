@@ -654,6 +654,9 @@ extern "C" int pkv_beam_select(const pkv_beam* args, int device, void* stream) {
   if (rows * chunks > 0x7fffffff / kThreads) return PKV_EUNSUPPORTED;
   if (g.num_groups == 0) return PKV_OK;
   if (!g.best_scores || !g.best_beams || !g.best_tokens || !g.logits || !g.scores) return PKV_EINVAL;
+  // A group's scores are read before its own best ones are written, but other groups' may not be.
+  const bool in_place = g.best_scores == g.scores && g.count == g.num_beams;
+  if (!in_place && g.best_scores < g.scores + rows && g.scores < g.best_scores + g.num_groups * g.count) return PKV_EINVAL;
   const int64_t need = pkv_beam_workspace_bytes(g.num_groups, g.num_beams, g.vocab_size, g.count);
   if (!g.workspace || !aligned16(g.workspace) || g.workspace_bytes < need) return PKV_EINVAL;
   Select a{};

@@ -617,8 +617,9 @@ def beam_select(
     that have ended: such a beam has one, ``end_token`` at its own score. ``beams`` are places in the group, as
     :func:`beam_reorder` takes them.
 
-    ``workspace``: scratch of :func:`beam_workspace_bytes` bytes, allocated when None; calls that may run at the same time
-    need their own. The same call gives the same bits.
+    ``out``: an earlier result to write to. Its ``scores`` may be ``scores`` themselves where ``count`` is ``num_beams``, and share no
+    memory with them otherwise. ``workspace``: scratch of :func:`beam_workspace_bytes` bytes, allocated when None; calls that may run
+    at the same time need their own. The same call gives the same bits.
     """
     device = _one_device(logits, scores) if finished is None else _one_device(logits, scores, finished)
     if logits.dim() != 2 or logits.dtype not in _DTYPE_CODES:
@@ -647,6 +648,9 @@ def beam_select(
         for name, tensor, dtype in zip(out._fields, out, (torch.float32, torch.int32, torch.int32)):
             if tensor.shape != shape or tensor.dtype != dtype or not tensor.is_contiguous() or tensor.device != logits.device:
                 raise ValueError(f"out.{name} must be contiguous {str(dtype)[6:]} of shape (groups, count)")
+        away = out.scores.data_ptr() - scores.data_ptr()  # in place, or apart
+        if not (away == 0 and count == num_beams) and -4 * groups * count < away < 4 * rows:
+            raise ValueError("out.scores must be scores themselves, where count is num_beams, or share no memory with them")
     if groups == 0:
         return out
     if workspace is None:

@@ -319,6 +319,32 @@ def test_two_streams_at_once_and_a_replayed_graph(device):
         assert all(torch.equal(a, e) for a, e in zip(held, eager))
 
 
+@pytest.mark.parametrize("groups,vocab", [(1, 700), (300, 700), (40, 9001)])
+def test_scores_updated_in_place(device, groups, vocab):
+    """The best scores over the scores, where there are as many; in other parts of their memory they are refused."""
+    import torch
+
+    from paged_kv_serving_amd import ops
+
+    beams = 4
+    logits, scores = rows_of(groups, beams, vocab, "float32", groups)
+    logits, before = logits.to(device), torch.as_tensor(scores, dtype=torch.float32).to(device)
+    held = before.clone()
+    for _ in range(3):
+        want = ops.beam_select(logits, before, num_beams=beams)
+        out = ops.BeamChoice(held.view(groups, beams), torch.empty_like(want.beams), torch.empty_like(want.tokens))
+        got = ops.beam_select(logits, held, num_beams=beams, out=out)
+        assert all(torch.equal(a, b) for a, b in zip(got, want)) and got.scores.data_ptr() == held.data_ptr()
+        before = want.scores.view(-1)
+    room = torch.zeros(5 * groups * beams, device=device)
+    rows = groups * beams
+    for count, first in ((2 * beams, 0), (2 * beams, 1), (beams, 1), (beams, rows - 1), (2, 0)):
+        for a, b in ((0, first), (2 * rows, 2 * rows - first)):  # where the scores begin, and the best ones
+            out = ops.BeamChoice(room[b : b + groups * count].view(groups, count), *(torch.empty((groups, count), dtype=torch.int32, device=device) for _ in range(2)))
+            with pytest.raises(ValueError, match="memory"):
+                ops.beam_select(logits, room[a : a + rows], num_beams=beams, count=count, out=out)
+
+
 def test_select_refusals(device):
     import torch
 

@@ -96,6 +96,12 @@ def test_tables_that_share_memory_are_refused(lib, away) -> None:
     assert refused(lib.pkv_beam_reorder, structure("pkv_reorder"), REORDER, new_tables=2 * FAKE + away) == EINVAL
 
 
+@pytest.mark.parametrize("count,away", [(8, -23 * 4), (8, -4), (8, 0), (8, 4), (8, 11 * 4), (4, -11 * 4), (4, 4), (4, 11 * 4), (2, 0)])
+def test_best_scores_in_the_memory_of_the_scores_are_refused(lib, count, away) -> None:
+    """3 groups of 4 beams: 12 scores, 3 * count best ones."""
+    assert refused(lib.pkv_beam_select, structure("pkv_beam"), BEAM, count=count, best_scores=5 * FAKE + away) == EINVAL
+
+
 def test_no_arguments_and_nothing_to_do(lib) -> None:
     for function in (lib.pkv_step_metadata, lib.pkv_beam_select, lib.pkv_beam_reorder):
         assert function(None, 0, None) == EINVAL
