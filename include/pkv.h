@@ -734,7 +734,8 @@ int pkv_sample_tokens(const pkv_sample* args, int device, void* stream);
  *   slot_mapping             : int64 [num_tokens]; a slot outside the pool (padding: -1) is skipped.
  * The tokens of one block have to stand next to each other in the call, as a batch's slots do; where they do not, or where a
  * slot is named twice, that block's contents and scales are unspecified. A value that is not finite becomes NaN and counts
- * nothing for the scale. The same inputs give the same bits. Supported: head_dim 32, 64, 128, 256, fewer than 2^31 slots.
+ * nothing for the scale. Magnitudes of 248 * 2^120 (3.3e38) and more round to 2^128, which is no float32 number. The same inputs give
+ * the same bits. Supported: head_dim 32, 64, 128, 256, fewer than 2^31 slots.
  */
 typedef struct pkv_e4m3_append {
   void* key_pool;
@@ -761,7 +762,7 @@ int pkv_append_e4m3(const pkv_e4m3_append* args, int device, void* stream);
  *
  *   key_cache, value_cache   : e4m3 codes [num_blocks, block_size, num_kv_heads, head_dim], 16-byte aligned.
  *   key_scales, value_scales : float32 [num_blocks, num_kv_heads], powers of two from 2^-100 to 2^120. Of another
- *                              number its exponent alone counts.
+ *                              normal number its exponent alone counts; an infinity or NaN makes the block's keys or values NaN.
  * workspace                : of the bytes that pkv_attention_e4m3_workspace_bytes gives.
  * All else is pkv_window's; a window of INT32_MAX is plain causal attention. With num_splits 0, rows by themselves without a
  * window over blocks of a multiple of 16 tokens are cut into equal shares of the call's keys, whichever rows these are of, so a
@@ -877,7 +878,7 @@ int pkv_step_metadata(const pkv_step* args, int device, void* stream);
  *   workspace   : scratch of pkv_beam_workspace_bytes bytes, 16-byte aligned; calls that may run at the same time need
  *                 their own. Nothing in it needs to start at zero.
  * Up to PKV_BEAM_MAX beams and PKV_BEAM_MAX_COUNT continuations, which a group must have (count <= num_beams * vocab_size), up
- * to 2^20 rows. The same call gives the same bits.
+ * to 2^20 rows, and 2^25 logits of a group. The same call gives the same bits.
  */
 #define PKV_BEAM_MAX 64
 #define PKV_BEAM_MAX_COUNT 128

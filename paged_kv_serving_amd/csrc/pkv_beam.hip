@@ -108,9 +108,10 @@ __device__ __forceinline__ bool looked_at(const pkv_beam& g, int64_t row) {
 // least `count` logits reach, and few more: 8192 of them and 8 classes list about 23. Classes of lanes rather than neighbours:
 // a row's last chunk, which has numbers for the first threads alone, leaves no class empty. Each one's place is the number of
 // larger ones. Where too many reach it (128 classes: about 700; equal logits), bisection finds a number that fewer do.
-// 32 groups of 8 beams over 128256 float32 logits: about 36 us for 115 MB. Bound by the vector units at 22 us of it, the
-// exponentials' 17 operations being two thirds of them, which the reads of 18 us overlap with in part; the kernel takes 21 us
-// without them. Half the bytes (bf16) take the same time. 7 wavefronts on a SIMD take 1.3 us less than the 5 of 88 registers.
+// 32 groups of 8 beams over 128256 float32 logits, 131 MB: about 38 us. Bound by the vector units: their instructions, two thirds of
+// them the exponentials' 17 operations, take 20 us of issue, 81% of the cycles in which a CU has work, and overlap with the reads, 20 us,
+// in part; the kernel takes 21 us without the exponentials. Half the bytes (bf16) take the same time. 7 wavefronts on a SIMD take
+// 1.3 us less than the 5 of 88 registers.
 template <typename T, int kPer>
 __global__ __launch_bounds__(kThreads, 7) void chunk_kernel(const Select a) {
   constexpr int kVec = 16 / sizeof(T), kLoads = kPer / kVec, kAhead = kLoads < 3 ? kLoads : 3;
@@ -526,14 +527,14 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(const Select a) {
 // Reordering. One workgroup for a child and a layer, of every state; a child that takes its parent's block over has nothing to
 // copy. Every workgroup finds its group's moves by itself: the parents that earlier children named are a word of bits.
 // Bound: HBM for large blocks, latency for small ones. 32 groups of 8 beams, 32 layers of 16 KB blocks and their scales, 252 MB read and
-// written: 52 us, 4.8 TB/s.
+// written: 53 us, 4.8 TB/s.
 // ---------------------------------------------------------------------------------------------
 constexpr int kTogether = 4;  // units that a thread loads before it stores them
 struct Reorder {
   pkv_reorder g;
   int32_t unit[PKV_BEAM_STATES];  // bytes that are moved together: 16, 4 or 1
   // Whether every state's block is one batch of a wavefront. The wavefronts then have a state each, and the states' latencies run
-  // at the same time: 18 groups of 16 beams, 22 layers, 1 KB each of keys and values with their scales, 24 us, together 31.
+  // at the same time: 18 groups of 16 beams, 22 layers, 1 KB each of keys and values with their scales, 20 us, together 28.
   bool apart;
 };
 

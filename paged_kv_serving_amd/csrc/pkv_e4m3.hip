@@ -138,7 +138,7 @@ __device__ __forceinline__ float finite_size(float x) {
 // codes are scaled down. No two wavefronts write the same block and head, so nothing waits for another. Here a run of more
 // than kHeld tokens. Where blocks have more, kLong tokens (32 or 64) are held as they are stored, in registers that would cost a kernel of small
 // blocks its wavefronts; longer runs are read twice, the second time from the caches. 16 x 512 tokens of 32 heads x 128,
-// bfloat16, in blocks of 64: 51 us, read twice 66; 8 x 512, float32, in blocks of 32 with kLong 32 and 64: 34 and 53, of 64: 47
+// bfloat16, in blocks of 64: 50 us, read twice 66; 8 x 512, float32, in blocks of 32 with kLong 32 and 64: 33 and 53, of 64: 47
 // and 38.
 // ---------------------------------------------------------------------------------------------
 template <typename T, int D, int kLong>
@@ -289,8 +289,8 @@ __device__ __forceinline__ void append_runs(const Append& a, int which, int32_t 
 
 // A wavefront has the runs that begin in its window of kHeld tokens, of one head, keys or values. Short ones are taken together, as
 // many as end within kHeld tokens: one after the other, the latency of each (2 us) counted.
-// Bound: HBM for long prompts, latency for single tokens. 16 x 512 tokens of 32 heads x 128, bfloat16, in blocks of 16, 201 MB: 43 us,
-// 4.7 TB/s; 64 single tokens of 8 heads x 128 5 us.
+// Bound: HBM for long prompts, latency for single tokens. 16 x 512 tokens of 32 heads x 128, bfloat16, in blocks of 16, 202 MB: 44 us,
+// 4.6 TB/s; 64 single tokens of 8 heads x 128 5 us.
 template <typename T, int D, int kLong>
 __global__ __launch_bounds__(kThreads) void append_kernel(const Append a) {
   // Items: keys and values of a head, heads, then windows.

@@ -380,7 +380,7 @@ __device__ __forceinline__ Words<N> load_words(const void* p) {
 //
 // kOrder: also the aligned blocks in the order of the keys that their rows see (three rows of a block speak for it), the most first, for
 // as many blocks as the workgroup has threads. The tiles' workgroups then end together: 8 x 512 rows behind up to 2048 others,
-// 32/8 heads x 128 over e4m3 codes, 250 -> 208 us.
+// 32/8 heads x 128 over e4m3 codes, 248 -> 201 us.
 constexpr int kListThreads = 1024;  // the order's keys hold a block's number in ten bits
 template <bool kOrder>
 __global__ __launch_bounds__(kListThreads) void list_kernel(const Window a) {
@@ -854,8 +854,8 @@ __global__ __launch_bounds__(kRowWaves * kPair * kWave) void row_kernel(const Wi
 // The codes of two neighbouring keys are interleaved before they are widened, which gives the value operand's pairs at
 // once. The next round's keys are asked for as soon as the present one's are scores, its values when the present ones are used.
 //
-// Bound: HBM. 64 rows of 16384 keys, 32/8 heads x 128, bfloat16 queries, 2.15 GB: 351 us, 6.1 TB/s (a copy of these bytes
-// by the same pieces alone: 6.7; by the general row pass above, which exchanges slots and scales between lanes, 560).
+// Bound: HBM. 64 rows of 16384 keys, 32/8 heads x 128, bfloat16 queries, 2.15 GB: 361 us, 6.0 TB/s (reads of these bytes
+// by the same pieces alone: 6.7; by the general row pass above, which exchanges slots and scales between lanes, 477).
 // ---------------------------------------------------------------------------------------------
 template <typename QT, int D>
 struct PageShape {
@@ -1107,7 +1107,7 @@ __global__ __launch_bounds__(kRowWaves * kPair * kWave) void page_kernel(const W
 }
 
 // The listed rows of a call with tiles, item by item of workgroup `block` of `blocks`. 20 rows of 2481 to 2853 keys beside a run of 10,
-// 32/8 heads x 128, bfloat16, blocks of 16: 39 us, of one token, which the general row pass takes, 51.
+// 32/8 heads x 128, bfloat16, blocks of 16: 38 us, of one token, which the general row pass takes, 49.
 template <typename QT, int D>
 __device__ __forceinline__ void page_pass(const Window& a, RowScratch<D, kWaves, 1>& shared, uint32_t block, uint32_t blocks) {
   constexpr int kKeys = 16 * PageShape<QT, D>::kBlocks;
@@ -1299,9 +1299,12 @@ __global__ __launch_bounds__(kThreads) void stream_join_kernel(const Window a) {
 // at two wavefronts per SIMD: a step's values are waited for before its products. Float32 queries over bfloat16
 // 234 us (three products for one), over float32 438 (six, at one wavefront per SIMD). One piece of P instead of two was
 // 9% faster.
+// Over e4m3 codes, without a window (86 GFLOP): 170 us, replayed back to back 201. The staged codes and scales take all 256
+// registers and 11 more are spilled (48 bytes a lane); over bfloat16 244 do. The CUs have work in 73% of the cycles, and in these the
+// matrix units are busy in 35%, vector instructions issue in 48% and LDS works in 39%. Float32 queries: 364 us, one wavefront per SIMD.
 // ---------------------------------------------------------------------------------------------
 // float32 queries of head_dim 256 have tiles over codes alone (float32 pools' pieces do not fit LDS): over pools their rows go by
-// themselves (codes, 5 x 455 rows behind up to 2055 others, 8 heads: 422 us, by themselves 3277).
+// themselves (codes, 5 x 455 rows behind up to 2055 others, 8 heads: 254 us, by themselves 3277).
 constexpr bool tiles_of(int q_size, int head_dim) { return q_size == 2 || head_dim <= 128; }
 
 template <typename QT, typename KVT, int D>
@@ -2137,8 +2140,8 @@ Plan codes_plan(const pkv_window& g) {
       p.bytes = pkv_window_workspace_bytes(g.num_queries, g.num_heads, g.head_dim, g.max_query_len, p.splits);
     }
     // A tile's runs one after the other cost their latencies; where tiles are few and runs surely shorter than they are, several
-    // workgroups share them. 6 x 27 rows, 8 heads x 128, bfloat16: 18 us, in one workgroup each 54; 2 x 12 rows of up to 1191
-    // keys, 8/2 heads x 128, float32: 26 us and 42.
+    // workgroups share them. 6 x 27 rows, 8 heads x 128, bfloat16: 17 us, in one workgroup each 52; 2 x 12 rows of up to 1191
+    // keys, 8/2 heads x 128, float32: 24 us and 40.
     const int64_t parts = groups * p.splits, longest = g.max_query_len;
     // Of longer runs a tile may still hold the end of one and the start of the next: two workgroups for it, one of them mostly without
     // any, cost what their look does (7 x 211 rows, 16/8 heads x 32, float32: 25 us, with one 35; 2 x 465 rows beside 15, 8/1 heads x

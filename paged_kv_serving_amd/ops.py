@@ -1838,8 +1838,8 @@ def paged_attention_e4m3(
     None (and is, unless given): every key up to the row's own position is seen then.
 
     ``key_cache``/``value_cache``: contiguous float8_e4m3fn ``[num_blocks, block_size, kv_heads, head_dim]``;
-    ``key_scales``/``value_scales``: contiguous float32 ``[num_blocks, kv_heads]``, powers of two (of another number its
-    power of two alone counts). Codes are widened to bfloat16, which holds a code times its scale exactly, on their way
+    ``key_scales``/``value_scales``: contiguous float32 ``[num_blocks, kv_heads]``, powers of two (of another normal number its
+    exponent alone counts; an infinity or NaN makes the block's keys or values NaN). Codes are widened to bfloat16, which holds a code times its scale exactly, on their way
     into the products. Queries are float32 or bfloat16. ``workspace`` has :func:`e4m3_workspace_bytes` bytes. Without
     ``num_splits`` and a window, decode rows over blocks of a multiple of 16 tokens are cut into equal shares of the call's
     keys, whichever rows these are of: what else is in a batch may change a row's result by roundings.
