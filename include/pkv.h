@@ -827,6 +827,7 @@ int pkv_attention_e4m3(const pkv_e4m3_attention* args, int device, void* stream)
  *                              num_rows at most.
  *   context_lens_out         : int32 [num_seqs], output: the context lengths that the step's attention sees. Not the input.
  *   next_free_out            : int32 [1], output: next_free behind the blocks that were taken. Not the input.
+ * No output, the tables among them, may share memory with an input.
  * A request is not served, and changes nothing, where the blocks needed up to and with it (by requests not refused for the other
  * reasons) are more than are free and it needs any, where its rows pass num_rows, where its table is too narrow, or where
  * its context is shorter than its query: its rows are padding then, and its context length out is context - query (0 where that

@@ -132,7 +132,23 @@ extern "C" int pkv_step_metadata(const pkv_step* args, int device, void* stream)
   if (g.num_seqs > 0 && (!g.query_lens || !g.context_lens || !g.context_lens_out || (!g.block_tables && g.table_stride > 0))) return PKV_EINVAL;
   if (g.num_rows > 0 && (!g.query_seq || !g.query_positions || !g.positions || !g.slot_mapping)) return PKV_EINVAL;
   if (g.num_free > 0 && !g.free_blocks) return PKV_EINVAL;
-  if (g.next_free == g.next_free_out || (g.num_seqs > 0 && g.context_lens == g.context_lens_out)) return PKV_EINVAL;
+  // Every workgroup reads the inputs while others write: no memory of both. Table entries alone are read and written.
+  struct Range {
+    const void* at;
+    int64_t bytes;
+  };
+  const int64_t requests = 4 * static_cast<int64_t>(g.num_seqs);
+  const Range read[] = {{g.query_lens, requests}, {g.context_lens, requests}, {g.free_blocks, 4 * static_cast<int64_t>(g.num_free)}, {g.next_free, g.next_free ? 4 : 0}};
+  const Range written[] = {{g.query_seq, 4 * g.num_rows}, {g.query_positions, 4 * g.num_rows}, {g.positions, 8 * g.num_rows}, {g.slot_mapping, 8 * g.num_rows},
+                           {g.query_starts, requests + 4}, {g.context_lens_out, requests}, {g.next_free_out, 4},
+                           {g.block_tables, requests * g.table_stride}};
+  for (const Range& in : read) {
+    const uintptr_t from = reinterpret_cast<uintptr_t>(in.at);
+    for (const Range& out : written) {
+      const uintptr_t to = reinterpret_cast<uintptr_t>(out.at);
+      if (in.bytes > 0 && out.bytes > 0 && from < to + out.bytes && to < from + in.bytes) return PKV_EINVAL;
+    }
+  }
   DeviceGuard guard(device);
   if (!guard.ok()) return PKV_EHIP;
   const uint32_t groups = static_cast<uint32_t>(std::max<int64_t>(1, (g.num_rows + kThreads - 1) / kThreads));

@@ -767,9 +767,8 @@ def step_metadata(
 
     A request that cannot be served changes nothing, has padding rows and its context without this step's tokens: where the
     free blocks do not suffice for the requests up to and with it, and it needs any; where its rows pass ``num_rows``, its table is
-    too narrow, or its context shorter than its query. ``out``: an earlier result to write to; it must not hold
-    ``context_lens`` or ``next_free`` given here. The call can be captured into a graph, whose requests then grow from replay to
-    replay.
+    too narrow, or its context shorter than its query. ``out``: an earlier result to write to; it, like ``block_tables``, must
+    share no memory with the call's inputs. The call can be captured into a graph, whose requests then grow from replay to replay.
     """
     device = _one_device(query_lens, context_lens, block_tables, free_blocks) if next_free is None else _one_device(
         query_lens, context_lens, block_tables, free_blocks, next_free)  # fmt: skip
@@ -799,15 +798,13 @@ def step_metadata(
             dtype = torch.int64 if name in wide else torch.int32
             if tensor.dtype != dtype or tensor.shape != (size,) or not tensor.is_contiguous() or tensor.device != query_lens.device:
                 raise ValueError(f"out.{name} must be contiguous {str(dtype)[6:]} with {size} entries")
-        if (next_free is not None and out.next_free.data_ptr() == next_free.data_ptr()) or (
-            seqs and out.context_lens.data_ptr() == context_lens.data_ptr()
-        ):
-            raise ValueError("out must not hold the call's own context_lens or next_free")
     rc = _host().step_metadata(
         query_lens.data_ptr(), context_lens.data_ptr(), block_tables.data_ptr(), free_blocks.data_ptr(),
         0 if next_free is None else next_free.data_ptr(), *(tensor.data_ptr() for tensor in out), num_rows, seqs, width,
         free_blocks.shape[0], block_size, device, _stream(device),
     )  # fmt: skip
+    if rc == _native.PKV_EINVAL:  # all else has been looked at
+        raise ValueError("out and block_tables must share no memory with the call's own inputs")
     _native.check(rc, "pkv_step_metadata")
     return out
 
@@ -1839,8 +1836,8 @@ def paged_attention_e4m3(
 
     ``key_cache``/``value_cache``: contiguous float8_e4m3fn ``[num_blocks, block_size, kv_heads, head_dim]``;
     ``key_scales``/``value_scales``: contiguous float32 ``[num_blocks, kv_heads]``, powers of two (of another normal number its
-    exponent alone counts; an infinity or NaN makes the block's keys or values NaN). Codes are widened to bfloat16, which holds a code times its scale exactly, on their way
-    into the products. Queries are float32 or bfloat16. ``workspace`` has :func:`e4m3_workspace_bytes` bytes. Without
+    exponent alone counts; an infinity or NaN makes the block's keys or values NaN). Codes are widened to bfloat16, which holds a
+    code times its scale exactly, on their way into the products. Queries are float32 or bfloat16. ``workspace`` has :func:`e4m3_workspace_bytes` bytes. Without
     ``num_splits`` and a window, decode rows over blocks of a multiple of 16 tokens are cut into equal shares of the call's
     keys, whichever rows these are of: what else is in a batch may change a row's result by roundings.
     """

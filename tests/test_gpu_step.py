@@ -174,3 +174,32 @@ def test_refusals(device):
         ops.step_metadata(**{**good, "out": out, "next_free": out.next_free})
     with pytest.raises(ValueError, match="own"):
         ops.step_metadata(**{**good, "out": out, "context_lens": out.context_lens})
+
+
+def test_outputs_in_the_memory_of_an_input_are_refused(device):
+    """Parts of one buffer: each output over each input and, where the inputs lie apart, the same result as from buffers of their own."""
+    import torch
+
+    from paged_kv_serving_amd import ops
+
+    room = torch.zeros(400, dtype=torch.int32, device=device)
+    room[:8] = torch.tensor([1, 2, 0, 3, 5, 17, 30, 3], dtype=torch.int32)
+    query, context, free, next_free = room[:4], room[4:8], room[8:20], room[20:21]
+    free.copy_(torch.arange(12, dtype=torch.int32))
+    tables = torch.arange(100, 112, dtype=torch.int32, device=device).view(4, 3)
+    want_tables = tables.clone()
+    want = ops.step_metadata(query.clone(), context.clone(), want_tables, free.clone(), next_free.clone(), block_size=16, num_rows=8)
+    wide = room[24:88].view(torch.int64)
+    out = ops.StepMetadata(room[100:108], room[108:116], wide[:8], wide[8:16], room[116:121], room[121:125], room[125:126])
+    got = ops.step_metadata(query, context, tables, free, next_free, block_size=16, num_rows=8, out=out)
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and torch.equal(tables, want_tables)
+    for name, size in (("query_seq", 8), ("query_positions", 8), ("query_starts", 5), ("context_lens", 4), ("next_free", 1)):
+        for first in (0, 3, 7, 19, 20):  # over the lengths, the list of free blocks, its place
+            with pytest.raises(ValueError, match="own inputs"):
+                ops.step_metadata(query, context, tables, free, next_free, block_size=16, num_rows=8, out=out._replace(**{name: room[first : first + size]}))
+    with pytest.raises(ValueError, match="own inputs"):
+        ops.step_metadata(query, context, room[10:22].view(4, 3), free, next_free, block_size=16, num_rows=8)
+    same = context.clone()  # one tensor as two inputs: prompts without a cached token
+    both = ops.step_metadata(same, same, tables.clone(), free, block_size=16, num_rows=60)
+    apart = ops.step_metadata(same, same.clone(), tables.clone(), free, block_size=16, num_rows=60)
+    assert all(torch.equal(a, b) for a, b in zip(both, apart))

@@ -68,6 +68,16 @@ def test_step_refusals(lib, changes, code) -> None:
     assert refused(lib.pkv_step_metadata, structure("pkv_step"), STEP, **changes) == code
 
 
+@pytest.mark.parametrize("output,size", [
+    ("query_seq", 120), ("query_positions", 120), ("positions", 240), ("slot_mapping", 240), ("query_starts", 20), ("context_lens_out", 16),
+    ("next_free_out", 4), ("block_tables", 160),
+])  # fmt: skip
+@pytest.mark.parametrize("read,bytes_read", [("query_lens", 16), ("context_lens", 16), ("free_blocks", 80), ("next_free", 4)])
+def test_step_outputs_in_the_memory_of_an_input_are_refused(lib, output, size, read, bytes_read) -> None:
+    for away in (4 - size, 0, bytes_read - 4):
+        assert refused(lib.pkv_step_metadata, structure("pkv_step"), STEP, **{output: STEP[read] + away}) == EINVAL
+
+
 @pytest.mark.parametrize("changes,code", [
     ({"num_groups": -1}, EINVAL), ({"num_beams": 0}, EINVAL), ({"vocab_size": 0}, EINVAL), ({"count": 0}, EINVAL), ({"dtype": 2}, EINVAL),
     ({"row_stride": 99}, EINVAL), ({"num_beams": 65}, EUNSUPPORTED), ({"count": 129}, EUNSUPPORTED), ({"num_groups": 1 << 19}, EUNSUPPORTED),
